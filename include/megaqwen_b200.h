@@ -65,7 +65,10 @@ enum {
     MQ_ERR_BAD_TOKEN = 4,          /* input token outside [0, vocab) (device check) */
     MQ_ERR_BAD_POSITION = 5,       /* position outside [0, max_seq_len) (device check) */
     MQ_ERR_CUDA = 6,               /* a CUDA runtime call failed */
-    MQ_ERR_WORKSPACE = 7           /* workspace missing or too small */
+    MQ_ERR_WORKSPACE = 7,          /* workspace missing or too small */
+    MQ_ERR_BAD_SLOT = 8,           /* paged cache: slot out of range, named twice, or not empty (device check) */
+    MQ_ERR_BAD_PAGE = 9,           /* paged cache: page number out of range or in the wrong state (device check) */
+    MQ_ERR_NO_PAGES = 10           /* paged cache: not enough free pages (device check) */
 };
 
 /* ---- reference ABI -------------------------------------------------------
@@ -339,6 +342,188 @@ typedef struct mq_decode_batch_params {
 
 size_t mq_decode_batch_workspace_bytes(int batch, int max_seq_len);
 int mq_decode_batch(const mq_decode_batch_params* params, cudaStream_t stream);
+
+/* ---- paged KV cache ------------------------------------------------------------
+ * The reference keeps one contiguous cache per sequence; these operators have
+ * no counterpart there.  A pool holds pages of page_size positions of every
+ * layer and kv head, [num_pages, num_layers, num_kv_heads, page_size, head_dim]
+ * by default; the [page_size, head_dim] block is contiguous, the other strides
+ * (in elements, multiples of 8) are free.  A sequence is a row ("slot") of the
+ * page table, int32 [num_slots, table_cols], its first pages_of(length) entries
+ * being page numbers, and a length; refs[p] counts the slots that hold page p
+ * (0: free).  Only full pages are ever shared, so a page that is written has
+ * one owner.
+ *
+ * Nothing here synchronises or allocates.  Arguments that live on the device
+ * are checked there: `status` (device int32, optional) keeps the first error
+ * code, and a call whose arguments are wrong changes none of the tables.
+ * Workspaces hold nothing between calls; calls that overlap on the GPU need
+ * their own. */
+enum { MQ_BF16 = 0, MQ_FP16 = 1, MQ_FP32 = 2 };
+
+typedef struct mq_paged_pool {
+    void* k;
+    void* v;
+    signed char* index;          /* optional: page score index, records of 2 * head_dim + 16 bytes */
+    int dtype;                   /* MQ_BF16 or MQ_FP16 */
+    int num_pages;
+    int num_layers;
+    int num_kv_heads;
+    int page_size;               /* 16, 32, 64 or 128 */
+    int head_dim;                /* 64 or 128 */
+    long long k_page, k_layer, k_head;   /* strides in elements */
+    long long v_page, v_layer, v_head;
+    long long i_page, i_layer, i_head;   /* strides of the index in bytes, multiples of 16 */
+} mq_paged_pool;
+
+typedef struct mq_page_table {
+    int* table;                  /* device int32 [num_slots, cols], row stride row_stride */
+    int* lengths;                /* device int32 [num_slots] */
+    int* refs;                   /* device int32 [num_pages] */
+    int num_slots;               /* at most 65536 */
+    int cols;
+    int num_pages;               /* at most 2^20 */
+    int page_size;
+    long long row_stride;
+    int* status;                 /* device int32, optional */
+    void* workspace;             /* device, mq_paged_workspace_bytes(num_pages, n) bytes */
+    size_t workspace_bytes;
+} mq_page_table;
+
+size_t mq_paged_workspace_bytes(int num_pages, int n);
+
+/* Release n sequences: their pages' counts fall by one, their rows become -1,
+ * their lengths 0. */
+int mq_paged_free(const mq_page_table* t, const int* slots, int n, cudaStream_t stream);
+/* Grow n sequences to new_lengths (never below the present ones): the pages
+ * they lack are the lowest free ones, handed out in the order of `slots`. */
+int mq_paged_reserve(const mq_page_table* t, const int* slots, const int* new_lengths, int n, cudaStream_t stream);
+/* children[i], an empty slot, becomes a copy of parents[i]: full pages are
+ * shared, the filled rows of a last part page are copied (all layers) into the
+ * lowest free pages, in the order of `children`. */
+int mq_paged_fork(const mq_paged_pool* pool, const mq_page_table* t, const int* parents, const int* children, int n,
+                  cudaStream_t stream);
+/* Page src_pages[i] of `src` into page dst_pages[i] of `dst` (the same geometry
+ * and type; it may be the same pool, as long as no page is both read and
+ * written).  K, V and, when both pools have one, the index. */
+int mq_paged_copy(const mq_paged_pool* src, const mq_paged_pool* dst, const int* src_pages, const int* dst_pages,
+                  int n, int* status, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+/* Every page in use, in ascending order, into pages 0, 1, ... of another pool;
+ * out_table and out_refs (refs of dst->num_pages pages) name them there. */
+int mq_paged_compact(const mq_paged_pool* src, const mq_paged_pool* dst, const mq_page_table* t, int* out_table,
+                     long long out_row_stride, int* out_refs, cudaStream_t stream);
+
+/* Rotary positions, and optionally the write of the rotated K and of V into
+ * the pages.  Token i sits at positions[i]; with a pool it belongs to slot
+ * slots[i], whose pages must hold that position.  rotary_dim <= head_dim, even:
+ * channels past it pass through.  Pairs are (i, i + rotary_dim / 2), or
+ * (2i, 2i + 1) with interleaved.  cos/sin: fp32 [max_pos, rotary_dim / 2],
+ * y0 = x0 c - x1 s, y1 = x1 c + x0 s, each product and sum rounded to fp32.
+ * inverse turns the other way (the gradient of the rotation).
+ * With an index in the pool, a page whose last row is written gets its record:
+ * the channel-wise bounds of its keys as whole numbers HI[D], LO[D] times 2^e,
+ * then e: e = clamp(floor(log2 a) - 6, -60, 40) for the largest magnitude a of
+ * the bounds (0 if a = 0), HI and LO rounded to nearest even, at most 127 in
+ * magnitude. */
+typedef struct mq_rope_params {
+    const void* q;               /* [n, num_q_heads, head_dim], optional */
+    void* q_out;
+    const void* k;               /* [n, num_kv_heads, head_dim], with pool */
+    const void* v;
+    long long q_token, q_head, out_token, out_head, k_token, k_head, v_token, v_head;   /* strides in elements */
+    const int* positions;        /* device int32 [n] */
+    const int* slots;            /* device int32 [n], with pool */
+    const float* cos_table;
+    const float* sin_table;
+    long long cos_row, sin_row;  /* row strides in elements */
+    int max_pos;
+    int n;
+    int num_q_heads;
+    int head_dim;
+    int rotary_dim;
+    int interleaved;
+    int inverse;
+    int dtype;
+    int layer;
+    const mq_paged_pool* pool;   /* optional */
+    const int* table;            /* with pool: the page table */
+    long long table_row;
+    int num_slots;
+    int table_cols;
+    int* status;                 /* device int32, optional */
+} mq_rope_params;
+
+int mq_rope(const mq_rope_params* params, cudaStream_t stream);
+
+/* Attention over the pages.  The query tokens of sequence b are rows
+ * q_starts[b] .. q_starts[b+1] - 1 of q (one each when q_starts is NULL): the
+ * last positions of slot slots[b], whose keys are written already; each sees
+ * the positions up to its own.  Rows that see nothing are zero.
+ * Sequences group_starts[g] .. group_starts[g+1] - 1 share their first
+ * prefix_pages[g] pages (the same page numbers in their rows, as a fork leaves
+ * them): those are read once for the group.  num_groups 0: nothing is shared. */
+typedef struct mq_paged_attend_params {
+    const mq_paged_pool* pool;
+    const void* q;               /* [total_q, num_q_heads, head_dim], strides in elements, multiples of 8 */
+    long long q_token, q_head;
+    void* out;                   /* [total_q, num_q_heads, head_dim] contiguous */
+    const int* table;
+    long long table_row;
+    int num_slots;
+    int table_cols;
+    const int* lengths;          /* device int32 [num_slots] */
+    const int* slots;            /* device int32 [num_seqs] */
+    const int* q_starts;         /* device int32 [num_seqs + 1], optional */
+    const int* group_starts;     /* device int32 [num_groups + 1] */
+    const int* prefix_pages;     /* device int32 [num_groups] */
+    int num_seqs;                /* at most 2048 */
+    int num_groups;
+    int total_q;
+    int num_q_heads;             /* a multiple of the pool's kv heads */
+    int layer;
+    float scale;
+    int* status;                 /* device int32, optional */
+    void* workspace;             /* device, mq_paged_attend_workspace_bytes() */
+    size_t workspace_bytes;
+} mq_paged_attend_params;
+
+size_t mq_paged_attend_workspace_bytes(const mq_paged_attend_params* params);
+int mq_paged_attend(const mq_paged_attend_params* params, cudaStream_t stream);
+
+/* Attention over a few pages of the context, chosen for each query token and
+ * kv head by the pool's index.  Token i stands at positions[i] of slot
+ * slots[i].  Its own page is always read; of the pages before it, the
+ * top_k - 1 with the highest score (ties: the lowest page first), where
+ *   score(j) = max over the group's q heads of
+ *              2^(eq + e_j) sum_d (qi_d > 0 ? qi_d HI_jd : qi_d LO_jd),
+ * qi and eq being the head's query in whole numbers, as for the index.  All of
+ * it is exact, so the choice does not depend on any order of sums.
+ * selected [n, num_kv_heads, top_k]: the pages' places in the sequence,
+ * ascending, then -1. */
+typedef struct mq_paged_sparse_params {
+    const mq_paged_pool* pool;   /* with an index */
+    const void* q;
+    long long q_token, q_head;
+    void* out;
+    int* selected;               /* device int32 [n, num_kv_heads, top_k] */
+    const int* table;
+    long long table_row;
+    int num_slots;
+    int table_cols;              /* at most 49152 */
+    const int* slots;            /* device int32 [n] */
+    const int* positions;        /* device int32 [n] */
+    int n;
+    int num_q_heads;
+    int layer;
+    int top_k;
+    float scale;
+    int* status;
+    void* workspace;             /* device, mq_paged_sparse_workspace_bytes() */
+    size_t workspace_bytes;
+} mq_paged_sparse_params;
+
+size_t mq_paged_sparse_workspace_bytes(const mq_paged_sparse_params* params);
+int mq_paged_sparse(const mq_paged_sparse_params* params, cudaStream_t stream);
 
 /* Last status recorded by the reference-ABI launchers on this host thread. */
 int mq_get_last_error(void);

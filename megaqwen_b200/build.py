@@ -33,8 +33,10 @@ LIB = LIBDIR / "libmegaqwen_b200.so"
 EXT = PKG / ("_C" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
-CUDA_SOURCES = ["decode.cu", "prefill.cu", "decode_batch.cu"]
-CUDA_HEADERS = ["mq_ptx.cuh", "mq_tc.cuh", "gemm_tc.cuh", "gemm_small.cuh", "gemm_persist.cuh", "gemm_pair.cuh", "attn_tc.cuh", "prefill_kernels.cuh", "attn_fa.cuh"]
+CUDA_SOURCES = ["decode.cu", "prefill.cu", "decode_batch.cu", "paged_pages.cu", "paged_rope.cu", "paged_attn.cu"]
+EXT_SOURCES = ["ext.cpp", "ext_paged.cpp"]
+CUDA_HEADERS = ["mq_ptx.cuh", "mq_tc.cuh", "gemm_tc.cuh", "gemm_small.cuh", "gemm_persist.cuh", "gemm_pair.cuh", "attn_tc.cuh", "prefill_kernels.cuh", "attn_fa.cuh",
+                "paged_common.cuh", "paged_attn.cuh"]
 
 
 def _nvcc() -> str:
@@ -66,7 +68,7 @@ def build_lib(verbose: bool = False, force: bool = False) -> Path:
         return LIB
     LIBDIR.mkdir(exist_ok=True)
     cmd = [_nvcc(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
-           "-Xptxas", "-v", f"-I{INCLUDE}", f"-I{CSRC}", *srcs, "-o", LIB]
+           "--threads", "0", "-Xptxas", "-v", f"-I{INCLUDE}", f"-I{CSRC}", *srcs, "-o", LIB]
     if os.environ.get("MQ_DECODE_TRACE") == "1":
         cmd.insert(1, "-DMQ_DECODE_TRACE=1")
     if os.environ.get("MQ_PROFILE_HOOKS") == "1":
@@ -81,8 +83,8 @@ def build_ext(verbose: bool = False, force: bool = False) -> Path:
     import torch.utils.cpp_extension as ce
     import pybind11
 
-    src = CSRC / "ext.cpp"
-    deps = [src, INCLUDE / "megaqwen_b200.h", LIB, Path(__file__)]
+    srcs = [CSRC / s for s in EXT_SOURCES]
+    deps = srcs + [INCLUDE / "megaqwen_b200.h", LIB, Path(__file__)]
     if not force and not _stale(EXT, deps):
         return EXT
     incs = ce.include_paths(device_type="cuda") + [pybind11.get_include(), sysconfig.get_paths()["include"],
@@ -91,7 +93,7 @@ def build_ext(verbose: bool = False, force: bool = False) -> Path:
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H", "-w",
-           *[f"-I{i}" for i in incs], str(src), "-o", str(EXT),
+           *[f"-I{i}" for i in incs], *[str(s) for s in srcs], "-o", str(EXT),
            *[f"-L{d}" for d in libdirs if "torch" in d], f"-L{LIBDIR}",
            "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lmegaqwen_b200",
            "-Wl,-rpath,$ORIGIN/lib"]

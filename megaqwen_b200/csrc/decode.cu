@@ -2052,6 +2052,9 @@ const char* mq_error_string(int code) {
         case MQ_ERR_BAD_POSITION: return "position out of range";
         case MQ_ERR_CUDA: return "CUDA runtime error";
         case MQ_ERR_WORKSPACE: return "workspace missing or too small";
+        case MQ_ERR_BAD_SLOT: return "slot out of range, named twice or not empty";
+        case MQ_ERR_BAD_PAGE: return "page number out of range or in the wrong state";
+        case MQ_ERR_NO_PAGES: return "not enough free pages";
         default: return "unknown error";
     }
 }

@@ -1,0 +1,392 @@
+// Attention over the paged cache: batches that share a prefix, and sparse
+// attention over pages chosen by score.  Kernels in paged_attn.cuh; here the
+// choice of pages and the host side.
+#include <algorithm>
+
+#include "paged_attn.cuh"
+
+namespace mq {
+namespace paged {
+
+// ---- choosing pages -----------------------------------------------------------------------
+// One CTA per (token, kv head).  Scores of all earlier pages into shared
+// memory as order-preserving 32-bit keys, then a radix selection of the
+// (top_k - 1)-th largest (four passes of 8 bits over shared memory), then the
+// list in ascending order.  Reads 2 D + 1 bytes per page; the sums are whole
+// numbers (dp4a), exact below 2^24, so the keys do not depend on their order.
+constexpr int SEL_THREADS = 512;
+constexpr int SEL_WARPS = SEL_THREADS / 32;
+constexpr int MAX_SPARSE_COLS = 49152;
+constexpr int MAX_SPARSE_GROUP = 64;   // q heads per kv head
+
+struct SelArgs {
+    const signed char* index;   // at the layer
+    long long i_page, i_head;
+    const uint16_t* q;
+    long long q_tok, q_head;
+    const int* table;
+    long long table_row;
+    const int* slots;
+    const int* positions;
+    int* selected;
+    int num_slots, cols, pages, page, hkv, grp, top_k;
+    int* status;
+};
+
+__device__ __forceinline__ uint32_t order_key(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float two_to(int e) { return __int_as_float((e + 127) << 23); }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(SEL_THREADS) select_kernel(const SelArgs a) {
+    constexpr int LP = D / 16;          // lanes per page: 16 channels each
+    constexpr int PPW = 32 / LP;        // pages per warp step
+    extern __shared__ __align__(16) uint8_t sel_smem[];
+    uint32_t* keys = reinterpret_cast<uint32_t*>(sel_smem);                          // [cols]
+    signed char* qpos = reinterpret_cast<signed char*>(sel_smem + (((size_t)a.cols * 4 + 15) & ~(size_t)15));   // [grp][D]
+    signed char* qneg = qpos + a.grp * D;
+    float* qunit = reinterpret_cast<float*>(qneg + a.grp * D);                       // [grp]
+    __shared__ int hist[256];
+    __shared__ int sums[2][SEL_WARPS];
+    __shared__ uint32_t s_prefix;
+    __shared__ int s_need;
+    pdl_wait();
+    pdl_trigger();
+    const int t = blockIdx.x / a.hkv, h = blockIdx.x - t * a.hkv;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int* sel = a.selected + (long long)blockIdx.x * a.top_k;
+    const int slot = a.slots[t], pos = a.positions[t];
+    const bool bad_slot = slot < 0 || slot >= a.num_slots;
+    if (bad_slot || pos < 0 || pos / a.page >= a.cols) {
+        if (threadIdx.x == 0) note_status(a.status, bad_slot ? MQ_ERR_BAD_SLOT : MQ_ERR_BAD_POSITION);
+        for (int i = threadIdx.x; i < a.top_k; i += SEL_THREADS) sel[i] = -1;
+        return;
+    }
+    const int own = pos / a.page, want = a.top_k - 1;
+    if (own <= want || want == 0) {   // every page, or only the token's own: nothing to choose
+        for (int i = threadIdx.x; i < a.top_k; i += SEL_THREADS) sel[i] = want == 0 ? own : i <= own ? i : -1;
+        return;
+    }
+    // the group's queries in whole numbers, split by sign
+    for (int g = warp; g < a.grp; g += SEL_WARPS) {
+        const uint16_t* q = a.q + t * a.q_tok + (h * a.grp + g) * a.q_head;
+        float x[D / 32], m = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            x[i] = Elem<T>::up(q[lane + 32 * i]);
+            m = fmaxf(m, fabsf(x[i]));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        m = fminf(m, Elem<T>::MAX);
+        const int e = m > 0.f ? min(max(ilogbf(m) - 6, -60), 40) : 0;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const float r = fminf(fmaxf(rintf(x[i] * two_to(-e)), -127.f), 127.f);
+            const int v = x[i] == x[i] ? (int)r : 0;
+            qpos[g * D + lane + 32 * i] = (signed char)max(v, 0);
+            qneg[g * D + lane + 32 * i] = (signed char)min(v, 0);
+        }
+        if (lane == 0) qunit[g] = two_to(e);
+    }
+    __syncthreads();
+    const int part = lane % LP;
+    const signed char* ix = a.index + h * a.i_head;
+    const int* row = a.table + slot * a.table_row;
+#pragma unroll 2
+    for (int j0 = warp * PPW; j0 < own; j0 += SEL_WARPS * PPW) {
+        const int j = j0 + lane / LP;
+        int pid = j < own ? row[j] : -1;
+        const bool ok = pid >= 0 && pid < a.pages;
+        if (!ok && j < own) note_status(a.status, MQ_ERR_BAD_PAGE);
+        const signed char* rec = ix + (ok ? pid : 0) * a.i_page;
+        const int4 hi = *reinterpret_cast<const int4*>(rec + part * 16);
+        const int4 lo = *reinterpret_cast<const int4*>(rec + D + part * 16);
+        const int e = rec[2 * D];
+        float best = -INFINITY;
+        for (int g = 0; g < a.grp; ++g) {
+            const int4 p = *reinterpret_cast<const int4*>(qpos + g * D + part * 16);
+            const int4 n = *reinterpret_cast<const int4*>(qneg + g * D + part * 16);
+            int s = __dp4a(p.x, hi.x, 0);
+            s = __dp4a(p.y, hi.y, s);
+            s = __dp4a(p.z, hi.z, s);
+            s = __dp4a(p.w, hi.w, s);
+            s = __dp4a(n.x, lo.x, s);
+            s = __dp4a(n.y, lo.y, s);
+            s = __dp4a(n.z, lo.z, s);
+            s = __dp4a(n.w, lo.w, s);
+#pragma unroll
+            for (int o = LP / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            best = fmaxf(best, (float)s * qunit[g]);
+        }
+        // the record's exponent is within [-60, 40] when this library wrote it
+        if (part == 0 && j < own) keys[j] = ok ? order_key(best * two_to(min(max(e, -60), 40))) : 0u;
+    }
+    __syncthreads();
+
+    uint32_t prefix = 0, mask = 0;
+    int need = want;   // of the keys that match prefix under mask, the largest `need` are wanted
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (threadIdx.x < 256) hist[threadIdx.x] = 0;
+        __syncthreads();
+        for (int j = threadIdx.x; j < own; j += SEL_THREADS) {
+            const uint32_t k = keys[j];
+            if ((k & mask) == prefix) atomicAdd(&hist[k >> shift & 255u], 1);
+        }
+        __syncthreads();
+        if (warp == 0) {
+            // lane i holds bins 255 - 8 i .. 248 - 8 i; the bin in which the count passes `need`
+            int c[8], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                c[i] = hist[255 - 8 * lane - i];
+                sum += c[i];
+            }
+            int x = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            int above = x - sum;
+            if (above < need && need <= x) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (above < need && need <= above + c[i]) {
+                        s_prefix = prefix | (uint32_t)(255 - 8 * lane - i) << shift;
+                        s_need = need - above;
+                        above = need;   // found
+                    } else {
+                        above += c[i];
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        prefix = s_prefix;
+        need = s_need;
+        mask |= 255u << shift;
+    }
+    // keys above `prefix`, and the first `need` equal to it, in ascending order of the page
+    const int seg = (ceil_div(own, SEL_WARPS) + 31) & ~31;
+    const int lo = min(own, warp * seg), hi = min(own, lo + seg);
+    int gt = 0, eq = 0;
+    for (int i = lo; i < hi; i += 32) {
+        const uint32_t k = i + lane < hi ? keys[i + lane] : 0u;
+        gt += __popc(__ballot_sync(0xffffffffu, i + lane < hi && k > prefix));
+        eq += __popc(__ballot_sync(0xffffffffu, i + lane < hi && k == prefix));
+    }
+    if (lane == 0) {
+        sums[0][warp] = gt;
+        sums[1][warp] = eq;
+    }
+    __syncthreads();
+    gt = eq = 0;
+    for (int w = 0; w < warp; ++w) {
+        gt += sums[0][w];
+        eq += sums[1][w];
+    }
+    const unsigned below = (1u << lane) - 1u;
+    for (int i = lo; i < hi; i += 32) {
+        const uint32_t k = i + lane < hi ? keys[i + lane] : 0u;
+        const bool is_gt = i + lane < hi && k > prefix, is_eq = i + lane < hi && k == prefix;
+        const unsigned mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
+        const int eq_at = eq + __popc(me & below);
+        if (is_gt || (is_eq && eq_at < need)) sel[gt + __popc(mg & below) + min(eq_at, need)] = i + lane;
+        gt += __popc(mg);
+        eq += __popc(me);
+    }
+    if (threadIdx.x == 0) sel[want] = own;
+}
+
+// ---- host ----------------------------------------------------------------------------------
+
+PoolView view_of(const mq_paged_pool& p, int layer) {
+    return {(const uint16_t*)p.k + layer * p.k_layer, (const uint16_t*)p.v + layer * p.v_layer, p.k_page, p.k_head,
+            p.v_page, p.v_head, p.num_pages, p.page_size};
+}
+
+// CTAs of the work line: as many as an SM's registers hold (two of 128 threads
+// for head_dim 128, three for 64).
+int row_grid(int D) { return sm_count() * (D == 128 ? 2 : 3); }
+
+size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+size_t row_workspace(int D, long long tokens, int hq, bool attend, bool groups, WsView* v, void* base) {
+    size_t o = 256;
+    const size_t tok = o;
+    if (attend) o += up256((size_t)tokens * sizeof(TokInfo));
+    const size_t rowp = o;
+    if (groups) o += up256((size_t)2 * tokens * hq * (D + 4) * 4);
+    const size_t slots = o;
+    o += up256((size_t)2 * row_grid(D) * ROW_WARPS * RT * (D + 4) * 4);
+    if (v) {
+        uint8_t* b = (uint8_t*)base;
+        v->head = (int*)b;
+        v->tok = (TokInfo*)(b + tok);
+        v->rowp = (float*)(b + rowp);
+        v->slots = (float*)(b + slots);
+    }
+    return o;
+}
+
+template <typename T, int D, int MODE>
+int run_rows(const RowArgs& a, cudaStream_t st) {
+    auto kernel = rows_kernel<T, D, MODE>;
+    const size_t smem = (size_t)ROW_WARPS * RowWarp<T, D>::RING + (MODE == 0 ? sched_bytes(a.B, a.NG) : 0);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return note_cuda(e, "paged attention attribute");
+    const int grid = row_grid(D);
+    e = launch(kernel, dim3(grid), dim3(ROW_THREADS), smem, st, a);
+    const long long rows = (long long)a.total_q * a.hq;
+    if (e == cudaSuccess) {
+        // few rows have many parts each: eight warps to a row as long as that does not exceed two CTAs per SM
+        if (rows <= 2 * sm_count())
+            e = launch(join_kernel<T, D, MODE, 8>, dim3((unsigned)rows), dim3(256), 0, st, a, (long long)grid * ROW_WARPS);
+        else
+            e = launch(join_kernel<T, D, MODE, 1>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, a,
+                       (long long)grid * ROW_WARPS);
+    }
+    return e == cudaSuccess ? MQ_OK : note_cuda(e, "paged attention");
+}
+
+template <int MODE>
+int run_rows_any(const RowArgs& a, int dtype, int D, cudaStream_t st) {
+    if (dtype == MQ_BF16)
+        return D == 128 ? run_rows<__nv_bfloat16, 128, MODE>(a, st) : run_rows<__nv_bfloat16, 64, MODE>(a, st);
+    return D == 128 ? run_rows<__half, 128, MODE>(a, st) : run_rows<__half, 64, MODE>(a, st);
+}
+
+bool q_ok(const void* q, long long tok, long long head) {
+    return q && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && tok % 8 == 0 && head % 8 == 0;
+}
+
+template <typename T, int D>
+int run_select(const SelArgs& s, int n, cudaStream_t st) {
+    const size_t smem = (((size_t)s.cols * 4 + 15) & ~(size_t)15) + (size_t)s.grp * (2 * D + 4);
+    cudaError_t e = cudaFuncSetAttribute(select_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) e = launch(select_kernel<T, D>, dim3((unsigned)n * s.hkv), dim3(SEL_THREADS), smem, st, s);
+    return e == cudaSuccess ? MQ_OK : note_cuda(e, "page selection");
+}
+
+}  // namespace paged
+}  // namespace mq
+
+using namespace mq::paged;
+
+extern "C" {
+
+size_t mq_paged_attend_workspace_bytes(const mq_paged_attend_params* p) {
+    if (!p || !p->pool || p->total_q < 0) return 0;
+    return row_workspace(p->pool->head_dim, p->total_q, p->num_q_heads, true, p->num_groups > 0, nullptr, nullptr);
+}
+
+int mq_paged_attend(const mq_paged_attend_params* p, cudaStream_t st) {
+    if (!p || !pool_ok(p->pool) || p->num_seqs < 0 || p->num_seqs > MAX_SEQS || p->total_q < 0 || p->num_groups < 0 ||
+        p->num_groups > p->num_seqs || p->num_q_heads < 1 || p->num_q_heads % p->pool->num_kv_heads || p->layer < 0 ||
+        p->layer >= p->pool->num_layers || p->num_slots < 1 || p->table_cols < 1 ||
+        (!p->q_starts && p->num_seqs != p->total_q) || (p->num_groups && (!p->group_starts || !p->prefix_pages)))
+        return MQ_ERR_INVALID_ARGUMENT;
+    if (!p->total_q || !p->num_seqs) return p->total_q ? MQ_ERR_INVALID_ARGUMENT : MQ_OK;
+    if (!q_ok(p->q, p->q_token, p->q_head) || !p->out || (reinterpret_cast<uintptr_t>(p->out) & 15) || !p->table ||
+        !p->lengths || !p->slots || (long long)p->total_q * p->num_q_heads > 0x7fffffffll)
+        return MQ_ERR_INVALID_ARGUMENT;
+    if (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255) ||
+        p->workspace_bytes < mq_paged_attend_workspace_bytes(p))
+        return MQ_ERR_WORKSPACE;
+    RowArgs a = {};
+    a.pool = view_of(*p->pool, p->layer);
+    a.q = (const uint16_t*)p->q;
+    a.q_tok = p->q_token;
+    a.q_head = p->q_head;
+    a.out = (uint16_t*)p->out;
+    a.table = p->table;
+    a.table_row = p->table_row;
+    a.num_slots = p->num_slots;
+    a.cols = p->table_cols;
+    a.lengths = p->lengths;
+    a.slots = p->slots;
+    a.q_starts = p->q_starts;
+    a.group_starts = p->group_starts;
+    a.prefix_pages = p->prefix_pages;
+    a.B = p->num_seqs;
+    a.NG = p->num_groups;
+    a.total_q = p->total_q;
+    a.hq = p->num_q_heads;
+    a.hkv = p->pool->num_kv_heads;
+    a.scale_log2 = p->scale * 1.4426950408889634f;
+    a.status = p->status;
+    const int D = p->pool->head_dim;
+    row_workspace(D, p->total_q, p->num_q_heads, true, p->num_groups > 0, &a.ws, p->workspace);
+    return run_rows_any<0>(a, p->pool->dtype, D, st);
+}
+
+size_t mq_paged_sparse_workspace_bytes(const mq_paged_sparse_params* p) {
+    if (!p || !p->pool || p->n < 0) return 0;
+    return row_workspace(p->pool->head_dim, p->n, p->num_q_heads, false, false, nullptr, nullptr);
+}
+
+int mq_paged_sparse(const mq_paged_sparse_params* p, cudaStream_t st) {
+    if (!p || !pool_ok(p->pool) || !p->pool->index || p->n < 0 || p->num_q_heads < 1 ||
+        p->num_q_heads % p->pool->num_kv_heads || p->num_q_heads / p->pool->num_kv_heads > MAX_SPARSE_GROUP || p->layer < 0 ||
+        p->layer >= p->pool->num_layers || p->num_slots < 1 || p->table_cols < 1 || p->table_cols > MAX_SPARSE_COLS ||
+        p->top_k < 1 || p->top_k > MAX_SPARSE_COLS || (long long)p->n * p->num_q_heads > 0x7fffffffll)
+        return MQ_ERR_INVALID_ARGUMENT;
+    if (!p->n) return MQ_OK;
+    if (!q_ok(p->q, p->q_token, p->q_head) || !p->out || (reinterpret_cast<uintptr_t>(p->out) & 15) || !p->selected ||
+        !p->table || !p->slots || !p->positions)
+        return MQ_ERR_INVALID_ARGUMENT;
+    if (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255) ||
+        p->workspace_bytes < mq_paged_sparse_workspace_bytes(p))
+        return MQ_ERR_WORKSPACE;
+    const mq_paged_pool& o = *p->pool;
+    SelArgs s = {};
+    s.index = o.index + p->layer * o.i_layer;
+    s.i_page = o.i_page;
+    s.i_head = o.i_head;
+    s.q = (const uint16_t*)p->q;
+    s.q_tok = p->q_token;
+    s.q_head = p->q_head;
+    s.table = p->table;
+    s.table_row = p->table_row;
+    s.slots = p->slots;
+    s.positions = p->positions;
+    s.selected = p->selected;
+    s.num_slots = p->num_slots;
+    s.cols = p->table_cols;
+    s.pages = o.num_pages;
+    s.page = o.page_size;
+    s.hkv = o.num_kv_heads;
+    s.grp = p->num_q_heads / o.num_kv_heads;
+    s.top_k = p->top_k;
+    s.status = p->status;
+    const int rc = o.dtype == MQ_BF16
+                       ? (o.head_dim == 128 ? run_select<__nv_bfloat16, 128>(s, p->n, st) : run_select<__nv_bfloat16, 64>(s, p->n, st))
+                       : (o.head_dim == 128 ? run_select<__half, 128>(s, p->n, st) : run_select<__half, 64>(s, p->n, st));
+    if (rc) return rc;
+    RowArgs a = {};
+    a.pool = view_of(o, p->layer);
+    a.q = s.q;
+    a.q_tok = p->q_token;
+    a.q_head = p->q_head;
+    a.out = (uint16_t*)p->out;
+    a.table = p->table;
+    a.table_row = p->table_row;
+    a.num_slots = p->num_slots;
+    a.cols = p->table_cols;
+    a.slots = p->slots;
+    a.positions = p->positions;
+    a.selected = p->selected;
+    a.total_q = p->n;
+    a.hq = p->num_q_heads;
+    a.hkv = o.num_kv_heads;
+    a.top_k = p->top_k;
+    a.scale_log2 = p->scale * 1.4426950408889634f;
+    a.status = p->status;
+    row_workspace(o.head_dim, p->n, p->num_q_heads, false, false, &a.ws, p->workspace);
+    return run_rows_any<1>(a, o.dtype, o.head_dim, st);
+}
+
+}  // extern "C"

@@ -4,8 +4,13 @@
 #include <algorithm>
 
 #include "paged_attn.cuh"
+#include "paged_prefix.cuh"
 
 namespace mq {
+
+bool make_tmap_nd(CUtensorMap* map, const void* ptr, bool bf16, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                  const cuuint32_t* box);
+
 namespace paged {
 
 // ---- choosing pages -----------------------------------------------------------------------
@@ -214,22 +219,79 @@ int row_grid(int D) { return sm_count() * (D == 128 ? 2 : 3); }
 
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-size_t row_workspace(int D, long long tokens, int hq, bool attend, bool groups, WsView* v, void* base) {
+// The prefixes go to the tensor-core kernel when a group has more rows than the
+// 16 of a rows_kernel item on average (measured below at the launch).
+bool tc_prefix(long long tokens, int grp, int NG) { return NG > 0 && NG <= PFX_MAX_GROUPS && tokens * grp > 16ll * NG; }
+
+struct Shape {
+    int D, hq;
+    long long tokens;
+    bool attend, groups, tc;
+};
+
+size_t row_workspace(const Shape& s, WsView* v, void* base) {
     size_t o = 256;
-    const size_t tok = o;
-    if (attend) o += up256((size_t)tokens * sizeof(TokInfo));
-    const size_t rowp = o;
-    if (groups) o += up256((size_t)2 * tokens * hq * (D + 4) * 4);
-    const size_t slots = o;
-    o += up256((size_t)2 * row_grid(D) * ROW_WARPS * RT * (D + 4) * 4);
+    auto take = [&](size_t bytes) {
+        const size_t at = o;
+        o += up256(bytes);
+        return at;
+    };
+    const size_t rows = (size_t)s.tokens * s.hq * (s.D + 4) * 4;
+    const size_t tok = take(s.attend ? (size_t)s.tokens * sizeof(TokInfo) : 0);
+    const size_t own = take(s.groups ? rows : 0);
+    const size_t slots = take((size_t)2 * row_grid(s.D) * ROW_WARPS * RT * (s.D + 4) * 4);
+    const size_t pfx = take(s.groups ? (s.tc ? 2 * rows : rows) : 0);
+    const size_t pfx_slots = take(s.tc ? (size_t)2 * sm_count() * PROWS * (s.D + 4) * 4 : 0);
     if (v) {
         uint8_t* b = (uint8_t*)base;
-        v->head = (int*)b;
+        v->head = (long long*)b;
         v->tok = (TokInfo*)(b + tok);
-        v->rowp = (float*)(b + rowp);
+        v->own_rowp = (float*)(b + own);
         v->slots = (float*)(b + slots);
+        v->pfx_rowp = (float*)(b + pfx);
+        v->pfx_slots = (float*)(b + pfx_slots);
     }
     return o;
+}
+
+Shape shape_of(const mq_paged_attend_params* p) {
+    return {p->pool->head_dim, p->num_q_heads, p->total_q, true, p->num_groups > 0,
+            tc_prefix(p->total_q, p->num_q_heads / p->pool->num_kv_heads, p->num_groups)};
+}
+Shape shape_of(const mq_paged_sparse_params* p) {
+    return {p->pool->head_dim, p->num_q_heads, p->n, false, false, false};
+}
+
+// The pool's K or V as a rank-5 map of [64 of D, page] boxes.
+bool pool_map(CUtensorMap* m, const mq_paged_pool& p, const void* base, long long page, long long layer, long long head) {
+    const cuuint64_t row = (cuuint64_t)p.head_dim * 2, block = row * p.page_size;
+    const cuuint64_t dims[5] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.page_size, (cuuint64_t)p.num_kv_heads,
+                                (cuuint64_t)p.num_layers, (cuuint64_t)p.num_pages};
+    // the stride of a dimension of one is never used and may be anything
+    const cuuint64_t strides[4] = {row, p.num_kv_heads > 1 ? (cuuint64_t)head * 2 : block,
+                                   p.num_layers > 1 ? (cuuint64_t)layer * 2 : block,
+                                   p.num_pages > 1 ? (cuuint64_t)page * 2 : block};
+    const cuuint32_t box[5] = {64, (cuuint32_t)p.page_size, 1, 1, 1};
+    return make_tmap_nd(m, base, p.dtype == MQ_BF16, 5, dims, strides, box);
+}
+
+template <typename T, int D>
+int run_prefix(const RowArgs& a, const mq_paged_pool& pool, int layer, cudaStream_t st) {
+    CUtensorMap tk, tv;
+    if (!pool_map(&tk, pool, pool.k, pool.k_page, pool.k_layer, pool.k_head) ||
+        !pool_map(&tv, pool, pool.v, pool.v_page, pool.v_layer, pool.v_head))
+        return MQ_ERR_CUDA;
+    auto kernel = prefix_kernel<T, D>;
+    const size_t smem = PfxSmem<D>::bytes(a.NG);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) e = launch(kernel, dim3(sm_count()), dim3(PFX_THREADS), smem, st, tk, tv, a, layer);
+    return e == cudaSuccess ? MQ_OK : note_cuda(e, "paged prefix attention");
+}
+
+int run_prefix_any(const RowArgs& a, const mq_paged_pool& p, int layer, cudaStream_t st) {
+    if (p.dtype == MQ_BF16)
+        return p.head_dim == 128 ? run_prefix<__nv_bfloat16, 128>(a, p, layer, st) : run_prefix<__nv_bfloat16, 64>(a, p, layer, st);
+    return p.head_dim == 128 ? run_prefix<__half, 128>(a, p, layer, st) : run_prefix<__half, 64>(a, p, layer, st);
 }
 
 template <typename T, int D, int MODE>
@@ -279,8 +341,8 @@ using namespace mq::paged;
 extern "C" {
 
 size_t mq_paged_attend_workspace_bytes(const mq_paged_attend_params* p) {
-    if (!p || !p->pool || p->total_q < 0) return 0;
-    return row_workspace(p->pool->head_dim, p->total_q, p->num_q_heads, true, p->num_groups > 0, nullptr, nullptr);
+    if (!p || !p->pool || p->total_q < 0 || p->pool->num_kv_heads < 1) return 0;
+    return row_workspace(shape_of(p), nullptr, nullptr);
 }
 
 int mq_paged_attend(const mq_paged_attend_params* p, cudaStream_t st) {
@@ -318,14 +380,19 @@ int mq_paged_attend(const mq_paged_attend_params* p, cudaStream_t st) {
     a.hkv = p->pool->num_kv_heads;
     a.scale_log2 = p->scale * 1.4426950408889634f;
     a.status = p->status;
-    const int D = p->pool->head_dim;
-    row_workspace(D, p->total_q, p->num_q_heads, true, p->num_groups > 0, &a.ws, p->workspace);
-    return run_rows_any<0>(a, p->pool->dtype, D, st);
+    const Shape s = shape_of(p);
+    row_workspace(s, &a.ws, p->workspace);
+    a.tc = s.tc;
+    if (a.tc) {
+        const int rc = run_prefix_any(a, *p->pool, p->layer, st);
+        if (rc) return rc;
+    }
+    return run_rows_any<0>(a, p->pool->dtype, s.D, st);
 }
 
 size_t mq_paged_sparse_workspace_bytes(const mq_paged_sparse_params* p) {
     if (!p || !p->pool || p->n < 0) return 0;
-    return row_workspace(p->pool->head_dim, p->n, p->num_q_heads, false, false, nullptr, nullptr);
+    return row_workspace(shape_of(p), nullptr, nullptr);
 }
 
 int mq_paged_sparse(const mq_paged_sparse_params* p, cudaStream_t st) {
@@ -385,7 +452,7 @@ int mq_paged_sparse(const mq_paged_sparse_params* p, cudaStream_t st) {
     a.top_k = p->top_k;
     a.scale_log2 = p->scale * 1.4426950408889634f;
     a.status = p->status;
-    row_workspace(o.head_dim, p->n, p->num_q_heads, false, false, &a.ws, p->workspace);
+    row_workspace(shape_of(p), &a.ws, p->workspace);
     return run_rows_any<1>(a, o.dtype, o.head_dim, st);
 }
 

@@ -27,6 +27,8 @@ constexpr int ROW_THREADS = 128;
 constexpr int ROW_WARPS = ROW_THREADS / 32;
 constexpr int STAGES = 3;
 constexpr int MAX_SEQS = 2048;
+constexpr int PK = 128;            // keys per tile and query rows per item of the tensor-core prefix kernel
+constexpr int PROWS = 256;
 
 struct PoolView {
     const uint16_t* k;   // at the layer
@@ -40,14 +42,19 @@ struct PoolView {
 struct TokInfo {
     long long own_base, pfx_base;
     int own_ng, own_nrt, own_r0;
-    int pfx_ng, pfx_nrt, pfx_r0;
+    int pfx_ng, pfx_nrt, pfx_r0, pfx_rows;
 };
 
+// Part rows are m, l, pad, pad, acc[D].  A run's split item sits in slot
+// 2 * worker + 1 when the run has the item's start, else in slot 2 * worker;
+// a whole item with another part beside it sits at its output row.
 struct WsView {
-    int* head;          // [0] the call's arguments were in order; [2..3] quota (long long)
+    long long* head;    // [0] the call's arguments were in order, [1] groups per warp, [2] prefix tiles per CTA
     TokInfo* tok;       // [total_q]
-    float* rowp;        // [2][total_q * Hq][D + 4]: whole items that still have another part (0 prefix, 1 own)
-    float* slots;       // [2 * warps][RT][D + 4]: parts of split items
+    float* own_rowp;    // [total_q * Hq][D + 4]
+    float* slots;       // [2 * warps][RT][D + 4]
+    float* pfx_rowp;    // [total_q * Hq][D + 4], twice that with the tensor-core prefix (its two streams)
+    float* pfx_slots;   // [2 * CTAs][PROWS][D + 4], tensor-core prefix only
 };
 
 struct RowArgs {
@@ -66,6 +73,7 @@ struct RowArgs {
     const int* positions;   // sparse
     const int* selected;    // sparse
     int B, NG, total_q, hq, hkv, top_k;
+    int tc;                 // prefixes run on the tensor-core kernel
     float scale_log2;
     int* status;
     WsView ws;
@@ -119,7 +127,18 @@ __device__ __forceinline__ int own_groups(const RowArgs& a, const Sched& s, int 
     return s.len[b] > lo ? ceil_div(s.len[b] - lo, GRP) : 0;
 }
 
-// Returns false (for every thread) when the starts are out of order.
+// Groups (or tiles) of a prefix item and its rows, in the units of the kernel that runs it.
+__device__ __forceinline__ int pfx_groups(const RowArgs& a, int eff) {
+    return a.tc ? ceil_div(eff * a.pool.page, PK) : eff * (a.pool.page / GRP);
+}
+__device__ __forceinline__ int pfx_tiles(const RowArgs& a, int toks, int grp) {
+    const int rt = a.tc ? PROWS : RT;
+    return (int)(((long long)toks * grp + rt - 1) / rt);
+}
+
+// Returns false (for every thread) when the starts are out of order.  PFX: the
+// prefixes alone (s.len and s.grp are not used).
+template <bool PFX>
 __device__ inline bool build_sched(const RowArgs& a, const Sched& s, long long* scratch /* [blockDim / 32] */) {
     const int tid = threadIdx.x, nt = blockDim.x;
     bool bad = false;
@@ -142,11 +161,11 @@ __device__ inline bool build_sched(const RowArgs& a, const Sched& s, long long* 
         const int slot = a.slots[b], ql = q_start(a, b + 1) - q_start(a, b);
         int len = 0;
         if (slot < 0 || slot >= a.num_slots) {
-            if (blockIdx.x == 0) note_status(a.status, MQ_ERR_BAD_SLOT);
+            if (!PFX && blockIdx.x == 0) note_status(a.status, MQ_ERR_BAD_SLOT);
         } else {
             len = a.lengths[slot];
             if (len < 0 || pages_of(len, a.pool.page) > a.cols) {
-                if (blockIdx.x == 0) note_status(a.status, MQ_ERR_BAD_POSITION);
+                if (!PFX && blockIdx.x == 0) note_status(a.status, MQ_ERR_BAD_POSITION);
                 len = 0;
             }
         }
@@ -160,8 +179,10 @@ __device__ inline bool build_sched(const RowArgs& a, const Sched& s, long long* 
             }
             if (s.gs[lo] <= b && b < s.gs[lo + 1]) g = lo;
         }
-        s.len[b] = len;
-        s.grp[b] = g;
+        if (!PFX) {
+            s.len[b] = len;
+            s.grp[b] = g;
+        }
         // the shared part ends where the first query token of any member stands, so all its rows see all of it
         if (g >= 0 && ql > 0) atomicMin(&s.eff[g], max(0, len - ql) / a.pool.page);
     }
@@ -169,19 +190,13 @@ __device__ inline bool build_sched(const RowArgs& a, const Sched& s, long long* 
     for (int g = tid; g < a.NG; g += nt)
         if (s.gs[g + 1] - s.gs[g] < 2) s.eff[g] = 0;   // a group of one shares nothing
     __syncthreads();
-    const int E = a.NG + a.B, grp = a.hq / a.hkv;
+    const int E = a.NG + (PFX ? 0 : a.B), grp = a.hq / a.hkv;
     const int per = ceil_div(E, nt), e0 = min(E, tid * per), e1 = min(E, e0 + per);
     auto cost = [&](int e) -> long long {
-        int toks, ng;
-        if (e < a.NG) {
-            toks = q_start(a, s.gs[e + 1]) - q_start(a, s.gs[e]);
-            ng = s.eff[e] * (a.pool.page / GRP);
-        } else {
-            const int b = e - a.NG;
-            toks = q_start(a, b + 1) - q_start(a, b);
-            ng = own_groups(a, s, b);
-        }
-        return (long long)((toks * (long long)grp + RT - 1) / RT) * ng;
+        if (e < a.NG)
+            return (long long)pfx_tiles(a, q_start(a, s.gs[e + 1]) - q_start(a, s.gs[e]), grp) * pfx_groups(a, s.eff[e]);
+        const int b = e - a.NG;
+        return ((q_start(a, b + 1) - q_start(a, b)) * (long long)grp + RT - 1) / RT * own_groups(a, s, b);
     };
     long long sum = 0;
     for (int e = e0; e < e1; ++e) sum += cost(e);
@@ -431,31 +446,33 @@ __global__ void __launch_bounds__(ROW_THREADS) rows_kernel(const RowArgs a) {
     pdl_wait();
     pdl_trigger();
     Sched s;
-    long long work;
+    long long work, origin = 0;   // where this kernel's work starts on the line
     const int sp_ng = MODE == 1 ? a.top_k * (page / GRP) : 0, sp_nrt = ceil_div(grp, RT);
     if (MODE == 0) {
         s = sched_of(smem + ROW_WARPS * W::RING, a.B, a.NG);
-        const bool ok = build_sched(a, s, scratch);
+        const bool ok = build_sched<false>(a, s, scratch);
         if (blockIdx.x == 0 && threadIdx.x == 0) {
             if (!ok) note_status(a.status, MQ_ERR_INVALID_ARGUMENT);
             a.ws.head[0] = ok;
         }
         if (!ok) return;
-        work = s.off[a.NG + a.B] * a.hkv;
-        if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<long long*>(a.ws.head + 2) = quota_of(work, warps);
+        origin = a.tc ? s.off[a.NG] * a.hkv : 0;
+        work = s.off[a.NG + a.B] * a.hkv - origin;
+        if (blockIdx.x == 0 && threadIdx.x == 0) a.ws.head[1] = quota_of(work, warps);
         // the join's view of the line, a share of the sequences per CTA
         for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
             const int q0 = q_start(a, b), q1 = q_start(a, b + 1), g = s.grp[b];
             TokInfo ti = {};
-            ti.own_base = s.off[a.NG + b] * a.hkv;
+            ti.own_base = s.off[a.NG + b] * a.hkv - origin;
             ti.own_ng = own_groups(a, s, b);
             ti.own_nrt = (int)(((long long)(q1 - q0) * grp + RT - 1) / RT);
             int g0 = 0;
             if (g >= 0 && s.eff[g] > 0) {
                 g0 = q_start(a, s.gs[g]);
                 ti.pfx_base = s.off[g] * a.hkv;
-                ti.pfx_ng = s.eff[g] * (page / GRP);
-                ti.pfx_nrt = (int)(((long long)(q_start(a, s.gs[g + 1]) - g0) * grp + RT - 1) / RT);
+                ti.pfx_ng = pfx_groups(a, s.eff[g]);
+                ti.pfx_rows = (q_start(a, s.gs[g + 1]) - g0) * grp;
+                ti.pfx_nrt = pfx_tiles(a, q_start(a, s.gs[g + 1]) - g0, grp);
             }
             for (int i = q0 + threadIdx.x; i < q1; i += ROW_THREADS) {
                 ti.own_r0 = (i - q0) * grp;
@@ -479,7 +496,7 @@ __global__ void __launch_bounds__(ROW_THREADS) rows_kernel(const RowArgs a) {
         int tok0, h, rt, rows_all, ng, gi, slot, len = 0, ql = 0, base = 0;
         bool prefix = false, other = false;
         if (MODE == 0) {
-            const long long xh = x / a.hkv;
+            const long long xh = (x + origin) / a.hkv;
             int lo = 0, hi = a.NG + a.B;
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
@@ -508,7 +525,7 @@ __global__ void __launch_bounds__(ROW_THREADS) rows_kernel(const RowArgs a) {
                 while (q_start(a, bs + 1) == q_start(a, bs)) ++bs;
             slot = a.slots[bs];
             rows_all = ql * grp;
-            const long long rel = x - s.off[lo] * a.hkv;
+            const long long rel = x + origin - s.off[lo] * a.hkv;
             const int nrt = ceil_div(rows_all, RT), it = (int)(rel / ng);
             gi = (int)(rel - (long long)it * ng);
             h = it / nrt;
@@ -603,7 +620,7 @@ __global__ void __launch_bounds__(ROW_THREADS) rows_kernel(const RowArgs a) {
             if (!whole)
                 w.put_part(a.ws.slots + ((2 * wid + (gi == 0)) * RT + r) * W::LD, i);
             else if (prefix || other)
-                w.put_part(a.ws.rowp + ((prefix ? 0 : (long long)a.total_q * a.hq) + row) * W::LD, i);
+                w.put_part((prefix ? a.ws.pfx_rowp : a.ws.own_rowp) + row * W::LD, i);
             else
                 w.put_out(a.out + row * D, i);
         }
@@ -626,48 +643,73 @@ __global__ void __launch_bounds__(256) join_kernel(const RowArgs a, long long ro
     const int tok = (int)(rowi / a.hq), head = (int)(rowi - (long long)tok * a.hq), grp = a.hq / a.hkv;
     const int h = head / grp;
     uint16_t* out = a.out + rowi * D;
-    const float* base[2] = {nullptr, nullptr};   // first part of the prefix and of the own work
-    int parts[2] = {0, 0}, row[2] = {0, 0};
-    long long w0[2] = {0, 0};
-    long long quota;
+    // the row's parts: np0 of the prefix (sub of them per run), then np1 of its own
+    const float *src0 = nullptr, *src1 = nullptr;
+    long long step0 = 0, step1 = 0;   // floats between parts
+    int np0 = 0, np1 = 0, sub0 = 1;
+    long long first0 = 0, first1 = 0, sub_step0 = 0;   // the first part of a split item is one slot further on
     if (MODE == 0) {
         if (!a.ws.head[0]) {   // refused: zeros
             for (int d = threadIdx.x & (SPLIT > 1 ? 255 : 31); d < D; d += SPLIT > 1 ? 256 : 32) out[d] = 0;
             return;
         }
-        quota = *reinterpret_cast<const long long*>(a.ws.head + 2);
-    } else {
-        quota = quota_of((long long)a.total_q * a.hkv * ceil_div(grp, RT) * (a.top_k * (a.pool.page / GRP)), row_warps);
     }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    const long long quota =
+        MODE == 0 ? a.ws.head[1]
+                  : quota_of((long long)a.total_q * a.hkv * ceil_div(grp, RT) * (a.top_k * (a.pool.page / GRP)), row_warps);
+    {
+        int ng, r;
         long long start;
-        int ng;
         if (MODE == 0) {
             const TokInfo& ti = a.ws.tok[tok];
-            ng = k ? ti.own_ng : ti.pfx_ng;
-            const int r = (k ? ti.own_r0 : ti.pfx_r0) + head % grp;
-            start = (k ? ti.own_base : ti.pfx_base) + ((long long)h * (k ? ti.own_nrt : ti.pfx_nrt) + r / RT) * ng;
-            row[k] = r % RT;
+            ng = ti.own_ng;
+            r = ti.own_r0 + head % grp;
+            start = ti.own_base + ((long long)h * ti.own_nrt + r / RT) * ng;
+            if (ti.pfx_ng) {
+                const int R = a.tc ? PROWS : RT, pr = ti.pfx_r0 + head % grp, in = pr % R;
+                const long long ps = ti.pfx_base + ((long long)h * ti.pfx_nrt + pr / R) * ti.pfx_ng;
+                const long long pq = a.tc ? a.ws.head[2] : quota, w0 = ps / pq;
+                const int runs = (int)((ps + ti.pfx_ng - 1) / pq - w0) + 1;
+                if (a.tc && min(PROWS, ti.pfx_rows - (pr - in)) <= 128) sub0 = 2;   // both streams worked on this row
+                np0 = runs * sub0;
+                if (runs == 1) {
+                    src0 = a.ws.pfx_rowp + rowi * LD;
+                    sub_step0 = (long long)a.total_q * a.hq * LD;
+                } else {
+                    src0 = (a.tc ? a.ws.pfx_slots : a.ws.slots) + (2 * w0 * R + in) * LD;
+                    step0 = 2ll * R * LD;
+                    first0 = (long long)R * LD;
+                    sub_step0 = 128ll * LD;
+                }
+            }
         } else {
-            if (k == 0) continue;
-            const int nrt = ceil_div(grp, RT), r = head % grp;
+            const int nrt = ceil_div(grp, RT);
+            r = head % grp;
             ng = a.top_k * (a.pool.page / GRP);
             start = (((long long)tok * a.hkv + h) * nrt + r / RT) * ng;
-            row[k] = r % RT;
         }
-        if (!ng) continue;
-        w0[k] = start / quota;
-        parts[k] = (int)((start + ng - 1) / quota - w0[k]) + 1;
-        if (parts[k] == 1) base[k] = a.ws.rowp + ((k ? (long long)a.total_q * a.hq : 0) + rowi) * LD;
+        if (ng) {
+            const long long w0 = start / quota;
+            np1 = (int)((start + ng - 1) / quota - w0) + 1;
+            if (np1 == 1) {
+                if (!np0) return;   // written by the only warp that had it
+                src1 = a.ws.own_rowp + rowi * LD;
+            } else {
+                src1 = a.ws.slots + (2 * w0 * RT + r % RT) * LD;
+                step1 = 2ll * RT * LD;
+                first1 = (long long)RT * LD;
+            }
+        }
     }
-    if (parts[0] == 0 && parts[1] == 1) return;   // written by the only warp that had it
     auto part = [&](int i) -> const float* {
-        const int k = i < parts[0] ? 0 : 1, j = k ? i - parts[0] : i;
-        if (base[k]) return base[k];
-        return a.ws.slots + ((2 * (w0[k] + j) + (j == 0)) * RT + row[k]) * LD;
+        if (i < np0) {
+            const int j = i / sub0;
+            return src0 + j * step0 + (j == 0 ? first0 : 0) + (i - j * sub0) * sub_step0;
+        }
+        i -= np0;
+        return src1 + i * step1 + (i == 0 ? first1 : 0);
     };
-    const int np = parts[0] + parts[1];
+    const int np = np0 + np1;
     float M = -INFINITY;
     for (int i = sub + SPLIT * lane; i < np; i += SPLIT * 32) M = fmaxf(M, __ldcg(part(i)));
 #pragma unroll

@@ -14,15 +14,21 @@ bool make_tmap_nd(CUtensorMap* map, const void* ptr, bool bf16, int rank, const 
 namespace paged {
 
 // ---- choosing pages -----------------------------------------------------------------------
-// One CTA per (token, kv head).  Scores of all earlier pages into shared
-// memory as order-preserving 32-bit keys, then a radix selection of the
-// (top_k - 1)-th largest (four passes of 8 bits over shared memory), then the
-// list in ascending order.  Reads 2 D + 1 bytes per page; the sums are whole
-// numbers (dp4a), exact below 2^24, so the keys do not depend on their order.
-constexpr int SEL_THREADS = 512;
-constexpr int SEL_WARPS = SEL_THREADS / 32;
+// One item per (kv head, token), NW warps to an item.  Scores of all earlier
+// pages into shared memory as order-preserving 32-bit keys, then a radix
+// selection of the (top_k - 1)-th largest over the bits in which the keys
+// differ (8 at a time, ending as soon as a whole bin is taken), then the list
+// in ascending order.  Reads 2 D + 1 bytes per page, four pages of a lane in
+// flight; the sums are whole numbers (dp4a), exact below 2^24, so the keys do
+// not depend on their order.
+//
+// NW 16, an item per CTA: few items, whose reads have to be spread.  NW 1,
+// eight items per CTA (consecutive tokens of one head, which read the same
+// records): many items, where the barriers of a CTA per item cost more than the
+// reads (500 tokens x 8 heads, 250 pages each: 121 us with a CTA per item).
 constexpr int MAX_SPARSE_COLS = 49152;
 constexpr int MAX_SPARSE_GROUP = 64;   // q heads per kv head
+constexpr int SEL_UNROLL = 4;
 
 struct SelArgs {
     const signed char* index;   // at the layer
@@ -34,7 +40,7 @@ struct SelArgs {
     const int* slots;
     const int* positions;
     int* selected;
-    int num_slots, cols, pages, page, hkv, grp, top_k;
+    int n, num_slots, cols, pages, shift, hkv, grp, top_k;
     int* status;
 };
 
@@ -44,43 +50,66 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 }
 __device__ __forceinline__ float two_to(int e) { return __int_as_float((e + 127) << 23); }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(SEL_THREADS) select_kernel(const SelArgs a) {
+template <int D>
+__host__ __device__ inline size_t sel_item_bytes(int cols, int grp) {
+    return (((size_t)cols * 4 + (size_t)grp * (2 * D + 4)) + 15) & ~(size_t)15;
+}
+
+template <typename T, int D, int NW>
+__global__ void __launch_bounds__(NW == 1 ? 256 : NW * 32) select_kernel(const SelArgs a) {
     constexpr int LP = D / 16;          // lanes per page: 16 channels each
     constexpr int PPW = 32 / LP;        // pages per warp step
+    constexpr int ITEMS = NW == 1 ? 8 : 1, NT = NW * 32;
     extern __shared__ __align__(16) uint8_t sel_smem[];
-    uint32_t* keys = reinterpret_cast<uint32_t*>(sel_smem);                          // [cols]
-    signed char* qpos = reinterpret_cast<signed char*>(sel_smem + (((size_t)a.cols * 4 + 15) & ~(size_t)15));   // [grp][D]
+    __shared__ int hist[ITEMS][256];
+    __shared__ int sums[2][NW];
+    __shared__ uint32_t s_pick[ITEMS][2];
+    const int lane = threadIdx.x & 31, sub = NW == 1 ? threadIdx.x >> 5 : 0;
+    const int warp = NW == 1 ? 0 : threadIdx.x >> 5, tid = NW == 1 ? lane : threadIdx.x;
+    uint8_t* mem = sel_smem + sub * sel_item_bytes<D>(a.cols, a.grp);
+    signed char* qpos = reinterpret_cast<signed char*>(mem);               // [grp][D]
     signed char* qneg = qpos + a.grp * D;
-    float* qunit = reinterpret_cast<float*>(qneg + a.grp * D);                       // [grp]
-    __shared__ int hist[256];
-    __shared__ int sums[2][SEL_WARPS];
-    __shared__ uint32_t s_prefix;
-    __shared__ int s_need;
+    float* qunit = reinterpret_cast<float*>(qneg + a.grp * D);             // [grp]
+    uint32_t* keys = reinterpret_cast<uint32_t*>(qunit + a.grp);           // [cols]
+    auto sync = [&]() {
+        if (NW == 1) __syncwarp();
+        else __syncthreads();
+    };
     pdl_wait();
     pdl_trigger();
-    const int t = blockIdx.x / a.hkv, h = blockIdx.x - t * a.hkv;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int* sel = a.selected + (long long)blockIdx.x * a.top_k;
-    const int slot = a.slots[t], pos = a.positions[t];
+    const uint32_t item = blockIdx.x * ITEMS + sub;
+    if (item >= (uint32_t)a.n * a.hkv) return;
+    const int h = (int)(item / (uint32_t)a.n), t = (int)(item - (uint32_t)h * a.n);
+    int* sel = a.selected + ((long long)t * a.hkv + h) * a.top_k;
+    const int slot = __ldg(a.slots + t), pos = __ldg(a.positions + t);
     const bool bad_slot = slot < 0 || slot >= a.num_slots;
-    if (bad_slot || pos < 0 || pos / a.page >= a.cols) {
-        if (threadIdx.x == 0) note_status(a.status, bad_slot ? MQ_ERR_BAD_SLOT : MQ_ERR_BAD_POSITION);
-        for (int i = threadIdx.x; i < a.top_k; i += SEL_THREADS) sel[i] = -1;
+    if (bad_slot || pos < 0 || pos >> a.shift >= a.cols) {
+        if (tid == 0) note_status(a.status, bad_slot ? MQ_ERR_BAD_SLOT : MQ_ERR_BAD_POSITION);
+        for (int i = tid; i < a.top_k; i += NT) sel[i] = -1;
         return;
     }
-    const int own = pos / a.page, want = a.top_k - 1;
+    const int own = pos >> a.shift, want = a.top_k - 1;
     if (own <= want || want == 0) {   // every page, or only the token's own: nothing to choose
-        for (int i = threadIdx.x; i < a.top_k; i += SEL_THREADS) sel[i] = want == 0 ? own : i <= own ? i : -1;
+        for (int i = tid; i < a.top_k; i += NT) sel[i] = want == 0 ? own : i <= own ? i : -1;
         return;
+    }
+    // the pages, looked up in one sweep; each place is overwritten by its page's key
+    const int* row = a.table + slot * a.table_row;
+    for (int j = tid; j < own; j += NT) {
+        int pid = __ldg(row + j);
+        if (pid < 0 || pid >= a.pages) {
+            note_status(a.status, MQ_ERR_BAD_PAGE);
+            pid = -1;
+        }
+        keys[j] = (uint32_t)pid;
     }
     // the group's queries in whole numbers, split by sign
-    for (int g = warp; g < a.grp; g += SEL_WARPS) {
+    for (int g = warp; g < a.grp; g += NW) {
         const uint16_t* q = a.q + t * a.q_tok + (h * a.grp + g) * a.q_head;
         float x[D / 32], m = 0.f;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
-            x[i] = Elem<T>::up(q[lane + 32 * i]);
+            x[i] = Elem<T>::up(__ldg(q + lane + 32 * i));
             m = fmaxf(m, fabsf(x[i]));
         }
 #pragma unroll
@@ -96,57 +125,92 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const SelArgs a) {
         }
         if (lane == 0) qunit[g] = two_to(e);
     }
-    __syncthreads();
+    sync();
     const int part = lane % LP;
     const signed char* ix = a.index + h * a.i_head;
-    const int* row = a.table + slot * a.table_row;
-#pragma unroll 2
-    for (int j0 = warp * PPW; j0 < own; j0 += SEL_WARPS * PPW) {
-        const int j = j0 + lane / LP;
-        int pid = j < own ? row[j] : -1;
-        const bool ok = pid >= 0 && pid < a.pages;
-        if (!ok && j < own) note_status(a.status, MQ_ERR_BAD_PAGE);
-        const signed char* rec = ix + (ok ? pid : 0) * a.i_page;
-        const int4 hi = *reinterpret_cast<const int4*>(rec + part * 16);
-        const int4 lo = *reinterpret_cast<const int4*>(rec + D + part * 16);
-        const int e = rec[2 * D];
-        float best = -INFINITY;
+    uint32_t kmin = 0xffffffffu, kmax = 0;
+#pragma unroll 1
+    for (int j0 = warp * PPW + lane / LP; j0 - lane / LP < own; j0 += NW * PPW * SEL_UNROLL) {
+        int4 hi[SEL_UNROLL], lo[SEL_UNROLL];
+        int ex[SEL_UNROLL];
+        bool ok[SEL_UNROLL];
+#pragma unroll
+        for (int u = 0; u < SEL_UNROLL; ++u) {
+            const int j = j0 + u * NW * PPW;
+            const int pid = j < own ? (int)keys[j] : -1;
+            ok[u] = pid >= 0;
+            const signed char* rec = ix + (ok[u] ? pid : 0) * a.i_page;
+            hi[u] = __ldg(reinterpret_cast<const int4*>(rec + part * 16));
+            lo[u] = __ldg(reinterpret_cast<const int4*>(rec + D + part * 16));
+            ex[u] = __ldg(rec + 2 * D);
+        }
+        float best[SEL_UNROLL];
+#pragma unroll
+        for (int u = 0; u < SEL_UNROLL; ++u) best[u] = -INFINITY;
         for (int g = 0; g < a.grp; ++g) {
             const int4 p = *reinterpret_cast<const int4*>(qpos + g * D + part * 16);
             const int4 n = *reinterpret_cast<const int4*>(qneg + g * D + part * 16);
-            int s = __dp4a(p.x, hi.x, 0);
-            s = __dp4a(p.y, hi.y, s);
-            s = __dp4a(p.z, hi.z, s);
-            s = __dp4a(p.w, hi.w, s);
-            s = __dp4a(n.x, lo.x, s);
-            s = __dp4a(n.y, lo.y, s);
-            s = __dp4a(n.z, lo.z, s);
-            s = __dp4a(n.w, lo.w, s);
+            const float unit = qunit[g];
 #pragma unroll
-            for (int o = LP / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            best = fmaxf(best, (float)s * qunit[g]);
+            for (int u = 0; u < SEL_UNROLL; ++u) {
+                int s = __dp4a(p.x, hi[u].x, 0);
+                s = __dp4a(p.y, hi[u].y, s);
+                s = __dp4a(p.z, hi[u].z, s);
+                s = __dp4a(p.w, hi[u].w, s);
+                s = __dp4a(n.x, lo[u].x, s);
+                s = __dp4a(n.y, lo[u].y, s);
+                s = __dp4a(n.z, lo[u].z, s);
+                s = __dp4a(n.w, lo[u].w, s);
+#pragma unroll
+                for (int o = LP / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                best[u] = fmaxf(best[u], (float)s * unit);
+            }
         }
-        // the record's exponent is within [-60, 40] when this library wrote it
-        if (part == 0 && j < own) keys[j] = ok ? order_key(best * two_to(min(max(e, -60), 40))) : 0u;
+        __syncwarp();   // the page numbers are read
+#pragma unroll
+        for (int u = 0; u < SEL_UNROLL; ++u) {
+            const int j = j0 + u * NW * PPW;
+            if (j < own) {
+                // the record's exponent is within [-60, 40] when this library wrote it
+                const uint32_t key = ok[u] ? order_key(best[u] * two_to(min(max(ex[u], -60), 40))) : 0u;
+                if (part == 0) keys[j] = key;
+                kmin = min(kmin, key);
+                kmax = max(kmax, key);
+            }
+        }
     }
-    __syncthreads();
-
-    uint32_t prefix = 0, mask = 0;
-    int need = want;   // of the keys that match prefix under mask, the largest `need` are wanted
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (threadIdx.x < 256) hist[threadIdx.x] = 0;
-        __syncthreads();
-        for (int j = threadIdx.x; j < own; j += SEL_THREADS) {
-            const uint32_t k = keys[j];
-            if ((k & mask) == prefix) atomicAdd(&hist[k >> shift & 255u], 1);
+    kmin = __reduce_min_sync(0xffffffffu, kmin);
+    kmax = __reduce_max_sync(0xffffffffu, kmax);
+    if (NW > 1) {
+        if (lane == 0) {
+            sums[0][warp] = (int)kmin;
+            sums[1][warp] = (int)kmax;
         }
         __syncthreads();
+        kmin = __reduce_min_sync(0xffffffffu, (uint32_t)sums[0][lane % NW]);
+        kmax = __reduce_max_sync(0xffffffffu, (uint32_t)sums[1][lane % NW]);
+    } else {
+        __syncwarp();
+    }
+
+    // keys agree above bit `bits`; of those that match `prefix` under `mask` the largest `need` are wanted
+    int bits = 32 - __clz((int)(kmin ^ kmax)), need = want;
+    uint32_t mask = bits == 32 ? 0u : 0xffffffffu << bits, prefix = kmax & mask;
+    while (bits > 0) {
+        const int shift = max(bits - 8, 0);
+        for (int i = tid; i < 256; i += NT) hist[sub][i] = 0;
+        sync();
+        for (int j = tid; j < own; j += NT) {
+            const uint32_t k = keys[j];
+            if ((k & mask) == prefix) atomicAdd(&hist[sub][(k & ~mask) >> shift], 1);
+        }
+        sync();
         if (warp == 0) {
             // lane i holds bins 255 - 8 i .. 248 - 8 i; the bin in which the count passes `need`
             int c[8], sum = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                c[i] = hist[255 - 8 * lane - i];
+                c[i] = hist[sub][255 - 8 * lane - i];
                 sum += c[i];
             }
             int x = sum;
@@ -160,8 +224,9 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const SelArgs a) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     if (above < need && need <= above + c[i]) {
-                        s_prefix = prefix | (uint32_t)(255 - 8 * lane - i) << shift;
-                        s_need = need - above;
+                        s_pick[sub][0] = prefix | (uint32_t)(255 - 8 * lane - i) << shift;
+                        // what is wanted of the bin, and whether that is all of it
+                        s_pick[sub][1] = (uint32_t)(need - above) << 1 | (need - above == c[i] ? 1u : 0u);
                         above = need;   // found
                     } else {
                         above += c[i];
@@ -169,33 +234,37 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const SelArgs a) {
                 }
             }
         }
-        __syncthreads();
-        prefix = s_prefix;
-        need = s_need;
-        mask |= 255u << shift;
+        sync();
+        prefix = s_pick[sub][0];
+        need = (int)(s_pick[sub][1] >> 1);
+        mask = 0xffffffffu << shift;
+        bits = s_pick[sub][1] & 1u ? 0 : shift;
+        sync();
     }
-    // keys above `prefix`, and the first `need` equal to it, in ascending order of the page
-    const int seg = (ceil_div(own, SEL_WARPS) + 31) & ~31;
+    // keys above the bin, and the first `need` in it, in ascending order of the page
+    const int seg = (ceil_div(own, NW) + 31) & ~31;
     const int lo = min(own, warp * seg), hi = min(own, lo + seg);
     int gt = 0, eq = 0;
-    for (int i = lo; i < hi; i += 32) {
-        const uint32_t k = i + lane < hi ? keys[i + lane] : 0u;
-        gt += __popc(__ballot_sync(0xffffffffu, i + lane < hi && k > prefix));
-        eq += __popc(__ballot_sync(0xffffffffu, i + lane < hi && k == prefix));
-    }
-    if (lane == 0) {
-        sums[0][warp] = gt;
-        sums[1][warp] = eq;
-    }
-    __syncthreads();
-    gt = eq = 0;
-    for (int w = 0; w < warp; ++w) {
-        gt += sums[0][w];
-        eq += sums[1][w];
+    if (NW > 1) {
+        for (int i = lo; i < hi; i += 32) {
+            const uint32_t k = i + lane < hi ? keys[i + lane] & mask : 0u;
+            gt += __popc(__ballot_sync(0xffffffffu, i + lane < hi && k > prefix));
+            eq += __popc(__ballot_sync(0xffffffffu, i + lane < hi && k == prefix));
+        }
+        if (lane == 0) {
+            sums[0][warp] = gt;
+            sums[1][warp] = eq;
+        }
+        __syncthreads();
+        gt = eq = 0;
+        for (int w = 0; w < warp; ++w) {
+            gt += sums[0][w];
+            eq += sums[1][w];
+        }
     }
     const unsigned below = (1u << lane) - 1u;
     for (int i = lo; i < hi; i += 32) {
-        const uint32_t k = i + lane < hi ? keys[i + lane] : 0u;
+        const uint32_t k = i + lane < hi ? keys[i + lane] & mask : 0u;
         const bool is_gt = i + lane < hi && k > prefix, is_eq = i + lane < hi && k == prefix;
         const unsigned mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
         const int eq_at = eq + __popc(me & below);
@@ -203,14 +272,14 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const SelArgs a) {
         gt += __popc(mg);
         eq += __popc(me);
     }
-    if (threadIdx.x == 0) sel[want] = own;
+    if (tid == 0) sel[want] = own;
 }
 
 // ---- host ----------------------------------------------------------------------------------
 
 PoolView view_of(const mq_paged_pool& p, int layer) {
     return {(const uint16_t*)p.k + layer * p.k_layer, (const uint16_t*)p.v + layer * p.v_layer, p.k_page, p.k_head,
-            p.v_page, p.v_head, p.num_pages, p.page_size};
+            p.v_page, p.v_head, p.num_pages, p.page_size, __builtin_ctz((unsigned)p.page_size)};
 }
 
 // CTAs of the work line: as many as an SM's registers hold (two of 128 threads
@@ -220,8 +289,11 @@ int row_grid(int D) { return sm_count() * (D == 128 ? 2 : 3); }
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // The prefixes go to the tensor-core kernel when a group has more rows than the
-// 16 of a rows_kernel item on average (measured below at the launch).
-bool tc_prefix(long long tokens, int grp, int NG) { return NG > 0 && NG <= PFX_MAX_GROUPS && tokens * grp > 16ll * NG; }
+// 16 of a rows_kernel item on average.  (A scale of zero stays out: there a
+// masked score of minus infinity would not stay one.)
+bool tc_prefix(long long tokens, int grp, int NG, float scale) {
+    return NG > 0 && NG <= PFX_MAX_GROUPS && tokens * grp > 16ll * NG && scale != 0.f;
+}
 
 struct Shape {
     int D, hq;
@@ -244,7 +316,7 @@ size_t row_workspace(const Shape& s, WsView* v, void* base) {
     const size_t pfx_slots = take(s.tc ? (size_t)2 * sm_count() * PROWS * (s.D + 4) * 4 : 0);
     if (v) {
         uint8_t* b = (uint8_t*)base;
-        v->head = (long long*)b;
+        v->head = (uint32_t*)b;
         v->tok = (TokInfo*)(b + tok);
         v->own_rowp = (float*)(b + own);
         v->slots = (float*)(b + slots);
@@ -256,7 +328,7 @@ size_t row_workspace(const Shape& s, WsView* v, void* base) {
 
 Shape shape_of(const mq_paged_attend_params* p) {
     return {p->pool->head_dim, p->num_q_heads, p->total_q, true, p->num_groups > 0,
-            tc_prefix(p->total_q, p->num_q_heads / p->pool->num_kv_heads, p->num_groups)};
+            tc_prefix(p->total_q, p->num_q_heads / p->pool->num_kv_heads, p->num_groups, p->scale)};
 }
 Shape shape_of(const mq_paged_sparse_params* p) {
     return {p->pool->head_dim, p->num_q_heads, p->n, false, false, false};
@@ -304,12 +376,12 @@ int run_rows(const RowArgs& a, cudaStream_t st) {
     e = launch(kernel, dim3(grid), dim3(ROW_THREADS), smem, st, a);
     const long long rows = (long long)a.total_q * a.hq;
     if (e == cudaSuccess) {
-        // few rows have many parts each: eight warps to a row as long as that does not exceed two CTAs per SM
-        if (rows <= 2 * sm_count())
-            e = launch(join_kernel<T, D, MODE, 8>, dim3((unsigned)rows), dim3(256), 0, st, a, (long long)grid * ROW_WARPS);
+        // eight warps to a row until that is several waves of CTAs
+        if (rows <= 32 * sm_count())
+            e = launch(join_kernel<T, D, MODE, 8>, dim3((unsigned)rows), dim3(256), 0, st, a, (uint32_t)grid * ROW_WARPS);
         else
             e = launch(join_kernel<T, D, MODE, 1>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, a,
-                       (long long)grid * ROW_WARPS);
+                       (uint32_t)grid * ROW_WARPS);
     }
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "paged attention");
 }
@@ -325,12 +397,23 @@ bool q_ok(const void* q, long long tok, long long head) {
     return q && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && tok % 8 == 0 && head % 8 == 0;
 }
 
-template <typename T, int D>
-int run_select(const SelArgs& s, int n, cudaStream_t st) {
-    const size_t smem = (((size_t)s.cols * 4 + 15) & ~(size_t)15) + (size_t)s.grp * (2 * D + 4);
-    cudaError_t e = cudaFuncSetAttribute(select_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = launch(select_kernel<T, D>, dim3((unsigned)n * s.hkv), dim3(SEL_THREADS), smem, st, s);
+template <typename T, int D, int NW>
+int launch_select(const SelArgs& s, cudaStream_t st) {
+    constexpr int ITEMS = NW == 1 ? 8 : 1;
+    const size_t smem = ITEMS * sel_item_bytes<D>(s.cols, s.grp);
+    const long long items = (long long)s.n * s.hkv;
+    auto kernel = select_kernel<T, D, NW>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) e = launch(kernel, dim3((unsigned)((items + ITEMS - 1) / ITEMS)), dim3(NW == 1 ? 256 : NW * 32), smem, st, s);
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "page selection");
+}
+
+template <typename T, int D>
+int run_select(const SelArgs& s, cudaStream_t st) {
+    // a warp to an item once eight of them fill every SM and eight items' keys fit (64 KB)
+    if ((long long)s.n * s.hkv >= 8ll * sm_count() && 8 * sel_item_bytes<D>(s.cols, s.grp) <= 65536)
+        return launch_select<T, D, 1>(s, st);
+    return launch_select<T, D, 16>(s, st);
 }
 
 }  // namespace paged
@@ -378,6 +461,7 @@ int mq_paged_attend(const mq_paged_attend_params* p, cudaStream_t st) {
     a.total_q = p->total_q;
     a.hq = p->num_q_heads;
     a.hkv = p->pool->num_kv_heads;
+    a.grp = a.hq / a.hkv;
     a.scale_log2 = p->scale * 1.4426950408889634f;
     a.status = p->status;
     const Shape s = shape_of(p);
@@ -402,6 +486,10 @@ int mq_paged_sparse(const mq_paged_sparse_params* p, cudaStream_t st) {
         p->top_k < 1 || p->top_k > MAX_SPARSE_COLS || (long long)p->n * p->num_q_heads > 0x7fffffffll)
         return MQ_ERR_INVALID_ARGUMENT;
     if (!p->n) return MQ_OK;
+    // the work line is counted in 31 bits
+    if ((long long)p->n * p->pool->num_kv_heads * ceil_div(p->num_q_heads / p->pool->num_kv_heads, RT) *
+            ((long long)p->top_k * (p->pool->page_size / GRP) + ITEM_UNITS) > 0x7fffffffll)
+        return MQ_ERR_INVALID_ARGUMENT;
     if (!q_ok(p->q, p->q_token, p->q_head) || !p->out || (reinterpret_cast<uintptr_t>(p->out) & 15) || !p->selected ||
         !p->table || !p->slots || !p->positions)
         return MQ_ERR_INVALID_ARGUMENT;
@@ -424,14 +512,15 @@ int mq_paged_sparse(const mq_paged_sparse_params* p, cudaStream_t st) {
     s.num_slots = p->num_slots;
     s.cols = p->table_cols;
     s.pages = o.num_pages;
-    s.page = o.page_size;
+    s.n = p->n;
+    s.shift = __builtin_ctz((unsigned)o.page_size);
     s.hkv = o.num_kv_heads;
     s.grp = p->num_q_heads / o.num_kv_heads;
     s.top_k = p->top_k;
     s.status = p->status;
     const int rc = o.dtype == MQ_BF16
-                       ? (o.head_dim == 128 ? run_select<__nv_bfloat16, 128>(s, p->n, st) : run_select<__nv_bfloat16, 64>(s, p->n, st))
-                       : (o.head_dim == 128 ? run_select<__half, 128>(s, p->n, st) : run_select<__half, 64>(s, p->n, st));
+                       ? (o.head_dim == 128 ? run_select<__nv_bfloat16, 128>(s, st) : run_select<__nv_bfloat16, 64>(s, st))
+                       : (o.head_dim == 128 ? run_select<__half, 128>(s, st) : run_select<__half, 64>(s, st));
     if (rc) return rc;
     RowArgs a = {};
     a.pool = view_of(o, p->layer);
@@ -449,6 +538,7 @@ int mq_paged_sparse(const mq_paged_sparse_params* p, cudaStream_t st) {
     a.total_q = p->n;
     a.hq = p->num_q_heads;
     a.hkv = o.num_kv_heads;
+    a.grp = a.hq / a.hkv;
     a.top_k = p->top_k;
     a.scale_log2 = p->scale * 1.4426950408889634f;
     a.status = p->status;

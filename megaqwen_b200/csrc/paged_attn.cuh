@@ -34,13 +34,15 @@ struct PoolView {
     const uint16_t* k;   // at the layer
     const uint16_t* v;
     long long k_page, k_head, v_page, v_head;   // elements
-    int pages, page;
+    int pages, page, shift;   // page = 1 << shift
 };
+
+__device__ __forceinline__ int pages_for(int len, int shift) { return len <= 0 ? 0 : ((len - 1) >> shift) + 1; }
 
 // What the join needs to know of a token: where its items start on the work
 // line (kv head 0, row tile 0), how long one is, and the token's first row.
 struct TokInfo {
-    long long own_base, pfx_base;
+    uint32_t own_base, pfx_base;
     int own_ng, own_nrt, own_r0;
     int pfx_ng, pfx_nrt, pfx_r0, pfx_rows;
 };
@@ -49,7 +51,7 @@ struct TokInfo {
 // 2 * worker + 1 when the run has the item's start, else in slot 2 * worker;
 // a whole item with another part beside it sits at its output row.
 struct WsView {
-    long long* head;    // [0] the call's arguments were in order, [1] groups per warp, [2] prefix tiles per CTA
+    uint32_t* head;     // [0] the call's arguments were in order, [1] units per warp, [2] units per prefix CTA
     TokInfo* tok;       // [total_q]
     float* own_rowp;    // [total_q * Hq][D + 4]
     float* slots;       // [2 * warps][RT][D + 4]
@@ -72,7 +74,7 @@ struct RowArgs {
     const int* prefix_pages;
     const int* positions;   // sparse
     const int* selected;    // sparse
-    int B, NG, total_q, hq, hkv, top_k;
+    int B, NG, total_q, hq, hkv, grp, top_k;   // grp = hq / hkv
     int tc;                 // prefixes run on the tensor-core kernel
     float scale_log2;
     int* status;
@@ -97,22 +99,27 @@ __device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t& r0, uint32_t& r1, u
 }
 
 // ---- the work line of an attend call --------------------------------------------------
-// Entities: the groups' shared prefixes, then the sequences' own parts.  Built
-// by every CTA for itself in shared memory (a few loads per sequence; a launch
-// of its own would cost more).
+// Entities: the groups' shared prefixes, then the sequences' own parts.  Each
+// has kv heads x row tiles items; an item takes ITEM_UNITS + its 16-position
+// groups (or prefix tiles) of the line, the first units standing for what an
+// item costs beside them (its rows, its part).  Built by every CTA for itself
+// in shared memory (a few loads per sequence; a launch of its own would cost
+// more).
+constexpr int ITEM_UNITS = 2;
+
 struct Sched {
-    long long* off;   // [NG + B + 1] groups of 16 positions before entity e, for one kv head
+    uint32_t* off;    // [NG + B + 1] units before entity e, for one kv head
     int* len;         // [B] length of the sequence, 0 when its slot is wrong
     int* grp;         // [B] its group, or -1
     int* eff;         // [NG] shared pages read for the whole group
     int* gs;          // [NG + 1]
 };
 __host__ __device__ inline size_t sched_bytes(int B, int NG) {
-    return ((size_t)(NG + B + 1) * 8 + (size_t)B * 8 + (size_t)(2 * NG + 1) * 4 + 15) & ~(size_t)15;
+    return ((size_t)(NG + B + 1) * 4 + (size_t)B * 8 + (size_t)(2 * NG + 1) * 4 + 15) & ~(size_t)15;
 }
 __device__ inline Sched sched_of(uint8_t* p, int B, int NG) {
     Sched s;
-    s.off = (long long*)p;
+    s.off = (uint32_t*)p;
     s.len = (int*)(s.off + NG + B + 1);
     s.grp = s.len + B;
     s.eff = s.grp + B;
@@ -120,111 +127,143 @@ __device__ inline Sched sched_of(uint8_t* p, int B, int NG) {
     return s;
 }
 
-__device__ __forceinline__ int q_start(const RowArgs& a, int b) { return a.q_starts ? a.q_starts[b] : b; }
+__device__ __forceinline__ int q_start(const RowArgs& a, int b) { return a.q_starts ? __ldg(a.q_starts + b) : b; }
 
 __device__ __forceinline__ int own_groups(const RowArgs& a, const Sched& s, int b) {
-    const int lo = s.grp[b] >= 0 ? s.eff[s.grp[b]] * a.pool.page : 0;
-    return s.len[b] > lo ? ceil_div(s.len[b] - lo, GRP) : 0;
+    const int lo = s.grp[b] >= 0 ? s.eff[s.grp[b]] << a.pool.shift : 0;
+    return s.len[b] > lo ? ((s.len[b] - lo - 1) >> 4) + 1 : 0;
 }
+__device__ __forceinline__ int row_tiles(int rows) { return (int)(((uint32_t)rows + RT - 1) >> 4); }
 
 // Groups (or tiles) of a prefix item and its rows, in the units of the kernel that runs it.
 __device__ __forceinline__ int pfx_groups(const RowArgs& a, int eff) {
-    return a.tc ? ceil_div(eff * a.pool.page, PK) : eff * (a.pool.page / GRP);
+    return a.tc ? (int)((((uint32_t)eff << a.pool.shift) + PK - 1) >> 7) : eff << (a.pool.shift - 4);
 }
-__device__ __forceinline__ int pfx_tiles(const RowArgs& a, int toks, int grp) {
-    const int rt = a.tc ? PROWS : RT;
-    return (int)(((long long)toks * grp + rt - 1) / rt);
+__device__ __forceinline__ int pfx_tiles(const RowArgs& a, int rows) {
+    return a.tc ? (int)(((uint32_t)rows + PROWS - 1) >> 8) : row_tiles(rows);
 }
 
-// Returns false (for every thread) when the starts are out of order.  PFX: the
-// prefixes alone (s.len and s.grp are not used).
-template <bool PFX>
-__device__ inline bool build_sched(const RowArgs& a, const Sched& s, long long* scratch /* [blockDim / 32] */) {
-    const int tid = threadIdx.x, nt = blockDim.x;
+// Returns false (for every thread) when the starts are out of order or the
+// line is longer than 2^31 units.  PFX: the prefixes alone (s.len and s.grp
+// are not used).  NT threads.
+template <bool PFX, int NT>
+__device__ inline bool build_sched(const RowArgs& a, const Sched& s, unsigned long long* scratch /* [NT / 32] */) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     bool bad = false;
-    for (int g = tid; a.NG && g <= a.NG; g += nt) {   // without groups there are no arrays of them
-        const int x = a.group_starts[g];
-        if (x < 0 || x > a.B) bad = true;
-        s.gs[g] = x;   // used only when every start is in order
-        if (g < a.NG) {
-            if (a.group_starts[g + 1] < x) bad = true;
-            s.eff[g] = min(max(a.prefix_pages[g], 0), a.cols);
+    // the first sequence's slot and length are on their way while the starts are checked
+    int slot0 = -1, len0 = 0;
+    if (tid < a.B) {
+        slot0 = __ldg(a.slots + tid);
+        if (slot0 >= 0 && slot0 < a.num_slots) len0 = __ldg(a.lengths + slot0);
+    }
+    if (a.NG) {   // without groups there are no arrays of them
+        for (int g = tid; g <= a.NG; g += NT) {
+            const int x = __ldg(a.group_starts + g);
+            if (x < 0 || x > a.B) bad = true;
+            s.gs[g] = x;   // used only when every start is in order
+            if (g < a.NG) {
+                const int members = __ldg(a.group_starts + g + 1) - x;
+                if (members < 0) bad = true;
+                s.eff[g] = members < 2 ? 0 : min(max(__ldg(a.prefix_pages + g), 0), a.cols);   // one alone shares nothing
+            }
         }
     }
     if (a.q_starts) {
-        for (int b = tid; b < a.B; b += nt)
-            if (a.q_starts[b + 1] < a.q_starts[b]) bad = true;
-        if (tid == 0 && (a.q_starts[0] != 0 || a.q_starts[a.B] != a.total_q)) bad = true;
+        for (int b = tid; b < a.B; b += NT)
+            if (__ldg(a.q_starts + b + 1) < __ldg(a.q_starts + b)) bad = true;
+        if (tid == 0 && (__ldg(a.q_starts) != 0 || __ldg(a.q_starts + a.B) != a.total_q)) bad = true;
     }
     if (__syncthreads_or(bad)) return false;
-    for (int b = tid; b < a.B; b += nt) {
-        const int slot = a.slots[b], ql = q_start(a, b + 1) - q_start(a, b);
-        int len = 0;
-        if (slot < 0 || slot >= a.num_slots) {
-            if (!PFX && blockIdx.x == 0) note_status(a.status, MQ_ERR_BAD_SLOT);
-        } else {
-            len = a.lengths[slot];
-            if (len < 0 || pages_of(len, a.pool.page) > a.cols) {
-                if (!PFX && blockIdx.x == 0) note_status(a.status, MQ_ERR_BAD_POSITION);
-                len = 0;
+    for (int b0 = tid & ~31; b0 < a.B; b0 += NT) {   // a warp's 32 sequences together
+        const int b = b0 + lane;
+        const bool in = b < a.B;
+        int len = 0, ql = 0, g = -1;
+        if (in) {
+            const int slot = b == tid ? slot0 : __ldg(a.slots + b);
+            ql = q_start(a, b + 1) - q_start(a, b);
+            if (slot < 0 || slot >= a.num_slots) {
+                if (!PFX && blockIdx.x == 0) note_status(a.status, MQ_ERR_BAD_SLOT);
+            } else {
+                len = b == tid ? len0 : __ldg(a.lengths + slot);
+                if (len < 0 || pages_for(len, a.pool.shift) > a.cols) {
+                    if (!PFX && blockIdx.x == 0) note_status(a.status, MQ_ERR_BAD_POSITION);
+                    len = 0;
+                }
+            }
+            if (a.NG) {
+                int lo = 0, hi = a.NG;   // the last group that starts at or before b
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (s.gs[mid] <= b) lo = mid;
+                    else hi = mid;
+                }
+                if (s.gs[lo] <= b && b < s.gs[lo + 1]) g = lo;
+            }
+            if (!PFX) {
+                s.len[b] = len;
+                s.grp[b] = g;
             }
         }
-        int g = -1;
         if (a.NG) {
-            int lo = 0, hi = a.NG;   // the last group that starts at or before b
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (s.gs[mid] <= b) lo = mid;
-                else hi = mid;
+            // the shared part ends where the first query token of any member stands, so all its rows
+            // see all of it; one update for the warp when its sequences are of one group
+            const int pages = g >= 0 && ql > 0 ? max(0, len - ql) >> a.pool.shift : 0x7fffffff;
+            const int g0 = __shfl_sync(0xffffffffu, g, 0);
+            const bool alone = __all_sync(0xffffffffu, g == g0 || !in);
+            const int least = __reduce_min_sync(0xffffffffu, pages);
+            if (alone) {
+                if (lane == 0 && g0 >= 0) atomicMin(&s.eff[g0], least);
+            } else if (g >= 0) {
+                atomicMin(&s.eff[g], pages);
             }
-            if (s.gs[lo] <= b && b < s.gs[lo + 1]) g = lo;
         }
-        if (!PFX) {
-            s.len[b] = len;
-            s.grp[b] = g;
-        }
-        // the shared part ends where the first query token of any member stands, so all its rows see all of it
-        if (g >= 0 && ql > 0) atomicMin(&s.eff[g], max(0, len - ql) / a.pool.page);
     }
     __syncthreads();
-    for (int g = tid; g < a.NG; g += nt)
-        if (s.gs[g + 1] - s.gs[g] < 2) s.eff[g] = 0;   // a group of one shares nothing
-    __syncthreads();
-    const int E = a.NG + (PFX ? 0 : a.B), grp = a.hq / a.hkv;
-    const int per = ceil_div(E, nt), e0 = min(E, tid * per), e1 = min(E, e0 + per);
-    auto cost = [&](int e) -> long long {
-        if (e < a.NG)
-            return (long long)pfx_tiles(a, q_start(a, s.gs[e + 1]) - q_start(a, s.gs[e]), grp) * pfx_groups(a, s.eff[e]);
-        const int b = e - a.NG;
-        return ((q_start(a, b + 1) - q_start(a, b)) * (long long)grp + RT - 1) / RT * own_groups(a, s, b);
-    };
-    long long sum = 0;
-    for (int e = e0; e < e1; ++e) sum += cost(e);
-    const int lane = tid & 31, warp = tid >> 5;
-    long long x = sum;
+    const int E = a.NG + (PFX ? 0 : a.B);
+    unsigned long long carry = 0;
+    for (int e0 = 0; e0 < E; e0 += NT) {   // NT entities at a time
+        const int e = e0 + tid;
+        unsigned long long cost = 0;
+        if (e < E) {
+            int tiles, ng;
+            if (e < a.NG) {
+                tiles = pfx_tiles(a, (q_start(a, s.gs[e + 1]) - q_start(a, s.gs[e])) * a.grp);
+                ng = pfx_groups(a, s.eff[e]);
+            } else {
+                const int b = e - a.NG;
+                tiles = row_tiles((q_start(a, b + 1) - q_start(a, b)) * a.grp);
+                ng = own_groups(a, s, b);
+            }
+            if (ng) cost = (unsigned long long)(unsigned)tiles * (unsigned)(ng + ITEM_UNITS);
+        }
+        unsigned long long x = cost;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) scratch[warp] = x;
+        __syncthreads();
+        unsigned long long before = carry;
+#pragma unroll
+        for (int w = 0; w < NT / 32; ++w) {
+            const unsigned long long v = scratch[w];
+            if (w < warp) before += v;
+            carry += v;
+        }
+        if (e < E) s.off[e] = (uint32_t)(before + x - cost);
+        __syncthreads();
     }
-    if (lane == 31) scratch[warp] = x;
+    if (tid == 0) s.off[E] = (uint32_t)carry;
     __syncthreads();
-    long long at = x - sum;
-    for (int w = 0; w < warp; ++w) at += scratch[w];
-    for (int e = e0; e < e1; ++e) {
-        s.off[e] = at;
-        at += cost(e);
-    }
-    if (tid == nt - 1) s.off[E] = at;
-    __syncthreads();
-    return true;
+    return carry * (unsigned)a.hkv < 0x7fffffffull;
 }
 
-// Groups per warp: an equal share, but at least two, so that a short call is
-// not cut into more parts than its join is worth.
-__host__ __device__ __forceinline__ long long quota_of(long long work, long long warps) {
-    const long long q = (work + warps - 1) / warps;
-    return q < 2 ? 2 : q;
+// Units per worker: an equal share, but at least an item's own units and two
+// groups, so that a short call is not cut into more parts than its join is worth.
+__device__ __forceinline__ uint32_t quota_of(uint32_t work, uint32_t workers) {
+    const uint32_t q = work / workers + (work % workers ? 1u : 0u);
+    return max(q, (uint32_t)ITEM_UNITS + 2u);
 }
 
 // One warp's 16-position group step and item bookkeeping.
@@ -256,7 +295,7 @@ struct RowWarp {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint16_t* x = p[i & 1];
-                qa[k][i] = x ? *reinterpret_cast<const uint32_t*>(x + 16 * k + 8 * (i >> 1) + 2 * t) : 0u;
+                qa[k][i] = x ? __ldg(reinterpret_cast<const uint32_t*>(x + 16 * k + 8 * (i >> 1) + 2 * t)) : 0u;
             }
     }
 
@@ -433,205 +472,291 @@ struct RowWarp {
     }
 };
 
+// An item as the loading side leaves it for the computing side.
+struct ItemBox {
+    int tok0, h, r0, rows, first;   // rows r0 .. r0 + rows - 1 of the entity; position limit of row r: first + r / grp
+    int fixed;                      // the limit of every row, or -1
+    int n, flags;                   // groups of this run
+};
+constexpr int BOXES = 4;            // the ring spans at most STAGES items, and the one in hand
+enum { BOX_START = 1, BOX_WHOLE = 2, BOX_PREFIX = 4, BOX_OTHER = 8 };
+
 // MODE 0: attend (prefixes and own parts from the schedule).  MODE 1: sparse
 // (token t's item reads the pages selected[t][h][..], top_k of them).
+//
+// Each warp walks its run of the line twice at once: a loading side, STAGES - 1
+// groups ahead, that finds items, looks up pages and issues copies, and a
+// computing side that follows.  The loads of an item's first groups (and its q
+// rows, touched into L1) are under way while the item before is computed; with
+// items of a few groups each the latency would otherwise be paid per item
+// (measured: 5500 cycles for an item of one group).
 template <typename T, int D, int MODE>
 __global__ void __launch_bounds__(ROW_THREADS) rows_kernel(const RowArgs a) {
     using W = RowWarp<T, D>;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long long scratch[ROW_WARPS];
+    __shared__ unsigned long long scratch[ROW_WARPS];
+    __shared__ ItemBox boxes[ROW_WARPS][BOXES];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long wid = (long long)blockIdx.x * ROW_WARPS + warp, warps = (long long)gridDim.x * ROW_WARPS;
-    const int grp = a.hq / a.hkv, page = a.pool.page;
+    const uint32_t wid = blockIdx.x * ROW_WARPS + warp, warps = gridDim.x * ROW_WARPS;
+    const int grp = a.grp, shift = a.pool.shift, page = a.pool.page;
     pdl_wait();
     pdl_trigger();
     Sched s;
-    long long work, origin = 0;   // where this kernel's work starts on the line
-    const int sp_ng = MODE == 1 ? a.top_k * (page / GRP) : 0, sp_nrt = ceil_div(grp, RT);
+    uint32_t work, origin = 0;   // where this kernel's work starts on the line
+    const int sp_nrt = row_tiles(grp), sp_ng = a.top_k << (shift - 4);
     if (MODE == 0) {
         s = sched_of(smem + ROW_WARPS * W::RING, a.B, a.NG);
-        const bool ok = build_sched<false>(a, s, scratch);
-        if (blockIdx.x == 0 && threadIdx.x == 0) {
-            if (!ok) note_status(a.status, MQ_ERR_INVALID_ARGUMENT);
-            a.ws.head[0] = ok;
+        const bool ok = build_sched<false, ROW_THREADS>(a, s, scratch);
+        if (!ok) {
+            if (blockIdx.x == 0 && threadIdx.x == 0) {
+                note_status(a.status, MQ_ERR_INVALID_ARGUMENT);
+                a.ws.head[0] = 0;
+            }
+            return;
         }
-        if (!ok) return;
         origin = a.tc ? s.off[a.NG] * a.hkv : 0;
         work = s.off[a.NG + a.B] * a.hkv - origin;
-        if (blockIdx.x == 0 && threadIdx.x == 0) a.ws.head[1] = quota_of(work, warps);
-        // the join's view of the line, a share of the sequences per CTA
-        for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-            const int q0 = q_start(a, b), q1 = q_start(a, b + 1), g = s.grp[b];
-            TokInfo ti = {};
-            ti.own_base = s.off[a.NG + b] * a.hkv - origin;
-            ti.own_ng = own_groups(a, s, b);
-            ti.own_nrt = (int)(((long long)(q1 - q0) * grp + RT - 1) / RT);
-            int g0 = 0;
-            if (g >= 0 && s.eff[g] > 0) {
-                g0 = q_start(a, s.gs[g]);
-                ti.pfx_base = s.off[g] * a.hkv;
-                ti.pfx_ng = pfx_groups(a, s.eff[g]);
-                ti.pfx_rows = (q_start(a, s.gs[g + 1]) - g0) * grp;
-                ti.pfx_nrt = pfx_tiles(a, q_start(a, s.gs[g + 1]) - g0, grp);
-            }
-            for (int i = q0 + threadIdx.x; i < q1; i += ROW_THREADS) {
-                ti.own_r0 = (i - q0) * grp;
-                ti.pfx_r0 = (i - g0) * grp;
-                a.ws.tok[i] = ti;
-            }
-        }
     } else {
-        work = (long long)a.total_q * a.hkv * sp_nrt * sp_ng;
+        work = (uint32_t)a.total_q * a.hkv * sp_nrt * (sp_ng + ITEM_UNITS);
     }
-    const long long quota = quota_of(work, warps);
-    long long x = wid * quota;
-    const long long xe = min(x + quota, work);
+    const uint32_t quota = quota_of(work, warps);
+
+    // ---- the loading side ----
+    uint32_t x = min(wid * quota, work);   // wid * quota < 2^32: work < 2^31, and quota is about work / warps
+    const uint32_t xe = min(x + quota, work);
+    int e, it, items, ng, nrt;             // entity, item in it, its items, an item's groups and row tiles
+    int slot, base, tok0, rows_all, first, fixed;   // of the entity
+    bool prefix = false, other = false;
+    auto open = [&]() {   // entity e
+        if (MODE == 0) {
+            prefix = e < a.NG;
+            int b0, b1;
+            first = base = 0;
+            fixed = -1;
+            other = false;
+            if (prefix) {
+                b0 = s.gs[e];
+                b1 = s.gs[e + 1];
+                ng = pfx_groups(a, s.eff[e]);
+                fixed = ng * GRP;
+            } else {
+                b0 = e - a.NG;
+                b1 = b0 + 1;
+                ng = own_groups(a, s, b0);
+                other = s.grp[b0] >= 0 && s.eff[s.grp[b0]] > 0;
+                base = other ? s.eff[s.grp[b0]] << shift : 0;
+            }
+            tok0 = q_start(a, b0);
+            const int ql = q_start(a, b1) - tok0;
+            rows_all = ql * grp;
+            if (!prefix) first = s.len[b0] - ql + 1;
+            nrt = prefix ? pfx_tiles(a, rows_all) : row_tiles(rows_all);
+            items = ng ? nrt * a.hkv : 0;
+            if (items) {
+                // a prefix is read through a member's row of the table; a member without query tokens may have none
+                while (prefix && q_start(a, b0 + 1) == q_start(a, b0)) ++b0;
+                slot = __ldg(a.slots + b0);
+            }
+        } else {
+            // (kv head, token), the head outermost: tokens side by side read the same pages' rows of
+            // one head, and those of one head fit L2
+            tok0 = e % a.total_q;
+            slot = __ldg(a.slots + tok0);
+            fixed = __ldg(a.positions + tok0) + 1;
+            rows_all = grp;
+            ng = sp_ng;
+            items = nrt = sp_nrt;
+            first = base = 0;
+        }
+    };
+    int h = 0, g0 = 0, n = 0, k = 0, lim_hi = 0;   // the item's head, its first group and groups in this run, the next one
+    int ids = -1, at = 0;                          // lane i: page and position of the i-th of a batch of 32 groups
+    int ring_at = -1;                              // lane i: position of the group in stage i, or -1 for nothing
+    int stage_l = 0, pushed = 0;
+    auto look = [&]() {
+        const int kk = k + lane;
+        bool want = false;
+        ids = -1;
+        at = 0;
+        if (kk < n) {
+            if (MODE == 0) {
+                at = base + (g0 + kk) * GRP;
+                ids = __ldg(a.table + slot * a.table_row + (at >> shift));
+                want = true;
+            } else {
+                const int j = (g0 + kk) >> (shift - 4);
+                const int c = __ldg(a.selected + ((long long)tok0 * a.hkv + h) * a.top_k + j);
+                if (c >= 0) {   // listed: the slot and the column are in range
+                    at = (c << shift) + (g0 + kk - (j << (shift - 4))) * GRP;
+                    ids = __ldg(a.table + slot * a.table_row + c);
+                    want = true;
+                }
+            }
+            if (ids < 0 || ids >= a.pool.pages) {
+                if (want) note_status(a.status, MQ_ERR_BAD_PAGE);
+                ids = -1;
+            }
+            if (at >= lim_hi) ids = -1;   // past what any row of the tile sees
+        }
+    };
+    // The item at x, if the run has groups of it, into the box.
+    auto next_item = [&]() -> bool {
+        while (x < xe) {
+            while (it >= items) {
+                ++e;
+                it = 0;
+                open();
+            }
+            // x lies in item `it`, which starts at x - within
+            const uint32_t start = MODE == 0 ? s.off[e] * a.hkv - origin + (uint32_t)it * (ng + ITEM_UNITS)
+                                             : ((uint32_t)e * items + it) * (ng + ITEM_UNITS);
+            const uint32_t lo = max(x, start + ITEM_UNITS), hi = min(xe, start + ITEM_UNITS + ng);
+            x = max(x, hi);
+            const int i = it;
+            if (hi == start + ITEM_UNITS + ng) ++it;   // done with it
+            if (lo >= hi) {
+                x = xe;   // the run ends in the item's own units
+                return false;
+            }
+            h = MODE == 0 ? i / nrt : e / a.total_q;
+            const int r0 = (MODE == 0 ? i - h * nrt : i) * RT, rows = min(RT, rows_all - r0);
+            g0 = (int)(lo - start) - ITEM_UNITS;
+            n = (int)(hi - lo);
+            k = 0;
+            lim_hi = fixed >= 0 ? fixed : first + (r0 + rows - 1) / grp;
+            if (lane == 0) {
+                ItemBox& b = boxes[warp][pushed % BOXES];
+                b.tok0 = tok0;
+                b.h = h;
+                b.r0 = r0;
+                b.rows = rows;
+                b.first = first;
+                b.fixed = fixed;
+                b.n = n;
+                b.flags = (g0 == 0 ? BOX_START : 0) | (n == ng ? BOX_WHOLE : 0) | (prefix ? BOX_PREFIX : 0) | (other ? BOX_OTHER : 0);
+            }
+            if (lane < rows) {
+                const int r = r0 + lane;
+                const uint16_t* q = a.q + (long long)(tok0 + r / grp) * a.q_tok + (h * grp + r % grp) * a.q_head;
+                asm volatile("prefetch.global.L1 [%0];" ::"l"(q));
+                if (D == 128) asm volatile("prefetch.global.L1 [%0];" ::"l"(q + 64));
+            }
+            ++pushed;
+            look();
+            return true;
+        }
+        return false;
+    };
 
     W w;
     w.lane = lane;
     w.ring = smem_u32(smem) + warp * W::RING;
-    const int g = lane >> 2;
-    while (x < xe) {
-        // the item at x: entity, kv head, row tile, and the groups of it that are this warp's
-        int tok0, h, rt, rows_all, ng, gi, slot, len = 0, ql = 0, base = 0;
-        bool prefix = false, other = false;
+    if (x < xe) {   // where the run starts
         if (MODE == 0) {
-            const long long xh = (x + origin) / a.hkv;
+            const uint32_t xh = (x + origin) / (uint32_t)a.hkv;
             int lo = 0, hi = a.NG + a.B;
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
                 if (s.off[mid] <= xh) lo = mid;
                 else hi = mid;
             }
-            prefix = lo < a.NG;
-            int b0, b1;
-            if (prefix) {
-                b0 = s.gs[lo];
-                b1 = s.gs[lo + 1];
-                ng = s.eff[lo] * (page / GRP);
-            } else {
-                b0 = lo - a.NG;
-                b1 = b0 + 1;
-                ng = own_groups(a, s, b0);
-                len = s.len[b0];
-                other = s.grp[b0] >= 0 && s.eff[s.grp[b0]] > 0;
-                base = other ? s.eff[s.grp[b0]] * page : 0;
-            }
-            tok0 = q_start(a, b0);
-            ql = q_start(a, b1) - tok0;
-            // a prefix is read through a member's row of the table; a member without query tokens may have none
-            int bs = b0;
-            if (prefix)
-                while (q_start(a, bs + 1) == q_start(a, bs)) ++bs;
-            slot = a.slots[bs];
-            rows_all = ql * grp;
-            const long long rel = x + origin - s.off[lo] * a.hkv;
-            const int nrt = ceil_div(rows_all, RT), it = (int)(rel / ng);
-            gi = (int)(rel - (long long)it * ng);
-            h = it / nrt;
-            rt = it - h * nrt;
+            e = lo;
+            open();
+            it = (int)((x + origin - s.off[e] * a.hkv) / (uint32_t)(ng + ITEM_UNITS));
         } else {
-            ng = sp_ng;
-            const long long it = x / ng;
-            gi = (int)(x - it * ng);
-            rt = (int)(it % sp_nrt);
-            const long long th = it / sp_nrt;
-            h = (int)(th % a.hkv);
-            tok0 = (int)(th / a.hkv);
-            slot = a.slots[tok0];
-            rows_all = grp;
-            len = a.positions[tok0] + 1;
+            const uint32_t i = x / (uint32_t)(sp_ng + ITEM_UNITS);
+            e = (int)(i / (uint32_t)sp_nrt);
+            it = (int)(i - (uint32_t)e * sp_nrt);
+            open();
         }
-        const int n = (int)min((long long)(ng - gi), xe - x);
-        const int r0 = rt * RT, rows = min(RT, rows_all - r0);
-        w.load_q(a, tok0, h, grp, r0, rows);
-        w.reset();
-        // the positions that the tile's rows see: [base, lim(row)), lim rising with the row
-        const int first = len - ql + 1;
-        auto lim = [&](int r) -> int {
-            return MODE == 1 || prefix ? (prefix ? ng * GRP : len) : first + (r0 + min(r, rows - 1)) / grp;
-        };
-        const int lim_lo = lim(0), lim_hi = lim(rows - 1), lim_a = lim(g), lim_b = lim(g + 8);
+    }
+    auto fetch = [&]() {
+        int p = -1;
+        if (k < n || next_item()) {
+            if (k && (k & 31) == 0) look();
+            const int pid = __shfl_sync(0xffffffffu, ids, k & 31), p0 = __shfl_sync(0xffffffffu, at, k & 31);
+            if (pid >= 0) {
+                w.issue(a, stage_l, pid, p0 & (page - 1), h, lim_hi - p0);
+                p = p0;
+            }
+            ++k;
+        }
+        if (lane == stage_l) ring_at = p;
+        stage_l = stage_l == STAGES - 1 ? 0 : stage_l + 1;
+        cp_commit();
+    };
+#pragma unroll 1
+    for (int i = 0; i < STAGES - 1; ++i) fetch();
 
-        // lane i of `ids` knows page and position of the i-th group of a batch of 32
-        int ids = -1, at = 0;
-        auto look = [&](int k0) {
-            const int k = k0 + lane;
-            bool want = false;
-            ids = -1;
-            at = 0;
-            if (k < n) {
-                if (MODE == 0) {
-                    at = base + (gi + k) * GRP;
-                    ids = a.table[slot * a.table_row + at / page];
-                    want = true;
-                } else {
-                    const int per = page / GRP, j = (gi + k) / per;
-                    const int c = a.selected[((long long)tok0 * a.hkv + h) * a.top_k + j];
-                    if (c >= 0) {   // listed: the slot and the column are in range
-                        at = c * page + (gi + k - j * per) * GRP;
-                        ids = a.table[slot * a.table_row + c];
-                        want = true;
-                    }
-                }
-                if (ids < 0 || ids >= a.pool.pages) {
-                    if (want) note_status(a.status, MQ_ERR_BAD_PAGE);
-                    ids = -1;
-                }
-                if (at >= lim_hi) ids = -1;   // past what any row of the tile sees
-            }
-        };
-        int ids_n = -1, at_n = 0;   // the batch before, while the ring straddles two
-        look(0);
-        auto fetch = [&](int k) {
-            if (k < n) {
-                if (k && (k & 31) == 0) {
-                    ids_n = ids;
-                    at_n = at;
-                    look(k);
-                }
-                const int pid = __shfl_sync(0xffffffffu, ids, k & 31), p0 = __shfl_sync(0xffffffffu, at, k & 31);
-                if (pid >= 0) w.issue(a, k % STAGES, pid, p0 & (page - 1), h, lim_hi - p0);
-            }
-            cp_commit();
-        };
-#pragma unroll
-        for (int k = 0; k < STAGES - 1; ++k) fetch(k);
-        for (int k = 0; k < n; ++k) {
-            fetch(k + STAGES - 1);
+    // ---- the computing side ----
+    const int g = lane >> 2;
+    int stage_c = 0;
+    for (int popped = 0; popped < pushed; ++popped) {
+        __syncwarp();
+        const ItemBox b = boxes[warp][popped % BOXES];
+        w.load_q(a, b.tok0, b.h, grp, b.r0, b.rows);
+        w.reset();
+        auto lim = [&](int r) { return b.fixed >= 0 ? b.fixed : b.first + (b.r0 + min(r, b.rows - 1)) / grp; };
+        const int lim_lo = lim(0), lim_top = lim(b.rows - 1), lim_a = lim(g), lim_b = lim(g + 8);
+#pragma unroll 1
+        for (int i = 0; i < b.n; ++i) {
+            fetch();
             cp_wait<STAGES - 1>();
             __syncwarp();
-            // group k may belong to the batch before the one that was looked up last
-            const bool old = (k >> 5) < (min(k + STAGES - 1, n - 1) >> 5);
-            const int pid = __shfl_sync(0xffffffffu, old ? ids_n : ids, k & 31);
-            const int p0 = __shfl_sync(0xffffffffu, old ? at_n : at, k & 31);
-            if (pid >= 0) w.step(k % STAGES, lim_a - p0, lim_b - p0, lim_lo < min(p0 + GRP, lim_hi), a.scale_log2);
+            const int p0 = __shfl_sync(0xffffffffu, ring_at, stage_c);
+            if (p0 >= 0) w.step(stage_c, lim_a - p0, lim_b - p0, lim_lo < min(p0 + GRP, lim_top), a.scale_log2);
+            stage_c = stage_c == STAGES - 1 ? 0 : stage_c + 1;
             __syncwarp();
         }
-        cp_wait<0>();
         w.finish();
-        const bool whole = n == ng;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = g + 8 * i;
-            if (r >= rows) continue;
-            const int tok = tok0 + (r0 + r) / grp, head = h * grp + (r0 + r) % grp;
-            const long long row = (long long)tok * a.hq + head;
-            if (!whole)
-                w.put_part(a.ws.slots + ((2 * wid + (gi == 0)) * RT + r) * W::LD, i);
-            else if (prefix || other)
-                w.put_part((prefix ? a.ws.pfx_rowp : a.ws.own_rowp) + row * W::LD, i);
+            if (r >= b.rows) continue;
+            const int t = (b.r0 + r) / grp;
+            const long long row = (long long)(b.tok0 + t) * a.hq + b.h * grp + b.r0 + r - t * grp;
+            if (!(b.flags & BOX_WHOLE))
+                w.put_part(a.ws.slots + ((2ll * wid + (b.flags & BOX_START ? 1 : 0)) * RT + r) * W::LD, i);
+            else if (b.flags & (BOX_PREFIX | BOX_OTHER))
+                w.put_part((b.flags & BOX_PREFIX ? a.ws.pfx_rowp : a.ws.own_rowp) + row * W::LD, i);
             else
                 w.put_out(a.out + row * D, i);
         }
-        x += n;
+    }
+    cp_wait<0>();
+    if (MODE == 0) {
+        // the join's view of the line, a share of the sequences per warp
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            a.ws.head[0] = 1;
+            a.ws.head[1] = quota;
+        }
+        for (int b = (int)wid; b < a.B; b += (int)warps) {
+            const int q0 = q_start(a, b), q1 = q_start(a, b + 1), gr = s.grp[b];
+            TokInfo ti = {};
+            ti.own_base = s.off[a.NG + b] * a.hkv - origin;
+            ti.own_ng = own_groups(a, s, b);
+            ti.own_nrt = row_tiles((q1 - q0) * grp);
+            int p0 = 0;
+            if (gr >= 0 && s.eff[gr] > 0) {
+                p0 = q_start(a, s.gs[gr]);
+                ti.pfx_base = s.off[gr] * a.hkv;
+                ti.pfx_ng = pfx_groups(a, s.eff[gr]);
+                ti.pfx_rows = (q_start(a, s.gs[gr + 1]) - p0) * grp;
+                ti.pfx_nrt = pfx_tiles(a, ti.pfx_rows);
+            }
+            for (int i = q0 + lane; i < q1; i += 32) {
+                ti.own_r0 = (i - q0) * grp;
+                ti.pfx_r0 = (i - p0) * grp;
+                a.ws.tok[i] = ti;
+            }
+        }
     }
 }
 
 // ---- the join ----------------------------------------------------------------------------
 // SPLIT warps share a row (few rows, many parts) or each warp has its own.
 template <typename T, int D, int MODE, int SPLIT>
-__global__ void __launch_bounds__(256) join_kernel(const RowArgs a, long long row_warps) {
+__global__ void __launch_bounds__(256) join_kernel(const RowArgs a, uint32_t row_warps) {
     constexpr int LD = D + 4, V = D / 32;
     __shared__ float sm_m[8], sm_l[8], sm_o[8][D];
     pdl_wait();
@@ -640,8 +765,8 @@ __global__ void __launch_bounds__(256) join_kernel(const RowArgs a, long long ro
     const long long rowi = SPLIT > 1 ? blockIdx.x : (long long)blockIdx.x * 8 + warp;
     if (rowi >= (long long)a.total_q * a.hq) return;
     const int sub = SPLIT > 1 ? warp : 0;
-    const int tok = (int)(rowi / a.hq), head = (int)(rowi - (long long)tok * a.hq), grp = a.hq / a.hkv;
-    const int h = head / grp;
+    const int tok = (int)((uint32_t)rowi / (uint32_t)a.hq), head = (int)(rowi - (long long)tok * a.hq);   // rows fit 31 bits
+    const int grp = a.grp, h = head / grp;
     uint16_t* out = a.out + rowi * D;
     // the row's parts: np0 of the prefix (sub of them per run), then np1 of its own
     const float *src0 = nullptr, *src1 = nullptr;
@@ -654,21 +779,22 @@ __global__ void __launch_bounds__(256) join_kernel(const RowArgs a, long long ro
             return;
         }
     }
-    const long long quota =
+    const int sp_ng = MODE == 1 ? a.top_k << (a.pool.shift - 4) : 0;
+    const uint32_t quota =
         MODE == 0 ? a.ws.head[1]
-                  : quota_of((long long)a.total_q * a.hkv * ceil_div(grp, RT) * (a.top_k * (a.pool.page / GRP)), row_warps);
+                  : quota_of((uint32_t)a.total_q * a.hkv * row_tiles(grp) * (sp_ng + ITEM_UNITS), row_warps);
     {
         int ng, r;
-        long long start;
+        uint32_t start;   // the item's first group on the line
         if (MODE == 0) {
-            const TokInfo& ti = a.ws.tok[tok];
+            const TokInfo ti = a.ws.tok[tok];
             ng = ti.own_ng;
             r = ti.own_r0 + head % grp;
-            start = ti.own_base + ((long long)h * ti.own_nrt + r / RT) * ng;
+            start = ti.own_base + ((uint32_t)h * ti.own_nrt + r / RT) * (ng + ITEM_UNITS) + ITEM_UNITS;
             if (ti.pfx_ng) {
-                const int R = a.tc ? PROWS : RT, pr = ti.pfx_r0 + head % grp, in = pr % R;
-                const long long ps = ti.pfx_base + ((long long)h * ti.pfx_nrt + pr / R) * ti.pfx_ng;
-                const long long pq = a.tc ? a.ws.head[2] : quota, w0 = ps / pq;
+                const int R = a.tc ? PROWS : RT, pr = ti.pfx_r0 + head % grp, in = pr & (R - 1);
+                const uint32_t ps = ti.pfx_base + ((uint32_t)h * ti.pfx_nrt + (uint32_t)(pr - in) / R) * (ti.pfx_ng + ITEM_UNITS) + ITEM_UNITS;
+                const uint32_t pq = a.tc ? a.ws.head[2] : quota, w0 = ps / pq;
                 const int runs = (int)((ps + ti.pfx_ng - 1) / pq - w0) + 1;
                 if (a.tc && min(PROWS, ti.pfx_rows - (pr - in)) <= 128) sub0 = 2;   // both streams worked on this row
                 np0 = runs * sub0;
@@ -676,26 +802,26 @@ __global__ void __launch_bounds__(256) join_kernel(const RowArgs a, long long ro
                     src0 = a.ws.pfx_rowp + rowi * LD;
                     sub_step0 = (long long)a.total_q * a.hq * LD;
                 } else {
-                    src0 = (a.tc ? a.ws.pfx_slots : a.ws.slots) + (2 * w0 * R + in) * LD;
+                    src0 = (a.tc ? a.ws.pfx_slots : a.ws.slots) + (2ll * w0 * R + in) * LD;
                     step0 = 2ll * R * LD;
                     first0 = (long long)R * LD;
                     sub_step0 = 128ll * LD;
                 }
             }
         } else {
-            const int nrt = ceil_div(grp, RT);
+            const int nrt = row_tiles(grp);
             r = head % grp;
-            ng = a.top_k * (a.pool.page / GRP);
-            start = (((long long)tok * a.hkv + h) * nrt + r / RT) * ng;
+            ng = sp_ng;
+            start = (((uint32_t)h * a.total_q + tok) * nrt + r / RT) * (ng + ITEM_UNITS) + ITEM_UNITS;
         }
         if (ng) {
-            const long long w0 = start / quota;
+            const uint32_t w0 = start / quota;
             np1 = (int)((start + ng - 1) / quota - w0) + 1;
             if (np1 == 1) {
                 if (!np0) return;   // written by the only warp that had it
                 src1 = a.ws.own_rowp + rowi * LD;
             } else {
-                src1 = a.ws.slots + (2 * w0 * RT + r % RT) * LD;
+                src1 = a.ws.slots + (2ll * w0 * RT + r % RT) * LD;
                 step1 = 2ll * RT * LD;
                 first1 = (long long)RT * LD;
             }
@@ -710,26 +836,51 @@ __global__ void __launch_bounds__(256) join_kernel(const RowArgs a, long long ro
         return src1 + i * step1 + (i == 0 ? first1 : 0);
     };
     const int np = np0 + np1;
-    float M = -INFINITY;
-    for (int i = sub + SPLIT * lane; i < np; i += SPLIT * 32) M = fmaxf(M, __ldcg(part(i)));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const float U = M == -INFINITY ? 0.f : M;
-    float L = 0.f, acc[V];
+    // A batch of 32 parts at a time: lane i finds part i and its maximum and sum (one round
+    // trip), then the rows of acc are read eight in flight, whatever their weights are.
+    float M = -INFINITY, L = 0.f, acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
-#pragma unroll 4
-    for (int i = sub; i < np; i += SPLIT) {
-        const float* p = part(i);
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p));
-        const float e = exp2f(ml.x - U);
-        L += ml.y * e;
-        if (V == 4) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p + 4) + lane);
-            acc[0] += v.x * e; acc[1] += v.y * e; acc[V - 2] += v.z * e; acc[V - 1] += v.w * e;
-        } else {
-            const float2 v = __ldcg(reinterpret_cast<const float2*>(p + 4) + lane);
-            acc[0] += v.x * e; acc[1] += v.y * e;
+    for (int i0 = sub; i0 < np; i0 += SPLIT * 32) {
+        const int mine = i0 + SPLIT * lane, cnt = min(32, (np - i0 + SPLIT - 1) / SPLIT);
+        const float* p = mine < np ? part(mine) : nullptr;
+        const float2 ml = p ? __ldcg(reinterpret_cast<const float2*>(p)) : make_float2(-INFINITY, 0.f);
+        float bm = ml.x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, o));
+        const float N = fmaxf(M, bm), U = N == -INFINITY ? 0.f : N;
+        const float c = exp2f(M - U), e = exp2f(ml.x - U);   // 0 for what is not there
+        M = N;
+        float l = ml.y * e;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        L = L * c + l;
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] *= c;
+#pragma unroll 1
+        for (int k = 0; k < cnt; k += 8) {
+            float v[8][V], w[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const float* r = reinterpret_cast<const float*>(
+                    __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), (k + q) & 31));
+                w[q] = __shfl_sync(0xffffffffu, e, (k + q) & 31);
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[q][i] = 0.f;
+                if (k + q < cnt) {
+                    if (V == 4) {
+                        const float4 x = __ldcg(reinterpret_cast<const float4*>(r + 4) + lane);
+                        v[q][0] = x.x; v[q][1] = x.y; v[q][V - 2] = x.z; v[q][V - 1] = x.w;
+                    } else {
+                        const float2 x = __ldcg(reinterpret_cast<const float2*>(r + 4) + lane);
+                        v[q][0] = x.x; v[q][1] = x.y;
+                    }
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[i] += v[q][i] * (k + q < cnt ? w[q] : 0.f);
         }
     }
     if (SPLIT > 1) {

@@ -45,7 +45,7 @@ struct PfxSmem {
     static constexpr int TILE = (D / 64) * PATOM;
     static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE, BAR = 6 * TILE;
     static constexpr int SCHED = BAR + 256;
-    static constexpr size_t bytes(int NG) { return SCHED + (size_t)(NG + 1) * 8 + (size_t)(2 * NG + 1) * 4 + 16 + 1024; }
+    static constexpr size_t bytes(int NG) { return SCHED + (size_t)(NG + 1) * 4 + (size_t)(2 * NG + 1) * 4 + 16 + 1024; }
 };
 
 struct PfxSeg {
@@ -86,8 +86,46 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// Tiles per CTA: an equal share, at least two (both streams have one).
-__host__ __device__ __forceinline__ long long pfx_quota(long long work, long long ctas) { return quota_of(work, ctas); }
+// The same value in every lane, in a form the compiler knows to be uniform.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+template <typename P>
+__device__ __forceinline__ P* from_lane(P* p, int lane) {
+    return reinterpret_cast<P*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), lane));
+}
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r != 0;
+}
+
+// 64 consecutive 32-bit columns of this warp's TMEM lanes, waited for.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float* v) {
+    uint32_t r[64];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(PFX_THREADS, 1)
@@ -108,8 +146,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
     uint64_t* drain = bars + 16;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 17);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-    __shared__ long long scratch[PFX_THREADS / 32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    __shared__ unsigned long long scratch[PFX_THREADS / 32];
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -140,20 +178,22 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
     pdl_trigger();
 
     Sched s;
-    s.off = reinterpret_cast<long long*>(smem + L::SCHED);
+    s.off = reinterpret_cast<uint32_t*>(smem + L::SCHED);
     s.eff = reinterpret_cast<int*>(s.off + a.NG + 1);
     s.gs = s.eff + a.NG;
     s.len = s.grp = nullptr;
-    const bool in_order = build_sched<true>(a, s, scratch);
-    const long long work = in_order ? s.off[a.NG] * a.hkv : 0;
-    const long long quota = pfx_quota(work, gridDim.x);
+    const bool in_order = build_sched<true, PFX_THREADS>(a, s, scratch);
+    const uint32_t work = in_order ? s.off[a.NG] * a.hkv : 0;
+    const uint32_t quota = quota_of(work, gridDim.x);
     if (blockIdx.x == 0 && threadIdx.x == 0) a.ws.head[2] = quota;
-    const long long x0 = blockIdx.x * quota, xe = min(x0 + quota, work);
-    const int grp = a.hq / a.hkv, page = a.pool.page;
+    const uint32_t x0 = min(blockIdx.x * quota, work), xe = min(x0 + quota, work);
+    const int grp = a.grp, page = a.pool.page;
 
-    auto segment = [&](long long x) {
+    // The item at x and the tiles of it in this run (n <= 0: the run has only its own
+    // units); x moves past them.
+    auto segment = [&](uint32_t& x) {
         PfxSeg e;
-        const long long xh = x / a.hkv;
+        const uint32_t xh = x / (uint32_t)a.hkv;
         int lo = 0, hi = a.NG;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
@@ -161,18 +201,20 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
             else hi = mid;
         }
         e.g = lo;
-        e.ng = ceil_div(s.eff[lo] * page, PK);
-        const long long rel = x - s.off[lo] * a.hkv;
+        e.ng = pfx_groups(a, s.eff[lo]);
+        const uint32_t rel = x - s.off[lo] * a.hkv, len = e.ng + ITEM_UNITS, it = rel / len;
+        const int pos = (int)(rel - it * len), left = (int)min(len - pos, xe - x);
         const int all = (q_start(a, s.gs[lo + 1]) - q_start(a, s.gs[lo])) * grp;
-        const int nrt = ceil_div(all, PROWS), it = (int)(rel / e.ng);
-        e.t0 = (int)(rel - (long long)it * e.ng);
-        e.h = it / nrt;
-        e.r0 = (it - e.h * nrt) * PROWS;
+        const int nrt = pfx_tiles(a, all);
+        e.t0 = max(pos - ITEM_UNITS, 0);
+        e.n = max(pos + left - ITEM_UNITS, 0) - e.t0;
+        e.h = (int)(it / (uint32_t)nrt);
+        e.r0 = ((int)it - e.h * nrt) * PROWS;
         e.rows = min(PROWS, all - e.r0);
         e.two = e.rows > 128;
-        e.n = (int)min((long long)(e.ng - e.t0), xe - x);
         e.start = e.t0 == 0;
         e.whole = e.n == e.ng;
+        x += left;
         return e;
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
@@ -196,15 +238,16 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
         const int chunks = PK / page;
         int c = 0;   // tiles so far
         bool ok = true;
-        for (long long x = x0; ok && x < xe;) {
+        for (uint32_t x = x0; ok && x < xe;) {
             const PfxSeg e = segment(x);
+            if (e.n <= 0) continue;
             int b = s.gs[e.g];   // any member's row of the table will do; one without query tokens may have none
             while (q_start(a, b + 1) == q_start(a, b)) ++b;
-            const int* row = a.table + a.slots[b] * a.table_row;
+            const int* row = a.table + __ldg(a.slots + b) * a.table_row;
             const int last = s.eff[e.g] - 1;
             // past the end of the prefix the last page is loaded again: its scores are masked, and its
             // values (not stale shared memory) meet the zero weights
-            auto look = [&](int j) { return lane < chunks ? row[min((e.t0 + j) * chunks + lane, last)] : 0; };
+            auto look = [&](int j) { return lane < chunks ? __ldg(row + min((e.t0 + j) * chunks + lane, last)) : 0; };
             int next = look(0);
             for (int j = 0; j < e.n; ++j, ++c) {
                 int pid = next;
@@ -227,7 +270,6 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
                         tma_load_5d(ring + st * TILE + i * PATOM + lane * page * 128, map, 64 * i, 0, e.h, layer, pid, &full[st]);
                 }
             }
-            x += e.n;
         }
         if (!ok && lane == 0) give_up();
         // copies in flight land before the CTA may end, whatever became of their readers
@@ -237,118 +279,129 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t id_s = pfx_idesc<T>(PK, false), id_o = pfx_idesc<T>(D, true);
-            int c = 0;                          // K tiles of the segments before
-            int np[2] = {0, 0};                 // PVs issued per stream
-            int nq[2] = {0, 0};                 // Q tiles used per stream
-            bool ok = true;
-            for (long long x = x0; ok && x < xe;) {
-                const PfxSeg e = segment(x);
-                int pend[2] = {-1, -1};         // the tile whose PV is due
-                bool first[2] = {true, true};
-                const int c0 = c;
-                auto pv = [&](int q) -> bool {
-                    const int j = pend[q], vc = c0 + j;
-                    if (!wait(&p_full[q], np[q] & 1)) return false;
-                    if (!wait(&v_full[vc & 1], (vc >> 1) & 1)) return false;
-                    tc_fence_after();
-                    const uint32_t sv = smem_u32(smem + L::V + (vc & 1) * TILE);
-                    const uint32_t p = tmem + q * 128, o = tmem + 256 + q * 128;
+        // ---- MMA: the whole warp walks, one elected lane issues.  All 512 columns of
+        // TMEM are this CTA's, so their addresses start at 0 ----
+        constexpr uint32_t id_s = pfx_idesc<T>(PK, false), id_o = pfx_idesc<T>(D, true);
+        const uint32_t base = (smem_u32(pfx_raw) + 1023u) & ~1023u;
+        int c0 = 0;                         // K tiles of the segments before
+        uint32_t np0 = 0, np1 = 0;          // PVs issued per stream
+        uint32_t nq0 = 0, nq1 = 0;          // Q tiles used per stream
+        bool ok = true;
+        auto ready = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); };
+        auto scores = [&](int q, int kc, bool last_use) {
+            const uint32_t sq = base + L::Q + q * TILE, sk = base + L::K + (kc & 1) * TILE;
 #pragma unroll
-                    for (int half = 0; half < 2; ++half)   // the values, then the remainders
-#pragma unroll
-                        for (int k = 0; k < PK / 16; ++k)
-                            tc_mma_f16_ts(o, p + half * 64 + k * 8, sw128_mnmajor_desc(sv + k * 2048), id_o,
-                                          !first[q] || half || k);
-                    first[q] = false;
-                    ++np[q];
-                    pend[q] = -1;
-                    if (!e.two || q == 1) tc_commit(&v_empty[vc & 1]);
-                    return true;
-                };
-                const int steps = e.two ? 2 * e.n : e.n;
-                for (int i = 0; ok && i < steps; ++i) {
-                    const int q = i & 1, j = e.two ? i >> 1 : i;
-                    if (i < 2) {
-                        ok = wait(&q_full[q], nq[q] & 1);
-                        ++nq[q];
-                        if (!ok) break;
-                    }
-                    if (pend[q] >= 0 && !pv(q)) {
-                        ok = false;
-                        break;
-                    }
-                    const int kc = c0 + j;
-                    if (!wait(&k_full[kc & 1], (kc >> 1) & 1)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t sq = smem_u32(smem + L::Q + q * TILE), sk = smem_u32(smem + L::K + (kc & 1) * TILE);
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint32_t off = (k >> 2) * PATOM + (k & 3) * 32;
-                        tc_mma_f16(tmem + q * 128, sw128_kmajor_desc(sq + off), sw128_kmajor_desc(sk + off), id_s, k != 0);
-                    }
-                    tc_commit(&s_full[q]);
-                    if (!e.two || q == 1) tc_commit(&k_empty[kc & 1]);
-                    pend[q] = j;
-                }
-                // the last PV of each stream, the older tile first
-                for (int i = 0; ok && i < 2; ++i) {
-                    const int q = (steps + i) & 1;
-                    if (pend[q] < 0) continue;
-                    if (!pv(q)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_commit(&o_full[q]);
-                }
-                c += e.n;
-                x += e.n;
+            for (int k = 0; k < D / 16; ++k) {
+                const uint32_t off = (k >> 2) * PATOM + (k & 3) * 32;
+                tc_mma_f16(q * 128, sw128_kmajor_desc(sq + off), sw128_kmajor_desc(sk + off), id_s, k != 0);
             }
-            if (!ok) give_up();
-            tc_commit(drain);   // MMAs in flight end before TMEM goes
-            const long long t0 = clock64();
-            while (!mbar_try_wait(drain, 0) && clock64() - t0 < PFX_TIMEOUT) {
+            tc_commit(&s_full[q]);
+            if (last_use) tc_commit(&k_empty[kc & 1]);
+        };
+        auto values = [&](int q, int vc, bool first, bool last_use, bool done) {
+            const uint32_t sv = base + L::V + (vc & 1) * TILE, o = 256 + q * 128;
+#pragma unroll
+            for (int k = 0; k < PK / 16; ++k) {
+                // 16 keys: 8 columns of values, the remainders 16 columns on
+                const uint32_t p = q * 128 + 32 * (k >> 1) + 8 * (k & 1);
+                const uint64_t dv = sw128_mnmajor_desc(sv + k * 2048);
+                tc_mma_f16_ts(o, p, dv, id_o, !first || k);
+                tc_mma_f16_ts(o, p + 16, dv, id_o, 1);
             }
+            if (last_use) tc_commit(&v_empty[vc & 1]);
+            if (done) tc_commit(&o_full[q]);
+        };
+        for (uint32_t x = x0; ok && x < xe;) {
+            const PfxSeg e = segment(x);
+            const int n = uniform(e.n);
+            if (n <= 0) continue;
+            const bool two = uniform(e.two);
+            const int steps = two ? 2 * n : n;
+            // step i: the stream's PV of its tile before (step i - 2), then its S of this one.  All
+            // that the step needs is waited for first: a wait behind issued MMAs takes as long
+            // as those do (measured: 350 to 500 idle cycles for each)
+            for (int i = 0; ok && i < steps + 2; ++i) {
+                const int q = i & 1;
+                const bool pv = i >= 2, sc = i < steps;
+                const int vc = c0 + (two ? (i - 2) >> 1 : i - 2), kc = c0 + (two ? i >> 1 : i);
+                if (!pv && !sc) continue;   // a run of one tile: stream B has none
+                if (sc) {
+                    if (!pv) ok = ready(&q_full[q], (q ? nq1++ : nq0++) & 1);
+                    ok = ok && ready(&k_full[kc & 1], (kc >> 1) & 1);
+                }
+                if (pv) {
+                    ok = ok && ready(&v_full[vc & 1], (vc >> 1) & 1);
+                    ok = ok && ready(&p_full[q], (q ? np1++ : np0++) & 1);
+                }
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    if (pv) values(q, vc, i < 4, !two || q == 1, !sc);
+                    if (sc) scores(q, kc, !two || q == 1);
+                }
+                __syncwarp();
+            }
+            c0 += n;
+        }
+        if (!ok && lane == 0) give_up();
+        if (elect_one()) tc_commit(drain);   // MMAs in flight end before TMEM goes
+        __syncwarp();
+        const long long t0 = clock64();
+        while (!mbar_try_wait(drain, 0) && clock64() - t0 < PFX_TIMEOUT) {
         }
     } else {
         // ---- softmax of stream q: a thread per row ----
         const int q = warp < 7 ? 0 : 1;
         const int quad = warp & 3;                     // the TMEM lanes this warp may touch
-        const int r = quad * 32 + lane;
+        const float scale = fabsf(a.scale_log2);
+        const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
         const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
         const uint32_t sa = tmem + lane_off + q * 128, oa = tmem + lane_off + 256 + q * 128;
         constexpr float GROW = 8.f;
         int ns = 0, no = 0;
         bool ok = true;
-        for (long long x = x0; ok && x < xe;) {
+        for (uint32_t x = x0; ok && x < xe;) {
             const PfxSeg e = segment(x);
-            x += e.n;
+            if (e.n <= 0) continue;
             const int mine = e.two ? e.n : (e.n + 1 - q) >> 1;   // this stream's tiles
-            const int rr = e.two ? q * 128 + r : r;              // row in the item
-            const bool live = rr < e.rows;
-            const int row = e.r0 + rr, tok = q_start(a, s.gs[e.g]) + row / grp, head = e.h * grp + row % grp;
-            const long long orow = (long long)tok * a.hq + head;
+            // lane k knows where row k of this warp comes from and where its part goes (a whole
+            // item's to its output row, a split one's to a slot)
+            const uint16_t* src = nullptr;
             float* part = nullptr;
-            if (live)
-                part = e.whole ? a.ws.pfx_rowp + ((e.two ? 0 : (long long)q * a.total_q * a.hq) + orow) * LD
-                               : a.ws.pfx_slots + ((2ll * blockIdx.x + e.start) * PROWS + (e.two ? rr : q * 128 + r)) * LD;
+            {
+                const int w = quad * 32 + lane, wr = e.two ? q * 128 + w : w;
+                if (wr < e.rows) {
+                    const int t = (e.r0 + wr) / grp, head = e.h * grp + e.r0 + wr - t * grp, tok = q_start(a, s.gs[e.g]) + t;
+                    src = a.q + tok * a.q_tok + head * a.q_head;
+                    part = !e.whole ? a.ws.pfx_slots + ((2ll * blockIdx.x + e.start) * PROWS + q * 128 + w) * LD
+                                    : a.ws.pfx_rowp + ((e.two ? 0 : (long long)q * a.total_q * a.hq) + (long long)tok * a.hq + head) * LD;
+                }
+            }
             if (!mine) {   // a run of one tile: this stream's part is empty
-                if (live)
+                if (part)
                     for (int i = 0; i < LD; ++i) part[i] = i == 0 ? -INFINITY : 0.f;
                 continue;
             }
-            // Q rows, swizzled as TMA would; rows past the end are zero
+            // Q rows, swizzled as TMA would, zeros past the end; a negative scale turns their
+            // signs.  LPR lanes side by side on a row, eight loads in flight.
             {
-                uint8_t* dst = smem + L::Q + q * TILE + r * 128;
-                const uint16_t* src = a.q + tok * a.q_tok + head * a.q_head;
+                constexpr int LPR = D / 8, RPI = 32 / LPR;
+                const int ch = lane % LPR, sub = lane / LPR;
+#pragma unroll 1
+                for (int k0 = 0; k0 < 32; k0 += 8 * RPI) {
+                    uint4 v[8];
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    const uint4 v = live ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(dst + (i >> 3) * PATOM + (((i & 7) ^ (r & 7)) << 4)) = v;
+                    for (int i = 0; i < 8; ++i) {
+                        const uint16_t* row = from_lane(src, k0 + i * RPI + sub);
+                        v[i] = row ? __ldg(reinterpret_cast<const uint4*>(row + ch * 8)) : make_uint4(0, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int w = quad * 32 + k0 + i * RPI + sub;
+                        v[i].x ^= sign; v[i].y ^= sign; v[i].z ^= sign; v[i].w ^= sign;
+                        *reinterpret_cast<uint4*>(smem + L::Q + q * TILE + (ch >> 3) * PATOM + w * 128 +
+                                                  (((ch & 7) ^ (w & 7)) << 4)) = v[i];
+                    }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -364,19 +417,28 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
                 tc_fence_after();
                 const int t = e.t0 + (e.two ? j : 2 * j + q);
                 const int valid = s.eff[e.g] * page - t * PK;
-                float sv[PK];
-#pragma unroll
-                for (int i = 0; i < PK; i += 32) tmem_ld32(sa + i, sv + i);
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int i = 0; i < PK; ++i) sv[i] *= a.scale_log2;
+                // the end of the prefix: scores past it are set to minus infinity in TMEM
                 if (valid < PK) {
+#pragma unroll 1
+                    for (int i = 0; i < PK; i += 32) {
+                        float sv[32];
+                        tmem_ld32(sa + i, sv);
 #pragma unroll
-                    for (int i = 0; i < PK; ++i) sv[i] = i < valid ? sv[i] : -INFINITY;
+                        for (int k = 0; k < 32; ++k) sv[k] = i + k < valid ? sv[k] : -INFINITY;
+                        tmem_st32(sa + i, sv);
+                    }
                 }
+                // two passes over S in TMEM: the code stays small (a run is a few tiles long, and
+                // fetching unrolled code the first time cost more than reading S twice)
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                for (int i = 0; i < PK; i += 64) {
+                    float sv[64];
+                    tmem_ld64(sa + i, sv);
 #pragma unroll
-                for (int i = 0; i < PK; ++i) mx[i & 3] = fmaxf(mx[i & 3], sv[i]);
-                const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    for (int k = 0; k < 64; ++k) mx[k & 3] = fmaxf(mx[k & 3], sv[k]);
+                }
+                const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
                 // a row's maximum moves only when it grew by more than 2^8; weights stay below 256
                 float corr = 1.f;
                 if (tmax > m + GROW) {
@@ -397,19 +459,21 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
                 }
                 const float u = m == -INFINITY ? 0.f : m;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+#pragma unroll 1
                 for (int i = 0; i < PK; i += 32) {
-                    uint32_t hi[16], lo[16];
+                    float sv[32];
+                    uint32_t pk[32];   // 32 weights in 16 columns, their remainders in the next 16
+                    tmem_ld32(sa + i, sv);
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        const float p0 = ex2(sv[i + 2 * k] - u), p1 = ex2(sv[i + 2 * k + 1] - u);
+                        const float p0 = ex2(fmaf(sv[2 * k], scale, -u)), p1 = ex2(fmaf(sv[2 * k + 1], scale, -u));
                         sum[k & 3] += p0 + p1;
-                        hi[k] = Elem<T>::pack(p0, p1);
-                        const float2 b = Elem<T>::up2(hi[k]);
-                        lo[k] = Elem<T>::pack(p0 - b.x, p1 - b.y);
+                        pk[k] = Elem<T>::pack(p0, p1);
+                        const float2 b = Elem<T>::up2(pk[k]);
+                        pk[16 + k] = Elem<T>::pack(p0 - b.x, p1 - b.y);
                     }
-                    tmem_st16_nowait(sa + i / 2, hi);
-                    tmem_st16_nowait(sa + 64 + i / 2, lo);
+                    tmem_st16_nowait(sa + i, pk);
+                    tmem_st16_nowait(sa + i + 16, pk + 16);
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_st_wait();
@@ -425,15 +489,34 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
                 break;
             }
             tc_fence_after();
-            if (live) *reinterpret_cast<float4*>(part) = make_float4(m, l, 0.f, 0.f);
+            // the part rows, 64 columns at a time through this warp's rows of the Q tile (every S
+            // that reads it is done), so that 16 lanes write 256 contiguous bytes of a row
+            {
+                constexpr int W = D / 2, LPR = W / 4;   // 32 rows x 64 (D 128) or 32 (D 64) floats
+                auto stage = [&](int row, int c) -> float4* {   // 16-byte piece c of a row, in this warp's own Q rows
+                    return reinterpret_cast<float4*>(smem + L::Q + q * TILE + (c >> 3) * PATOM + (quad * 32 + row) * 128 +
+                                                     (((c & 7) ^ (row & 7)) << 4));
+                };
+                if (part) *reinterpret_cast<float4*>(part) = make_float4(m, l, 0.f, 0.f);
+#pragma unroll 1
+                for (int i = 0; i < D; i += W) {
 #pragma unroll
-            for (int i = 0; i < D; i += 32) {
-                float v[32];
-                tmem_ld32(oa + i, v);
-                if (live) {
+                    for (int c = 0; c < W; c += 32) {
+                        float v[32];
+                        tmem_ld32(oa + i + c, v);
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4)
-                        *reinterpret_cast<float4*>(part + 4 + i + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                        for (int k = 0; k < 32; k += 4)
+                            *stage(lane, (c + k) >> 2) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                    }
+                    __syncwarp();
+                    constexpr int RPI = 32 / LPR;
+                    const int ch = lane % LPR, sub = lane / LPR;
+#pragma unroll 4
+                    for (int k = sub; k < 32; k += RPI) {
+                        float* to = from_lane(part, k);
+                        if (to) *reinterpret_cast<float4*>(to + 4 + i + ch * 4) = *stage(k, ch);
+                    }
+                    __syncwarp();
                 }
             }
             tc_fence_before();

@@ -2,6 +2,7 @@
 // attention over pages chosen by score.  Kernels in paged_attn.cuh; here the
 // choice of pages and the host side.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_attn.cuh"
 #include "paged_prefix.cuh"
@@ -282,8 +283,22 @@ PoolView view_of(const mq_paged_pool& p, int layer) {
             p.v_page, p.v_head, p.num_pages, p.page_size, __builtin_ctz((unsigned)p.page_size)};
 }
 
-// CTAs of the work line: as many as an SM's registers hold (two of 128 threads
-// for head_dim 128, three for 64).
+// f(T{}, integral_constant<D>) for the pool's type and head_dim.
+template <typename F>
+int dispatch(int dtype, int D, F f) {
+    using D64 = std::integral_constant<int, 64>;
+    using D128 = std::integral_constant<int, 128>;
+    if (dtype == MQ_BF16) return D == 128 ? f(__nv_bfloat16{}, D128{}) : f(__nv_bfloat16{}, D64{});
+    return D == 128 ? f(__half{}, D128{}) : f(__half{}, D64{});
+}
+
+void set_rt(RowArgs& a, bool eight) {
+    a.rt = eight ? 8 : 16;
+    a.rt_shift = eight ? 3 : 4;
+}
+
+// CTAs of the work line, two to an SM for head_dim 128 (rings of 96 KB) and
+// three for 64 (registers).
 int row_grid(int D) { return sm_count() * (D == 128 ? 2 : 3); }
 
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -311,7 +326,7 @@ size_t row_workspace(const Shape& s, WsView* v, void* base) {
     const size_t rows = (size_t)s.tokens * s.hq * (s.D + 4) * 4;
     const size_t tok = take(s.attend ? (size_t)s.tokens * sizeof(TokInfo) : 0);
     const size_t own = take(s.groups ? rows : 0);
-    const size_t slots = take((size_t)2 * row_grid(s.D) * ROW_WARPS * RT * (s.D + 4) * 4);
+    const size_t slots = take((size_t)2 * row_grid(s.D) * ROW_WARPS * MAX_RT * (s.D + 4) * 4);
     const size_t pfx = take(s.groups ? (s.tc ? 2 * rows : rows) : 0);
     const size_t pfx_slots = take(s.tc ? (size_t)2 * sm_count() * PROWS * (s.D + 4) * 4 : 0);
     if (v) {
@@ -334,8 +349,8 @@ Shape shape_of(const mq_paged_sparse_params* p) {
     return {p->pool->head_dim, p->num_q_heads, p->n, false, false, false};
 }
 
-// The pool's K or V as a rank-5 map of [64 of D, page] boxes.
-bool pool_map(CUtensorMap* m, const mq_paged_pool& p, const void* base, long long page, long long layer, long long head) {
+// The pool's K or V as a rank-5 map of boxes of 64 channels x `rows` rows of a page.
+bool pool_map(CUtensorMap* m, const mq_paged_pool& p, const void* base, long long page, long long layer, long long head, int rows) {
     const cuuint64_t row = (cuuint64_t)p.head_dim * 2, block = row * p.page_size;
     const cuuint64_t dims[5] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.page_size, (cuuint64_t)p.num_kv_heads,
                                 (cuuint64_t)p.num_layers, (cuuint64_t)p.num_pages};
@@ -343,41 +358,38 @@ bool pool_map(CUtensorMap* m, const mq_paged_pool& p, const void* base, long lon
     const cuuint64_t strides[4] = {row, p.num_kv_heads > 1 ? (cuuint64_t)head * 2 : block,
                                    p.num_layers > 1 ? (cuuint64_t)layer * 2 : block,
                                    p.num_pages > 1 ? (cuuint64_t)page * 2 : block};
-    const cuuint32_t box[5] = {64, (cuuint32_t)p.page_size, 1, 1, 1};
+    const cuuint32_t box[5] = {64, (cuuint32_t)rows, 1, 1, 1};
     return make_tmap_nd(m, base, p.dtype == MQ_BF16, 5, dims, strides, box);
+}
+bool pool_maps(CUtensorMap* k, CUtensorMap* v, const mq_paged_pool& p, int rows) {
+    return pool_map(k, p, p.k, p.k_page, p.k_layer, p.k_head, rows) && pool_map(v, p, p.v, p.v_page, p.v_layer, p.v_head, rows);
 }
 
 template <typename T, int D>
-int run_prefix(const RowArgs& a, const mq_paged_pool& pool, int layer, cudaStream_t st) {
+int run_prefix(const RowArgs& a, const mq_paged_pool& pool, cudaStream_t st) {
     CUtensorMap tk, tv;
-    if (!pool_map(&tk, pool, pool.k, pool.k_page, pool.k_layer, pool.k_head) ||
-        !pool_map(&tv, pool, pool.v, pool.v_page, pool.v_layer, pool.v_head))
-        return MQ_ERR_CUDA;
+    if (!pool_maps(&tk, &tv, pool, pool.page_size)) return MQ_ERR_CUDA;
     auto kernel = prefix_kernel<T, D>;
     const size_t smem = PfxSmem<D>::bytes(a.NG);
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = launch(kernel, dim3(sm_count()), dim3(PFX_THREADS), smem, st, tk, tv, a, layer);
+    if (e == cudaSuccess) e = launch(kernel, dim3(sm_count()), dim3(PFX_THREADS), smem, st, tk, tv, a);
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "paged prefix attention");
 }
 
-int run_prefix_any(const RowArgs& a, const mq_paged_pool& p, int layer, cudaStream_t st) {
-    if (p.dtype == MQ_BF16)
-        return p.head_dim == 128 ? run_prefix<__nv_bfloat16, 128>(a, p, layer, st) : run_prefix<__nv_bfloat16, 64>(a, p, layer, st);
-    return p.head_dim == 128 ? run_prefix<__half, 128>(a, p, layer, st) : run_prefix<__half, 64>(a, p, layer, st);
-}
-
-template <typename T, int D, int MODE>
-int run_rows(const RowArgs& a, cudaStream_t st) {
-    auto kernel = rows_kernel<T, D, MODE>;
-    const size_t smem = (size_t)ROW_WARPS * RowWarp<T, D>::RING + (MODE == 0 ? sched_bytes(a.B, a.NG) : 0);
+template <typename T, int D, int MODE, int NT>
+int run_rows(const RowArgs& a, const mq_paged_pool& pool, cudaStream_t st) {
+    CUtensorMap tk, tv;
+    if (!pool_maps(&tk, &tv, pool, GRP)) return MQ_ERR_CUDA;
+    auto kernel = rows_kernel<T, D, MODE, NT>;
+    const size_t smem = (size_t)ROW_WARPS * RowWarp<T, D, NT>::RING + 1024 + (MODE == 0 ? sched_bytes(a.B, a.NG) : 0);
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return note_cuda(e, "paged attention attribute");
     const int grid = row_grid(D);
-    e = launch(kernel, dim3(grid), dim3(ROW_THREADS), smem, st, a);
+    e = launch(kernel, dim3(grid), dim3(ROW_THREADS), smem, st, tk, tv, a);
     const long long rows = (long long)a.total_q * a.hq;
     if (e == cudaSuccess) {
         // eight warps to a row until that is several waves of CTAs
-        if (rows <= 32 * sm_count())
+        if (rows <= 8 * sm_count())
             e = launch(join_kernel<T, D, MODE, 8>, dim3((unsigned)rows), dim3(256), 0, st, a, (uint32_t)grid * ROW_WARPS);
         else
             e = launch(join_kernel<T, D, MODE, 1>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, a,
@@ -386,11 +398,13 @@ int run_rows(const RowArgs& a, cudaStream_t st) {
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "paged attention");
 }
 
-template <int MODE>
-int run_rows_any(const RowArgs& a, int dtype, int D, cudaStream_t st) {
-    if (dtype == MQ_BF16)
-        return D == 128 ? run_rows<__nv_bfloat16, 128, MODE>(a, st) : run_rows<__nv_bfloat16, 64, MODE>(a, st);
-    return D == 128 ? run_rows<__half, 128, MODE>(a, st) : run_rows<__half, 64, MODE>(a, st);
+template <typename T, int D>
+int run_attend(const RowArgs& a, const mq_paged_pool& pool, cudaStream_t st) {
+    if (a.tc) {
+        const int rc = run_prefix<T, D>(a, pool, st);
+        if (rc) return rc;
+    }
+    return a.rt == 8 ? run_rows<T, D, 0, 1>(a, pool, st) : run_rows<T, D, 0, 2>(a, pool, st);
 }
 
 bool q_ok(const void* q, long long tok, long long head) {
@@ -467,11 +481,12 @@ int mq_paged_attend(const mq_paged_attend_params* p, cudaStream_t st) {
     const Shape s = shape_of(p);
     row_workspace(s, &a.ws, p->workspace);
     a.tc = s.tc;
-    if (a.tc) {
-        const int rc = run_prefix_any(a, *p->pool, p->layer, st);
-        if (rc) return rc;
-    }
-    return run_rows_any<0>(a, p->pool->dtype, s.D, st);
+    a.layer = p->layer;
+    // 8 rows to an item when a sequence (and a group whose prefix is not on the tensor-core kernel) has no
+    // more on average: half the tensor work a group; otherwise 16, so that the keys are read half as often
+    const long long rows = (long long)a.total_q * a.grp;
+    set_rt(a, rows <= 8ll * a.B && (!a.NG || a.tc || rows <= 8ll * a.NG));
+    return dispatch(p->pool->dtype, s.D, [&](auto T, auto D) { return run_attend<decltype(T), decltype(D)::value>(a, *p->pool, st); });
 }
 
 size_t mq_paged_sparse_workspace_bytes(const mq_paged_sparse_params* p) {
@@ -487,7 +502,7 @@ int mq_paged_sparse(const mq_paged_sparse_params* p, cudaStream_t st) {
         return MQ_ERR_INVALID_ARGUMENT;
     if (!p->n) return MQ_OK;
     // the work line is counted in 31 bits
-    if ((long long)p->n * p->pool->num_kv_heads * ceil_div(p->num_q_heads / p->pool->num_kv_heads, RT) *
+    if ((long long)p->n * p->pool->num_kv_heads * ceil_div(p->num_q_heads / p->pool->num_kv_heads, 8) *
             ((long long)p->top_k * (p->pool->page_size / GRP) + ITEM_UNITS) > 0x7fffffffll)
         return MQ_ERR_INVALID_ARGUMENT;
     if (!q_ok(p->q, p->q_token, p->q_head) || !p->out || (reinterpret_cast<uintptr_t>(p->out) & 15) || !p->selected ||
@@ -518,9 +533,7 @@ int mq_paged_sparse(const mq_paged_sparse_params* p, cudaStream_t st) {
     s.grp = p->num_q_heads / o.num_kv_heads;
     s.top_k = p->top_k;
     s.status = p->status;
-    const int rc = o.dtype == MQ_BF16
-                       ? (o.head_dim == 128 ? run_select<__nv_bfloat16, 128>(s, st) : run_select<__nv_bfloat16, 64>(s, st))
-                       : (o.head_dim == 128 ? run_select<__half, 128>(s, st) : run_select<__half, 64>(s, st));
+    const int rc = dispatch(o.dtype, o.head_dim, [&](auto T, auto D) { return run_select<decltype(T), decltype(D)::value>(s, st); });
     if (rc) return rc;
     RowArgs a = {};
     a.pool = view_of(o, p->layer);
@@ -543,7 +556,13 @@ int mq_paged_sparse(const mq_paged_sparse_params* p, cudaStream_t st) {
     a.scale_log2 = p->scale * 1.4426950408889634f;
     a.status = p->status;
     row_workspace(shape_of(p), &a.ws, p->workspace);
-    return run_rows_any<1>(a, o.dtype, o.head_dim, st);
+    a.layer = p->layer;
+    set_rt(a, a.grp <= 8);
+    return dispatch(o.dtype, o.head_dim, [&](auto T, auto D) {
+        using E = decltype(T);
+        constexpr int d = decltype(D)::value;
+        return a.rt == 8 ? run_rows<E, d, 1, 1>(a, o, st) : run_rows<E, d, 1, 2>(a, o, st);
+    });
 }
 
 }  // extern "C"

@@ -6,23 +6,28 @@
 // (m, l, acc) of one row join as acc = sum acc_i 2^(m_i - M), l likewise.
 //
 // Bound: the keys and values are read once from HBM, 4 D bytes per position
-// and kv head against 4 D flops per row, so with up to 16 rows the tensor work
-// (mma.sync m16n8k16, rows on the M side) hides behind the loads.  What has to
-// be had is bytes in flight on every SM, whatever the lengths: the unit of
-// work is one warp's 16-position group, all groups of all (sequence, kv head)
-// items laid end to end and cut into equal runs, one per warp.  A warp keeps
-// its own ring of cp.async stages and never waits for another one.  A run that
-// ends inside an item leaves a part in the workspace; the join kernel adds the
-// parts in the order of the positions, so results do not depend on timing.
+// and kv head against 4 D flops per row.  With few rows the tensor work has to
+// be small enough to hide: mma.sync m16n8k16 with the 16 positions (or 16 head
+// dims) on the M side and the rows as N, so that up to 8 rows cost 8 + 16
+// MMAs a group for head_dim 128 (rows on the M side cost twice that and 788
+// instructions a group, and bound the kernel: 340 us against 2.1 GB from L2).
+// What else has to be had is bytes in flight on every SM, whatever the
+// lengths: the unit of work is one warp's 16-position group, all groups of all
+// (sequence, kv head) items laid end to end and cut into equal runs, one per
+// warp.  A warp keeps its own ring of TMA stages and never waits for another
+// one.  A run that ends inside an item leaves a part in the workspace; the join
+// kernel adds the parts in the order of the positions, so results do not
+// depend on timing.
 #pragma once
 
+#include "mq_tc.cuh"
 #include "paged_common.cuh"
 
 namespace mq {
 namespace paged {
 
 constexpr int GRP = 16;            // positions per group (a page holds a whole number of them)
-constexpr int RT = 16;             // query rows per item
+constexpr int MAX_RT = 16;         // query rows per item: 8 or 16
 constexpr int ROW_THREADS = 128;
 constexpr int ROW_WARPS = ROW_THREADS / 32;
 constexpr int STAGES = 3;
@@ -54,7 +59,7 @@ struct WsView {
     uint32_t* head;     // [0] the call's arguments were in order, [1] units per warp, [2] units per prefix CTA
     TokInfo* tok;       // [total_q]
     float* own_rowp;    // [total_q * Hq][D + 4]
-    float* slots;       // [2 * warps][RT][D + 4]
+    float* slots;       // [2 * warps][rt][D + 4]
     float* pfx_rowp;    // [total_q * Hq][D + 4], twice that with the tensor-core prefix (its two streams)
     float* pfx_slots;   // [2 * CTAs][PROWS][D + 4], tensor-core prefix only
 };
@@ -75,20 +80,27 @@ struct RowArgs {
     const int* positions;   // sparse
     const int* selected;    // sparse
     int B, NG, total_q, hq, hkv, grp, top_k;   // grp = hq / hkv
+    int rt, rt_shift;       // query rows per item of rows_kernel
+    int layer;
     int tc;                 // prefixes run on the tensor-core kernel
     float scale_log2;
     int* status;
     WsView ws;
 };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int x, int row, int h, int l, int p,
+                                            uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(h), "r"(l), "r"(p), "r"(bar)
+        : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ uint32_t movm_t(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
 }
+constexpr long long WAIT_CYCLES = 4000000000ll;   // bound of every wait, about two seconds
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(a) : "memory");
@@ -133,14 +145,14 @@ __device__ __forceinline__ int own_groups(const RowArgs& a, const Sched& s, int 
     const int lo = s.grp[b] >= 0 ? s.eff[s.grp[b]] << a.pool.shift : 0;
     return s.len[b] > lo ? ((s.len[b] - lo - 1) >> 4) + 1 : 0;
 }
-__device__ __forceinline__ int row_tiles(int rows) { return (int)(((uint32_t)rows + RT - 1) >> 4); }
+__device__ __forceinline__ int row_tiles(const RowArgs& a, int rows) { return (int)(((uint32_t)rows + a.rt - 1) >> a.rt_shift); }
 
 // Groups (or tiles) of a prefix item and its rows, in the units of the kernel that runs it.
 __device__ __forceinline__ int pfx_groups(const RowArgs& a, int eff) {
     return a.tc ? (int)((((uint32_t)eff << a.pool.shift) + PK - 1) >> 7) : eff << (a.pool.shift - 4);
 }
 __device__ __forceinline__ int pfx_tiles(const RowArgs& a, int rows) {
-    return a.tc ? (int)(((uint32_t)rows + PROWS - 1) >> 8) : row_tiles(rows);
+    return a.tc ? (int)(((uint32_t)rows + PROWS - 1) >> 8) : row_tiles(a, rows);
 }
 
 // Returns false (for every thread) when the starts are out of order or the
@@ -231,7 +243,7 @@ __device__ inline bool build_sched(const RowArgs& a, const Sched& s, unsigned lo
                 ng = pfx_groups(a, s.eff[e]);
             } else {
                 const int b = e - a.NG;
-                tiles = row_tiles((q_start(a, b + 1) - q_start(a, b)) * a.grp);
+                tiles = row_tiles(a, (q_start(a, b + 1) - q_start(a, b)) * a.grp);
                 ng = own_groups(a, s, b);
             }
             if (ng) cost = (unsigned long long)(unsigned)tiles * (unsigned)(ng + ITEM_UNITS);
@@ -266,132 +278,131 @@ __device__ __forceinline__ uint32_t quota_of(uint32_t work, uint32_t workers) {
     return max(q, (uint32_t)ITEM_UNITS + 2u);
 }
 
-// One warp's 16-position group step and item bookkeeping.
-template <typename T, int D>
+// One warp's 16-position group step, for NT tiles of 8 query rows.
+// Lane (g, t) = (lane / 4, lane % 4) works for rows 8 n + 2 t and + 1.
+template <typename T, int D, int NT>
 struct RowWarp {
-    static constexpr int TILE = GRP * D * 2;         // bytes of one K or V group
+    static constexpr int BOX = GRP * 128;             // bytes of 16 rows x 64 channels, 128-byte swizzle
+    static constexpr int TILE = (D / 64) * BOX;       // a K or V group
     static constexpr int STAGE = 2 * TILE;
     static constexpr int RING = STAGES * STAGE;
-    static constexpr int CH = D / 8;                  // 16-byte chunks per row
-    static constexpr int KS = D / 16;                 // k-steps of Q K^T
+    static constexpr int KS = D / 16;                 // k-steps of K Q^T, and 16-dim tiles of O^T
     static constexpr int LD = D + 4;                  // floats of a stored part row: m, l, pad, pad, acc
 
-    uint32_t ring;     // this warp's ring, shared-memory address
+    uint32_t ring;     // this warp's ring, shared-memory address (1024-byte aligned)
     int lane;
-    uint32_t qa[KS][4];
-    float o[D / 8][4];
-    float m[2], l[2];
+    uint32_t qb[NT][KS][2];
+    float o[NT][KS][4];
+    float m[NT][2], l[NT][2];
 
+    // Q^T as the B operand: row 8 n + g, dims 16 k + 2 t (+ 8)
     __device__ __forceinline__ void load_q(const RowArgs& a, int tok0, int h, int grp, int r0, int rows) {
         const int g = lane >> 2, t = lane & 3;
-        const uint16_t* p[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = r0 + g + 8 * i;
-            p[i] = g + 8 * i < rows ? a.q + (long long)(tok0 + r / grp) * a.q_tok + (h * grp + r % grp) * a.q_head : nullptr;
-        }
+        for (int n = 0; n < NT; ++n) {
+            const int r = r0 + 8 * n + g, tok = r / grp;
+            const uint16_t* p = 8 * n + g < rows ? a.q + (long long)(tok0 + tok) * a.q_tok + (h * grp + r - tok * grp) * a.q_head : nullptr;
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
+            for (int k = 0; k < KS; ++k)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint16_t* x = p[i & 1];
-                qa[k][i] = x ? __ldg(reinterpret_cast<const uint32_t*>(x + 16 * k + 8 * (i >> 1) + 2 * t)) : 0u;
-            }
-    }
-
-    // Rows 0 .. vis - 1 of the group at row `row` of page `pid`, zeros past them.
-    __device__ __forceinline__ void issue(const RowArgs& a, int stage, int pid, int row, int h, int vis) {
-        const uint16_t* kp = a.pool.k + pid * a.pool.k_page + h * a.pool.k_head + row * D;
-        const uint16_t* vp = a.pool.v + pid * a.pool.v_page + h * a.pool.v_head + row * D;
-        const uint32_t s = ring + stage * STAGE;
-#pragma unroll
-        for (int j = 0; j < GRP * CH / 32; ++j) {
-            const int c = lane + 32 * j, r = c / CH, x = c % CH;
-            const uint32_t off = r * (D * 2) + ((x ^ (r & 7)) << 4);
-            const bool ok = r < vis;
-            cp16(s + off, ok ? kp + r * D + x * 8 : a.pool.k, ok);
-            cp16(s + TILE + off, ok ? vp + r * D + x * 8 : a.pool.v, ok);
+                for (int i = 0; i < 2; ++i)
+                    qb[n][k][i] = p ? __ldg(reinterpret_cast<const uint32_t*>(p + 16 * k + 8 * i + 2 * t)) : 0u;
         }
     }
 
     __device__ __forceinline__ void reset() {
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        m[0] = m[1] = -INFINITY;
-        l[0] = l[1] = 0.f;
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int i = 0; i < KS; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+        }
     }
 
-    // lim0 / lim1: positions of the group (0 .. 16) that rows g and g + 8 see.
+    // 16-byte piece c of row r of a tile
+    static __device__ __forceinline__ uint32_t piece(int r, int c) {
+        return (c >> 3) * BOX + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+    }
+
+    // Rows vis .. 15 of V are zeroed: stale rows must not meet the zero weights as NaN.
+    __device__ __forceinline__ void clear_rows(int stage, int vis) {
+        const uint32_t vs = ring + stage * STAGE + TILE;
+        for (int i = vis * (D / 8) + lane; i < GRP * (D / 8); i += 32)
+            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(vs + piece(i / (D / 8), i % (D / 8))), "r"(0) : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the next copy into this stage
+        __syncwarp();
+    }
+
+    // lim: positions of the group (below 1: none, 16 and up: all) that rows 8 n + 2 t + i see.
     // `mixed`: the rows of the tile do not all see the same positions.
-    __device__ __forceinline__ void step(int stage, int lim0, int lim1, bool mixed, float scale) {
+    __device__ __forceinline__ void step(int stage, const int (&lim)[NT][2], bool mixed, float scale) {
         const uint32_t ks = ring + stage * STAGE, vs = ks + TILE;
-        const int t = lane & 3;
-        const int mat = lane >> 3, r8 = lane & 7;
-        float s[2][4], s2[2][4];   // two chains per tile: even and odd k-steps
+        const int g = lane >> 2, mat = lane >> 3, r8 = lane & 7;
+        // S^T = K Q^T: positions g, g + 8; rows 2 t, 2 t + 1.  Even and odd k-steps in chains of their own.
+        float s[NT][4], s2[NT][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[0][i] = s[1][i] = s2[0][i] = s2[1][i] = 0.f;
-        const int krow = (mat >> 1) * 8 + r8;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[n][i] = s2[n][i] = 0.f;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-            uint32_t b0, b1, b2, b3;
-            ldsm4(ks + krow * (D * 2) + (((2 * k + (mat & 1)) ^ r8) << 4), b0, b1, b2, b3);
-            Elem<T>::mma(k & 1 ? s2[0] : s[0], qa[k], b0, b1);
-            Elem<T>::mma(k & 1 ? s2[1] : s[1], qa[k], b2, b3);
-        }
-        float mx[2] = {-INFINITY, -INFINITY};
+            uint32_t f[4];
+            ldsm4(ks + piece((mat & 1) * 8 + r8, 2 * k + (mat >> 1)), f[0], f[1], f[2], f[3]);
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < NT; ++n) Elem<T>::mma(k & 1 ? s2[n] : s[n], f, qb[n][k][0], qb[n][k][1]);
+        }
+        uint32_t ph[NT][2], pr[NT][2];   // P^T as the B operand, value and remainder: positions 2 t (+ 8), row g
+        bool moved = false;
+        float corr[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int p = 8 * n + 2 * t + (i & 1);
-                const float x = (s[n][i] + s2[n][i]) * scale;
-                s[n][i] = p < (i < 2 ? lim0 : lim1) ? x : -INFINITY;
-                mx[i >> 1] = fmaxf(mx[i >> 1], s[n][i]);
+                const int p = g + 8 * (i >> 1);
+                s[n][i] = p < lim[n][i & 1] ? (s[n][i] + s2[n][i]) * scale : -INFINITY;
             }
-        float corr[2];
+            float u[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-            const float mn = fmaxf(m[i], mx[i]);
-            corr[i] = mn == m[i] ? 1.f : exp2f(m[i] - mn);   // m = -inf: nothing summed yet
-            m[i] = mn;
-        }
-        const float u0 = m[0] == -INFINITY ? 0.f : m[0], u1 = m[1] == -INFINITY ? 0.f : m[1];
+            for (int i = 0; i < 2; ++i) {
+                float mx = fmaxf(s[n][i], s[n][2 + i]);
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            s[n][0] = exp2f(s[n][0] - u0);
-            s[n][1] = exp2f(s[n][1] - u0);
-            s[n][2] = exp2f(s[n][2] - u1);
-            s[n][3] = exp2f(s[n][3] - u1);
-        }
-        l[0] = l[0] * corr[0] + ((s[0][0] + s[0][1]) + (s[1][0] + s[1][1]));
-        l[1] = l[1] * corr[1] + ((s[0][2] + s[0][3]) + (s[1][2] + s[1][3]));
-        if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+                for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                const float mn = fmaxf(m[n][i], mx);
+                corr[n][i] = mn == m[n][i] ? 1.f : exp2f(m[n][i] - mn);   // m = -inf: nothing summed yet
+                moved |= mn != m[n][i];
+                m[n][i] = mn;
+                u[i] = mn == -INFINITY ? 0.f : mn;
+            }
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                o[i][0] *= corr[0];
-                o[i][1] *= corr[0];
-                o[i][2] *= corr[1];
-                o[i][3] *= corr[1];
+            for (int i = 0; i < 4; ++i) s[n][i] = exp2f(s[n][i] - u[i & 1]);
+            l[n][0] = l[n][0] * corr[n][0] + (s[n][0] + s[n][2]);
+            l[n][1] = l[n][1] * corr[n][1] + (s[n][1] + s[n][3]);
+            // two pieces of the 16-bit type: one would cost as much accuracy as rounding the output does
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t v = Elem<T>::pack(s[n][2 * i], s[n][2 * i + 1]);
+                const float2 b = Elem<T>::up2(v);
+                ph[n][i] = movm_t(v);
+                pr[n][i] = movm_t(Elem<T>::pack(s[n][2 * i] - b.x, s[n][2 * i + 1] - b.y));
             }
         }
-        // P as the A operand, in two pieces of the 16-bit type (value and
-        // remainder): one piece would cost as much accuracy as rounding the output does
-        uint32_t pa[4], pr[4];
+        if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float x = s[i >> 1][2 * (i & 1)], y = s[i >> 1][2 * (i & 1) + 1];
-            pa[i] = Elem<T>::pack(x, y);
-            const float2 b = Elem<T>::up2(pa[i]);
-            pr[i] = Elem<T>::pack(x - b.x, y - b.y);
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    o[n][i][0] *= corr[n][0];
+                    o[n][i][1] *= corr[n][1];
+                    o[n][i][2] *= corr[n][0];
+                    o[n][i][3] *= corr[n][1];
+                }
         }
-        const int vrow = (mat & 1) * 8 + r8;
         bool slow = false;
         if (mixed) {   // a masked weight of zero must not meet an infinity or NaN
             bool odd = false;
 #pragma unroll
-            for (int j = 0; j < GRP * CH / 32; ++j) {
+            for (int j = 0; j < TILE / 512; ++j) {
                 uint32_t w[4];
                 asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
                              : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(vs + (lane + 32 * j) * 16) : "memory");
@@ -402,45 +413,48 @@ struct RowWarp {
             }
             slow = __any_sync(0xffffffffu, odd);
         }
+        const int vrow = (mat >> 1) * 8 + r8;
         if (!slow) {
+            // O^T += V^T P^T: dims g, g + 8 of a 16-dim tile; rows 2 t, 2 t + 1
 #pragma unroll
-            for (int n = 0; n < D / 16; ++n) {
-                uint32_t b0, b1, b2, b3;
-                ldsm4t(vs + vrow * (D * 2) + (((2 * n + (mat >> 1)) ^ r8) << 4), b0, b1, b2, b3);
-                Elem<T>::mma(o[2 * n], pa, b0, b1);
-                Elem<T>::mma(o[2 * n + 1], pa, b2, b3);
-                Elem<T>::mma(o[2 * n], pr, b0, b1);
-                Elem<T>::mma(o[2 * n + 1], pr, b2, b3);
+            for (int i = 0; i < KS; ++i) {
+                uint32_t f[4];
+                ldsm4t(vs + piece(vrow, 2 * i + (mat & 1)), f[0], f[1], f[2], f[3]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    Elem<T>::mma(o[n][i], f, ph[n][0], ph[n][1]);
+                    Elem<T>::mma(o[n][i], f, pr[n][0], pr[n][1]);
+                }
             }
         } else {
             // one position at a time, added only to the rows that see it
+            const int t = lane & 3;
 #pragma unroll 1
             for (int p = 0; p < GRP; ++p) {
-                uint32_t qa1[4], qr1[4], keep[2];
+                uint32_t keep[2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i)   // this lane's columns 8 i + 2 t and + 1
+                for (int i = 0; i < 2; ++i)   // this lane's positions 8 i + 2 t and + 1
                     keep[i] = p == 8 * i + 2 * t ? 0xffffu : p == 8 * i + 2 * t + 1 ? 0xffff0000u : 0u;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    qa1[i] = pa[i] & keep[i >> 1];
-                    qr1[i] = pr[i] & keep[i >> 1];
-                }
+                for (int i = 0; i < KS; ++i) {
+                    uint32_t f[4];
+                    ldsm4t(vs + piece(vrow, 2 * i + (mat & 1)), f[0], f[1], f[2], f[3]);
+                    f[0] &= keep[0];
+                    f[1] &= keep[0];
+                    f[2] &= keep[1];
+                    f[3] &= keep[1];
 #pragma unroll
-                for (int n = 0; n < D / 16; ++n) {
-                    uint32_t b[4];
-                    ldsm4t(vs + vrow * (D * 2) + (((2 * n + (mat >> 1)) ^ r8) << 4), b[0], b[1], b[2], b[3]);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
+                    for (int n = 0; n < NT; ++n) {
                         float x[4] = {0.f, 0.f, 0.f, 0.f};
-                        Elem<T>::mma(x, qa1, b[2 * e] & keep[0], b[2 * e + 1] & keep[1]);
-                        Elem<T>::mma(x, qr1, b[2 * e] & keep[0], b[2 * e + 1] & keep[1]);
-                        if (p < lim0) {
-                            o[2 * n + e][0] += x[0];
-                            o[2 * n + e][1] += x[1];
+                        Elem<T>::mma(x, f, ph[n][0] & keep[0], ph[n][1] & keep[1]);
+                        Elem<T>::mma(x, f, pr[n][0] & keep[0], pr[n][1] & keep[1]);
+                        if (p < lim[n][0]) {
+                            o[n][i][0] += x[0];
+                            o[n][i][2] += x[2];
                         }
-                        if (p < lim1) {
-                            o[2 * n + e][2] += x[2];
-                            o[2 * n + e][3] += x[3];
+                        if (p < lim[n][1]) {
+                            o[n][i][1] += x[1];
+                            o[n][i][3] += x[3];
                         }
                     }
                 }
@@ -450,25 +464,30 @@ struct RowWarp {
 
     __device__ __forceinline__ void finish() {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], x);
+    }
+    // Row 8 n + 2 t + i, unnormalised, to a part row; eight lanes write 32 contiguous bytes.
+    __device__ __forceinline__ void put_part(float* dst, int n, int i) {
+        const int g = lane >> 2;
+        if (g == 0) *reinterpret_cast<float2*>(dst) = make_float2(m[n][i], l[n][i]);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            dst[4 + 16 * k + g] = o[n][k][i];
+            dst[4 + 16 * k + 8 + g] = o[n][k][2 + i];
         }
     }
-    // Row g + 8 i of the tile, unnormalised, to a part row.
-    __device__ __forceinline__ void put_part(float* dst, int i) {
-        const int t = lane & 3;
-        if (t == 0) *reinterpret_cast<float2*>(dst) = make_float2(m[i], l[i]);
+    __device__ __forceinline__ void put_out(uint16_t* dst, int n, int i) {
+        const int g = lane >> 2;
+        const float inv = l[n][i] != 0.f ? 1.f / l[n][i] : 0.f;   // a row that sees nothing is zero (NaN stays NaN)
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-            *reinterpret_cast<float2*>(dst + 4 + 8 * n + 2 * t) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
-    }
-    __device__ __forceinline__ void put_out(uint16_t* dst, int i) {
-        const int t = lane & 3;
-        const float inv = l[i] != 0.f ? 1.f / l[i] : 0.f;   // a row that sees nothing is zero (NaN stays NaN)
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-            *reinterpret_cast<uint32_t*>(dst + 8 * n + 2 * t) = Elem<T>::pack(o[n][2 * i] * inv, o[n][2 * i + 1] * inv);
+        for (int k = 0; k < KS; ++k) {
+            dst[16 * k + g] = Elem<T>::down(o[n][k][i] * inv);
+            dst[16 * k + 8 + g] = Elem<T>::down(o[n][k][2 + i] * inv);
+        }
     }
 };
 
@@ -490,20 +509,31 @@ enum { BOX_START = 1, BOX_WHOLE = 2, BOX_PREFIX = 4, BOX_OTHER = 8 };
 // rows, touched into L1) are under way while the item before is computed; with
 // items of a few groups each the latency would otherwise be paid per item
 // (measured: 5500 cycles for an item of one group).
-template <typename T, int D, int MODE>
-__global__ void __launch_bounds__(ROW_THREADS) rows_kernel(const RowArgs a) {
-    using W = RowWarp<T, D>;
-    extern __shared__ __align__(128) uint8_t smem[];
+template <typename T, int D, int MODE, int NT>
+__global__ void __launch_bounds__(ROW_THREADS)
+rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const RowArgs a) {
+    using W = RowWarp<T, D, NT>;
+    constexpr int RT = 8 * NT;
+    extern __shared__ uint8_t rows_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(rows_raw) + 1023) & ~uintptr_t(1023));
     __shared__ unsigned long long scratch[ROW_WARPS];
+    __shared__ uint64_t full[ROW_WARPS][STAGES];
     __shared__ ItemBox boxes[ROW_WARPS][BOXES];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t wid = blockIdx.x * ROW_WARPS + warp, warps = gridDim.x * ROW_WARPS;
     const int grp = a.grp, shift = a.pool.shift, page = a.pool.page;
+    if (lane == 0) {
+        for (int i = 0; i < STAGES; ++i) mbar_init(&full[warp][i], 1);
+        fence_mbar_init();
+        prefetch_tmap(&tmK);
+        prefetch_tmap(&tmV);
+    }
+    __syncwarp();
     pdl_wait();
     pdl_trigger();
     Sched s;
     uint32_t work, origin = 0;   // where this kernel's work starts on the line
-    const int sp_nrt = row_tiles(grp), sp_ng = a.top_k << (shift - 4);
+    const int sp_nrt = row_tiles(a, grp), sp_ng = a.top_k << (shift - 4);
     if (MODE == 0) {
         s = sched_of(smem + ROW_WARPS * W::RING, a.B, a.NG);
         const bool ok = build_sched<false, ROW_THREADS>(a, s, scratch);
@@ -550,7 +580,7 @@ __global__ void __launch_bounds__(ROW_THREADS) rows_kernel(const RowArgs a) {
             const int ql = q_start(a, b1) - tok0;
             rows_all = ql * grp;
             if (!prefix) first = s.len[b0] - ql + 1;
-            nrt = prefix ? pfx_tiles(a, rows_all) : row_tiles(rows_all);
+            nrt = prefix ? pfx_tiles(a, rows_all) : row_tiles(a, rows_all);
             items = ng ? nrt * a.hkv : 0;
             if (items) {
                 // a prefix is read through a member's row of the table; a member without query tokens may have none
@@ -676,54 +706,97 @@ __global__ void __launch_bounds__(ROW_THREADS) rows_kernel(const RowArgs a) {
             if (k && (k & 31) == 0) look();
             const int pid = __shfl_sync(0xffffffffu, ids, k & 31), p0 = __shfl_sync(0xffffffffu, at, k & 31);
             if (pid >= 0) {
-                w.issue(a, stage_l, pid, p0 & (page - 1), h, lim_hi - p0);
+                if (lane == 0) {
+                    const uint32_t bar = smem_u32(&full[warp][stage_l]), dst = w.ring + stage_l * W::STAGE;
+                    mbar_arrive_expect_tx(&full[warp][stage_l], W::STAGE);
+#pragma unroll
+                    for (int i = 0; i < D / 64; ++i) {
+                        tma_load_5d(dst + i * W::BOX, &tmK, 64 * i, p0 & (page - 1), h, a.layer, pid, bar);
+                        tma_load_5d(dst + W::TILE + i * W::BOX, &tmV, 64 * i, p0 & (page - 1), h, a.layer, pid, bar);
+                    }
+                }
                 p = p0;
             }
             ++k;
         }
         if (lane == stage_l) ring_at = p;
         stage_l = stage_l == STAGES - 1 ? 0 : stage_l + 1;
-        cp_commit();
     };
 #pragma unroll 1
     for (int i = 0; i < STAGES - 1; ++i) fetch();
 
     // ---- the computing side ----
-    const int g = lane >> 2;
+    const int t = lane & 3;
     int stage_c = 0;
-    for (int popped = 0; popped < pushed; ++popped) {
+    uint32_t phase = 0;      // bit i: parity of stage i's next copy
+    bool ok = true;
+    auto landed = [&](int stage) -> bool {
+        const long long t0 = clock64();
+        bool here;
+        while (!(here = mbar_try_wait(&full[warp][stage], phase >> stage & 1)) && clock64() - t0 < WAIT_CYCLES) {
+        }
+        phase ^= 1u << stage;
+        return __all_sync(0xffffffffu, here);
+    };
+    for (int popped = 0; ok && popped < pushed; ++popped) {
         __syncwarp();
         const ItemBox b = boxes[warp][popped % BOXES];
         w.load_q(a, b.tok0, b.h, grp, b.r0, b.rows);
         w.reset();
-        auto lim = [&](int r) { return b.fixed >= 0 ? b.fixed : b.first + (b.r0 + min(r, b.rows - 1)) / grp; };
-        const int lim_lo = lim(0), lim_top = lim(b.rows - 1), lim_a = lim(g), lim_b = lim(g + 8);
+        auto limit = [&](int r) { return b.fixed >= 0 ? b.fixed : b.first + (b.r0 + min(r, b.rows - 1)) / grp; };
+        const int lim_lo = limit(0), lim_top = limit(b.rows - 1);
+        int lim[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) lim[n][i] = limit(8 * n + 2 * t + i);
 #pragma unroll 1
         for (int i = 0; i < b.n; ++i) {
             fetch();
-            cp_wait<STAGES - 1>();
-            __syncwarp();
             const int p0 = __shfl_sync(0xffffffffu, ring_at, stage_c);
-            if (p0 >= 0) w.step(stage_c, lim_a - p0, lim_b - p0, lim_lo < min(p0 + GRP, lim_top), a.scale_log2);
+            if (p0 >= 0) {
+                if (!landed(stage_c)) {
+                    ok = false;
+                    break;
+                }
+                if (lim_top - p0 < GRP) w.clear_rows(stage_c, lim_top - p0);
+                int rel[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    rel[n][0] = lim[n][0] - p0;
+                    rel[n][1] = lim[n][1] - p0;
+                }
+                w.step(stage_c, rel, lim_lo < min(p0 + GRP, lim_top), a.scale_log2);
+            }
             stage_c = stage_c == STAGES - 1 ? 0 : stage_c + 1;
-            __syncwarp();
+            __syncwarp();   // every lane is past its reads of the stage
         }
+        if (!ok) break;
         w.finish();
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = g + 8 * i;
-            if (r >= b.rows) continue;
-            const int t = (b.r0 + r) / grp;
-            const long long row = (long long)(b.tok0 + t) * a.hq + b.h * grp + b.r0 + r - t * grp;
-            if (!(b.flags & BOX_WHOLE))
-                w.put_part(a.ws.slots + ((2ll * wid + (b.flags & BOX_START ? 1 : 0)) * RT + r) * W::LD, i);
-            else if (b.flags & (BOX_PREFIX | BOX_OTHER))
-                w.put_part((b.flags & BOX_PREFIX ? a.ws.pfx_rowp : a.ws.own_rowp) + row * W::LD, i);
-            else
-                w.put_out(a.out + row * D, i);
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = 8 * n + 2 * t + i;
+                if (r >= b.rows) continue;
+                const int tk = (b.r0 + r) / grp;
+                const long long row = (long long)(b.tok0 + tk) * a.hq + b.h * grp + b.r0 + r - tk * grp;
+                if (!(b.flags & BOX_WHOLE))
+                    w.put_part(a.ws.slots + ((2ll * wid + (b.flags & BOX_START ? 1 : 0)) * RT + r) * W::LD, n, i);
+                else if (b.flags & (BOX_PREFIX | BOX_OTHER))
+                    w.put_part((b.flags & BOX_PREFIX ? a.ws.pfx_rowp : a.ws.own_rowp) + row * W::LD, n, i);
+                else
+                    w.put_out(a.out + row * D, n, i);
+            }
+    }
+    if (!ok) {
+        if (lane == 0) note_status(a.status, MQ_ERR_PIPE_TIMEOUT);
+        // copies in flight land before the CTA may end: the stages after the one that did not
+        for (int i = 1; i < STAGES; ++i) {
+            stage_c = stage_c == STAGES - 1 ? 0 : stage_c + 1;
+            if (__shfl_sync(0xffffffffu, ring_at, stage_c) >= 0) landed(stage_c);
         }
     }
-    cp_wait<0>();
     if (MODE == 0) {
         // the join's view of the line, a share of the sequences per warp
         if (blockIdx.x == 0 && threadIdx.x == 0) {
@@ -735,7 +808,7 @@ __global__ void __launch_bounds__(ROW_THREADS) rows_kernel(const RowArgs a) {
             TokInfo ti = {};
             ti.own_base = s.off[a.NG + b] * a.hkv - origin;
             ti.own_ng = own_groups(a, s, b);
-            ti.own_nrt = row_tiles((q1 - q0) * grp);
+            ti.own_nrt = row_tiles(a, (q1 - q0) * grp);
             int p0 = 0;
             if (gr >= 0 && s.eff[gr] > 0) {
                 p0 = q_start(a, s.gs[gr]);
@@ -766,7 +839,7 @@ __global__ void __launch_bounds__(256) join_kernel(const RowArgs a, uint32_t row
     if (rowi >= (long long)a.total_q * a.hq) return;
     const int sub = SPLIT > 1 ? warp : 0;
     const int tok = (int)((uint32_t)rowi / (uint32_t)a.hq), head = (int)(rowi - (long long)tok * a.hq);   // rows fit 31 bits
-    const int grp = a.grp, h = head / grp;
+    const int grp = a.grp, h = head / grp, RT = a.rt;
     uint16_t* out = a.out + rowi * D;
     // the row's parts: np0 of the prefix (sub of them per run), then np1 of its own
     const float *src0 = nullptr, *src1 = nullptr;
@@ -782,7 +855,7 @@ __global__ void __launch_bounds__(256) join_kernel(const RowArgs a, uint32_t row
     const int sp_ng = MODE == 1 ? a.top_k << (a.pool.shift - 4) : 0;
     const uint32_t quota =
         MODE == 0 ? a.ws.head[1]
-                  : quota_of((uint32_t)a.total_q * a.hkv * row_tiles(grp) * (sp_ng + ITEM_UNITS), row_warps);
+                  : quota_of((uint32_t)a.total_q * a.hkv * row_tiles(a, grp) * (sp_ng + ITEM_UNITS), row_warps);
     {
         int ng, r;
         uint32_t start;   // the item's first group on the line
@@ -790,7 +863,7 @@ __global__ void __launch_bounds__(256) join_kernel(const RowArgs a, uint32_t row
             const TokInfo ti = a.ws.tok[tok];
             ng = ti.own_ng;
             r = ti.own_r0 + head % grp;
-            start = ti.own_base + ((uint32_t)h * ti.own_nrt + r / RT) * (ng + ITEM_UNITS) + ITEM_UNITS;
+            start = ti.own_base + ((uint32_t)h * ti.own_nrt + (r >> a.rt_shift)) * (ng + ITEM_UNITS) + ITEM_UNITS;
             if (ti.pfx_ng) {
                 const int R = a.tc ? PROWS : RT, pr = ti.pfx_r0 + head % grp, in = pr & (R - 1);
                 const uint32_t ps = ti.pfx_base + ((uint32_t)h * ti.pfx_nrt + (uint32_t)(pr - in) / R) * (ti.pfx_ng + ITEM_UNITS) + ITEM_UNITS;
@@ -809,10 +882,10 @@ __global__ void __launch_bounds__(256) join_kernel(const RowArgs a, uint32_t row
                 }
             }
         } else {
-            const int nrt = row_tiles(grp);
+            const int nrt = row_tiles(a, grp);
             r = head % grp;
             ng = sp_ng;
-            start = (((uint32_t)h * a.total_q + tok) * nrt + r / RT) * (ng + ITEM_UNITS) + ITEM_UNITS;
+            start = (((uint32_t)h * a.total_q + tok) * nrt + (r >> a.rt_shift)) * (ng + ITEM_UNITS) + ITEM_UNITS;
         }
         if (ng) {
             const uint32_t w0 = start / quota;
@@ -821,7 +894,7 @@ __global__ void __launch_bounds__(256) join_kernel(const RowArgs a, uint32_t row
                 if (!np0) return;   // written by the only warp that had it
                 src1 = a.ws.own_rowp + rowi * LD;
             } else {
-                src1 = a.ws.slots + (2ll * w0 * RT + r % RT) * LD;
+                src1 = a.ws.slots + (2ll * w0 * RT + (r & (RT - 1))) * LD;
                 step1 = 2ll * RT * LD;
                 first1 = (long long)RT * LD;
             }

@@ -38,7 +38,6 @@ namespace paged {
 constexpr int PATOM = 128 * 128;         // bytes of 128 rows x 64 elements, 128-byte swizzle
 constexpr int PFX_THREADS = 352;
 constexpr int PFX_MAX_GROUPS = 256;
-constexpr long long PFX_TIMEOUT = 4000000000ll;   // cycles, about two seconds
 
 template <int D>
 struct PfxSmem {
@@ -70,14 +69,6 @@ template <typename T>
 __device__ constexpr uint32_t pfx_idesc(int N, bool b_mn) {
     const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;   // bf16 or f16, the same for A and B
     return (1u << 4) | (f << 7) | (f << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-}
-
-__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, int x, int row, int h, int l, int p,
-                                            uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
-        ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(row), "r"(h), "r"(l), "r"(p), "r"(smem_u32(bar))
-        : "memory");
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -129,7 +120,7 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float* v) {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(PFX_THREADS, 1)
-prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const RowArgs a, int layer) {
+prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const RowArgs a) {
     using L = PfxSmem<D>;
     constexpr int TILE = L::TILE, LD = D + 4;
     extern __shared__ uint8_t pfx_raw[];
@@ -220,7 +211,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
     auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
         const long long t0 = clock64();
         while (!mbar_try_wait(bar, parity)) {
-            if (*abort_flag || clock64() - t0 > PFX_TIMEOUT) return false;
+            if (*abort_flag || clock64() - t0 > WAIT_CYCLES) return false;
         }
         return true;
     };
@@ -267,7 +258,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
                 if (lane < chunks) {
 #pragma unroll
                     for (int i = 0; i < D / 64; ++i)
-                        tma_load_5d(ring + st * TILE + i * PATOM + lane * page * 128, map, 64 * i, 0, e.h, layer, pid, &full[st]);
+                        tma_load_5d(smem_u32(ring + st * TILE + i * PATOM + lane * page * 128), map, 64 * i, 0, e.h, a.layer, pid, smem_u32(&full[st]));
                 }
             }
         }
@@ -275,7 +266,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
         // copies in flight land before the CTA may end, whatever became of their readers
         for (int k = max(0, c - 2); k < c; ++k) {
             const long long t0 = clock64();
-            while (!mbar_try_wait(&full[k & 1], (k >> 1) & 1) && clock64() - t0 < PFX_TIMEOUT) {
+            while (!mbar_try_wait(&full[k & 1], (k >> 1) & 1) && clock64() - t0 < WAIT_CYCLES) {
             }
         }
     } else if (warp == 1) {
@@ -347,7 +338,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
         if (elect_one()) tc_commit(drain);   // MMAs in flight end before TMEM goes
         __syncwarp();
         const long long t0 = clock64();
-        while (!mbar_try_wait(drain, 0) && clock64() - t0 < PFX_TIMEOUT) {
+        while (!mbar_try_wait(drain, 0) && clock64() - t0 < WAIT_CYCLES) {
         }
     } else {
         // ---- softmax of stream q: a thread per row ----

@@ -30,7 +30,7 @@ constexpr int GRP = 16;            // positions per group (a page holds a whole 
 constexpr int MAX_RT = 16;         // query rows per item: 8 or 16
 constexpr int ROW_THREADS = 128;
 constexpr int ROW_WARPS = ROW_THREADS / 32;
-constexpr int STAGES = 3;
+constexpr int STAGES = 2;
 constexpr int MAX_SEQS = 2048;
 constexpr int PK = 128;            // keys per tile and query rows per item of the tensor-core prefix kernel
 constexpr int PROWS = 256;
@@ -510,7 +510,7 @@ enum { BOX_START = 1, BOX_WHOLE = 2, BOX_PREFIX = 4, BOX_OTHER = 8 };
 // items of a few groups each the latency would otherwise be paid per item
 // (measured: 5500 cycles for an item of one group).
 template <typename T, int D, int MODE, int NT>
-__global__ void __launch_bounds__(ROW_THREADS)
+__global__ void __launch_bounds__(ROW_THREADS, NT == 2 && D == 128 ? 2 : 3)
 rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const RowArgs a) {
     using W = RowWarp<T, D, NT>;
     constexpr int RT = 8 * NT;
@@ -827,17 +827,17 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
 }
 
 // ---- the join ----------------------------------------------------------------------------
-// SPLIT warps share a row (few rows, many parts) or each warp has its own.
+// SPLIT warps share a row (the fewer rows, the more parts each), 8 / SPLIT rows to a CTA.
 template <typename T, int D, int MODE, int SPLIT>
-__global__ void __launch_bounds__(256) join_kernel(const RowArgs a, uint32_t row_warps) {
+__global__ void __launch_bounds__(256, 3) join_kernel(const RowArgs a, uint32_t row_warps) {
     constexpr int LD = D + 4, V = D / 32;
     __shared__ float sm_m[8], sm_l[8], sm_o[8][D];
     pdl_wait();
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long rowi = SPLIT > 1 ? blockIdx.x : (long long)blockIdx.x * 8 + warp;
+    const long long rowi = (long long)blockIdx.x * (8 / SPLIT) + warp / SPLIT;
     if (rowi >= (long long)a.total_q * a.hq) return;
-    const int sub = SPLIT > 1 ? warp : 0;
+    const int sub = warp % SPLIT;
     const int tok = (int)((uint32_t)rowi / (uint32_t)a.hq), head = (int)(rowi - (long long)tok * a.hq);   // rows fit 31 bits
     const int grp = a.grp, h = head / grp, RT = a.rt;
     uint16_t* out = a.out + rowi * D;
@@ -848,7 +848,7 @@ __global__ void __launch_bounds__(256) join_kernel(const RowArgs a, uint32_t row
     long long first0 = 0, first1 = 0, sub_step0 = 0;   // the first part of a split item is one slot further on
     if (MODE == 0) {
         if (!a.ws.head[0]) {   // refused: zeros
-            for (int d = threadIdx.x & (SPLIT > 1 ? 255 : 31); d < D; d += SPLIT > 1 ? 256 : 32) out[d] = 0;
+            for (int d = sub * 32 + lane; d < D; d += SPLIT * 32) out[d] = 0;
             return;
         }
     }
@@ -963,21 +963,21 @@ __global__ void __launch_bounds__(256) join_kernel(const RowArgs a, uint32_t row
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) sm_o[warp][lane * V + i] = acc[i];
-        __syncthreads();
-        if (warp) return;
+        named_bar_sync(1 + warp / SPLIT, SPLIT * 32);   // the row's warps (all or none of them got here)
+        if (sub) return;
         float MM = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < SPLIT; ++k) MM = fmaxf(MM, sm_m[k]);
+        for (int k = 0; k < SPLIT; ++k) MM = fmaxf(MM, sm_m[warp + k]);
         const float UU = MM == -INFINITY ? 0.f : MM;
         L = 0.f;
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] = 0.f;
 #pragma unroll
         for (int k = 0; k < SPLIT; ++k) {
-            const float e = exp2f(sm_m[k] - UU);
-            L += sm_l[k] * e;
+            const float e = exp2f(sm_m[warp + k] - UU);
+            L += sm_l[warp + k] * e;
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] += sm_o[k][lane * V + i] * e;
+            for (int i = 0; i < V; ++i) acc[i] += sm_o[warp + k][lane * V + i] * e;
         }
     }
     const float inv = L != 0.f ? 1.f / L : 0.f;

@@ -3,9 +3,7 @@
 //
 // Memory-bound: each token's q, k and v are read once and written once,
 // (Hq + 2 Hkv) D elements each way; the cos/sin row of a token is shared by its
-// heads.  One CTA per token: a thread keeps one 16-channel unit's cos/sin in
-// registers and walks over heads with it, so the tables cost one read per
-// thread and not one per head.
+// heads and comes from L1.
 #include "paged_common.cuh"
 
 namespace mq {
@@ -30,7 +28,7 @@ struct RopeArgs {
     long long kp_page, kp_head, vp_page, vp_head;
     const int* table;
     long long table_row;
-    int slots_n, cols, pages, page;
+    int slots_n, cols, pages, page, shift;   // page = 1 << shift
     int* status;
 };
 
@@ -42,30 +40,30 @@ __device__ __forceinline__ void turn(float& x0, float& x1, float c, float s) {
     x1 = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
 }
 
-// Where token `t` goes.  page -1: nowhere (no cache, or a wrong place).
+// Where a token goes.  page -1: nowhere (no cache, or a wrong place).
 struct Place {
     int pos, page, row;
     bool ok;   // the position is inside the tables
 };
-__device__ __forceinline__ Place place_of(const RopeArgs& a, int t, bool report) {
+__device__ __forceinline__ Place place_of(const RopeArgs& a, int pos, int slot, bool report) {
     Place p;
-    p.pos = a.positions[t];
+    p.pos = pos;
     p.page = -1;
     p.row = 0;
-    p.ok = p.pos >= 0 && p.pos < a.max_pos;
+    p.ok = pos >= 0 && pos < a.max_pos;
     if (!p.ok) {
         if (report) note_status(a.status, MQ_ERR_BAD_POSITION);
     } else if (a.kp) {
-        const int slot = a.slots[t], c = p.pos / a.page;
+        const int c = pos >> a.shift;
         if (slot < 0 || slot >= a.slots_n) {
             if (report) note_status(a.status, MQ_ERR_BAD_SLOT);
         } else if (c >= a.cols) {
             if (report) note_status(a.status, MQ_ERR_BAD_POSITION);
         } else {
-            const int g = a.table[slot * a.table_row + c];
+            const int g = __ldg(a.table + slot * a.table_row + c);
             if (g >= 0 && g < a.pages) {
                 p.page = g;
-                p.row = p.pos - c * a.page;
+                p.row = pos & (a.page - 1);
             } else if (report) {
                 note_status(a.status, MQ_ERR_BAD_PAGE);
             }
@@ -74,88 +72,99 @@ __device__ __forceinline__ Place place_of(const RopeArgs& a, int t, bool report)
     return p;
 }
 
-// Head h of the token: q heads first, then k, then v.  Sets the pointers;
-// false when nothing is to be written.
-__device__ __forceinline__ bool head_of(const RopeArgs& a, int t, int h, int D, const Place& p, const uint16_t*& src,
-                                        uint16_t*& dst, bool& rotate) {
-    if (h < a.hq) {
-        src = a.q + t * a.q_tok + h * a.q_head;
-        dst = a.q_out + t * a.o_tok + h * a.o_head;
-        rotate = true;
-        return true;
-    }
-    if (p.page < 0) return false;
-    const int g = h - a.hq;
-    if (g < a.hkv) {
-        src = a.k + t * a.k_tok + g * a.k_head;
-        dst = a.kp + p.page * a.kp_page + g * a.kp_head + p.row * D;
-        rotate = true;
-    } else {
-        src = a.v + t * a.v_tok + (g - a.hkv) * a.v_head;
-        dst = a.vp + p.page * a.vp_page + (g - a.hkv) * a.vp_head + p.row * D;
-        rotate = false;
-    }
-    return true;
+// Head h of a token: q heads first, then k, then v.
+__device__ __forceinline__ const uint16_t* src_of(const RopeArgs& a, int t, int h) {
+    if (h < a.hq) return a.q + t * a.q_tok + h * a.q_head;
+    h -= a.hq;
+    return h < a.hkv ? a.k + t * a.k_tok + h * a.k_head : a.v + t * a.v_tok + (h - a.hkv) * a.v_head;
+}
+// Where it is written, or null.
+__device__ __forceinline__ uint16_t* dst_of(const RopeArgs& a, int t, int h, int D, const Place& p) {
+    if (h < a.hq) return a.q_out + t * a.o_tok + h * a.o_head;
+    if (p.page < 0) return nullptr;
+    h -= a.hq;
+    return h < a.hkv ? a.kp + p.page * a.kp_page + h * a.kp_head + p.row * D
+                     : a.vp + p.page * a.vp_page + (h - a.hkv) * a.vp_head + p.row * D;
 }
 
 // Vector path: rotary_dim a multiple of 16, every address a multiple of 16
-// bytes.  A unit is 16 channels of a head: for the half layout the 8 pairs
-// (8u + i, 8u + i + R / 2), otherwise 16 channels in a row.
+// bytes.  A unit is two pieces of 8 channels of a head, chosen so that a piece's
+// neighbour lane has the neighbouring piece: for the half layout the 8 pairs
+// (8u + i, 8u + i + R / 2), or two pieces past R; interleaved, pieces u and
+// D / 16 + u, each four pairs or past R.  One CTA per token;
+// a thread keeps its unit's cos/sin in registers and takes two heads at a time.
+// The reads of the heads do not wait for the token's place (position, then
+// table: two dependent reads), which would otherwise be paid one after another.
 template <typename T, int D, bool INTER>
 __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs a) {
     constexpr int UNITS = D / 16, LANES = ROPE_THREADS / UNITS;
     pdl_wait();
     pdl_trigger();
     const int t = blockIdx.x, u = threadIdx.x % UNITS;
-    const Place p = place_of(a, t, threadIdx.x == 0);
-    const bool rot_unit = u < a.rot / 16;
+    const int pos = __ldg(a.positions + t), slot = a.kp ? __ldg(a.slots + t) : 0;
     const int heads = a.hq + (a.kp ? 2 * a.hkv : 0);
-    // first channels of the unit's two 8-channel pieces
-    const int c0 = !INTER && rot_unit ? 8 * u : 16 * u;
-    const int c1 = !INTER && rot_unit ? 8 * u + a.rot / 2 : 16 * u + 8;
-    const int r0 = c0, r1 = rot_unit && !INTER ? c1 : c0 + 8;
-    // pieces of a v head (never rotated) are taken in the same places: a permutation of the units
+    // first channels of the two pieces, and whether they are turned
+    const int pairs = a.rot / 16;   // half layout: units that turn
+    const int r0 = INTER || u < pairs ? 8 * u : a.rot + 8 * (u - pairs);
+    const int r1 = INTER ? D / 2 + 8 * u : u < pairs ? r0 + a.rot / 2 : r0 + (D - a.rot) / 2;
+    const bool turn0 = r0 < a.rot, turn1 = INTER ? r1 < a.rot : turn0;
+    Place p;
     float cs[8], sn[8];
-    if (rot_unit && p.ok) {
+    for (int h = threadIdx.x / UNITS; h < heads; h += 2 * LANES) {
+        const bool two = h + LANES < heads;
+        uint4 x[2], y[2];
 #pragma unroll
-        for (int i = 0; i < 8; i += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(a.cos_t + p.pos * a.cos_row + 8 * u + i);
-            const float4 y = *reinterpret_cast<const float4*>(a.sin_t + p.pos * a.sin_row + 8 * u + i);
-            cs[i] = x.x; cs[i + 1] = x.y; cs[i + 2] = x.z; cs[i + 3] = x.w;
-            sn[i] = y.x; sn[i + 1] = y.y; sn[i + 2] = y.z; sn[i + 3] = y.w;
+        for (int i = 0; i < 2; ++i) {
+            if (i && !two) break;
+            const uint16_t* src = src_of(a, t, h + i * LANES);
+            x[i] = __ldg(reinterpret_cast<const uint4*>(src + r0));
+            y[i] = __ldg(reinterpret_cast<const uint4*>(src + r1));
         }
-        if (a.inverse) {
+        if (h < LANES) {   // the first time round
+            p = place_of(a, pos, slot, threadIdx.x == 0);
+            if (turn0 && p.ok) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sn[i] = -sn[i];
-        }
-    }
-#pragma unroll 2
-    for (int h = threadIdx.x / UNITS; h < heads; h += LANES) {
-        const uint16_t* src;
-        uint16_t* dst;
-        bool rotate;
-        if (!head_of(a, t, h, D, p, src, dst, rotate)) continue;
-        uint4 x = *reinterpret_cast<const uint4*>(src + r0), y = *reinterpret_cast<const uint4*>(src + r1);
-        if (!p.ok) x = y = make_uint4(0, 0, 0, 0);   // a position outside the tables has no rotation
-        if (rotate && rot_unit && p.ok) {
-            uint32_t* xv = reinterpret_cast<uint32_t*>(&x);
-            uint32_t* yv = reinterpret_cast<uint32_t*>(&y);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float2 e = Elem<T>::up2(xv[i]), f = Elem<T>::up2(yv[i]);
-                if (INTER) {   // pairs are neighbours: x holds pairs 8u .. 8u + 3, y the next four
-                    turn(e.x, e.y, cs[i], sn[i]);
-                    turn(f.x, f.y, cs[4 + i], sn[4 + i]);
-                } else {
-                    turn(e.x, f.x, cs[2 * i], sn[2 * i]);
-                    turn(e.y, f.y, cs[2 * i + 1], sn[2 * i + 1]);
+                for (int i = 0; i < 8; i += 4) {
+                    if (i && !turn1) break;   // (half layout: both or none)
+                    const int pair = INTER ? (i ? r1 : r0) / 2 : r0 + i;
+                    const float4 c = __ldg(reinterpret_cast<const float4*>(a.cos_t + pos * a.cos_row + pair));
+                    const float4 s = __ldg(reinterpret_cast<const float4*>(a.sin_t + pos * a.sin_row + pair));
+                    cs[i] = c.x; cs[i + 1] = c.y; cs[i + 2] = c.z; cs[i + 3] = c.w;
+                    sn[i] = s.x; sn[i + 1] = s.y; sn[i + 2] = s.z; sn[i + 3] = s.w;
                 }
-                xv[i] = Elem<T>::pack(e.x, e.y);
-                yv[i] = Elem<T>::pack(f.x, f.y);
+                if (a.inverse) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sn[i] = -sn[i];
+                }
             }
         }
-        *reinterpret_cast<uint4*>(dst + r0) = x;
-        *reinterpret_cast<uint4*>(dst + r1) = y;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (i && !two) break;
+            uint16_t* dst = dst_of(a, t, h + i * LANES, D, p);
+            if (!dst) continue;
+            if (!p.ok) {
+                x[i] = y[i] = make_uint4(0, 0, 0, 0);   // a position outside the tables has no rotation
+            } else if (turn0 && h + i * LANES < a.hq + a.hkv) {
+                uint32_t* xv = reinterpret_cast<uint32_t*>(&x[i]);
+                uint32_t* yv = reinterpret_cast<uint32_t*>(&y[i]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float2 e = Elem<T>::up2(xv[k]), f = Elem<T>::up2(yv[k]);
+                    if (INTER) {   // pairs are neighbours
+                        turn(e.x, e.y, cs[k], sn[k]);
+                        if (turn1) turn(f.x, f.y, cs[4 + k], sn[4 + k]);
+                    } else {
+                        turn(e.x, f.x, cs[2 * k], sn[2 * k]);
+                        turn(e.y, f.y, cs[2 * k + 1], sn[2 * k + 1]);
+                    }
+                    xv[k] = Elem<T>::pack(e.x, e.y);
+                    if (!INTER || turn1) yv[k] = Elem<T>::pack(f.x, f.y);
+                }
+            }
+            *reinterpret_cast<uint4*>(dst + r0) = x[i];
+            *reinterpret_cast<uint4*>(dst + r1) = y[i];
+        }
     }
 }
 
@@ -165,19 +174,18 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_any_kernel(const RopeArgs a
     pdl_wait();
     pdl_trigger();
     const int t = blockIdx.x, half = a.rot / 2;
-    const Place p = place_of(a, t, threadIdx.x == 0);
+    const Place p = place_of(a, __ldg(a.positions + t), a.kp ? __ldg(a.slots + t) : 0, threadIdx.x == 0);
     const int heads = a.hq + (a.kp ? 2 * a.hkv : 0);
     for (int e = threadIdx.x; e < heads * (D / 2); e += ROPE_THREADS) {
         const int h = e / (D / 2), i = e - h * (D / 2);
-        const uint16_t* src;
-        uint16_t* dst;
-        bool rotate;
-        if (!head_of(a, t, h, D, p, src, dst, rotate)) continue;
+        const uint16_t* src = src_of(a, t, h);
+        uint16_t* dst = dst_of(a, t, h, D, p);
+        if (!dst) continue;
         const bool in = i < half;
         const int c0 = in && !inter ? i : 2 * i, c1 = in && !inter ? i + half : 2 * i + 1;
         uint16_t x = src[c0], y = src[c1];
         if (!p.ok) x = y = 0;
-        if (rotate && in && p.ok) {
+        if (h < a.hq + a.hkv && in && p.ok) {
             float f = Elem<T>::up(x), g = Elem<T>::up(y);
             const float c = a.cos_t[p.pos * a.cos_row + i], s = a.sin_t[p.pos * a.sin_row + i];
             turn(f, g, c, a.inverse ? -s : s);
@@ -190,86 +198,96 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_any_kernel(const RopeArgs a
 }
 
 // ---- the index of full pages ------------------------------------------------------------
-// CTA (chunk of 128 tokens, kv head): for each token of the chunk that is the
-// last row of its page, the bounds of the page's keys over its rows (read from
-// L2, where the kernel before left them).  Bounds are exact (no arithmetic on
-// the keys), so the record does not depend on the order of the rows.
-constexpr int INDEX_THREADS = 256, INDEX_TOKENS = 128;
+// CTA (chunk of 512 tokens, kv head): the tokens of the chunk that are the last
+// row of their page are dealt to its warps; a warp takes the bounds of one
+// page's keys (read from L2, where the kernel before left them, eight rows of
+// 16 bytes a lane in flight).  Bounds are exact (no arithmetic on the keys), so
+// the record does not depend on the order of the rows.
+constexpr int INDEX_THREADS = 256, INDEX_TOKENS = 512;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(INDEX_THREADS) index_kernel(const RopeArgs a, int n, signed char* __restrict__ index,
                                                               long long i_page, long long i_head) {
-    constexpr int PIECES = D / 8, ROWS = INDEX_THREADS / PIECES;   // 8 channels a thread, ROWS rows at once
+    constexpr int PIECES = D / 8, ROWS = 32 / PIECES;   // 8 channels a lane, ROWS rows side by side
     __shared__ int list[INDEX_TOKENS];
     __shared__ int count;
-    __shared__ float red[2][ROWS][D];
-    __shared__ float amax[D / 32];
     pdl_wait();
     pdl_trigger();
     if (threadIdx.x == 0) count = 0;
     __syncthreads();
-    const int t = blockIdx.x * INDEX_TOKENS + threadIdx.x, h = blockIdx.y;
-    if (threadIdx.x < INDEX_TOKENS && t < n && a.positions[t] % a.page == a.page - 1) {
-        const Place p = place_of(a, t, false);
-        if (p.page >= 0) list[atomicAdd(&count, 1)] = p.page;
+    const int h = blockIdx.y;
+#pragma unroll
+    for (int i = 0; i < INDEX_TOKENS; i += INDEX_THREADS) {
+        const int t = blockIdx.x * INDEX_TOKENS + i + threadIdx.x;
+        if (t >= n) break;
+        const int pos = __ldg(a.positions + t), slot = __ldg(a.slots + t);
+        if ((pos & (a.page - 1)) == a.page - 1) {
+            const Place p = place_of(a, pos, slot, false);
+            if (p.page >= 0) list[atomicAdd(&count, 1)] = p.page;
+        }
     }
     __syncthreads();
-    const int piece = threadIdx.x % PIECES, r0 = threadIdx.x / PIECES;
-    for (int e = 0; e < count; ++e) {
-        const uint16_t* k = a.kp + list[e] * a.kp_page + h * a.kp_head;
+    const int lane = threadIdx.x & 31, piece = lane % PIECES;
+    for (int e = threadIdx.x >> 5; e < count; e += INDEX_THREADS / 32) {
+        const uint16_t* k = a.kp + list[e] * a.kp_page + h * a.kp_head + (lane / PIECES) * D + piece * 8;
         float hi[8], lo[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             hi[i] = -INFINITY;
             lo[i] = INFINITY;
         }
-        for (int r = r0; r < a.page; r += ROWS) {
-            const uint4 x = *reinterpret_cast<const uint4*>(k + r * D + piece * 8);
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        for (int r = 0; r < a.page; r += 8 * ROWS) {   // page >= 16: with two rows side by side one batch, or more
+            uint4 x[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 f = Elem<T>::up2(w[i]);
-                hi[2 * i] = fmaxf(hi[2 * i], f.x);
-                lo[2 * i] = fminf(lo[2 * i], f.x);
-                hi[2 * i + 1] = fmaxf(hi[2 * i + 1], f.y);
-                lo[2 * i + 1] = fminf(lo[2 * i + 1], f.y);
+            for (int i = 0; i < 8; ++i) {
+                const int row = r + i * ROWS;   // past the page (16 rows, four side by side): the first rows again
+                x[i] = *reinterpret_cast<const uint4*>(k + (row < a.page ? row : 0) * D);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float2 f = Elem<T>::up2(w[c]);
+                    hi[2 * c] = fmaxf(hi[2 * c], f.x);
+                    lo[2 * c] = fminf(lo[2 * c], f.x);
+                    hi[2 * c + 1] = fmaxf(hi[2 * c + 1], f.y);
+                    lo[2 * c + 1] = fminf(lo[2 * c + 1], f.y);
+                }
             }
         }
+        float m = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            red[0][r0][piece * 8 + i] = hi[i];
-            red[1][r0][piece * 8 + i] = lo[i];
-        }
-        __syncthreads();
-        float H = -INFINITY, L = INFINITY;
-        const int d = threadIdx.x;
-        if (d < D) {
-            for (int r = 0; r < ROWS; ++r) {
-                H = fmaxf(H, red[0][r][d]);
-                L = fminf(L, red[1][r][d]);
+#pragma unroll
+            for (int o = PIECES; o < 32; o <<= 1) {
+                hi[i] = fmaxf(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], o));
+                lo[i] = fminf(lo[i], __shfl_xor_sync(0xffffffffu, lo[i], o));
             }
             // infinite keys count as the type's largest, and a channel of nothing but NaN as zero
-            if (!(H >= L)) H = L = 0.f;
-            H = fminf(fmaxf(H, -Elem<T>::MAX), Elem<T>::MAX);
-            L = fminf(fmaxf(L, -Elem<T>::MAX), Elem<T>::MAX);
-            float m = fmaxf(fabsf(H), fabsf(L));
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            if ((d & 31) == 0) amax[d >> 5] = m;
+            if (!(hi[i] >= lo[i])) hi[i] = lo[i] = 0.f;
+            hi[i] = fminf(fmaxf(hi[i], -Elem<T>::MAX), Elem<T>::MAX);
+            lo[i] = fminf(fmaxf(lo[i], -Elem<T>::MAX), Elem<T>::MAX);
+            m = fmaxf(m, fmaxf(fabsf(hi[i]), fabsf(lo[i])));
         }
-        __syncthreads();
-        if (d < D) {
-            float m = amax[0];
 #pragma unroll
-            for (int i = 1; i < D / 32; ++i) m = fmaxf(m, amax[i]);
-            const int ex = m > 0.f ? min(max(ilogbf(m) - 6, -60), 40) : 0;
-            const float unit = __int_as_float((127 - ex) << 23);   // 2^-ex
-            signed char* rec = index + list[e] * i_page + h * i_head;
-            rec[d] = (signed char)fminf(fmaxf(rintf(H * unit), -127.f), 127.f);
-            rec[D + d] = (signed char)fminf(fmaxf(rintf(L * unit), -127.f), 127.f);
-            if (d < 16) rec[2 * D + d] = d == 0 ? (signed char)ex : 0;
+        for (int o = 1; o < PIECES; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const int ex = m > 0.f ? min(max(ilogbf(m) - 6, -60), 40) : 0;
+        const float unit = __int_as_float((127 - ex) << 23);   // 2^-ex
+        signed char* rec = index + list[e] * i_page + h * i_head;
+        if (lane < PIECES) {
+            auto whole = [&](const float* v) {
+                uint32_t w[2] = {0, 0};
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    w[i >> 2] |= (uint32_t)((int)fminf(fmaxf(rintf(v[i] * unit), -127.f), 127.f) & 255) << (8 * (i & 3));
+                return make_uint2(w[0], w[1]);
+            };
+            *reinterpret_cast<uint2*>(rec + piece * 8) = whole(hi);
+            *reinterpret_cast<uint2*>(rec + D + piece * 8) = whole(lo);
+        } else if (lane == PIECES) {
+            *reinterpret_cast<uint4*>(rec + 2 * D) = make_uint4((uint32_t)(ex & 255), 0, 0, 0);
         }
-        __syncthreads();
     }
 }
 
@@ -288,9 +306,9 @@ int run_rope(const mq_rope_params* p, const RopeArgs& a, bool vec, cudaStream_t 
     if (e != cudaSuccess) return note_cuda(e, "rope");
     if (!p->pool || !p->pool->index) return MQ_OK;
     signed char* ix = p->pool->index + p->layer * p->pool->i_layer;
-    const dim3 grid(ceil_div(p->n, INDEX_TOKENS), p->pool->num_kv_heads);
-    e = D == 128 ? launch(index_kernel<T, 128>, grid, dim3(INDEX_THREADS), 0, st, a, p->n, ix, p->pool->i_page, p->pool->i_head)
-                 : launch(index_kernel<T, 64>, grid, dim3(INDEX_THREADS), 0, st, a, p->n, ix, p->pool->i_page, p->pool->i_head);
+    const dim3 chunks(ceil_div(p->n, INDEX_TOKENS), p->pool->num_kv_heads);
+    e = D == 128 ? launch(index_kernel<T, 128>, chunks, dim3(INDEX_THREADS), 0, st, a, p->n, ix, p->pool->i_page, p->pool->i_head)
+                 : launch(index_kernel<T, 64>, chunks, dim3(INDEX_THREADS), 0, st, a, p->n, ix, p->pool->i_page, p->pool->i_head);
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "page index");
 }
 
@@ -348,6 +366,7 @@ extern "C" int mq_rope(const mq_rope_params* p, cudaStream_t st) {
         a.cols = p->table_cols;
         a.pages = o.num_pages;
         a.page = o.page_size;
+        a.shift = __builtin_ctz((unsigned)o.page_size);
         odd |= (p->k_token | p->k_head | p->v_token | p->v_head) % 8;
         vec = vec && al16(p->k) && al16(p->v);
     }

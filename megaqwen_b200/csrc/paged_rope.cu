@@ -96,7 +96,7 @@ __device__ __forceinline__ uint16_t* dst_of(const RopeArgs& a, int t, int h, int
 // The reads of the heads do not wait for the token's place (position, then
 // table: two dependent reads), which would otherwise be paid one after another.
 template <typename T, int D, bool INTER>
-__global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs a) {
+__global__ void __launch_bounds__(ROPE_THREADS, 10) rope_kernel(const RopeArgs a) {
     constexpr int UNITS = D / 16, LANES = ROPE_THREADS / UNITS;
     pdl_wait();
     pdl_trigger();
@@ -117,8 +117,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs a) {
         for (int i = 0; i < 2; ++i) {
             if (i && !two) break;
             const uint16_t* src = src_of(a, t, h + i * LANES);
-            x[i] = __ldg(reinterpret_cast<const uint4*>(src + r0));
-            y[i] = __ldg(reinterpret_cast<const uint4*>(src + r1));
+            x[i] = __ldcs(reinterpret_cast<const uint4*>(src + r0));
+            y[i] = __ldcs(reinterpret_cast<const uint4*>(src + r1));
         }
         if (h < LANES) {   // the first time round
             p = place_of(a, pos, slot, threadIdx.x == 0);
@@ -162,8 +162,15 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs a) {
                     if (!INTER || turn1) yv[k] = Elem<T>::pack(f.x, f.y);
                 }
             }
-            *reinterpret_cast<uint4*>(dst + r0) = x[i];
-            *reinterpret_cast<uint4*>(dst + r1) = y[i];
+            // everything but K streams through L2 (read and written once here), so that the index
+            // kernel finds the keys there (65 MB of them among 530 MB)
+            if (h + i * LANES >= a.hq && h + i * LANES < a.hq + a.hkv) {
+                *reinterpret_cast<uint4*>(dst + r0) = x[i];
+                *reinterpret_cast<uint4*>(dst + r1) = y[i];
+            } else {
+                __stcs(reinterpret_cast<uint4*>(dst + r0), x[i]);
+                __stcs(reinterpret_cast<uint4*>(dst + r1), y[i]);
+            }
         }
     }
 }

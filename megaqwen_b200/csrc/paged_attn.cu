@@ -19,17 +19,20 @@ namespace paged {
 // pages into shared memory as order-preserving 32-bit keys, then a radix
 // selection of the (top_k - 1)-th largest over the bits in which the keys
 // differ (8 at a time, ending as soon as a whole bin is taken), then the list
-// in ascending order.  Reads 2 D + 1 bytes per page, four pages of a lane in
-// flight; the sums are whole numbers (dp4a), exact below 2^24, so the keys do
-// not depend on their order.
+// in ascending order.  Reads 2 D + 1 bytes per page, 16 bytes a lane, 32 pages
+// of a warp in flight.  The products run on mma.sync m16n8k32 (16 pages, 8 q
+// heads, 32 channels; dp4a took 110 instructions for what is 8 MMAs with two
+// heads): whole numbers, exact below 2^24, so the keys do not depend on their
+// order.
 //
-// NW 16, an item per CTA: few items, whose reads have to be spread.  NW 1,
-// eight items per CTA (consecutive tokens of one head, which read the same
-// records): many items, where the barriers of a CTA per item cost more than the
-// reads (500 tokens x 8 heads, 250 pages each: 121 us with a CTA per item).
+// NW 16, an item per cluster of up to 8 CTAs: few items, whose reads have to be
+// spread; each CTA scores a share of the pages and the first one collects the
+// keys.  NW 1, eight items per CTA (consecutive tokens of one head, which read
+// the same records): many items, where the barriers of a CTA per item cost more
+// than the reads.
 constexpr int MAX_SPARSE_COLS = 49152;
 constexpr int MAX_SPARSE_GROUP = 64;   // q heads per kv head
-constexpr int SEL_UNROLL = 4;
+constexpr int SEL_UNROLL = 2;      // 16-page steps in flight
 
 struct SelArgs {
     const signed char* index;   // at the layer
@@ -51,15 +54,40 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 }
 __device__ __forceinline__ float two_to(int e) { return __int_as_float((e + 127) << 23); }
 
+// heads are padded to a multiple of 8 with zeros
 template <int D>
 __host__ __device__ inline size_t sel_item_bytes(int cols, int grp) {
-    return (((size_t)cols * 4 + (size_t)grp * (2 * D + 4)) + 15) & ~(size_t)15;
+    return (((size_t)cols * 4 + (size_t)((grp + 7) & ~7) * (2 * D + 4)) + 15) & ~(size_t)15;
+}
+
+__device__ __forceinline__ void mma_s8(int* d, const int* a, int b0, int b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t ld_peer(uint32_t addr, uint32_t rank) {
+    uint32_t at, v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
 }
 
 template <typename T, int D, int NW>
 __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 32) select_kernel(const SelArgs a) {
-    constexpr int LP = D / 16;          // lanes per page: 16 channels each
-    constexpr int PPW = 32 / LP;        // pages per warp step
     constexpr int ITEMS = NW == 1 ? 8 : 1, NT = NW * 32;
     extern __shared__ __align__(16) uint8_t sel_smem[];
     __shared__ int hist[ITEMS][256];
@@ -68,17 +96,19 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 32) select_kernel(const S
     const int lane = threadIdx.x & 31, sub = NW == 1 ? threadIdx.x >> 5 : 0;
     const int warp = NW == 1 ? 0 : threadIdx.x >> 5, tid = NW == 1 ? lane : threadIdx.x;
     uint8_t* mem = sel_smem + sub * sel_item_bytes<D>(a.cols, a.grp);
-    signed char* qpos = reinterpret_cast<signed char*>(mem);               // [grp][D]
-    signed char* qneg = qpos + a.grp * D;
-    float* qunit = reinterpret_cast<float*>(qneg + a.grp * D);             // [grp]
-    uint32_t* keys = reinterpret_cast<uint32_t*>(qunit + a.grp);           // [cols]
+    const int heads = (a.grp + 7) & ~7;
+    signed char* qpos = reinterpret_cast<signed char*>(mem);               // [heads][D]
+    signed char* qneg = qpos + heads * D;
+    float* qunit = reinterpret_cast<float*>(qneg + heads * D);             // [heads], 0 past grp
+    uint32_t* keys = reinterpret_cast<uint32_t*>(qunit + heads);           // [cols]
     auto sync = [&]() {
         if (NW == 1) __syncwarp();
         else __syncthreads();
     };
     pdl_wait();
     pdl_trigger();
-    const uint32_t item = blockIdx.x * ITEMS + sub;
+    const uint32_t rank = NW == 1 ? 0 : cluster_rank(), ranks = NW == 1 ? 1 : cluster_size();
+    const uint32_t item = NW == 1 ? blockIdx.x * ITEMS + sub : blockIdx.x / ranks;
     if (item >= (uint32_t)a.n * a.hkv) return;
     const int h = (int)(item / (uint32_t)a.n), t = (int)(item - (uint32_t)h * a.n);
     int* sel = a.selected + ((long long)t * a.hkv + h) * a.top_k;
@@ -86,17 +116,19 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 32) select_kernel(const S
     const bool bad_slot = slot < 0 || slot >= a.num_slots;
     if (bad_slot || pos < 0 || pos >> a.shift >= a.cols) {
         if (tid == 0) note_status(a.status, bad_slot ? MQ_ERR_BAD_SLOT : MQ_ERR_BAD_POSITION);
-        for (int i = tid; i < a.top_k; i += NT) sel[i] = -1;
+        for (int i = tid; rank == 0 && i < a.top_k; i += NT) sel[i] = -1;
         return;
     }
     const int own = pos >> a.shift, want = a.top_k - 1;
     if (own <= want || want == 0) {   // every page, or only the token's own: nothing to choose
-        for (int i = tid; i < a.top_k; i += NT) sel[i] = want == 0 ? own : i <= own ? i : -1;
+        for (int i = tid; rank == 0 && i < a.top_k; i += NT) sel[i] = want == 0 ? own : i <= own ? i : -1;
         return;
     }
-    // the pages, looked up in one sweep; each place is overwritten by its page's key
+    // this CTA's share of the pages, looked up in one sweep; each place is overwritten by its page's key
+    const int share = ranks == 1 ? own : (ceil_div(own, (int)ranks) + 15) & ~15;
+    const int p0 = min(own, (int)rank * share), p1 = min(own, p0 + share);
     const int* row = a.table + slot * a.table_row;
-    for (int j = tid; j < own; j += NT) {
+    for (int j = p0 + tid; j < p1; j += NT) {
         int pid = __ldg(row + j);
         if (pid < 0 || pid >= a.pages) {
             note_status(a.status, MQ_ERR_BAD_PAGE);
@@ -105,13 +137,18 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 32) select_kernel(const S
         keys[j] = (uint32_t)pid;
     }
     // the group's queries in whole numbers, split by sign
-    for (int g = warp; g < a.grp; g += NW) {
-        const uint16_t* q = a.q + t * a.q_tok + (h * a.grp + g) * a.q_head;
+    for (int g = warp; g < heads; g += NW) {
         float x[D / 32], m = 0.f;
+        if (g < a.grp) {
+            const uint16_t* q = a.q + t * a.q_tok + (h * a.grp + g) * a.q_head;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            x[i] = Elem<T>::up(__ldg(q + lane + 32 * i));
-            m = fmaxf(m, fabsf(x[i]));
+            for (int i = 0; i < D / 32; ++i) {
+                x[i] = Elem<T>::up(__ldg(q + lane + 32 * i));
+                m = fmaxf(m, fabsf(x[i]));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) x[i] = 0.f;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -127,58 +164,85 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 32) select_kernel(const S
         if (lane == 0) qunit[g] = two_to(e);
     }
     sync();
-    const int part = lane % LP;
+    // 16 pages a step: lane (g, t) reads channels 16 t .. of each 64-channel block of pages g and g + 8, whose
+    // words are the A operand of two MMAs; the k index is permuted alike in both operands
+    const int g = lane >> 2, tq = lane & 3;
     const signed char* ix = a.index + h * a.i_head;
     uint32_t kmin = 0xffffffffu, kmax = 0;
 #pragma unroll 1
-    for (int j0 = warp * PPW + lane / LP; j0 - lane / LP < own; j0 += NW * PPW * SEL_UNROLL) {
-        int4 hi[SEL_UNROLL], lo[SEL_UNROLL];
-        int ex[SEL_UNROLL];
-        bool ok[SEL_UNROLL];
+    for (int j0 = p0 + warp * 16; j0 < p1; j0 += NW * 16 * SEL_UNROLL) {
+        int4 w[SEL_UNROLL][2][2 * D / 64];   // [step][page g, g + 8][HI blocks, LO blocks]
+        int ex[SEL_UNROLL][2];
+        bool ok[SEL_UNROLL][2];
 #pragma unroll
-        for (int u = 0; u < SEL_UNROLL; ++u) {
-            const int j = j0 + u * NW * PPW;
-            const int pid = j < own ? (int)keys[j] : -1;
-            ok[u] = pid >= 0;
-            const signed char* rec = ix + (ok[u] ? pid : 0) * a.i_page;
-            hi[u] = __ldg(reinterpret_cast<const int4*>(rec + part * 16));
-            lo[u] = __ldg(reinterpret_cast<const int4*>(rec + D + part * 16));
-            ex[u] = __ldg(rec + 2 * D);
-        }
-        float best[SEL_UNROLL];
+        for (int u = 0; u < SEL_UNROLL; ++u)
 #pragma unroll
-        for (int u = 0; u < SEL_UNROLL; ++u) best[u] = -INFINITY;
-        for (int g = 0; g < a.grp; ++g) {
-            const int4 p = *reinterpret_cast<const int4*>(qpos + g * D + part * 16);
-            const int4 n = *reinterpret_cast<const int4*>(qneg + g * D + part * 16);
-            const float unit = qunit[g];
+            for (int r = 0; r < 2; ++r) {
+                const int j = j0 + u * NW * 16 + g + 8 * r;
+                const int pid = j < p1 ? (int)keys[j] : -1;
+                ok[u][r] = pid >= 0;
+                const signed char* rec = ix + (pid >= 0 ? pid : 0) * a.i_page;
+#pragma unroll
+                for (int b = 0; b < 2 * D / 64; ++b) w[u][r][b] = __ldg(reinterpret_cast<const int4*>(rec + 64 * b + 16 * tq));
+                ex[u][r] = __ldg(rec + 2 * D);
+            }
+        float best[SEL_UNROLL][2];
+#pragma unroll
+        for (int u = 0; u < SEL_UNROLL; ++u) best[u][0] = best[u][1] = -INFINITY;
+        for (int h0 = 0; h0 < a.grp; h0 += 8) {
+            int4 q[2 * D / 64];
+#pragma unroll
+            for (int b = 0; b < 2 * D / 64; ++b)
+                q[b] = *reinterpret_cast<const int4*>((b < D / 64 ? qpos : qneg) + (h0 + g) * D + (b % (D / 64)) * 64 + 16 * tq);
+            const float u0 = qunit[h0 + 2 * tq], u1 = qunit[h0 + 2 * tq + 1];
+            const bool in0 = h0 + 2 * tq < a.grp, in1 = h0 + 2 * tq + 1 < a.grp;
 #pragma unroll
             for (int u = 0; u < SEL_UNROLL; ++u) {
-                int s = __dp4a(p.x, hi[u].x, 0);
-                s = __dp4a(p.y, hi[u].y, s);
-                s = __dp4a(p.z, hi[u].z, s);
-                s = __dp4a(p.w, hi[u].w, s);
-                s = __dp4a(n.x, lo[u].x, s);
-                s = __dp4a(n.y, lo[u].y, s);
-                s = __dp4a(n.z, lo[u].z, s);
-                s = __dp4a(n.w, lo[u].w, s);
+                int c[4] = {0, 0, 0, 0};
 #pragma unroll
-                for (int o = LP / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                best[u] = fmaxf(best[u], (float)s * unit);
+                for (int b = 0; b < 2 * D / 64; ++b) {
+                    const int4 x = w[u][0][b], y = w[u][1][b];
+                    const int a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
+                    mma_s8(c, a0, q[b].x, q[b].y);
+                    mma_s8(c, a1, q[b].z, q[b].w);
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    if (in0) best[u][r] = fmaxf(best[u][r], (float)c[2 * r] * u0);
+                    if (in1) best[u][r] = fmaxf(best[u][r], (float)c[2 * r + 1] * u1);
+                }
             }
         }
         __syncwarp();   // the page numbers are read
 #pragma unroll
-        for (int u = 0; u < SEL_UNROLL; ++u) {
-            const int j = j0 + u * NW * PPW;
-            if (j < own) {
-                // the record's exponent is within [-60, 40] when this library wrote it
-                const uint32_t key = ok[u] ? order_key(best[u] * two_to(min(max(ex[u], -60), 40))) : 0u;
-                if (part == 0) keys[j] = key;
+        for (int u = 0; u < SEL_UNROLL; ++u)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float s = best[u][r];
+                s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, 1));
+                s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, 2));
+                const int j = j0 + u * NW * 16 + g + 8 * r;
+                if (j < p1) {
+                    // the record's exponent is within [-60, 40] when this library wrote it
+                    const uint32_t key = ok[u][r] ? order_key(s * two_to(min(max(ex[u][r], -60), 40))) : 0u;
+                    if (tq == 0) keys[j] = key;
+                    kmin = min(kmin, key);
+                    kmax = max(kmax, key);
+                }
+            }
+    }
+    if (NW > 1 && ranks > 1) {
+        cluster_sync();   // every share is scored
+        if (rank == 0) {
+            for (int j = share + tid; j < own; j += NT) {
+                const uint32_t key = ld_peer(smem_u32(keys + j), (uint32_t)(j / share));
+                keys[j] = key;
                 kmin = min(kmin, key);
                 kmax = max(kmax, key);
             }
         }
+        cluster_sync();   // and collected: the others' shared memory may go
+        if (rank) return;
     }
     kmin = __reduce_min_sync(0xffffffffu, kmin);
     kmax = __reduce_max_sync(0xffffffffu, kmax);
@@ -422,7 +486,25 @@ int launch_select(const SelArgs& s, cudaStream_t st) {
     const long long items = (long long)s.n * s.hkv;
     auto kernel = select_kernel<T, D, NW>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = launch(kernel, dim3((unsigned)((items + ITEMS - 1) / ITEMS)), dim3(NW == 1 ? 256 : NW * 32), smem, st, s);
+    if (e != cudaSuccess) return note_cuda(e, "page selection attribute");
+    // a cluster to an item: doubled while all its CTAs have an SM each and a CTA keeps 256 pages or more
+    unsigned ranks = 1;
+    while (NW > 1 && ranks < 8 && items * ranks * 2 <= sm_count() && s.cols >= 512 * (int)ranks) ranks *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((items + ITEMS - 1) / ITEMS) * ranks);
+    cfg.blockDim = dim3(NW == 1 ? 256 : NW * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ranks;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = NW > 1 ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, s);
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "page selection");
 }
 

@@ -20,8 +20,10 @@
 // cycles of the special-function units): the tensor core bounds the tile when
 // there are many rows, HBM when there are few.
 //
-// Warps: 0 K producer, 1 MMA (and TMEM owner), 2 V producer, 3-6 softmax of A,
-// 7-10 softmax of B (a thread per row; also load Q and store the parts).  K and
+// Warps: 0 K producer, 1 MMA (and TMEM owner), 2 V producer, 3-10 softmax of A,
+// 11-18 softmax of B (two threads to a row, 64 keys each; they also load Q and
+// store the parts).  With one thread to a row the softmax took 2650 cycles of a
+// tile and its latency, not the tensor core, set the pace (4940 cycles).  K and
 // V come page by page through a rank-5 tensor map, so the pool's strides are
 // free; V is taken as it lies ([key][dim], the MMA's MN-major B operand).
 // Every wait is bounded and ends in the status word.
@@ -36,14 +38,16 @@ namespace mq {
 namespace paged {
 
 constexpr int PATOM = 128 * 128;         // bytes of 128 rows x 64 elements, 128-byte swizzle
-constexpr int PFX_THREADS = 352;
+constexpr int PFX_THREADS = 608;
 constexpr int PFX_MAX_GROUPS = 256;
 
 template <int D>
 struct PfxSmem {
     static constexpr int TILE = (D / 64) * PATOM;
     static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE, BAR = 6 * TILE;
-    static constexpr int SCHED = BAR + 256;
+    static constexpr int RED = BAR + 256;               // fp32 [2 streams][2 tiles][2 halves][128] row maxima
+    static constexpr int SUM = RED + 2 * 2 * 2 * 128 * 4;   // fp32 [2 streams][2 halves][128] row sums
+    static constexpr int SCHED = SUM + 2 * 2 * 128 * 4;
     static constexpr size_t bytes(int NG) { return SCHED + (size_t)(NG + 1) * 4 + (size_t)(2 * NG + 1) * 4 + 16 + 1024; }
 };
 
@@ -142,13 +146,13 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&q_full[i], 4);
+            mbar_init(&q_full[i], 8);
             mbar_init(&k_full[i], 1);
             mbar_init(&k_empty[i], 1);
             mbar_init(&v_full[i], 1);
             mbar_init(&v_empty[i], 1);
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
+            mbar_init(&p_full[i], 8);
             mbar_init(&o_full[i], 1);
         }
         mbar_init(drain, 1);
@@ -341,17 +345,27 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
         while (!mbar_try_wait(drain, 0) && clock64() - t0 < WAIT_CYCLES) {
         }
     } else {
-        // ---- softmax of stream q: a thread per row ----
-        const int q = warp < 7 ? 0 : 1;
+        // ---- softmax of stream q, column half hh: a thread per row ----
+        const int q = (warp - 3) >> 3, hh = ((warp - 3) >> 2) & 1;
         const int quad = warp & 3;                     // the TMEM lanes this warp may touch
+        const int r = quad * 32 + lane;
         const float scale = fabsf(a.scale_log2);
         const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
         const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
-        const uint32_t sa = tmem + lane_off + q * 128, oa = tmem + lane_off + 256 + q * 128;
+        const uint32_t sa = tmem + lane_off + q * 128 + hh * 64, oa = tmem + lane_off + 256 + q * 128 + hh * (D / 2);
+        float* red = reinterpret_cast<float*>(smem + L::RED) + q * 512;
+        float* sums = reinterpret_cast<float*>(smem + L::SUM) + q * 256;
         constexpr float GROW = 8.f;
+        // the two warps of a row meet at a barrier of their own; one whose wait failed goes on to the end
+        // without waiting, so that its partner never stands alone
+        auto meet = [&]() { named_bar_sync(1 + q * 4 + quad, 64); };
         int ns = 0, no = 0;
         bool ok = true;
-        for (uint32_t x = x0; ok && x < xe;) {
+        auto got = [&](uint64_t* bar, uint32_t parity) {
+            if (ok) ok = __all_sync(0xffffffffu, wait(bar, parity));
+            return ok;
+        };
+        for (uint32_t x = x0; x < xe;) {
             const PfxSeg e = segment(x);
             if (e.n <= 0) continue;
             const int mine = e.two ? e.n : (e.n + 1 - q) >> 1;   // this stream's tiles
@@ -360,39 +374,37 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
             const uint16_t* src = nullptr;
             float* part = nullptr;
             {
-                const int w = quad * 32 + lane, wr = e.two ? q * 128 + w : w;
+                const int wr = e.two ? q * 128 + r : r;
                 if (wr < e.rows) {
                     const int t = (e.r0 + wr) / grp, head = e.h * grp + e.r0 + wr - t * grp, tok = q_start(a, s.gs[e.g]) + t;
                     src = a.q + tok * a.q_tok + head * a.q_head;
-                    part = !e.whole ? a.ws.pfx_slots + ((2ll * blockIdx.x + e.start) * PROWS + q * 128 + w) * LD
+                    part = !e.whole ? a.ws.pfx_slots + ((2ll * blockIdx.x + e.start) * PROWS + q * 128 + r) * LD
                                     : a.ws.pfx_rowp + ((e.two ? 0 : (long long)q * a.total_q * a.hq) + (long long)tok * a.hq + head) * LD;
                 }
             }
             if (!mine) {   // a run of one tile: this stream's part is empty
-                if (part)
+                if (part && hh == 0)
                     for (int i = 0; i < LD; ++i) part[i] = i == 0 ? -INFINITY : 0.f;
                 continue;
             }
+            meet();   // both warps are done with the Q rows of the item before
             // Q rows, swizzled as TMA would, zeros past the end; a negative scale turns their
-            // signs.  LPR lanes side by side on a row, eight loads in flight.
+            // signs.  Half the rows each, LPR lanes side by side on a row, all loads in flight.
             {
-                constexpr int LPR = D / 8, RPI = 32 / LPR;
+                constexpr int LPR = D / 8, RPI = 32 / LPR, N = 16 / RPI;
                 const int ch = lane % LPR, sub = lane / LPR;
-#pragma unroll 1
-                for (int k0 = 0; k0 < 32; k0 += 8 * RPI) {
-                    uint4 v[8];
+                uint4 v[N];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint16_t* row = from_lane(src, k0 + i * RPI + sub);
-                        v[i] = row ? __ldg(reinterpret_cast<const uint4*>(row + ch * 8)) : make_uint4(0, 0, 0, 0);
-                    }
+                for (int i = 0; i < N; ++i) {
+                    const uint16_t* row = from_lane(src, hh * 16 + i * RPI + sub);
+                    v[i] = row ? __ldg(reinterpret_cast<const uint4*>(row + ch * 8)) : make_uint4(0, 0, 0, 0);
+                }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int w = quad * 32 + k0 + i * RPI + sub;
-                        v[i].x ^= sign; v[i].y ^= sign; v[i].z ^= sign; v[i].w ^= sign;
-                        *reinterpret_cast<uint4*>(smem + L::Q + q * TILE + (ch >> 3) * PATOM + w * 128 +
-                                                  (((ch & 7) ^ (w & 7)) << 4)) = v[i];
-                    }
+                for (int i = 0; i < N; ++i) {
+                    const int w = quad * 32 + hh * 16 + i * RPI + sub;
+                    v[i].x ^= sign; v[i].y ^= sign; v[i].z ^= sign; v[i].w ^= sign;
+                    *reinterpret_cast<uint4*>(smem + L::Q + q * TILE + (ch >> 3) * PATOM + w * 128 +
+                                              (((ch & 7) ^ (w & 7)) << 4)) = v[i];
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -400,36 +412,34 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
             }
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < mine; ++j, ++ns) {
-                ok = wait(&s_full[q], ns & 1);
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
+                float tmax = -INFINITY;
                 const int t = e.t0 + (e.two ? j : 2 * j + q);
-                const int valid = s.eff[e.g] * page - t * PK;
-                // the end of the prefix: scores past it are set to minus infinity in TMEM
-                if (valid < PK) {
+                if (got(&s_full[q], ns & 1)) {
+                    tc_fence_after();
+                    const int valid = s.eff[e.g] * page - t * PK - hh * 64;
+                    // the end of the prefix: scores past it are set to minus infinity in TMEM
+                    if (valid < 64) {
 #pragma unroll 1
-                    for (int i = 0; i < PK; i += 32) {
-                        float sv[32];
-                        tmem_ld32(sa + i, sv);
+                        for (int i = 0; i < 64; i += 32) {
+                            float sv[32];
+                            tmem_ld32(sa + i, sv);
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) sv[k] = i + k < valid ? sv[k] : -INFINITY;
-                        tmem_st32(sa + i, sv);
+                            for (int k = 0; k < 32; ++k) sv[k] = i + k < valid ? sv[k] : -INFINITY;
+                            tmem_st32(sa + i, sv);
+                        }
                     }
-                }
-                // two passes over S in TMEM: the code stays small (a run is a few tiles long, and
-                // fetching unrolled code the first time cost more than reading S twice)
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-                for (int i = 0; i < PK; i += 64) {
-                    float sv[64];
-                    tmem_ld64(sa + i, sv);
+                    // two passes over S in TMEM: the code stays small (a run is a few tiles long, and
+                    // fetching unrolled code the first time cost more than reading S twice)
+                    float sv[64], mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    tmem_ld64(sa, sv);
 #pragma unroll
                     for (int k = 0; k < 64; ++k) mx[k & 3] = fmaxf(mx[k & 3], sv[k]);
+                    tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
                 }
-                const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+                red[((j & 1) * 2 + hh) * 128 + r] = tmax;
+                meet();
+                if (!ok) continue;
+                tmax = fmaxf(tmax, red[((j & 1) * 2 + (hh ^ 1)) * 128 + r]);
                 // a row's maximum moves only when it grew by more than 2^8; weights stay below 256
                 float corr = 1.f;
                 if (tmax > m + GROW) {
@@ -438,9 +448,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
                 }
                 l *= corr;
                 if (j && __any_sync(0xffffffffu, corr != 1.f)) {
-                    // s_full covers the PV before it, so O is at rest
+                    // s_full covers the PV before it, so O is at rest; half its columns each
 #pragma unroll 1
-                    for (int i = 0; i < D; i += 16) {
+                    for (int i = 0; i < D / 2; i += 16) {
                         float v[16];
                         tmem_ld16(oa + i, v);
 #pragma unroll
@@ -451,7 +461,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
                 const float u = m == -INFINITY ? 0.f : m;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-                for (int i = 0; i < PK; i += 32) {
+                for (int i = 0; i < 64; i += 32) {
                     float sv[32];
                     uint32_t pk[32];   // 32 weights in 16 columns, their remainders in the next 16
                     tmem_ld32(sa + i, sv);
@@ -472,43 +482,37 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[q]);
             }
-            if (!ok) break;
-            ok = wait(&o_full[q], no & 1);
+            const bool done = got(&o_full[q], no & 1);
             ++no;
-            if (!__all_sync(0xffffffffu, ok)) {
-                ok = false;
-                break;
-            }
+            sums[hh * 128 + r] = l;
+            meet();
+            if (!done) continue;
             tc_fence_after();
-            // the part rows, 64 columns at a time through this warp's rows of the Q tile (every S
-            // that reads it is done), so that 16 lanes write 256 contiguous bytes of a row
-            {
-                constexpr int W = D / 2, LPR = W / 4;   // 32 rows x 64 (D 128) or 32 (D 64) floats
-                auto stage = [&](int row, int c) -> float4* {   // 16-byte piece c of a row, in this warp's own Q rows
-                    return reinterpret_cast<float4*>(smem + L::Q + q * TILE + (c >> 3) * PATOM + (quad * 32 + row) * 128 +
-                                                     (((c & 7) ^ (row & 7)) << 4));
-                };
-                if (part) *reinterpret_cast<float4*>(part) = make_float4(m, l, 0.f, 0.f);
+            l += sums[(hh ^ 1) * 128 + r];
+            // the part rows, this half's columns, a quarter of D at a time through half of the row's bytes of
+            // the Q tile (every S that reads it is done), so that lanes side by side write 64 or 128 bytes of a row
+            if (part && hh == 0) *reinterpret_cast<float4*>(part) = make_float4(m, l, 0.f, 0.f);
+            constexpr int W = D / 4, LPR = W / 4, RPI = 32 / LPR;
+            auto stage = [&](int row, int c) -> float4* {   // 16-byte piece c of this half's share of a row
+                const int at = D == 128 ? c : hh * 4 + c;
+                return reinterpret_cast<float4*>(smem + L::Q + q * TILE + (D == 128 ? hh * PATOM : 0) + (quad * 32 + row) * 128 +
+                                                 ((at ^ (row & 7)) << 4));
+            };
 #pragma unroll 1
-                for (int i = 0; i < D; i += W) {
+            for (int i = 0; i < D / 2; i += W) {
+                float v[W];
+                if (W == 32) tmem_ld32(oa + i, v);
+                else tmem_ld16(oa + i, v);
 #pragma unroll
-                    for (int c = 0; c < W; c += 32) {
-                        float v[32];
-                        tmem_ld32(oa + i + c, v);
-#pragma unroll
-                        for (int k = 0; k < 32; k += 4)
-                            *stage(lane, (c + k) >> 2) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-                    }
-                    __syncwarp();
-                    constexpr int RPI = 32 / LPR;
-                    const int ch = lane % LPR, sub = lane / LPR;
+                for (int k = 0; k < W; k += 4) *stage(lane, k >> 2) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                __syncwarp();
+                const int ch = lane % LPR, sub = lane / LPR;
 #pragma unroll 4
-                    for (int k = sub; k < 32; k += RPI) {
-                        float* to = from_lane(part, k);
-                        if (to) *reinterpret_cast<float4*>(to + 4 + i + ch * 4) = *stage(k, ch);
-                    }
-                    __syncwarp();
+                for (int k = sub; k < 32; k += RPI) {
+                    float* to = from_lane(part, k);
+                    if (to) *reinterpret_cast<float4*>(to + 4 + hh * (D / 2) + i + ch * 4) = *stage(k, ch);
                 }
+                __syncwarp();
             }
             tc_fence_before();
         }

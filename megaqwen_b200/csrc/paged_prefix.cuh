@@ -282,7 +282,6 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
         uint32_t np0 = 0, np1 = 0;          // PVs issued per stream
         uint32_t nq0 = 0, nq1 = 0;          // Q tiles used per stream
         bool ok = true;
-        auto ready = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); };
         auto scores = [&](int q, int kc, bool last_use) {
             const uint32_t sq = base + L::Q + q * TILE, sk = base + L::K + (kc & 1) * TILE;
 #pragma unroll
@@ -312,22 +311,24 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
             if (n <= 0) continue;
             const bool two = uniform(e.two);
             const int steps = two ? 2 * n : n;
-            // step i: the stream's PV of its tile before (step i - 2), then its S of this one.  All
-            // that the step needs is waited for first: a wait behind issued MMAs takes as long
-            // as those do (measured: 350 to 500 idle cycles for each)
+            // step i: the stream's PV of its tile before (step i - 2), then its S of this one.  What the
+            // step needs is waited for by four lanes at once.  (A second MMA warp, one for each stream, was
+            // slower, 73 us against 58 for a 32k prefix: MMAs of two accumulators taking turns run slower than
+            // runs of one.)
             for (int i = 0; ok && i < steps + 2; ++i) {
                 const int q = i & 1;
                 const bool pv = i >= 2, sc = i < steps;
                 const int vc = c0 + (two ? (i - 2) >> 1 : i - 2), kc = c0 + (two ? i >> 1 : i);
                 if (!pv && !sc) continue;   // a run of one tile: stream B has none
-                if (sc) {
-                    if (!pv) ok = ready(&q_full[q], (q ? nq1++ : nq0++) & 1);
-                    ok = ok && ready(&k_full[kc & 1], (kc >> 1) & 1);
-                }
-                if (pv) {
-                    ok = ok && ready(&v_full[vc & 1], (vc >> 1) & 1);
-                    ok = ok && ready(&p_full[q], (q ? np1++ : np0++) & 1);
-                }
+                uint64_t* bar = nullptr;
+                uint32_t parity = 0;
+                if (lane == 0 && sc) bar = &k_full[kc & 1], parity = kc >> 1;
+                if (lane == 1 && pv) bar = &v_full[vc & 1], parity = vc >> 1;
+                if (lane == 2 && pv) bar = &p_full[q], parity = q ? np1 : np0;
+                if (lane == 3 && !pv) bar = &q_full[q], parity = q ? nq1 : nq0;
+                ok = __all_sync(0xffffffffu, !bar || wait(bar, parity & 1));
+                if (pv) (q ? np1 : np0)++;
+                else (q ? nq1 : nq0)++;
                 if (!ok) break;
                 tc_fence_after();
                 if (elect_one()) {

@@ -4,6 +4,7 @@
 // counterpart; Python names are in megaqwen_b200/paged.py.
 
 #include <torch/extension.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -26,6 +27,13 @@ void raise_rc(int rc, const char* where) {
         fail(std::string(where) + ": " + mq_error_string(rc) + " (code " + std::to_string(rc) + ")" +
              (rc == MQ_ERR_CUDA ? std::string(" ") + mq_last_error_detail() : ""));
 }
+
+// Uninitialised tensors straight from the caching allocator: the dispatcher's
+// path costs about half of a short call's host time.
+Tensor blank(at::IntArrayRef sizes, torch::ScalarType type, const torch::Device& dev) {
+    return Tensor(at::detail::empty_cuda(sizes, type, dev, c10::nullopt));
+}
+Tensor scratch(size_t bytes, const torch::Device& dev) { return blank({(int64_t)bytes}, torch::kUInt8, dev); }
 
 cudaStream_t stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
@@ -125,7 +133,7 @@ struct Table {
         c.status = status_of(status, dev);
         if (workspace) {
             c.workspace_bytes = mq_paged_workspace_bytes(c.num_pages, (int)n);
-            ws = torch::empty({(int64_t)c.workspace_bytes}, torch::dtype(torch::kUInt8).device(dev));
+            ws = scratch(c.workspace_bytes, dev);
             c.workspace = ws.data_ptr();
         }
     }
@@ -174,8 +182,7 @@ void paged_copy(Tensor k, Tensor v, Tensor src, Tensor dst, OptTensor dst_k, Opt
     same_pools(a, b);
     const int n = (int)src.numel();
     c10::cuda::CUDAGuard guard(k.device());
-    Tensor ws = torch::empty({(int64_t)mq_paged_workspace_bytes(b.num_pages, n)},
-                             torch::dtype(torch::kUInt8).device(k.device()));
+    Tensor ws = scratch(mq_paged_workspace_bytes(b.num_pages, n), k.device());
     raise_rc(mq_paged_copy(&a, &b, ints(src, k.device(), "src"), ints(dst, k.device(), "dst", n), n,
                            status_of(status, k.device()), ws.data_ptr(), (size_t)ws.numel(), stream_of(k)), "paged copy");
 }
@@ -231,7 +238,7 @@ Tensor rope(Tensor x, Tensor positions, Tensor cos, Tensor sin, bool interleaved
     const auto dev = x.device();
     rope_args(p, cos, sin, dev, x.size(2), interleaved, inverse);
     c10::cuda::CUDAGuard guard(dev);
-    Tensor out = torch::empty(x.sizes(), x.options());
+    Tensor out = blank(x.sizes(), x.scalar_type(), dev);
     p.positions = ints(positions, dev, "positions", x.size(0));
     p.q = x.data_ptr();
     p.q_out = out.data_ptr();
@@ -260,7 +267,7 @@ Tensor rope_append(Tensor q, Tensor k, Tensor v, Tensor k_pages, Tensor v_pages,
     mq_rope_params p = {};
     rope_args(p, cos, sin, dev, D, interleaved, false);
     c10::cuda::CUDAGuard guard(dev);
-    Tensor out = torch::empty(q.sizes(), q.options());
+    Tensor out = blank(q.sizes(), q.scalar_type(), dev);
     p.dtype = pool.dtype;
     p.q = q.data_ptr();
     p.q_out = out.data_ptr();
@@ -324,7 +331,7 @@ Tensor attend(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor len
     if (q.size(0) && !slots.numel()) fail("query tokens without sequences");
     c10::cuda::CUDAGuard guard(dev);
     const Tensor qq = pieces(q);
-    Tensor out = torch::empty(q.sizes(), q.options());
+    Tensor out = blank(q.sizes(), q.scalar_type(), dev);
     if (!out.numel()) return out;
     p.pool = &pool;
     p.q = qq.data_ptr();
@@ -340,7 +347,7 @@ Tensor attend(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor len
     p.scale = scale.has_value() ? (float)*scale : 1.0f / std::sqrt((float)pool.head_dim);
     p.status = status_of(status, dev);
     p.workspace_bytes = mq_paged_attend_workspace_bytes(&p);
-    Tensor ws = torch::empty({(int64_t)p.workspace_bytes}, torch::dtype(torch::kUInt8).device(dev));
+    Tensor ws = scratch(p.workspace_bytes, dev);
     p.workspace = ws.data_ptr();
     raise_rc(mq_paged_attend(&p, stream_of(q)), "attend");
     return out;
@@ -364,8 +371,8 @@ std::tuple<Tensor, Tensor> sparse_attend(Tensor q, Tensor k_pages, Tensor v_page
     p.positions = ints(positions, dev, "positions", q.size(0));
     c10::cuda::CUDAGuard guard(dev);
     const Tensor qq = pieces(q);
-    Tensor out = torch::empty(q.sizes(), q.options());
-    Tensor sel = torch::empty({q.size(0), pool.num_kv_heads, top_k}, torch::dtype(torch::kInt32).device(dev));
+    Tensor out = blank(q.sizes(), q.scalar_type(), dev);
+    Tensor sel = blank({q.size(0), pool.num_kv_heads, top_k}, torch::kInt32, dev);
     if (!out.numel()) return std::make_tuple(out, sel);
     p.pool = &pool;
     p.q = qq.data_ptr();
@@ -382,7 +389,7 @@ std::tuple<Tensor, Tensor> sparse_attend(Tensor q, Tensor k_pages, Tensor v_page
     p.scale = scale.has_value() ? (float)*scale : 1.0f / std::sqrt((float)pool.head_dim);
     p.status = status_of(status, dev);
     p.workspace_bytes = mq_paged_sparse_workspace_bytes(&p);
-    Tensor ws = torch::empty({(int64_t)p.workspace_bytes}, torch::dtype(torch::kUInt8).device(dev));
+    Tensor ws = scratch(p.workspace_bytes, dev);
     p.workspace = ws.data_ptr();
     raise_rc(mq_paged_sparse(&p, stream_of(q)), "sparse_attend");
     return std::make_tuple(out, sel);

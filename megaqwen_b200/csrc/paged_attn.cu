@@ -435,7 +435,8 @@ int run_prefix(const RowArgs& a, const mq_paged_pool& pool, cudaStream_t st) {
     if (!pool_maps(&tk, &tv, pool, pool.page_size)) return MQ_ERR_CUDA;
     auto kernel = prefix_kernel<T, D>;
     const size_t smem = PfxSmem<D>::bytes(a.NG);
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static SmemLimit limit;
+    cudaError_t e = allow_smem(kernel, smem, limit);
     if (e == cudaSuccess) e = launch(kernel, dim3(sm_count()), dim3(PFX_THREADS), smem, st, tk, tv, a);
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "paged prefix attention");
 }
@@ -446,7 +447,8 @@ int run_rows(const RowArgs& a, const mq_paged_pool& pool, cudaStream_t st) {
     if (!pool_maps(&tk, &tv, pool, GRP)) return MQ_ERR_CUDA;
     auto kernel = rows_kernel<T, D, MODE, NT>;
     const size_t smem = (size_t)ROW_WARPS * RowWarp<T, D, NT>::RING + 1024 + (MODE == 0 ? sched_bytes(a.B, a.NG) : 0);
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static SmemLimit limit;
+    cudaError_t e = allow_smem(kernel, smem, limit);
     if (e != cudaSuccess) return note_cuda(e, "paged attention attribute");
     const int grid = row_grid(D, 8 * NT);
     e = launch(kernel, dim3(grid), dim3(ROW_THREADS), smem, st, tk, tv, a);
@@ -485,7 +487,8 @@ int launch_select(const SelArgs& s, cudaStream_t st) {
     const size_t smem = ITEMS * sel_item_bytes<D>(s.cols, s.grp);
     const long long items = (long long)s.n * s.hkv;
     auto kernel = select_kernel<T, D, NW>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static SmemLimit limit;
+    cudaError_t e = allow_smem(kernel, smem, limit);
     if (e != cudaSuccess) return note_cuda(e, "page selection attribute");
     // a cluster to an item: doubled while all its CTAs have an SM each and a CTA keeps 256 pages or more
     unsigned ranks = 1;

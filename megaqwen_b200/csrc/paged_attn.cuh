@@ -46,10 +46,11 @@ __device__ __forceinline__ int pages_for(int len, int shift) { return len <= 0 ?
 
 // What the join needs to know of a token: where its items start on the work
 // line (kv head 0, row tile 0), how long one is, and the token's first row.
-struct TokInfo {
+struct alignas(16) TokInfo {
     uint32_t own_base, pfx_base;
     int own_ng, own_nrt, own_r0;
     int pfx_ng, pfx_nrt, pfx_r0, pfx_rows;
+    int pad[3];
 };
 
 // Part rows are m, l, pad, pad, acc[D].  A run's split item sits in slot
@@ -232,28 +233,42 @@ __device__ inline bool build_sched(const RowArgs& a, const Sched& s, unsigned lo
     }
     __syncthreads();
     const int E = a.NG + (PFX ? 0 : a.B);
-    unsigned long long carry = 0;
-    for (int e0 = 0; e0 < E; e0 += NT) {   // NT entities at a time
-        const int e = e0 + tid;
-        unsigned long long cost = 0;
-        if (e < E) {
-            int tiles, ng;
-            if (e < a.NG) {
-                tiles = pfx_tiles(a, (q_start(a, s.gs[e + 1]) - q_start(a, s.gs[e])) * a.grp);
-                ng = pfx_groups(a, s.eff[e]);
-            } else {
-                const int b = e - a.NG;
-                tiles = row_tiles(a, (q_start(a, b + 1) - q_start(a, b)) * a.grp);
-                ng = own_groups(a, s, b);
-            }
-            if (ng) cost = (unsigned long long)(unsigned)tiles * (unsigned)(ng + ITEM_UNITS);
+    auto cost_of = [&](int e) -> unsigned long long {
+        int tiles, ng;
+        if (e < a.NG) {
+            tiles = pfx_tiles(a, (q_start(a, s.gs[e + 1]) - q_start(a, s.gs[e])) * a.grp);
+            ng = pfx_groups(a, s.eff[e]);
+        } else {
+            const int b = e - a.NG;
+            tiles = row_tiles(a, (q_start(a, b + 1) - q_start(a, b)) * a.grp);
+            ng = own_groups(a, s, b);
         }
-        unsigned long long x = cost;
+        return ng ? (unsigned long long)(unsigned)tiles * (unsigned)(ng + ITEM_UNITS) : 0;
+    };
+    auto sum_up = [&](unsigned long long x) {   // inclusive, over the warp
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
+        return x;
+    };
+    unsigned long long carry = 0;
+    if (E <= 32) {   // one warp's worth
+        if (warp == 0) {
+            const unsigned long long cost = lane < E ? cost_of(lane) : 0, x = sum_up(cost);
+            if (lane < E) s.off[lane] = (uint32_t)(x - cost);
+            if (lane == 31) {
+                s.off[E] = (uint32_t)x;
+                scratch[0] = x;
+            }
+        }
+        __syncthreads();
+        return scratch[0] * (unsigned)a.hkv < 0x7fffffffull;
+    }
+    for (int e0 = 0; e0 < E; e0 += NT) {   // NT entities at a time
+        const int e = e0 + tid;
+        const unsigned long long cost = e < E ? cost_of(e) : 0, x = sum_up(cost);
         if (lane == 31) scratch[warp] = x;
         __syncthreads();
         unsigned long long before = carry;
@@ -529,7 +544,9 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         prefetch_tmap(&tmV);
     }
     __syncwarp();
-    pdl_wait();
+    // After a prefix kernel nothing of its is read here: it started dependents only when everything before it
+    // was complete, so this kernel goes ahead beside its tail and waits for it at the end (the join needs both).
+    if (MODE == 1 || !a.tc) pdl_wait();
     pdl_trigger();
     Sched s;
     uint32_t work, origin = 0;   // where this kernel's work starts on the line
@@ -542,6 +559,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 note_status(a.status, MQ_ERR_INVALID_ARGUMENT);
                 a.ws.head[0] = 0;
             }
+            if (a.tc) pdl_wait();
             return;
         }
         origin = a.tc ? s.off[a.NG] * a.hkv : 0;
@@ -823,6 +841,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 a.ws.tok[i] = ti;
             }
         }
+        if (a.tc) pdl_wait();
     }
 }
 
@@ -832,8 +851,6 @@ template <typename T, int D, int MODE, int SPLIT>
 __global__ void __launch_bounds__(256, 3) join_kernel(const RowArgs a, uint32_t row_warps) {
     constexpr int LD = D + 4, V = D / 32;
     __shared__ float sm_m[8], sm_l[8], sm_o[8][D];
-    pdl_wait();
-    pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long rowi = (long long)blockIdx.x * (8 / SPLIT) + warp / SPLIT;
     if (rowi >= (long long)a.total_q * a.hq) return;
@@ -841,33 +858,47 @@ __global__ void __launch_bounds__(256, 3) join_kernel(const RowArgs a, uint32_t 
     const int tok = (int)((uint32_t)rowi / (uint32_t)a.hq), head = (int)(rowi - (long long)tok * a.hq);   // rows fit 31 bits
     const int grp = a.grp, h = head / grp, RT = a.rt;
     uint16_t* out = a.out + rowi * D;
+    pdl_wait();
+    pdl_trigger();
+    // both reads under way before either is looked at
+    uint4 hd = make_uint4(0, 0, 0, 0);
+    union {
+        uint4 w[3];
+        TokInfo ti;
+    } u;
+    if (MODE == 0) {
+        hd = __ldcg(reinterpret_cast<const uint4*>(a.ws.head));
+        const uint4* p = reinterpret_cast<const uint4*>(a.ws.tok + tok);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) u.w[i] = __ldcg(p + i);
+    }
     // the row's parts: np0 of the prefix (sub of them per run), then np1 of its own
     const float *src0 = nullptr, *src1 = nullptr;
     long long step0 = 0, step1 = 0;   // floats between parts
     int np0 = 0, np1 = 0, sub0 = 1;
     long long first0 = 0, first1 = 0, sub_step0 = 0;   // the first part of a split item is one slot further on
     if (MODE == 0) {
-        if (!a.ws.head[0]) {   // refused: zeros
+        if (!hd.x) {   // refused: zeros
             for (int d = sub * 32 + lane; d < D; d += SPLIT * 32) out[d] = 0;
             return;
         }
     }
     const int sp_ng = MODE == 1 ? a.top_k << (a.pool.shift - 4) : 0;
     const uint32_t quota =
-        MODE == 0 ? a.ws.head[1]
+        MODE == 0 ? hd.y
                   : quota_of((uint32_t)a.total_q * a.hkv * row_tiles(a, grp) * (sp_ng + ITEM_UNITS), row_warps);
     {
         int ng, r;
         uint32_t start;   // the item's first group on the line
         if (MODE == 0) {
-            const TokInfo ti = a.ws.tok[tok];
+            const TokInfo& ti = u.ti;
             ng = ti.own_ng;
             r = ti.own_r0 + head % grp;
             start = ti.own_base + ((uint32_t)h * ti.own_nrt + (r >> a.rt_shift)) * (ng + ITEM_UNITS) + ITEM_UNITS;
             if (ti.pfx_ng) {
                 const int R = a.tc ? PROWS : RT, pr = ti.pfx_r0 + head % grp, in = pr & (R - 1);
                 const uint32_t ps = ti.pfx_base + ((uint32_t)h * ti.pfx_nrt + (uint32_t)(pr - in) / R) * (ti.pfx_ng + ITEM_UNITS) + ITEM_UNITS;
-                const uint32_t pq = a.tc ? a.ws.head[2] : quota, w0 = ps / pq;
+                const uint32_t pq = a.tc ? hd.z : quota, w0 = ps / pq;
                 const int runs = (int)((ps + ti.pfx_ng - 1) / pq - w0) + 1;
                 if (a.tc && min(PROWS, ti.pfx_rows - (pr - in)) <= 128) sub0 = 2;   // both streams worked on this row
                 np0 = runs * sub0;

@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "megaqwen_b200.h"
@@ -72,6 +73,23 @@ inline int sm_count() {
     if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 148;
     if (!sms[dev]) cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
     return sms[dev] > 0 ? sms[dev] : 148;
+}
+
+// Raises a kernel's shared-memory limit where it is not high enough yet (the
+// driver call is worth avoiding in a call of a few microseconds).  `set` is the
+// kernel's own record, one entry per device.
+struct SmemLimit {
+    std::atomic<int> bytes[64];
+};
+template <typename K>
+cudaError_t allow_smem(K kernel, size_t bytes, SmemLimit& set) {
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 64 && set.bytes[dev].load(std::memory_order_relaxed) >= (int)bytes) return cudaSuccess;
+    const cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (r == cudaSuccess && dev < 64) set.bytes[dev].store((int)bytes, std::memory_order_relaxed);
+    return r;
 }
 
 // Every kernel here is launched as a programmatic dependent of the kernel

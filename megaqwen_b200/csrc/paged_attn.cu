@@ -15,24 +15,25 @@ bool make_tmap_nd(CUtensorMap* map, const void* ptr, bool bf16, int rank, const 
 namespace paged {
 
 // ---- choosing pages -----------------------------------------------------------------------
-// One item per (kv head, token), NW warps to an item.  Scores of all earlier
-// pages into shared memory as order-preserving 32-bit keys, then a radix
-// selection of the (top_k - 1)-th largest over the bits in which the keys
-// differ (8 at a time, ending as soon as a whole bin is taken), then the list
-// in ascending order.  Reads 2 D + 1 bytes per page, 16 bytes a lane, 32 pages
-// of a warp in flight.  The products run on mma.sync m16n8k32 (16 pages, 8 q
-// heads, 32 channels; dp4a took 110 instructions for what is 8 MMAs with two
-// heads): whole numbers, exact below 2^24, so the keys do not depend on their
-// order.
+// Scores of all earlier pages into shared memory as order-preserving 32-bit
+// keys, then a radix selection of the (top_k - 1)-th largest over the bits in
+// which the keys differ (8 at a time; a bin of up to 32 keys is ranked pair by
+// pair), then the list in ascending order.  Reads 2 D + 1 bytes per page.  The
+// products run on mma.sync m16n8k32 (16 pages, 8 columns, 32 channels; dp4a took
+// 110 instructions for what is 8 MMAs with two heads): whole numbers, exact below
+// 2^24, so the keys do not depend on their order.
 //
-// NW 16, an item per cluster of up to 8 CTAs: few items, whose reads have to be
-// spread; each CTA scores a share of the pages and the first one collects the
-// keys.  NW 1, eight items per CTA (consecutive tokens of one head, which read
-// the same records): many items, where the barriers of a CTA per item cost more
-// than the reads.
+// Two forms.  select_one_kernel: an item is a (kv head, token), a cluster of up to
+// 8 CTAs to an item, each scoring a share of the pages; for few items, whose reads
+// have to be spread.  select_eight_kernel: eight tokens of one kv head to a CTA,
+// each page's record read once for all of them that stand in the same sequence;
+// for many items (500 tokens x 8 heads, 250 pages each: 54 us with a warp to an
+// item of its own, 121 us with a CTA).
 constexpr int MAX_SPARSE_COLS = 49152;
 constexpr int MAX_SPARSE_GROUP = 64;   // q heads per kv head
-constexpr int SEL_UNROLL = 2;      // 16-page steps in flight
+constexpr int SEL_UNROLL = 2;          // 16-page steps in flight
+constexpr int SEL_WARPS = 16;          // of select_one_kernel
+constexpr int SEL_TOKENS = 8;          // of select_eight_kernel, a warp each
 
 struct SelArgs {
     const signed char* index;   // at the layer
@@ -56,8 +57,12 @@ __device__ __forceinline__ float two_to(int e) { return __int_as_float((e + 127)
 
 // heads are padded to a multiple of 8 with zeros
 template <int D>
-__host__ __device__ inline size_t sel_item_bytes(int cols, int grp) {
-    return (((size_t)cols * 4 + (size_t)((grp + 7) & ~7) * (2 * D + 4)) + 15) & ~(size_t)15;
+size_t sel_one_bytes(int cols, int grp) {
+    return (size_t)cols * 4 + (size_t)((grp + 7) & ~7) * (2 * D + 4);
+}
+template <int D>
+size_t sel_eight_bytes(int cols, int grp) {
+    return SEL_TOKENS * ((size_t)cols * 4 + (size_t)grp * (2 * D + 4));
 }
 
 __device__ __forceinline__ void mma_s8(int* d, const int* a, int b0, int b1) {
@@ -79,117 +84,302 @@ __device__ __forceinline__ uint32_t cluster_size() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ uint32_t ld_peer(uint32_t addr, uint32_t rank) {
-    uint32_t at, v;
+__device__ __forceinline__ void st_peer(uint32_t addr, uint32_t rank, uint32_t v) {
+    uint32_t at;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-    return v;
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
 
-template <typename T, int D, int NW>
-__global__ void __launch_bounds__(NW == 1 ? 256 : NW * 32) select_kernel(const SelArgs a) {
-    constexpr int ITEMS = NW == 1 ? 8 : 1, NT = NW * 32;
-    extern __shared__ __align__(16) uint8_t sel_smem[];
-    __shared__ int hist[ITEMS][256];
-    __shared__ int sums[2][NW];
-    __shared__ uint32_t s_pick[ITEMS][2];
-    const int lane = threadIdx.x & 31, sub = NW == 1 ? threadIdx.x >> 5 : 0;
-    const int warp = NW == 1 ? 0 : threadIdx.x >> 5, tid = NW == 1 ? lane : threadIdx.x;
-    uint8_t* mem = sel_smem + sub * sel_item_bytes<D>(a.cols, a.grp);
-    const int heads = (a.grp + 7) & ~7;
-    signed char* qpos = reinterpret_cast<signed char*>(mem);               // [heads][D]
-    signed char* qneg = qpos + heads * D;
-    float* qunit = reinterpret_cast<float*>(qneg + heads * D);             // [heads], 0 past grp
-    uint32_t* keys = reinterpret_cast<uint32_t*>(qunit + heads);           // [cols]
+// One head of a query in whole numbers, split by sign, by one warp; returns the unit.
+template <typename T, int D>
+__device__ __forceinline__ float whole_query(const float (&x)[D / 32], signed char* pos, signed char* neg, int lane) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) m = fmaxf(m, fabsf(x[i]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    m = fminf(m, Elem<T>::MAX);
+    const int e = m > 0.f ? min(max(ilogbf(m) - 6, -60), 40) : 0;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+        const float r = fminf(fmaxf(rintf(x[i] * two_to(-e)), -127.f), 127.f);
+        const int v = x[i] == x[i] ? (int)r : 0;
+        pos[lane + 32 * i] = (signed char)max(v, 0);
+        neg[lane + 32 * i] = (signed char)min(v, 0);
+    }
+    return two_to(e);
+}
+template <typename T, int D>
+__device__ __forceinline__ void load_query(float (&x)[D / 32], const uint16_t* q, int lane) {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) x[i] = q ? Elem<T>::up(__ldg(q + lane + 32 * i)) : 0.f;
+}
+
+// 16 pages a step: lane (g, t) reads channels 16 t .. of each 64-channel block of
+// pages g and g + 8, whose words are the A operand of two MMAs; the k index is
+// permuted alike in both operands.  Blocks: HI, then LO.
+template <int D>
+struct PageStep {
+    int4 w[2][2 * D / 64];
+    int ex[2];
+    __device__ __forceinline__ void load(const signed char* ix, long long i_page, const int (&pid)[2], int tq) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const signed char* rec = ix + (pid[r] >= 0 ? pid[r] : 0) * i_page;
+#pragma unroll
+            for (int b = 0; b < 2 * D / 64; ++b) w[r][b] = __ldg(reinterpret_cast<const int4*>(rec + 64 * b + 16 * tq));
+            ex[r] = __ldg(rec + 2 * D);
+        }
+    }
+    __device__ __forceinline__ void dot(int (&c)[4], const int4 (&q)[2 * D / 64]) const {
+        c[0] = c[1] = c[2] = c[3] = 0;
+#pragma unroll
+        for (int b = 0; b < 2 * D / 64; ++b) {
+            const int4 x = w[0][b], y = w[1][b];
+            const int a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
+            mma_s8(c, a0, q[b].x, q[b].y);
+            mma_s8(c, a1, q[b].z, q[b].w);
+        }
+    }
+    // the record's exponent is within [-60, 40] when this library wrote it
+    __device__ __forceinline__ uint32_t key(int r, float score, bool there) const {
+        return there ? order_key(score * two_to(min(max(ex[r], -60), 40))) : 0u;
+    }
+};
+
+// What a selection needs beside its keys.
+struct Picker {
+    int* hist;        // [256]
+    int* list;        // [32]
+    uint32_t* pick;   // [4]
+    int* sums;        // [2][NW]
+};
+
+// The `want` largest of keys[0 .. own - 1] (ties: the lowest first), 0 < want < own,
+// as places in ascending order into sel.  NW warps together.
+template <int NW>
+__device__ __forceinline__ void choose(const uint32_t* keys, int own, int want, int* sel, const Picker& s, int warp, int lane) {
+    constexpr int NT = NW * 32;
+    const int tid = warp * 32 + lane;
     auto sync = [&]() {
         if (NW == 1) __syncwarp();
         else __syncthreads();
     };
+    uint32_t kmin = 0xffffffffu, kmax = 0;
+    for (int j = tid; j < own; j += NT) {
+        kmin = min(kmin, keys[j]);
+        kmax = max(kmax, keys[j]);
+    }
+    kmin = __reduce_min_sync(0xffffffffu, kmin);
+    kmax = __reduce_max_sync(0xffffffffu, kmax);
+    if (NW > 1) {
+        if (lane == 0) {
+            s.sums[warp] = (int)kmin;
+            s.sums[NW + warp] = (int)kmax;
+        }
+        __syncthreads();
+        kmin = __reduce_min_sync(0xffffffffu, (uint32_t)s.sums[lane % NW]);
+        kmax = __reduce_max_sync(0xffffffffu, (uint32_t)s.sums[NW + lane % NW]);
+    }
+    // keys agree above bit `bits`; of those that match `prefix` under `mask` the largest `need` are wanted
+    int bits = 32 - __clz((int)(kmin ^ kmax)), need = want;
+    uint32_t mask = bits == 32 ? 0u : 0xffffffffu << bits, prefix = kmax & mask;
+    while (bits > 0) {
+        const int shift = max(bits - 8, 0);
+        for (int i = tid; i < 256; i += NT) s.hist[i] = 0;
+        if (tid == 0) s.pick[2] = 0;
+        sync();
+        for (int j = tid; j < own; j += NT) {
+            const uint32_t k = keys[j];
+            if ((k & mask) == prefix) atomicAdd(&s.hist[(k & ~mask) >> shift], 1);
+        }
+        sync();
+        if (warp == 0) {
+            // lane i holds bins 255 - 8 i .. 248 - 8 i; the bin in which the count passes `need`
+            int c[8], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                c[i] = s.hist[255 - 8 * lane - i];
+                sum += c[i];
+            }
+            int x = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            int above = x - sum;
+            if (above < need && need <= x) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (above < need && need <= above + c[i]) {
+                        s.pick[0] = prefix | (uint32_t)(255 - 8 * lane - i) << shift;
+                        s.pick[1] = (uint32_t)(need - above);   // wanted of the bin
+                        s.pick[3] = (uint32_t)c[i];
+                        above = need;   // found
+                    } else {
+                        above += c[i];
+                    }
+                }
+            }
+        }
+        sync();
+        prefix = s.pick[0];
+        need = (int)s.pick[1];
+        const int in_bin = (int)s.pick[3];
+        mask = 0xffffffffu << shift;
+        bits = shift;
+        if (need == in_bin || bits == 0) break;   // all of the bin, or all its keys are equal
+        if (in_bin <= 32) {
+            // few keys: rank them against each other, equal ones by their place
+            for (int j = tid; j < own; j += NT)
+                if ((keys[j] & mask) == prefix) s.list[atomicAdd(&s.pick[2], 1u)] = j;
+            sync();
+            if (warp == 0) {
+                const int at = lane < in_bin ? s.list[lane] : 0x7fffffff;
+                const uint32_t k = lane < in_bin ? keys[at] : 0u;
+                int rank = 0;
+                for (int i = 0; i < in_bin; ++i) {
+                    const uint32_t ki = __shfl_sync(0xffffffffu, k, i);
+                    const int ai = __shfl_sync(0xffffffffu, at, i);
+                    rank += ki > k || (ki == k && ai < at);
+                }
+                const unsigned last = __ballot_sync(0xffffffffu, lane < in_bin && rank == need - 1);
+                const uint32_t low = __shfl_sync(0xffffffffu, k, __ffs((int)last) - 1);
+                const unsigned same = __ballot_sync(0xffffffffu, lane < in_bin && rank < need && k == low);
+                if (lane == 0) {
+                    s.pick[0] = low;
+                    s.pick[1] = (uint32_t)__popc(same);
+                }
+            }
+            sync();
+            prefix = s.pick[0];
+            need = (int)s.pick[1];
+            mask = 0xffffffffu;
+            break;
+        }
+        sync();   // the pick is read before the next pass writes it
+    }
+    // keys above the bin, and the first `need` in it, in ascending order of the page
+    const int seg = (ceil_div(own, NW) + 31) & ~31;
+    const int lo = min(own, warp * seg), hi = min(own, lo + seg);
+    int gt = 0, eq = 0;
+    if (NW > 1) {
+        for (int i = lo; i < hi; i += 32) {
+            const uint32_t k = i + lane < hi ? keys[i + lane] & mask : 0u;
+            gt += __popc(__ballot_sync(0xffffffffu, i + lane < hi && k > prefix));
+            eq += __popc(__ballot_sync(0xffffffffu, i + lane < hi && k == prefix));
+        }
+        if (lane == 0) {
+            s.sums[warp] = gt;
+            s.sums[NW + warp] = eq;
+        }
+        __syncthreads();
+        gt = eq = 0;
+        for (int w = 0; w < warp; ++w) {
+            gt += s.sums[w];
+            eq += s.sums[NW + w];
+        }
+    }
+    const unsigned below = (1u << lane) - 1u;
+    for (int i = lo; i < hi; i += 32) {
+        const uint32_t k = i + lane < hi ? keys[i + lane] & mask : 0u;
+        const bool is_gt = i + lane < hi && k > prefix, is_eq = i + lane < hi && k == prefix;
+        const unsigned mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
+        const int eq_at = eq + __popc(me & below);
+        if (is_gt || (is_eq && eq_at < need)) sel[gt + __popc(mg & below) + min(eq_at, need)] = i + lane;
+        gt += __popc(mg);
+        eq += __popc(me);
+    }
+}
+
+// Where token t's choice is clear without scores (a wrong place, every page, only
+// its own), writes it and returns 0; otherwise the number of pages to score.
+// `write`: this group of nt threads writes.
+__device__ __forceinline__ int pages_to_score(const SelArgs& a, int slot, int pos, int* sel, bool write, int tid, int nt) {
+    const bool bad_slot = slot < 0 || slot >= a.num_slots;
+    const int own = pos >> a.shift, want = a.top_k - 1;
+    if (bad_slot || pos < 0 || own >= a.cols) {
+        if (write && tid == 0) note_status(a.status, bad_slot ? MQ_ERR_BAD_SLOT : MQ_ERR_BAD_POSITION);
+        for (int i = tid; write && i < a.top_k; i += nt) sel[i] = -1;
+        return 0;
+    }
+    if (own <= want || want == 0) {
+        for (int i = tid; write && i < a.top_k; i += nt) sel[i] = want == 0 ? own : i <= own ? i : -1;
+        return 0;
+    }
+    return own;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(SEL_WARPS * 32) select_one_kernel(const SelArgs a) {
+    constexpr int NW = SEL_WARPS, NT = NW * 32;
+    extern __shared__ __align__(16) uint8_t sel_smem[];
+    __shared__ int hist[256], sums[2 * NW], list[32];
+    __shared__ uint32_t pick[4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = threadIdx.x;
+    const int heads = (a.grp + 7) & ~7;
+    signed char* qpos = reinterpret_cast<signed char*>(sel_smem);          // [heads][D]
+    signed char* qneg = qpos + heads * D;
+    float* qunit = reinterpret_cast<float*>(qneg + heads * D);             // [heads]
+    uint32_t* keys = reinterpret_cast<uint32_t*>(qunit + heads);           // [cols]
     pdl_wait();
     pdl_trigger();
-    const uint32_t rank = NW == 1 ? 0 : cluster_rank(), ranks = NW == 1 ? 1 : cluster_size();
-    const uint32_t item = NW == 1 ? blockIdx.x * ITEMS + sub : blockIdx.x / ranks;
-    if (item >= (uint32_t)a.n * a.hkv) return;
+    const uint32_t rank = cluster_rank(), ranks = cluster_size();
+    const uint32_t item = blockIdx.x / ranks;
     const int h = (int)(item / (uint32_t)a.n), t = (int)(item - (uint32_t)h * a.n);
     int* sel = a.selected + ((long long)t * a.hkv + h) * a.top_k;
-    const int slot = __ldg(a.slots + t), pos = __ldg(a.positions + t);
-    const bool bad_slot = slot < 0 || slot >= a.num_slots;
-    if (bad_slot || pos < 0 || pos >> a.shift >= a.cols) {
-        if (tid == 0) note_status(a.status, bad_slot ? MQ_ERR_BAD_SLOT : MQ_ERR_BAD_POSITION);
-        for (int i = tid; rank == 0 && i < a.top_k; i += NT) sel[i] = -1;
-        return;
-    }
-    const int own = pos >> a.shift, want = a.top_k - 1;
-    if (own <= want || want == 0) {   // every page, or only the token's own: nothing to choose
-        for (int i = tid; rank == 0 && i < a.top_k; i += NT) sel[i] = want == 0 ? own : i <= own ? i : -1;
-        return;
-    }
+    const int slot = __ldg(a.slots + t);
+    const int own = pages_to_score(a, slot, __ldg(a.positions + t), sel, rank == 0, tid, NT);
+    if (!own) return;   // all CTAs of the cluster alike
     // this CTA's share of the pages, looked up in one sweep; each place is overwritten by its page's key
     const int share = ranks == 1 ? own : (ceil_div(own, (int)ranks) + 15) & ~15;
     const int p0 = min(own, (int)rank * share), p1 = min(own, p0 + share);
     const int* row = a.table + slot * a.table_row;
-    for (int j = p0 + tid; j < p1; j += NT) {
-        int pid = __ldg(row + j);
-        if (pid < 0 || pid >= a.pages) {
-            note_status(a.status, MQ_ERR_BAD_PAGE);
-            pid = -1;
-        }
-        keys[j] = (uint32_t)pid;
-    }
-    // the group's queries in whole numbers, split by sign
-    for (int g = warp; g < heads; g += NW) {
-        float x[D / 32], m = 0.f;
-        if (g < a.grp) {
-            const uint16_t* q = a.q + t * a.q_tok + (h * a.grp + g) * a.q_head;
+    const uint16_t* q0 = a.q + t * a.q_tok + (long long)h * a.grp * a.q_head;
+    float x[D / 32];   // a warp's first head is on its way before the sweep
+    load_query<T, D>(x, warp < a.grp ? q0 + warp * a.q_head : nullptr, lane);
+    for (int j0 = p0; j0 < p1; j0 += 4 * NT) {
+        int pid[4];
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-                x[i] = Elem<T>::up(__ldg(q + lane + 32 * i));
-                m = fmaxf(m, fabsf(x[i]));
+        for (int i = 0; i < 4; ++i) pid[i] = j0 + i * NT + tid < p1 ? __ldg(row + j0 + i * NT + tid) : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = j0 + i * NT + tid;
+            if (j >= p1) break;
+            if (pid[i] < 0 || pid[i] >= a.pages) {
+                note_status(a.status, MQ_ERR_BAD_PAGE);
+                pid[i] = -1;
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) x[i] = 0.f;
+            keys[j] = (uint32_t)pid[i];
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        m = fminf(m, Elem<T>::MAX);
-        const int e = m > 0.f ? min(max(ilogbf(m) - 6, -60), 40) : 0;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            const float r = fminf(fmaxf(rintf(x[i] * two_to(-e)), -127.f), 127.f);
-            const int v = x[i] == x[i] ? (int)r : 0;
-            qpos[g * D + lane + 32 * i] = (signed char)max(v, 0);
-            qneg[g * D + lane + 32 * i] = (signed char)min(v, 0);
-        }
-        if (lane == 0) qunit[g] = two_to(e);
     }
-    sync();
-    // 16 pages a step: lane (g, t) reads channels 16 t .. of each 64-channel block of pages g and g + 8, whose
-    // words are the A operand of two MMAs; the k index is permuted alike in both operands
+    for (int g = warp; g < heads; g += NW) {
+        if (g != warp) load_query<T, D>(x, g < a.grp ? q0 + g * a.q_head : nullptr, lane);
+        const float unit = whole_query<T, D>(x, qpos + g * D, qneg + g * D, lane);
+        if (lane == 0) qunit[g] = unit;
+    }
+    if (ranks > 1) cluster_sync();   // (every CTA runs: its shared memory may be written)
+    else __syncthreads();
     const int g = lane >> 2, tq = lane & 3;
     const signed char* ix = a.index + h * a.i_head;
-    uint32_t kmin = 0xffffffffu, kmax = 0;
 #pragma unroll 1
     for (int j0 = p0 + warp * 16; j0 < p1; j0 += NW * 16 * SEL_UNROLL) {
-        int4 w[SEL_UNROLL][2][2 * D / 64];   // [step][page g, g + 8][HI blocks, LO blocks]
-        int ex[SEL_UNROLL][2];
-        bool ok[SEL_UNROLL][2];
+        PageStep<D> st[SEL_UNROLL];
+        int pid[SEL_UNROLL][2];
 #pragma unroll
-        for (int u = 0; u < SEL_UNROLL; ++u)
+        for (int u = 0; u < SEL_UNROLL; ++u) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const int j = j0 + u * NW * 16 + g + 8 * r;
-                const int pid = j < p1 ? (int)keys[j] : -1;
-                ok[u][r] = pid >= 0;
-                const signed char* rec = ix + (pid >= 0 ? pid : 0) * a.i_page;
-#pragma unroll
-                for (int b = 0; b < 2 * D / 64; ++b) w[u][r][b] = __ldg(reinterpret_cast<const int4*>(rec + 64 * b + 16 * tq));
-                ex[u][r] = __ldg(rec + 2 * D);
+                pid[u][r] = j < p1 ? (int)keys[j] : -1;
             }
+            st[u].load(ix, a.i_page, pid[u], tq);
+        }
         float best[SEL_UNROLL][2];
 #pragma unroll
         for (int u = 0; u < SEL_UNROLL; ++u) best[u][0] = best[u][1] = -INFINITY;
-        for (int h0 = 0; h0 < a.grp; h0 += 8) {
+        for (int h0 = 0; h0 < a.grp; h0 += 8) {   // columns: 8 heads
             int4 q[2 * D / 64];
 #pragma unroll
             for (int b = 0; b < 2 * D / 64; ++b)
@@ -198,14 +388,8 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 32) select_kernel(const S
             const bool in0 = h0 + 2 * tq < a.grp, in1 = h0 + 2 * tq + 1 < a.grp;
 #pragma unroll
             for (int u = 0; u < SEL_UNROLL; ++u) {
-                int c[4] = {0, 0, 0, 0};
-#pragma unroll
-                for (int b = 0; b < 2 * D / 64; ++b) {
-                    const int4 x = w[u][0][b], y = w[u][1][b];
-                    const int a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
-                    mma_s8(c, a0, q[b].x, q[b].y);
-                    mma_s8(c, a1, q[b].z, q[b].w);
-                }
+                int c[4];
+                st[u].dot(c, q);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     if (in0) best[u][r] = fmaxf(best[u][r], (float)c[2 * r] * u0);
@@ -222,122 +406,131 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 32) select_kernel(const S
                 s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, 1));
                 s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, 2));
                 const int j = j0 + u * NW * 16 + g + 8 * r;
-                if (j < p1) {
-                    // the record's exponent is within [-60, 40] when this library wrote it
-                    const uint32_t key = ok[u][r] ? order_key(s * two_to(min(max(ex[u][r], -60), 40))) : 0u;
-                    if (tq == 0) keys[j] = key;
-                    kmin = min(kmin, key);
-                    kmax = max(kmax, key);
+                if (j < p1 && tq == 0) {
+                    const uint32_t key = st[u].key(r, s, pid[u][r] >= 0);
+                    if (rank == 0) keys[j] = key;
+                    else st_peer(smem_u32(keys + j), 0, key);   // places that the first CTA uses for nothing else
                 }
             }
     }
-    if (NW > 1 && ranks > 1) {
-        cluster_sync();   // every share is scored
-        if (rank == 0) {
-            for (int j = share + tid; j < own; j += NT) {
-                const uint32_t key = ld_peer(smem_u32(keys + j), (uint32_t)(j / share));
-                keys[j] = key;
-                kmin = min(kmin, key);
-                kmax = max(kmax, key);
-            }
-        }
-        cluster_sync();   // and collected: the others' shared memory may go
+    if (ranks > 1) {
+        cluster_sync();   // every share is scored and in the first CTA
         if (rank) return;
-    }
-    kmin = __reduce_min_sync(0xffffffffu, kmin);
-    kmax = __reduce_max_sync(0xffffffffu, kmax);
-    if (NW > 1) {
-        if (lane == 0) {
-            sums[0][warp] = (int)kmin;
-            sums[1][warp] = (int)kmax;
-        }
-        __syncthreads();
-        kmin = __reduce_min_sync(0xffffffffu, (uint32_t)sums[0][lane % NW]);
-        kmax = __reduce_max_sync(0xffffffffu, (uint32_t)sums[1][lane % NW]);
     } else {
-        __syncwarp();
+        __syncthreads();
     }
+    choose<NW>(keys, own, a.top_k - 1, sel, {hist, list, pick, sums}, warp, lane);
+    if (tid == 0) sel[a.top_k - 1] = own;
+}
 
-    // keys agree above bit `bits`; of those that match `prefix` under `mask` the largest `need` are wanted
-    int bits = 32 - __clz((int)(kmin ^ kmax)), need = want;
-    uint32_t mask = bits == 32 ? 0u : 0xffffffffu << bits, prefix = kmax & mask;
-    while (bits > 0) {
-        const int shift = max(bits - 8, 0);
-        for (int i = tid; i < 256; i += NT) hist[sub][i] = 0;
-        sync();
-        for (int j = tid; j < own; j += NT) {
-            const uint32_t k = keys[j];
-            if ((k & mask) == prefix) atomicAdd(&hist[sub][(k & ~mask) >> shift], 1);
+template <typename T, int D>
+__global__ void __launch_bounds__(SEL_TOKENS * 32) select_eight_kernel(const SelArgs a) {
+    constexpr int N = SEL_TOKENS;
+    extern __shared__ __align__(16) uint8_t sel_smem[];
+    __shared__ int hist[N][256], list[N][32], owns[N], slot_of[N];
+    __shared__ uint32_t pick[N][4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    signed char* qpos = reinterpret_cast<signed char*>(sel_smem);          // [grp][N][D]
+    signed char* qneg = qpos + a.grp * N * D;
+    float* qunit = reinterpret_cast<float*>(qneg + a.grp * N * D);         // [grp][N]
+    uint32_t* keys = reinterpret_cast<uint32_t*>(qunit + a.grp * N);       // [N][cols]
+    pdl_wait();
+    pdl_trigger();
+    const int blocks = ceil_div(a.n, N), h = blockIdx.x / blocks, t = (blockIdx.x - h * blocks) * N + warp;
+    // a warp to a token: what it has to choose from, its queries
+    int own = 0, slot = -1;
+    int* sel = a.selected + ((long long)t * a.hkv + h) * a.top_k;
+    if (t < a.n) {
+        slot = __ldg(a.slots + t);
+        own = pages_to_score(a, slot, __ldg(a.positions + t), sel, true, lane, 32);
+    }
+    if (lane == 0) {
+        owns[warp] = own;
+        slot_of[warp] = slot;
+    }
+    for (int g = 0; g < a.grp; ++g) {
+        float x[D / 32];
+        load_query<T, D>(x, own ? a.q + t * a.q_tok + (h * a.grp + g) * a.q_head : nullptr, lane);
+        const float unit = whole_query<T, D>(x, qpos + (g * N + warp) * D, qneg + (g * N + warp) * D, lane);
+        if (lane == 0) qunit[g * N + warp] = unit;
+    }
+    __syncthreads();
+    const int g = lane >> 2, tq = lane & 3;
+    const signed char* ix = a.index + h * a.i_head;
+    const int own0 = owns[2 * tq], own1 = owns[2 * tq + 1];
+    // sequence by sequence: usually all eight stand in one
+    for (int lead = 0; lead < N; ++lead) {
+        if (!owns[lead]) continue;
+        const int seq = slot_of[lead];
+        int top = 0;
+        bool first = true;
+        for (int i = 0; i < N; ++i) {
+            if (!owns[i] || slot_of[i] != seq) continue;
+            if (i < lead) first = false;
+            top = max(top, owns[i]);
         }
-        sync();
-        if (warp == 0) {
-            // lane i holds bins 255 - 8 i .. 248 - 8 i; the bin in which the count passes `need`
-            int c[8], sum = 0;
+        if (!first) continue;
+        const int lim0 = slot_of[2 * tq] == seq ? own0 : 0, lim1 = slot_of[2 * tq + 1] == seq ? own1 : 0;
+        const int* row = a.table + seq * a.table_row;
+        int next[SEL_UNROLL][2];
+        auto look = [&](int j0) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                c[i] = hist[sub][255 - 8 * lane - i];
-                sum += c[i];
-            }
-            int x = sum;
+            for (int u = 0; u < SEL_UNROLL; ++u)
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
-            }
-            int above = x - sum;
-            if (above < need && need <= x) {
+                for (int r = 0; r < 2; ++r) {
+                    const int j = j0 + u * N * 16 + g + 8 * r;
+                    next[u][r] = j < top ? __ldg(row + j) : -1;
+                }
+        };
+        look(warp * 16);
+#pragma unroll 1
+        for (int j0 = warp * 16; j0 < top; j0 += N * 16 * SEL_UNROLL) {
+            PageStep<D> st[SEL_UNROLL];
+            int pid[SEL_UNROLL][2];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (above < need && need <= above + c[i]) {
-                        s_pick[sub][0] = prefix | (uint32_t)(255 - 8 * lane - i) << shift;
-                        // what is wanted of the bin, and whether that is all of it
-                        s_pick[sub][1] = (uint32_t)(need - above) << 1 | (need - above == c[i] ? 1u : 0u);
-                        above = need;   // found
-                    } else {
-                        above += c[i];
+            for (int u = 0; u < SEL_UNROLL; ++u) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    pid[u][r] = next[u][r];
+                    if (j0 + u * N * 16 + g + 8 * r < top && (pid[u][r] < 0 || pid[u][r] >= a.pages)) {
+                        note_status(a.status, MQ_ERR_BAD_PAGE);
+                        pid[u][r] = -1;
                     }
                 }
+                st[u].load(ix, a.i_page, pid[u], tq);
             }
+            look(j0 + N * 16 * SEL_UNROLL);
+            float best[SEL_UNROLL][4];   // page g: tokens 2 t, 2 t + 1; page g + 8
+#pragma unroll
+            for (int u = 0; u < SEL_UNROLL; ++u) best[u][0] = best[u][1] = best[u][2] = best[u][3] = -INFINITY;
+            for (int hd = 0; hd < a.grp; ++hd) {   // columns: one head of the 8 tokens
+                int4 q[2 * D / 64];
+#pragma unroll
+                for (int b = 0; b < 2 * D / 64; ++b)
+                    q[b] = *reinterpret_cast<const int4*>((b < D / 64 ? qpos : qneg) + (hd * N + g) * D + (b % (D / 64)) * 64 + 16 * tq);
+                const float u0 = qunit[hd * N + 2 * tq], u1 = qunit[hd * N + 2 * tq + 1];
+#pragma unroll
+                for (int u = 0; u < SEL_UNROLL; ++u) {
+                    int c[4];
+                    st[u].dot(c, q);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) best[u][i] = fmaxf(best[u][i], (float)c[i] * (i & 1 ? u1 : u0));
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < SEL_UNROLL; ++u)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int j = j0 + u * N * 16 + g + 8 * r;
+                    if (j < lim0) keys[(long long)(2 * tq) * a.cols + j] = st[u].key(r, best[u][2 * r], pid[u][r] >= 0);
+                    if (j < lim1) keys[(long long)(2 * tq + 1) * a.cols + j] = st[u].key(r, best[u][2 * r + 1], pid[u][r] >= 0);
+                }
         }
-        sync();
-        prefix = s_pick[sub][0];
-        need = (int)(s_pick[sub][1] >> 1);
-        mask = 0xffffffffu << shift;
-        bits = s_pick[sub][1] & 1u ? 0 : shift;
-        sync();
     }
-    // keys above the bin, and the first `need` in it, in ascending order of the page
-    const int seg = (ceil_div(own, NW) + 31) & ~31;
-    const int lo = min(own, warp * seg), hi = min(own, lo + seg);
-    int gt = 0, eq = 0;
-    if (NW > 1) {
-        for (int i = lo; i < hi; i += 32) {
-            const uint32_t k = i + lane < hi ? keys[i + lane] & mask : 0u;
-            gt += __popc(__ballot_sync(0xffffffffu, i + lane < hi && k > prefix));
-            eq += __popc(__ballot_sync(0xffffffffu, i + lane < hi && k == prefix));
-        }
-        if (lane == 0) {
-            sums[0][warp] = gt;
-            sums[1][warp] = eq;
-        }
-        __syncthreads();
-        gt = eq = 0;
-        for (int w = 0; w < warp; ++w) {
-            gt += sums[0][w];
-            eq += sums[1][w];
-        }
-    }
-    const unsigned below = (1u << lane) - 1u;
-    for (int i = lo; i < hi; i += 32) {
-        const uint32_t k = i + lane < hi ? keys[i + lane] & mask : 0u;
-        const bool is_gt = i + lane < hi && k > prefix, is_eq = i + lane < hi && k == prefix;
-        const unsigned mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
-        const int eq_at = eq + __popc(me & below);
-        if (is_gt || (is_eq && eq_at < need)) sel[gt + __popc(mg & below) + min(eq_at, need)] = i + lane;
-        gt += __popc(mg);
-        eq += __popc(me);
-    }
-    if (tid == 0) sel[want] = own;
+    __syncthreads();
+    if (!own) return;
+    choose<1>(keys + (long long)warp * a.cols, own, a.top_k - 1, sel, {hist[warp], list[warp], pick[warp], nullptr}, 0, lane);
+    if (lane == 0) sel[a.top_k - 1] = own;
 }
 
 // ---- host ----------------------------------------------------------------------------------
@@ -454,16 +647,17 @@ int run_rows(const RowArgs& a, const mq_paged_pool& pool, cudaStream_t st) {
     e = launch(kernel, dim3(grid), dim3(ROW_THREADS), smem, st, tk, tv, a);
     const long long rows = (long long)a.total_q * a.hq;
     if (e == cudaSuccess) {
-        // the fewer rows, the more parts each has: eight warps to a row while those are two CTAs per SM,
-        // four up to eight rows per SM (1024 rows of 34 parts: 10.9 us against 14.6 with one; 2048 rows of 20:
-        // 15.6 against 11)
+        // As many warps to a row as leave all CTAs resident at once (three to an SM): a second wave costs more
+        // than the warps save (1024 rows of 34 parts, 512 CTAs: 14 us).
         auto join = [&](auto split) {
             constexpr int S = decltype(split)::value;
             return launch(join_kernel<T, D, MODE, S>, dim3((unsigned)((rows * S + 7) / 8)), dim3(256), 0, st, a, (uint32_t)grid * ROW_WARPS);
         };
-        e = rows <= 2 * sm_count()    ? join(std::integral_constant<int, 8>{})
-            : rows <= 8 * sm_count() ? join(std::integral_constant<int, 4>{})
-                                      : join(std::integral_constant<int, 1>{});
+        const long long room = 3ll * sm_count() * 8 / rows;   // warps to a row
+        e = room >= 8   ? join(std::integral_constant<int, 8>{})
+            : room >= 4 ? join(std::integral_constant<int, 4>{})
+            : room >= 2 ? join(std::integral_constant<int, 2>{})
+                        : join(std::integral_constant<int, 1>{});
     }
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "paged attention");
 }
@@ -481,21 +675,28 @@ bool q_ok(const void* q, long long tok, long long head) {
     return q && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && tok % 8 == 0 && head % 8 == 0;
 }
 
-template <typename T, int D, int NW>
-int launch_select(const SelArgs& s, cudaStream_t st) {
-    constexpr int ITEMS = NW == 1 ? 8 : 1;
-    const size_t smem = ITEMS * sel_item_bytes<D>(s.cols, s.grp);
+template <typename T, int D>
+int run_select(const SelArgs& s, cudaStream_t st) {
     const long long items = (long long)s.n * s.hkv;
-    auto kernel = select_kernel<T, D, NW>;
+    // eight tokens to a CTA once that gives every SM a CTA of them and their keys fit (96 KB)
+    if (items >= (long long)SEL_TOKENS * sm_count() && s.n >= SEL_TOKENS && sel_eight_bytes<D>(s.cols, s.grp) <= 98304) {
+        static SmemLimit limit;
+        const size_t smem = sel_eight_bytes<D>(s.cols, s.grp);
+        cudaError_t e = allow_smem(select_eight_kernel<T, D>, smem, limit);
+        if (e == cudaSuccess)
+            e = launch(select_eight_kernel<T, D>, dim3((unsigned)ceil_div(s.n, SEL_TOKENS) * s.hkv), dim3(SEL_TOKENS * 32), smem, st, s);
+        return e == cudaSuccess ? MQ_OK : note_cuda(e, "page selection");
+    }
     static SmemLimit limit;
-    cudaError_t e = allow_smem(kernel, smem, limit);
+    const size_t smem = sel_one_bytes<D>(s.cols, s.grp);
+    cudaError_t e = allow_smem(select_one_kernel<T, D>, smem, limit);
     if (e != cudaSuccess) return note_cuda(e, "page selection attribute");
     // a cluster to an item: doubled while all its CTAs have an SM each and a CTA keeps 256 pages or more
     unsigned ranks = 1;
-    while (NW > 1 && ranks < 8 && items * ranks * 2 <= sm_count() && s.cols >= 512 * (int)ranks) ranks *= 2;
+    while (ranks < 8 && items * ranks * 2 <= sm_count() && s.cols >= 512 * (int)ranks) ranks *= 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((items + ITEMS - 1) / ITEMS) * ranks);
-    cfg.blockDim = dim3(NW == 1 ? 256 : NW * 32);
+    cfg.gridDim = dim3((unsigned)items * ranks);
+    cfg.blockDim = dim3(SEL_WARPS * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -506,17 +707,9 @@ int launch_select(const SelArgs& s, cudaStream_t st) {
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = NW > 1 ? 2 : 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, s);
+    cfg.numAttrs = 2;
+    e = cudaLaunchKernelEx(&cfg, select_one_kernel<T, D>, s);
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "page selection");
-}
-
-template <typename T, int D>
-int run_select(const SelArgs& s, cudaStream_t st) {
-    // a warp to an item once eight of them fill every SM and eight items' keys fit (64 KB)
-    if ((long long)s.n * s.hkv >= 8ll * sm_count() && 8 * sel_item_bytes<D>(s.cols, s.grp) <= 65536)
-        return launch_select<T, D, 1>(s, st);
-    return launch_select<T, D, 16>(s, st);
 }
 
 }  // namespace paged

@@ -730,6 +730,30 @@ def test_sparse(paged, dtype, d, page, hkv, grp, top_k):
     check_sparse(paged, p, hkv * grp, idx, [p.slots[4]] * 7, pos, [4] * 7, top_k)
 
 
+@pytest.mark.parametrize("dtype,d,grp", [(torch.bfloat16, 64, 2), (torch.float16, 128, 1), (torch.bfloat16, 64, 9)])
+def test_sparse_many_tokens(paged, dtype, d, grp):
+    """Enough tokens for eight to a CTA: runs of one sequence, sequences taking turns, a count that is no multiple of
+    eight, tokens with nothing to choose among them."""
+    page, hkv, top_k = 16, 8, 4
+    lens = [900, 300, 40]
+    p = Pool(lens, page, hkv, d, dtype, seed=grp)
+    idx = full_index(p, 2, hkv, d)
+    seqs = [0] * 90 + [i % 3 for i in range(40)] + [1] * 25
+    pos = [(i * 131) % lens[s] for i, s in enumerate(seqs)]
+    check_sparse(paged, p, hkv * grp, idx, [p.slots[s] for s in seqs], pos, seqs, top_k)
+
+
+def test_sparse_long_table(paged):
+    """More pages than one CTA scores: a cluster per item, and keys all in one bin (pages in few kinds)."""
+    page, d = 16, 64
+    p = Pool([16 * 3000 - 5], page, 1, d, torch.bfloat16, seed=7)
+    idx = full_index(p, 2, 1, d)
+    check_sparse(paged, p, 2, idx, p.slots, [16 * 3000 - 6], [0], 40)
+    p.k[:] = p.k[:7].repeat(p.k.shape[0] // 7 + 1, 1, 1, 1, 1)[:p.k.shape[0]]
+    idx = full_index(p, 2, 1, d)
+    check_sparse(paged, p, 2, idx, p.slots, [16 * 3000 - 6], [0], 500)
+
+
 def test_sparse_ties(paged):
     """Equal scores: the lowest pages win; zero queries make every score equal."""
     page, d = 16, 64

@@ -1,0 +1,170 @@
+"""Qwen3 decoding on the paged KV cache: prompts shared between samples.
+
+:class:`PagedDecoder` runs the model of this package with its projections as
+plain matrix products and everything around the cache on the operators of
+:mod:`megaqwen_b200.paged`: rotary positions and the write of K and V in one
+pass, pages reserved, forked and freed on the device, attention that reads a
+shared prompt once for all its samples, or a chosen part of a long context.
+The batched decoder of the native library (``MegakernelBatchDecoder``) is the
+faster one for sequences that share nothing.
+
+The reference decodes one sequence from one contiguous cache; there is no
+counterpart.  Numerics follow it: activations, residual stream, norms and
+softmax in fp32, K/V and RoPE tables in bf16; q is rounded to bf16 too, the
+cache operators' type.
+"""
+from __future__ import annotations
+
+from typing import List, Optional, Sequence, Tuple
+
+import torch
+import torch.nn.functional as F
+
+from .paged import PagedKVCache
+from .weights import (HEAD_DIM, NUM_KV_HEADS, NUM_Q_HEADS, Q_SIZE, KV_SIZE, RMS_NORM_EPS, Qwen3Weights, rope_tables)
+
+
+def _rms_norm(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
+    x = x.float()
+    return x * torch.rsqrt((x * x).mean(-1, keepdim=True) + RMS_NORM_EPS) * w
+
+
+def _product(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
+    """fp32 activations by bf16 weights ``[out, in]``, fp32 result: the activations as two bf16 pieces, side by side in
+    one product, so that the weights are read once and the activations are not rounded."""
+    x = x.float()
+    hi = x.to(w.dtype)
+    y = torch.mm(torch.cat([hi, (x - hi.float()).to(w.dtype)]), w.T, out_dtype=torch.float32)
+    return y[:x.shape[0]] + y[x.shape[0]:]
+
+
+class PagedDecoder:
+    """``max_seqs`` sequences on a pool of ``num_pages`` pages.
+
+    ``sparse_pages``: decode steps read at most this many pages per query and
+    kv head (chosen by score); ``None`` reads everything.
+    """
+
+    def __init__(self, weights: Qwen3Weights, num_pages: int, max_seqs: int, max_seq_len: int = 4096, page_size: int = 64,
+                 sparse_pages: Optional[int] = None):
+        dev = weights.embed.device
+        self.embed, self.final_norm, self.sparse_pages = weights.embed, weights.final_norm.float(), sparse_pages
+        self.layers = []
+        for layer in weights.layers:
+            self.layers.append({
+                "qkv": torch.cat([layer["q_proj"], layer["k_proj"], layer["v_proj"]]),
+                "gate_up": torch.cat([layer["gate_proj"], layer["up_proj"]]),
+                **{k: layer[k] for k in ("o_proj", "down_proj")},
+                **{k: layer[k].float() for k in ("input_layernorm", "post_attention_layernorm", "q_norm", "k_norm")},
+            })
+        cos, sin = rope_tables(max_seq_len, device=dev)   # the reference's bf16 values, one half of the duplicated columns
+        self.cos, self.sin = (x[:, :HEAD_DIM // 2].float().contiguous() for x in (cos, sin))
+        self.cache = PagedKVCache(num_pages, max_seqs, -(-max_seq_len // page_size), num_layers=len(self.layers),
+                                  page_size=page_size, device=dev, index=sparse_pages is not None)
+        self.max_seq_len = max_seq_len
+        self.lengths = [0] * max_seqs
+        self._family: List[Optional[Tuple[int, int]]] = [None] * max_seqs   # (family, pages it shares)
+        self._families = 0
+        self._plan = None
+
+    def _ints(self, x) -> torch.Tensor:
+        return torch.tensor(x, dtype=torch.int32, device=self.embed.device)
+
+    def _forward(self, ids, slots, positions, attend) -> torch.Tensor:
+        """Hidden states of the tokens after the final norm; ``attend(layer, q)`` reads the cache."""
+        h = self.embed[ids].float()
+        n = h.shape[0]
+        for li, w in enumerate(self.layers):
+            x = _rms_norm(h, w["input_layernorm"])
+            q, k, v = _product(x, w["qkv"]).split([Q_SIZE, KV_SIZE, KV_SIZE], -1)
+            q = _rms_norm(q.view(n, NUM_Q_HEADS, HEAD_DIM), w["q_norm"]).to(self.embed.dtype)
+            k = _rms_norm(k.view(n, NUM_KV_HEADS, HEAD_DIM), w["k_norm"]).to(self.embed.dtype)
+            v = v.view(n, NUM_KV_HEADS, HEAD_DIM).to(self.embed.dtype)
+            q = self.cache.append(li, q, k, v, slots, positions, self.cos, self.sin)
+            h = h + _product(attend(li, q).view(n, Q_SIZE), w["o_proj"])
+            x = _rms_norm(h, w["post_attention_layernorm"])
+            gate, up = _product(x, w["gate_up"]).chunk(2, -1)
+            h = h + _product(F.silu(gate) * up, w["down_proj"])
+        return _rms_norm(h, self.final_norm)
+
+    def _logits(self, h: torch.Tensor) -> torch.Tensor:
+        return _product(h, self.embed)
+
+    @torch.no_grad()
+    def prefill(self, slot: int, ids: Sequence[int]) -> torch.Tensor:
+        """Appends a prompt (or a further piece of one) to a sequence; fp32 logits of its last token."""
+        n, start = len(ids), self.lengths[slot]
+        if n < 1 or start + n > self.max_seq_len:
+            raise ValueError("prompt is empty or exceeds max_seq_len")
+        self.cache.reserve([slot], [start + n])
+        self.lengths[slot] = start + n
+        one = self._ints([slot])
+        starts = self._ints([0, n])
+        h = self._forward(torch.as_tensor(ids, device=self.embed.device).long(), one.expand(n).contiguous(),
+                          torch.arange(start, start + n, dtype=torch.int32, device=self.embed.device),
+                          lambda li, q: self.cache.attend(li, q, one, q_starts=starts))
+        return self._logits(h[-1:])[0]
+
+    def fork(self, parent: int, children: Sequence[int]) -> None:
+        """Empty slots become copies of a sequence; decode steps read what they share once for all of them."""
+        self.cache.fork([parent] * len(children), list(children))
+        shared = (self._families, self.lengths[parent] // self.cache.page_size)
+        self._families += 1
+        for s in [parent, *children]:
+            self.lengths[s] = self.lengths[parent]
+            self._family[s] = shared
+        self._plan = None
+
+    def free(self, slots: Sequence[int]) -> None:
+        self.cache.free(list(slots))
+        for s in slots:
+            self.lengths[s], self._family[s] = 0, None
+        self._plan = None
+
+    def _groups(self, slots):
+        """Order of the batch that puts families side by side, and their starts and pages; kept while the batch stays."""
+        key = tuple(slots)
+        if self._plan is None or self._plan[0] != key:
+            order = sorted(range(len(slots)), key=lambda i: (self._family[slots[i]] is None, self._family[slots[i]] or (0, 0)))
+            starts, pages = [], []
+            last = object()
+            for at, i in enumerate(order):
+                f = self._family[slots[i]]
+                if f is None:
+                    break
+                if f != last:
+                    starts.append(at)
+                    pages.append(f[1])
+                    last = f
+            else:
+                at = len(order)
+            groups = (self._ints(starts + [at]), self._ints(pages)) if starts else (None, None)
+            back = torch.tensor(order, device=self.embed.device)
+            self._plan = (key, order, back, self._ints([slots[i] for i in order]), *groups)
+        return self._plan[1:]
+
+    @torch.no_grad()
+    def step(self, slots: Sequence[int], tokens: torch.Tensor) -> torch.Tensor:
+        """One token for each of the named sequences: fp32 logits ``[len(slots), vocab]``.  No host synchronisation."""
+        slots = list(slots)
+        if len(set(slots)) != len(slots) or any(self.lengths[s] >= self.max_seq_len for s in slots):
+            raise ValueError("a sequence is named twice or full")
+        order, back, dev_slots, starts, pages = self._groups(slots)
+        positions = self._ints([self.lengths[slots[i]] for i in order])
+        self.cache.reserve(dev_slots, positions + 1)
+        for s in slots:
+            self.lengths[s] += 1
+        if self.sparse_pages is None:
+            def attend(li, q):
+                return self.cache.attend(li, q, dev_slots, group_starts=starts, prefix_pages=pages)
+        else:
+            def attend(li, q):
+                return self.cache.sparse_attend(li, q, dev_slots, positions, self.sparse_pages)[0]
+        h = self._forward(tokens.to(self.embed.device).long()[back], dev_slots, positions, attend)
+        out = torch.empty_like(h)
+        out[back] = h
+        return self._logits(out)
+
+    def check(self) -> None:
+        """Raises if a device-side check of the cache failed (synchronises)."""
+        self.cache.check()

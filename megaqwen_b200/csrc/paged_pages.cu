@@ -143,6 +143,10 @@ __device__ bool slots_ok(const int* slots, int n, int num_slots, unsigned* bits)
     return !__syncthreads_or(bad);
 }
 
+// Short lists of a plan stay in shared memory: a search through them in global
+// memory was half of a reservation's time.
+constexpr int NEAR_OFF = 1024, NEAR_IDS = 2048;
+
 // ---- free ----------------------------------------------------------------------------
 // One CTA per sequence.  Each checks the whole list itself (it is short, and a
 // second launch would cost more), so a wrong list changes nothing anywhere.
@@ -177,13 +181,14 @@ __global__ void __launch_bounds__(256) free_kernel(Tab t, const int* __restrict_
 __global__ void __launch_bounds__(PLAN_THREADS) reserve_kernel(Tab t, const int* __restrict__ slots,
                                                                const int* __restrict__ new_lengths, int n, Plan pl) {
     __shared__ unsigned bits[MAX_SLOTS / 32];
-    __shared__ int sm[PLAN_WARPS];
+    __shared__ int sm[PLAN_WARPS], near_off[NEAR_OFF], near_ids[NEAR_IDS];
     pdl_wait();
     pdl_trigger();
     if (!slots_ok(slots, n, t.slots, bits)) {
         if (threadIdx.x == 0) note_status(t.status, MQ_ERR_BAD_SLOT);
         return;
     }
+    int* off = n <= NEAR_OFF ? near_off : pl.off;
     int need = 0;
     bool bad = false;
     for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
@@ -197,7 +202,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) reserve_kernel(Tab t, const int*
         }
         int sum;
         const int at = block_scan(k, sm, &sum);
-        if (i < n) pl.off[i] = need + at;
+        if (i < n) off[i] = need + at;
         need = min(need + sum, t.pages + 1);
         if (need > t.pages) break;
     }
@@ -205,7 +210,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) reserve_kernel(Tab t, const int*
         if (threadIdx.x == 0) note_status(t.status, MQ_ERR_BAD_POSITION);
         return;
     }
-    if (need > 0 && (need > t.pages || find_pages(t.refs, t.pages, false, pl.ids, need, nullptr, sm) < need)) {
+    int* ids = need <= NEAR_IDS ? near_ids : pl.ids;
+    if (need > 0 && (need > t.pages || find_pages(t.refs, t.pages, false, ids, need, nullptr, sm) < need)) {
         if (threadIdx.x == 0) note_status(t.status, MQ_ERR_NO_PAGES);
         return;
     }
@@ -214,11 +220,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) reserve_kernel(Tab t, const int*
         int lo = 0, hi = n;   // the last sequence whose pages start at or before r
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (pl.off[mid] <= r) lo = mid;
+            if (off[mid] <= r) lo = mid;
             else hi = mid;
         }
-        const int s = slots[lo], p = pl.ids[r];
-        t.table[s * t.row + pages_of(t.lengths[s], t.page) + r - pl.off[lo]] = p;
+        const int s = slots[lo], p = ids[r];
+        t.table[s * t.row + pages_of(t.lengths[s], t.page) + r - off[lo]] = p;
         t.refs[p] = 1;
     }
     __syncthreads();   // the old lengths are read above
@@ -289,10 +295,11 @@ __device__ void move_units(const Geo& g, const Plan& pl, int moves, long long wi
 __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(Tab t, const int* __restrict__ parents,
                                                                  const int* __restrict__ children, int n, Plan pl) {
     __shared__ unsigned bits[MAX_SLOTS / 32];
-    __shared__ int sm[PLAN_WARPS];
+    __shared__ int sm[PLAN_WARPS], near_off[NEAR_OFF], near_ids[NEAR_IDS];
     pdl_wait();
     pdl_trigger();
     if (threadIdx.x == 0) pl.head[1] = 0;
+    int* off = n <= NEAR_OFF ? near_off : pl.off;
     bool bad = !slots_ok(children, n, t.slots, bits);
     if (!bad) {   // the same for every thread
         for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
@@ -326,7 +333,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(Tab t, const in
         if (i < n) {
             pl.src[i] = src;
             pl.rows[i] = part;
-            pl.off[i] = copies + at;
+            off[i] = part > 0 ? copies + at : -1;
         }
         copies += sum;
     }
@@ -335,11 +342,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(Tab t, const in
         if (threadIdx.x == 0) note_status(t.status, any1 ? MQ_ERR_BAD_POSITION : MQ_ERR_BAD_PAGE);
         return;
     }
-    if (copies > 0 && find_pages(t.refs, t.pages, false, pl.ids, copies, nullptr, sm) < copies) {
+    int* ids = copies <= NEAR_IDS ? near_ids : pl.ids;
+    if (copies > 0 && find_pages(t.refs, t.pages, false, ids, copies, nullptr, sm) < copies) {
         if (threadIdx.x == 0) note_status(t.status, MQ_ERR_NO_PAGES);
         return;
     }
-    for (int i = threadIdx.x; i < n; i += PLAN_THREADS) pl.dst[i] = pl.rows[i] > 0 ? pl.ids[pl.off[i]] : -1;
+    for (int i = threadIdx.x; i < n; i += PLAN_THREADS) pl.dst[i] = off[i] >= 0 ? ids[off[i]] : -1;
     if (threadIdx.x == 0) pl.head[1] = 1;
 }
 

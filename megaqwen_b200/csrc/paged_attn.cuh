@@ -18,6 +18,12 @@
 // one.  A run that ends inside an item leaves a part in the workspace; the join
 // kernel adds the parts in the order of the positions, so results do not
 // depend on timing.
+//
+// Measured: 16 sequences of 64k, 2048 chosen positions each, 134 MB: 26 us (5.1
+// TB/s, 0.79 of the copy rate); 500 tokens x 8 kv heads x 1024 positions, 2.1 GB
+// of which 134 MB are distinct: 170 us (12.3 TB/s, from L2); own parts of 64
+// sequences behind a prefix, 67 MB in 512 items: 17 us (3.9 TB/s: items of 16
+// groups on average, one or two to a warp).
 #pragma once
 
 #include "mq_tc.cuh"
@@ -846,6 +852,9 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
 }
 
 // ---- the join ----------------------------------------------------------------------------
+// acc = sum of the parts' acc_i 2^(m_i - M) over sum l_i 2^(m_i - M).  Bound by the
+// latency of three dependent reads (what a token has, the parts' m and l, their acc):
+// 1024 rows of 34 parts, 18 MB: 9 us; 2048 rows of 20: 9 us.
 // SPLIT warps share a row (the fewer rows, the more parts each), 8 / SPLIT rows to a CTA.
 template <typename T, int D, int MODE, int SPLIT>
 __global__ void __launch_bounds__(256, 3) join_kernel(const RowArgs a, uint32_t row_warps) {

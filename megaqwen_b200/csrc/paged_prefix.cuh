@@ -14,16 +14,21 @@
 //     the odd ones, and leave two parts.
 // While one stream's softmax runs, the tensor core works for the other:
 //   PV_A(j), S_A(j+1) | PV_B(j), S_B(j+1) | ...
-// P overwrites S in place as two 16-bit pieces (value and remainder, 64 columns
-// each), so the weights keep 16 bits and more; that makes 24 MMAs of 128 x 128
-// x 16 per tile and stream (1536 cycles) against 16384 exponentials (1024
-// cycles of the special-function units): the tensor core bounds the tile when
-// there are many rows, HBM when there are few.
+// P overwrites S in place as two 16-bit pieces (value and remainder, side by
+// side per 32 keys), so the weights keep 16 bits and more; that makes 24 MMAs of
+// 128 x 128 x 16 per tile and stream, 1536 cycles, against 16384 exponentials,
+// 1024 cycles of the special-function units.
+//
+// Bound: the chain softmax (2400 cycles) -> PV, S (1900 with commits) -> hand-over
+// of a stream; the two streams overlap and a pair of tiles takes 5100 cycles.  32k
+// keys x 256 rows x 8 kv heads: 57 us, 34 GFLOP without the remainders' MMAs (0.36
+// of the measured bf16 rate; 51 GFLOP with them).  Few rows (8k x 128 x 8): 18 us
+// for 34 MB, mostly a run's start and end (schedule 3.4 us, q and first tiles 5 us,
+// parts 2.3 us).
 //
 // Warps: 0 K producer, 1 MMA (and TMEM owner), 2 V producer, 3-10 softmax of A,
 // 11-18 softmax of B (two threads to a row, 64 keys each; they also load Q and
-// store the parts).  With one thread to a row the softmax took 2650 cycles of a
-// tile and its latency, not the tensor core, set the pace (4940 cycles).  K and
+// store the parts; with one thread to a row 8k x 64 took 52 us and not 50).  K and
 // V come page by page through a rank-5 tensor map, so the pool's strides are
 // free; V is taken as it lies ([key][dim], the MMA's MN-major B operand).
 // Every wait is bounded and ends in the status word.

@@ -3,7 +3,9 @@
 //
 // Memory-bound: each token's q, k and v are read once and written once,
 // (Hq + 2 Hkv) D elements each way; the cos/sin row of a token is shared by its
-// heads and comes from L1.
+// heads and comes from L1.  32008 tokens of 16 + 8 + 8 heads x 128, 528 MB: 92 us,
+// 5.7 TB/s, 0.88 of the copy rate (with the index 114 us: its 65 MB of keys are
+// read again).
 #include <algorithm>
 
 #include "paged_common.cuh"

@@ -459,6 +459,9 @@ int mq_rope(const mq_rope_params* params, cudaStream_t stream);
  * q_starts[b] .. q_starts[b+1] - 1 of q (one each when q_starts is NULL): the
  * last positions of slot slots[b], whose keys are written already; each sees
  * the positions up to its own.  Rows that see nothing are zero.
+ * An infinity or NaN among the values that a row sees leaves its results in
+ * that channel not finite (infinity or NaN: the weights meet it in two
+ * pieces); among those that it does not see it changes nothing.
  * Sequences group_starts[g] .. group_starts[g+1] - 1 share their first
  * prefix_pages[g] pages (the same page numbers in their rows, as a fork leaves
  * them): those are read once for the group.  num_groups 0: nothing is shared. */

@@ -5,6 +5,7 @@
 #include <type_traits>
 
 #include "paged_attn.cuh"
+#include "paged_by_page.cuh"
 #include "paged_prefix.cuh"
 
 namespace mq {
@@ -27,11 +28,11 @@ namespace paged {
 // 8 CTAs to an item, each scoring a share of the pages; for few items, whose reads
 // have to be spread.  select_eight_kernel: eight tokens of one kv head to a CTA,
 // each page's record read once for all of them that stand in the same sequence;
-// for many items (500 tokens x 8 heads, 250 pages each: 54 us with a warp to an
-// item of its own, 121 us with a CTA).
+// for many items (500 tokens x 8 heads, 250 pages each: 29 us; 54 with a warp to
+// an item of its own, 121 with a CTA).
 constexpr int MAX_SPARSE_COLS = 49152;
 constexpr int MAX_SPARSE_GROUP = 64;   // q heads per kv head
-constexpr int SEL_UNROLL = 2;          // 16-page steps in flight
+constexpr int SEL_UNROLL = 2;          // of select_one_kernel: 16-page steps in flight
 constexpr int SEL_WARPS = 16;          // of select_one_kernel
 constexpr int SEL_TOKENS = 8;          // of select_eight_kernel, a warp each
 
@@ -47,6 +48,8 @@ struct SelArgs {
     int* selected;
     int n, num_slots, cols, pages, shift, hkv, grp, top_k;
     int* status;
+    uint32_t* count;   // page by page: how many tokens chose (kv head, page), and each token's rank there
+    int* rank;
 };
 
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -424,8 +427,9 @@ __global__ void __launch_bounds__(SEL_WARPS * 32) select_one_kernel(const SelArg
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(SEL_TOKENS * 32) select_eight_kernel(const SelArgs a) {
-    constexpr int N = SEL_TOKENS;
+__global__ void __launch_bounds__(SEL_TOKENS * 32, 3) select_eight_kernel(const SelArgs a) {
+    // one 16-page step in flight, three CTAs to an SM: 29 us for 500 tokens; two steps, two CTAs: 32
+    constexpr int N = SEL_TOKENS, UNROLL = 1;
     extern __shared__ __align__(16) uint8_t sel_smem[];
     __shared__ int hist[N][256], list[N][32], owns[N], slot_of[N];
     __shared__ uint32_t pick[N][4];
@@ -472,10 +476,10 @@ __global__ void __launch_bounds__(SEL_TOKENS * 32) select_eight_kernel(const Sel
         if (!first) continue;
         const int lim0 = slot_of[2 * tq] == seq ? own0 : 0, lim1 = slot_of[2 * tq + 1] == seq ? own1 : 0;
         const int* row = a.table + seq * a.table_row;
-        int next[SEL_UNROLL][2];
+        int next[UNROLL][2];
         auto look = [&](int j0) {
 #pragma unroll
-            for (int u = 0; u < SEL_UNROLL; ++u)
+            for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     const int j = j0 + u * N * 16 + g + 8 * r;
@@ -484,11 +488,11 @@ __global__ void __launch_bounds__(SEL_TOKENS * 32) select_eight_kernel(const Sel
         };
         look(warp * 16);
 #pragma unroll 1
-        for (int j0 = warp * 16; j0 < top; j0 += N * 16 * SEL_UNROLL) {
-            PageStep<D> st[SEL_UNROLL];
-            int pid[SEL_UNROLL][2];
+        for (int j0 = warp * 16; j0 < top; j0 += N * 16 * UNROLL) {
+            PageStep<D> st[UNROLL];
+            int pid[UNROLL][2];
 #pragma unroll
-            for (int u = 0; u < SEL_UNROLL; ++u) {
+            for (int u = 0; u < UNROLL; ++u) {
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     pid[u][r] = next[u][r];
@@ -499,10 +503,10 @@ __global__ void __launch_bounds__(SEL_TOKENS * 32) select_eight_kernel(const Sel
                 }
                 st[u].load(ix, a.i_page, pid[u], tq);
             }
-            look(j0 + N * 16 * SEL_UNROLL);
-            float best[SEL_UNROLL][4];   // page g: tokens 2 t, 2 t + 1; page g + 8
+            look(j0 + N * 16 * UNROLL);
+            float best[UNROLL][4];   // page g: tokens 2 t, 2 t + 1; page g + 8
 #pragma unroll
-            for (int u = 0; u < SEL_UNROLL; ++u) best[u][0] = best[u][1] = best[u][2] = best[u][3] = -INFINITY;
+            for (int u = 0; u < UNROLL; ++u) best[u][0] = best[u][1] = best[u][2] = best[u][3] = -INFINITY;
             for (int hd = 0; hd < a.grp; ++hd) {   // columns: one head of the 8 tokens
                 int4 q[2 * D / 64];
 #pragma unroll
@@ -510,7 +514,7 @@ __global__ void __launch_bounds__(SEL_TOKENS * 32) select_eight_kernel(const Sel
                     q[b] = *reinterpret_cast<const int4*>((b < D / 64 ? qpos : qneg) + (hd * N + g) * D + (b % (D / 64)) * 64 + 16 * tq);
                 const float u0 = qunit[hd * N + 2 * tq], u1 = qunit[hd * N + 2 * tq + 1];
 #pragma unroll
-                for (int u = 0; u < SEL_UNROLL; ++u) {
+                for (int u = 0; u < UNROLL; ++u) {
                     int c[4];
                     st[u].dot(c, q);
 #pragma unroll
@@ -518,7 +522,7 @@ __global__ void __launch_bounds__(SEL_TOKENS * 32) select_eight_kernel(const Sel
                 }
             }
 #pragma unroll
-            for (int u = 0; u < SEL_UNROLL; ++u)
+            for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     const int j = j0 + u * N * 16 + g + 8 * r;
@@ -528,9 +532,22 @@ __global__ void __launch_bounds__(SEL_TOKENS * 32) select_eight_kernel(const Sel
         }
     }
     __syncthreads();
-    if (!own) return;
-    choose<1>(keys + (long long)warp * a.cols, own, a.top_k - 1, sel, {hist[warp], list[warp], pick[warp], nullptr}, 0, lane);
-    if (lane == 0) sel[a.top_k - 1] = own;
+    if (own) {
+        choose<1>(keys + (long long)warp * a.cols, own, a.top_k - 1, sel, {hist[warp], list[warp], pick[warp], nullptr}, 0, lane);
+        if (lane == 0) sel[a.top_k - 1] = own;
+    }
+    if (!a.count || t >= a.n) return;
+    __syncwarp();
+    for (int k = lane; k < a.top_k; k += 32) {
+        const int c = sel[k];   // listed: the slot and the column are in range
+        int rank = -1;
+        if (c >= 0) {
+            const int pid = __ldg(a.table + slot * a.table_row + c);
+            if (pid >= 0 && pid < a.pages) rank = (int)atomicAdd(a.count + (long long)h * a.pages + pid, 1u);
+            else note_status(a.status, MQ_ERR_BAD_PAGE);
+        }
+        a.rank[((long long)t * a.hkv + h) * a.top_k + k] = rank;
+    }
 }
 
 // ---- host ----------------------------------------------------------------------------------
@@ -554,9 +571,37 @@ void set_rt(RowArgs& a, bool eight) {
     a.rt_shift = eight ? 3 : 4;
 }
 
+// The choice kernel takes eight tokens to a CTA once that gives every SM a CTA of them and their keys fit (96 KB).
+bool eight_fit(int n, int hkv, int D, int cols, int grp) {
+    return (long long)n * hkv >= (long long)SEL_TOKENS * sm_count() && n >= SEL_TOKENS &&
+           (D == 128 ? sel_eight_bytes<128>(cols, grp) : sel_eight_bytes<64>(cols, grp)) <= 98304;
+}
+
 // CTAs of the work line, two to an SM for head_dim 128 (rings of 96 KB) and
 // three for 64 (registers).
 int row_grid(int D, int rt) { return sm_count() * (D == 128 && rt == 16 ? 2 : 3); }
+
+// The page-by-page form's rounds: parts that stay in L2 from the kernel that writes them to the join.
+constexpr size_t PART_BYTES = 96u << 20;
+constexpr int BY_PAGE_TOKENS = 64;
+
+// Tokens per round of the page-by-page form, or 0 where each token reads its own pages.  Page by page when
+//  - there are more tokens than slots, so that some stand in one sequence (150 tokens of one context: 59 us against
+//    79; of 256 sequences with nothing in common: 237 against 216),
+//  - a page's keys and values are 16 times its parts for one token or more (500 tokens on two contexts of 16k, page
+//    over group 64: 105 us against 202, 32: 107 against 205, 16: 204 against 216, 8: 378 against 235),
+//  - the choice kernel takes eight tokens at a time (it counts for this form), a round holds 64 tokens or more, and
+//    the pool has no more than 16 pages for each choice (the counts are cleared and read, 8 bytes a page).
+int by_page_tokens(const mq_paged_sparse_params* p) {
+    const mq_paged_pool& o = *p->pool;
+    const int grp = p->num_q_heads / o.num_kv_heads, D = o.head_dim;
+    const size_t part = 4 * (size_t)(D + 4), token = part * p->num_q_heads * p->top_k;
+    const size_t most = PART_BYTES / token;
+    if (most < BY_PAGE_TOKENS || p->n < BY_PAGE_TOKENS || o.page_size < 16 * grp || p->n <= p->num_slots) return 0;
+    const int rounds = ceil_div(p->n, (int)(most < 0x7fffffff ? most : 0x7fffffff)), n = ceil_div(p->n, rounds);
+    if (!eight_fit(n, o.num_kv_heads, D, p->table_cols, grp) || o.num_pages > 16ll * n * p->top_k) return 0;
+    return n;
+}
 
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
@@ -598,6 +643,25 @@ size_t row_workspace(const Shape& s, WsView* v, void* base) {
     return o;
 }
 
+size_t by_page_workspace(const mq_paged_sparse_params* p, int n, ByPage* v, void* base) {
+    const size_t bins = (size_t)p->pool->num_kv_heads * p->pool->num_pages;
+    const size_t entries = (size_t)n * p->pool->num_kv_heads * p->top_k;
+    const size_t off = up256(16 + bins * 4), items = off + up256(bins * 4), list = items + up256(entries * 16);
+    const size_t rank = list + up256(entries * 16), parts = rank + up256(entries * 4);
+    if (v) {
+        uint8_t* b = (uint8_t*)base;
+        v->cursor = (unsigned long long*)b;
+        v->count = (uint32_t*)(b + 16);
+        v->off = (uint32_t*)(b + off);
+        v->items = (int4*)(b + items);
+        v->list = (int4*)(b + list);
+        v->rank = (int*)(b + rank);
+        v->parts = (float*)(b + parts);
+        v->per_item = 8 * BY_PAGE_NT / (p->num_q_heads / p->pool->num_kv_heads);
+    }
+    return parts + (size_t)n * p->num_q_heads * p->top_k * (p->pool->head_dim + 4) * 4;
+}
+
 Shape shape_of(const mq_paged_attend_params* p) {
     return {p->pool->head_dim, p->num_q_heads, p->total_q, true, p->num_groups > 0,
             tc_prefix(p->total_q, p->num_q_heads / p->pool->num_kv_heads, p->num_groups, p->scale)};
@@ -606,26 +670,23 @@ Shape shape_of(const mq_paged_sparse_params* p) {
     return {p->pool->head_dim, p->num_q_heads, p->n, false, false, false};
 }
 
-// The pool's K or V as a rank-5 map of boxes of 64 channels x `rows` rows of a page.
-bool pool_map(CUtensorMap* m, const mq_paged_pool& p, const void* base, long long page, long long layer, long long head, int rows) {
+// A layer's K or V as a rank-5 map of boxes of `rows` rows of a page, `blocks` blocks of 64 channels.
+bool pool_map(CUtensorMap* m, const mq_paged_pool& p, const void* base, long long page, long long head, int rows, int blocks) {
     const cuuint64_t row = (cuuint64_t)p.head_dim * 2, block = row * p.page_size;
-    const cuuint64_t dims[5] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.page_size, (cuuint64_t)p.num_kv_heads,
-                                (cuuint64_t)p.num_layers, (cuuint64_t)p.num_pages};
+    const cuuint64_t dims[5] = {64, (cuuint64_t)p.page_size, (cuuint64_t)p.head_dim / 64, (cuuint64_t)p.num_kv_heads, (cuuint64_t)p.num_pages};
     // the stride of a dimension of one is never used and may be anything
-    const cuuint64_t strides[4] = {row, p.num_kv_heads > 1 ? (cuuint64_t)head * 2 : block,
-                                   p.num_layers > 1 ? (cuuint64_t)layer * 2 : block,
-                                   p.num_pages > 1 ? (cuuint64_t)page * 2 : block};
-    const cuuint32_t box[5] = {64, (cuuint32_t)rows, 1, 1, 1};
+    const cuuint64_t strides[4] = {row, 128, p.num_kv_heads > 1 ? (cuuint64_t)head * 2 : block, p.num_pages > 1 ? (cuuint64_t)page * 2 : block};
+    const cuuint32_t box[5] = {64, (cuuint32_t)rows, (cuuint32_t)blocks, 1, 1};
     return make_tmap_nd(m, base, p.dtype == MQ_BF16, 5, dims, strides, box);
 }
-bool pool_maps(CUtensorMap* k, CUtensorMap* v, const mq_paged_pool& p, int rows) {
-    return pool_map(k, p, p.k, p.k_page, p.k_layer, p.k_head, rows) && pool_map(v, p, p.v, p.v_page, p.v_layer, p.v_head, rows);
+bool pool_maps(CUtensorMap* k, CUtensorMap* v, const mq_paged_pool& p, const PoolView& at, int rows, int blocks) {
+    return pool_map(k, p, at.k, at.k_page, at.k_head, rows, blocks) && pool_map(v, p, at.v, at.v_page, at.v_head, rows, blocks);
 }
 
 template <typename T, int D>
 int run_prefix(const RowArgs& a, const mq_paged_pool& pool, cudaStream_t st) {
     CUtensorMap tk, tv;
-    if (!pool_maps(&tk, &tv, pool, pool.page_size)) return MQ_ERR_CUDA;
+    if (!pool_maps(&tk, &tv, pool, a.pool, pool.page_size, 1)) return MQ_ERR_CUDA;
     auto kernel = prefix_kernel<T, D>;
     const size_t smem = PfxSmem<D>::bytes(a.NG);
     static SmemLimit limit;
@@ -634,10 +695,26 @@ int run_prefix(const RowArgs& a, const mq_paged_pool& pool, cudaStream_t st) {
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "paged prefix attention");
 }
 
+template <typename T, int D, int MODE>
+cudaError_t run_join(const RowArgs& a, uint32_t row_warps, cudaStream_t st) {
+    const long long rows = (long long)a.total_q * a.hq;
+    // As many warps to a row as leave all CTAs resident at once (three to an SM): a second wave costs more
+    // than the warps save (1024 rows of 34 parts, 512 CTAs: 14 us).
+    auto join = [&](auto split) {
+        constexpr int S = decltype(split)::value;
+        return launch(join_kernel<T, D, MODE, S>, dim3((unsigned)((rows * S + 7) / 8)), dim3(256), 0, st, a, row_warps);
+    };
+    const long long room = 3ll * sm_count() * 8 / rows;   // warps to a row
+    return room >= 8   ? join(std::integral_constant<int, 8>{})
+           : room >= 4 ? join(std::integral_constant<int, 4>{})
+           : room >= 2 ? join(std::integral_constant<int, 2>{})
+                       : join(std::integral_constant<int, 1>{});
+}
+
 template <typename T, int D, int MODE, int NT>
 int run_rows(const RowArgs& a, const mq_paged_pool& pool, cudaStream_t st) {
     CUtensorMap tk, tv;
-    if (!pool_maps(&tk, &tv, pool, GRP)) return MQ_ERR_CUDA;
+    if (!pool_maps(&tk, &tv, pool, a.pool, GRP, D / 64)) return MQ_ERR_CUDA;
     auto kernel = rows_kernel<T, D, MODE, NT>;
     const size_t smem = (size_t)ROW_WARPS * RowWarp<T, D, NT>::RING + 1024 + (MODE == 0 ? sched_bytes(a.B, a.NG) : 0);
     static SmemLimit limit;
@@ -645,20 +722,7 @@ int run_rows(const RowArgs& a, const mq_paged_pool& pool, cudaStream_t st) {
     if (e != cudaSuccess) return note_cuda(e, "paged attention attribute");
     const int grid = row_grid(D, 8 * NT);
     e = launch(kernel, dim3(grid), dim3(ROW_THREADS), smem, st, tk, tv, a);
-    const long long rows = (long long)a.total_q * a.hq;
-    if (e == cudaSuccess) {
-        // As many warps to a row as leave all CTAs resident at once (three to an SM): a second wave costs more
-        // than the warps save (1024 rows of 34 parts, 512 CTAs: 14 us).
-        auto join = [&](auto split) {
-            constexpr int S = decltype(split)::value;
-            return launch(join_kernel<T, D, MODE, S>, dim3((unsigned)((rows * S + 7) / 8)), dim3(256), 0, st, a, (uint32_t)grid * ROW_WARPS);
-        };
-        const long long room = 3ll * sm_count() * 8 / rows;   // warps to a row
-        e = room >= 8   ? join(std::integral_constant<int, 8>{})
-            : room >= 4 ? join(std::integral_constant<int, 4>{})
-            : room >= 2 ? join(std::integral_constant<int, 2>{})
-                        : join(std::integral_constant<int, 1>{});
-    }
+    if (e == cudaSuccess) e = run_join<T, D, MODE>(a, (uint32_t)grid * ROW_WARPS, st);
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "paged attention");
 }
 
@@ -671,6 +735,23 @@ int run_attend(const RowArgs& a, const mq_paged_pool& pool, cudaStream_t st) {
     return a.rt == 8 ? run_rows<T, D, 0, 1>(a, pool, st) : run_rows<T, D, 0, 2>(a, pool, st);
 }
 
+// After the choice, whose counts are in place.
+template <typename T, int D>
+int run_by_page(const RowArgs& a, const mq_paged_pool& pool, cudaStream_t st) {
+    CUtensorMap tk, tv;
+    if (!pool_maps(&tk, &tv, pool, a.pool, GRP, D / 64)) return MQ_ERR_CUDA;
+    auto kernel = by_page_kernel<T, D>;
+    const size_t smem = (size_t)ROW_WARPS * RowWarp<T, D, BY_PAGE_NT>::RING + 1024;
+    static SmemLimit limit;
+    cudaError_t e = allow_smem(kernel, smem, limit);
+    const long long bins = (long long)a.hkv * a.pool.pages, entries = (long long)a.total_q * a.hkv * a.top_k;
+    if (e == cudaSuccess) e = launch(plan_kernel, dim3((unsigned)((bins + 255) / 256)), dim3(256), 0, st, a.bp, a.hkv, a.pool.pages);
+    if (e == cudaSuccess) e = launch(list_kernel, dim3((unsigned)((entries + 255) / 256)), dim3(256), 0, st, a);
+    if (e == cudaSuccess) e = launch(kernel, dim3(row_grid(D, 8 * BY_PAGE_NT)), dim3(ROW_THREADS), smem, st, tk, tv, a);
+    if (e == cudaSuccess) e = run_join<T, D, 2>(a, 0, st);
+    return e == cudaSuccess ? MQ_OK : note_cuda(e, "paged attention by page");
+}
+
 bool q_ok(const void* q, long long tok, long long head) {
     return q && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && tok % 8 == 0 && head % 8 == 0;
 }
@@ -678,8 +759,7 @@ bool q_ok(const void* q, long long tok, long long head) {
 template <typename T, int D>
 int run_select(const SelArgs& s, cudaStream_t st) {
     const long long items = (long long)s.n * s.hkv;
-    // eight tokens to a CTA once that gives every SM a CTA of them and their keys fit (96 KB)
-    if (items >= (long long)SEL_TOKENS * sm_count() && s.n >= SEL_TOKENS && sel_eight_bytes<D>(s.cols, s.grp) <= 98304) {
+    if (s.count || eight_fit(s.n, s.hkv, D, s.cols, s.grp)) {   // (page by page: whatever a last round has left)
         static SmemLimit limit;
         const size_t smem = sel_eight_bytes<D>(s.cols, s.grp);
         cudaError_t e = allow_smem(select_eight_kernel<T, D>, smem, limit);
@@ -763,7 +843,6 @@ int mq_paged_attend(const mq_paged_attend_params* p, cudaStream_t st) {
     const Shape s = shape_of(p);
     row_workspace(s, &a.ws, p->workspace);
     a.tc = s.tc;
-    a.layer = p->layer;
     // 8 rows to an item when a sequence (and a group whose prefix is not on the tensor-core kernel) has no
     // more on average: half the tensor work a group; otherwise 16, so that the keys are read half as often
     const long long rows = (long long)a.total_q * a.grp;
@@ -772,8 +851,9 @@ int mq_paged_attend(const mq_paged_attend_params* p, cudaStream_t st) {
 }
 
 size_t mq_paged_sparse_workspace_bytes(const mq_paged_sparse_params* p) {
-    if (!p || !p->pool || p->n < 0) return 0;
-    return row_workspace(shape_of(p), nullptr, nullptr);
+    if (!p || !p->pool || p->n < 0 || p->pool->num_kv_heads < 1 || p->num_q_heads < p->pool->num_kv_heads || p->top_k < 1) return 0;
+    const int n = by_page_tokens(p);
+    return n ? by_page_workspace(p, n, nullptr, nullptr) : row_workspace(shape_of(p), nullptr, nullptr);
 }
 
 int mq_paged_sparse(const mq_paged_sparse_params* p, cudaStream_t st) {
@@ -815,8 +895,6 @@ int mq_paged_sparse(const mq_paged_sparse_params* p, cudaStream_t st) {
     s.grp = p->num_q_heads / o.num_kv_heads;
     s.top_k = p->top_k;
     s.status = p->status;
-    const int rc = dispatch(o.dtype, o.head_dim, [&](auto T, auto D) { return run_select<decltype(T), decltype(D)::value>(s, st); });
-    if (rc) return rc;
     RowArgs a = {};
     a.pool = view_of(o, p->layer);
     a.q = s.q;
@@ -837,14 +915,37 @@ int mq_paged_sparse(const mq_paged_sparse_params* p, cudaStream_t st) {
     a.top_k = p->top_k;
     a.scale_log2 = p->scale * 1.4426950408889634f;
     a.status = p->status;
-    row_workspace(shape_of(p), &a.ws, p->workspace);
-    a.layer = p->layer;
     set_rt(a, a.grp <= 8);
-    return dispatch(o.dtype, o.head_dim, [&](auto T, auto D) {
-        using E = decltype(T);
-        constexpr int d = decltype(D)::value;
-        return a.rt == 8 ? run_rows<E, d, 1, 1>(a, o, st) : run_rows<E, d, 1, 2>(a, o, st);
-    });
+    const int round = by_page_tokens(p);
+    if (round) by_page_workspace(p, round, &a.bp, p->workspace);
+    else row_workspace(shape_of(p), &a.ws, p->workspace);
+    for (long long t0 = 0; t0 < p->n; t0 += round ? round : p->n) {
+        s.n = a.total_q = round ? (int)std::min<long long>(round, p->n - t0) : p->n;
+        s.q = a.q = (const uint16_t*)p->q + t0 * p->q_token;
+        a.out = (uint16_t*)p->out + t0 * a.hq * o.head_dim;
+        a.selected = s.selected = p->selected + t0 * a.hkv * a.top_k;
+        a.slots = s.slots = p->slots + t0;
+        a.positions = s.positions = p->positions + t0;
+        if (round) {
+            s.count = a.bp.count;
+            s.rank = a.bp.rank;
+            const long long words = (16 + (long long)a.hkv * o.num_pages * 4 + 15) / 16;
+            const long long blocks = (words + 255) / 256, most = 2ll * sm_count();
+            const cudaError_t e = launch(clear_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st,
+                                         reinterpret_cast<uint4*>(a.bp.cursor), words);
+            if (e != cudaSuccess) return mq::note_cuda(e, "paged attention by page");
+        }
+        const int rc = dispatch(o.dtype, o.head_dim, [&](auto T, auto D) {
+            using E = decltype(T);
+            constexpr int d = decltype(D)::value;
+            const int r = run_select<E, d>(s, st);
+            if (r) return r;
+            if (round) return run_by_page<E, d>(a, o, st);
+            return a.rt == 8 ? run_rows<E, d, 1, 1>(a, o, st) : run_rows<E, d, 1, 2>(a, o, st);
+        });
+        if (rc) return rc;
+    }
+    return MQ_OK;
 }
 
 }  // extern "C"

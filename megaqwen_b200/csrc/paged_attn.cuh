@@ -10,7 +10,7 @@
 // be small enough to hide: mma.sync m16n8k16 with the 16 positions (or 16 head
 // dims) on the M side and the rows as N, so that up to 8 rows cost 8 + 16
 // MMAs a group for head_dim 128 (rows on the M side cost twice that and 788
-// instructions a group, and bound the kernel: 340 us against 2.1 GB from L2).
+// instructions a group, and bound the kernel: 340 us for 2.1 GB from L2).
 // What else has to be had is bytes in flight on every SM, whatever the
 // lengths: the unit of work is one warp's 16-position group, all groups of all
 // (sequence, kv head) items laid end to end and cut into equal runs, one per
@@ -20,10 +20,11 @@
 // depend on timing.
 //
 // Measured: 16 sequences of 64k, 2048 chosen positions each, 134 MB: 26 us (5.1
-// TB/s, 0.79 of the copy rate); 500 tokens x 8 kv heads x 1024 positions, 2.1 GB
-// of which 134 MB are distinct: 170 us (12.3 TB/s, from L2); own parts of 64
-// sequences behind a prefix, 67 MB in 512 items: 17 us (3.9 TB/s: items of 16
-// groups on average, one or two to a warp).
+// TB/s, 0.79 of the copy rate); own parts of 64 sequences
+// behind a prefix, 67 MB in 512 items: 17 us (3.9 TB/s: items of 16 groups on
+// average, one or two to a warp).  From L2 it reaches 12.3 TB/s (500 tokens x 8
+// kv heads x 1024 positions, 2.1 GB of which 134 MB are distinct, 170 us), which
+// is why such calls go page by page (paged_by_page.cuh).
 #pragma once
 
 #include "mq_tc.cuh"
@@ -71,6 +72,18 @@ struct WsView {
     float* pfx_slots;   // [2 * CTAs][PROWS][D + 4], tensor-core prefix only
 };
 
+// Sparse attention page by page (paged_by_page.cuh).
+struct ByPage {
+    uint32_t* count;              // [kv heads x pages] tokens that chose the page
+    unsigned long long* cursor;   // items << 32 | list entries taken
+    uint32_t* off;                // [kv heads x pages] the page's place in the list
+    int4* items;                  // kv head, page, place in the list, tokens
+    int4* list;                   // token, choice, positions of the page that it sees
+    int* rank;                    // [n, kv heads, top_k] place in the page's stretch, or -1
+    float* parts;                 // [n, q heads, top_k][D + 4]
+    int per_item;                 // tokens
+};
+
 struct RowArgs {
     PoolView pool;
     const uint16_t* q;
@@ -88,24 +101,31 @@ struct RowArgs {
     const int* selected;    // sparse
     int B, NG, total_q, hq, hkv, grp, top_k;   // grp = hq / hkv
     int rt, rt_shift;       // query rows per item of rows_kernel
-    int layer;
     int tc;                 // prefixes run on the tensor-core kernel
     float scale_log2;
     int* status;
     WsView ws;
+    ByPage bp;
 };
 
-__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int x, int row, int h, int l, int p,
-                                            uint32_t bar) {
+// A box of a page: rows from `row`, blocks of 64 channels from `block`, by a map whose base is at the layer.
+__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, int row, int block, int h, int page,
+                                              uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
-        ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(h), "r"(l), "r"(p), "r"(bar)
+        ::"r"(dst), "l"(map), "r"(0), "r"(row), "r"(block), "r"(h), "r"(page), "r"(bar)
         : "memory");
 }
 __device__ __forceinline__ uint32_t movm_t(uint32_t a) {
     uint32_t d;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
+}
+// 2^x; 2^-inf = 0, and results below the normal numbers are 0
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 constexpr long long WAIT_CYCLES = 4000000000ll;   // bound of every wait, about two seconds
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
@@ -317,17 +337,18 @@ struct RowWarp {
     float m[NT][2], l[NT][2];
 
     // Q^T as the B operand: row 8 n + g, dims 16 k + 2 t (+ 8)
+    __device__ __forceinline__ void load_row(int n, const uint16_t* p) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                qb[n][k][i] = p ? __ldg(reinterpret_cast<const uint32_t*>(p + 16 * k + 8 * i + 2 * (lane & 3))) : 0u;
+    }
     __device__ __forceinline__ void load_q(const RowArgs& a, int tok0, int h, int grp, int r0, int rows) {
-        const int g = lane >> 2, t = lane & 3;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int r = r0 + 8 * n + g, tok = r / grp;
-            const uint16_t* p = 8 * n + g < rows ? a.q + (long long)(tok0 + tok) * a.q_tok + (h * grp + r - tok * grp) * a.q_head : nullptr;
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    qb[n][k][i] = p ? __ldg(reinterpret_cast<const uint32_t*>(p + 16 * k + 8 * i + 2 * t)) : 0u;
+            const int i = 8 * n + (lane >> 2), r = r0 + i, tok = r / grp;
+            load_row(n, i < rows ? a.q + (long long)(tok0 + tok) * a.q_tok + (h * grp + r - tok * grp) * a.q_head : nullptr);
         }
     }
 
@@ -356,7 +377,9 @@ struct RowWarp {
     }
 
     // lim: positions of the group (below 1: none, 16 and up: all) that rows 8 n + 2 t + i see.
-    // `mixed`: the rows of the tile do not all see the same positions.
+    // `mixed`: the rows of the tile do not all see the same positions.  SOLO: a row's sums may not depend on
+    // the rows beside it, not in their last bit; `mixed`: a row does not see all positions.
+    template <bool SOLO>
     __device__ __forceinline__ void step(int stage, const int (&lim)[NT][2], bool mixed, float scale) {
         const uint32_t ks = ring + stage * STAGE, vs = ks + TILE;
         const int g = lane >> 2, mat = lane >> 3, r8 = lane & 7;
@@ -390,13 +413,13 @@ struct RowWarp {
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
                 const float mn = fmaxf(m[n][i], mx);
-                corr[n][i] = mn == m[n][i] ? 1.f : exp2f(m[n][i] - mn);   // m = -inf: nothing summed yet
+                corr[n][i] = mn == m[n][i] ? 1.f : ex2(m[n][i] - mn);   // m = -inf: nothing summed yet
                 moved |= mn != m[n][i];
                 m[n][i] = mn;
                 u[i] = mn == -INFINITY ? 0.f : mn;
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][i] = exp2f(s[n][i] - u[i & 1]);
+            for (int i = 0; i < 4; ++i) s[n][i] = ex2(s[n][i] - u[i & 1]);
             l[n][0] = l[n][0] * corr[n][0] + (s[n][0] + s[n][2]);
             l[n][1] = l[n][1] * corr[n][1] + (s[n][1] + s[n][3]);
             // two pieces of the 16-bit type: one would cost as much accuracy as rounding the output does
@@ -448,8 +471,25 @@ struct RowWarp {
                 }
             }
         } else {
+            if (SOLO) {   // rows that see all positions, as in any other tile
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    uint32_t f[4];
+                    ldsm4t(vs + piece(vrow, 2 * i + (mat & 1)), f[0], f[1], f[2], f[3]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float x[4] = {o[n][i][0], o[n][i][1], o[n][i][2], o[n][i][3]};
+                        Elem<T>::mma(x, f, ph[n][0], ph[n][1]);
+                        Elem<T>::mma(x, f, pr[n][0], pr[n][1]);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            if (lim[n][c & 1] >= GRP) o[n][i][c] = x[c];
+                    }
+                }
+            }
             // one position at a time, added only to the rows that see it
             const int t = lane & 3;
+            auto takes = [&](int p, int lim_r) { return p < lim_r && !(SOLO && lim_r >= GRP); };
 #pragma unroll 1
             for (int p = 0; p < GRP; ++p) {
                 uint32_t keep[2];
@@ -469,11 +509,11 @@ struct RowWarp {
                         float x[4] = {0.f, 0.f, 0.f, 0.f};
                         Elem<T>::mma(x, f, ph[n][0] & keep[0], ph[n][1] & keep[1]);
                         Elem<T>::mma(x, f, pr[n][0] & keep[0], pr[n][1] & keep[1]);
-                        if (p < lim[n][0]) {
+                        if (takes(p, lim[n][0])) {
                             o[n][i][0] += x[0];
                             o[n][i][2] += x[2];
                         }
-                        if (p < lim[n][1]) {
+                        if (takes(p, lim[n][1])) {
                             o[n][i][1] += x[1];
                             o[n][i][3] += x[3];
                         }
@@ -733,11 +773,8 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 if (lane == 0) {
                     const uint32_t bar = smem_u32(&full[warp][stage_l]), dst = w.ring + stage_l * W::STAGE;
                     mbar_arrive_expect_tx(&full[warp][stage_l], W::STAGE);
-#pragma unroll
-                    for (int i = 0; i < D / 64; ++i) {
-                        tma_load_5d(dst + i * W::BOX, &tmK, 64 * i, p0 & (page - 1), h, a.layer, pid, bar);
-                        tma_load_5d(dst + W::TILE + i * W::BOX, &tmV, 64 * i, p0 & (page - 1), h, a.layer, pid, bar);
-                    }
+                    tma_load_page(dst, &tmK, p0 & (page - 1), 0, h, pid, bar);
+                    tma_load_page(dst + W::TILE, &tmV, p0 & (page - 1), 0, h, pid, bar);
                 }
                 p = p0;
             }
@@ -790,7 +827,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     rel[n][0] = lim[n][0] - p0;
                     rel[n][1] = lim[n][1] - p0;
                 }
-                w.step(stage_c, rel, lim_lo < min(p0 + GRP, lim_top), a.scale_log2);
+                w.template step<false>(stage_c, rel, lim_lo < min(p0 + GRP, lim_top), a.scale_log2);
             }
             stage_c = stage_c == STAGES - 1 ? 0 : stage_c + 1;
             __syncwarp();   // every lane is past its reads of the stage
@@ -855,6 +892,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
 // acc = sum of the parts' acc_i 2^(m_i - M) over sum l_i 2^(m_i - M).  Bound by the
 // latency of three dependent reads (what a token has, the parts' m and l, their acc):
 // 1024 rows of 34 parts, 18 MB: 9 us; 2048 rows of 20: 9 us.
+// MODE 2: sparse page by page, a part to each page that a token chose.
 // SPLIT warps share a row (the fewer rows, the more parts each), 8 / SPLIT rows to a CTA.
 template <typename T, int D, int MODE, int SPLIT>
 __global__ void __launch_bounds__(256, 3) join_kernel(const RowArgs a, uint32_t row_warps) {
@@ -892,11 +930,18 @@ __global__ void __launch_bounds__(256, 3) join_kernel(const RowArgs a, uint32_t 
             return;
         }
     }
+    const int* there = nullptr;
+    if (MODE == 2) {
+        there = a.bp.rank + ((long long)tok * a.hkv + h) * a.top_k;
+        src1 = a.bp.parts + rowi * a.top_k * LD;
+        step1 = LD;
+        np1 = a.top_k;
+    }
     const int sp_ng = MODE == 1 ? a.top_k << (a.pool.shift - 4) : 0;
     const uint32_t quota =
         MODE == 0 ? hd.y
                   : quota_of((uint32_t)a.total_q * a.hkv * row_tiles(a, grp) * (sp_ng + ITEM_UNITS), row_warps);
-    {
+    if (MODE != 2) {
         int ng, r;
         uint32_t start;   // the item's first group on the line
         if (MODE == 0) {
@@ -957,7 +1002,12 @@ __global__ void __launch_bounds__(256, 3) join_kernel(const RowArgs a, uint32_t 
     for (int i0 = sub; i0 < np; i0 += SPLIT * 32) {
         const int mine = i0 + SPLIT * lane, cnt = min(32, (np - i0 + SPLIT - 1) / SPLIT);
         const float* p = mine < np ? part(mine) : nullptr;
-        const float2 ml = p ? __ldcg(reinterpret_cast<const float2*>(p)) : make_float2(-INFINITY, 0.f);
+        const int at = MODE == 2 && mine < np ? __ldcg(there + mine) : 0;
+        float2 ml = p ? __ldcg(reinterpret_cast<const float2*>(p)) : make_float2(-INFINITY, 0.f);
+        if (at < 0) {   // nothing was written there
+            p = nullptr;
+            ml = make_float2(-INFINITY, 0.f);
+        }
         float bm = ml.x;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, o));
@@ -980,7 +1030,7 @@ __global__ void __launch_bounds__(256, 3) join_kernel(const RowArgs a, uint32_t 
                 w[q] = __shfl_sync(0xffffffffu, e, (k + q) & 31);
 #pragma unroll
                 for (int i = 0; i < V; ++i) v[q][i] = 0.f;
-                if (k + q < cnt) {
+                if (k + q < cnt && (MODE != 2 || r)) {
                     if (V == 4) {
                         const float4 x = __ldcg(reinterpret_cast<const float4*>(r + 4) + lane);
                         v[q][0] = x.x; v[q][1] = x.y; v[q][V - 2] = x.z; v[q][V - 1] = x.w;

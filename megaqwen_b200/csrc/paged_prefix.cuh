@@ -80,12 +80,6 @@ __device__ constexpr uint32_t pfx_idesc(int N, bool b_mn) {
     return (1u << 4) | (f << 7) | (f << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // The same value in every lane, in a form the compiler knows to be uniform.
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
@@ -267,7 +261,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
                 if (lane < chunks) {
 #pragma unroll
                     for (int i = 0; i < D / 64; ++i)
-                        tma_load_5d(smem_u32(ring + st * TILE + i * PATOM + lane * page * 128), map, 64 * i, 0, e.h, a.layer, pid, smem_u32(&full[st]));
+                        tma_load_page(smem_u32(ring + st * TILE + i * PATOM + lane * page * 128), map, 0, i, e.h, pid, smem_u32(&full[st]));
                 }
             }
         }

@@ -767,6 +767,84 @@ def test_sparse_ties(paged):
                  q=torch.zeros(1, 2, d, dtype=torch.bfloat16, device="cuda"))
 
 
+@pytest.mark.parametrize("dtype,d,page,grp,top_k", [(torch.bfloat16, 128, 32, 2, 5), (torch.float16, 64, 64, 3, 3), (torch.bfloat16, 64, 128, 8, 2),
+                                                    (torch.float16, 128, 16, 1, 1)])
+def test_sparse_by_page(paged, dtype, d, page, grp, top_k):
+    """More tokens than slots, pages that are large beside their parts: a page is read once for all tokens that chose
+    it.  Pages chosen by one token and by scores of them, tokens with fewer pages than top_k, q with strides."""
+    hkv = 8
+    lens = [12 * page + 3, 5 * page, page - 3]
+    p = Pool(lens, page, hkv, d, dtype, seed=grp)
+    idx = full_index(p, 2, hkv, d)
+    seqs = [0] * 100 + [i % 3 for i in range(30)] + [1] * 25
+    pos = [(i * 37) % lens[s] for i, s in enumerate(seqs)]
+    q = normal(p.g, len(seqs), hkv * grp + 2, d + 8, dtype=dtype, std=1.5)[:, 1:-1, :d]
+    check_sparse(paged, p, hkv * grp, idx, [p.slots[s] for s in seqs], pos, seqs, top_k, q=q)
+
+
+def test_sparse_by_page_bad_values(paged):
+    """Infinities and NaN where no token of the call looks, and beside tokens that do not see them; wrong places; pages
+    out of range.  Rows must not depend on which others share their page, so two calls agree in every bit."""
+    page, hkv, grp, d, n = 64, 8, 2, 128, 160
+    p = Pool([640, 200], page, hkv, d, torch.bfloat16, seed=3)
+    idx = full_index(p, 2, hkv, d)
+    slots = [p.slots[0]] * (n - 20) + [p.slots[1]] * 20
+    seqs = [0] * (n - 20) + [1] * 20
+    pos = [(i * 7) % 600 for i in range(n - 20)] + [180 + i % 20 for i in range(20)]
+    q = normal(p.g, n, hkv * grp, d, std=1.5)
+    kw = dict(layer=1, top_k=4)
+    ref, want = paged.sparse_attend(q, p.k, p.v, idx, p.table, dev(slots), dev(pos), **kw)
+    # positions 600 .. 639 of sequence 0 and 200 .. 255 of sequence 1 are seen by no token
+    for row, at in ((p.rows[0][9], 24), (p.rows[1][3], 8)):
+        p.k[row, :, :, at:] = math.nan
+        p.v[row, :, :, at:] = math.inf
+    out, sel = paged.sparse_attend(q, p.k, p.v, idx, p.table, dev(slots), dev(pos), **kw)
+    assert torch.equal(sel, want)
+    close(out, ref.double(), p.v[:, 1].float().nan_to_num(posinf=0).abs().max().item())
+    # an infinity in the middle of a page reaches the tokens behind it alone
+    p.v[p.rows[0][9], 1, :, 10, 5] = math.inf
+    out, sel = paged.sparse_attend(q, p.k, p.v, idx, p.table, dev(slots), dev(pos), **kw)
+    sees = dev([s == 0 and x >= 9 * page + 10 for s, x in zip(seqs, pos)]).bool()
+    assert sees.any() and not torch.isfinite(out[sees][:, :, 5]).any()
+    rest = out.clone()
+    rest[sees, :, 5] = 0
+    assert torch.isfinite(rest).all()
+    same = ref.clone()
+    same[sees, :, 5] = 0
+    close(rest, same.double(), p.v[:, 1].float().nan_to_num(posinf=0).abs().max().item())
+    bits = out.view(torch.int16)   # (a NaN is not equal to itself)
+    for _ in range(5):
+        assert torch.equal(paged.sparse_attend(q, p.k, p.v, idx, p.table, dev(slots), dev(pos), **kw)[0].view(torch.int16), bits)
+    # wrong places: zeros there, the others as before
+    for i, slot, x, code in ((3, 99, 5, 8), (70, p.slots[0], -1, 5), (159, p.slots[1], 10 ** 9, 5)):
+        s2, p2, status = list(slots), list(pos), dev([0])
+        s2[i], p2[i] = slot, x
+        got, sel = paged.sparse_attend(q, p.k, p.v, idx, p.table, dev(s2), dev(p2), status=status, **kw)
+        assert status.item() == code and not got[i].any() and (sel[i] == -1).all()
+        keep = torch.arange(n, device="cuda") != i
+        assert torch.equal(got[keep].view(torch.int16), bits[keep])
+    table, status = p.table.clone(), dev([0])
+    table[p.slots[1], 3] = p.k.shape[0]
+    got, _ = paged.sparse_attend(q, p.k, p.v, idx, table, dev(slots), dev(pos), status=status, **kw)
+    assert status.item() == 9 and torch.isfinite(got[n - 20:]).all() and torch.equal(got[:n - 20].view(torch.int16), bits[:n - 20])
+
+
+def test_sparse_by_page_rounds(paged):
+    """So many choices to a token that its parts do not all fit at once: the same as a few tokens at a time."""
+    page, hkv, d, top_k, n = 16, 8, 64, 300, 470
+    p = Pool([340 * page, 40 * page], page, hkv, d, torch.bfloat16, seed=9)
+    idx = torch.zeros(p.k.shape[0], 2, hkv, 2 * d + 16, dtype=torch.int8, device="cuda")
+    idx[:, 1, :, :2 * d + 1] = torch.stack([index_ref(p.k[:, 1, h]) for h in range(hkv)], 1)
+    slots = dev([p.slots[i % 7 == 0] for i in range(n)])
+    pos = dev([40 * page - 1 - i % 50 if i % 7 == 0 else 340 * page - 1 - i for i in range(n)])
+    q = normal(p.g, n, hkv, d, std=1.5)
+    out, sel = paged.sparse_attend(q, p.k, p.v, idx, p.table, slots, pos, layer=1, top_k=top_k)
+    for i in range(0, n, 47):
+        ref, want = paged.sparse_attend(q[i:i + 47], p.k, p.v, idx, p.table, slots[i:i + 47], pos[i:i + 47], layer=1, top_k=top_k)
+        assert torch.equal(sel[i:i + 47], want)
+        close(out[i:i + 47], ref.double(), p.v.abs().max().item())
+
+
 def test_sparse_all_pages_is_full_attention(paged):
     p = Pool([333], 32, 2, 128, torch.float16, seed=5)
     idx = torch.zeros(p.k.shape[0], 2, 2, 272, dtype=torch.int8, device="cuda")

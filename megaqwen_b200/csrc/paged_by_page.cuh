@@ -15,8 +15,8 @@
 // costs are the parts, 4 (D + 4) bytes per (token, q head, page), written and
 // read once, and three small launches.
 //
-// Measured, the same 500 tokens: clearing, plan and list 14 us together (4, 5
-// and 6, mostly launch), by_page_kernel 65, join of 68 MB 16; the whole call 107
+// Measured, the same 500 tokens: clearing, plan and list 12 us together (2, 4
+// and 5, mostly launch), by_page_kernel 61, join of 68 MB 16; the whole call 107
 // us against 205.  by_page_kernel reads 0.33 GB (10000 items of 32 KB) and waits
 // mostly for its own arithmetic: 8 warps to an SM (255 registers), each with the
 // chain K Q^T, maximum, 2^x, V^T P^T per 16 positions; the tensor pipe is at
@@ -102,7 +102,7 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* m
         : "memory");
 }
 
-constexpr int BY_PAGE_NT = 2;   // tiles of 8 rows to an item (one, with three CTAs to an SM: 75 us against 65)
+constexpr int BY_PAGE_NT = 2;   // tiles of 8 rows to an item (one, with three CTAs to an SM: 75 us against 61)
 
 // An item's tokens as the loading side leaves them for the computing side.
 struct PageBox {

@@ -155,7 +155,8 @@ struct Picker {
     int* hist;        // [256]
     int* list;        // [32]
     uint32_t* pick;   // [4]
-    int* sums;        // [2][NW]
+    int* ends;        // [2][NW] each warp's smallest and largest key
+    int* sums;        // [2][NW] each warp's counts
 };
 
 // The `want` largest of keys[0 .. own - 1] (ties: the lowest first), 0 < want < own,
@@ -177,12 +178,12 @@ __device__ __forceinline__ void choose(const uint32_t* keys, int own, int want, 
     kmax = __reduce_max_sync(0xffffffffu, kmax);
     if (NW > 1) {
         if (lane == 0) {
-            s.sums[warp] = (int)kmin;
-            s.sums[NW + warp] = (int)kmax;
+            s.ends[warp] = (int)kmin;
+            s.ends[NW + warp] = (int)kmax;
         }
         __syncthreads();
-        kmin = __reduce_min_sync(0xffffffffu, (uint32_t)s.sums[lane % NW]);
-        kmax = __reduce_max_sync(0xffffffffu, (uint32_t)s.sums[NW + lane % NW]);
+        kmin = __reduce_min_sync(0xffffffffu, (uint32_t)s.ends[lane % NW]);
+        kmax = __reduce_max_sync(0xffffffffu, (uint32_t)s.ends[NW + lane % NW]);
     }
     // keys agree above bit `bits`; of those that match `prefix` under `mask` the largest `need` are wanted
     int bits = 32 - __clz((int)(kmin ^ kmax)), need = want;
@@ -273,7 +274,7 @@ __device__ __forceinline__ void choose(const uint32_t* keys, int own, int want, 
             gt += __popc(__ballot_sync(0xffffffffu, i + lane < hi && k > prefix));
             eq += __popc(__ballot_sync(0xffffffffu, i + lane < hi && k == prefix));
         }
-        if (lane == 0) {
+        if (lane == 0) {   // (not into `ends`: with all keys equal no barrier lies between its reads and this)
             s.sums[warp] = gt;
             s.sums[NW + warp] = eq;
         }
@@ -318,7 +319,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(SEL_WARPS * 32) select_one_kernel(const SelArgs a) {
     constexpr int NW = SEL_WARPS, NT = NW * 32;
     extern __shared__ __align__(16) uint8_t sel_smem[];
-    __shared__ int hist[256], sums[2 * NW], list[32];
+    __shared__ int hist[256], ends[2 * NW], sums[2 * NW], list[32];
     __shared__ uint32_t pick[4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = threadIdx.x;
     const int heads = (a.grp + 7) & ~7;
@@ -422,7 +423,7 @@ __global__ void __launch_bounds__(SEL_WARPS * 32) select_one_kernel(const SelArg
     } else {
         __syncthreads();
     }
-    choose<NW>(keys, own, a.top_k - 1, sel, {hist, list, pick, sums}, warp, lane);
+    choose<NW>(keys, own, a.top_k - 1, sel, {hist, list, pick, ends, sums}, warp, lane);
     if (tid == 0) sel[a.top_k - 1] = own;
 }
 
@@ -533,7 +534,7 @@ __global__ void __launch_bounds__(SEL_TOKENS * 32, 3) select_eight_kernel(const 
     }
     __syncthreads();
     if (own) {
-        choose<1>(keys + (long long)warp * a.cols, own, a.top_k - 1, sel, {hist[warp], list[warp], pick[warp], nullptr}, 0, lane);
+        choose<1>(keys + (long long)warp * a.cols, own, a.top_k - 1, sel, {hist[warp], list[warp], pick[warp], nullptr, nullptr}, 0, lane);
         if (lane == 0) sel[a.top_k - 1] = own;
     }
     if (!a.count || t >= a.n) return;

@@ -767,6 +767,22 @@ def test_sparse_ties(paged):
                  q=torch.zeros(1, 2, d, dtype=torch.bfloat16, device="cuda"))
 
 
+@pytest.mark.parametrize("pages,n,hkv", [(40, 140, 8), (3, 140, 8), (600, 70, 8), (3000, 2, 4)])
+def test_sparse_ties_everywhere(paged, pages, n, hkv):
+    """All keys of every item equal (queries of zeros), many items to a call and many calls: most warps of an item have
+    no pages, and none may go ahead of another's reads.  One CTA to an item, and clusters (3000 pages)."""
+    page, d, top_k = 16, 64, min(6, pages - 1)
+    p = Pool([pages * page], page, hkv, d, torch.bfloat16, seed=1)
+    idx = torch.randint(-127, 128, (p.k.shape[0], 2, hkv, 2 * d + 16), dtype=torch.int8, device="cuda", generator=p.g)
+    idx[..., 2 * d] = 0
+    q = torch.zeros(n, hkv, d, dtype=torch.bfloat16, device="cuda")
+    kw = dict(layer=1, top_k=top_k)
+    args = (q, p.k, p.v, idx, p.table, dev(p.slots * n), dev([pages * page - 1] * n))
+    want = dev(list(range(top_k - 1)) + [pages - 1]).expand(n, hkv, top_k)
+    for _ in range(100):
+        assert torch.equal(paged.sparse_attend(*args, **kw)[1], want)
+
+
 @pytest.mark.parametrize("dtype,d,page,grp,top_k", [(torch.bfloat16, 128, 32, 2, 5), (torch.float16, 64, 64, 3, 3), (torch.bfloat16, 64, 128, 8, 2),
                                                     (torch.float16, 128, 16, 1, 1)])
 def test_sparse_by_page(paged, dtype, d, page, grp, top_k):

@@ -404,12 +404,14 @@ int mq_paged_reserve(const mq_page_table* t, const int* slots, const int* new_le
 int mq_paged_fork(const mq_paged_pool* pool, const mq_page_table* t, const int* parents, const int* children, int n,
                   cudaStream_t stream);
 /* Page src_pages[i] of `src` into page dst_pages[i] of `dst` (the same geometry
- * and type; it may be the same pool, as long as no page is both read and
- * written).  K, V and, when both pools have one, the index. */
+ * and type).  K, V and, when both pools have one, the index.  It may be the
+ * same pool, or another view of its pages, as long as no page is both read and
+ * written (checked on the device); pools that share memory in another way than
+ * page on page are refused. */
 int mq_paged_copy(const mq_paged_pool* src, const mq_paged_pool* dst, const int* src_pages, const int* dst_pages,
                   int n, int* status, void* workspace, size_t workspace_bytes, cudaStream_t stream);
-/* Every page in use, in ascending order, into pages 0, 1, ... of another pool;
- * out_table and out_refs (refs of dst->num_pages pages) name them there. */
+/* Every page in use, in ascending order, into pages 0, 1, ... of another pool,
+ * which shares no page with the first; out_table and out_refs (refs of dst->num_pages pages) name them there. */
 int mq_paged_compact(const mq_paged_pool* src, const mq_paged_pool* dst, const mq_page_table* t, int* out_table,
                      long long out_row_stride, int* out_refs, cudaStream_t stream);
 

@@ -267,6 +267,63 @@ Geo geo_of(const mq_paged_pool* s, const mq_paged_pool* d, bool index) {
     return g;
 }
 
+// How the pages of `b` lie on those of `a`, when both may be views of one storage: apart; a page p of `a` on page
+// p + *shift of `b` alone; or tangled (any other way, or not to be told).  The [page, head_dim] blocks of one side do
+// not overlap each other.
+enum Lie { APART, SHIFTED, TANGLED };
+Lie lie_of(const Side& a, int na, const Side& b, int nb, int layers, int heads, long long block, long long* shift) {
+    if (!a.base || !b.base) return APART;
+    const auto end = [&](const Side& s, int n, bool high) {   // the lowest byte, or the one after the highest
+        long long at = reinterpret_cast<long long>(s.base) + (high ? block : 0);
+        for (const long long x : {(n - 1) * s.page, (layers - 1) * s.layer, (heads - 1) * s.head})
+            if (high ? x > 0 : x < 0) at += x;
+        return at;
+    };
+    if (end(a, na, true) <= end(b, nb, false) || end(b, nb, true) <= end(a, na, false)) return APART;
+    const long long page = nb > 1 ? b.page : a.page;
+    if ((na > 1 && nb > 1 && a.page != b.page) || (layers > 1 && a.layer != b.layer) || (heads > 1 && a.head != b.head) ||
+        ((na > 1 || nb > 1) && page < block))
+        return TANGLED;
+    if (a.base == b.base) {
+        *shift = 0;
+        return SHIFTED;
+    }
+    if ((2ll * layers - 1) * (2ll * heads - 1) > 1 << 20) return TANGLED;
+    bool found = false;
+    for (int l = 1 - layers; l < layers; ++l)
+        for (int h = 1 - heads; h < heads; ++h) {
+            // a block of b less one of a: off + d pages, for d pages between them
+            const long long off = (b.base - a.base) + l * a.layer + h * a.head;
+            const long long d0 = na > 1 || nb > 1 ? -off / page : 0;
+            for (long long d = d0 - 1; d <= d0 + 1; ++d) {
+                const long long apart = off + d * page;
+                if (d <= -na || d >= nb || apart >= block || apart <= -block) continue;
+                if (found && *shift != d) return TANGLED;
+                found = true;
+                *shift = d;
+            }
+        }
+    return found ? SHIFTED : APART;
+}
+
+// The same for two pools: every tensor of one against those of the other.
+Lie lie_of(const Geo& g, int na, int nb, int page, long long* shift) {
+    const bool same = g.src[0].base == g.dst[0].base && g.src[1].base == g.dst[1].base;
+    bool found = false;
+    for (int i = 0; i < 3; ++i)
+        for (int j = 0; j < 3; ++j) {
+            if ((i == 2) != (j == 2) || (same && i != j)) continue;
+            long long d = 0;
+            const Lie lie = lie_of(g.src[i], na, g.dst[j], nb, g.layers, g.heads, i == 2 ? g.record : (long long)page * g.row_bytes, &d);
+            if (lie == TANGLED || (lie == SHIFTED && found && d != *shift)) return TANGLED;
+            if (lie == SHIFTED) {
+                found = true;
+                *shift = d;
+            }
+        }
+    return found ? SHIFTED : APART;
+}
+
 // Copies `bytes` (a multiple of 16) by one warp, eight 16-byte pieces in flight per lane.
 __device__ __forceinline__ void warp_copy(char* __restrict__ d, const char* __restrict__ s, int bytes, int lane) {
     int i = lane * 16;
@@ -383,9 +440,10 @@ __global__ void __launch_bounds__(MOVE_THREADS) fork_move_kernel(Geo g, Tab t, c
 }
 
 // ---- copy ----------------------------------------------------------------------------
+// `shared`: page p read is page p + shift written, where that is one of the dst_pages.
 __global__ void __launch_bounds__(PLAN_THREADS) copy_plan_kernel(const int* __restrict__ src, const int* __restrict__ dst,
-                                                                 int n, int src_pages, int dst_pages, int same, int page,
-                                                                 int* status, Plan pl) {
+                                                                 int n, int src_pages, int dst_pages, bool shared,
+                                                                 long long shift, int page, int* status, Plan pl) {
     pdl_wait();
     pdl_trigger();
     if (threadIdx.x == 0) pl.head[1] = 0;
@@ -401,9 +459,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) copy_plan_kernel(const int* __re
         pl.rows[i] = page;
     }
     bad = __syncthreads_or(bad);
-    if (!bad && same)
-        for (int i = threadIdx.x; i < n; i += PLAN_THREADS)
-            if (__ldcg(&pl.bits[src[i] >> 5]) >> (src[i] & 31) & 1u) bad = true;
+    if (!bad && shared)
+        for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
+            const long long d = src[i] + shift;
+            if (d >= 0 && d < dst_pages && __ldcg(&pl.bits[d >> 5]) >> (d & 31) & 1u) bad = true;
+        }
     bad = __syncthreads_or(bad);
     if (threadIdx.x == 0) {
         if (bad) note_status(status, MQ_ERR_BAD_PAGE);
@@ -514,14 +574,16 @@ int mq_paged_copy(const mq_paged_pool* src, const mq_paged_pool* dst, const int*
                   int* status, void* workspace, size_t workspace_bytes, cudaStream_t st) {
     if (!pool_ok(src) || !pool_ok(dst) || !same_geometry(src, dst) || n < 0 || (n && (!src_pages || !dst_pages)))
         return MQ_ERR_INVALID_ARGUMENT;
+    const Geo g = geo_of(src, dst, true);
+    long long shift = 0;
+    const Lie lie = lie_of(g, src->num_pages, dst->num_pages, src->page_size, &shift);
+    if (lie == TANGLED) return MQ_ERR_INVALID_ARGUMENT;
     if (!n) return MQ_OK;
     if (!workspace || workspace_bytes < mq_paged_workspace_bytes(dst->num_pages, n)) return MQ_ERR_WORKSPACE;
     const Plan pl = plan_of(workspace, dst->num_pages, n);
-    const int same = src->k == dst->k || src->v == dst->v;
     cudaError_t e = launch(copy_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, st, src_pages, dst_pages, n, src->num_pages,
-                           dst->num_pages, same, src->page_size, status, pl);
-    if (e == cudaSuccess)
-        e = launch(move_kernel, dim3(move_grid()), dim3(MOVE_THREADS), 0, st, geo_of(src, dst, true), pl);
+                           dst->num_pages, lie == SHIFTED, shift, src->page_size, status, pl);
+    if (e == cudaSuccess) e = launch(move_kernel, dim3(move_grid()), dim3(MOVE_THREADS), 0, st, g, pl);
     return done(e, "paged copy");
 }
 
@@ -529,13 +591,16 @@ int mq_paged_compact(const mq_paged_pool* src, const mq_paged_pool* dst, const m
                      long long out_row_stride, int* out_refs, cudaStream_t st) {
     if (!pool_ok(src) || !pool_ok(dst) || !same_geometry(src, dst) || !tab_ok(t, 0, false) || !out_table || !out_refs ||
         src->num_pages != t->num_pages || src->page_size != t->page_size || out_row_stride < t->cols ||
-        src->k == dst->k || src->v == dst->v || out_table == t->table || out_refs == t->refs)
+        out_table == t->table || out_refs == t->refs)
         return MQ_ERR_INVALID_ARGUMENT;
+    const Geo g = geo_of(src, dst, true);
+    long long shift = 0;
+    if (lie_of(g, src->num_pages, dst->num_pages, src->page_size, &shift) != APART) return MQ_ERR_INVALID_ARGUMENT;
     if (!t->workspace || t->workspace_bytes < mq_paged_workspace_bytes(t->num_pages, 0)) return MQ_ERR_WORKSPACE;
     const Plan pl = plan_of(t->workspace, t->num_pages, 0);
     cudaError_t e = launch(compact_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, st, tab_of(t), dst->num_pages, pl);
     if (e == cudaSuccess)
-        e = launch(compact_move_kernel, dim3(move_grid()), dim3(MOVE_THREADS), 0, st, geo_of(src, dst, true), tab_of(t),
+        e = launch(compact_move_kernel, dim3(move_grid()), dim3(MOVE_THREADS), 0, st, g, tab_of(t),
                    dst->num_pages, out_table, out_row_stride, out_refs, pl);
     return done(e, "paged compact");
 }

@@ -414,6 +414,34 @@ def test_copy_pages(paged):
         status.zero_()
 
 
+def test_copy_between_views(paged):
+    """Pools that are views of one storage: a page that is read and written is found under both of its numbers, and
+    pages past the smaller pool are no matter."""
+    g = gen(4)
+    k, v = normal(g, 4000, 1, 1, 16, 64), normal(g, 4000, 1, 1, 16, 64)
+    ix = torch.randint(-127, 127, (4000, 1, 1, 144), dtype=torch.int8, device="cuda", generator=g)
+    for lo, n, src, dst, ok in [
+        (0, 4, [3999, 5, 2000], [1, 0, 3], True), (0, 4, [3, 9], [2, 3], False), (0, 40, [33], [33], False),
+        (4, 3000, [4, 3999, 0], [1, 2, 2999], True), (4, 3000, [6, 7], [3, 9], False), (4, 3000, [0, 1, 2, 3], [3, 2, 1, 0], True),
+        (3990, 10, [3994], [4], False), (3990, 10, [4, 3989], [4, 5], True), (3990, 10, [0], [10], False),
+    ]:
+        want, status = [x.clone() for x in (k, v, ix)], dev([0])
+        if ok:
+            for x in want:
+                x[[lo + d for d in dst]] = x[src]
+        cut = slice(lo, lo + n)
+        paged.copy(k, v, dev(src), dev(dst), dst_k_pages=k[cut], dst_v_pages=v[cut], index=ix, dst_index=ix[cut], status=status)
+        assert status.item() == (0 if ok else 9)
+        assert all(torch.equal(a, b) for a, b in zip(want, (k, v, ix)))
+        paged.copy(k[cut], v[cut], dev(dst), dev(src), dst_k_pages=k, dst_v_pages=v, status=status.zero_())
+        assert status.item() == (0 if ok else 9)
+    # pools that share memory in another way, and pages gathered into a view of their own pool
+    with pytest.raises(RuntimeError, match="invalid argument"):
+        paged.copy(k, v, dev([0]), dev([9]), dst_k_pages=k[1:3999], dst_v_pages=v[2:4000])
+    with pytest.raises(RuntimeError, match="invalid argument"):
+        paged.compact(k, v, dev([[0]]), dev([1] * 4000), k[5:9], v[5:9], dev([[0]]), dev([0] * 4))
+
+
 def test_refused_tables_change_nothing(paged):
     page, d = 16, 64
     cache = paged.PagedKVCache(10, 6, 4, num_layers=1, num_kv_heads=1, head_dim=d, page_size=page)

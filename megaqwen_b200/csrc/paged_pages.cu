@@ -357,11 +357,12 @@ __device__ void move_units(const Geo& g, const Plan& pl, int moves, long long wi
 // ---- fork ----------------------------------------------------------------------------
 __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(Tab t, const int* __restrict__ parents,
                                                                  const int* __restrict__ children, int n, Plan pl) {
-    __shared__ unsigned bits[MAX_SLOTS / 32];
+    __shared__ unsigned bits[MAX_SLOTS / 32], looked[MAX_SLOTS / 32];
     __shared__ int sm[PLAN_WARPS], near_off[NEAR_OFF], near_ids[NEAR_IDS];
     pdl_wait();
     pdl_trigger();
     if (threadIdx.x == 0) pl.head[1] = 0;
+    for (int i = threadIdx.x; i < ceil_div(t.slots, 32); i += PLAN_THREADS) looked[i] = 0;   // (slots_ok synchronises)
     int* off = n <= NEAR_OFF ? near_off : pl.off;
     bool bad = !slots_ok(children, n, t.slots, bits);
     if (!bad) {   // the same for every thread
@@ -387,7 +388,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(Tab t, const in
                 part = len % t.page;
                 if (part) {
                     src = t.table[parents[i] * t.row + len / t.page];
-                    if (src < 0 || src >= t.pages) wrong |= 2;
+                    if (src < 0 || src >= t.pages || t.refs[src] <= 0) wrong |= 2;
                 }
             }
         }
@@ -399,6 +400,19 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(Tab t, const in
             off[i] = part > 0 ? copies + at : -1;
         }
         copies += sum;
+    }
+    // every full page of every parent in range and in use; a warp to a parent, and each parent once
+    for (int i = threadIdx.x >> 5; i < n; i += PLAN_WARPS) {
+        const int lane = threadIdx.x & 31, p = parents[i];
+        int first = 0;
+        if (lane == 0) first = !(atomicOr(&looked[p >> 5], 1u << (p & 31)) >> (p & 31) & 1u);
+        if (!__shfl_sync(0xffffffffu, first, 0)) continue;
+        const int full = min(t.lengths[p] / t.page, t.cols);   // (a length beyond the row is refused above)
+#pragma unroll 4
+        for (int c = lane; c < full; c += 32) {
+            const int g = t.table[p * t.row + c];
+            if (g < 0 || g >= t.pages || t.refs[g] <= 0) wrong |= 2;
+        }
     }
     const int any1 = __syncthreads_or(wrong & 1), any2 = __syncthreads_or(wrong & 2);
     if (any1 || any2) {
@@ -426,9 +440,8 @@ __global__ void __launch_bounds__(MOVE_THREADS) fork_move_kernel(Geo g, Tab t, c
         const int len = t.lengths[par], full = len / t.page, dst = pl.dst[i];
         int p = -1;
         if (c < full) {
-            p = t.table[par * t.row + c];
-            if (p >= 0 && p < t.pages) atomicAdd(&t.refs[p], 1);
-            else note_status(t.status, MQ_ERR_BAD_PAGE);
+            p = t.table[par * t.row + c];   // in range: the plan looked at it
+            atomicAdd(&t.refs[p], 1);
         } else if (c == full && dst >= 0) {
             p = dst;
             t.refs[p] = 1;

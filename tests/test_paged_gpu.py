@@ -491,6 +491,26 @@ def test_refused_tables_change_nothing(paged):
     assert same()
 
 
+def bad_rows(paged, run):
+    """A cache whose slot 1 (40 full pages and a part) holds pages that are out of range or not in use; run(cache) may
+    change nothing and leaves code 9."""
+    page = 16
+    for col, bad in ((0, -1), (0, 10 ** 6), (17, 80), (39, 75), (40, -5), (40, 76)):
+        cache = paged.PagedKVCache(80, 6, 48, num_layers=1, num_kv_heads=1, head_dim=64, page_size=page)
+        cache.reserve([0, 1], [20, 40 * page + 5])     # 2 + 41 pages; 43 and up are free
+        cache.check()
+        cache.page_table[1, col] = bad
+        before = [x.clone() for x in (cache.page_table, cache.lengths, cache.refs, cache.k_pages)]
+        run(cache)
+        with pytest.raises(RuntimeError, match="page number"):
+            cache.check()
+        assert all(torch.equal(a, b) for a, b in zip(before, (cache.page_table, cache.lengths, cache.refs, cache.k_pages))), (col, bad)
+
+
+def test_fork_of_bad_rows_changes_nothing(paged):
+    bad_rows(paged, lambda cache: cache.fork([0, 1, 1], [2, 3, 4]))
+
+
 # ---- attention ---------------------------------------------------------------------------------------------------------
 
 def check_attend(paged, p, hq, qlens, groups=None, prefix=None, layer=1, scale=None, q=None, std=2.0):

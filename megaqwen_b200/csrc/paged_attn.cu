@@ -74,24 +74,6 @@ __device__ __forceinline__ void mma_s8(int* d, const int* a, int b0, int b1) {
         : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void st_peer(uint32_t addr, uint32_t rank, uint32_t v) {
-    uint32_t at;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
-}
 
 // One head of a query in whole numbers, split by sign, by one warp; returns the unit.
 template <typename T, int D>
@@ -775,21 +757,7 @@ int run_select(const SelArgs& s, cudaStream_t st) {
     // a cluster to an item: doubled while all its CTAs have an SM each and a CTA keeps 256 pages or more
     unsigned ranks = 1;
     while (ranks < 8 && items * ranks * 2 <= sm_count() && s.cols >= 512 * (int)ranks) ranks *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)items * ranks);
-    cfg.blockDim = dim3(SEL_WARPS * 32);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = ranks;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, select_one_kernel<T, D>, s);
+    e = launch_cluster(select_one_kernel<T, D>, (unsigned)items * ranks, ranks, dim3(SEL_WARPS * 32), smem, st, s);
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "page selection");
 }
 

@@ -154,33 +154,58 @@ __device__ bool slots_ok(const int* slots, int n, int num_slots, unsigned* bits)
 constexpr int NEAR_OFF = 1024, NEAR_IDS = 2048;
 
 // ---- free ----------------------------------------------------------------------------
-// One CTA per sequence.  Each checks the whole list itself (it is short, and a
-// second launch would cost more), so a wrong list changes nothing anywhere.
-__global__ void __launch_bounds__(256) free_kernel(Tab t, const int* __restrict__ slots, int n) {
+// One cluster over all entries of the list's rows.  The counts are taken down first;
+// where one of them was not there to take (a page out of range, not in use, or held by
+// more of the rows than its count says), every count is put back and nothing else is
+// written.  Each CTA checks the list of slots itself (it is short).
+__global__ void __launch_bounds__(PLAN_THREADS) free_kernel(Tab t, const int* __restrict__ slots, int n) {
     __shared__ unsigned bits[MAX_SLOTS / 32];
+    __shared__ int wrong;
     pdl_wait();
     pdl_trigger();
-    if (!slots_ok(slots, n, t.slots, bits)) {
-        if (blockIdx.x == 0 && threadIdx.x == 0) note_status(t.status, MQ_ERR_BAD_SLOT);
+    const int ranks = (int)cluster_size(), rank = (int)cluster_rank();   // (the grid is one cluster)
+    if (threadIdx.x == 0) wrong = 0;
+    if (!slots_ok(slots, n, t.slots, bits)) {   // all CTAs alike
+        if (rank == 0 && threadIdx.x == 0) note_status(t.status, MQ_ERR_BAD_SLOT);
         return;
     }
-    const int s = slots[blockIdx.x];
-    int* row = t.table + s * t.row;
-    const int used = min(pages_of(t.lengths[s], t.page), t.cols);
-    __syncthreads();   // the length is read before thread 0 clears it
-    for (int c = threadIdx.x; c < t.cols; c += blockDim.x) {
-        if (c < used) {
+    if (ranks > 1) cluster_sync();   // every CTA runs and has its `wrong`: it may be written
+    // a warp to a sequence
+    const int lane = threadIdx.x & 31, warp = rank * PLAN_WARPS + (threadIdx.x >> 5), warps = ranks * PLAN_WARPS;
+    bool bad = false;
+    for (int i = warp; i < n; i += warps) {
+        const int s = slots[i], used = min(pages_of(t.lengths[s], t.page), t.cols);
+        const int* row = t.table + s * t.row;
+#pragma unroll 4
+        for (int c = lane; c < used; c += 32) {
             const int p = row[c];
-            if (p < 0 || p >= t.pages) {
-                note_status(t.status, MQ_ERR_BAD_PAGE);
-            } else if (atomicSub(&t.refs[p], 1) <= 0) {
-                atomicAdd(&t.refs[p], 1);
-                note_status(t.status, MQ_ERR_BAD_PAGE);
+            if (p < 0 || p >= t.pages || atomicSub(&t.refs[p], 1) <= 0) bad = true;
+        }
+    }
+    bad = __syncthreads_or(bad);
+    if (ranks > 1) {
+        if (bad && threadIdx.x == 0)
+            for (int r = 0; r < ranks; ++r) st_peer(smem_u32(&wrong), r, 1u);
+        __syncwarp();
+        cluster_sync();   // also orders the counts taken before those put back
+        bad = *(volatile int*)&wrong;
+    }
+    if (bad) {
+        if (rank == 0 && threadIdx.x == 0) note_status(t.status, MQ_ERR_BAD_PAGE);
+        for (int i = warp; i < n; i += warps) {
+            const int s = slots[i], used = min(pages_of(t.lengths[s], t.page), t.cols);
+            for (int c = lane; c < used; c += 32) {
+                const int p = t.table[s * t.row + c];
+                if (p >= 0 && p < t.pages) atomicAdd(&t.refs[p], 1);
             }
         }
-        row[c] = -1;
+        return;
     }
-    if (threadIdx.x == 0) t.lengths[s] = 0;
+    for (int i = warp; i < n; i += warps) {
+        const int s = slots[i];
+        for (int c = lane; c < t.cols; c += 32) t.table[s * t.row + c] = -1;
+        if (lane == 0) t.lengths[s] = 0;
+    }
 }
 
 // ---- reserve -------------------------------------------------------------------------
@@ -557,7 +582,9 @@ size_t mq_paged_workspace_bytes(int num_pages, int n) {
 int mq_paged_free(const mq_page_table* t, const int* slots, int n, cudaStream_t st) {
     if (!tab_ok(t, n, true) || (n && !slots)) return MQ_ERR_INVALID_ARGUMENT;
     if (!n) return MQ_OK;
-    return done(launch(free_kernel, dim3(n), dim3(256), 0, st, tab_of(t), slots, n), "paged free");
+    unsigned ranks = 1;   // a warp to a sequence; 64 sequences take the same time with 1, 2 and 8 CTAs
+    while (ranks < 8 && (int)ranks * PLAN_WARPS < n) ranks *= 2;
+    return done(launch_cluster(free_kernel, ranks, ranks, dim3(PLAN_THREADS), 0, st, tab_of(t), slots, n), "paged free");
 }
 
 int mq_paged_reserve(const mq_page_table* t, const int* slots, const int* new_lengths, int n, cudaStream_t st) {

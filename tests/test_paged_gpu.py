@@ -511,6 +511,33 @@ def test_fork_of_bad_rows_changes_nothing(paged):
     bad_rows(paged, lambda cache: cache.fork([0, 1, 1], [2, 3, 4]))
 
 
+def test_free_of_bad_rows_changes_nothing(paged):
+    bad_rows(paged, lambda cache: cache.free([0, 1]))
+
+
+def test_free_of_many(paged):
+    """Lists from one to several hundred sequences (more than one CTA), pages shared by all of them; a page held by more of
+    the rows than its count says."""
+    page, slots = 16, 400
+    cache = paged.PagedKVCache(2000, slots, 40, num_layers=1, num_kv_heads=1, head_dim=64, page_size=page)
+    for n in (1, 31, 32, 33, 64, 200, 399):
+        cache.reserve([0], [30 * page + 3])
+        kids = list(range(1, n + 1)) if n < slots - 1 else list(range(1, slots))
+        cache.fork([0] * len(kids), kids)
+        cache.reserve(kids[::2], [30 * page + 3 + 17 * (i % 5) for i in range(len(kids[::2]))])
+        cache.check()
+        before = [x.clone() for x in (cache.page_table, cache.lengths, cache.refs)]
+        cache.refs[cache.page_table[0, 7].long()] = n      # n + 1 rows hold it
+        cache.free([0] + kids)
+        with pytest.raises(RuntimeError, match="page number"):
+            cache.check()
+        cache.refs[cache.page_table[0, 7].long()] = n + 1
+        assert all(torch.equal(a, b) for a, b in zip(before, (cache.page_table, cache.lengths, cache.refs)))
+        cache.free([0] + kids)
+        cache.check()
+        assert (cache.page_table == -1).all() and not cache.lengths.any() and not cache.refs.any()
+
+
 # ---- attention ---------------------------------------------------------------------------------------------------------
 
 def check_attend(paged, p, hq, qlens, groups=None, prefix=None, layer=1, scale=None, q=None, std=2.0):

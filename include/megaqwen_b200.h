@@ -356,7 +356,10 @@ int mq_decode_batch(const mq_decode_batch_params* params, cudaStream_t stream);
  *
  * Nothing here synchronises or allocates.  Arguments that live on the device
  * are checked there: `status` (device int32, optional) keeps the first error
- * code, and a call whose arguments are wrong changes none of the tables.
+ * code, and a call whose arguments are wrong changes none of the tables (free,
+ * reserve and fork check the rows that they read, too).  Attention reads a wrong
+ * slot, length or position as an empty sequence, and leaves out the positions of
+ * a page that is out of range.
  * Workspaces hold nothing between calls; calls that overlap on the GPU need
  * their own. */
 enum { MQ_BF16 = 0, MQ_FP16 = 1, MQ_FP32 = 2 };

@@ -4,7 +4,7 @@
 // Work: items of (group, kv head, 256 query rows) x 128-key tiles, laid end to
 // end and cut into equal runs, one per CTA (one CTA per SM).  Every row sees
 // every key of the prefix (the schedule ends it before the first query token),
-// so there is no mask but the end of the last tile.
+// so there is no mask but the end of the last tile (and pages that are out of range).
 //
 // A CTA runs two streams, A and B, each with its own Q tile (128 rows), its own
 // S / P buffer and its own O accumulator in TMEM (4 x 128 columns):
@@ -211,6 +211,11 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
         x += left;
         return e;
     };
+    auto row_of = [&](const PfxSeg& e) -> const int* {
+        int b = s.gs[e.g];   // any member's row of the table will do; one without query tokens may have none
+        while (q_start(a, b + 1) == q_start(a, b)) ++b;
+        return a.table + __ldg(a.slots + b) * a.table_row;
+    };
     auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
         const long long t0 = clock64();
         while (!mbar_try_wait(bar, parity)) {
@@ -235,9 +240,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
         for (uint32_t x = x0; ok && x < xe;) {
             const PfxSeg e = segment(x);
             if (e.n <= 0) continue;
-            int b = s.gs[e.g];   // any member's row of the table will do; one without query tokens may have none
-            while (q_start(a, b + 1) == q_start(a, b)) ++b;
-            const int* row = a.table + __ldg(a.slots + b) * a.table_row;
+            const int* row = row_of(e);
             const int last = s.eff[e.g] - 1;
             // past the end of the prefix the last page is loaded again: its scores are masked, and its
             // values (not stale shared memory) meet the zero weights
@@ -248,7 +251,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
                 if (j + 1 < e.n) next = look(j + 1);
                 if (lane < chunks && (pid < 0 || pid >= a.pool.pages)) {
                     note_status(a.status, MQ_ERR_BAD_PAGE);
-                    pid = a.pool.pages;   // outside the map: zeros
+                    pid = a.pool.pages;   // outside the map: zeros (and its scores are masked)
                 }
                 const int st = c & 1;
                 bool here = c < 2 || wait(&empty[st], ((c >> 1) - 1) & 1);
@@ -414,17 +417,24 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
             for (int j = 0; j < mine; ++j, ++ns) {
                 float tmax = -INFINITY;
                 const int t = e.t0 + (e.two ? j : 2 * j + q);
+                // the tile's pages that are out of range (looked up while its scores are on their way)
+                unsigned none;
+                {
+                    const int pid = __ldg(row_of(e) + min(t * (PK / page) + min(lane, PK / page - 1), s.eff[e.g] - 1));
+                    none = __ballot_sync(0xffffffffu, pid < 0 || pid >= a.pool.pages);
+                }
                 if (got(&s_full[q], ns & 1)) {
                     tc_fence_after();
                     const int valid = s.eff[e.g] * page - t * PK - hh * 64;
-                    // the end of the prefix: scores past it are set to minus infinity in TMEM
-                    if (valid < 64) {
+                    // the end of the prefix, and pages that are not there: their scores are set to minus infinity in TMEM
+                    if (valid < 64 || none) {
 #pragma unroll 1
                         for (int i = 0; i < 64; i += 32) {
                             float sv[32];
                             tmem_ld32(sa + i, sv);
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) sv[k] = i + k < valid ? sv[k] : -INFINITY;
+                            for (int k = 0; k < 32; ++k)
+                                sv[k] = i + k < valid && !(none >> ((hh * 64 + i + k) >> a.pool.shift) & 1) ? sv[k] : -INFINITY;
                             tmem_st32(sa + i, sv);
                         }
                     }

@@ -20,8 +20,9 @@ synchronises, and outputs come from the current stream's allocator):
 ``sparse_attend``  attention over the pages that a cheap score selects
 
 Arguments that live on the GPU are checked there: a wrong slot, page or
-position writes its code to ``status`` (int32 ``[1]``, if given), changes no
-table, and reads as an empty sequence.  :class:`PagedKVCache` holds the tensors
+position writes its code to ``status`` (int32 ``[1]``, if given) and changes no
+table; attention reads a wrong slot or position as an empty sequence and leaves
+out the positions of a page that is out of range.  :class:`PagedKVCache` holds the tensors
 and raises from :meth:`PagedKVCache.check`.
 """
 from __future__ import annotations

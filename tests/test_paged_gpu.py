@@ -692,6 +692,29 @@ def test_attend_wrong_tables(paged):
     assert code == 1 and not out.any()
 
 
+@pytest.mark.parametrize("d,page,hkv,grp,members,pages", [(128, 16, 2, 2, 40, 21), (64, 64, 1, 4, 9, 5), (128, 128, 1, 8, 30, 3),
+                                                          (64, 32, 2, 1, 3, 9)])
+def test_attend_bad_shared_pages(paged, d, page, hkv, grp, members, pages):
+    """A page out of range is left out: its positions count for no row, whichever kernel reads the prefix."""
+    lens = [pages * page + 1 + 5 * b for b in range(members)]
+    p = Pool(lens, page, hkv, d, torch.bfloat16, seed=pages, share={b: (0, pages) for b in range(1, members)})
+    q = normal(p.g, members, hkv * grp, d, std=2.0)
+    for bad in ([0], [pages - 1], [1, 2], list(range(pages))):
+        table = p.table.clone()
+        for i, col in enumerate(bad):
+            table[:members + 1, col] = (-1, p.k.shape[0], 10 ** 9)[i % 3]
+        for kw in ({}, dict(group_starts=dev([0, members]), prefix_pages=dev([pages]))):
+            status = dev([0])
+            out = paged.attend(q, p.k, p.v, table, p.lengths, dev(p.slots), layer=1, status=status, **kw)
+            assert status.item() == 9
+            for b in range(0, members, 4):
+                k, v = p.kv(b, 1)
+                seen = torch.ones(lens[b], dtype=torch.bool, device="cuda")
+                for col in bad:
+                    seen[col * page:(col + 1) * page] = False
+                close(out[b], softmax_rows(q[b], k, v, seen, 1.0 / math.sqrt(d)), v.abs().max().item())
+
+
 def test_attend_past_32_bits(paged):
     """Pages whose offsets in the pool pass 2^31 elements."""
     page, layers, hkv, d = 128, 28, 8, 128

@@ -293,10 +293,11 @@ Tensor rope_append(Tensor q, Tensor k, Tensor v, Tensor k_pages, Tensor v_pages,
     return out;
 }
 
-// q as the kernels read it: 16-byte pieces of a head row
+// q as the kernels read it: 16-byte pieces of a head row (a contiguous q may start anywhere, so a copy and not
+// contiguous(), which would hand it back)
 Tensor pieces(const Tensor& q) {
     const bool ok = (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15) == 0 && q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0;
-    return ok ? q : q.contiguous();
+    return ok ? q : q.clone(at::MemoryFormat::Contiguous);
 }
 
 int q_heads(const Tensor& q, const mq_paged_pool& pool) {

@@ -664,6 +664,27 @@ def test_attend_strided_and_layers(paged):
     assert torch.equal(paged.attend(odd[..., 1:d + 1], p.k, p.v, p.table, p.lengths, dev(p.slots), layer=2), b)
 
 
+def test_contiguous_q_at_odd_offsets(paged):
+    """A contiguous q whose first element is on no 16-byte boundary, and one token whose strides are odd."""
+    page, hkv, d = 16, 2, 64
+    p = Pool([70, 33], page, hkv, d, torch.bfloat16, seed=1)
+    idx = full_index(p, 2, hkv, d)
+    q = normal(p.g, 2, 4, d)
+    want = check_attend(paged, p, 4, [1, 1], q=q)
+    pos, slots = dev([69, 32]), dev(p.slots)
+    chosen, sel = paged.sparse_attend(q, p.k, p.v, idx, p.table, slots, pos, layer=1, top_k=3)
+    flat = torch.zeros(q.numel() + 8, dtype=q.dtype, device="cuda")
+    for lo in (1, 3, 4):
+        x = flat[lo:lo + q.numel()].view(q.shape)
+        x.copy_(q)
+        assert x.is_contiguous() and x.data_ptr() % 16
+        assert torch.equal(paged.attend(x, p.k, p.v, p.table, p.lengths, slots, layer=1), want)
+        out = paged.sparse_attend(x, p.k, p.v, idx, p.table, slots, pos, layer=1, top_k=3)
+        assert torch.equal(out[0], chosen) and torch.equal(out[1], sel)
+    one = q[1:].as_strided((1, 4, d), (5 * d + 1, d, 1))
+    assert torch.equal(paged.attend(one, p.k, p.v, p.table, p.lengths, slots[1:], layer=1), want[1:])
+
+
 def test_attend_wrong_tables(paged):
     page = 16
     p = Pool([40, 20, 30], page, 1, 64, torch.bfloat16, seed=6)

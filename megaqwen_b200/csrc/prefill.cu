@@ -32,10 +32,19 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-// K-major bf16 matrix [rows, cols] with row stride ld (elements); box 64 x 128,
-// 128-byte swizzle (matches sw128_kmajor_desc).
+// The encoder needs the device's context on the calling thread.  A thread whose
+// first CUDA call this is has none (cudaGetDevice alone does not bind it).
+template <typename F>
+bool encoded(F encode) {
+    if (encode() == CUDA_SUCCESS) return true;
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && encode() == CUDA_SUCCESS;
+}
+
 }  // namespace
 
+// K-major bf16 matrix [rows, cols] with row stride ld (elements); box 64 x 128,
+// 128-byte swizzle (matches sw128_kmajor_desc).
 bool make_tmap(CUtensorMap* map, const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows) {
     auto fn = encode_fn();
     if (!fn) return false;
@@ -43,9 +52,11 @@ bool make_tmap(CUtensorMap* map, const void* ptr, uint64_t rows, uint64_t cols, 
     cuuint64_t strides[1] = {ld * 2};
     cuuint32_t box[2] = {GEMM_BK, box_rows};
     cuuint32_t estr[2] = {1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return encoded([&] {
+        return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
 }
 
 // 16-bit tensor of up to five dimensions (innermost first, strides in bytes
@@ -55,10 +66,12 @@ bool make_tmap_nd(CUtensorMap* map, const void* ptr, bool bf16, int rank, const 
     auto fn = encode_fn();
     if (!fn) return false;
     const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank,
-              const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return encoded([&] {
+        return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank,
+                  const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
 }
 
 namespace {

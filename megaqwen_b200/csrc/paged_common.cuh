@@ -75,21 +75,31 @@ inline int sm_count() {
     return sms[dev] > 0 ? sms[dev] : 148;
 }
 
-// Raises a kernel's shared-memory limit where it is not high enough yet (the
-// driver call is worth avoiding in a call of a few microseconds).  `set` is the
-// kernel's own record, one entry per device.
+// Raises a kernel's shared-memory limit to the largest that the device allows, on
+// its first use there (the driver call is worth avoiding in a call of a few
+// microseconds).  `set` is the kernel's own record, one entry per device: the limit
+// that is in place.  Every thread that gets to set it sets the same, so it does not
+// matter who is first.
 struct SmemLimit {
     std::atomic<int> bytes[64];
 };
 template <typename K>
 cudaError_t allow_smem(K kernel, size_t bytes, SmemLimit& set) {
-    int dev = 0;
-    const cudaError_t e = cudaGetDevice(&dev);
+    int dev = 0, most = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    if (dev < 64 && set.bytes[dev].load(std::memory_order_relaxed) >= (int)bytes) return cudaSuccess;
-    const cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (r == cudaSuccess && dev < 64) set.bytes[dev].store((int)bytes, std::memory_order_relaxed);
-    return r;
+    if (dev < 64) most = set.bytes[dev].load(std::memory_order_relaxed);
+    if (!most) {
+        cudaFuncAttributes at;
+        e = cudaFuncGetAttributes(&at, kernel);
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+        if (e != cudaSuccess) return e;
+        most -= (int)at.sharedSizeBytes;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) set.bytes[dev].store(most, std::memory_order_relaxed);
+    }
+    return bytes <= (size_t)most ? cudaSuccess : cudaErrorInvalidValue;
 }
 
 // Thread-block clusters of the one-dimensional grids here.

@@ -89,5 +89,11 @@ def test_a_thread_without_a_context():
     run(1)
 
 
+def test_sizes_that_differ_at_once():
+    """What is set up on a kernel's first use must not depend on which of several sizes is first."""
+    for _ in range(3):
+        run(8)
+
+
 if __name__ == "__main__":
     main(int(sys.argv[1]))

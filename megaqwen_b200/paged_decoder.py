@@ -15,6 +15,8 @@ cache operators' type.
 """
 from __future__ import annotations
 
+from collections import Counter
+from itertools import count
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -43,6 +45,11 @@ class PagedDecoder:
 
     ``sparse_pages``: decode steps read at most this many pages per query and
     kv head (chosen by score); ``None`` reads everything.
+
+    The host keeps account of lengths and pages, so a call that the cache would
+    refuse raises before anything is changed on either side.  :meth:`check`
+    raises what the device found all the same (the cache used directly, say) and
+    takes lengths and pages over from there.
     """
 
     def __init__(self, weights: Qwen3Weights, num_pages: int, max_seqs: int, max_seq_len: int = 4096, page_size: int = 64,
@@ -62,13 +69,40 @@ class PagedDecoder:
         self.cache = PagedKVCache(num_pages, max_seqs, -(-max_seq_len // page_size), num_layers=len(self.layers),
                                   page_size=page_size, device=dev, index=sparse_pages is not None)
         self.max_seq_len = max_seq_len
-        self.lengths = [0] * max_seqs
-        self._family: List[Optional[Tuple[int, int]]] = [None] * max_seqs   # (family, pages it shares)
         self._families = 0
+        self._take_over()
+
+    def _take_over(self) -> None:
+        """Lengths and pages as the device has them (synchronises)."""
+        c = self.cache
+        self.lengths: List[int] = c.lengths.tolist()
+        table = c.page_table.tolist()
+        # each sequence's pages, and how many sequences hold a page; pages handed out from here on get names of their own
+        self._pages = [row[:-(-n // c.page_size)] for row, n in zip(table, self.lengths)]
+        self._held = Counter(p for row in self._pages for p in row)
+        self._free_pages = c.free_pages()
+        self._names = count(c.refs.numel())
+        self._family: List[Optional[Tuple[int, int]]] = [None] * len(self.lengths)   # (family, pages it shares)
         self._plan = None
 
-    def _ints(self, x) -> torch.Tensor:
-        return torch.tensor(x, dtype=torch.int32, device=self.embed.device)
+    def _grow(self, slots: Sequence[int], lengths: Sequence[int]) -> None:
+        """Accounts for sequences that grow; raises without a change where the pages do not suffice."""
+        need = [-(-n // self.cache.page_size) - len(self._pages[s]) for s, n in zip(slots, lengths)]
+        if sum(need) > self._free_pages:
+            raise RuntimeError("paged cache: not enough free pages")
+        self._free_pages -= sum(need)
+        for s, n, k in zip(slots, lengths, need):
+            new = [next(self._names) for _ in range(k)]
+            self._pages[s] += new
+            self._held.update(new)
+            self.lengths[s] = n
+
+    def _known(self, slots: Sequence[int]) -> None:
+        if len(set(slots)) != len(slots) or any(not 0 <= s < len(self.lengths) for s in slots):
+            raise ValueError("a sequence is named twice or out of range")
+
+    def _ints(self, x, dtype: torch.dtype = torch.int32) -> torch.Tensor:
+        return torch.as_tensor(x, dtype=dtype, device=self.embed.device)
 
     def _forward(self, ids, slots, positions, attend) -> torch.Tensor:
         """Hidden states of the tokens after the final norm; ``attend(layer, q)`` reads the cache."""
@@ -93,11 +127,12 @@ class PagedDecoder:
     @torch.no_grad()
     def prefill(self, slot: int, ids: Sequence[int]) -> torch.Tensor:
         """Appends a prompt (or a further piece of one) to a sequence; fp32 logits of its last token."""
+        self._known([slot])
         n, start = len(ids), self.lengths[slot]
         if n < 1 or start + n > self.max_seq_len:
             raise ValueError("prompt is empty or exceeds max_seq_len")
+        self._grow([slot], [start + n])
         self.cache.reserve([slot], [start + n])
-        self.lengths[slot] = start + n
         one = self._ints([slot])
         starts = self._ints([0, n])
         h = self._forward(torch.as_tensor(ids, device=self.embed.device).long(), one.expand(n).contiguous(),
@@ -107,18 +142,37 @@ class PagedDecoder:
 
     def fork(self, parent: int, children: Sequence[int]) -> None:
         """Empty slots become copies of a sequence; decode steps read what they share once for all of them."""
-        self.cache.fork([parent] * len(children), list(children))
-        shared = (self._families, self.lengths[parent] // self.cache.page_size)
-        self._families += 1
+        children = list(children)
+        self._known([parent, *children])
+        if any(self.lengths[s] for s in children):
+            raise ValueError("a child must be an empty slot")
+        full, part = divmod(self.lengths[parent], self.cache.page_size)
+        if part and len(children) > self._free_pages:
+            raise RuntimeError("paged cache: not enough free pages")
+        if not children:
+            return
+        self.cache.fork([parent] * len(children), children)
+        shared = self._pages[parent][:full]
+        for s in children:
+            self._pages[s] = list(shared)
+            self._held.update(shared)
+        self._grow(children, [self.lengths[parent]] * len(children))
         for s in [parent, *children]:
-            self.lengths[s] = self.lengths[parent]
-            self._family[s] = shared
+            self._family[s] = (self._families, full)
+        self._families += 1
         self._plan = None
 
     def free(self, slots: Sequence[int]) -> None:
-        self.cache.free(list(slots))
+        slots = list(slots)
+        self._known(slots)
+        self.cache.free(slots)
         for s in slots:
-            self.lengths[s], self._family[s] = 0, None
+            for p in self._pages[s]:
+                self._held[p] -= 1
+                if not self._held[p]:
+                    del self._held[p]
+                    self._free_pages += 1
+            self._pages[s], self.lengths[s], self._family[s] = [], 0, None
         self._plan = None
 
     def _groups(self, slots):
@@ -139,7 +193,7 @@ class PagedDecoder:
             else:
                 at = len(order)
             groups = (self._ints(starts + [at]), self._ints(pages)) if starts else (None, None)
-            back = torch.tensor(order, device=self.embed.device)
+            back = self._ints(order, torch.int64)
             self._plan = (key, order, back, self._ints([slots[i] for i in order]), *groups)
         return self._plan[1:]
 
@@ -147,13 +201,13 @@ class PagedDecoder:
     def step(self, slots: Sequence[int], tokens: torch.Tensor) -> torch.Tensor:
         """One token for each of the named sequences: fp32 logits ``[len(slots), vocab]``.  No host synchronisation."""
         slots = list(slots)
-        if len(set(slots)) != len(slots) or any(self.lengths[s] >= self.max_seq_len for s in slots):
-            raise ValueError("a sequence is named twice or full")
+        self._known(slots)
+        if any(self.lengths[s] >= self.max_seq_len for s in slots):
+            raise ValueError("a sequence is full")
+        self._grow(slots, [self.lengths[s] + 1 for s in slots])
         order, back, dev_slots, starts, pages = self._groups(slots)
-        positions = self._ints([self.lengths[slots[i]] for i in order])
+        positions = self._ints([self.lengths[slots[i]] - 1 for i in order])
         self.cache.reserve(dev_slots, positions + 1)
-        for s in slots:
-            self.lengths[s] += 1
         if self.sparse_pages is None:
             def attend(li, q):
                 return self.cache.attend(li, q, dev_slots, group_starts=starts, prefix_pages=pages)
@@ -166,5 +220,9 @@ class PagedDecoder:
         return self._logits(out)
 
     def check(self) -> None:
-        """Raises if a device-side check of the cache failed (synchronises)."""
-        self.cache.check()
+        """Raises if a device-side check failed, with lengths and pages then as the device has them (synchronises)."""
+        try:
+            self.cache.check()
+        except RuntimeError:
+            self._take_over()
+            raise

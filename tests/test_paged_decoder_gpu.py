@@ -69,6 +69,60 @@ def test_sparse_steps_of_every_page_match_dense():
     assert torch.isfinite(got[2]).all()
 
 
+def decoder(**kw):
+    from megaqwen_b200.paged_decoder import PagedDecoder
+    return PagedDecoder(make_weights(LAYERS).to("cuda"), **{**dict(num_pages=6, max_seqs=5, max_seq_len=256, page_size=16), **kw})
+
+
+def prompt_of(n, seed):
+    return seeded_prompt(n, seed=seed).tolist()
+
+
+def test_refused_calls_leave_the_decoder_as_it_was():
+    """Not enough pages, slots that are not empty: what follows is right."""
+    a, b = prompt_of(60, 4), prompt_of(40, 5)
+    dec = decoder()
+    dec.prefill(0, a)                       # four of six pages
+    with pytest.raises(RuntimeError, match="free pages"):
+        dec.prefill(1, b)
+        dec.check()
+    with pytest.raises((RuntimeError, ValueError), match="free pages|empty slot|not empty"):
+        dec.fork(0, [1, 2, 3])              # a part page each
+        dec.check()
+    close(dec.prefill(1, b[:32]), oracle_with(b[:32])[1])
+    with pytest.raises((RuntimeError, ValueError), match="empty"):
+        dec.fork(0, [1])
+        dec.check()
+    with pytest.raises(RuntimeError, match="free pages"):
+        dec.step([1], torch.tensor([b[32]]))    # a seventh page
+        dec.check()
+    oracle, _ = oracle_with(a)
+    close(dec.step([0], torch.tensor([7]))[0], oracle.decode_step(7, len(a)))
+    assert dec.lengths == dec.cache.lengths.tolist() == [61, 32, 0, 0, 0]
+    dec.free([0])
+    close(dec.prefill(1, b[32:]), oracle_with(b)[1])
+    dec.free([1])
+    dec.check()
+    assert dec.cache.free_pages() == 6
+
+
+def test_errors_found_on_the_device():
+    """Pages taken behind the decoder's back: its calls are refused there, and after check() it knows how things stand."""
+    b = prompt_of(40, 5)
+    dec = decoder()
+    dec.cache.reserve([3], [70])
+    dec.prefill(1, b)
+    with pytest.raises(RuntimeError, match="free pages"):
+        dec.check()
+    assert dec.lengths == [0, 0, 0, 70, 0]
+    dec.free([3])
+    close(dec.prefill(1, b), oracle_with(b)[1])
+    dec.fork(1, [0, 2])
+    oracle, _ = oracle_with(b)
+    close(dec.step([2, 0], torch.tensor([9, 9]))[1], oracle.decode_step(9, 40))
+    dec.check()
+
+
 def test_example_runs(capsys):
     spec = importlib.util.spec_from_file_location("shared_prompt", ROOT / "examples" / "shared_prompt.py")
     mod = importlib.util.module_from_spec(spec)

@@ -47,8 +47,11 @@ sparse_attend = _C.paged_sparse_attend
 
 INDEX_PAD = 16   # bytes of an index record after the two bounds: the exponent and padding
 
+BAD_TOKEN = 4
 STATUS = {
     1: "starts out of order",
+    3: "a wait of a kernel ran out",
+    BAD_TOKEN: "token id out of range",
     5: "position out of range",
     8: "slot out of range, named twice or not empty",
     9: "page number out of range or in the wrong state",

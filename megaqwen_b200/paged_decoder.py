@@ -22,7 +22,7 @@ from typing import List, Optional, Sequence, Tuple
 import torch
 import torch.nn.functional as F
 
-from .paged import PagedKVCache
+from .paged import BAD_TOKEN, PagedKVCache
 from .weights import (HEAD_DIM, NUM_KV_HEADS, NUM_Q_HEADS, Q_SIZE, KV_SIZE, RMS_NORM_EPS, Qwen3Weights, rope_tables)
 
 
@@ -104,6 +104,23 @@ class PagedDecoder:
     def _ints(self, x, dtype: torch.dtype = torch.int32) -> torch.Tensor:
         return torch.as_tensor(x, dtype=dtype, device=self.embed.device)
 
+    def _tokens(self, ids, n: int) -> torch.Tensor:
+        """n token ids on the device.  One out of range raises if it is known on the host; on the device it is read as
+        the nearest one and :meth:`check` raises."""
+        ids = torch.as_tensor(ids)
+        if ids.numel() != n or ids.is_floating_point():
+            raise ValueError("there must be one token id for each sequence")
+        ids, top = ids.reshape(-1), self.embed.shape[0] - 1
+        if ids.device.type == "cpu":
+            if n and not 0 <= int(ids.min()) <= int(ids.max()) <= top:
+                raise ValueError("token id out of range")
+            return self._ints(ids, torch.int64)
+        ids = ids.long()
+        safe = ids.clamp(0, top)
+        status = self.cache.status
+        status.copy_(torch.where((safe != ids).any() & (status == 0), BAD_TOKEN, status))
+        return safe
+
     def _forward(self, ids, slots, positions, attend) -> torch.Tensor:
         """Hidden states of the tokens after the final norm; ``attend(layer, q)`` reads the cache."""
         h = self.embed[ids].float()
@@ -131,11 +148,12 @@ class PagedDecoder:
         n, start = len(ids), self.lengths[slot]
         if n < 1 or start + n > self.max_seq_len:
             raise ValueError("prompt is empty or exceeds max_seq_len")
+        ids = self._tokens(ids, n)
         self._grow([slot], [start + n])
         self.cache.reserve([slot], [start + n])
         one = self._ints([slot])
         starts = self._ints([0, n])
-        h = self._forward(torch.as_tensor(ids, device=self.embed.device).long(), one.expand(n).contiguous(),
+        h = self._forward(ids, one.expand(n).contiguous(),
                           torch.arange(start, start + n, dtype=torch.int32, device=self.embed.device),
                           lambda li, q: self.cache.attend(li, q, one, q_starts=starts))
         return self._logits(h[-1:])[0]
@@ -204,6 +222,9 @@ class PagedDecoder:
         self._known(slots)
         if any(self.lengths[s] >= self.max_seq_len for s in slots):
             raise ValueError("a sequence is full")
+        tokens = self._tokens(tokens, len(slots))
+        if not slots:
+            return self.embed.new_empty((0, self.embed.shape[0]), dtype=torch.float32)
         self._grow(slots, [self.lengths[s] + 1 for s in slots])
         order, back, dev_slots, starts, pages = self._groups(slots)
         positions = self._ints([self.lengths[slots[i]] - 1 for i in order])
@@ -214,7 +235,7 @@ class PagedDecoder:
         else:
             def attend(li, q):
                 return self.cache.sparse_attend(li, q, dev_slots, positions, self.sparse_pages)[0]
-        h = self._forward(tokens.to(self.embed.device).long()[back], dev_slots, positions, attend)
+        h = self._forward(tokens[back], dev_slots, positions, attend)
         out = torch.empty_like(h)
         out[back] = h
         return self._logits(out)

@@ -123,6 +123,33 @@ def test_errors_found_on_the_device():
     dec.check()
 
 
+def test_tokens_and_slots_that_are_wrong():
+    b = prompt_of(20, 6)
+    dec = decoder()
+    vocab = dec.embed.shape[0]
+    for bad in ([-1], [vocab], []):
+        with pytest.raises(ValueError):
+            dec.prefill(0, bad)
+    for slot in (-1, 5):
+        with pytest.raises(ValueError):
+            dec.prefill(slot, b)
+    dec.prefill(0, b)
+    for slots, tokens in (([0], []), ([0], [1, 2]), ([0, 0], [1, 2]), ([-1], [1]), ([9], [1]), ([0], [vocab]), ([0], [0.5])):
+        with pytest.raises(ValueError):
+            dec.step(slots, torch.tensor(tokens))
+    for call in (lambda: dec.free([0, 0]), lambda: dec.free([7]), lambda: dec.fork(9, [1]), lambda: dec.fork(0, [1, 1]), lambda: dec.fork(0, [0])):
+        with pytest.raises(ValueError):
+            call()
+    assert dec.step([], torch.tensor([], dtype=torch.long)).shape == (0, vocab)
+    oracle, _ = oracle_with(b)
+    close(dec.step([0], torch.tensor([3]))[0], oracle.decode_step(3, 20))
+    dec.check()
+    dec.step([0], torch.tensor([vocab], device="cuda"))      # known on the device alone
+    with pytest.raises(RuntimeError, match="token"):
+        dec.check()
+    dec.check()
+
+
 def test_example_runs(capsys):
     spec = importlib.util.spec_from_file_location("shared_prompt", ROOT / "examples" / "shared_prompt.py")
     mod = importlib.util.module_from_spec(spec)

@@ -59,6 +59,14 @@ STATUS = {
 }
 
 
+def to_device(x, dtype: torch.dtype, device) -> torch.Tensor:
+    """x (a list, or a tensor) as a tensor there, without waiting for the GPU: host data goes through pinned memory."""
+    x = torch.as_tensor(x, dtype=dtype)
+    if x.device.type == "cpu" and torch.device(device).type == "cuda":
+        return x.pin_memory().to(device, non_blocking=True)
+    return x.to(device)
+
+
 def rope_tables(max_pos: int, rotary_dim: int = HEAD_DIM, theta: float = ROPE_THETA, scaling: Optional[dict] = None,
                 device="cuda") -> Tuple[torch.Tensor, torch.Tensor]:
     """fp32 cos and sin ``[max_pos, rotary_dim / 2]`` for :func:`rope_append`.
@@ -142,7 +150,7 @@ class PagedKVCache:
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
 
     def _ints(self, x) -> torch.Tensor:
-        return torch.as_tensor(x, dtype=torch.int32, device=self.k_pages.device).reshape(-1)
+        return to_device(x, torch.int32, self.k_pages.device).reshape(-1)
 
     def check(self) -> None:
         """Raises the first device-side error since the last check (synchronises)."""

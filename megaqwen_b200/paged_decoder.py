@@ -22,7 +22,7 @@ from typing import List, Optional, Sequence, Tuple
 import torch
 import torch.nn.functional as F
 
-from .paged import BAD_TOKEN, PagedKVCache
+from .paged import BAD_TOKEN, PagedKVCache, to_device
 from .weights import (HEAD_DIM, NUM_KV_HEADS, NUM_Q_HEADS, Q_SIZE, KV_SIZE, RMS_NORM_EPS, Qwen3Weights, rope_tables)
 
 
@@ -102,7 +102,7 @@ class PagedDecoder:
             raise ValueError("a sequence is named twice or out of range")
 
     def _ints(self, x, dtype: torch.dtype = torch.int32) -> torch.Tensor:
-        return torch.as_tensor(x, dtype=dtype, device=self.embed.device)
+        return to_device(x, dtype, self.embed.device)
 
     def _tokens(self, ids, n: int) -> torch.Tensor:
         """n token ids on the device.  One out of range raises if it is known on the host; on the device it is read as
@@ -226,8 +226,8 @@ class PagedDecoder:
         if not slots:
             return self.embed.new_empty((0, self.embed.shape[0]), dtype=torch.float32)
         self._grow(slots, [self.lengths[s] + 1 for s in slots])
-        order, back, dev_slots, starts, pages = self._groups(slots)
-        positions = self._ints([self.lengths[slots[i]] - 1 for i in order])
+        _, back, dev_slots, starts, pages = self._groups(slots)
+        positions = self.cache.lengths[dev_slots]
         self.cache.reserve(dev_slots, positions + 1)
         if self.sparse_pages is None:
             def attend(li, q):

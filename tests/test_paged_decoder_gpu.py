@@ -150,6 +150,24 @@ def test_tokens_and_slots_that_are_wrong():
     dec.check()
 
 
+def test_steps_do_not_synchronise():
+    dec = decoder(num_pages=40)
+    dec.prefill(0, prompt_of(40, 5))
+    dec.fork(0, [1, 2])
+    tokens = torch.tensor([1, 2, 3], device="cuda")
+    dec.step([0, 1, 2], tokens)
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        for _ in range(20):
+            tokens = dec.step([0, 1, 2], tokens).argmax(-1)
+        dec.step([2, 0], tokens[:2])
+        dec.free([1])
+        dec.fork(0, [1])
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    dec.check()
+
+
 def test_example_runs(capsys):
     spec = importlib.util.spec_from_file_location("shared_prompt", ROOT / "examples" / "shared_prompt.py")
     mod = importlib.util.module_from_spec(spec)

@@ -175,7 +175,8 @@ class PagedKVCache:
         free(self.page_table, self.lengths, self.refs, self._ints(slots), self.page_size, status=self.status)
 
     def compact(self, num_pages: int) -> "PagedKVCache":
-        """This cache with its pages in use gathered into a pool of num_pages."""
+        """This cache with its pages in use gathered into a pool of num_pages.  Where they do not fit, both caches'
+        :meth:`check` raises and the new one is empty."""
         if num_pages < 1:
             raise ValueError("num_pages must be positive")
         new = object.__new__(PagedKVCache)
@@ -185,10 +186,11 @@ class PagedKVCache:
         new.index = None if self.index is None else self.index.new_zeros((num_pages,) + tuple(self.index.shape[1:]))
         new.page_table = torch.full_like(self.page_table, -1)
         new.refs = self.refs.new_zeros(num_pages)
-        new.lengths = self.lengths.clone()
         new.status = torch.zeros_like(self.status)
         compact(self.k_pages, self.v_pages, self.page_table, self.refs, new.k_pages, new.v_pages, new.page_table,
-                new.refs, index=self.index, out_index=new.index, status=self.status)
+                new.refs, index=self.index, out_index=new.index, status=new.status)
+        new.lengths = torch.where(new.status == 0, self.lengths, 0)
+        self.status.copy_(torch.where(self.status == 0, new.status, self.status))
         return new
 
     def append(self, layer: int, q, k, v, slots, positions, cos, sin, interleaved: bool = False) -> torch.Tensor:

@@ -414,6 +414,26 @@ def test_copy_pages(paged):
         status.zero_()
 
 
+def test_compact_that_does_not_fit(paged):
+    """Neither cache passes for sound, and the new one is empty; an error from before is the old cache's alone."""
+    cache = paged.PagedKVCache(10, 3, 8, num_layers=1, num_kv_heads=1, head_dim=64, page_size=16)
+    cache.reserve([0, 1], [40, 17])
+    small = cache.compact(4)
+    for c in (cache, small):
+        with pytest.raises(RuntimeError, match="free pages"):
+            c.check()
+    assert not small.lengths.any() and small.free_pages() == 4
+    small.reserve([2], [64])
+    small.check()
+    cache.reserve([1], [3])
+    new = cache.compact(5)
+    new.check()
+    assert new.lengths.tolist() == [40, 17, 0] and new.free_pages() == 0
+    with pytest.raises(RuntimeError, match="position"):
+        cache.check()
+    cache.check()
+
+
 def test_copy_between_views(paged):
     """Pools that are views of one storage: a page that is read and written is found under both of its numbers, and
     pages past the smaller pool are no matter."""

@@ -684,6 +684,60 @@ def test_attend_strided_and_layers(paged):
     assert torch.equal(paged.attend(odd[..., 1:d + 1], p.k, p.v, p.table, p.lengths, dev(p.slots), layer=2), b)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [-0.09, 0.0, 0.3])
+@pytest.mark.parametrize("d,members", [(128, 40), (64, 2)])
+def test_attend_scales(paged, dtype, scale, d, members):
+    """Any sign and none: own parts alone, a shared prefix on the tensor cores (but for zero) and in the row kernel."""
+    page, pages = 32, 5
+    lens = [pages * page + 1 + 3 * b for b in range(members)] + [70]
+    p = Pool(lens, page, 2, d, dtype, seed=members, share={b: (0, pages) for b in range(1, members)})
+    q = normal(p.g, len(lens), 4, d, dtype=dtype, std=2.0)
+    check_attend(paged, p, 4, [1] * len(lens), scale=scale, q=q)
+    check_attend(paged, p, 4, [1] * len(lens), groups=[members], prefix=[pages], scale=scale, q=q)
+    # every page selected: the same as reading everything
+    idx = torch.zeros(p.k.shape[0], 2, 2, 2 * d + 16, dtype=torch.int8, device="cuda")
+    want = paged.attend(q, p.k, p.v, p.table, p.lengths, dev(p.slots), layer=1, scale=scale)
+    out, _ = paged.sparse_attend(q, p.k, p.v, idx, p.table, dev(p.slots), dev([n - 1 for n in lens]), layer=1, top_k=40, scale=scale)
+    # (twice check_attend's bound: both are rounded)
+    tol = 2 * ROUND[dtype] * want.double().abs() + 2.0 ** -12 * p.v.abs().max().item()
+    assert bool(((out.double() - want.double()).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("groups,members,grp", [(256, 3, 8), (257, 3, 8), (600, 3, 2), (1024, 2, 1)])
+def test_attend_many_groups(paged, groups, members, grp):
+    """Around the most groups of the tensor-core kernel, and the most sequences of a call (2048)."""
+    page, d = 16, 64
+    lens, share = [], {}
+    for g in range(groups):
+        for i in range(members):
+            if i:
+                share[len(lens)] = (len(lens) - i, 2)
+            lens.append(2 * page + 1 + (7 * len(lens)) % 23)
+    p = Pool(lens, page, 1, d, torch.bfloat16, layers=1, seed=groups, share=share)
+    n = len(lens)
+    q = normal(p.g, n, grp, d, std=2.0)
+    status = dev([0])
+    starts = torch.arange(0, n + 1, members, dtype=torch.int32, device="cuda")
+    out = paged.attend(q, p.k, p.v, p.table, p.lengths, dev(p.slots), layer=0, group_starts=starts, prefix_pages=dev([2] * groups),
+                       status=status)
+    assert status.item() == 0
+    for b in list(range(0, n, 97)) + [n - 1]:
+        k, v = p.kv(b, 0)
+        close(out[b], softmax_rows(q[b], k, v, torch.ones(lens[b], dtype=torch.bool, device="cuda"), d ** -0.5), v.abs().max().item())
+    # nothing declared shared: other sums, the same result within twice the bound
+    flat = paged.attend(q, p.k, p.v, p.table, p.lengths, dev(p.slots), layer=0)
+    tol = 2 * ROUND[out.dtype] * flat.double().abs() + 2.0 ** -12 * p.v.abs().max().item()
+    assert bool(((out.double() - flat.double()).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("d,page,hkv,grp", [(128, 64, 2, 2), (64, 16, 1, 5)])
+def test_attend_prompts(paged, d, page, hkv, grp):
+    """Whole prompts and a chunk behind a context, of many row tiles each, beside a single token."""
+    p = Pool([1300, 1777, 513, 900], page, hkv, d, torch.bfloat16, layers=1, seed=d)
+    check_attend(paged, p, hkv * grp, [1300, 700, 513, 1], layer=0)
+
+
 def test_contiguous_q_at_odd_offsets(paged):
     """A contiguous q whose first element is on no 16-byte boundary, and one token whose strides are odd."""
     page, hkv, d = 16, 2, 64

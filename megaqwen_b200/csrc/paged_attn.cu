@@ -589,8 +589,15 @@ int by_page_tokens(const mq_paged_sparse_params* p) {
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // The prefixes go to the tensor-core kernel when a group has more rows than the
-// 16 of a rows_kernel item on average.  (A scale of zero stays out: there a
-// masked score of minus infinity would not stay one.)
+// 16 of a rows_kernel item on average, so that the row kernel would read the prefix
+// more than once.  How long the prefix is stands on the device, so the rule cannot
+// look at it; tensor cores against rows for one group of two q heads per kv head,
+// 8 kv heads x 128, own parts of 100 (us a call):
+//   behind      64          1k          8k          32k         128k
+//    9 seqs  23.2 / 14.3  22.2 / 15.9  23.8 / 21.8  46 / 48    125 / 173
+//   32 seqs  24.3 / 15.8  23.1 / 17.2  31.4 / 30.9  50 / 83    133 / 340
+//   64 seqs  25.7 / 17.2  24.0 / 21.5  35.1 / 48.0  57 / 155   142 / 528
+// (A scale of zero stays out: there a masked score of minus infinity would not stay one.)
 bool tc_prefix(long long tokens, int grp, int NG, float scale) {
     return NG > 0 && NG <= PFX_MAX_GROUPS && tokens * grp > 16ll * NG && scale != 0.f;
 }

@@ -385,9 +385,12 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
                                     : a.ws.pfx_rowp + ((e.two ? 0 : (long long)q * a.total_q * a.hq) + (long long)tok * a.hq + head) * LD;
                 }
             }
-            if (!mine) {   // a run of one tile: this stream's part is empty
-                if (part && hh == 0)
-                    for (int i = 0; i < LD; ++i) part[i] = i == 0 ? -INFINITY : 0.f;
+            if (!mine) {   // a run of one tile: this stream's part is empty (half the rows each, a row by all lanes)
+#pragma unroll 1
+                for (int k = hh * 16; k < hh * 16 + 16; ++k) {
+                    float4* to = reinterpret_cast<float4*>(from_lane(part, k));
+                    for (int i = lane; to && i < LD / 4; i += 32) to[i] = make_float4(i == 0 ? -INFINITY : 0.f, 0.f, 0.f, 0.f);
+                }
                 continue;
             }
             meet();   // both warps are done with the Q rows of the item before
@@ -430,11 +433,13 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
                     if (valid < 64 || none) {
 #pragma unroll 1
                         for (int i = 0; i < 64; i += 32) {
+                            uint32_t live = valid >= i + 32 ? 0xffffffffu : valid > i ? (1u << (valid - i)) - 1u : 0u;
+                            for (int k = 0; k < 32; k += 16)   // a page is 16 keys or more
+                                if (none >> ((hh * 64 + i + k) >> a.pool.shift) & 1u) live &= ~(0xffffu << k);
                             float sv[32];
                             tmem_ld32(sa + i, sv);
 #pragma unroll
-                            for (int k = 0; k < 32; ++k)
-                                sv[k] = i + k < valid && !(none >> ((hh * 64 + i + k) >> a.pool.shift) & 1) ? sv[k] : -INFINITY;
+                            for (int k = 0; k < 32; ++k) sv[k] = live >> k & 1u ? sv[k] : -INFINITY;
                             tmem_st32(sa + i, sv);
                         }
                     }

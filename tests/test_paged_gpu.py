@@ -834,6 +834,45 @@ def test_attend_past_32_bits(paged):
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("d,members,grp", [(128, 40, 2), (64, 12, 4)])
+def test_steps_without_a_pause(paged, d, members, grp):
+    """Reserve, append and attend (a shared prefix on the tensor cores, the own parts beside it) step after step with
+    nothing between them: the same bits as with a synchronisation after every call."""
+    page, hkv, layers, steps = 16, 2, 3, 50
+    g = gen(d)
+    cos, sin = paged.rope_tables(600, d)
+    first = [normal(g, 200, (1 + i) * hkv, d) for i in (0, 0)]
+    new = [[[normal(g, members, h, d) for h in (hkv * grp, hkv, hkv)] for _ in range(layers)] for _ in range(steps)]
+    got = []
+    for wait in (True, False):
+        def pause():
+            if wait:
+                torch.cuda.synchronize()
+        c = paged.PagedKVCache(13 + members * 6, members + 1, 20, num_layers=layers, num_kv_heads=hkv, head_dim=d, page_size=page)
+        c.reserve([0], [200])
+        for layer in range(layers):
+            c.append(layer, first[0], first[0], first[1], dev([0] * 200), dev(list(range(200))), cos, sin)
+        kids = list(range(1, members + 1))
+        c.fork([0] * members, kids)
+        slots, gs, pp, one = dev(kids), dev([0, members]), dev([12]), dev([1] * members)
+        torch.cuda.synchronize()
+        outs = []
+        for step in range(steps):
+            pos = c.lengths[slots]
+            pause()
+            c.reserve(slots, pos + one)
+            pause()
+            for layer in range(layers):
+                q, k, v = new[step][layer]
+                q = c.append(layer, q, k, v, slots, pos, cos, sin)
+                pause()
+                outs.append(c.attend(layer, q, slots, group_starts=gs, prefix_pages=pp))
+                pause()
+        c.check()
+        got.append(torch.stack(outs))
+    assert torch.equal(*got)
+
+
 def test_other_stream_and_graph(paged):
     p = Pool([500, 300], 64, 2, 128, torch.bfloat16, seed=3)
     q = normal(p.g, 2, 4, 128)

@@ -356,13 +356,13 @@ int mq_decode_batch(const mq_decode_batch_params* params, cudaStream_t stream);
  *
  * Nothing here synchronises or allocates.  Arguments that live on the device
  * are checked there: `status` (device int32, optional) keeps the first error
- * code, and a call whose arguments are wrong changes none of the tables (free,
- * reserve and fork check the rows that they read, too).  Attention reads a wrong
+ * code, and a call whose arguments are wrong changes none of the tables (free
+ * and fork check the rows that they read, too).  Attention reads a wrong
  * slot, length or position as an empty sequence, and leaves out the positions of
  * a page that is out of range.
  * Workspaces hold nothing between calls; calls that overlap on the GPU need
  * their own. */
-enum { MQ_BF16 = 0, MQ_FP16 = 1, MQ_FP32 = 2 };
+enum { MQ_BF16 = 0, MQ_FP16 = 1 };
 
 typedef struct mq_paged_pool {
     void* k;
@@ -429,7 +429,9 @@ int mq_paged_compact(const mq_paged_pool* src, const mq_paged_pool* dst, const m
  * the channel-wise bounds of its keys as whole numbers HI[D], LO[D] times 2^e,
  * then e: e = clamp(floor(log2 a) - 6, -60, 40) for the largest magnitude a of
  * the bounds (0 if a = 0), HI and LO rounded to nearest even, at most 127 in
- * magnitude. */
+ * magnitude.  (A row that is written again later changes the record only when
+ * the last row is written after it, as it is when a sequence is taken up again
+ * from an earlier position.) */
 typedef struct mq_rope_params {
     const void* q;               /* [n, num_q_heads, head_dim], optional */
     void* q_out;

@@ -560,8 +560,10 @@ bool eight_fit(int n, int hkv, int D, int cols, int grp) {
            (D == 128 ? sel_eight_bytes<128>(cols, grp) : sel_eight_bytes<64>(cols, grp)) <= 98304;
 }
 
-// CTAs of the work line, two to an SM for head_dim 128 (rings of 96 KB) and
-// three for 64 (registers).
+// CTAs of the work line: two to an SM for head_dim 128 with 16 rows to an item (up to
+// 255 registers a thread), three otherwise (168).  The rings take 64 KB of shared memory
+// (head_dim 64: 32); with the schedule of a call near 2048 sequences and groups (48 KB)
+// fewer fit, and the rest of the grid runs after them.
 int row_grid(int D, int rt) { return sm_count() * (D == 128 && rt == 16 ? 2 : 3); }
 
 // The page-by-page form's rounds: parts that stay in L2 from the kernel that writes them to the join.
@@ -569,8 +571,10 @@ constexpr size_t PART_BYTES = 96u << 20;
 constexpr int BY_PAGE_TOKENS = 64;
 
 // Tokens per round of the page-by-page form, or 0 where each token reads its own pages.  Page by page when
-//  - there are more tokens than slots, so that some stand in one sequence (150 tokens of one context: 59 us against
-//    79; of 256 sequences with nothing in common: 237 against 216),
+//  - there are more tokens than the table has slots, so that some stand in one sequence (150 / 250 tokens of one context of
+//    16k: 47 / 61 us against 69 / 96; of 256 sequences with nothing in common: 237 against 216).  Which sequences a call
+//    holds stands on the device, so tokens of one sequence in a table of more slots than the call has tokens stay with the
+//    other form: the 69 / 96 us, and not the 237 for a decode batch,
 //  - a page's keys and values are 16 times its parts for one token or more (500 tokens on two contexts of 16k, page
 //    over group 64: 105 us against 202, 32: 107 against 205, 16: 204 against 216, 8: 378 against 235),
 //  - the choice kernel takes eight tokens at a time (it counts for this form), a round holds 64 tokens or more, and

@@ -164,14 +164,21 @@ __global__ void __launch_bounds__(PLAN_THREADS) free_kernel(Tab t, const int* __
     pdl_wait();
     pdl_trigger();
     const int ranks = (int)cluster_size(), rank = (int)cluster_rank();   // (the grid is one cluster)
+    // a warp to a sequence; its first row is on its way to L1 while the list is checked
+    const int per = blockDim.x / 32, lane = threadIdx.x & 31, warp = rank * per + (threadIdx.x >> 5), warps = ranks * per;
     if (threadIdx.x == 0) wrong = 0;
+    if (warp < n) {
+        const int s = slots[warp];
+        if (s >= 0 && s < t.slots) {
+            asm volatile("prefetch.global.L1 [%0];" ::"l"(t.lengths + s));
+            if (lane < t.cols) asm volatile("prefetch.global.L1 [%0];" ::"l"(t.table + s * t.row + lane));
+        }
+    }
     if (!slots_ok(slots, n, t.slots, bits)) {   // all CTAs alike
         if (rank == 0 && threadIdx.x == 0) note_status(t.status, MQ_ERR_BAD_SLOT);
         return;
     }
     if (ranks > 1) cluster_sync();   // every CTA runs and has its `wrong`: it may be written
-    // a warp to a sequence
-    const int lane = threadIdx.x & 31, warp = rank * PLAN_WARPS + (threadIdx.x >> 5), warps = ranks * PLAN_WARPS;
     bool bad = false;
     for (int i = warp; i < n; i += warps) {
         const int s = slots[i], used = min(pages_of(t.lengths[s], t.page), t.cols);
@@ -402,6 +409,20 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(Tab t, const in
         return;
     }
     int copies = 0, wrong = 0;
+    // every full page of every parent in range and in use; a warp to a parent, and each parent once
+    // (from the last warp down, so that a short list's first warp goes on to the part pages meanwhile)
+    for (int i = PLAN_WARPS - 1 - (threadIdx.x >> 5); i < n; i += PLAN_WARPS) {
+        const int lane = threadIdx.x & 31, p = parents[i];
+        int first = 0;
+        if (lane == 0) first = !(atomicOr(&looked[p >> 5], 1u << (p & 31)) >> (p & 31) & 1u);
+        if (!__shfl_sync(0xffffffffu, first, 0)) continue;
+        const int full = min(t.lengths[p] / t.page, t.cols);   // (a length beyond the row is refused below)
+#pragma unroll 4
+        for (int c = lane; c < full; c += 32) {
+            const int g = t.table[p * t.row + c];
+            if (g < 0 || g >= t.pages || t.refs[g] <= 0) wrong |= 2;
+        }
+    }
     for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
         const int i = i0 + threadIdx.x;
         int part = 0, src = -1;
@@ -425,19 +446,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(Tab t, const in
             off[i] = part > 0 ? copies + at : -1;
         }
         copies += sum;
-    }
-    // every full page of every parent in range and in use; a warp to a parent, and each parent once
-    for (int i = threadIdx.x >> 5; i < n; i += PLAN_WARPS) {
-        const int lane = threadIdx.x & 31, p = parents[i];
-        int first = 0;
-        if (lane == 0) first = !(atomicOr(&looked[p >> 5], 1u << (p & 31)) >> (p & 31) & 1u);
-        if (!__shfl_sync(0xffffffffu, first, 0)) continue;
-        const int full = min(t.lengths[p] / t.page, t.cols);   // (a length beyond the row is refused above)
-#pragma unroll 4
-        for (int c = lane; c < full; c += 32) {
-            const int g = t.table[p * t.row + c];
-            if (g < 0 || g >= t.pages || t.refs[g] <= 0) wrong |= 2;
-        }
     }
     const int any1 = __syncthreads_or(wrong & 1), any2 = __syncthreads_or(wrong & 2);
     if (any1 || any2) {
@@ -582,6 +590,7 @@ size_t mq_paged_workspace_bytes(int num_pages, int n) {
 int mq_paged_free(const mq_page_table* t, const int* slots, int n, cudaStream_t st) {
     if (!tab_ok(t, n, true) || (n && !slots)) return MQ_ERR_INVALID_ARGUMENT;
     if (!n) return MQ_OK;
+    if (n <= 8) return done(launch(free_kernel, dim3(1), dim3(256), 0, st, tab_of(t), slots, n), "paged free");
     unsigned ranks = 1;   // a warp to a sequence; 64 sequences take the same time with 1, 2 and 8 CTAs
     while (ranks < 8 && (int)ranks * PLAN_WARPS < n) ranks *= 2;
     return done(launch_cluster(free_kernel, ranks, ranks, dim3(PLAN_THREADS), 0, st, tab_of(t), slots, n), "paged free");

@@ -417,15 +417,20 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
                 if (lane == 0) mbar_arrive(&q_full[q]);
             }
             float m = -INFINITY, l = 0.f;
+            // lane i: whether page `at + i` of the prefix is out of range (the last one, past the end)
+            auto gone = [&](int at) {
+                const int pid = __ldg(row_of(e) + min(at + lane, s.eff[e.g] - 1));
+                return pid < 0 || pid >= a.pool.pages;
+            };
+            // looked up once per run, while the first scores are on their way, and again tile by tile only if there are any
+            bool holes = false;
+#pragma unroll 1
+            for (int i = 0; i < e.n * (PK / page); i += 32) holes |= gone(e.t0 * (PK / page) + i);
+            holes = __any_sync(0xffffffffu, holes);
             for (int j = 0; j < mine; ++j, ++ns) {
                 float tmax = -INFINITY;
                 const int t = e.t0 + (e.two ? j : 2 * j + q);
-                // the tile's pages that are out of range (looked up while its scores are on their way)
-                unsigned none;
-                {
-                    const int pid = __ldg(row_of(e) + min(t * (PK / page) + min(lane, PK / page - 1), s.eff[e.g] - 1));
-                    none = __ballot_sync(0xffffffffu, pid < 0 || pid >= a.pool.pages);
-                }
+                const unsigned none = holes ? __ballot_sync(0xffffffffu, gone(t * (PK / page))) : 0u;
                 if (got(&s_full[q], ns & 1)) {
                     tc_fence_after();
                     const int valid = s.eff[e.g] * page - t * PK - hh * 64;

@@ -5,14 +5,15 @@
 // same tables.  Each operation that needs a decision over all pages makes it
 // in one CTA ("plan": validation, a scan of the counts, a list of moves in the
 // workspace), and a second, wide kernel carries it out; plan and move are
-// chained by programmatic dependent launch.  A plan that finds its arguments
-// wrong writes the status word and a move count of zero, and nothing changes.
+// chained by programmatic dependent launch.  A plan that finds its arguments, or the
+// rows that they name, wrong writes the status word and a move count of zero, and
+// nothing changes; free and reserve alike.
 //
 // Bound: HBM for the moves, a page's rows read and written once by warps of 16-byte
 // accesses, eight in flight.  153 pages of 28 layers (1.14 GB both ways) into
 // another pool: 181 us, 6.3 TB/s, 0.96 of the copy rate; 64 copies of 40 rows of
-// one page (294 MB written, 4.6 MB read): 50 us, 5.9 TB/s.  Latency for the plans:
-// 4 to 7 us each, a dozen dependent reads of one CTA.
+// one page (294 MB written, 4.6 MB read): 50 us, 5.9 TB/s.  Latency for the plans, free and
+// reserve: 4 to 7 us each, a dozen dependent reads of one CTA.
 #include <algorithm>
 
 #include "paged_common.cuh"

@@ -60,10 +60,11 @@ STATUS = {
 
 
 def to_device(x, dtype: torch.dtype, device) -> torch.Tensor:
-    """x (a list, or a tensor) as a tensor there, without waiting for the GPU: host data goes through pinned memory."""
+    """x (a list, or a tensor) as a tensor there, without waiting for the GPU: host data goes through pinned memory of its
+    own, so the caller may write to x again at once."""
     x = torch.as_tensor(x, dtype=dtype)
     if x.device.type == "cpu" and torch.device(device).type == "cuda":
-        return x.pin_memory().to(device, non_blocking=True)
+        return (x.clone() if x.is_pinned() else x).pin_memory().to(device, non_blocking=True)
     return x.to(device)
 
 

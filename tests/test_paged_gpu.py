@@ -414,6 +414,19 @@ def test_copy_pages(paged):
         status.zero_()
 
 
+def test_host_lists_may_be_written_again(paged):
+    """Lists and tensors of the host are read before the call returns, however far behind the GPU is."""
+    cache = paged.PagedKVCache(10, 3, 8, num_layers=1, num_kv_heads=1, head_dim=64, page_size=16)
+    for make in (torch.Tensor.clone, torch.Tensor.pin_memory):
+        slots, lens = make(torch.tensor([0, 2], dtype=torch.int32)), make(torch.tensor([40, 17], dtype=torch.int32))
+        torch.cuda._sleep(50_000_000)
+        cache.reserve(slots, lens)
+        slots[:], lens[:] = 1, 3
+        cache.check()
+        assert cache.lengths.tolist() == [40, 0, 17]
+        cache.free([0, 2])
+
+
 def test_compact_that_does_not_fit(paged):
     """Neither cache passes for sound, and the new one is empty; an error from before is the old cache's alone."""
     cache = paged.PagedKVCache(10, 3, 8, num_layers=1, num_kv_heads=1, head_dim=64, page_size=16)

@@ -108,14 +108,14 @@ class PagedDecoder:
         """n token ids on the device.  One out of range raises if it is known on the host; on the device it is read as
         the nearest one and :meth:`check` raises."""
         ids = torch.as_tensor(ids)
-        if ids.numel() != n or ids.is_floating_point():
+        if ids.numel() != n or (n and ids.is_floating_point()):   # (an empty list becomes a float tensor)
             raise ValueError("there must be one token id for each sequence")
         ids, top = ids.reshape(-1), self.embed.shape[0] - 1
         if ids.device.type == "cpu":
             if n and not 0 <= int(ids.min()) <= int(ids.max()) <= top:
                 raise ValueError("token id out of range")
             return self._ints(ids, torch.int64)
-        ids = ids.long()
+        ids = ids.to(self.embed.device).long()
         safe = ids.clamp(0, top)
         status = self.cache.status
         status.copy_(torch.where((safe != ids).any() & (status == 0), BAD_TOKEN, status))

@@ -140,7 +140,7 @@ def test_tokens_and_slots_that_are_wrong():
     for call in (lambda: dec.free([0, 0]), lambda: dec.free([7]), lambda: dec.fork(9, [1]), lambda: dec.fork(0, [1, 1]), lambda: dec.fork(0, [0])):
         with pytest.raises(ValueError):
             call()
-    assert dec.step([], torch.tensor([], dtype=torch.long)).shape == (0, vocab)
+    assert dec.step([], torch.tensor([], dtype=torch.long)).shape == dec.step([], []).shape == (0, vocab)
     oracle, _ = oracle_with(b)
     close(dec.step([0], torch.tensor([3]))[0], oracle.decode_step(3, 20))
     dec.check()

@@ -500,6 +500,48 @@ typedef struct mq_paged_attend_params {
 size_t mq_paged_attend_workspace_bytes(const mq_paged_attend_params* params);
 int mq_paged_attend(const mq_paged_attend_params* params, cudaStream_t stream);
 
+/* Attention under a mask.  As mq_paged_attend without groups: the query tokens
+ * of sequence b are rows q_starts[b] .. q_starts[b+1] - 1 of q (one each when
+ * q_starts is NULL), the last positions of slot slots[b], whose keys are written
+ * already.  Rows that see nothing are zero; what an infinity or NaN among the
+ * values does is as there.
+ *
+ * mq_paged_window: a token at position p sees the positions j <= p with
+ * p - j < window or j < sinks.  Pages that no token sees are not read: their
+ * entries in the table may be anything.
+ *
+ * mq_paged_tree: the query tokens of a sequence are a tree, at most 256 nodes.
+ * parents[i] is the parent of node i as its place in the sequence's own tree,
+ * smaller than the node's, or -1 for a root.  A node sees every position before
+ * the tree's first, its ancestors and itself.  A parent that does not come
+ * before its node, or a tree of more nodes, is reported (code 1); such a node
+ * counts as a root, such a sequence as empty. */
+typedef struct mq_paged_span_params {
+    const mq_paged_pool* pool;
+    const void* q;               /* [total_q, num_q_heads, head_dim], strides in elements, multiples of 8 */
+    long long q_token, q_head;
+    void* out;                   /* [total_q, num_q_heads, head_dim] contiguous */
+    const int* table;
+    long long table_row;
+    int num_slots;
+    int table_cols;
+    const int* lengths;          /* device int32 [num_slots], the query tokens included */
+    const int* slots;            /* device int32 [num_seqs] */
+    const int* q_starts;         /* device int32 [num_seqs + 1], optional */
+    int num_seqs;                /* at most 2048 */
+    int total_q;
+    int num_q_heads;             /* a multiple of the pool's kv heads */
+    int layer;
+    float scale;
+    int* status;                 /* device int32, optional */
+    void* workspace;             /* device, mq_paged_span_workspace_bytes() */
+    size_t workspace_bytes;
+} mq_paged_span_params;
+
+size_t mq_paged_span_workspace_bytes(const mq_paged_span_params* params);
+int mq_paged_window(const mq_paged_span_params* params, int window, int sinks, cudaStream_t stream);
+int mq_paged_tree(const mq_paged_span_params* params, const int* parents, cudaStream_t stream);
+
 /* Attention over a few pages of the context, chosen for each query token and
  * kv head by the pool's index.  Token i stands at positions[i] of slot
  * slots[i].  Its own page is always read; of the pages before it, the

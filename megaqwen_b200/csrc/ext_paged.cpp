@@ -354,6 +354,67 @@ Tensor attend(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor len
     return out;
 }
 
+// The part that window_attend and tree_attend share; run(params, stream) makes the call.
+template <typename Run>
+Tensor span_attend(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths,
+                   const Tensor& slots, int64_t layer, const OptTensor& q_starts, c10::optional<double> scale,
+                   const OptTensor& status, const char* name, Run run) {
+    const mq_paged_pool pool = pool_of(k_pages, v_pages, c10::nullopt);
+    const auto dev = k_pages.device();
+    heads(q, "q", -1, pool.head_dim, k_pages);
+    table_ok(table, dev);
+    if (layer < 0 || layer >= pool.num_layers) fail("layer out of range");
+    mq_paged_span_params p = {};
+    p.num_q_heads = q_heads(q, pool);
+    p.slots = ints(slots, dev, "slots");
+    if (slots.numel() > 2048) fail("at most 2048 sequences per call");
+    p.num_seqs = (int)slots.numel();
+    if (q.size(0) > 0x7fffffffll) fail("too many query tokens");
+    p.total_q = (int)q.size(0);
+    if (q_starts.has_value()) p.q_starts = ints(*q_starts, dev, "q_starts", slots.numel() + 1);
+    else if (q.size(0) != slots.numel()) fail("without q_starts, q must have one token per sequence");
+    if (q.size(0) && !slots.numel()) fail("query tokens without sequences");
+    p.lengths = ints(lengths, dev, "lengths", table.size(0));
+    p.status = status_of(status, dev);
+    c10::cuda::CUDAGuard guard(dev);
+    const Tensor qq = pieces(q);
+    Tensor out = blank(q.sizes(), q.scalar_type(), dev);
+    if (!out.numel()) return out;
+    p.pool = &pool;
+    p.q = qq.data_ptr();
+    p.q_token = qq.stride(0);
+    p.q_head = qq.stride(1);
+    p.out = out.data_ptr();
+    p.table = table.data_ptr<int>();
+    p.table_row = row_of(table);
+    p.num_slots = (int)table.size(0);
+    p.table_cols = (int)table.size(1);
+    p.layer = (int)layer;
+    p.scale = scale.has_value() ? (float)*scale : 1.0f / std::sqrt((float)pool.head_dim);
+    p.workspace_bytes = mq_paged_span_workspace_bytes(&p);
+    Tensor ws = scratch(p.workspace_bytes, dev);
+    p.workspace = ws.data_ptr();
+    raise_rc(run(&p, stream_of(q)), name);
+    return out;
+}
+
+Tensor window_attend(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor lengths, Tensor slots, int64_t layer,
+                     int64_t window, int64_t sinks, OptTensor q_starts, c10::optional<double> scale, OptTensor status) {
+    if (window < 1) fail("window must be positive");
+    if (sinks < 0) fail("sinks must not be negative");
+    const int w = (int)std::min<int64_t>(window, 0x7fffffff), n = (int)std::min<int64_t>(sinks, 0x7fffffff);
+    return span_attend(q, k_pages, v_pages, table, lengths, slots, layer, q_starts, scale, status, "window_attend",
+                       [&](const mq_paged_span_params* p, cudaStream_t st) { return mq_paged_window(p, w, n, st); });
+}
+
+Tensor tree_attend(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor lengths, Tensor slots, Tensor parents,
+                   int64_t layer, OptTensor q_starts, c10::optional<double> scale, OptTensor status) {
+    if (!k_pages.is_cuda()) fail("k_pages must be a CUDA tensor");
+    const int* up = ints(parents, k_pages.device(), "parents", q.dim() == 3 ? q.size(0) : -1);
+    return span_attend(q, k_pages, v_pages, table, lengths, slots, layer, q_starts, scale, status, "tree_attend",
+                       [&](const mq_paged_span_params* p, cudaStream_t st) { return mq_paged_tree(p, up, st); });
+}
+
 std::tuple<Tensor, Tensor> sparse_attend(Tensor q, Tensor k_pages, Tensor v_pages, Tensor index, Tensor table,
                                          Tensor slots, Tensor positions, int64_t layer, int64_t top_k,
                                          c10::optional<double> scale, OptTensor status) {
@@ -422,6 +483,12 @@ void bind_paged(py::module_& m) {
           py::arg("lengths"), py::arg("slots"), py::arg("layer"), py::arg("q_starts") = none,
           py::arg("group_starts") = none, py::arg("prefix_pages") = none, py::arg("scale") = none,
           py::arg("status") = none);
+    m.def("paged_window_attend", &window_attend, py::arg("q"), py::arg("k_pages"), py::arg("v_pages"),
+          py::arg("page_table"), py::arg("lengths"), py::arg("slots"), py::arg("layer"), py::arg("window"),
+          py::arg("sinks") = 0, py::arg("q_starts") = none, py::arg("scale") = none, py::arg("status") = none);
+    m.def("paged_tree_attend", &tree_attend, py::arg("q"), py::arg("k_pages"), py::arg("v_pages"), py::arg("page_table"),
+          py::arg("lengths"), py::arg("slots"), py::arg("parents"), py::arg("layer"), py::arg("q_starts") = none,
+          py::arg("scale") = none, py::arg("status") = none);
     m.def("paged_sparse_attend", &sparse_attend, py::arg("q"), py::arg("k_pages"), py::arg("v_pages"), py::arg("index"),
           py::arg("page_table"), py::arg("slots"), py::arg("positions"), py::arg("layer"), py::arg("top_k"),
           py::arg("scale") = none, py::arg("status") = none);

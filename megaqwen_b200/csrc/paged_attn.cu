@@ -660,6 +660,7 @@ Shape shape_of(const mq_paged_attend_params* p) {
     return {p->pool->head_dim, p->num_q_heads, p->total_q, true, p->num_groups > 0,
             tc_prefix(p->total_q, p->num_q_heads / p->pool->num_kv_heads, p->num_groups, p->scale)};
 }
+Shape shape_of(const mq_paged_span_params* p) { return {p->pool->head_dim, p->num_q_heads, p->total_q, true, false, false}; }
 Shape shape_of(const mq_paged_sparse_params* p) {
     return {p->pool->head_dim, p->num_q_heads, p->n, false, false, false};
 }
@@ -710,13 +711,13 @@ int run_rows(const RowArgs& a, const mq_paged_pool& pool, cudaStream_t st) {
     CUtensorMap tk, tv;
     if (!pool_maps(&tk, &tv, pool, a.pool, GRP, D / 64)) return MQ_ERR_CUDA;
     auto kernel = rows_kernel<T, D, MODE, NT>;
-    const size_t smem = (size_t)ROW_WARPS * RowWarp<T, D, NT>::RING + 1024 + (MODE == 0 ? sched_bytes(a.B, a.NG) : 0);
+    const size_t smem = (size_t)ROW_WARPS * RowWarp<T, D, NT>::RING + 1024 + (MODE == 1 ? 0 : sched_bytes(a.B, a.NG));
     static SmemLimit limit;
     cudaError_t e = allow_smem(kernel, smem, limit);
     if (e != cudaSuccess) return note_cuda(e, "paged attention attribute");
     const int grid = row_grid(D, 8 * NT);
     e = launch(kernel, dim3(grid), dim3(ROW_THREADS), smem, st, tk, tv, a);
-    if (e == cudaSuccess) e = run_join<T, D, MODE>(a, (uint32_t)grid * ROW_WARPS, st);
+    if (e == cudaSuccess) e = run_join<T, D, MODE == 3 ? 0 : MODE>(a, (uint32_t)grid * ROW_WARPS, st);
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "paged attention");
 }
 
@@ -828,6 +829,69 @@ int mq_paged_attend(const mq_paged_attend_params* p, cudaStream_t st) {
     const long long rows = (long long)a.total_q * a.grp;
     set_rt(a, rows <= 8ll * a.B && (!a.NG || a.tc || rows <= 8ll * a.NG));
     return dispatch(p->pool->dtype, s.D, [&](auto T, auto D) { return run_attend<decltype(T), decltype(D)::value>(a, *p->pool, st); });
+}
+
+size_t mq_paged_span_workspace_bytes(const mq_paged_span_params* p) {
+    if (!p || !p->pool || p->total_q < 0 || p->pool->num_kv_heads < 1) return 0;
+    return row_workspace(shape_of(p), nullptr, nullptr);
+}
+
+namespace {
+int run_span(const mq_paged_span_params* p, int window, int sinks, const int* parents, cudaStream_t st) {
+    if (!pool_ok(p->pool) || p->num_seqs < 0 || p->num_seqs > MAX_SEQS || p->total_q < 0 || p->num_q_heads < 1 ||
+        p->num_q_heads % p->pool->num_kv_heads || p->layer < 0 || p->layer >= p->pool->num_layers || p->num_slots < 1 ||
+        p->table_cols < 1 || (!p->q_starts && p->num_seqs != p->total_q))
+        return MQ_ERR_INVALID_ARGUMENT;
+    if (!p->total_q || !p->num_seqs) return p->total_q ? MQ_ERR_INVALID_ARGUMENT : MQ_OK;
+    if (!q_ok(p->q, p->q_token, p->q_head) || !p->out || (reinterpret_cast<uintptr_t>(p->out) & 15) || !p->table ||
+        !p->lengths || !p->slots || (long long)p->total_q * p->num_q_heads > 0x7fffffffll)
+        return MQ_ERR_INVALID_ARGUMENT;
+    if (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255) ||
+        p->workspace_bytes < mq_paged_span_workspace_bytes(p))
+        return MQ_ERR_WORKSPACE;
+    RowArgs a = {};
+    a.pool = view_of(*p->pool, p->layer);
+    a.q = (const uint16_t*)p->q;
+    a.q_tok = p->q_token;
+    a.q_head = p->q_head;
+    a.out = (uint16_t*)p->out;
+    a.table = p->table;
+    a.table_row = p->table_row;
+    a.num_slots = p->num_slots;
+    a.cols = p->table_cols;
+    a.lengths = p->lengths;
+    a.slots = p->slots;
+    a.q_starts = p->q_starts;
+    a.B = p->num_seqs;
+    a.total_q = p->total_q;
+    a.hq = p->num_q_heads;
+    a.hkv = p->pool->num_kv_heads;
+    a.grp = a.hq / a.hkv;
+    a.scale_log2 = p->scale * 1.4426950408889634f;
+    a.status = p->status;
+    a.window = window;
+    a.sinks = sinks;
+    a.parents = parents;
+    const Shape s = shape_of(p);
+    row_workspace(s, &a.ws, p->workspace);
+    set_rt(a, (long long)a.total_q * a.grp <= 8ll * a.B);   // as for attend
+    return dispatch(p->pool->dtype, s.D, [&](auto T, auto D) {
+        using E = decltype(T);
+        constexpr int d = decltype(D)::value;
+        return a.rt == 8 ? run_rows<E, d, 3, 1>(a, *p->pool, st) : run_rows<E, d, 3, 2>(a, *p->pool, st);
+    });
+}
+}  // namespace
+
+int mq_paged_window(const mq_paged_span_params* p, int window, int sinks, cudaStream_t st) {
+    if (!p || window < 1 || sinks < 0) return MQ_ERR_INVALID_ARGUMENT;
+    // (a window longer than any sequence is as good as the longest; sums with it stay below 2^31)
+    return run_span(p, std::min(window, 1 << 30), std::min(sinks, 1 << 30), nullptr, st);
+}
+
+int mq_paged_tree(const mq_paged_span_params* p, const int* parents, cudaStream_t st) {
+    if (!p || (p->total_q && !parents)) return MQ_ERR_INVALID_ARGUMENT;
+    return run_span(p, 0, 0, parents, st);
 }
 
 size_t mq_paged_sparse_workspace_bytes(const mq_paged_sparse_params* p) {

@@ -39,6 +39,8 @@ constexpr int ROW_THREADS = 128;
 constexpr int ROW_WARPS = ROW_THREADS / 32;
 constexpr int STAGES = 2;
 constexpr int MAX_SEQS = 2048;
+constexpr int MAX_TREE = 256;      // nodes of a drafted tree
+constexpr int TREE_WORDS = MAX_TREE / 32;
 constexpr int PK = 128;            // keys per tile and query rows per item of the tensor-core prefix kernel
 constexpr int PROWS = 256;
 
@@ -106,6 +108,8 @@ struct RowArgs {
     int* status;
     WsView ws;
     ByPage bp;
+    int window, sinks;      // windowed: a token sees the last `window` positions up to its own and the first `sinks`
+    const int* parents;     // trees: the query tokens are nodes, a node's parent within its tree or -1
 };
 
 // A box of a page: rows from `row`, blocks of 64 channels from `block`, by a map whose base is at the layer.
@@ -168,7 +172,17 @@ __device__ inline Sched sched_of(uint8_t* p, int B, int NG) {
 
 __device__ __forceinline__ int q_start(const RowArgs& a, int b) { return a.q_starts ? __ldg(a.q_starts + b) : b; }
 
+// Sink groups of a windowed sequence, and the groups of a row tile: the window of its first row to the last row's own
+// position spans at most window + (tokens of the tile) - 1 positions.
+__device__ __forceinline__ int groups_of(int len) { return len > 0 ? ((len - 1) >> 4) + 1 : 0; }
+__device__ __forceinline__ int sink_groups(const RowArgs& a, int len) { return min(groups_of(a.sinks), groups_of(len)); }
+__device__ __forceinline__ int window_groups(const RowArgs& a, int len) {
+    const int tokens = (a.rt + a.grp - 2) / a.grp + 1;   // that a tile of rt rows may touch
+    return min(groups_of(len), sink_groups(a, len) + ((a.window + tokens - 2) >> 4) + 2);
+}
+
 __device__ __forceinline__ int own_groups(const RowArgs& a, const Sched& s, int b) {
+    if (a.window) return window_groups(a, s.len[b]);
     const int lo = s.grp[b] >= 0 ? s.eff[s.grp[b]] << a.pool.shift : 0;
     return s.len[b] > lo ? ((s.len[b] - lo - 1) >> 4) + 1 : 0;
 }
@@ -226,6 +240,10 @@ __device__ inline bool build_sched(const RowArgs& a, const Sched& s, unsigned lo
                 len = b == tid ? len0 : __ldg(a.lengths + slot);
                 if (len < 0 || pages_for(len, a.pool.shift) > a.cols) {
                     if (!PFX && blockIdx.x == 0) note_status(a.status, MQ_ERR_BAD_POSITION);
+                    len = 0;
+                }
+                if (a.parents && ql > MAX_TREE) {
+                    if (!PFX && blockIdx.x == 0) note_status(a.status, MQ_ERR_INVALID_ARGUMENT);
                     len = 0;
                 }
             }
@@ -379,10 +397,12 @@ struct RowWarp {
     // lim: positions of the group (below 1: none, 16 and up: all) that rows 8 n + 2 t + i see.
     // `mixed`: the rows of the tile do not all see the same positions.  SOLO: a row's sums may not depend on
     // the rows beside it, not in their last bit; `mixed`: a row does not see all positions.
-    template <bool SOLO>
+    // MASK: lim is not a count but a mask of the positions.
+    template <bool SOLO, bool MASK = false>
     __device__ __forceinline__ void step(int stage, const int (&lim)[NT][2], bool mixed, float scale) {
         const uint32_t ks = ring + stage * STAGE, vs = ks + TILE;
         const int g = lane >> 2, mat = lane >> 3, r8 = lane & 7;
+        auto sees = [&](int p, int lim_r) { return MASK ? (lim_r >> p & 1) != 0 : p < lim_r; };
         // S^T = K Q^T: positions g, g + 8; rows 2 t, 2 t + 1.  Even and odd k-steps in chains of their own.
         float s[NT][4], s2[NT][4];
 #pragma unroll
@@ -404,7 +424,7 @@ struct RowWarp {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int p = g + 8 * (i >> 1);
-                s[n][i] = p < lim[n][i & 1] ? (s[n][i] + s2[n][i]) * scale : -INFINITY;
+                s[n][i] = sees(p, lim[n][i & 1]) ? (s[n][i] + s2[n][i]) * scale : -INFINITY;
             }
             float u[2];
 #pragma unroll
@@ -489,7 +509,7 @@ struct RowWarp {
             }
             // one position at a time, added only to the rows that see it
             const int t = lane & 3;
-            auto takes = [&](int p, int lim_r) { return p < lim_r && !(SOLO && lim_r >= GRP); };
+            auto takes = [&](int p, int lim_r) { return sees(p, lim_r) && !(SOLO && lim_r >= GRP); };
 #pragma unroll 1
             for (int p = 0; p < GRP; ++p) {
                 uint32_t keep[2];
@@ -552,6 +572,24 @@ struct RowWarp {
     }
 };
 
+// The ancestors of node i of the tree whose first token is tok0, itself among them, as bits.  A parent that does not
+// come before its child counts as none.
+__device__ __forceinline__ void climb(const RowArgs& a, int tok0, int i, uint32_t* bits) {
+    while (i >= 0) {
+        bits[i >> 5] |= 1u << (i & 31);
+        const int up = __ldg(a.parents + tok0 + i);
+        if (up >= i || up < -1) note_status(a.status, MQ_ERR_INVALID_ARGUMENT);
+        i = up >= i ? -1 : up;
+    }
+}
+// 16 bits of them from bit `at` on (which may lie before the first).
+__device__ __forceinline__ int ancestors(const uint32_t* bits, int at) {
+    if (at < 0) return at > -16 ? (int)(bits[0] << -at & 0xffffu) : 0;
+    const int w = at >> 5;
+    if (w >= TREE_WORDS) return 0;
+    return (int)(__funnelshift_r(bits[w], w + 1 < TREE_WORDS ? bits[w + 1] : 0u, at & 31) & 0xffffu);
+}
+
 // An item as the loading side leaves it for the computing side.
 struct ItemBox {
     int tok0, h, r0, rows, first;   // rows r0 .. r0 + rows - 1 of the entity; position limit of row r: first + r / grp
@@ -562,7 +600,11 @@ constexpr int BOXES = 4;            // the ring spans at most STAGES items, and 
 enum { BOX_START = 1, BOX_WHOLE = 2, BOX_PREFIX = 4, BOX_OTHER = 8 };
 
 // MODE 0: attend (prefixes and own parts from the schedule).  MODE 1: sparse
-// (token t's item reads the pages selected[t][h][..], top_k of them).
+// (token t's item reads the pages selected[t][h][..], top_k of them).  MODE 3:
+// own parts under a mask, a sliding window with sinks or a tree of drafted tokens:
+// a row's positions in a group are 16 bits (windowed: two cuts; a tree: a piece of
+// the node's ancestors, walked up once for an item), and the groups that no row of
+// a tile sees are not read.
 //
 // Each warp walks its run of the line twice at once: a loading side, STAGES - 1
 // groups ahead, that finds items, looks up pages and issues copies, and a
@@ -580,6 +622,8 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     __shared__ unsigned long long scratch[ROW_WARPS];
     __shared__ uint64_t full[ROW_WARPS][STAGES];
     __shared__ ItemBox boxes[ROW_WARPS][BOXES];
+    constexpr bool LINE = MODE == 0 || MODE == 3;
+    __shared__ uint32_t above[MODE == 3 ? ROW_WARPS : 1][MODE == 3 ? RT : 1][MODE == 3 ? TREE_WORDS : 1];   // a row's ancestors
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t wid = blockIdx.x * ROW_WARPS + warp, warps = gridDim.x * ROW_WARPS;
     const int grp = a.grp, shift = a.pool.shift, page = a.pool.page;
@@ -597,7 +641,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     Sched s;
     uint32_t work, origin = 0;   // where this kernel's work starts on the line
     const int sp_nrt = row_tiles(a, grp), sp_ng = a.top_k << (shift - 4);
-    if (MODE == 0) {
+    if (LINE) {
         s = sched_of(smem + ROW_WARPS * W::RING, a.B, a.NG);
         const bool ok = build_sched<false, ROW_THREADS>(a, s, scratch);
         if (!ok) {
@@ -622,7 +666,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     int slot, base, tok0, rows_all, first, fixed;   // of the entity
     bool prefix = false, other = false;
     auto open = [&]() {   // entity e
-        if (MODE == 0) {
+        if (LINE) {
             prefix = e < a.NG;
             int b0, b1;
             first = base = 0;
@@ -664,6 +708,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         }
     };
     int h = 0, g0 = 0, n = 0, k = 0, lim_hi = 0;   // the item's head, its first group and groups in this run, the next one
+    int lim_lo = 0, g_sink = 0, g_skip = 0;        // windowed: where its rows' windows begin, sink groups, groups left out behind them
     int ids = -1, at = 0;                          // lane i: page and position of the i-th of a batch of 32 groups
     int ring_at = -1;                              // lane i: position of the group in stage i, or -1 for nothing
     int stage_l = 0, pushed = 0;
@@ -673,10 +718,13 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         ids = -1;
         at = 0;
         if (kk < n) {
-            if (MODE == 0) {
+            if (LINE) {
                 at = base + (g0 + kk) * GRP;
-                ids = __ldg(a.table + slot * a.table_row + (at >> shift));
-                want = true;
+                if (MODE == 3 && g0 + kk >= g_sink) at += g_skip * GRP;
+                // past the end, or between the sinks and the windows: in no row's sight
+                if (MODE == 3 && (at >= lim_hi || (at >= a.sinks && at + GRP <= lim_lo))) at = 0x7fffffff;
+                else ids = __ldg(a.table + slot * a.table_row + (at >> shift));
+                want = MODE != 3 || at != 0x7fffffff;
             } else {
                 const int j = (g0 + kk) >> (shift - 4);
                 const int c = __ldg(a.selected + ((long long)tok0 * a.hkv + h) * a.top_k + j);
@@ -702,7 +750,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 open();
             }
             // x lies in item `it`, which starts at x - within
-            const uint32_t start = MODE == 0 ? s.off[e] * a.hkv - origin + (uint32_t)it * (ng + ITEM_UNITS)
+            const uint32_t start = LINE ? s.off[e] * a.hkv - origin + (uint32_t)it * (ng + ITEM_UNITS)
                                              : ((uint32_t)e * items + it) * (ng + ITEM_UNITS);
             const uint32_t lo = max(x, start + ITEM_UNITS), hi = min(xe, start + ITEM_UNITS + ng);
             x = max(x, hi);
@@ -712,12 +760,18 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 x = xe;   // the run ends in the item's own units
                 return false;
             }
-            h = MODE == 0 ? i / nrt : e / a.total_q;
-            const int r0 = (MODE == 0 ? i - h * nrt : i) * RT, rows = min(RT, rows_all - r0);
+            h = LINE ? i / nrt : e / a.total_q;
+            const int r0 = (LINE ? i - h * nrt : i) * RT, rows = min(RT, rows_all - r0);
             g0 = (int)(lo - start) - ITEM_UNITS;
             n = (int)(hi - lo);
             k = 0;
             lim_hi = fixed >= 0 ? fixed : first + (r0 + rows - 1) / grp;
+            if (MODE == 3 && a.window) {
+                lim_lo = first + r0 / grp - a.window;
+                g_sink = min(groups_of(a.sinks), ng);
+                // a tile whose groups are all of the sequence's leaves none out
+                g_skip = ng == groups_of(s.len[e]) ? 0 : max(0, max(lim_lo, 0) / GRP - g_sink);
+            }
             if (lane == 0) {
                 ItemBox& b = boxes[warp][pushed % BOXES];
                 b.tok0 = tok0;
@@ -746,7 +800,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     w.lane = lane;
     w.ring = smem_u32(smem) + warp * W::RING;
     if (x < xe) {   // where the run starts
-        if (MODE == 0) {
+        if (LINE) {
             const uint32_t xh = (x + origin) / (uint32_t)a.hkv;
             int lo = 0, hi = a.NG + a.B;
             while (hi - lo > 1) {
@@ -805,7 +859,8 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         w.load_q(a, b.tok0, b.h, grp, b.r0, b.rows);
         w.reset();
         auto limit = [&](int r) { return b.fixed >= 0 ? b.fixed : b.first + (b.r0 + min(r, b.rows - 1)) / grp; };
-        const int lim_lo = limit(0), lim_top = limit(b.rows - 1);
+        const int lim_first = limit(0), lim_top = limit(b.rows - 1);
+        bool walked = false;
         int lim[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -820,14 +875,50 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     ok = false;
                     break;
                 }
-                if (lim_top - p0 < GRP) w.clear_rows(stage_c, lim_top - p0);
                 int rel[NT][2];
+                if (MODE == 3) {
+                    auto low = [](int k) { return (1 << min(max(k, 0), 16)) - 1; };
+                    const int base_c = b.first - 1;   // a tree's first position
+                    if (a.parents && !walked && p0 + GRP > base_c) {
+                        walked = true;
+                        if (lane < RT) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    rel[n][0] = lim[n][0] - p0;
-                    rel[n][1] = lim[n][1] - p0;
+                            for (int i = 0; i < TREE_WORDS; ++i) above[MODE == 3 ? warp : 0][lane][i] = 0;
+                            if (lane < b.rows) climb(a, b.tok0, (b.r0 + lane) / grp, above[MODE == 3 ? warp : 0][lane]);
+                        }
+                        __syncwarp();
+                    }
+                    bool full = true, none = true;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            int bits;
+                            if (a.parents) {
+                                bits = low(base_c - p0);
+                                if (walked) {
+                                    const int r = min(8 * n + 2 * t + i, b.rows - 1);
+                                    bits |= ancestors(above[MODE == 3 ? warp : 0][r], p0 - base_c);
+                                }
+                            } else {
+                                bits = low(lim[n][i] - p0);
+                                bits &= ~low(lim[n][i] - a.window - p0) | low(a.sinks - p0);
+                            }
+                            rel[n][i] = bits;
+                            full &= bits == 0xffff;
+                            none &= bits == 0;
+                        }
+                    if (!__all_sync(0xffffffffu, none))
+                        w.template step<false, true>(stage_c, rel, !__all_sync(0xffffffffu, full), a.scale_log2);
+                } else {
+                    if (lim_top - p0 < GRP) w.clear_rows(stage_c, lim_top - p0);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        rel[n][0] = lim[n][0] - p0;
+                        rel[n][1] = lim[n][1] - p0;
+                    }
+                    w.template step<false>(stage_c, rel, lim_first < min(p0 + GRP, lim_top), a.scale_log2);
                 }
-                w.template step<false>(stage_c, rel, lim_lo < min(p0 + GRP, lim_top), a.scale_log2);
             }
             stage_c = stage_c == STAGES - 1 ? 0 : stage_c + 1;
             __syncwarp();   // every lane is past its reads of the stage
@@ -858,7 +949,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
             if (__shfl_sync(0xffffffffu, ring_at, stage_c) >= 0) landed(stage_c);
         }
     }
-    if (MODE == 0) {
+    if (LINE) {
         // the join's view of the line, a share of the sequences per warp
         if (blockIdx.x == 0 && threadIdx.x == 0) {
             a.ws.head[0] = 1;

@@ -18,6 +18,8 @@ synchronises, and outputs come from the current stream's allocator):
 ``reserve`` ``fork`` ``free`` ``copy`` ``compact``   pages and their bookkeeping
 ``attend``         attention, shared prefixes read once per group
 ``sparse_attend``  attention over the pages that a cheap score selects
+``window_attend``  attention over the last positions and a few first ones (sinks)
+``tree_attend``    attention of a tree of drafted tokens
 
 Arguments that live on the GPU are checked there: a wrong slot, page or
 position writes its code to ``status`` (int32 ``[1]``, if given) and changes no
@@ -44,6 +46,8 @@ copy = _C.paged_copy
 compact = _C.paged_compact
 attend = _C.paged_attend
 sparse_attend = _C.paged_sparse_attend
+window_attend = _C.paged_window_attend
+tree_attend = _C.paged_tree_attend
 
 INDEX_PAD = 16   # bytes of an index record after the two bounds: the exponent and padding
 
@@ -201,6 +205,14 @@ class PagedKVCache:
     def attend(self, layer: int, q, slots, q_starts=None, group_starts=None, prefix_pages=None, scale=None) -> torch.Tensor:
         return attend(q, self.k_pages, self.v_pages, self.page_table, self.lengths, slots, layer=layer, q_starts=q_starts,
                       group_starts=group_starts, prefix_pages=prefix_pages, scale=scale, status=self.status)
+
+    def window_attend(self, layer: int, q, slots, window: int, sinks: int = 0, q_starts=None, scale=None) -> torch.Tensor:
+        return window_attend(q, self.k_pages, self.v_pages, self.page_table, self.lengths, slots, layer=layer, window=window,
+                             sinks=sinks, q_starts=q_starts, scale=scale, status=self.status)
+
+    def tree_attend(self, layer: int, q, slots, parents, q_starts=None, scale=None) -> torch.Tensor:
+        return tree_attend(q, self.k_pages, self.v_pages, self.page_table, self.lengths, slots, parents, layer=layer,
+                           q_starts=q_starts, scale=scale, status=self.status)
 
     def sparse_attend(self, layer: int, q, slots, positions, top_k: int, scale=None):
         if self.index is None:

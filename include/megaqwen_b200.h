@@ -362,7 +362,7 @@ int mq_decode_batch(const mq_decode_batch_params* params, cudaStream_t stream);
  * a page that is out of range.
  * Workspaces hold nothing between calls; calls that overlap on the GPU need
  * their own. */
-enum { MQ_BF16 = 0, MQ_FP16 = 1 };
+enum { MQ_BF16 = 0, MQ_FP16 = 1, MQ_FP32 = 2 /* logits of mq_sample alone */ };
 
 typedef struct mq_paged_pool {
     void* k;
@@ -417,6 +417,26 @@ int mq_paged_copy(const mq_paged_pool* src, const mq_paged_pool* dst, const int*
  * which shares no page with the first; out_table and out_refs (refs of dst->num_pages pages) name them there. */
 int mq_paged_compact(const mq_paged_pool* src, const mq_paged_pool* dst, const mq_page_table* t, int* out_table,
                      long long out_row_stride, int* out_refs, cudaStream_t stream);
+
+/* What a drafted tree becomes once a token has been chosen at each of its nodes.
+ * The nodes of sequence i are entries q_starts[i] .. q_starts[i+1] - 1 (one each
+ * when q_starts is NULL), at most 256, and the last positions of slot slots[i];
+ * parents as for mq_paged_tree.  The first node, the root, is accepted; from a
+ * node on, the first of its children whose token is the one chosen at the node.
+ * path: the accepted nodes' places in the tree, emitted: the tokens chosen
+ * there (the drafted ones that were right, then one more), both [total] in the
+ * layout of the nodes and -1 behind the last; count [n]: how many they are, 0
+ * for a sequence without nodes.  The accepted rows of K and V move to the
+ * tree's first positions (all layers), the sequence ends behind them, and pages
+ * past its end lose a holder.  A page that is written must have no other holder.
+ * With an index in the pool, the records of the pages that are full then are
+ * written again.  A call that is wrong anywhere changes nothing but its outputs
+ * (-1 and 0).  t->workspace: mq_paged_accept_workspace_bytes(total) bytes,
+ * aligned to 16. */
+size_t mq_paged_accept_workspace_bytes(int total);
+int mq_paged_accept(const mq_paged_pool* pool, const mq_page_table* t, const int* slots, const int* q_starts,
+                    const int* parents, const int* tokens, const int* chosen, int n, int total, int* path, int* emitted,
+                    int* count, cudaStream_t stream);
 
 /* Rotary positions, and optionally the write of the rotated K and of V into
  * the pages.  Token i sits at positions[i]; with a pool it belongs to slot
@@ -576,6 +596,43 @@ typedef struct mq_paged_sparse_params {
 
 size_t mq_paged_sparse_workspace_bytes(const mq_paged_sparse_params* params);
 int mq_paged_sparse(const mq_paged_sparse_params* params, cudaStream_t stream);
+
+/* ---- sampling --------------------------------------------------------------------
+ * A token for each of n rows of logits [n, vocab] (vocab at most 2^20), by the
+ * number u[i] in [0, 1).  With w = exp((logit - the row's largest) / temperature):
+ *   the top_k largest logits stay (0 or less, or vocab or more: all; equal ones
+ *   in the order of their numbers);
+ *   of those, in descending order, the tokens before which less than top_p times
+ *   their sum of w lies (1 or more: all), the first at least;
+ *   of those, the tokens with w >= min_p (0 or less: all).
+ * The token is the first, in ascending order of the number, up to which the sum
+ * of w over what stays exceeds u times its total.  Weights are computed in 64
+ * bits and summed exactly (as multiples of 2^-43 of the largest), so the token
+ * does not depend on an order of sums.
+ * A temperature of 0 or less takes the largest logit (the first of equal ones).
+ * A NaN counts as a logit of minus infinity, which is never drawn; a row of
+ * nothing else gives -1; an infinity leaves only its like.  NaN as a parameter:
+ * a temperature of 0, no top_p, no min_p; u below 0 or NaN counts as 0, from 1
+ * on it gives the last token that stays. */
+typedef struct mq_sample_params {
+    const void* logits;          /* [n, vocab], rows contiguous */
+    long long row_stride;        /* elements */
+    int dtype;                   /* MQ_FP32, MQ_BF16 or MQ_FP16 */
+    int n;
+    int vocab;
+    const float* u;              /* device fp32 [n] */
+    const float* temperatures;   /* device [n] each, optional: the value below for all rows */
+    const int* top_ks;
+    const float* top_ps;
+    const float* min_ps;
+    float temperature;
+    int top_k;
+    float top_p;
+    float min_p;
+    int* tokens;                 /* device int32 [n] */
+} mq_sample_params;
+
+int mq_sample(const mq_sample_params* params, cudaStream_t stream);
 
 /* Last status recorded by the reference-ABI launchers on this host thread. */
 int mq_get_last_error(void);

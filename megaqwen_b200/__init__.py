@@ -43,7 +43,7 @@ def __getattr__(name):
         return _load_native()
     if name in _NATIVE:
         return getattr(_load_native(), name)
-    if name in ("megakernel_decode", "chat", "paged"):
+    if name in ("megakernel_decode", "chat", "paged", "sampling"):
         return importlib.import_module("." + name, __name__)
     raise AttributeError(f"module 'megaqwen_b200' has no attribute {name!r}")
 

@@ -936,7 +936,8 @@ private:
     mq_decode_batch_params p_;
 };
 
-void bind_paged(py::module_& m);   // ext_paged.cpp
+void bind_paged(py::module_& m);
+void bind_sampling(py::module_& m);   // ext_sampling.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "B200 (sm_100a) Qwen3-0.6B decode engine: reference-compatible torch extension";
@@ -1024,4 +1025,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("prefill_workspace_bytes", [](int b, int s) { return (int64_t)mq_prefill_workspace_bytes(b, s); });
     m.def("version", []() { return std::string(mq_version()); });
     bind_paged(m);
+    bind_sampling(m);
 }

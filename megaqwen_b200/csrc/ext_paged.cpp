@@ -166,6 +166,35 @@ void paged_fork(Tensor k, Tensor v, Tensor table, Tensor lengths, Tensor refs, T
                            ints(children, k.device(), "children"), (int)children.numel(), stream_of(k)), "paged fork");
 }
 
+std::tuple<Tensor, Tensor, Tensor> paged_accept(Tensor k, Tensor v, Tensor table, Tensor lengths, Tensor refs, Tensor slots,
+                                                Tensor parents, Tensor tokens, Tensor chosen, OptTensor q_starts,
+                                                OptTensor index, OptTensor status) {
+    const mq_paged_pool pool = pool_of(k, v, index);
+    const auto dev = k.device();
+    on(table, dev, "page_table");
+    const int* s = ints(slots, dev, "slots");
+    const int n = (int)slots.numel();
+    const int* up = ints(parents, dev, "parents");
+    const int total = (int)parents.numel();
+    const int* tok = ints(tokens, dev, "tokens", total);
+    const int* at = ints(chosen, dev, "chosen", total);
+    const int* starts = nullptr;
+    if (q_starts.has_value()) starts = ints(*q_starts, dev, "q_starts", n + 1ll);
+    else if (n != total) fail("without q_starts, a sequence must have one node");
+    if (total && !n) fail("nodes without sequences");
+    c10::cuda::CUDAGuard guard(dev);
+    Table t(table, lengths, refs, pool.page_size, n, status, false);
+    if (refs.numel() != k.size(0)) fail("refs must have one entry per page");
+    Tensor path = blank({total}, torch::kInt32, dev), emitted = blank({total}, torch::kInt32, dev),
+           count = blank({n}, torch::kInt32, dev);
+    t.c.workspace_bytes = mq_paged_accept_workspace_bytes(total);
+    t.ws = scratch(t.c.workspace_bytes, dev);
+    t.c.workspace = t.ws.data_ptr();
+    raise_rc(mq_paged_accept(&pool, &t.c, s, starts, up, tok, at, n, total, path.data_ptr<int>(), emitted.data_ptr<int>(),
+                             count.data_ptr<int>(), stream_of(k)), "paged accept");
+    return std::make_tuple(path, emitted, count);
+}
+
 void same_pools(const mq_paged_pool& a, const mq_paged_pool& b) {
     if (a.dtype != b.dtype || a.num_layers != b.num_layers || a.num_kv_heads != b.num_kv_heads ||
         a.page_size != b.page_size || a.head_dim != b.head_dim)
@@ -473,6 +502,9 @@ void bind_paged(py::module_& m) {
           py::arg("new_lengths"), py::arg("page_size"), py::arg("status") = none);
     m.def("paged_fork", &paged_fork, py::arg("k_pages"), py::arg("v_pages"), py::arg("page_table"), py::arg("lengths"),
           py::arg("refs"), py::arg("parents"), py::arg("children"), py::arg("status") = none);
+    m.def("paged_accept", &paged_accept, py::arg("k_pages"), py::arg("v_pages"), py::arg("page_table"), py::arg("lengths"),
+          py::arg("refs"), py::arg("slots"), py::arg("parents"), py::arg("tokens"), py::arg("chosen"),
+          py::arg("q_starts") = none, py::arg("index") = none, py::arg("status") = none);
     m.def("paged_copy", &paged_copy, py::arg("k_pages"), py::arg("v_pages"), py::arg("src"), py::arg("dst"),
           py::arg("dst_k_pages") = none, py::arg("dst_v_pages") = none, py::arg("index") = none,
           py::arg("dst_index") = none, py::arg("status") = none);

@@ -122,6 +122,12 @@ __device__ __forceinline__ void st_peer(uint32_t addr, uint32_t rank, uint32_t v
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
 
+__device__ __forceinline__ void red_peer_max(uint32_t addr, uint32_t rank, int v) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+    asm volatile("red.relaxed.cluster.shared::cluster.max.s32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+
 // Every kernel here is launched as a programmatic dependent of the kernel
 // before it in the stream and begins with pdl_wait, so stream order holds and
 // only the launch itself overlaps the previous kernel's tail.
@@ -160,6 +166,10 @@ cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, unsigned ran
     cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kernel, ((KArgs)args)...);
 }
+
+// The index records of the pages whose last row is one of the n positions, in every layer (paged_rope.cu).
+int reindex(const mq_paged_pool* pool, const int* table, long long table_row, int num_slots, int cols, const int* positions,
+            const int* slots, int n, cudaStream_t st);
 
 inline bool pool_ok(const mq_paged_pool* p) {
     return p && p->k && p->v && (p->dtype == MQ_BF16 || p->dtype == MQ_FP16) && p->num_pages >= 1 && p->num_layers >= 1 &&

@@ -1,4 +1,4 @@
-// Pages of the paged KV cache: reserve, fork, free, copy, compact.
+// Pages of the paged KV cache: reserve, fork, free, copy, compact, accept.
 //
 // Bookkeeping is exact and independent of scheduling: pages are handed out
 // lowest number first, in the order of the caller's list, so two runs give the
@@ -561,6 +561,224 @@ __global__ void __launch_bounds__(MOVE_THREADS) compact_move_kernel(Geo g, Tab t
     move_units(g, pl, live, tid >> 5, nt >> 5, threadIdx.x & 31);
 }
 
+// ---- accept --------------------------------------------------------------------------
+// The drafted tree of a sequence is its last positions, the root first.  A walk starts there and goes on to the first child
+// whose token is the one chosen at the node it stands on; the rows of the nodes passed move to the tree's first positions,
+// the sequence ends behind them, and pages past its end are given back.
+//
+// One cluster plans, a warp to a sequence: the walk looks at 32 nodes at a time (a ballot finds the lowest child), which
+// is the latency of a chain of reads for each node passed.  As for free, the counts of the pages to give back are taken
+// down first, and put back where any sequence turns out wrong.  The move kernel takes (sequence, tensor, four layers, head)
+// to a warp, ACCEPT_ROWS rows of each layer in flight: a row only ever moves down, from row path[i] >= i of the tree to
+// row i, so a batch of rows that is read before it is written cannot overwrite what a later batch reads.
+constexpr int ACCEPT_TREE = 256;    // nodes
+constexpr int ACCEPT_ROWS = 8, ACCEPT_LAYERS = 4;
+
+struct AcceptArgs {
+    const int* slots;
+    const int* q_starts;
+    const int* parents;
+    const int* tokens;
+    const int* chosen;
+    int n, total;
+    int* path;
+    int* emitted;
+    int* count;
+    int* head;        // [0] the plan was accepted
+    int4* moves;      // [total] page and row read, page and row written
+    int* positions;   // [total] of the accepted tokens, or -1
+    int* token_slot;  // [total]
+};
+
+__device__ __forceinline__ int tree_start(const AcceptArgs& a, int i) { return a.q_starts ? a.q_starts[i] : i; }
+
+__global__ void __launch_bounds__(PLAN_THREADS) accept_plan_kernel(Tab t, AcceptArgs a) {
+    __shared__ unsigned bits[MAX_SLOTS / 32];
+    __shared__ int wrong;   // the highest code found
+    pdl_wait();
+    pdl_trigger();
+    const int ranks = (int)cluster_size(), rank = (int)cluster_rank();   // (the grid is one cluster)
+    const int per = blockDim.x / 32, lane = threadIdx.x & 31, warp = rank * per + (threadIdx.x >> 5), warps = ranks * per;
+    if (threadIdx.x == 0) wrong = 0;
+    int code = 0;
+    if (a.q_starts) {
+        for (int i = threadIdx.x; i < a.n; i += blockDim.x)
+            if (a.q_starts[i + 1] < a.q_starts[i]) code = MQ_ERR_INVALID_ARGUMENT;
+        if (threadIdx.x == 0 && (a.q_starts[0] != 0 || a.q_starts[a.n] != a.total)) code = MQ_ERR_INVALID_ARGUMENT;
+    }
+    bool in_order = !__syncthreads_or(code);
+    if (in_order && !slots_ok(a.slots, a.n, t.slots, bits)) {
+        in_order = false;
+        code = MQ_ERR_BAD_SLOT;
+    }
+    if (!in_order) {   // all CTAs alike
+        if (rank == 0 && code) note_status(t.status, code);
+        for (long long i = (long long)rank * blockDim.x + threadIdx.x; i < max(a.total, a.n); i += ranks * blockDim.x) {
+            if (i < a.total) a.path[i] = a.emitted[i] = -1;
+            if (i < a.n) a.count[i] = 0;
+        }
+        if (rank == 0 && threadIdx.x == 0) a.head[0] = 0;
+        return;
+    }
+    if (ranks > 1) cluster_sync();   // every CTA runs and has its `wrong`: it may be written
+    else __syncthreads();
+    const int shift = __ffs(t.page) - 1;
+    // pages of sequence s from column c0 on give up (or get back) one holder
+    auto give_back = [&](const int* row, int c0, int c1, int d) {
+        bool bad = false;
+        for (int c = c0 + lane; c < c1; c += 32) {
+            const int p = row[c];
+            if (p < 0 || p >= t.pages || atomicAdd(&t.refs[p], d) + min(d, 0) < 0) bad = true;
+        }
+        return bad;
+    };
+    for (int i = warp; i < a.n; i += warps) {
+        const int s = a.slots[i], q0 = tree_start(a, i), ql = tree_start(a, i + 1) - q0, len = t.lengths[s];
+        const int* row = t.table + s * t.row;
+        if (ql > ACCEPT_TREE) {
+            code = max(code, (int)MQ_ERR_INVALID_ARGUMENT);
+            if (lane == 0) a.count[i] = -1;
+            continue;
+        }
+        if (len < ql || pages_of(len, t.page) > t.cols) {
+            code = max(code, (int)MQ_ERR_BAD_POSITION);
+            if (lane == 0) a.count[i] = -1;
+            continue;
+        }
+        if (!ql) {
+            if (lane == 0) a.count[i] = 0;
+            continue;
+        }
+        int up[ACCEPT_TREE / 32], tok[ACCEPT_TREE / 32];
+#pragma unroll
+        for (int k = 0; k < ACCEPT_TREE / 32; ++k) {
+            const int node = k * 32 + lane;
+            up[k] = -1;
+            tok[k] = 0;
+            if (node < ql) {
+                up[k] = __ldg(a.parents + q0 + node);
+                tok[k] = __ldg(a.tokens + q0 + node);
+                if (up[k] >= node || up[k] < -1) code = max(code, (int)MQ_ERR_INVALID_ARGUMENT);
+            }
+        }
+        int at = 0, m = 0;
+        while (true) {   // a child comes after its parent, so this ends (a wrong parent is no child of it either)
+            const int want = __ldg(a.chosen + q0 + at);
+            if (lane == 0) {
+                a.path[q0 + m] = at;
+                a.emitted[q0 + m] = want;
+            }
+            ++m;
+            int next = -1;
+#pragma unroll
+            for (int k = 0; k < ACCEPT_TREE / 32; ++k) {
+                if (next >= 0 || k * 32 >= ql) break;
+                const unsigned hit = __ballot_sync(0xffffffffu, up[k] == at && tok[k] == want && k * 32 + lane > at && k * 32 + lane < ql);
+                if (hit) next = k * 32 + __ffs((int)hit) - 1;
+            }
+            if (next < 0) break;
+            at = next;
+        }
+        for (int k = m + lane; k < ql; k += 32) a.path[q0 + k] = a.emitted[q0 + k] = -1;
+        if (lane == 0) a.count[i] = m;
+        __syncwarp();
+        // the pages of the rows that move, those written with no other holder
+        const int base = len - ql;
+        bool bad = false;
+        for (int k = lane; k < m; k += 32) {
+            const int from = a.path[q0 + k];
+            if (from == k) continue;
+            const int sp = row[(base + from) >> shift], dp = row[(base + k) >> shift];
+            if (sp < 0 || sp >= t.pages || dp < 0 || dp >= t.pages || t.refs[dp] != 1) bad = true;
+        }
+        if (give_back(row, pages_of(base + m, t.page), pages_of(len, t.page), -1)) bad = true;
+        if (bad) code = max(code, (int)MQ_ERR_BAD_PAGE);
+    }
+    if (code) atomicMax(&wrong, code);
+    __syncthreads();
+    if (ranks > 1) {
+        const int mine = wrong;
+        __syncthreads();
+        if (mine && threadIdx.x < ranks) red_peer_max(smem_u32(&wrong), threadIdx.x, mine);
+        __syncwarp();
+        cluster_sync();   // also orders the counts taken before those put back
+    }
+    code = *(volatile int*)&wrong;
+    if (rank == 0 && threadIdx.x == 0) {
+        if (code) note_status(t.status, code);
+        a.head[0] = code == 0;
+    }
+    for (int i = warp; i < a.n; i += warps) {
+        const int s = a.slots[i], q0 = tree_start(a, i), ql = tree_start(a, i + 1) - q0, len = t.lengths[s], m = a.count[i];
+        int* row = t.table + s * t.row;
+        const int base = len - ql, keep = pages_of(base + m, t.page), used = pages_of(len, t.page);
+        __syncwarp();
+        if (code) {
+            if (m > 0) give_back(row, keep, used, 1);   // (below 1: its pages were not looked at)
+            for (int k = lane; k < ql; k += 32) a.path[q0 + k] = a.emitted[q0 + k] = -1;
+            if (lane == 0) a.count[i] = 0;
+            continue;
+        }
+        if (!ql) continue;
+        for (int k = lane; k < ql; k += 32) {
+            int4 mv = make_int4(-1, 0, -1, 0);
+            const int from = k < m ? a.path[q0 + k] : k;
+            if (from != k) {
+                const int sp = base + from, dp = base + k;
+                mv = make_int4(row[sp >> shift], sp & (t.page - 1), row[dp >> shift], dp & (t.page - 1));
+            }
+            a.moves[q0 + k] = mv;
+            a.positions[q0 + k] = k < m ? base + k : -1;
+            a.token_slot[q0 + k] = s;
+        }
+        __syncwarp();
+        for (int c = keep + lane; c < used; c += 32) row[c] = -1;
+        if (lane == 0) t.lengths[s] = base + m;
+    }
+}
+
+template <int D>
+__global__ void __launch_bounds__(MOVE_THREADS) accept_move_kernel(Geo g, AcceptArgs a) {
+    constexpr int LPR = D / 8, SIDE = 32 / LPR, STEPS = ACCEPT_ROWS / SIDE;   // lanes to a row, rows side by side
+    pdl_wait();
+    pdl_trigger();
+    if (!a.head[0]) return;
+    const int lane = threadIdx.x & 31, piece = lane % LPR, sub = lane / LPR;
+    const long long wid = ((long long)blockIdx.x * MOVE_THREADS + threadIdx.x) >> 5, nw = (long long)gridDim.x * MOVE_THREADS >> 5;
+    const int chunks = ceil_div(g.layers, ACCEPT_LAYERS), per = 2 * chunks * g.heads;
+    for (long long u = wid; u < (long long)a.n * per; u += nw) {
+        const int i = (int)(u / per), r = (int)(u - (long long)i * per), h = r % g.heads, lc = r / g.heads % chunks;
+        const Side& side = g.src[r / (g.heads * chunks)];
+        const int m = a.count[i];
+        if (m < 2) continue;
+        const int4* mv = a.moves + tree_start(a, i);
+        const int l0 = lc * ACCEPT_LAYERS, layers = min(ACCEPT_LAYERS, g.layers - l0);
+        char* at = side.base + l0 * side.layer + h * side.head + piece * 16;
+#pragma unroll 1
+        for (int k = 1; k < m; k += ACCEPT_ROWS) {   // (the root is in its place)
+            uint4 v[STEPS][ACCEPT_LAYERS];
+            char* to[STEPS];
+#pragma unroll
+            for (int x = 0; x < STEPS; ++x) {
+                const int j = k + x * SIDE + sub;
+                const int4 e = j < m ? mv[j] : make_int4(-1, 0, -1, 0);
+                to[x] = e.x >= 0 ? at + e.z * side.page + e.w * (D * 2) : nullptr;
+                const char* from = at + e.x * side.page + e.y * (D * 2);
+#pragma unroll
+                for (int l = 0; l < ACCEPT_LAYERS; ++l)
+                    if (e.x >= 0 && l < layers) v[x][l] = *reinterpret_cast<const uint4*>(from + l * side.layer);
+            }
+            __syncwarp();   // every row of the batch is read
+#pragma unroll
+            for (int x = 0; x < STEPS; ++x)
+#pragma unroll
+                for (int l = 0; l < ACCEPT_LAYERS; ++l)
+                    if (to[x] && l < layers) *reinterpret_cast<uint4*>(to[x] + l * side.layer) = v[x][l];
+            __syncwarp();
+        }
+    }
+}
+
 bool tab_ok(const mq_page_table* t, int n, bool lengths) {
     return t && t->table && (t->lengths || !lengths) && t->refs && t->num_slots >= 1 && t->num_slots <= MAX_SLOTS &&
            t->cols >= 1 && t->num_pages >= 1 && t->num_pages <= MAX_PAGES && t->row_stride >= t->cols && n >= 0 && n <= t->num_slots &&
@@ -653,6 +871,38 @@ int mq_paged_compact(const mq_paged_pool* src, const mq_paged_pool* dst, const m
         e = launch(compact_move_kernel, dim3(move_grid()), dim3(MOVE_THREADS), 0, st, g, tab_of(t),
                    dst->num_pages, out_table, out_row_stride, out_refs, pl);
     return done(e, "paged compact");
+}
+
+size_t mq_paged_accept_workspace_bytes(int total) { return total < 0 ? 0 : 256 + (size_t)total * (sizeof(int4) + 2 * sizeof(int)); }
+
+int mq_paged_accept(const mq_paged_pool* pool, const mq_page_table* t, const int* slots, const int* q_starts,
+                    const int* parents, const int* tokens, const int* chosen, int n, int total, int* path, int* emitted,
+                    int* count, cudaStream_t st) {
+    if (!pool_ok(pool) || !tab_ok(t, n, true) || pool->num_pages != t->num_pages || pool->page_size != t->page_size || total < 0 ||
+        (n && (!slots || !count)) || (!q_starts && n != total) || (total && (!n || !parents || !tokens || !chosen || !path || !emitted)))
+        return MQ_ERR_INVALID_ARGUMENT;
+    if (!n) return MQ_OK;
+    if (!t->workspace || (reinterpret_cast<uintptr_t>(t->workspace) & 15) ||
+        t->workspace_bytes < mq_paged_accept_workspace_bytes(total))
+        return MQ_ERR_WORKSPACE;
+    AcceptArgs a = {slots, q_starts, parents, tokens, chosen, n, total, path, emitted, count};
+    a.head = (int*)t->workspace;
+    a.moves = (int4*)((char*)t->workspace + 256);
+    a.positions = (int*)(a.moves + total);
+    a.token_slot = a.positions + total;
+    unsigned ranks = 1;   // a warp to a sequence, as for free
+    while (ranks < 8 && (int)ranks * PLAN_WARPS < n) ranks *= 2;
+    const unsigned threads = n <= 8 ? 256 : PLAN_THREADS;
+    cudaError_t e = launch_cluster(accept_plan_kernel, ranks, ranks, dim3(threads), 0, st, tab_of(t), a);
+    if (e != cudaSuccess) return mq::note_cuda(e, "paged accept");
+    if (!total) return MQ_OK;
+    const Geo g = geo_of(pool, pool, false);
+    const long long units = (long long)n * 2 * ceil_div(g.layers, ACCEPT_LAYERS) * g.heads;
+    const unsigned grid = (unsigned)std::min<long long>((units + MOVE_THREADS / 32 - 1) / (MOVE_THREADS / 32), move_grid());
+    e = pool->head_dim == 128 ? launch(accept_move_kernel<128>, dim3(grid), dim3(MOVE_THREADS), 0, st, g, a)
+                              : launch(accept_move_kernel<64>, dim3(grid), dim3(MOVE_THREADS), 0, st, g, a);
+    if (e != cudaSuccess) return mq::note_cuda(e, "paged accept");
+    return pool->index ? reindex(pool, t->table, t->row_stride, t->num_slots, t->cols, a.positions, a.token_slot, total, st) : MQ_OK;
 }
 
 }  // extern "C"

@@ -322,6 +322,14 @@ __global__ void __launch_bounds__(INDEX_THREADS) index_kernel(const RopeArgs a, 
 }
 
 template <typename T>
+cudaError_t index_layer(const mq_paged_pool* p, const RopeArgs& a, int layer, int n, cudaStream_t st) {
+    signed char* ix = p->index + layer * p->i_layer;
+    const dim3 chunks(ceil_div(n, INDEX_TOKENS), p->num_kv_heads);
+    return p->head_dim == 128 ? launch(index_kernel<T, 128>, chunks, dim3(INDEX_THREADS), 0, st, a, n, ix, p->i_page, p->i_head)
+                              : launch(index_kernel<T, 64>, chunks, dim3(INDEX_THREADS), 0, st, a, n, ix, p->i_page, p->i_head);
+}
+
+template <typename T>
 int run_rope(const mq_rope_params* p, const RopeArgs& a, bool vec, cudaStream_t st) {
     const int D = p->head_dim;
     const dim3 grid(std::min(p->n, 8 * sm_count()));
@@ -336,11 +344,31 @@ int run_rope(const mq_rope_params* p, const RopeArgs& a, bool vec, cudaStream_t 
                            : launch(rope_kernel<T, 64, false>, grid, dim3(ROPE_THREADS), 0, st, a, p->n);
     if (e != cudaSuccess) return note_cuda(e, "rope");
     if (!p->pool || !p->pool->index) return MQ_OK;
-    signed char* ix = p->pool->index + p->layer * p->pool->i_layer;
-    const dim3 chunks(ceil_div(p->n, INDEX_TOKENS), p->pool->num_kv_heads);
-    e = D == 128 ? launch(index_kernel<T, 128>, chunks, dim3(INDEX_THREADS), 0, st, a, p->n, ix, p->pool->i_page, p->pool->i_head)
-                 : launch(index_kernel<T, 64>, chunks, dim3(INDEX_THREADS), 0, st, a, p->n, ix, p->pool->i_page, p->pool->i_head);
+    e = index_layer<T>(p->pool, a, p->layer, p->n, st);
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "page index");
+}
+
+int reindex(const mq_paged_pool* p, const int* table, long long table_row, int num_slots, int cols, const int* positions,
+            const int* slots, int n, cudaStream_t st) {
+    RopeArgs a = {};
+    a.positions = positions;
+    a.slots = slots;
+    a.max_pos = 0x7fffffff;
+    a.kp_page = p->k_page;
+    a.kp_head = p->k_head;
+    a.table = table;
+    a.table_row = table_row;
+    a.slots_n = num_slots;
+    a.cols = cols;
+    a.pages = p->num_pages;
+    a.page = p->page_size;
+    a.shift = __builtin_ctz((unsigned)p->page_size);
+    for (int l = 0; l < p->num_layers; ++l) {
+        a.kp = (uint16_t*)p->k + l * p->k_layer;
+        const cudaError_t e = p->dtype == MQ_BF16 ? index_layer<__nv_bfloat16>(p, a, l, n, st) : index_layer<__half>(p, a, l, n, st);
+        if (e != cudaSuccess) return note_cuda(e, "page index");
+    }
+    return MQ_OK;
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

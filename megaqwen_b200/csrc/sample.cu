@@ -1,0 +1,551 @@
+// A token for each row of logits: temperature, top-k, top-p and min-p, drawn
+// with a given number per row.
+//
+// Mathematics: w_i = 2^((l_i - max) log2(e) / T).  Tokens in descending order of
+// their logit, equal ones in ascending order of their number; the first top_k
+// stay; of those the ones before which less than top_p of their sum lies; of
+// those the ones with w >= min_p.  The token is the first, in ascending order of
+// the number, up to which the sum of what stays exceeds u times its total.
+//
+// Every one of these is a border between tokens, so the answer has to be that of
+// the definition and not of an order of sums: a token's place in the order is a
+// whole number (its logit's bits, made to ascend, over its number turned
+// around), and its weight is computed in 64 bits and held as a multiple of
+// 2^-43, so that sums are exact, in any order, up to 2^20 tokens.  In 32 bits a
+// flat row of 152k tokens would get another token once in a hundred draws.
+//
+// Bound: HBM reads the row once, 4 or 2 bytes a token; what is done with it costs
+// more.  A cluster of up to 8 CTAs takes a row, each a contiguous share of it,
+// and keeps it in shared memory, so that the passes (maximum; a histogram over
+// the logits; the tokens of the bin in which a border lies, sorted; the sums)
+// stay on the SMs.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "paged_common.cuh"
+
+namespace mq {
+namespace sampling {
+
+using paged::allow_smem;
+using paged::ceil_div;
+using paged::cluster_rank;
+using paged::cluster_size;
+using paged::cluster_sync;
+using paged::launch_cluster;
+using paged::SmemLimit;
+using paged::sm_count;
+
+using u64 = unsigned long long;
+
+constexpr int NT = 512, NW = NT / 32;
+constexpr int BINS = 2048;          // four to a thread
+constexpr int CAP = 1024;           // tokens that are sorted
+constexpr int MAX_RANKS = 8;
+constexpr int FRAC = 43;            // a weight of 1 is 2^43
+constexpr int MAX_VOCAB = 1 << 20;  // a row's sum stays below 2^63
+constexpr float COUNT_SPAN = 40.f;  // logits below the maximum that the histogram of a count spreads over its bins
+constexpr double MASS_SPAN = 44.0;  // octaves below the maximum past which a weight is nothing
+
+struct Args {
+    const void* logits;
+    long long row;        // elements between rows
+    int n, vocab, share;  // share: tokens to a CTA
+    const float* u;
+    const float* temperature;   // per row, or null for the value
+    const int* top_k;
+    const float* top_p;
+    const float* min_p;
+    float temperature_v, top_p_v, min_p_v;
+    int top_k_v;
+    int* out;
+};
+
+template <typename T>
+__device__ __forceinline__ float up(T x);
+template <>
+__device__ __forceinline__ float up(float x) { return x; }
+template <>
+__device__ __forceinline__ float up(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float up(__half x) { return __half2float(x); }
+
+__device__ __forceinline__ uint32_t order_key(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ u64 place_key(float x, int token) { return (u64)order_key(x) << 32 | (uint32_t)~token; }
+__device__ __forceinline__ int token_of(u64 key) { return (int)~(uint32_t)key; }
+__device__ __forceinline__ float logit_of(u64 key) {
+    const uint32_t k = (uint32_t)(key >> 32);
+    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
+// Remote shared memory of the cluster.
+__device__ __forceinline__ uint32_t peer(const void* p, uint32_t rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ void peer_st(uint32_t at, u64 v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
+}
+__device__ __forceinline__ uint4 peer_ld4(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t peer_ld(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
+// What a CTA needs beside its share of the row.
+struct Shared {
+    uint32_t count[BINS];             // of this CTA
+    uint32_t low[BINS], high[BINS];   // its weights' sums
+    u64 list[CAP];
+    u64 slot[2][MAX_RANKS][4];        // what the CTAs tell each other, two turns of it
+    u64 warp_sum[NW];
+    u64 found[4];
+    double two_to[32];                // 2^(j / 32)
+    int taken;
+};
+
+// The row's weights.  2^y by a table of 2^(j / 32) and the Taylor polynomial of 2^f, |f| <= 1 / 64, up to f^5 (the next
+// term is below 2^-48).
+struct Weight {
+    double scale, top;   // log2(e) / T; the maximum
+    float max;
+    __device__ __forceinline__ double octaves(float l) const { return l == max ? 0.0 : ((double)l - top) * scale; }
+    __device__ __forceinline__ u64 of(double y, const double* two_to) const {
+        if (!(y > -(double)FRAC - 1.0)) return 0;
+        constexpr double MAGIC = 6755399441055744.0;   // 1.5 x 2^52: rounds to whole numbers
+        const double t = fma(y, 32.0, MAGIC), f = fma(t - MAGIC, -1.0 / 32.0, y);
+        const int n = __double2loint(t);
+        double p = 1.3333558146428443e-03;             // ln(2)^k / k!
+        p = fma(p, f, 9.6181291076284772e-03);
+        p = fma(p, f, 5.5504108664821580e-02);
+        p = fma(p, f, 2.4022650695910071e-01);
+        p = fma(p, f, 6.9314718055994531e-01);
+        p = fma(p, f, 1.0) * two_to[n & 31];
+        const u64 b = (u64)__double_as_longlong(p);
+        const int s = 52 - FRAC - ((int)(b >> 52) - 1023) - (n >> 5);   // 9 or more: rounded to the nearest
+        return ((b & 0xfffffffffffffull | 1ull << 52) + (1ull << (s - 1))) >> s;
+    }
+    __device__ __forceinline__ u64 of(float l, const double* two_to) const { return of(octaves(l), two_to); }
+};
+
+// Exclusive sum over the CTA's threads; total for every thread.
+template <typename V>
+__device__ __forceinline__ V block_scan(V v, u64* sm, V* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    V x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const V y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) sm[warp] = x;
+    __syncthreads();
+    V before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        const V s = (V)sm[w];
+        if (w < warp) before += s;
+        all += s;
+    }
+    __syncthreads();
+    *total = all;
+    return before + x - v;
+}
+
+// list[0 .. n - 1] in descending order, n <= CAP; the places up to the next power of two are filled with 0.
+__device__ __forceinline__ void sort_down(u64* list, int n) {
+    int size = 32;
+    while (size < n) size <<= 1;
+    for (int i = n + threadIdx.x; i < size; i += NT) list[i] = 0;
+    __syncthreads();
+    for (int k = 2; k <= size; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            for (int i = threadIdx.x; i < size / 2; i += NT) {
+                const int a = 2 * i - (i & (j - 1)), b = a + j;   // a has bit j clear
+                const u64 x = list[a], y = list[b];
+                if ((x < y) == ((a & k) == 0)) {
+                    list[a] = y;
+                    list[b] = x;
+                }
+            }
+            __syncthreads();
+        }
+}
+
+template <typename T, bool NEAR>   // NEAR: the share of the row stays in shared memory
+__global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
+    extern __shared__ __align__(16) uint8_t sample_raw[];
+    Shared& s = *reinterpret_cast<Shared*>(sample_raw);
+    pdl_wait();
+    pdl_trigger();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int ranks = (int)cluster_size(), rank = (int)cluster_rank();
+    const int r = blockIdx.x / ranks;
+    const T* row = reinterpret_cast<const T*>(a.logits) + (long long)r * a.row;
+    const int lo = min(a.vocab, rank * a.share), n = min(a.vocab, lo + a.share) - lo;
+    const T* x = row + lo;
+    if (tid < 32) s.two_to[tid] = exp2((double)tid / 32.0);
+    // the share, 16 bytes at a time, where it lies as in global memory to 16 bytes
+    u64 best = 0;
+    float least = INFINITY;
+    auto look = [&](float v, int i) {
+        v = v == v ? v + 0.f : -INFINITY;   // NaN is never drawn; -0 is 0
+        best = max(best, place_key(v, lo + i));
+        if (v > -INFINITY) least = fminf(least, v);
+    };
+    constexpr int PER = 16 / sizeof(T);
+    const int off = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));   // elements past a 16-byte border
+    T* near = reinterpret_cast<T*>(sample_raw + ((sizeof(Shared) + 15) & ~(size_t)15));
+    {
+        const int head = min(n, off ? PER - off : 0), body = (n - head) / PER, tail = n - head - body * PER;
+        if (tid < head) {
+            look(up(x[tid]), tid);
+            if (NEAR) near[off + tid] = x[tid];
+        }
+        const uint4* from = reinterpret_cast<const uint4*>(x + head);
+        uint4* to = reinterpret_cast<uint4*>(near + (off ? PER : 0));
+        constexpr int DEEP = 4;
+        for (int i0 = tid; i0 < body; i0 += NT * DEEP) {
+            uint4 v[DEEP];
+#pragma unroll
+            for (int k = 0; k < DEEP; ++k)
+                if (i0 + k * NT < body) v[k] = __ldg(from + i0 + k * NT);
+#pragma unroll
+            for (int k = 0; k < DEEP; ++k) {
+                const int i = i0 + k * NT;
+                if (i >= body) break;
+                if (NEAR) to[i] = v[k];
+                const T* e = reinterpret_cast<const T*>(&v[k]);
+#pragma unroll
+                for (int c = 0; c < PER; ++c) look(up(e[c]), head + i * PER + c);
+            }
+        }
+        if (tid < tail) {
+            const int i = head + body * PER + tid;
+            look(up(x[i]), i);
+            if (NEAR) near[off + i] = x[i];
+        }
+    }
+    auto at = [&](int i) -> float {
+        const float v = NEAR ? up(near[off + i]) : up(__ldg(x + i));
+        return v == v ? v + 0.f : -INFINITY;
+    };
+    int turn = 0;
+    // every CTA's four words to every CTA, all threads' writes before visible to all
+    auto tell = [&](u64 v0, u64 v1, u64 v2, u64 v3) {   // the values of thread 0
+        if (tid == 0) s.found[0] = v0, s.found[1] = v1, s.found[2] = v2, s.found[3] = v3;
+        __syncthreads();
+        turn ^= 1;
+        if (tid < 4 * ranks) peer_st(peer(&s.slot[turn][rank][tid & 3], tid >> 2), s.found[tid & 3]);
+        cluster_sync();
+    };
+    {   // the maximum and the smallest finite logit
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+            least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+        }
+        if (lane == 0) {
+            s.warp_sum[warp] = best;
+            s.list[warp] = order_key(least);
+        }
+        __syncthreads();
+        u64 b = 0, l = ~0ull;
+        for (int w = 0; w < NW; ++w) {
+            b = max(b, s.warp_sum[w]);
+            l = min(l, s.list[w]);
+        }
+        if (ranks > 1) cluster_sync();   // every CTA runs: its shared memory may be written
+        tell(b, l, 0, 0);
+        best = 0;
+        l = ~0ull;
+        for (int c = 0; c < ranks; ++c) {
+            best = max(best, s.slot[turn][c][0]);
+            l = min(l, s.slot[turn][c][1]);
+        }
+        least = logit_of(l << 32);
+    }
+    const float top = logit_of(best);
+    const float temp = a.temperature ? __ldg(a.temperature + r) : a.temperature_v;
+    if (!(temp > 0.f) || top == -INFINITY) {   // all CTAs alike
+        if (rank == 0 && tid == 0) a.out[r] = top == -INFINITY ? -1 : token_of(best);
+        return;
+    }
+    const int top_k = a.top_k ? __ldg(a.top_k + r) : a.top_k_v;
+    const float top_p = a.top_p ? __ldg(a.top_p + r) : a.top_p_v;
+    const float min_p = a.min_p ? __ldg(a.min_p + r) : a.min_p_v;
+    const float u = __ldg(a.u + r);
+    const bool by_count = top_k > 0 && top_k < a.vocab, by_mass = top_p < 1.f;
+    const Weight w = {1.4426950408889634 / (double)temp, (double)top, top};
+    const double floor_y = min_p > 0.f ? log2((double)fminf(min_p, 1.f)) : -INFINITY;
+
+    u64 bar = 0;   // tokens whose key is below this are out
+    // The key of the last token that stays: by count the want-th, by mass the last one before which less than top_p of the
+    // sum lies.  `before` of it (tokens or weight) has passed when the keys from lo_key to hi_key begin.
+    auto border = [&](bool mass, u64 want) -> u64 {
+        // first level: bins of equal width in the logit, from the maximum down
+        const float span = fminf(top - least, mass ? (float)(MASS_SPAN / w.scale) : COUNT_SPAN);
+        const float fine = span > 0.f ? (float)BINS / span : 0.f;
+        auto bin_of = [&](float l) -> int {
+            const float d = (top - l) * fine;   // (the maximum at +infinity: NaN for itself, +infinity for others)
+            return l == top ? 0 : d < (float)(BINS - 1) ? (int)d : BINS - 1;
+        };
+        u64 lo_key = 0, hi_key = ~0ull, before = 0, target = want, count = 0;
+        bool first = true;
+        int bin = 0, shift = 0;
+        while (true) {
+            for (int i = tid; i < BINS; i += NT) s.count[i] = s.low[i] = s.high[i] = 0;
+            __syncthreads();
+            for (int i = tid; i < n; i += NT) {
+                const float l = at(i);
+                const u64 key = place_key(l, lo + i);
+                if (key < bar || key < lo_key || key > hi_key) continue;
+                const int b = first ? bin_of(l) : (int)((hi_key - key) >> shift);
+                atomicAdd(&s.count[b], 1u);
+                if (mass) {
+                    const u64 v = w.of(l, s.two_to);
+                    if (v) {
+                        const uint32_t lo32 = (uint32_t)v, old = atomicAdd(&s.low[b], lo32);
+                        const uint32_t hi32 = (uint32_t)(v >> 32) + (old + lo32 < old ? 1u : 0u);
+                        if (hi32) atomicAdd(&s.high[b], hi32);
+                    }
+                }
+            }
+            if (ranks > 1) cluster_sync();
+            else __syncthreads();
+            // four bins to a thread, over all CTAs
+            uint32_t c4[4] = {0, 0, 0, 0};
+            u64 m4[4] = {0, 0, 0, 0};
+            for (int c = 0; c < ranks; ++c) {
+                const uint4 q = peer_ld4(peer(&s.count[4 * tid], c));
+                c4[0] += q.x, c4[1] += q.y, c4[2] += q.z, c4[3] += q.w;
+                if (mass) {
+                    const uint4 l = peer_ld4(peer(&s.low[4 * tid], c)), h = peer_ld4(peer(&s.high[4 * tid], c));
+                    m4[0] += (u64)h.x << 32 | l.x, m4[1] += (u64)h.y << 32 | l.y;
+                    m4[2] += (u64)h.z << 32 | l.z, m4[3] += (u64)h.w << 32 | l.w;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (!mass) m4[k] = c4[k];
+            u64 total;
+            u64 at_bin = before + block_scan<u64>(m4[0] + m4[1] + m4[2] + m4[3], s.warp_sum, &total);
+            if (mass && first) {
+                // a token stays while less than top_p of the sum lies before it: the border is the last one before which
+                // less than `target` units lie
+                const double t = (double)top_p * (double)total;
+                target = t > 0.0 ? (u64)ceil(t) : 0;
+                target = max(target, 1ull);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (at_bin < target && target <= at_bin + m4[k]) {
+                    s.found[0] = 4 * tid + k;
+                    s.found[1] = at_bin;
+                    s.found[2] = c4[k];
+                }
+                at_bin += m4[k];
+            }
+            __syncthreads();
+            bin = (int)s.found[0];
+            before = s.found[1];
+            count = s.found[2];
+            __syncthreads();
+            if (count <= CAP) break;
+            // too many: the keys of the bin, cut again
+            if (first) {
+                u64 kl = ~0ull, kh = 0;
+                for (int i = tid; i < n; i += NT) {
+                    const float l = at(i);
+                    const u64 key = place_key(l, lo + i);
+                    if (key < bar || bin_of(l) != bin) continue;
+                    kl = min(kl, key);
+                    kh = max(kh, key);
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    kl = min(kl, __shfl_xor_sync(0xffffffffu, kl, o));
+                    kh = max(kh, __shfl_xor_sync(0xffffffffu, kh, o));
+                }
+                if (lane == 0) {
+                    s.warp_sum[warp] = kl;
+                    s.list[warp] = kh;
+                }
+                __syncthreads();
+                for (int k = 0; k < NW; ++k) {
+                    kl = min(kl, s.warp_sum[k]);
+                    kh = max(kh, s.list[k]);
+                }
+                tell(kl, kh, 0, 0);
+                lo_key = ~0ull;
+                hi_key = 0;
+                for (int c = 0; c < ranks; ++c) {
+                    lo_key = min(lo_key, s.slot[turn][c][0]);
+                    hi_key = max(hi_key, s.slot[turn][c][1]);
+                }
+            } else {
+                hi_key -= (u64)bin << shift;
+                lo_key = max(lo_key, hi_key - ((1ull << shift) - 1));
+                if (ranks > 1) cluster_sync();   // the counts are read before they are cleared
+            }
+            first = false;
+            const u64 range = hi_key - lo_key;
+            shift = max(0, 64 - __clzll((long long)range) - 11);   // 2048 bins
+        }
+        // the bin's tokens, in every CTA's list
+        if (!first) {
+            hi_key -= (u64)bin << shift;
+            lo_key = max(lo_key, hi_key - ((1ull << shift) - 1));
+        }
+        uint32_t base = 0;
+        for (int c = 0; c < rank; ++c) base += peer_ld(peer(&s.count[bin], c));
+        if (tid == 0) s.taken = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += NT) {
+            const float l = at(i);
+            const u64 key = place_key(l, lo + i);
+            if (key < bar || key < lo_key || key > hi_key || (first && bin_of(l) != bin)) continue;
+            const uint32_t place = base + atomicAdd(&s.taken, 1);
+            for (int c = 0; c < ranks; ++c) peer_st(peer(&s.list[place], c), key);
+        }
+        if (ranks > 1) cluster_sync();
+        else __syncthreads();
+        sort_down(s.list, (int)count);
+        if (!mass) {
+            const u64 key = s.list[target - before - 1];
+            __syncthreads();
+            return key;
+        }
+        // the last of the list before which less than `target` lies
+        constexpr int EACH = CAP / NT;
+        u64 v[EACH], sum = 0, total;
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) {
+            const int i = tid * EACH + k;
+            v[k] = i < (int)count ? w.of(logit_of(s.list[i]), s.two_to) : 0;
+            sum += v[k];
+        }
+        u64 lies = before + block_scan<u64>(sum, s.warp_sum, &total);
+        uint32_t last = 0;
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) {
+            const int i = tid * EACH + k;
+            if (i < (int)count && lies < target) last = i + 1;
+            lies += v[k];
+        }
+        last = __reduce_max_sync(0xffffffffu, last);
+        if (lane == 0) s.warp_sum[warp] = last;
+        __syncthreads();
+        u64 most = 1;
+        for (int k = 0; k < NW; ++k) most = max(most, s.warp_sum[k]);
+        const u64 key = s.list[most - 1];
+        __syncthreads();
+        return key;
+    };
+    if (by_count) bar = border(false, (u64)top_k);
+    if (by_mass) bar = border(true, 0);
+
+    // the sums of what stays, in the order of the tokens: a contiguous piece to a warp
+    auto weight_at = [&](int i) -> u64 {
+        const float l = at(i);
+        if (place_key(l, lo + i) < bar) return 0;
+        const double y = w.octaves(l);
+        return y >= floor_y ? w.of(y, s.two_to) : 0;
+    };
+    const int piece = ceil_div(ceil_div(max(n, 1), NW), 32) * 32, i0 = min(n, warp * piece), i1 = min(n, i0 + piece);
+    u64 sum = 0;
+    for (int i = i0 + lane; i < i1; i += 32) sum += weight_at(i);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) s.warp_sum[warp] = sum;
+    __syncthreads();
+    u64 mine = 0;
+    for (int k = 0; k < NW; ++k) mine += s.warp_sum[k];
+    tell(mine, 0, 0, 0);
+    u64 total = 0, begin = 0;
+    for (int c = 0; c < ranks; ++c) {
+        if (c == rank) begin = total;
+        total += s.slot[turn][c][0];
+    }
+    const double aim = (u > 0.f ? (double)u : 0.0) * (double)total;   // (NaN counts as 0)
+    const u64 target = aim < (double)total ? min((u64)aim, total - 1) : total - 1;   // the first sum above it
+    if (target < begin || target - begin >= mine) return;
+    u64 passed = begin;
+    int k = 0;
+    for (; k < NW - 1 && target >= passed + s.warp_sum[k]; ++k) passed += s.warp_sum[k];
+    __syncthreads();
+    // the piece, over all threads
+    const int p0 = min(n, k * piece), p1 = min(n, p0 + piece), each = ceil_div(p1 - p0, NT);
+    const int j0 = min(p1, p0 + tid * each), j1 = min(p1, j0 + each);
+    sum = 0;
+    for (int i = j0; i < j1; ++i) sum += weight_at(i);
+    u64 all;
+    u64 here = passed + block_scan<u64>(sum, s.warp_sum, &all);
+    if (here <= target && target < here + sum)
+        for (int i = j0; i < j1; ++i) {
+            here += weight_at(i);
+            if (target < here) {
+                a.out[r] = lo + i;
+                break;
+            }
+        }
+}
+
+size_t smem_of(int share, int size, bool near) {
+    return ((sizeof(Shared) + 15) & ~(size_t)15) + (near ? (size_t)share * size + 32 : 0);
+}
+
+template <typename T>
+int run(Args a, cudaStream_t st) {
+    // as many CTAs to a row as leave each 4096 tokens or more
+    unsigned ranks = 1;
+    while (ranks < MAX_RANKS && a.vocab > 4096 * (int)ranks) ranks *= 2;
+    a.share = (ceil_div(a.vocab, (int)ranks) + 7) & ~7;
+    const bool near = smem_of(a.share, sizeof(T), true) <= 220 * 1024;
+    const size_t smem = smem_of(a.share, sizeof(T), near);
+    static SmemLimit limits[2];
+    const auto kernel = near ? sample_kernel<T, true> : sample_kernel<T, false>;
+    cudaError_t e = allow_smem(kernel, smem, limits[near]);
+    if (e == cudaSuccess) e = launch_cluster(kernel, (unsigned)a.n * ranks, ranks, dim3(NT), smem, st, a);
+    return e == cudaSuccess ? MQ_OK : note_cuda(e, "sample");
+}
+
+}  // namespace sampling
+}  // namespace mq
+
+extern "C" int mq_sample(const mq_sample_params* p, cudaStream_t st) {
+    if (!p || p->n < 0 || p->vocab < 1 || p->vocab > mq::sampling::MAX_VOCAB || p->n > (1 << 24)) return MQ_ERR_INVALID_ARGUMENT;
+    if (!p->n) return MQ_OK;
+    const size_t size = p->dtype == MQ_FP32 ? 4 : 2;
+    if (!p->logits || !p->u || !p->tokens || (reinterpret_cast<uintptr_t>(p->logits) % size) ||
+        (p->dtype != MQ_FP32 && p->dtype != MQ_BF16 && p->dtype != MQ_FP16))
+        return MQ_ERR_INVALID_ARGUMENT;
+    mq::sampling::Args a = {};
+    a.logits = p->logits;
+    a.row = p->row_stride;
+    a.n = p->n;
+    a.vocab = p->vocab;
+    a.u = p->u;
+    a.temperature = p->temperatures;
+    a.top_k = p->top_ks;
+    a.top_p = p->top_ps;
+    a.min_p = p->min_ps;
+    a.temperature_v = p->temperature;
+    a.top_k_v = p->top_k;
+    a.top_p_v = p->top_p;
+    a.min_p_v = p->min_p;
+    a.out = p->tokens;
+    return p->dtype == MQ_FP32   ? mq::sampling::run<float>(a, st)
+           : p->dtype == MQ_BF16 ? mq::sampling::run<__nv_bfloat16>(a, st)
+                                 : mq::sampling::run<__half>(a, st);
+}

@@ -20,6 +20,7 @@ synchronises, and outputs come from the current stream's allocator):
 ``sparse_attend``  attention over the pages that a cheap score selects
 ``window_attend``  attention over the last positions and a few first ones (sinks)
 ``tree_attend``    attention of a tree of drafted tokens
+``accept``         the tree's accepted path, and the cache cut down to it
 
 Arguments that live on the GPU are checked there: a wrong slot, page or
 position writes its code to ``status`` (int32 ``[1]``, if given) and changes no
@@ -48,6 +49,7 @@ attend = _C.paged_attend
 sparse_attend = _C.paged_sparse_attend
 window_attend = _C.paged_window_attend
 tree_attend = _C.paged_tree_attend
+accept = _C.paged_accept
 
 INDEX_PAD = 16   # bytes of an index record after the two bounds: the exponent and padding
 
@@ -178,6 +180,13 @@ class PagedKVCache:
 
     def free(self, slots) -> None:
         free(self.page_table, self.lengths, self.refs, self._ints(slots), self.page_size, status=self.status)
+
+    def accept(self, slots, parents, tokens, chosen, q_starts=None):
+        """The drafted trees that end the named sequences, cut down to what was chosen: (path, emitted, count) as for
+        :func:`accept`."""
+        return accept(self.k_pages, self.v_pages, self.page_table, self.lengths, self.refs, self._ints(slots),
+                      self._ints(parents), self._ints(tokens), self._ints(chosen),
+                      q_starts=None if q_starts is None else self._ints(q_starts), index=self.index, status=self.status)
 
     def compact(self, num_pages: int) -> "PagedKVCache":
         """This cache with its pages in use gathered into a pool of num_pages.  Where they do not fit, both caches'

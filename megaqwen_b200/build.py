@@ -37,7 +37,7 @@ CUDA_SOURCES = ["decode.cu", "prefill.cu", "decode_batch.cu", "paged_pages.cu", 
                 "sample.cu"]
 EXT_SOURCES = ["ext.cpp", "ext_paged.cpp", "ext_sampling.cpp"]
 CUDA_HEADERS = ["mq_ptx.cuh", "mq_tc.cuh", "gemm_tc.cuh", "gemm_small.cuh", "gemm_persist.cuh", "gemm_pair.cuh", "attn_tc.cuh", "prefill_kernels.cuh", "attn_fa.cuh",
-                "paged_common.cuh", "paged_attn.cuh", "paged_by_page.cuh", "paged_prefix.cuh"]
+                "paged_common.cuh", "paged_attn.cuh", "paged_by_page.cuh", "paged_prefix.cuh", "paged_span.cuh"]
 
 
 def _nvcc() -> str:

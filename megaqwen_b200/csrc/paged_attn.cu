@@ -7,6 +7,7 @@
 #include "paged_attn.cuh"
 #include "paged_by_page.cuh"
 #include "paged_prefix.cuh"
+#include "paged_span.cuh"
 
 namespace mq {
 
@@ -660,6 +661,19 @@ Shape shape_of(const mq_paged_attend_params* p) {
     return {p->pool->head_dim, p->num_q_heads, p->total_q, true, p->num_groups > 0,
             tc_prefix(p->total_q, p->num_q_heads / p->pool->num_kv_heads, p->num_groups, p->scale)};
 }
+// The tensor-core kernel takes calls of more rows to a sequence than the 16 of a rows_kernel item on average.
+bool tc_span(const mq_paged_span_params* p) {
+    const int grp = p->num_q_heads / p->pool->num_kv_heads;
+    return (long long)p->total_q * grp > 16ll * p->num_seqs && grp <= PROWS / 2;
+}
+size_t span_workspace(const mq_paged_span_params* p, SpanCut** cuts, float** slots, void* base) {
+    const size_t at = up256(sm_count() * sizeof(SpanCut));
+    if (cuts) {
+        *cuts = (SpanCut*)base;
+        *slots = (float*)((uint8_t*)base + at);
+    }
+    return at + (size_t)2 * sm_count() * PROWS * (p->pool->head_dim + 4) * 4;
+}
 Shape shape_of(const mq_paged_span_params* p) { return {p->pool->head_dim, p->num_q_heads, p->total_q, true, false, false}; }
 Shape shape_of(const mq_paged_sparse_params* p) {
     return {p->pool->head_dim, p->num_q_heads, p->n, false, false, false};
@@ -688,6 +702,20 @@ int run_prefix(const RowArgs& a, const mq_paged_pool& pool, cudaStream_t st) {
     cudaError_t e = allow_smem(kernel, smem, limit);
     if (e == cudaSuccess) e = launch(kernel, dim3(sm_count()), dim3(PFX_THREADS), smem, st, tk, tv, a);
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "paged prefix attention");
+}
+
+template <typename T, int D>
+int run_span_tc(const RowArgs& a, SpanCut* cuts, const mq_paged_pool& pool, cudaStream_t st) {
+    CUtensorMap tk, tv;
+    if (!pool_maps(&tk, &tv, pool, a.pool, pool.page_size, 1)) return MQ_ERR_CUDA;
+    auto kernel = span_kernel<T, D>;
+    const size_t smem = SpanSmem<D>::bytes(a.B);
+    static SmemLimit limit;
+    cudaError_t e = allow_smem(kernel, smem, limit);
+    const int grid = sm_count();
+    if (e == cudaSuccess) e = launch(kernel, dim3(grid), dim3(SPAN_THREADS), smem, st, tk, tv, a, cuts);
+    if (e == cudaSuccess) e = launch(span_join_kernel<T, D>, dim3(grid, PROWS / SPAN_JOIN_ROWS), dim3(256), 0, st, a, (const SpanCut*)cuts);
+    return e == cudaSuccess ? MQ_OK : note_cuda(e, "paged attention under a mask");
 }
 
 template <typename T, int D, int MODE>
@@ -833,7 +861,7 @@ int mq_paged_attend(const mq_paged_attend_params* p, cudaStream_t st) {
 
 size_t mq_paged_span_workspace_bytes(const mq_paged_span_params* p) {
     if (!p || !p->pool || p->total_q < 0 || p->pool->num_kv_heads < 1) return 0;
-    return row_workspace(shape_of(p), nullptr, nullptr);
+    return tc_span(p) ? span_workspace(p, nullptr, nullptr, nullptr) : row_workspace(shape_of(p), nullptr, nullptr);
 }
 
 namespace {
@@ -873,6 +901,13 @@ int run_span(const mq_paged_span_params* p, int window, int sinks, const int* pa
     a.sinks = sinks;
     a.parents = parents;
     const Shape s = shape_of(p);
+    if (tc_span(p)) {
+        SpanCut* cuts;
+        span_workspace(p, &cuts, &a.ws.pfx_slots, p->workspace);
+        return dispatch(p->pool->dtype, s.D, [&](auto T, auto D) {
+            return run_span_tc<decltype(T), decltype(D)::value>(a, cuts, *p->pool, st);
+        });
+    }
     row_workspace(s, &a.ws, p->workspace);
     set_rt(a, (long long)a.total_q * a.grp <= 8ll * a.B);   // as for attend
     return dispatch(p->pool->dtype, s.D, [&](auto T, auto D) {

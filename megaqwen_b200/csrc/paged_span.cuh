@@ -1,0 +1,787 @@
+// Attention under a mask for many query rows, on the 5th-generation tensor
+// cores: sliding windows with sinks, trees of drafted tokens.
+//
+// Work: items of (sequence, kv head, up to 256 query rows: whole tokens) x the
+// 128-key tiles that any of its rows sees, a windowed item's sink tiles first.
+// Items lie end to end on a line that is cut into equal runs, one per CTA (one
+// CTA per SM), each item as long as it has tiles.
+//
+// A CTA runs two streams, A and B, as the shared-prefix kernel does
+// (paged_prefix.cuh): with more than 128 rows each has half of them and every tile
+// is used by both; with up to 128 rows both take the same ones, A the even tiles
+// and B the odd, and their two accumulators, side by side in TMEM, are joined when
+// the item ends.  Weights go into the second product as two 16-bit pieces.
+//
+// Masks: a tile that some row does not see whole has its scores set to minus
+// infinity in TMEM by two cuts (windowed) or by the node's ancestors (a tree),
+// whose tiles are few; other tiles take no test.  An infinity or NaN among values
+// that a row does not see must not meet its zero weight: a warp of its own looks
+// through the masked tiles' values, puts zeros in their place and notes where they
+// were, and a row that does see one has a NaN in that channel at the end.
+//
+// An item that a run's end cuts leaves a part (m, l, acc) per row and run, which
+// the join adds in the order of the positions.
+#pragma once
+
+#include "paged_prefix.cuh"
+
+namespace mq {
+namespace paged {
+
+constexpr int SPAN_THREADS = 640;   // warps: 0 K, 1 MMA, 2 V, 3-10 softmax of A, 11-18 of B, 19 looks through V
+
+template <int D>
+struct SpanSmem {
+    static constexpr int TILE = (D / 64) * PATOM;
+    static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE, BAR = 6 * TILE;
+    static constexpr int RED = BAR + 256;                     // fp32 [2 streams][2 tiles][2 halves][128] row maxima
+    static constexpr int SUM = RED + 2 * 2 * 2 * 128 * 4;     // fp32 [2 streams][2 halves][128] row sums
+    static constexpr int TOP = SUM + 2 * 2 * 128 * 4;         // fp32 [2 streams][128] their reference
+    static constexpr int ODD = TOP + 2 * 128 * 4;             // [2 stages][128 keys][D / 8]: a bit for each value that is not finite
+    static constexpr int HIT = ODD + 2 * 128 * (D / 8);       // u64 [2 streams][2 halves][128]: channels in which a row met one
+    static constexpr int SCHED = HIT + 2 * 2 * 128 * 8;
+    static constexpr size_t bytes(int B) { return SCHED + (size_t)(2 * B + 1) * 4 + 1024; }
+};
+
+// An item that is cut: the worker with its first tile leaves this for the join.
+struct alignas(16) SpanCut {
+    int tok0, h, rows, runs;   // rows 0: none
+};
+
+struct SpanSeg {
+    int b, h, tok0, rows;         // tok0: the tile's first token; rows: of this item
+    int seq0, pf, pl;             // the sequence's first token; positions of the tile's first and last token
+    int st, wt, ng;               // sink tiles, first window tile, tiles in all
+    int t0, n, runs;              // of this run; runs that share the item
+    bool two, start, whole;
+};
+
+// Tiles of a row tile whose tokens stand at pf .. pl: st of the sinks, then wt .. the one of pl.
+__device__ __forceinline__ int span_tiles(const RowArgs& a, int pf, int pl, int& st, int& wt) {
+    st = wt = 0;
+    if (pl < 0) return 0;
+    const int end = (pl >> 7) + 1;
+    if (a.window) {
+        wt = max(pf - a.window + 1, 0) >> 7;
+        st = min(a.sinks > 0 ? ((a.sinks - 1) >> 7) + 1 : 0, wt);
+    }
+    return st + end - wt;
+}
+
+// 64 positions from `at` on that a row at position p sees; node: its place in the tree whose first token is seq0.
+__device__ __forceinline__ unsigned long long span_sees(const RowArgs& a, int p, int at, int node, int seq0) {
+    auto low = [](int k) { return k >= 64 ? ~0ull : k <= 0 ? 0ull : (1ull << k) - 1ull; };
+    if (!a.parents) return low(p + 1 - at) & (~low(p + 1 - a.window - at) | low(a.sinks - at));
+    const int base = p - node;
+    unsigned long long bits = low(base - at);
+    if (at + 64 <= base) return bits;
+    while (node >= 0) {
+        const int i = base + node - at;
+        if (i >= 0 && i < 64 && base + node >= 0) bits |= 1ull << i;
+        const int up = __ldg(a.parents + seq0 + node);
+        if (up >= node || up < -1) note_status(a.status, MQ_ERR_INVALID_ARGUMENT);
+        node = up >= node ? -1 : up;
+    }
+    return bits;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(SPAN_THREADS, 1)
+span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const RowArgs a,
+            SpanCut* __restrict__ cuts) {
+    using L = SpanSmem<D>;
+    constexpr int TILE = L::TILE, LD = D + 4, NT = SPAN_THREADS;
+    extern __shared__ uint8_t pfx_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pfx_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR);
+    uint64_t* q_full = bars;          // [2] streams
+    uint64_t* k_full = bars + 2;      // [2] stages
+    uint64_t* k_empty = bars + 4;
+    uint64_t* v_full = bars + 6;
+    uint64_t* v_empty = bars + 8;
+    uint64_t* v_ready = bars + 10;    // [2] stages: looked through
+    uint64_t* s_full = bars + 12;     // [2] streams: S is there (and every MMA issued before it is done)
+    uint64_t* p_full = bars + 14;     // [2] P is stored, O is rescaled
+    uint64_t* o_full = bars + 16;     // [2] the run's last PV is done
+    uint64_t* drain = bars + 18;
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 19);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+    volatile int* odd_tile = abort_flag + 1;   // [2] stages: the tile holds values that are not finite
+    __shared__ uint32_t scratch[NT / 32];
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&q_full[i], 8);
+            mbar_init(&k_full[i], 1);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], 1);
+            mbar_init(&v_empty[i], 1);
+            mbar_init(&v_ready[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 8);
+            mbar_init(&o_full[i], 1);
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+        prefetch_tmap(&tmK);
+        prefetch_tmap(&tmV);
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_holder, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_holder;
+    pdl_wait();
+    pdl_trigger();
+
+    // ---- the line: off[b] units before sequence b, for one kv head ----
+    uint32_t* off = reinterpret_cast<uint32_t*>(smem + L::SCHED);   // [B + 1]
+    int* lens = reinterpret_cast<int*>(off + a.B + 1);              // [B], 0 where nothing is read
+    const int grp = a.grp, page = a.pool.page, tpt = PROWS / grp;   // tokens to a row tile
+    bool bad = false;
+    if (a.q_starts) {
+        for (int b = threadIdx.x; b < a.B; b += NT)
+            if (__ldg(a.q_starts + b + 1) < __ldg(a.q_starts + b)) bad = true;
+        if (threadIdx.x == 0 && (__ldg(a.q_starts) != 0 || __ldg(a.q_starts + a.B) != a.total_q)) bad = true;
+    }
+    bool in_order = !__syncthreads_or(bad);
+    {
+        unsigned long long carry = 0;
+        for (int b0 = 0; in_order && b0 < a.B; b0 += NT) {
+            const int b = b0 + threadIdx.x;
+            unsigned long long cost = 0;
+            if (b < a.B) {
+                const int slot = __ldg(a.slots + b), ql = q_start(a, b + 1) - q_start(a, b);
+                int len = 0, code = 0;
+                if (slot < 0 || slot >= a.num_slots) {
+                    code = MQ_ERR_BAD_SLOT;
+                } else {
+                    len = __ldg(a.lengths + slot);
+                    if (len < 0 || pages_for(len, a.pool.shift) > a.cols) code = MQ_ERR_BAD_POSITION;
+                    else if (a.parents && ql > MAX_TREE) code = MQ_ERR_INVALID_ARGUMENT;
+                }
+                if (code) {
+                    len = 0;
+                    if (blockIdx.x == 0) note_status(a.status, code);
+                }
+                lens[b] = len;
+                int st, wt;
+                for (int i = 0; len && i < ql; i += tpt) {
+                    const int n = span_tiles(a, len - ql + i, len - ql + min(i + tpt, ql) - 1, st, wt);
+                    cost += n ? n + ITEM_UNITS : 0;
+                }
+            }
+            unsigned long long x = cost;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            const bool big = x > 0x7fffffffull;   // a sum that does not fit is refused below
+            if (lane == 31) scratch[warp] = big ? 0x7fffffffu : (uint32_t)x;
+            __syncthreads();
+            unsigned long long before = carry;
+            for (int w = 0; w < NT / 32; ++w) {
+                const uint32_t v = scratch[w];
+                if (w < warp) before += v;
+                carry += v;
+            }
+            if (b < a.B) off[b] = (uint32_t)(before + x - cost);
+            __syncthreads();
+        }
+        if (carry * (unsigned)a.hkv >= 0x7fffffffull) in_order = false;
+        if (threadIdx.x == 0) off[a.B] = (uint32_t)carry;
+    }
+    __syncthreads();
+    if (!in_order && blockIdx.x == 0 && threadIdx.x == 0) note_status(a.status, MQ_ERR_INVALID_ARGUMENT);
+    const uint32_t work = in_order ? off[a.B] * a.hkv : 0, quota = quota_of(work, gridDim.x);
+    const uint32_t x0 = min(blockIdx.x * quota, work), xe = min(x0 + quota, work);
+
+    // The item at x and the tiles of it in this run (n <= 0: the run has only its own units); x moves past them.
+    // Called by whole warps.
+    auto segment = [&](uint32_t& x) {
+        SpanSeg e;
+        const uint32_t xh = x / (uint32_t)a.hkv;
+        int lo = 0, hi = a.B;   // the last sequence that starts at or before, of those with work
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (off[mid] <= xh) lo = mid;
+            else hi = mid;
+        }
+        e.b = lo;
+        const uint32_t one = off[lo + 1] - off[lo];
+        uint32_t rel = x - off[lo] * a.hkv;
+        e.h = (int)(rel / one);
+        rel -= e.h * one;
+        e.seq0 = q_start(a, lo);
+        const int ql = q_start(a, lo + 1) - e.seq0, p0 = lens[lo] - ql;
+        for (int i0 = 0;; i0 += 32) {   // the row tile, 32 at a time
+            const int i = (i0 + lane) * tpt;
+            int st, wt, n = 0;
+            if (i < ql) n = span_tiles(a, p0 + i, p0 + min(i + tpt, ql) - 1, st, wt);
+            const uint32_t cost = n ? n + ITEM_UNITS : 0;
+            uint32_t sum = cost;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += y;
+            }
+            const unsigned found = __ballot_sync(0xffffffffu, rel < sum);
+            if (!found && (i0 + 32) * tpt < ql) {
+                rel -= __shfl_sync(0xffffffffu, sum, 31);
+                continue;
+            }
+            const int at = found ? __ffs((int)found) - 1 : 0;   // (always found: x is within the sequence)
+            rel -= __shfl_sync(0xffffffffu, sum - cost, at);
+            const int first = (i0 + at) * tpt, last = min(first + tpt, ql) - 1;
+            e.tok0 = e.seq0 + first;
+            e.rows = (last - first + 1) * grp;
+            e.pf = p0 + first;
+            e.pl = p0 + last;
+            break;
+        }
+        e.ng = span_tiles(a, e.pf, e.pl, e.st, e.wt);
+        const int pos = (int)rel, left = (int)min((uint32_t)(e.ng + ITEM_UNITS - pos), xe - x);
+        e.t0 = max(pos - ITEM_UNITS, 0);
+        e.n = max(pos + left - ITEM_UNITS, 0) - e.t0;
+        e.two = e.rows > 128;
+        e.start = e.t0 == 0;
+        e.whole = e.n == e.ng;
+        const uint32_t ps = x - pos + ITEM_UNITS;   // the item's first tile on the line
+        e.runs = (int)((ps + e.ng - 1) / quota - ps / quota) + 1;
+        x += left;
+        return e;
+    };
+    auto tile_at = [&](const SpanSeg& e, int j) {   // first position of the run's j-th tile
+        const int t = e.t0 + j;
+        return (t < e.st ? t : e.wt + t - e.st) * PK;
+    };
+    // Every row sees all of the tile at `at`.
+    auto all_seen = [&](const SpanSeg& e, int at) {
+        if (a.parents) return at + PK <= e.seq0 - e.tok0 + e.pf;
+        return at + PK - 1 <= e.pf && (at > e.pl - a.window || at + PK <= a.sinks);
+    };
+    // Some row sees a position of the page at `at`: other pages' entries in the table are not looked at.
+    auto in_sight = [&](const SpanSeg& e, int at) {
+        return at <= e.pl && (a.parents || at < a.sinks || at + page > e.pf - a.window + 1);
+    };
+    auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        const long long t0 = clock64();
+        while (!mbar_try_wait(bar, parity)) {
+            if (*abort_flag || clock64() - t0 > WAIT_CYCLES) return false;
+        }
+        return true;
+    };
+    auto give_up = [&]() {
+        *abort_flag = 1;
+        note_status(a.status, MQ_ERR_PIPE_TIMEOUT);
+    };
+
+    if (warp == 0 || warp == 2) {
+        // ---- K and V producers: lane c loads the tile's c-th page ----
+        uint64_t* full = warp == 0 ? k_full : v_full;
+        uint64_t* empty = warp == 0 ? k_empty : v_empty;
+        const CUtensorMap* map = warp == 0 ? &tmK : &tmV;
+        uint8_t* ring = smem + (warp == 0 ? L::K : L::V);
+        const int chunks = PK / page;
+        int c = 0;   // tiles so far
+        bool ok = true, cut = false;
+        for (uint32_t x = x0; ok && x < xe;) {
+            const SpanSeg e = segment(x);
+            if (e.n <= 0) continue;
+            if (warp == 0 && e.start && !e.whole) {   // (the run's last item)
+                if (lane == 0) *reinterpret_cast<int4*>(cuts + blockIdx.x) = make_int4(e.tok0, e.h, e.rows, e.runs);
+                cut = true;
+            }
+            const int* row = a.table + __ldg(a.slots + e.b) * a.table_row;
+            // what no row sees is read as zeros, from outside the map
+            auto look = [&](int j) {
+                const int at = tile_at(e, j) + lane * page;
+                return lane < chunks && in_sight(e, at) ? __ldg(row + (at >> a.pool.shift)) : a.pool.pages;
+            };
+            int next = look(0);
+            for (int j = 0; j < e.n; ++j, ++c) {
+                int pid = next;
+                if (j + 1 < e.n) next = look(j + 1);
+                if (pid < 0 || pid >= a.pool.pages) {
+                    if (lane < chunks && in_sight(e, tile_at(e, j) + lane * page)) note_status(a.status, MQ_ERR_BAD_PAGE);
+                    pid = a.pool.pages;
+                }
+                const int st = c & 1;
+                const bool here = c < 2 || wait(&empty[st], ((c >> 1) - 1) & 1);
+                if (!__all_sync(0xffffffffu, here)) {
+                    ok = false;
+                    break;
+                }
+                if (lane == 0) mbar_arrive_expect_tx(&full[st], TILE);
+                __syncwarp();
+                if (lane < chunks) {
+#pragma unroll
+                    for (int i = 0; i < D / 64; ++i)
+                        tma_load_page(smem_u32(ring + st * TILE + i * PATOM + lane * page * 128), map, 0, i, e.h, pid, smem_u32(&full[st]));
+                }
+            }
+        }
+        if (warp == 0 && !cut && lane == 0) *reinterpret_cast<int4*>(cuts + blockIdx.x) = make_int4(0, 0, 0, 0);
+        if (!ok && lane == 0) give_up();
+        // copies in flight land before the CTA may end, whatever became of their readers
+        for (int k = max(0, c - 2); k < c; ++k) {
+            const long long t0 = clock64();
+            while (!mbar_try_wait(&full[k & 1], (k >> 1) & 1) && clock64() - t0 < WAIT_CYCLES) {
+            }
+        }
+    } else if (warp == 19) {
+        // ---- looks through the values of masked tiles ----
+        int c = 0;
+        bool ok = true;
+        for (uint32_t x = x0; ok && x < xe;) {
+            const SpanSeg e = segment(x);
+            for (int j = 0; j < e.n; ++j, ++c) {
+                const int st = c & 1;
+                ok = __all_sync(0xffffffffu, wait(&v_full[st], (c >> 1) & 1));
+                if (!ok) break;
+                if (!all_seen(e, tile_at(e, j))) {
+                    constexpr uint32_t M = Elem<T>::EXP_MASK * 0x10001u, U = (Elem<T>::EXP_MASK & -Elem<T>::EXP_MASK) * 0x10001u;
+                    uint8_t* vt = smem + L::V + st * TILE;
+                    uint32_t any = 0;
+#pragma unroll 8
+                    for (int i = lane; i < TILE / 16; i += 32) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(vt + i * 16);
+                        // an exponent of all ones and one more carries out of its field
+                        any |= ((w.x & M) + U) | ((w.y & M) + U) | ((w.z & M) + U) | ((w.w & M) + U);
+                    }
+                    const bool odd = __any_sync(0xffffffffu, any & 0x80008000u);
+                    if (odd) {
+                        uint8_t* bits = smem + L::ODD + st * 128 * (D / 8);
+                        for (int i = lane; i < TILE / 16; i += 32) {
+                            // 16-byte piece i: block of 64 channels, key, piece of it (swizzled by the key)
+                            const int key = i >> 3 & 127, ch = (i >> 10) * 8 + ((i & 7) ^ (key & 7));
+                            uint4 w = *reinterpret_cast<const uint4*>(vt + i * 16);
+                            uint32_t* v = reinterpret_cast<uint32_t*>(&w);
+                            uint32_t mark = 0;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const uint32_t f = (v[k] & M) + U;
+                                if (f & 0x8000u) mark |= 1u << (2 * k), v[k] &= 0xffff0000u;
+                                if (f & 0x80000000u) mark |= 2u << (2 * k), v[k] &= 0xffffu;
+                            }
+                            bits[key * (D / 8) + ch] = (uint8_t)mark;
+                            if (mark) *reinterpret_cast<uint4*>(vt + i * 16) = w;
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                    if (lane == 0) odd_tile[st] = odd;
+                    __syncwarp();
+                }
+                if (lane == 0) mbar_arrive(&v_ready[st]);
+            }
+        }
+        if (!ok && lane == 0) give_up();
+    } else if (warp == 1) {
+        // ---- MMA: the whole warp walks, one elected lane issues.  All 512 columns of
+        // TMEM are this CTA's, so their addresses start at 0 ----
+        constexpr uint32_t id_s = pfx_idesc<T>(PK, false), id_o = pfx_idesc<T>(D, true);
+        const uint32_t base = (smem_u32(pfx_raw) + 1023u) & ~1023u;
+        int c0 = 0;                         // tiles of the segments before
+        uint32_t np0 = 0, np1 = 0;          // PVs issued per stream
+        uint32_t nq0 = 0, nq1 = 0;          // Q tiles used per stream
+        bool ok = true;
+        auto scores = [&](int q, int kc, bool last_use) {
+            const uint32_t sq = base + L::Q + q * TILE, sk = base + L::K + (kc & 1) * TILE;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                const uint32_t o = (k >> 2) * PATOM + (k & 3) * 32;
+                tc_mma_f16(q * 128, sw128_kmajor_desc(sq + o), sw128_kmajor_desc(sk + o), id_s, k != 0);
+            }
+            tc_commit(&s_full[q]);
+            if (last_use) tc_commit(&k_empty[kc & 1]);
+        };
+        auto values = [&](int q, int vc, bool first, bool last_use, bool done) {
+            const uint32_t sv = base + L::V + (vc & 1) * TILE, o = 256 + q * 128;
+#pragma unroll
+            for (int k = 0; k < PK / 16; ++k) {
+                // 16 keys: 8 columns of values, the remainders 16 columns on
+                const uint32_t p = q * 128 + 32 * (k >> 1) + 8 * (k & 1);
+                const uint64_t dv = sw128_mnmajor_desc(sv + k * 2048);
+                tc_mma_f16_ts(o, p, dv, id_o, !first || k);
+                tc_mma_f16_ts(o, p + 16, dv, id_o, 1);
+            }
+            if (last_use) tc_commit(&v_empty[vc & 1]);
+            if (done) tc_commit(&o_full[q]);
+        };
+        for (uint32_t x = x0; ok && x < xe;) {
+            const SpanSeg e = segment(x);
+            const int n = uniform(e.n);
+            if (n <= 0) continue;
+            const bool two = uniform(e.two);
+            const int steps = two ? 2 * n : n;
+            // step i: the stream's PV of its tile before (step i - 2), then its S of this one.  What the
+            // step needs is waited for by four lanes at once.
+            for (int i = 0; ok && i < steps + 2; ++i) {
+                const int q = i & 1;
+                const bool pv = i >= 2, sc = i < steps;
+                const int vc = c0 + (two ? (i - 2) >> 1 : i - 2), kc = c0 + (two ? i >> 1 : i);
+                if (!pv && !sc) continue;   // a run of one tile: stream B has none
+                uint64_t* bar = nullptr;
+                uint32_t parity = 0;
+                if (lane == 0 && sc) bar = &k_full[kc & 1], parity = kc >> 1;
+                if (lane == 1 && pv) bar = &v_ready[vc & 1], parity = vc >> 1;
+                if (lane == 2 && pv) bar = &p_full[q], parity = q ? np1 : np0;
+                if (lane == 3 && !pv) bar = &q_full[q], parity = q ? nq1 : nq0;
+                ok = __all_sync(0xffffffffu, !bar || wait(bar, parity & 1));
+                if (pv) (q ? np1 : np0)++;
+                else (q ? nq1 : nq0)++;
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    if (pv) values(q, vc, i < 4, !two || q == 1, !sc);
+                    if (sc) scores(q, kc, !two || q == 1);
+                }
+                __syncwarp();
+            }
+            c0 += n;
+        }
+        if (!ok && lane == 0) give_up();
+        if (elect_one()) tc_commit(drain);   // MMAs in flight end before TMEM goes
+        __syncwarp();
+        const long long t0 = clock64();
+        while (!mbar_try_wait(drain, 0) && clock64() - t0 < WAIT_CYCLES) {
+        }
+    } else {
+        // ---- softmax of stream q, column half hh: two threads to a row ----
+        const int q = (warp - 3) >> 3, hh = ((warp - 3) >> 2) & 1;
+        const int quad = warp & 3;                     // the TMEM lanes this warp may touch
+        const int r = quad * 32 + lane;
+        // a scale of zero: a masked score of minus infinity stays one
+        const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);
+        const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+        const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+        const uint32_t sa = tmem + lane_off + q * 128 + hh * 64, oa = tmem + lane_off + 256;   // O of A, that of B 128 columns on
+        float* red = reinterpret_cast<float*>(smem + L::RED) + q * 512;
+        float* sums = reinterpret_cast<float*>(smem + L::SUM);                       // [stream][half][128]
+        float* tops = reinterpret_cast<float*>(smem + L::TOP);                       // [stream][128]
+        unsigned long long* hits = reinterpret_cast<unsigned long long*>(smem + L::HIT);   // [stream][half][128]
+        constexpr float GROW = 8.f;
+        // the two warps of a row meet at a barrier of their own, the four of both streams at another; one whose wait
+        // failed goes on to the end without waiting, so that its partners never stand alone
+        auto meet = [&]() { named_bar_sync(1 + q * 4 + quad, 64); };
+        auto meet4 = [&]() { named_bar_sync(9 + quad, 128); };
+        int ns = 0, nv = 0, no0 = 0, no1 = 0;   // scores taken, tiles of the segments before, results of A and B
+        bool ok = true;
+        auto got = [&](uint64_t* bar, uint32_t parity) {
+            if (ok) ok = __all_sync(0xffffffffu, wait(bar, parity));
+            return ok;
+        };
+        for (uint32_t x = x0; x < xe;) {
+            const SpanSeg e = segment(x);
+            if (e.n <= 0) continue;
+            const int mine = e.two ? e.n : (e.n + 1 - q) >> 1;   // this stream's tiles
+            const int wr = e.two ? q * 128 + r : r;              // the row in the item
+            const int tok = wr / grp, head = e.h * grp + wr - tok * grp;
+            const bool there = wr < e.rows;
+            const int pos = min(e.pf + tok, e.pl), node = e.tok0 - e.seq0 + pos - e.pf;
+            unsigned long long hit = 0;
+            float m = -INFINITY, l = 0.f;
+            if (mine) {
+                meet();   // both warps are done with the Q rows of the item before
+                // Q rows, swizzled as TMA would, zeros past the end; a negative scale turns their
+                // signs.  Half the rows each, LPR lanes side by side on a row, all loads in flight.
+                const uint16_t* src = there ? a.q + (long long)(e.tok0 + tok) * a.q_tok + head * a.q_head : nullptr;
+                constexpr int LPR = D / 8, RPI = 32 / LPR, N = 16 / RPI;
+                const int ch = lane % LPR, sub = lane / LPR;
+                uint4 v[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const uint16_t* row = from_lane(src, hh * 16 + i * RPI + sub);
+                    v[i] = row ? __ldg(reinterpret_cast<const uint4*>(row + ch * 8)) : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int w = quad * 32 + hh * 16 + i * RPI + sub;
+                    v[i].x ^= sign; v[i].y ^= sign; v[i].z ^= sign; v[i].w ^= sign;
+                    *reinterpret_cast<uint4*>(smem + L::Q + q * TILE + (ch >> 3) * PATOM + w * 128 +
+                                              (((ch & 7) ^ (w & 7)) << 4)) = v[i];
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[q]);
+            }
+            // lane c: whether the c-th page of the tile at `at` is out of range
+            const int* trow = a.table + __ldg(a.slots + e.b) * a.table_row;
+            auto gone = [&](int at, int c) {
+                at += c * page;
+                if (!in_sight(e, at)) return false;
+                const int pid = __ldg(trow + (at >> a.pool.shift));
+                return pid < 0 || pid >= a.pool.pages;
+            };
+            // looked up once per run, while the first scores are on their way, and again tile by tile only if there are any
+            bool holes = false;
+            if (mine) {
+                const int chunks = PK / page;
+#pragma unroll 1
+                for (int i = lane; i < e.n * chunks; i += 32) holes |= gone(tile_at(e, i / chunks), i % chunks);
+                holes = __any_sync(0xffffffffu, holes);
+            }
+            for (int j = 0; j < mine; ++j, ++ns) {
+                float tmax = -INFINITY;
+                const int jt = e.two ? j : 2 * j + q, at = tile_at(e, jt);
+                const unsigned none = holes ? __ballot_sync(0xffffffffu, lane < PK / page && gone(at, lane)) : 0u;
+                const bool masked = !all_seen(e, at);
+                if (got(&s_full[q], ns & 1)) {
+                    tc_fence_after();
+                    if (masked || none) {
+                        const unsigned long long live = masked ? span_sees(a, pos, at + hh * 64, node, e.seq0) : ~0ull;
+#pragma unroll 1
+                        for (int i = 0; i < 64; i += 32) {
+                            uint32_t lv = (uint32_t)(live >> i);
+                            for (int k = 0; k < 32; k += 16)   // a page is 16 keys or more
+                                if (none >> ((hh * 64 + i + k) >> a.pool.shift) & 1u) lv &= ~(0xffffu << k);
+                            if (__all_sync(0xffffffffu, lv == 0xffffffffu)) continue;
+                            float sv[32];
+                            tmem_ld32(sa + i, sv);
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) sv[k] = lv >> k & 1u ? sv[k] : -INFINITY;
+                            tmem_st32(sa + i, sv);
+                        }
+                    }
+                    // two passes over S in TMEM: the code stays small (a run is a few tiles long, and
+                    // fetching unrolled code the first time cost more than reading S twice)
+                    float sv[64], mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    tmem_ld64(sa, sv);
+#pragma unroll
+                    for (int k = 0; k < 64; ++k) mx[k & 3] = fmaxf(mx[k & 3], sv[k]);
+                    tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+                }
+                red[((j & 1) * 2 + hh) * 128 + r] = tmax;
+                meet();
+                if (!ok) continue;
+                tmax = fmaxf(tmax, red[((j & 1) * 2 + (hh ^ 1)) * 128 + r]);
+                // a row's maximum moves only when it grew by more than 2^8; weights stay below 256
+                float corr = 1.f;
+                if (tmax > m + GROW) {
+                    corr = ex2(m - tmax);   // 0 on the first tile
+                    m = tmax;
+                }
+                l *= corr;
+                if (j && __any_sync(0xffffffffu, corr != 1.f)) {
+                    // s_full covers the PV before it, so O is at rest; half its columns each
+#pragma unroll 1
+                    for (int i = 0; i < D / 2; i += 16) {
+                        float v[16];
+                        tmem_ld16(oa + q * 128 + hh * (D / 2) + i, v);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) v[k] *= corr;
+                        tmem_st16(oa + q * 128 + hh * (D / 2) + i, v);
+                    }
+                }
+                const float u = m == -INFINITY ? 0.f : m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+                for (int i = 0; i < 64; i += 32) {
+                    float sv[32];
+                    uint32_t pk[32];   // 32 weights in 16 columns, their remainders in the next 16
+                    tmem_ld32(sa + i, sv);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float p0 = ex2(fmaf(sv[2 * k], scale, -u)), p1 = ex2(fmaf(sv[2 * k + 1], scale, -u));
+                        sum[k & 3] += p0 + p1;
+                        pk[k] = Elem<T>::pack(p0, p1);
+                        const float2 b = Elem<T>::up2(pk[k]);
+                        pk[16 + k] = Elem<T>::pack(p0 - b.x, p1 - b.y);
+                    }
+                    tmem_st16_nowait(sa + i, pk);
+                    tmem_st16_nowait(sa + i + 16, pk + 16);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (masked) {
+                    // the tile's values are looked through, and stay until this stream's weights are used
+                    const int c = nv + jt, st = c & 1;
+                    if (got(&v_ready[st], (c >> 1) & 1) && odd_tile[st]) {
+                        const uint8_t* bits = smem + L::ODD + st * 128 * (D / 8) + hh * (D / 16);
+#pragma unroll 1
+                        for (int k0 = 0; k0 < PK; k0 += 64) {
+                            const unsigned long long live = span_sees(a, pos, at + k0, node, e.seq0);
+                            for (int k = 0; k < 64; ++k) {
+                                unsigned long long w;
+                                if (D == 128) w = *reinterpret_cast<const unsigned long long*>(bits + (k0 + k) * (D / 8));
+                                else w = *reinterpret_cast<const uint32_t*>(bits + (k0 + k) * (D / 8));
+                                if (live >> k & 1ull) hit |= w;
+                            }
+                        }
+                    }
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[q]);
+            }
+            nv += e.n;
+            // ---- the item's rows: what A and B have of them, when they share them ----
+            const bool b_too = e.two ? q == 1 : e.n > 1, a_too = e.two ? q == 0 : true;
+            if (a_too) got(&o_full[0], no0 & 1);
+            if (b_too) got(&o_full[1], no1 & 1);
+            ++no0;
+            no1 += e.two || e.n > 1;
+            tc_fence_after();
+            sums[(q * 2 + hh) * 128 + r] = l;
+            if (e.two) {
+                meet();
+                l += sums[(q * 2 + (hh ^ 1)) * 128 + r];
+            } else {
+                if (hh == 0) tops[q * 128 + r] = m;
+                hits[(q * 2 + hh) * 128 + r] = hit;
+                meet4();
+            }
+            // this thread's columns: its half, or with two streams on a row half of that
+            float e0 = 1.f, e1 = 1.f;   // weights of A's and B's accumulators
+            if (!e.two) {
+                const float ma = tops[r], mb = tops[128 + r];   // (B's is -inf when it had no tile)
+                m = fmaxf(ma, mb);
+                const float u = m == -INFINITY ? 0.f : m;
+                e0 = ex2(ma - u);
+                e1 = ex2(mb - u);
+                l = (sums[r] + sums[128 + r]) * e0 + (sums[256 + r] + sums[384 + r]) * e1;
+                hit = hits[hh * 128 + r] | hits[(2 + hh) * 128 + r];
+            }
+            const float inv = l != 0.f ? 1.f / l : 0.f;   // a row that sees nothing is zero (NaN stays NaN)
+            const int width = e.two ? D / 2 : D / 4, c_lo = hh * (D / 2) + (e.two ? 0 : q * (D / 4));
+            float* part = a.ws.pfx_slots + ((2ll * blockIdx.x + e.start) * PROWS + wr) * LD;
+            uint16_t* out = a.out + ((long long)(e.tok0 + tok) * a.hq + head) * D;
+            if (!e.whole && ok && there && hh == 0 && (e.two || q == 0))
+                *reinterpret_cast<float4*>(part) = make_float4(m, l, 0.f, 0.f);
+#pragma unroll 1
+            for (int i = 0; ok && i < width; i += 16) {
+                const int c = c_lo + i;
+                float v[16];
+                tmem_ld16(oa + (e.two ? q * 128 : 0) + c, v);
+                if (!e.two) {
+                    float w[16];
+                    if (b_too) tmem_ld16(oa + 128 + c, w);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) v[k] = b_too ? v[k] * e0 + w[k] * e1 : v[k] * e0;
+                }
+                const uint32_t odd = (uint32_t)(hit >> (c - hh * (D / 2))) & 0xffffu;
+                if (odd) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        if (odd >> k & 1u) v[k] = NAN;
+                }
+                if (!there) continue;
+                if (e.whole) {
+#pragma unroll
+                    for (int k = 0; k < 16; k += 8)
+                        *reinterpret_cast<uint4*>(out + c + k) =
+                            make_uint4(Elem<T>::pack(v[k] * inv, v[k + 1] * inv), Elem<T>::pack(v[k + 2] * inv, v[k + 3] * inv),
+                                       Elem<T>::pack(v[k + 4] * inv, v[k + 5] * inv), Elem<T>::pack(v[k + 6] * inv, v[k + 7] * inv));
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 16; k += 4)
+                        *reinterpret_cast<float4*>(part + 4 + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                }
+            }
+            tc_fence_before();
+            if (!e.two) meet4();   // both accumulators are read
+        }
+        if (!ok && lane == 0) give_up();
+    }
+    // rows that see nothing: sequences and row tiles without items (the whole call, when it is refused)
+    {
+        const int warps = gridDim.x * (NT / 32), wid = blockIdx.x * (NT / 32) + warp;
+        auto clear = [&](int t0, int t1) {
+            const long long words = (long long)(t1 - t0) * a.hq * (D / 8);
+            uint4* to = reinterpret_cast<uint4*>(a.out) + (long long)t0 * a.hq * (D / 8);
+            for (long long i = lane; i < words; i += 32) to[i] = make_uint4(0, 0, 0, 0);
+        };
+        if (!in_order) {
+            for (int t = wid; t < a.total_q; t += warps) clear(t, t + 1);
+        } else {
+            for (int b = wid; b < a.B; b += warps) {
+                const int t0 = q_start(a, b), ql = q_start(a, b + 1) - t0;
+                int none = ql;   // tokens of row tiles that stand before the first position
+                if (lens[b]) none = lens[b] >= ql ? 0 : min(ql, (ql - lens[b]) / tpt * tpt);
+                if (none > 0) clear(t0, t0 + none);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// The join of the items that were cut: acc = sum acc_i 2^(m_i - M) over sum l_i 2^(m_i - M).  blockIdx.y: a CTA's rows of
+// the cut; a warp to a row.
+constexpr int SPAN_JOIN_ROWS = 8;
+template <typename T, int D>
+__global__ void __launch_bounds__(256) span_join_kernel(const RowArgs a, const SpanCut* __restrict__ cuts) {
+    constexpr int LD = D + 4, V = D / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_trigger();
+    const int4 cut = __ldcg(reinterpret_cast<const int4*>(cuts + blockIdx.x));
+    const int row = blockIdx.y * SPAN_JOIN_ROWS + warp;
+    if (row >= cut.z) return;
+    const float* slots = a.ws.pfx_slots + (2ll * blockIdx.x * PROWS + row) * LD;
+    auto part = [&](int i) { return slots + (2ll * i + (i == 0)) * PROWS * LD; };
+    float M = -INFINITY, Ls = 0.f, acc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+    for (int i0 = 0; i0 < cut.w; i0 += 32) {
+        const int cnt = min(32, cut.w - i0);
+        const float2 ml = lane < cnt ? __ldcg(reinterpret_cast<const float2*>(part(i0 + lane))) : make_float2(-INFINITY, 0.f);
+        float bm = ml.x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, o));
+        const float N = fmaxf(M, bm), U = N == -INFINITY ? 0.f : N;
+        const float c = exp2f(M - U), e = exp2f(ml.x - U);   // 0 for what is not there
+        M = N;
+        float l = ml.y * e;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        Ls = Ls * c + l;
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] *= c;
+#pragma unroll 1
+        for (int k = 0; k < cnt; k += 4) {
+            float v[4][V], w[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                w[q] = __shfl_sync(0xffffffffu, e, (k + q) & 31);
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[q][i] = 0.f;
+                if (k + q < cnt) {
+                    const float* p = part(i0 + k + q) + 4 + lane * V;
+                    if (V == 4) {
+                        const float4 x = __ldcg(reinterpret_cast<const float4*>(p));
+                        v[q][0] = x.x; v[q][1] = x.y; v[q][V - 2] = x.z; v[q][V - 1] = x.w;
+                    } else {
+                        const float2 x = __ldcg(reinterpret_cast<const float2*>(p));
+                        v[q][0] = x.x; v[q][1] = x.y;
+                    }
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[i] += v[q][i] * (k + q < cnt ? w[q] : 0.f);
+        }
+    }
+    const float inv = Ls != 0.f ? 1.f / Ls : 0.f;
+    const int tok = row / a.grp;
+    uint16_t* out = a.out + ((long long)(cut.x + tok) * a.hq + cut.y * a.grp + row - tok * a.grp) * D;
+    if (V == 4)
+        *reinterpret_cast<uint2*>(out + lane * 4) =
+            make_uint2(Elem<T>::pack(acc[0] * inv, acc[1] * inv), Elem<T>::pack(acc[V - 2] * inv, acc[V - 1] * inv));
+    else
+        *reinterpret_cast<uint32_t*>(out + lane * 2) = Elem<T>::pack(acc[0] * inv, acc[1] * inv);
+}
+
+}  // namespace paged
+}  // namespace mq

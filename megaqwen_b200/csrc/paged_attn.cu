@@ -661,10 +661,12 @@ Shape shape_of(const mq_paged_attend_params* p) {
     return {p->pool->head_dim, p->num_q_heads, p->total_q, true, p->num_groups > 0,
             tc_prefix(p->total_q, p->num_q_heads / p->pool->num_kv_heads, p->num_groups, p->scale)};
 }
-// The tensor-core kernel takes calls of more rows to a sequence than the 16 of a rows_kernel item on average.
+// The tensor-core kernel takes calls of more rows to a sequence than the 16 of a rows_kernel item on average (q through a
+// tensor map, whose strides are positive).
 bool tc_span(const mq_paged_span_params* p) {
     const int grp = p->num_q_heads / p->pool->num_kv_heads;
-    return (long long)p->total_q * grp > 16ll * p->num_seqs && grp <= PROWS / 2;
+    return (long long)p->total_q * grp > 16ll * p->num_seqs && grp <= PROWS / 2 && (p->q_token > 0 || p->total_q == 1) &&
+           (p->q_head > 0 || p->num_q_heads == 1);
 }
 size_t span_workspace(const mq_paged_span_params* p, SpanCut** cuts, float** slots, void* base) {
     const size_t at = up256(sm_count() * sizeof(SpanCut));
@@ -704,16 +706,26 @@ int run_prefix(const RowArgs& a, const mq_paged_pool& pool, cudaStream_t st) {
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "paged prefix attention");
 }
 
+// q in boxes of the tokens of a stream, a kv head's q heads each, blocks of 64 channels.
+bool span_q_map(CUtensorMap* m, const RowArgs& a, int D, int dtype) {
+    const cuuint64_t dims[4] = {64, (cuuint64_t)D / 64, (cuuint64_t)a.hq, (cuuint64_t)a.total_q};
+    // the stride of a dimension of one is never used and may be anything
+    const cuuint64_t row = (cuuint64_t)D * 2;
+    const cuuint64_t strides[3] = {128, a.hq > 1 ? (cuuint64_t)a.q_head * 2 : row, a.total_q > 1 ? (cuuint64_t)a.q_tok * 2 : row * a.hq};
+    const cuuint32_t box[4] = {64, 1, (cuuint32_t)a.grp, (cuuint32_t)(PROWS / 2 / a.grp)};
+    return make_tmap_nd(m, a.q, dtype == MQ_BF16, 4, dims, strides, box);
+}
+
 template <typename T, int D>
 int run_span_tc(const RowArgs& a, SpanCut* cuts, const mq_paged_pool& pool, cudaStream_t st) {
-    CUtensorMap tk, tv;
-    if (!pool_maps(&tk, &tv, pool, a.pool, pool.page_size, 1)) return MQ_ERR_CUDA;
+    CUtensorMap tq, tk, tv;
+    if (!pool_maps(&tk, &tv, pool, a.pool, pool.page_size, 1) || !span_q_map(&tq, a, D, pool.dtype)) return MQ_ERR_CUDA;
     auto kernel = span_kernel<T, D>;
     const size_t smem = SpanSmem<D>::bytes(a.B);
     static SmemLimit limit;
     cudaError_t e = allow_smem(kernel, smem, limit);
     const int grid = sm_count();
-    if (e == cudaSuccess) e = launch(kernel, dim3(grid), dim3(SPAN_THREADS), smem, st, tk, tv, a, cuts);
+    if (e == cudaSuccess) e = launch(kernel, dim3(grid), dim3(SPAN_THREADS), smem, st, tq, tk, tv, a, cuts);
     if (e == cudaSuccess) e = launch(span_join_kernel<T, D>, dim3(grid, PROWS / SPAN_JOIN_ROWS), dim3(256), 0, st, a, (const SpanCut*)cuts);
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "paged attention under a mask");
 }

@@ -28,7 +28,7 @@
 namespace mq {
 namespace paged {
 
-constexpr int SPAN_THREADS = 640;   // warps: 0 K, 1 MMA, 2 V, 3-10 softmax of A, 11-18 of B, 19 looks through V
+constexpr int SPAN_THREADS = 640;   // warps: 0 K, 1 MMA, 2 Q and V, 3 looks through V, 4-11 softmax of A, 12-19 of B
 
 template <int D>
 struct SpanSmem {
@@ -53,7 +53,7 @@ struct SpanSeg {
     int seq0, pf, pl;             // the sequence's first token; positions of the tile's first and last token
     int st, wt, ng;               // sink tiles, first window tile, tiles in all
     int t0, n, runs;              // of this run; runs that share the item
-    bool two, start, whole;
+    bool two, both, start, whole;   // two: each stream has rows of its own; both: B works, too
 };
 
 // Tiles of a row tile whose tokens stand at pf .. pl: st of the sinks, then wt .. the one of pl.
@@ -85,10 +85,39 @@ __device__ __forceinline__ unsigned long long span_sees(const RowArgs& a, int p,
     return bits;
 }
 
+__device__ __forceinline__ void tma_load_heads(uint32_t dst, const CUtensorMap* map, int block, int head, int token, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        ::"r"(dst), "l"(map), "r"(0), "r"(block), "r"(head), "r"(token), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// Two fp32 values side by side.
+__device__ __forceinline__ uint64_t two_of(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ void halves(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(SPAN_THREADS, 1)
-span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const RowArgs a,
-            SpanCut* __restrict__ cuts) {
+span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+            const __grid_constant__ CUtensorMap tmV, const RowArgs a, SpanCut* __restrict__ cuts) {
     using L = SpanSmem<D>;
     constexpr int TILE = L::TILE, LD = D + 4, NT = SPAN_THREADS;
     extern __shared__ uint8_t pfx_raw[];
@@ -103,16 +132,19 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     uint64_t* s_full = bars + 12;     // [2] streams: S is there (and every MMA issued before it is done)
     uint64_t* p_full = bars + 14;     // [2] P is stored, O is rescaled
     uint64_t* o_full = bars + 16;     // [2] the run's last PV is done
-    uint64_t* drain = bars + 18;
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 19);
+    uint64_t* q_empty = bars + 18;    // [2]
+    uint64_t* drain = bars + 20;
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 21);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-    volatile int* odd_tile = abort_flag + 1;   // [2] stages: the tile holds values that are not finite
+    volatile int* holes = abort_flag + 1;      // a page out of range has been met
+    volatile int* odd_tile = abort_flag + 2;   // [2] stages: the tile holds values that are not finite
     __shared__ uint32_t scratch[NT / 32];
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&q_full[i], 8);
+            mbar_init(&q_full[i], 1);
+            mbar_init(&q_empty[i], 1);
             mbar_init(&k_full[i], 1);
             mbar_init(&k_empty[i], 1);
             mbar_init(&v_full[i], 1);
@@ -124,7 +156,9 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         }
         mbar_init(drain, 1);
         *abort_flag = 0;
+        *holes = 0;
         fence_mbar_init();
+        prefetch_tmap(&tmQ);
         prefetch_tmap(&tmK);
         prefetch_tmap(&tmV);
     }
@@ -142,7 +176,7 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     // ---- the line: off[b] units before sequence b, for one kv head ----
     uint32_t* off = reinterpret_cast<uint32_t*>(smem + L::SCHED);   // [B + 1]
     int* lens = reinterpret_cast<int*>(off + a.B + 1);              // [B], 0 where nothing is read
-    const int grp = a.grp, page = a.pool.page, tpt = PROWS / grp;   // tokens to a row tile
+    const int grp = a.grp, page = a.pool.page, tps = PROWS / 2 / grp, tpt = 2 * tps;   // tokens to a stream and to a row tile
     bool bad = false;
     if (a.q_starts) {
         for (int b = threadIdx.x; b < a.B; b += NT)
@@ -249,7 +283,8 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         const int pos = (int)rel, left = (int)min((uint32_t)(e.ng + ITEM_UNITS - pos), xe - x);
         e.t0 = max(pos - ITEM_UNITS, 0);
         e.n = max(pos + left - ITEM_UNITS, 0) - e.t0;
-        e.two = e.rows > 128;
+        e.two = e.rows > tps * grp;
+        e.both = e.two || e.n > 1;
         e.start = e.t0 == 0;
         e.whole = e.n == e.ng;
         const uint32_t ps = x - pos + ITEM_UNITS;   // the item's first tile on the line
@@ -283,20 +318,40 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     };
 
     if (warp == 0 || warp == 2) {
-        // ---- K and V producers: lane c loads the tile's c-th page ----
+        // ---- K and V producers: lane c loads the tile's c-th page.  That of V also loads the items' Q, a box of whole
+        // tokens for each stream, once the last scores of the item before are there ----
         uint64_t* full = warp == 0 ? k_full : v_full;
         uint64_t* empty = warp == 0 ? k_empty : v_empty;
         const CUtensorMap* map = warp == 0 ? &tmK : &tmV;
         uint8_t* ring = smem + (warp == 0 ? L::K : L::V);
         const int chunks = PK / page;
-        int c = 0;   // tiles so far
+        int c = 0, nq0 = 0, nq1 = 0;   // tiles so far, Q tiles of A and B
         bool ok = true, cut = false;
+        auto load_q = [&](const SpanSeg& e, int q, int used) {
+            if (used && !wait(&q_empty[q], (used - 1) & 1)) return false;
+            if (lane == 0) {
+                mbar_arrive_expect_tx(&q_full[q], (D / 64) * tps * grp * 128);
+#pragma unroll
+                for (int i = 0; i < D / 64; ++i)
+                    tma_load_heads(smem_u32(smem + L::Q + q * TILE + i * PATOM), &tmQ, i, e.h * grp,
+                                   e.tok0 + (e.two ? q * tps : 0), smem_u32(&q_full[q]));
+            }
+            return true;
+        };
         for (uint32_t x = x0; ok && x < xe;) {
             const SpanSeg e = segment(x);
             if (e.n <= 0) continue;
             if (warp == 0 && e.start && !e.whole) {   // (the run's last item)
                 if (lane == 0) *reinterpret_cast<int4*>(cuts + blockIdx.x) = make_int4(e.tok0, e.h, e.rows, e.runs);
                 cut = true;
+            }
+            if (warp == 2) {
+                ok = load_q(e, 0, nq0++);
+                if (ok && e.both) ok = load_q(e, 1, nq1++);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
             }
             const int* row = a.table + __ldg(a.slots + e.b) * a.table_row;
             // what no row sees is read as zeros, from outside the map
@@ -309,7 +364,10 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 int pid = next;
                 if (j + 1 < e.n) next = look(j + 1);
                 if (pid < 0 || pid >= a.pool.pages) {
-                    if (lane < chunks && in_sight(e, tile_at(e, j) + lane * page)) note_status(a.status, MQ_ERR_BAD_PAGE);
+                    if (lane < chunks && in_sight(e, tile_at(e, j) + lane * page)) {
+                        note_status(a.status, MQ_ERR_BAD_PAGE);
+                        *holes = 1;   // before the tile's scores are there
+                    }
                     pid = a.pool.pages;
                 }
                 const int st = c & 1;
@@ -330,12 +388,17 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         if (warp == 0 && !cut && lane == 0) *reinterpret_cast<int4*>(cuts + blockIdx.x) = make_int4(0, 0, 0, 0);
         if (!ok && lane == 0) give_up();
         // copies in flight land before the CTA may end, whatever became of their readers
-        for (int k = max(0, c - 2); k < c; ++k) {
+        auto land = [&](uint64_t* bar, uint32_t parity) {
             const long long t0 = clock64();
-            while (!mbar_try_wait(&full[k & 1], (k >> 1) & 1) && clock64() - t0 < WAIT_CYCLES) {
+            while (!mbar_try_wait(bar, parity) && clock64() - t0 < WAIT_CYCLES) {
             }
+        };
+        for (int k = max(0, c - 2); k < c; ++k) land(&full[k & 1], (k >> 1) & 1);
+        if (!ok && warp == 2) {   // (otherwise the scores of every Q tile have been waited for)
+            if (nq0) land(&q_full[0], (nq0 - 1) & 1);
+            if (nq1) land(&q_full[1], (nq1 - 1) & 1);
         }
-    } else if (warp == 19) {
+    } else if (warp == 3) {
         // ---- looks through the values of masked tiles ----
         int c = 0;
         bool ok = true;
@@ -385,13 +448,15 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     } else if (warp == 1) {
         // ---- MMA: the whole warp walks, one elected lane issues.  All 512 columns of
         // TMEM are this CTA's, so their addresses start at 0 ----
-        constexpr uint32_t id_s = pfx_idesc<T>(PK, false), id_o = pfx_idesc<T>(D, true);
+        constexpr uint32_t id_o = pfx_idesc<T>(D, true);
+        // a negative scale: the scores of -Q
+        const uint32_t id_s = pfx_idesc<T>(PK, false) | (a.scale_log2 < 0.f ? 1u << 13 : 0u);
         const uint32_t base = (smem_u32(pfx_raw) + 1023u) & ~1023u;
         int c0 = 0;                         // tiles of the segments before
         uint32_t np0 = 0, np1 = 0;          // PVs issued per stream
         uint32_t nq0 = 0, nq1 = 0;          // Q tiles used per stream
         bool ok = true;
-        auto scores = [&](int q, int kc, bool last_use) {
+        auto scores = [&](int q, int kc, bool last_use, bool last) {
             const uint32_t sq = base + L::Q + q * TILE, sk = base + L::K + (kc & 1) * TILE;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
@@ -400,16 +465,15 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
             }
             tc_commit(&s_full[q]);
             if (last_use) tc_commit(&k_empty[kc & 1]);
+            if (last) tc_commit(&q_empty[q]);
         };
         auto values = [&](int q, int vc, bool first, bool last_use, bool done) {
             const uint32_t sv = base + L::V + (vc & 1) * TILE, o = 256 + q * 128;
 #pragma unroll
             for (int k = 0; k < PK / 16; ++k) {
-                // 16 keys: 8 columns of values, the remainders 16 columns on
-                const uint32_t p = q * 128 + 32 * (k >> 1) + 8 * (k & 1);
-                const uint64_t dv = sw128_mnmajor_desc(sv + k * 2048);
-                tc_mma_f16_ts(o, p, dv, id_o, !first || k);
-                tc_mma_f16_ts(o, p + 16, dv, id_o, 1);
+                // 16 keys: 8 columns, those of a half in its own 64
+                const uint32_t p = q * 128 + 64 * (k >> 2) + 8 * (k & 3);
+                tc_mma_f16_ts(o, p, sw128_mnmajor_desc(sv + k * 2048), id_o, !first || k);
             }
             if (last_use) tc_commit(&v_empty[vc & 1]);
             if (done) tc_commit(&o_full[q]);
@@ -440,7 +504,7 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 tc_fence_after();
                 if (elect_one()) {
                     if (pv) values(q, vc, i < 4, !two || q == 1, !sc);
-                    if (sc) scores(q, kc, !two || q == 1);
+                    if (sc) scores(q, kc, !two || q == 1, i >= steps - 2);
                 }
                 __syncwarp();
             }
@@ -454,12 +518,11 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         }
     } else {
         // ---- softmax of stream q, column half hh: two threads to a row ----
-        const int q = (warp - 3) >> 3, hh = ((warp - 3) >> 2) & 1;
+        const int q = (warp - 4) >> 3, hh = ((warp - 4) >> 2) & 1;
         const int quad = warp & 3;                     // the TMEM lanes this warp may touch
         const int r = quad * 32 + lane;
         // a scale of zero: a masked score of minus infinity stays one
         const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);
-        const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
         const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
         const uint32_t sa = tmem + lane_off + q * 128 + hh * 64, oa = tmem + lane_off + 256;   // O of A, that of B 128 columns on
         float* red = reinterpret_cast<float*>(smem + L::RED) + q * 512;
@@ -477,85 +540,58 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
             if (ok) ok = __all_sync(0xffffffffu, wait(bar, parity));
             return ok;
         };
-        for (uint32_t x = x0; x < xe;) {
-            const SpanSeg e = segment(x);
-            if (e.n <= 0) continue;
+        const int tok_r = r / grp, head_r = r - tok_r * grp;   // of this row in its stream
+        SpanSeg next;
+        uint32_t x = x0;
+        next.n = 0;
+        // the next item with tiles, looked up while the last results of the one before are on their way
+        auto advance = [&]() {
+            next.n = 0;
+            while (x < xe && next.n <= 0) next = segment(x);
+        };
+        advance();
+        while (next.n > 0) {
+            const SpanSeg e = next;
             const int mine = e.two ? e.n : (e.n + 1 - q) >> 1;   // this stream's tiles
-            const int wr = e.two ? q * 128 + r : r;              // the row in the item
-            const int tok = wr / grp, head = e.h * grp + wr - tok * grp;
-            const bool there = wr < e.rows;
+            const int tok = (e.two ? q * tps : 0) + tok_r;       // the row's token in the item
+            const bool there = tok_r < tps && tok * grp < e.rows;
             const int pos = min(e.pf + tok, e.pl), node = e.tok0 - e.seq0 + pos - e.pf;
             unsigned long long hit = 0;
             float m = -INFINITY, l = 0.f;
-            if (mine) {
-                meet();   // both warps are done with the Q rows of the item before
-                // Q rows, swizzled as TMA would, zeros past the end; a negative scale turns their
-                // signs.  Half the rows each, LPR lanes side by side on a row, all loads in flight.
-                const uint16_t* src = there ? a.q + (long long)(e.tok0 + tok) * a.q_tok + head * a.q_head : nullptr;
-                constexpr int LPR = D / 8, RPI = 32 / LPR, N = 16 / RPI;
-                const int ch = lane % LPR, sub = lane / LPR;
-                uint4 v[N];
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const uint16_t* row = from_lane(src, hh * 16 + i * RPI + sub);
-                    v[i] = row ? __ldg(reinterpret_cast<const uint4*>(row + ch * 8)) : make_uint4(0, 0, 0, 0);
-                }
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int w = quad * 32 + hh * 16 + i * RPI + sub;
-                    v[i].x ^= sign; v[i].y ^= sign; v[i].z ^= sign; v[i].w ^= sign;
-                    *reinterpret_cast<uint4*>(smem + L::Q + q * TILE + (ch >> 3) * PATOM + w * 128 +
-                                              (((ch & 7) ^ (w & 7)) << 4)) = v[i];
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full[q]);
-            }
-            // lane c: whether the c-th page of the tile at `at` is out of range
-            const int* trow = a.table + __ldg(a.slots + e.b) * a.table_row;
-            auto gone = [&](int at, int c) {
-                at += c * page;
-                if (!in_sight(e, at)) return false;
-                const int pid = __ldg(trow + (at >> a.pool.shift));
-                return pid < 0 || pid >= a.pool.pages;
-            };
-            // looked up once per run, while the first scores are on their way, and again tile by tile only if there are any
-            bool holes = false;
-            if (mine) {
-                const int chunks = PK / page;
-#pragma unroll 1
-                for (int i = lane; i < e.n * chunks; i += 32) holes |= gone(tile_at(e, i / chunks), i % chunks);
-                holes = __any_sync(0xffffffffu, holes);
-            }
             for (int j = 0; j < mine; ++j, ++ns) {
                 float tmax = -INFINITY;
                 const int jt = e.two ? j : 2 * j + q, at = tile_at(e, jt);
-                const unsigned none = holes ? __ballot_sync(0xffffffffu, lane < PK / page && gone(at, lane)) : 0u;
                 const bool masked = !all_seen(e, at);
+                unsigned long long live = ~0ull;   // keys of this half that the row sees
+                if (masked) live = span_sees(a, pos, at + hh * 64, node, e.seq0);
                 if (got(&s_full[q], ns & 1)) {
                     tc_fence_after();
-                    if (masked || none) {
-                        const unsigned long long live = masked ? span_sees(a, pos, at + hh * 64, node, e.seq0) : ~0ull;
-#pragma unroll 1
-                        for (int i = 0; i < 64; i += 32) {
-                            uint32_t lv = (uint32_t)(live >> i);
-                            for (int k = 0; k < 32; k += 16)   // a page is 16 keys or more
-                                if (none >> ((hh * 64 + i + k) >> a.pool.shift) & 1u) lv &= ~(0xffffu << k);
-                            if (__all_sync(0xffffffffu, lv == 0xffffffffu)) continue;
-                            float sv[32];
-                            tmem_ld32(sa + i, sv);
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) sv[k] = lv >> k & 1u ? sv[k] : -INFINITY;
-                            tmem_st32(sa + i, sv);
+                    if (*holes) {   // pages out of range: their keys are left out
+                        const int* row = a.table + __ldg(a.slots + e.b) * a.table_row;
+                        for (int k = 0; k < 64; k += min(page, 64)) {
+                            const int p = (at + hh * 64 + k) & -page;
+                            const int pid = in_sight(e, p) ? __ldg(row + (p >> a.pool.shift)) : 0;
+                            if (pid < 0 || pid >= a.pool.pages) live &= ~((page >= 64 ? ~0ull : (1ull << page) - 1ull) << k);
                         }
                     }
-                    // two passes over S in TMEM: the code stays small (a run is a few tiles long, and
-                    // fetching unrolled code the first time cost more than reading S twice)
-                    float sv[64], mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    // two passes over S in TMEM: the registers do not hold it and the weights
+                    float sv[64], mx[4];
                     tmem_ld64(sa, sv);
+                    if (__any_sync(0xffffffffu, live != ~0ull)) {
+                        const uint32_t lo = (uint32_t)live, hi = (uint32_t)(live >> 32);
 #pragma unroll
-                    for (int k = 0; k < 64; ++k) mx[k & 3] = fmaxf(mx[k & 3], sv[k]);
-                    tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+                        for (int k = 0; k < 32; ++k) {
+                            sv[k] = lo >> k & 1u ? sv[k] : -INFINITY;
+                            sv[32 + k] = hi >> k & 1u ? sv[32 + k] : -INFINITY;
+                        }
+                        tmem_st32(sa, sv);
+                        tmem_st32(sa + 32, sv + 32);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mx[k] = fmaxf(sv[2 * k], sv[2 * k + 1]);
+#pragma unroll
+                    for (int k = 8; k < 64; k += 2) mx[(k >> 1) & 3] = max3(mx[(k >> 1) & 3], sv[k], sv[k + 1]);
+                    tmax = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale;
                 }
                 red[((j & 1) * 2 + hh) * 128 + r] = tmax;
                 meet();
@@ -579,25 +615,27 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                         tmem_st16(oa + q * 128 + hh * (D / 2) + i, v);
                     }
                 }
-                const float u = m == -INFINITY ? 0.f : m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
+                const uint64_t scale2 = two_of(scale, scale), u2 = m == -INFINITY ? 0ull : two_of(-m, -m);
+                uint64_t sum0 = 0ull, sum1 = 0ull;
+#pragma unroll
                 for (int i = 0; i < 64; i += 32) {
                     float sv[32];
-                    uint32_t pk[32];   // 32 weights in 16 columns, their remainders in the next 16
+                    uint32_t pk[16];   // 32 weights in 16 columns
                     tmem_ld32(sa + i, sv);
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        const float p0 = ex2(fmaf(sv[2 * k], scale, -u)), p1 = ex2(fmaf(sv[2 * k + 1], scale, -u));
-                        sum[k & 3] += p0 + p1;
+                        float p0, p1;
+                        halves(fma2(two_of(sv[2 * k], sv[2 * k + 1]), scale2, u2), p0, p1);
+                        p0 = ex2(p0);
+                        p1 = ex2(p1);
+                        (k & 1 ? sum1 : sum0) = add2(k & 1 ? sum1 : sum0, two_of(p0, p1));
                         pk[k] = Elem<T>::pack(p0, p1);
-                        const float2 b = Elem<T>::up2(pk[k]);
-                        pk[16 + k] = Elem<T>::pack(p0 - b.x, p1 - b.y);
                     }
-                    tmem_st16_nowait(sa + i, pk);
-                    tmem_st16_nowait(sa + i + 16, pk + 16);
+                    tmem_st16_nowait(sa + (i >> 1), pk);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                float s0, s1;
+                halves(add2(sum0, sum1), s0, s1);
+                l += s0 + s1;
                 if (masked) {
                     // the tile's values are looked through, and stay until this stream's weights are used
                     const int c = nv + jt, st = c & 1;
@@ -605,12 +643,13 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                         const uint8_t* bits = smem + L::ODD + st * 128 * (D / 8) + hh * (D / 16);
 #pragma unroll 1
                         for (int k0 = 0; k0 < PK; k0 += 64) {
-                            const unsigned long long live = span_sees(a, pos, at + k0, node, e.seq0);
+                            const unsigned long long seen = span_sees(a, pos, at + k0, node, e.seq0);
+#pragma unroll 1
                             for (int k = 0; k < 64; ++k) {
                                 unsigned long long w;
                                 if (D == 128) w = *reinterpret_cast<const unsigned long long*>(bits + (k0 + k) * (D / 8));
                                 else w = *reinterpret_cast<const uint32_t*>(bits + (k0 + k) * (D / 8));
-                                if (live >> k & 1ull) hit |= w;
+                                if (seen >> k & 1ull) hit |= w;
                             }
                         }
                     }
@@ -621,14 +660,15 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 if (lane == 0) mbar_arrive(&p_full[q]);
             }
             nv += e.n;
+            advance();
             // ---- the item's rows: what A and B have of them, when they share them ----
-            const bool b_too = e.two ? q == 1 : e.n > 1, a_too = e.two ? q == 0 : true;
-            if (a_too) got(&o_full[0], no0 & 1);
-            if (b_too) got(&o_full[1], no1 & 1);
+            if (!e.two || q == 0) got(&o_full[0], no0 & 1);
+            if (e.two ? q == 1 : e.both) got(&o_full[1], no1 & 1);
             ++no0;
-            no1 += e.two || e.n > 1;
+            no1 += e.both;
             tc_fence_after();
             sums[(q * 2 + hh) * 128 + r] = l;
+            float e0 = 1.f, e1 = 1.f;   // weights of A's and B's accumulators
             if (e.two) {
                 meet();
                 l += sums[(q * 2 + (hh ^ 1)) * 128 + r];
@@ -636,10 +676,6 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 if (hh == 0) tops[q * 128 + r] = m;
                 hits[(q * 2 + hh) * 128 + r] = hit;
                 meet4();
-            }
-            // this thread's columns: its half, or with two streams on a row half of that
-            float e0 = 1.f, e1 = 1.f;   // weights of A's and B's accumulators
-            if (!e.two) {
                 const float ma = tops[r], mb = tops[128 + r];   // (B's is -inf when it had no tile)
                 m = fmaxf(ma, mb);
                 const float u = m == -INFINITY ? 0.f : m;
@@ -649,9 +685,10 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 hit = hits[hh * 128 + r] | hits[(2 + hh) * 128 + r];
             }
             const float inv = l != 0.f ? 1.f / l : 0.f;   // a row that sees nothing is zero (NaN stays NaN)
+            // this thread's columns: its half, or with two streams on a row half of that
             const int width = e.two ? D / 2 : D / 4, c_lo = hh * (D / 2) + (e.two ? 0 : q * (D / 4));
-            float* part = a.ws.pfx_slots + ((2ll * blockIdx.x + e.start) * PROWS + wr) * LD;
-            uint16_t* out = a.out + ((long long)(e.tok0 + tok) * a.hq + head) * D;
+            float* part = a.ws.pfx_slots + ((2ll * blockIdx.x + e.start) * PROWS + tok * grp + head_r) * LD;
+            uint16_t* out = a.out + ((long long)(e.tok0 + tok) * a.hq + e.h * grp + head_r) * D;
             if (!e.whole && ok && there && hh == 0 && (e.two || q == 0))
                 *reinterpret_cast<float4*>(part) = make_float4(m, l, 0.f, 0.f);
 #pragma unroll 1
@@ -661,9 +698,9 @@ span_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 tmem_ld16(oa + (e.two ? q * 128 : 0) + c, v);
                 if (!e.two) {
                     float w[16];
-                    if (b_too) tmem_ld16(oa + 128 + c, w);
+                    if (e.both) tmem_ld16(oa + 128 + c, w);
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) v[k] = b_too ? v[k] * e0 + w[k] * e1 : v[k] * e0;
+                    for (int k = 0; k < 16; ++k) v[k] = e.both ? v[k] * e0 + w[k] * e1 : v[k] * e0;
                 }
                 const uint32_t odd = (uint32_t)(hit >> (c - hh * (D / 2))) & 0xffffu;
                 if (odd) {

@@ -1,7 +1,9 @@
 """Windowed attention and drafted trees on the paged cache against a plain implementation in 64 bits.
 
-Tolerances as for the other attention of the cache (test_paged_gpu.py): the output's one rounding, half a step of its type,
-and 2^-13 of the largest value for scores in fp32 and weights in two 16-bit pieces.
+Tolerances.  As for the other attention of the cache (test_paged_gpu.py): the output's one rounding, half a step h of its
+type, and 2^-13 of the largest value for scores in fp32 and weights in two 16-bit pieces.  Calls of more than 16 rows to a
+sequence run on a kernel that rounds each weight once to 16 bits: sum_j p_j (1 + d_j) v_j with |d_j| <= h, which is off by
+at most h sum_j p_j |v_j|, in the result (and rounded with it: h^2 of that, within the 2^-13).
 """
 from __future__ import annotations
 
@@ -10,7 +12,7 @@ import math
 import pytest
 import torch
 
-from test_paged_gpu import Pool, close, dev, gen, normal, softmax_rows
+from test_paged_gpu import ROUND, Pool, close, dev, gen, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -55,17 +57,39 @@ def tree_mask(parents, t):
     return seen.cuda()
 
 
+def once(tokens, group, seqs):
+    """Whether such a call rounds its weights once."""
+    return tokens * group > 16 * seqs
+
+
+def near(got, ref, vmax, rounded):
+    """ref: (the result, sum p |v|) in 64 bits."""
+    out, mass = ref
+    if not rounded:
+        return close(got, out, vmax)
+    tol = ROUND[got.dtype] * (out.abs() + mass) + 2.0 ** -13 * vmax + 2.0 ** -24
+    bad = (got.double() - out).abs() - tol
+    assert bool((bad <= 0).all()), f"over by {bad.max().item():.3e} (vmax {vmax:.3f})"
+
+
+def pick(ref, *at):
+    return tuple(x[at] for x in ref)
+
+
 def reference(p, b, q, seen, scale, layer):
-    """q [n, hq, d] of sequence b, seen [n, t]; in 64 bits, rows that see nothing are zero."""
+    """q [n, hq, d] of sequence b, seen [n, t]; in 64 bits, rows that see nothing are zero.  Also sum p |v|."""
     k, v = p.kv(b, layer)
     hq, hkv = q.shape[1], k.shape[1]
     grp = hq // hkv
     out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    mass = torch.zeros_like(out)
     for h in range(hq):
         z = (q[:, h].double() @ k[:, h // grp].T) * scale
         w = torch.softmax(z.masked_fill(~seen, -math.inf), -1)
-        out[:, h] = torch.where(seen.any(-1, keepdim=True), torch.where(seen, w, 0) @ v[:, h // grp], 0)
-    return out
+        w = torch.where(seen, w, 0)
+        out[:, h] = w @ v[:, h // grp]
+        mass[:, h] = w @ v[:, h // grp].abs()
+    return out, mass
 
 
 def check(p, call, qlens, masks, q, scale=None, layer=1):
@@ -78,7 +102,7 @@ def check(p, call, qlens, masks, q, scale=None, layer=1):
     for b, n in enumerate(qlens):
         if n:
             ref = reference(p, b, q[starts[b]:starts[b + 1]], masks[b], s, layer)
-            close(got[starts[b]:starts[b + 1]], ref, p.v.abs().max().item())
+            near(got[starts[b]:starts[b + 1]], ref, p.v.abs().max().item(), once(starts[-1], q.shape[1] // p.k.shape[2], len(qlens)))
     assert status.item() == 0
     return got
 
@@ -151,7 +175,11 @@ def test_window_of_everything_is_attend(paged, qlens):
     starts = dev(starts_of(qlens))
     a = paged.attend(q, p.k, p.v, p.table, p.lengths, dev(p.slots), layer=0, q_starts=starts)
     b = paged.window_attend(q, p.k, p.v, p.table, p.lengths, dev(p.slots), layer=0, window=500, q_starts=starts)
-    close(b, a.double(), p.v.abs().max().item())
+    for i, (n, t) in enumerate(zip(qlens, p.lens)):
+        rows = slice(i * qlens[0], i * qlens[0] + n)
+        ref = reference(p, i, q[rows], window_mask(n, t, t, 0), 1 / 8, 0)
+        for x in (a, b):
+            near(x[rows], ref, p.v.abs().max().item(), once(sum(qlens), 2, 2))
 
 
 @pytest.mark.parametrize("scale", [-0.09, 0.0, 0.3])
@@ -205,14 +233,14 @@ def test_window_masked_infinities(paged, n, d):
             seen = window_mask(n, t, window, sinks)
             sees = seen[:, at]
             ref = reference(p, 0, q, seen, 1 / math.sqrt(d), 1)
-            vmax = p.v.abs().max().item()
-            close(got[~sees], ref[~sees], vmax)
+            vmax, rounded = p.v.abs().max().item(), once(n, 2, 1)
+            near(got[~sees], pick(ref, ~sees), vmax, rounded)
             if key:
                 assert bool(got[sees].isnan().all())
             else:
                 assert not bool(got[sees][..., chan].isfinite().any())
                 other = [c for c in range(d) if c != chan]
-                close(got[sees][..., other], ref[sees][..., other], vmax)
+                near(got[sees][..., other], tuple(x[sees][..., other] for x in ref), vmax, rounded)
 
 
 # ---- trees -------------------------------------------------------------------------------------------------------
@@ -265,9 +293,9 @@ def test_tree_masked_infinities(paged, n):
             v[row[-1], 1, 0, (t - 1) % 32 + 1:] = bad
             got = paged.tree_attend(q, p.k, v, p.table, p.lengths, dev(p.slots), dev(tree), layer=1, q_starts=dev([0, n]))
             sees = seen[:, at]
-            close(got[~sees], ref[~sees], vmax)
+            near(got[~sees], pick(ref, ~sees), vmax, once(n, 2, 1))
             assert not bool(got[sees][..., 11].isfinite().any())
-            close(got[sees][..., 12:], ref[sees][..., 12:], vmax)
+            near(got[sees][..., 12:], tuple(x[sees][..., 12:] for x in ref), vmax, once(n, 2, 1))
 
 
 @pytest.mark.parametrize("n,other", [(5, 1), (100, 40)])
@@ -285,15 +313,16 @@ def test_tree_wrong_parents(paged, n, other):
                                 q_starts=dev([0, n, n + other]), status=status)
         assert status.item() == 1
         vmax = p.v.abs().max().item()
-        close(got[:n], reference(p, 0, q[:n], tree_mask(as_read, n + 50), 1 / 8, 1), vmax)
-        close(got[n:], reference(p, 1, q[n:], tree_mask(rest, other + 9), 1 / 8, 1), vmax)
+        rounded = once(n + other, 2, 2)
+        near(got[:n], reference(p, 0, q[:n], tree_mask(as_read, n + 50), 1 / 8, 1), vmax, rounded)
+        near(got[n:], reference(p, 1, q[n:], tree_mask(rest, other + 9), 1 / 8, 1), vmax, rounded)
     p = Pool([400, 40], 16, 2, 64, torch.bfloat16, seed=8)
     q = normal(p.g, 257 + 7, 4, 64)
     rest, status = random_tree(4, 7), dev([0])
     got = paged.tree_attend(q, p.k, p.v, p.table, p.lengths, dev(p.slots), dev([-1] * 257 + rest), layer=1,
                             q_starts=dev([0, 257, 264]), status=status)
     assert status.item() == 1 and not bool(got[:257].any())
-    close(got[257:], reference(p, 1, q[257:], tree_mask(rest, 40), 1 / 8, 1), p.v.abs().max().item())
+    near(got[257:], reference(p, 1, q[257:], tree_mask(rest, 40), 1 / 8, 1), p.v.abs().max().item(), True)
 
 
 # ---- both ----------------------------------------------------------------------------------------------------------
@@ -325,8 +354,8 @@ def test_more_tokens_than_positions(paged, n):
         vmax = p.v.abs().max().item()
         if n > 1:
             ref = reference(p, 0, q[1:n], masks[0][1:], 1 / 8, 1)
-            close(got[1:n], ref, vmax)
-        close(got[2 * n:], reference(p, 2, q[2 * n:], masks[2], 1 / 8, 1), vmax)
+            near(got[1:n], ref, vmax, once(3 * n, 2, 3))
+        near(got[2 * n:], reference(p, 2, q[2 * n:], masks[2], 1 / 8, 1), vmax, once(3 * n, 2, 3))
 
 
 @pytest.mark.parametrize("n", [2, 150])
@@ -335,37 +364,45 @@ def test_wrong_tables(paged, n):
     p = Pool([200, 160, 180], 16, 2, 64, torch.float16, seed=11)
     q = normal(p.g, 3 * n, 4, 64, dtype=torch.float16)
     starts = dev([0, n, 2 * n, 3 * n])
+    vmax, rounded = p.v.abs().max().item(), once(3 * n, 2, 3)
     for call, masks in calls(paged, p, n):
-        want = call(q, dev(p.slots), starts, None)
+        want = [reference(p, b, q[b * n:b * n + n], masks[b], 1 / 8, 1) for b in range(3)]
+
+        def others(got, *bad):
+            for b in range(3):
+                if b in bad:
+                    assert not bool(got[b * n:b * n + n].any())
+                else:
+                    near(got[b * n:b * n + n], want[b], vmax, rounded)
+
+        others(call(q, dev(p.slots), starts, None))
         for bad, code in ((-1, 8), (4, 8), (10 ** 9, 8)):
             status, slots = dev([0]), list(p.slots)
             slots[1] = bad
-            got = call(q, dev(slots), starts, status)
-            assert status.item() == code and not bool(got[n:2 * n].any())
-            close(got[:n], want[:n].double(), 5.0)
-            close(got[2 * n:], want[2 * n:].double(), 5.0)
+            others(call(q, dev(slots), starts, status), 1)
+            assert status.item() == code
         for length in (-3, 16 * p.table.shape[1] + 1):
             status, lengths = dev([0]), p.lengths.clone()
             lengths[p.slots[1]] = length
-            got = call(q, dev(p.slots), starts, status, lengths=lengths)
-            assert status.item() == 5 and not bool(got[n:2 * n].any())
-            close(got[:n], want[:n].double(), 5.0)
+            others(call(q, dev(p.slots), starts, status, lengths=lengths), 1)
+            assert status.item() == 5
         for wrong in ([0, 2 * n, n, 3 * n], [1, n, 2 * n, 3 * n], [0, n, 2 * n, 3 * n - 1], [-n, 0, n, 3 * n]):
             status = dev([0])
-            got = call(q, dev(p.slots), dev(wrong), status)
-            assert status.item() == 1 and not bool(got.any())
+            others(call(q, dev(p.slots), dev(wrong), status), 0, 1, 2)
+            assert status.item() == 1
         # a page out of range: its positions are left out
         for page in (-1, p.k.shape[0], 2 ** 31 - 1):
-            status, table = dev([0]), p.table.clone()
-            c = (p.lens[2] - 20) // 16
-            table[p.slots[2], c] = page
-            got = call(q, dev(p.slots), starts, status, table=table)
-            assert status.item() == 9
-            seen = masks[2].clone()
-            seen[:, c * 16:c * 16 + 16] = False
-            ref = reference(p, 2, q[2 * n:], seen, 1 / 8, 1)
-            close(got[2 * n:], ref, p.v.abs().max().item())
-            close(got[:2 * n], want[:2 * n].double(), 5.0)
+            for back in (20, 100):
+                status, table = dev([0]), p.table.clone()
+                c = (p.lens[2] - back) // 16
+                table[p.slots[2], c] = page
+                got = call(q, dev(p.slots), starts, status, table=table)
+                seen = masks[2].clone()
+                assert status.item() == (9 if bool(seen[:, c * 16:c * 16 + 16].any()) else 0)
+                seen[:, c * 16:c * 16 + 16] = False
+                near(got[2 * n:], reference(p, 2, q[2 * n:], seen, 1 / 8, 1), vmax, rounded)
+                for b in range(2):
+                    near(got[b * n:b * n + n], want[b], vmax, rounded)
 
 
 @pytest.mark.parametrize("n", [1, 40, 150])
@@ -382,7 +419,7 @@ def test_strides_layers_and_offsets(paged, n):
     for call, masks in calls(paged, p, n):
         want = call(q, dev(p.slots), starts, None, layer=2)
         for b in range(2):
-            close(want[b * n:b * n + n], reference(p, b, q[b * n:b * n + n], masks[b], 1 / 8, 2), p.v.abs().max().item())
+            near(want[b * n:b * n + n], reference(p, b, q[b * n:b * n + n], masks[b], 1 / 8, 2), p.v.abs().max().item(), once(2 * n, 2, 2))
         for other in (wide[:, :4, 8:72], odd):
             assert torch.equal(call(other, dev(p.slots), starts, None, layer=2), want)
         assert torch.equal(call(q, dev(p.slots), starts, None, layer=2, k=both[:, :, :, 0], v=both[:, :, :, 1]), want)
@@ -428,6 +465,7 @@ def test_past_32_bits(paged):
     table[0] = dev(at)
     t = 5 * page - 3
     kk, vv = (torch.cat([x[i, 0, 0] for i in at])[:t, None].double() for x in (k, v))
+    whole = type("", (), {"kv": lambda self, b, layer: (kk, vv)})()
     for n in (1, 100):
         q = normal(g, n, 2, d)
         tree = random_tree(n, n)
@@ -436,8 +474,7 @@ def test_past_32_bits(paged):
              window_mask(n, t, 300, 9)),
             (paged.tree_attend(q, k, v, table, dev([t]), dev([0]), dev(tree), layer=0, q_starts=dev([0, n])), tree_mask(tree, t)),
         ):
-            for i in range(0, n, 13):
-                close(got[i], softmax_rows(q[i], kk, vv, seen[i], 1 / math.sqrt(d)), vv.abs().max().item())
+            near(got, reference(whole, 0, q, seen, 1 / math.sqrt(d), 0), vv.abs().max().item(), once(n, 2, 1))
 
 
 def test_refusals(paged):

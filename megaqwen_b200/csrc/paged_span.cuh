@@ -28,18 +28,19 @@
 namespace mq {
 namespace paged {
 
-constexpr int SPAN_THREADS = 640;   // warps: 0 K, 1 MMA, 2 Q and V, 3 looks through V, 4-11 softmax of A, 12-19 of B
+constexpr int SPAN_THREADS = 384;   // warps: 0 items and K, 1 MMA, 2 Q and V, 3 looks through V, 4-7 softmax of A, 8-11 of B
+constexpr int SPAN_ITEMS = 4;       // ring of items between the first warp and the others
 
 template <int D>
 struct SpanSmem {
     static constexpr int TILE = (D / 64) * PATOM;
     static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE, BAR = 6 * TILE;
-    static constexpr int RED = BAR + 256;                     // fp32 [2 streams][2 tiles][2 halves][128] row maxima
-    static constexpr int SUM = RED + 2 * 2 * 2 * 128 * 4;     // fp32 [2 streams][2 halves][128] row sums
-    static constexpr int TOP = SUM + 2 * 2 * 128 * 4;         // fp32 [2 streams][128] their reference
-    static constexpr int ODD = TOP + 2 * 128 * 4;             // [2 stages][128 keys][D / 8]: a bit for each value that is not finite
-    static constexpr int HIT = ODD + 2 * 128 * (D / 8);       // u64 [2 streams][2 halves][128]: channels in which a row met one
-    static constexpr int SCHED = HIT + 2 * 2 * 128 * 8;
+    static constexpr int ITEM = BAR + 512;                    // SpanSeg [SPAN_ITEMS]
+    static constexpr int SUM = ITEM + SPAN_ITEMS * 64;        // fp32 [2 streams][128] row sums
+    static constexpr int TOP = SUM + 2 * 128 * 4;             // fp32 [2 streams][128] their reference
+    static constexpr int HIT = TOP + 2 * 128 * 4;             // u64 [2 streams][128][2]: channels in which a row met a value that is not finite
+    static constexpr int ODD = HIT + 2 * 128 * 16;            // [2 stages][128 keys][D / 8]: a bit for each such value
+    static constexpr int SCHED = ODD + 2 * 128 * (D / 8);
     static constexpr size_t bytes(int B) { return SCHED + (size_t)(2 * B + 1) * 4 + 1024; }
 };
 
@@ -48,13 +49,14 @@ struct alignas(16) SpanCut {
     int tok0, h, rows, runs;   // rows 0: none
 };
 
-struct SpanSeg {
-    int b, h, tok0, rows;         // tok0: the tile's first token; rows: of this item
+struct alignas(16) SpanSeg {
+    int slot, h, tok0, rows;      // tok0: the tile's first token; rows: of this item
     int seq0, pf, pl;             // the sequence's first token; positions of the tile's first and last token
     int st, wt, ng;               // sink tiles, first window tile, tiles in all
-    int t0, n, runs;              // of this run; runs that share the item
+    int t0, n, runs;              // of this run (n 0: the run is over); runs that share the item
     bool two, both, start, whole;   // two: each stream has rows of its own; both: B works, too
 };
+static_assert(sizeof(SpanSeg) <= 64, "an item of the ring");
 
 // Tiles of a row tile whose tokens stand at pf .. pl: st of the sinks, then wt .. the one of pl.
 __device__ __forceinline__ int span_tiles(const RowArgs& a, int pf, int pl, int& st, int& wt) {
@@ -96,6 +98,40 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+// 128 consecutive columns of this warp's TMEM lanes, waited for.
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, float* v) {
+    uint32_t r[128];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x128.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
+        "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
+        "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
+        "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
+        "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
+          "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
+          "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
+          "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
+          "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
+          "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
+          "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
+          "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
+          "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
+}
 // Two fp32 values side by side.
 __device__ __forceinline__ uint64_t two_of(float a, float b) {
     uint64_t d;
@@ -134,7 +170,10 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     uint64_t* o_full = bars + 16;     // [2] the run's last PV is done
     uint64_t* q_empty = bars + 18;    // [2]
     uint64_t* drain = bars + 20;
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 21);
+    uint64_t* pair = bars + 21;       // [4] the warps of A and B on the same rows
+    uint64_t* item_full = bars + 25;  // [SPAN_ITEMS]
+    uint64_t* item_empty = item_full + SPAN_ITEMS;
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(item_empty + SPAN_ITEMS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
     volatile int* holes = abort_flag + 1;      // a page out of range has been met
     volatile int* odd_tile = abort_flag + 2;   // [2] stages: the tile holds values that are not finite
@@ -151,10 +190,15 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
             mbar_init(&v_empty[i], 1);
             mbar_init(&v_ready[i], 1);
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 8);
+            mbar_init(&p_full[i], 4);
             mbar_init(&o_full[i], 1);
         }
         mbar_init(drain, 1);
+        for (int i = 0; i < 4; ++i) mbar_init(&pair[i], 2);
+        for (int i = 0; i < SPAN_ITEMS; ++i) {
+            mbar_init(&item_full[i], 1);
+            mbar_init(&item_empty[i], NT / 32 - 1);
+        }
         *abort_flag = 0;
         *holes = 0;
         fence_mbar_init();
@@ -237,7 +281,7 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     const uint32_t x0 = min(blockIdx.x * quota, work), xe = min(x0 + quota, work);
 
     // The item at x and the tiles of it in this run (n <= 0: the run has only its own units); x moves past them.
-    // Called by whole warps.
+    // By the first warp.
     auto segment = [&](uint32_t& x) {
         SpanSeg e;
         const uint32_t xh = x / (uint32_t)a.hkv;
@@ -247,7 +291,7 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
             if (off[mid] <= xh) lo = mid;
             else hi = mid;
         }
-        e.b = lo;
+        e.slot = __ldg(a.slots + lo);
         const uint32_t one = off[lo + 1] - off[lo];
         uint32_t rel = x - off[lo] * a.hkv;
         e.h = (int)(rel / one);
@@ -316,6 +360,21 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         *abort_flag = 1;
         note_status(a.status, MQ_ERR_PIPE_TIMEOUT);
     };
+    // The other warps' items, in the order in which the first one leaves them; false at the end of the run.
+    SpanSeg* items = reinterpret_cast<SpanSeg*>(smem + L::ITEM);
+    auto item_at = [&](int i) -> SpanSeg& { return *reinterpret_cast<SpanSeg*>(reinterpret_cast<uint8_t*>(items) + (i % SPAN_ITEMS) * 64); };
+    int taken = 0;
+    auto take = [&](SpanSeg& e, bool& ok) {
+        ok = ok && __all_sync(0xffffffffu, wait(&item_full[taken % SPAN_ITEMS], (taken / SPAN_ITEMS) & 1));
+        if (!ok) return false;
+        e = item_at(taken);
+        return e.n > 0;
+    };
+    auto done_with = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[taken % SPAN_ITEMS]);
+        ++taken;
+    };
 
     if (warp == 0 || warp == 2) {
         // ---- K and V producers: lane c loads the tile's c-th page.  That of V also loads the items' Q, a box of whole
@@ -338,14 +397,28 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
             }
             return true;
         };
-        for (uint32_t x = x0; ok && x < xe;) {
-            const SpanSeg e = segment(x);
-            if (e.n <= 0) continue;
-            if (warp == 0 && e.start && !e.whole) {   // (the run's last item)
-                if (lane == 0) *reinterpret_cast<int4*>(cuts + blockIdx.x) = make_int4(e.tok0, e.h, e.rows, e.runs);
-                cut = true;
-            }
-            if (warp == 2) {
+        uint32_t x = x0;
+        SpanSeg e;
+        while (ok) {
+            if (warp == 0) {
+                e.n = 0;
+                while (x < xe && e.n <= 0) e = segment(x);
+                if (taken >= SPAN_ITEMS)
+                    ok = __all_sync(0xffffffffu, wait(&item_empty[taken % SPAN_ITEMS], (taken / SPAN_ITEMS - 1) & 1));
+                if (!ok) break;
+                if (lane == 0) {
+                    item_at(taken) = e;
+                    mbar_arrive(&item_full[taken % SPAN_ITEMS]);
+                }
+                ++taken;
+                if (e.n <= 0) break;
+                if (e.start && !e.whole) {   // (the run's last item)
+                    if (lane == 0) *reinterpret_cast<int4*>(cuts + blockIdx.x) = make_int4(e.tok0, e.h, e.rows, e.runs);
+                    cut = true;
+                }
+            } else {
+                if (!take(e, ok)) break;
+                done_with();
                 ok = load_q(e, 0, nq0++);
                 if (ok && e.both) ok = load_q(e, 1, nq1++);
                 if (!__all_sync(0xffffffffu, ok)) {
@@ -353,7 +426,7 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                     break;
                 }
             }
-            const int* row = a.table + __ldg(a.slots + e.b) * a.table_row;
+            const int* row = a.table + e.slot * a.table_row;
             // what no row sees is read as zeros, from outside the map
             auto look = [&](int j) {
                 const int at = tile_at(e, j) + lane * page;
@@ -402,8 +475,7 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         // ---- looks through the values of masked tiles ----
         int c = 0;
         bool ok = true;
-        for (uint32_t x = x0; ok && x < xe;) {
-            const SpanSeg e = segment(x);
+        for (SpanSeg e; take(e, ok); done_with()) {
             for (int j = 0; j < e.n; ++j, ++c) {
                 const int st = c & 1;
                 ok = __all_sync(0xffffffffu, wait(&v_full[st], (c >> 1) & 1));
@@ -471,17 +543,14 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
             const uint32_t sv = base + L::V + (vc & 1) * TILE, o = 256 + q * 128;
 #pragma unroll
             for (int k = 0; k < PK / 16; ++k) {
-                // 16 keys: 8 columns, those of a half in its own 64
-                const uint32_t p = q * 128 + 64 * (k >> 2) + 8 * (k & 3);
+                const uint32_t p = q * 128 + 8 * k;   // 16 keys: 8 columns
                 tc_mma_f16_ts(o, p, sw128_mnmajor_desc(sv + k * 2048), id_o, !first || k);
             }
             if (last_use) tc_commit(&v_empty[vc & 1]);
             if (done) tc_commit(&o_full[q]);
         };
-        for (uint32_t x = x0; ok && x < xe;) {
-            const SpanSeg e = segment(x);
+        for (SpanSeg e; take(e, ok); done_with()) {
             const int n = uniform(e.n);
-            if (n <= 0) continue;
             const bool two = uniform(e.two);
             const int steps = two ? 2 * n : n;
             // step i: the stream's PV of its tile before (step i - 2), then its S of this one.  What the
@@ -517,86 +586,74 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         while (!mbar_try_wait(drain, 0) && clock64() - t0 < WAIT_CYCLES) {
         }
     } else {
-        // ---- softmax of stream q, column half hh: two threads to a row ----
-        const int q = (warp - 4) >> 3, hh = ((warp - 4) >> 2) & 1;
-        const int quad = warp & 3;                     // the TMEM lanes this warp may touch
+        // ---- softmax of stream q: a thread to a row ----
+        const int q = (warp - 4) >> 2, quad = warp & 3;   // quad: the TMEM lanes this warp may touch
         const int r = quad * 32 + lane;
         // a scale of zero: a masked score of minus infinity stays one
         const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);
         const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
-        const uint32_t sa = tmem + lane_off + q * 128 + hh * 64, oa = tmem + lane_off + 256;   // O of A, that of B 128 columns on
-        float* red = reinterpret_cast<float*>(smem + L::RED) + q * 512;
-        float* sums = reinterpret_cast<float*>(smem + L::SUM);                       // [stream][half][128]
-        float* tops = reinterpret_cast<float*>(smem + L::TOP);                       // [stream][128]
-        unsigned long long* hits = reinterpret_cast<unsigned long long*>(smem + L::HIT);   // [stream][half][128]
+        const uint32_t sa = tmem + lane_off + q * 128, oa = tmem + lane_off + 256;   // O of A, that of B 128 columns on
+        float* sums = reinterpret_cast<float*>(smem + L::SUM);   // [stream][128]
+        float* tops = reinterpret_cast<float*>(smem + L::TOP);
+        ulonglong2* hits = reinterpret_cast<ulonglong2*>(smem + L::HIT);
         constexpr float GROW = 8.f;
-        // the two warps of a row meet at a barrier of their own, the four of both streams at another; one whose wait
-        // failed goes on to the end without waiting, so that its partners never stand alone
-        auto meet = [&]() { named_bar_sync(1 + q * 4 + quad, 64); };
-        auto meet4 = [&]() { named_bar_sync(9 + quad, 128); };
-        int ns = 0, nv = 0, no0 = 0, no1 = 0;   // scores taken, tiles of the segments before, results of A and B
+        int ns = 0, nv = 0, no0 = 0, no1 = 0, np = 0;   // scores taken, tiles of the items before, results of A and B, meetings
         bool ok = true;
         auto got = [&](uint64_t* bar, uint32_t parity) {
             if (ok) ok = __all_sync(0xffffffffu, wait(bar, parity));
             return ok;
         };
-        const int tok_r = r / grp, head_r = r - tok_r * grp;   // of this row in its stream
-        SpanSeg next;
-        uint32_t x = x0;
-        next.n = 0;
-        // the next item with tiles, looked up while the last results of the one before are on their way
-        auto advance = [&]() {
-            next.n = 0;
-            while (x < xe && next.n <= 0) next = segment(x);
+        auto meet = [&]() {   // with the other stream's warp on the same rows
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pair[quad]);
+            got(&pair[quad], np++ & 1);
         };
-        advance();
-        while (next.n > 0) {
-            const SpanSeg e = next;
+        const int tok_r = r / grp, head_r = r - tok_r * grp;   // of this row in its stream
+        for (SpanSeg e; take(e, ok); done_with()) {
             const int mine = e.two ? e.n : (e.n + 1 - q) >> 1;   // this stream's tiles
             const int tok = (e.two ? q * tps : 0) + tok_r;       // the row's token in the item
             const bool there = tok_r < tps && tok * grp < e.rows;
             const int pos = min(e.pf + tok, e.pl), node = e.tok0 - e.seq0 + pos - e.pf;
-            unsigned long long hit = 0;
+            unsigned long long hit[2] = {0, 0};
             float m = -INFINITY, l = 0.f;
+#pragma unroll 1
             for (int j = 0; j < mine; ++j, ++ns) {
-                float tmax = -INFINITY;
                 const int jt = e.two ? j : 2 * j + q, at = tile_at(e, jt);
                 const bool masked = !all_seen(e, at);
-                unsigned long long live = ~0ull;   // keys of this half that the row sees
-                if (masked) live = span_sees(a, pos, at + hh * 64, node, e.seq0);
-                if (got(&s_full[q], ns & 1)) {
-                    tc_fence_after();
-                    if (*holes) {   // pages out of range: their keys are left out
-                        const int* row = a.table + __ldg(a.slots + e.b) * a.table_row;
-                        for (int k = 0; k < 64; k += min(page, 64)) {
-                            const int p = (at + hh * 64 + k) & -page;
-                            const int pid = in_sight(e, p) ? __ldg(row + (p >> a.pool.shift)) : 0;
-                            if (pid < 0 || pid >= a.pool.pages) live &= ~((page >= 64 ? ~0ull : (1ull << page) - 1ull) << k);
-                        }
-                    }
-                    // two passes over S in TMEM: the registers do not hold it and the weights
-                    float sv[64], mx[4];
-                    tmem_ld64(sa, sv);
-                    if (__any_sync(0xffffffffu, live != ~0ull)) {
-                        const uint32_t lo = (uint32_t)live, hi = (uint32_t)(live >> 32);
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            sv[k] = lo >> k & 1u ? sv[k] : -INFINITY;
-                            sv[32 + k] = hi >> k & 1u ? sv[32 + k] : -INFINITY;
-                        }
-                        tmem_st32(sa, sv);
-                        tmem_st32(sa + 32, sv + 32);
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) mx[k] = fmaxf(sv[2 * k], sv[2 * k + 1]);
-#pragma unroll
-                    for (int k = 8; k < 64; k += 2) mx[(k >> 1) & 3] = max3(mx[(k >> 1) & 3], sv[k], sv[k + 1]);
-                    tmax = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale;
+                unsigned long long live[2] = {~0ull, ~0ull};   // keys that the row sees
+                if (masked) {
+                    live[0] = span_sees(a, pos, at, node, e.seq0);
+                    live[1] = span_sees(a, pos, at + 64, node, e.seq0);
                 }
-                red[((j & 1) * 2 + hh) * 128 + r] = tmax;
-                meet();
-                if (!ok) continue;
-                tmax = fmaxf(tmax, red[((j & 1) * 2 + (hh ^ 1)) * 128 + r]);
+                if (!got(&s_full[q], ns & 1)) break;
+                tc_fence_after();
+                if (*holes) {   // pages out of range: their keys are left out
+                    const int* row = a.table + e.slot * a.table_row;
+                    for (int k = 0; k < PK; k += min(page, 64)) {
+                        const int p = (at + k) & -page;
+                        const int pid = in_sight(e, p) ? __ldg(row + (p >> a.pool.shift)) : 0;
+                        if (pid < 0 || pid >= a.pool.pages) {
+                            const unsigned long long gone = ~((page >= 64 ? ~0ull : (1ull << page) - 1ull) << (k & 63));
+                            if (k < 64) live[0] &= gone;
+                            else live[1] &= gone;
+                        }
+                    }
+                }
+                float sv[128], mx[4];
+                tmem_ld128(sa, sv);
+                if (__any_sync(0xffffffffu, (live[0] & live[1]) != ~0ull)) {
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t b = (uint32_t)(live[w >> 1] >> (32 * (w & 1)));
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) sv[32 * w + k] = b >> k & 1u ? sv[32 * w + k] : -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mx[k] = fmaxf(sv[2 * k], sv[2 * k + 1]);
+#pragma unroll
+                for (int k = 8; k < 128; k += 2) mx[(k >> 1) & 3] = max3(mx[(k >> 1) & 3], sv[k], sv[k + 1]);
+                const float tmax = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale;
                 // a row's maximum moves only when it grew by more than 2^8; weights stay below 256
                 float corr = 1.f;
                 if (tmax > m + GROW) {
@@ -605,27 +662,25 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                 }
                 l *= corr;
                 if (j && __any_sync(0xffffffffu, corr != 1.f)) {
-                    // s_full covers the PV before it, so O is at rest; half its columns each
+                    // s_full covers the PV before it, so O is at rest
 #pragma unroll 1
-                    for (int i = 0; i < D / 2; i += 16) {
+                    for (int i = 0; i < D; i += 16) {
                         float v[16];
-                        tmem_ld16(oa + q * 128 + hh * (D / 2) + i, v);
+                        tmem_ld16(oa + q * 128 + i, v);
 #pragma unroll
                         for (int k = 0; k < 16; ++k) v[k] *= corr;
-                        tmem_st16(oa + q * 128 + hh * (D / 2) + i, v);
+                        tmem_st16(oa + q * 128 + i, v);
                     }
                 }
                 const uint64_t scale2 = two_of(scale, scale), u2 = m == -INFINITY ? 0ull : two_of(-m, -m);
                 uint64_t sum0 = 0ull, sum1 = 0ull;
 #pragma unroll
-                for (int i = 0; i < 64; i += 32) {
-                    float sv[32];
-                    uint32_t pk[16];   // 32 weights in 16 columns
-                    tmem_ld32(sa + i, sv);
+                for (int i = 0; i < 128; i += 32) {
+                    uint32_t pk[16];   // 32 weights in 16 columns, over the scores
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                         float p0, p1;
-                        halves(fma2(two_of(sv[2 * k], sv[2 * k + 1]), scale2, u2), p0, p1);
+                        halves(fma2(two_of(sv[i + 2 * k], sv[i + 2 * k + 1]), scale2, u2), p0, p1);
                         p0 = ex2(p0);
                         p1 = ex2(p1);
                         (k & 1 ? sum1 : sum0) = add2(k & 1 ? sum1 : sum0, two_of(p0, p1));
@@ -640,17 +695,12 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                     // the tile's values are looked through, and stay until this stream's weights are used
                     const int c = nv + jt, st = c & 1;
                     if (got(&v_ready[st], (c >> 1) & 1) && odd_tile[st]) {
-                        const uint8_t* bits = smem + L::ODD + st * 128 * (D / 8) + hh * (D / 16);
+                        const uint8_t* bits = smem + L::ODD + st * 128 * (D / 8);
 #pragma unroll 1
-                        for (int k0 = 0; k0 < PK; k0 += 64) {
-                            const unsigned long long seen = span_sees(a, pos, at + k0, node, e.seq0);
-#pragma unroll 1
-                            for (int k = 0; k < 64; ++k) {
-                                unsigned long long w;
-                                if (D == 128) w = *reinterpret_cast<const unsigned long long*>(bits + (k0 + k) * (D / 8));
-                                else w = *reinterpret_cast<const uint32_t*>(bits + (k0 + k) * (D / 8));
-                                if (seen >> k & 1ull) hit |= w;
-                            }
+                        for (int k = 0; k < PK; ++k) {
+                            if (!((k < 64 ? live[0] : live[1]) >> (k & 63) & 1ull)) continue;
+                            hit[0] |= *reinterpret_cast<const unsigned long long*>(bits + k * (D / 8));
+                            if (D == 128) hit[1] |= *reinterpret_cast<const unsigned long long*>(bits + k * (D / 8) + 8 * (D / 128));
                         }
                     }
                 }
@@ -660,69 +710,84 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                 if (lane == 0) mbar_arrive(&p_full[q]);
             }
             nv += e.n;
-            advance();
             // ---- the item's rows: what A and B have of them, when they share them ----
             if (!e.two || q == 0) got(&o_full[0], no0 & 1);
             if (e.two ? q == 1 : e.both) got(&o_full[1], no1 & 1);
             ++no0;
             no1 += e.both;
             tc_fence_after();
-            sums[(q * 2 + hh) * 128 + r] = l;
             float e0 = 1.f, e1 = 1.f;   // weights of A's and B's accumulators
-            if (e.two) {
+            if (!e.two) {
+                sums[q * 128 + r] = l;
+                tops[q * 128 + r] = m;
+                hits[q * 128 + r] = make_ulonglong2(hit[0], hit[1]);
                 meet();
-                l += sums[(q * 2 + (hh ^ 1)) * 128 + r];
-            } else {
-                if (hh == 0) tops[q * 128 + r] = m;
-                hits[(q * 2 + hh) * 128 + r] = hit;
-                meet4();
                 const float ma = tops[r], mb = tops[128 + r];   // (B's is -inf when it had no tile)
                 m = fmaxf(ma, mb);
                 const float u = m == -INFINITY ? 0.f : m;
                 e0 = ex2(ma - u);
                 e1 = ex2(mb - u);
-                l = (sums[r] + sums[128 + r]) * e0 + (sums[256 + r] + sums[384 + r]) * e1;
-                hit = hits[hh * 128 + r] | hits[(2 + hh) * 128 + r];
+                l = sums[r] * e0 + sums[128 + r] * e1;
+                const ulonglong2 h0 = hits[r], h1 = hits[128 + r];
+                hit[0] = h0.x | h1.x;
+                hit[1] = h0.y | h1.y;
             }
             const float inv = l != 0.f ? 1.f / l : 0.f;   // a row that sees nothing is zero (NaN stays NaN)
-            // this thread's columns: its half, or with two streams on a row half of that
-            const int width = e.two ? D / 2 : D / 4, c_lo = hh * (D / 2) + (e.two ? 0 : q * (D / 4));
-            float* part = a.ws.pfx_slots + ((2ll * blockIdx.x + e.start) * PROWS + tok * grp + head_r) * LD;
-            uint16_t* out = a.out + ((long long)(e.tok0 + tok) * a.hq + e.h * grp + head_r) * D;
-            if (!e.whole && ok && there && hh == 0 && (e.two || q == 0))
-                *reinterpret_cast<float4*>(part) = make_float4(m, l, 0.f, 0.f);
+            // this thread's columns: the row's, or with two streams on it half of them
+            const int c_lo = e.two ? 0 : q * (D / 2), c_hi = e.two ? D : c_lo + D / 2;
+            float* part = there ? a.ws.pfx_slots + ((2ll * blockIdx.x + e.start) * PROWS + tok * grp + head_r) * LD : nullptr;
+            uint16_t* out = there ? a.out + ((long long)(e.tok0 + tok) * a.hq + e.h * grp + head_r) * D : nullptr;
+            if (!e.whole && ok && there && (e.two || q == 0)) *reinterpret_cast<float4*>(part) = make_float4(m, l, 0.f, 0.f);
 #pragma unroll 1
-            for (int i = 0; ok && i < width; i += 16) {
-                const int c = c_lo + i;
-                float v[16];
-                tmem_ld16(oa + (e.two ? q * 128 : 0) + c, v);
+            for (int c = c_lo; ok && c < c_hi; c += 32) {
+                float v[32];
+                tmem_ld32(oa + (e.two ? q * 128 : 0) + c, v);
                 if (!e.two) {
-                    float w[16];
-                    if (e.both) tmem_ld16(oa + 128 + c, w);
+                    float w[32];
+                    if (e.both) tmem_ld32(oa + 128 + c, w);
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) v[k] = e.both ? v[k] * e0 + w[k] * e1 : v[k] * e0;
+                    for (int k = 0; k < 32; ++k) v[k] = e.both ? v[k] * e0 + w[k] * e1 : v[k] * e0;
                 }
-                const uint32_t odd = (uint32_t)(hit >> (c - hh * (D / 2))) & 0xffffu;
+                const uint32_t odd = (uint32_t)(hit[c >> 6] >> (c & 63));
                 if (odd) {
 #pragma unroll
-                    for (int k = 0; k < 16; ++k)
+                    for (int k = 0; k < 32; ++k)
                         if (odd >> k & 1u) v[k] = NAN;
                 }
-                if (!there) continue;
-                if (e.whole) {
+                if (!e.whole) {
+                    if (there) {
 #pragma unroll
-                    for (int k = 0; k < 16; k += 8)
-                        *reinterpret_cast<uint4*>(out + c + k) =
-                            make_uint4(Elem<T>::pack(v[k] * inv, v[k + 1] * inv), Elem<T>::pack(v[k + 2] * inv, v[k + 3] * inv),
-                                       Elem<T>::pack(v[k + 4] * inv, v[k + 5] * inv), Elem<T>::pack(v[k + 6] * inv, v[k + 7] * inv));
-                } else {
+                        for (int k = 0; k < 32; k += 4)
+                            *reinterpret_cast<float4*>(part + 4 + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                    }
+                    continue;
+                }
+                // four pieces of 16 bytes; four lanes turn theirs into whole 64 bytes of their four rows, so that a
+                // store touches eight rows and not 32
+                uint32_t w[4][4];
 #pragma unroll
-                    for (int k = 0; k < 16; k += 4)
-                        *reinterpret_cast<float4*>(part + 4 + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                for (int k = 0; k < 16; ++k) w[k >> 2][k & 3] = Elem<T>::pack(v[2 * k] * inv, v[2 * k + 1] * inv);
+#pragma unroll
+                for (int x = 1; x < 4; x <<= 1) {
+                    const bool high = lane & x;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (i & x) continue;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t other = __shfl_xor_sync(0xffffffffu, high ? w[i][k] : w[i | x][k], x);
+                            (high ? w[i][k] : w[i | x][k]) = other;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint16_t* to = from_lane(out, (lane & ~3) + k);
+                    if (to) *reinterpret_cast<uint4*>(to + c + (lane & 3) * 8) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
                 }
             }
             tc_fence_before();
-            if (!e.two) meet4();   // both accumulators are read
+            if (!e.two) meet();   // both accumulators are read
         }
         if (!ok && lane == 0) give_up();
     }

@@ -6,11 +6,15 @@
 // Items lie end to end on a line that is cut into equal runs, one per CTA (one
 // CTA per SM), each item as long as it has tiles.
 //
-// A CTA runs two streams, A and B, as the shared-prefix kernel does
-// (paged_prefix.cuh): with more than 128 rows each has half of them and every tile
-// is used by both; with up to 128 rows both take the same ones, A the even tiles
-// and B the odd, and their two accumulators, side by side in TMEM, are joined when
-// the item ends.  Weights go into the second product as two 16-bit pieces.
+// A CTA runs two streams, A and B, each with its own rows of Q, two buffers for the
+// scores of 64 keys (weights overwrite their scores as 16-bit values) and its own
+// accumulator in TMEM.  With more than 128 rows each has half of them and takes both
+// halves of every tile; with up to 128 both take the same rows, A the first half of
+// each tile and B the second, and the accumulators, side by side in TMEM, are joined
+// when the item ends.  The tensor core is two steps of scores ahead of a stream's
+// softmax: PV_A(i), S_A(i + 2) | PV_B(i), S_B(i + 2) | ...  (With one buffer of 128
+// keys a stream's softmax waited for its own PV and S: 5.0k cycles for a tile of both
+// streams, in which the tensor core was busy for 2.6k.)
 //
 // Masks: a tile that some row does not see whole has its scores set to minus
 // infinity in TMEM by two cuts (windowed) or by the node's ancestors (a tree),
@@ -28,7 +32,8 @@
 namespace mq {
 namespace paged {
 
-constexpr int SPAN_THREADS = 384;   // warps: 0 items and K, 1 MMA, 2 Q and V, 3 looks through V, 4-7 softmax of A, 8-11 of B
+constexpr int SPAN_THREADS = 384;   // warps: 0 items and K, 1 MMA of A, 2 Q and V (loads, and looks through V), 3 MMA of B, 4-7 softmax of A, 8-11 of B
+constexpr int HK = 64;              // keys to a step of a stream
 constexpr int SPAN_ITEMS = 4;       // ring of items between the first warp and the others
 
 template <int D>
@@ -54,7 +59,7 @@ struct alignas(16) SpanSeg {
     int seq0, pf, pl;             // the sequence's first token; positions of the tile's first and last token
     int st, wt, ng;               // sink tiles, first window tile, tiles in all
     int t0, n, runs;              // of this run (n 0: the run is over); runs that share the item
-    bool two, both, start, whole;   // two: each stream has rows of its own; both: B works, too
+    bool two, start, whole;       // two: each stream has rows of its own
 };
 static_assert(sizeof(SpanSeg) <= 64, "an item of the ring");
 
@@ -93,44 +98,44 @@ __device__ __forceinline__ void tma_load_heads(uint32_t dst, const CUtensorMap* 
         ::"r"(dst), "l"(map), "r"(0), "r"(block), "r"(head), "r"(token), "r"(bar)
         : "memory");
 }
+// Operands in the 128-byte swizzle layout as sw128_kmajor_desc and sw128_mnmajor_desc have them: low word (address and
+// leading offset, in units of 16 bytes) and the high word that is alike for both.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t leading) { return ((addr >> 4) & 0x3fffu) | leading << 16; }
+constexpr uint32_t DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+        ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"((uint32_t)add), "n"(DESC_HI)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+        "mov.b64 b, {%2, %5};\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"((uint32_t)add), "n"(DESC_HI)
+        : "memory");
+}
+// As mbar_try_wait, but answers at once (try_wait may hold the thread for some microseconds).
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
-}
-// 128 consecutive columns of this warp's TMEM lanes, waited for.
-__device__ __forceinline__ void tmem_ld128(uint32_t taddr, float* v) {
-    uint32_t r[128];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x128.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
-        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
-        "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
-        "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
-        "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
-        "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
-          "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
-          "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
-          "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
-          "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
-          "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
-          "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
-          "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
-          "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
-        : "r"(taddr));
-#pragma unroll
-    for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
 }
 // Two fp32 values side by side.
 __device__ __forceinline__ uint64_t two_of(float a, float b) {
@@ -165,13 +170,13 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     uint64_t* v_full = bars + 6;
     uint64_t* v_empty = bars + 8;
     uint64_t* v_ready = bars + 10;    // [2] stages: looked through
-    uint64_t* s_full = bars + 12;     // [2] streams: S is there (and every MMA issued before it is done)
-    uint64_t* p_full = bars + 14;     // [2] P is stored, O is rescaled
-    uint64_t* o_full = bars + 16;     // [2] the run's last PV is done
-    uint64_t* q_empty = bars + 18;    // [2]
-    uint64_t* drain = bars + 20;
-    uint64_t* pair = bars + 21;       // [4] the warps of A and B on the same rows
-    uint64_t* item_full = bars + 25;  // [SPAN_ITEMS]
+    uint64_t* s_full = bars + 12;     // [2 streams][2 buffers] scores are there
+    uint64_t* p_full = bars + 16;     // [2][2] weights are stored, O is rescaled
+    uint64_t* o_full = bars + 20;     // [2] the PV of an item's last step but one is done, and that of the last
+    uint64_t* q_empty = bars + 22;    // [2]
+    uint64_t* drain = bars + 24;
+    uint64_t* pair = bars + 25;       // [4] the warps of A and B on the same rows
+    uint64_t* item_full = bars + 29;  // [SPAN_ITEMS]
     uint64_t* item_empty = item_full + SPAN_ITEMS;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(item_empty + SPAN_ITEMS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
@@ -185,15 +190,17 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
             mbar_init(&q_full[i], 1);
             mbar_init(&q_empty[i], 1);
             mbar_init(&k_full[i], 1);
-            mbar_init(&k_empty[i], 1);
+            mbar_init(&k_empty[i], 2);
             mbar_init(&v_full[i], 1);
-            mbar_init(&v_empty[i], 1);
+            mbar_init(&v_empty[i], 2);
             mbar_init(&v_ready[i], 1);
-            mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
+            mbar_init(&s_full[2 * i], 1);
+            mbar_init(&s_full[2 * i + 1], 1);
+            mbar_init(&p_full[2 * i], 4);
+            mbar_init(&p_full[2 * i + 1], 4);
             mbar_init(&o_full[i], 1);
         }
-        mbar_init(drain, 1);
+        mbar_init(drain, 2);
         for (int i = 0; i < 4; ++i) mbar_init(&pair[i], 2);
         for (int i = 0; i < SPAN_ITEMS; ++i) {
             mbar_init(&item_full[i], 1);
@@ -280,10 +287,18 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     const uint32_t work = in_order ? off[a.B] * a.hkv : 0, quota = quota_of(work, gridDim.x);
     const uint32_t x0 = min(blockIdx.x * quota, work), xe = min(x0 + quota, work);
 
-    // The item at x and the tiles of it in this run (n <= 0: the run has only its own units); x moves past them.
-    // By the first warp.
-    auto segment = [&](uint32_t& x) {
-        SpanSeg e;
+    // The run's items in order, by the first warp: the first one is looked up, the others follow it.
+    int it_b = 0, it_h = 0, it_i = 0, it_ql = 0, it_p0 = 0;   // sequence, head, the row tile's first token; of the sequence
+    uint32_t x = x0;
+    SpanSeg cur;
+    auto open = [&](int b) {
+        it_b = b;
+        cur.slot = __ldg(a.slots + b);
+        cur.seq0 = q_start(a, b);
+        it_ql = q_start(a, b + 1) - cur.seq0;
+        it_p0 = lens[b] - it_ql;
+    };
+    auto locate = [&]() -> int {   // units of the item before x
         const uint32_t xh = x / (uint32_t)a.hkv;
         int lo = 0, hi = a.B;   // the last sequence that starts at or before, of those with work
         while (hi - lo > 1) {
@@ -291,17 +306,15 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
             if (off[mid] <= xh) lo = mid;
             else hi = mid;
         }
-        e.slot = __ldg(a.slots + lo);
+        open(lo);
         const uint32_t one = off[lo + 1] - off[lo];
         uint32_t rel = x - off[lo] * a.hkv;
-        e.h = (int)(rel / one);
-        rel -= e.h * one;
-        e.seq0 = q_start(a, lo);
-        const int ql = q_start(a, lo + 1) - e.seq0, p0 = lens[lo] - ql;
+        it_h = (int)(rel / one);
+        rel -= it_h * one;
         for (int i0 = 0;; i0 += 32) {   // the row tile, 32 at a time
             const int i = (i0 + lane) * tpt;
             int st, wt, n = 0;
-            if (i < ql) n = span_tiles(a, p0 + i, p0 + min(i + tpt, ql) - 1, st, wt);
+            if (i < it_ql) n = span_tiles(a, it_p0 + i, it_p0 + min(i + tpt, it_ql) - 1, st, wt);
             const uint32_t cost = n ? n + ITEM_UNITS : 0;
             uint32_t sum = cost;
 #pragma unroll
@@ -310,46 +323,72 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                 if (lane >= o) sum += y;
             }
             const unsigned found = __ballot_sync(0xffffffffu, rel < sum);
-            if (!found && (i0 + 32) * tpt < ql) {
+            if (!found && (i0 + 32) * tpt < it_ql) {
                 rel -= __shfl_sync(0xffffffffu, sum, 31);
                 continue;
             }
             const int at = found ? __ffs((int)found) - 1 : 0;   // (always found: x is within the sequence)
             rel -= __shfl_sync(0xffffffffu, sum - cost, at);
-            const int first = (i0 + at) * tpt, last = min(first + tpt, ql) - 1;
-            e.tok0 = e.seq0 + first;
-            e.rows = (last - first + 1) * grp;
-            e.pf = p0 + first;
-            e.pl = p0 + last;
-            break;
+            it_i = (i0 + at) * tpt;
+            return (int)rel;
         }
-        e.ng = span_tiles(a, e.pf, e.pl, e.st, e.wt);
-        const int pos = (int)rel, left = (int)min((uint32_t)(e.ng + ITEM_UNITS - pos), xe - x);
-        e.t0 = max(pos - ITEM_UNITS, 0);
-        e.n = max(pos + left - ITEM_UNITS, 0) - e.t0;
-        e.two = e.rows > tps * grp;
-        e.both = e.two || e.n > 1;
-        e.start = e.t0 == 0;
-        e.whole = e.n == e.ng;
-        const uint32_t ps = x - pos + ITEM_UNITS;   // the item's first tile on the line
-        e.runs = (int)((ps + e.ng - 1) / quota - ps / quota) + 1;
-        x += left;
-        return e;
+    };
+    auto follow = [&]() {   // to the next row tile, head or sequence; x is on the line's work
+        it_i += tpt;
+        if (it_i < it_ql) return;
+        it_i = 0;
+        if (++it_h < a.hkv) return;
+        it_h = 0;
+        int b = it_b + 1;
+        while (off[b + 1] == off[b]) ++b;
+        open(b);
+    };
+    // The next item with tiles in this run, into cur; n = 0 at the run's end.
+    bool placed = false;
+    auto next_item = [&]() {
+        cur.n = 0;
+        while (x < xe && cur.n <= 0) {
+            int pos = 0;
+            if (!placed) pos = locate();
+            else follow();
+            placed = true;
+            const int last = min(it_i + tpt, it_ql) - 1;
+            cur.h = it_h;
+            cur.tok0 = cur.seq0 + it_i;
+            cur.rows = (last - it_i + 1) * grp;
+            cur.pf = it_p0 + it_i;
+            cur.pl = it_p0 + last;
+            cur.ng = span_tiles(a, cur.pf, cur.pl, cur.st, cur.wt);
+            if (!cur.ng) continue;   // (before the first position)
+            const int left = (int)min((uint32_t)(cur.ng + ITEM_UNITS - pos), xe - x);
+            cur.t0 = max(pos - ITEM_UNITS, 0);
+            cur.n = max(pos + left - ITEM_UNITS, 0) - cur.t0;
+            cur.two = cur.rows > tps * grp;
+            cur.start = cur.t0 == 0;
+            cur.whole = cur.n == cur.ng;
+            cur.runs = 1;
+            if (!cur.whole) {
+                const uint32_t ps = x - pos + ITEM_UNITS;   // the item's first tile on the line
+                cur.runs = (int)((ps + cur.ng - 1) / quota - ps / quota) + 1;
+            }
+            x += left;
+        }
     };
     auto tile_at = [&](const SpanSeg& e, int j) {   // first position of the run's j-th tile
         const int t = e.t0 + j;
         return (t < e.st ? t : e.wt + t - e.st) * PK;
     };
-    // Every row sees all of the tile at `at`.
-    auto all_seen = [&](const SpanSeg& e, int at) {
-        if (a.parents) return at + PK <= e.seq0 - e.tok0 + e.pf;
-        return at + PK - 1 <= e.pf && (at > e.pl - a.window || at + PK <= a.sinks);
+    // Every row sees all of the n keys at `at`.
+    auto all_seen = [&](const SpanSeg& e, int at, int n) {
+        if (a.parents) return at + n <= e.seq0 - e.tok0 + e.pf;
+        return at + n - 1 <= e.pf && (at > e.pl - a.window || at + n <= a.sinks);
     };
     // Some row sees a position of the page at `at`: other pages' entries in the table are not looked at.
     auto in_sight = [&](const SpanSeg& e, int at) {
         return at <= e.pl && (a.parents || at < a.sinks || at + page > e.pf - a.window + 1);
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        if (mbar_try_wait(bar, parity)) return true;
         const long long t0 = clock64();
         while (!mbar_try_wait(bar, parity)) {
             if (*abort_flag || clock64() - t0 > WAIT_CYCLES) return false;
@@ -376,208 +415,219 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         ++taken;
     };
 
-    if (warp == 0 || warp == 2) {
-        // ---- K and V producers: lane c loads the tile's c-th page.  That of V also loads the items' Q, a box of whole
-        // tokens for each stream, once the last scores of the item before are there ----
-        uint64_t* full = warp == 0 ? k_full : v_full;
-        uint64_t* empty = warp == 0 ? k_empty : v_empty;
-        const CUtensorMap* map = warp == 0 ? &tmK : &tmV;
-        uint8_t* ring = smem + (warp == 0 ? L::K : L::V);
-        const int chunks = PK / page;
-        int c = 0, nq0 = 0, nq1 = 0;   // tiles so far, Q tiles of A and B
-        bool ok = true, cut = false;
-        auto load_q = [&](const SpanSeg& e, int q, int used) {
-            if (used && !wait(&q_empty[q], (used - 1) & 1)) return false;
-            if (lane == 0) {
-                mbar_arrive_expect_tx(&q_full[q], (D / 64) * tps * grp * 128);
+    // copies in flight land before the CTA may end, whatever became of their readers
+    auto land = [&](uint64_t* bar, uint32_t parity) {
+        const long long t0 = clock64();
+        while (!mbar_try_wait(bar, parity) && clock64() - t0 < WAIT_CYCLES) {
+        }
+    };
+    // Page `c` of a tile for lane c: what no row sees is read as zeros, from outside the map.
+    const int chunks = PK / page;
+    auto look = [&](const SpanSeg& e, int j) {
+        const int at = tile_at(e, j) + lane * page;
+        if (lane >= chunks || !in_sight(e, at)) return a.pool.pages;
+        return __ldg(a.table + e.slot * a.table_row + (at >> a.pool.shift));
+    };
+    auto load_tile = [&](const SpanSeg& e, int j, int pid, const CUtensorMap* map, uint8_t* to, uint64_t* full) {
+        if (pid < 0 || pid >= a.pool.pages) {
+            if (lane < chunks && in_sight(e, tile_at(e, j) + lane * page)) {
+                note_status(a.status, MQ_ERR_BAD_PAGE);
+                *holes = 1;   // before the tile's scores are there
+            }
+            pid = a.pool.pages;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(full, TILE);
+        __syncwarp();
+        if (lane < chunks) {
 #pragma unroll
-                for (int i = 0; i < D / 64; ++i)
-                    tma_load_heads(smem_u32(smem + L::Q + q * TILE + i * PATOM), &tmQ, i, e.h * grp,
-                                   e.tok0 + (e.two ? q * tps : 0), smem_u32(&q_full[q]));
-            }
-            return true;
-        };
-        uint32_t x = x0;
-        SpanSeg e;
+            for (int i = 0; i < D / 64; ++i)
+                tma_load_page(smem_u32(to + i * PATOM + lane * page * 128), map, 0, i, e.h, pid, smem_u32(full));
+        }
+    };
+
+    if (warp == 0) {
+        // ---- the items, and K ----
+        int c = 0;   // tiles so far
+        bool ok = true, cut = false;
         while (ok) {
-            if (warp == 0) {
-                e.n = 0;
-                while (x < xe && e.n <= 0) e = segment(x);
-                if (taken >= SPAN_ITEMS)
-                    ok = __all_sync(0xffffffffu, wait(&item_empty[taken % SPAN_ITEMS], (taken / SPAN_ITEMS - 1) & 1));
-                if (!ok) break;
-                if (lane == 0) {
-                    item_at(taken) = e;
-                    mbar_arrive(&item_full[taken % SPAN_ITEMS]);
-                }
-                ++taken;
-                if (e.n <= 0) break;
-                if (e.start && !e.whole) {   // (the run's last item)
-                    if (lane == 0) *reinterpret_cast<int4*>(cuts + blockIdx.x) = make_int4(e.tok0, e.h, e.rows, e.runs);
-                    cut = true;
-                }
-            } else {
-                if (!take(e, ok)) break;
-                done_with();
-                ok = load_q(e, 0, nq0++);
-                if (ok && e.both) ok = load_q(e, 1, nq1++);
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    break;
-                }
+            next_item();
+            if (taken >= SPAN_ITEMS)
+                ok = __all_sync(0xffffffffu, wait(&item_empty[taken % SPAN_ITEMS], (taken / SPAN_ITEMS - 1) & 1));
+            if (!ok) break;
+            if (lane == 0) {
+                item_at(taken) = cur;
+                mbar_arrive(&item_full[taken % SPAN_ITEMS]);
             }
-            const int* row = a.table + e.slot * a.table_row;
-            // what no row sees is read as zeros, from outside the map
-            auto look = [&](int j) {
-                const int at = tile_at(e, j) + lane * page;
-                return lane < chunks && in_sight(e, at) ? __ldg(row + (at >> a.pool.shift)) : a.pool.pages;
-            };
-            int next = look(0);
-            for (int j = 0; j < e.n; ++j, ++c) {
-                int pid = next;
-                if (j + 1 < e.n) next = look(j + 1);
-                if (pid < 0 || pid >= a.pool.pages) {
-                    if (lane < chunks && in_sight(e, tile_at(e, j) + lane * page)) {
-                        note_status(a.status, MQ_ERR_BAD_PAGE);
-                        *holes = 1;   // before the tile's scores are there
+            ++taken;
+            if (cur.n <= 0) break;
+            if (cur.start && !cur.whole) {   // (the run's last item)
+                if (lane == 0) *reinterpret_cast<int4*>(cuts + blockIdx.x) = make_int4(cur.tok0, cur.h, cur.rows, cur.runs);
+                cut = true;
+            }
+            int next = look(cur, 0);
+            for (int j = 0; j < cur.n; ++j, ++c) {
+                const int pid = next, st = c & 1;
+                if (j + 1 < cur.n) next = look(cur, j + 1);
+                if (c >= 2) ok = __all_sync(0xffffffffu, wait(&k_empty[st], ((c >> 1) - 1) & 1));
+                if (!ok) break;
+                load_tile(cur, j, pid, &tmK, smem + L::K + st * TILE, &k_full[st]);
+            }
+        }
+        if (!cut && lane == 0) *reinterpret_cast<int4*>(cuts + blockIdx.x) = make_int4(0, 0, 0, 0);
+        if (!ok && lane == 0) give_up();
+        for (int k = max(0, c - 2); k < c; ++k) land(&k_full[k & 1], (k >> 1) & 1);
+    } else if (warp == 2) {
+        // ---- Q and V: loads, and what is looked through when it has landed.  Whatever is waited for, tiles of V that land
+        // meanwhile are passed on ----
+        int c = 0, seen = 0, nq = 0;   // tiles asked for, tiles passed on, items
+        uint32_t masked = 0;           // bit st: the tile in stage st is not seen whole by every row
+        bool ok = true;
+        auto pass_on = [&]() {
+            const int st = seen & 1;
+            if (masked >> st & 1u) {
+                constexpr uint32_t M = Elem<T>::EXP_MASK * 0x10001u, U = (Elem<T>::EXP_MASK & -Elem<T>::EXP_MASK) * 0x10001u;
+                uint8_t* vt = smem + L::V + st * TILE;
+                uint32_t any = 0;
+#pragma unroll 8
+                for (int i = lane; i < TILE / 16; i += 32) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(vt + i * 16);
+                    // an exponent of all ones and one more carries out of its field
+                    any |= ((w.x & M) + U) | ((w.y & M) + U) | ((w.z & M) + U) | ((w.w & M) + U);
+                }
+                const bool odd = __any_sync(0xffffffffu, any & 0x80008000u);
+                if (odd) {
+                    uint8_t* bits = smem + L::ODD + st * 128 * (D / 8);
+                    for (int i = lane; i < TILE / 16; i += 32) {
+                        // 16-byte piece i: block of 64 channels, key, piece of it (swizzled by the key)
+                        const int key = i >> 3 & 127, ch = (i >> 10) * 8 + ((i & 7) ^ (key & 7));
+                        uint4 w = *reinterpret_cast<const uint4*>(vt + i * 16);
+                        uint32_t* v = reinterpret_cast<uint32_t*>(&w);
+                        uint32_t mark = 0;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t f = (v[k] & M) + U;
+                            if (f & 0x8000u) mark |= 1u << (2 * k), v[k] &= 0xffff0000u;
+                            if (f & 0x80000000u) mark |= 2u << (2 * k), v[k] &= 0xffffu;
+                        }
+                        bits[key * (D / 8) + ch] = (uint8_t)mark;
+                        if (mark) *reinterpret_cast<uint4*>(vt + i * 16) = w;
                     }
-                    pid = a.pool.pages;
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
-                const int st = c & 1;
-                const bool here = c < 2 || wait(&empty[st], ((c >> 1) - 1) & 1);
-                if (!__all_sync(0xffffffffu, here)) {
-                    ok = false;
-                    break;
-                }
-                if (lane == 0) mbar_arrive_expect_tx(&full[st], TILE);
+                if (lane == 0) odd_tile[st] = odd;
                 __syncwarp();
-                if (lane < chunks) {
+            }
+            if (lane == 0) mbar_arrive(&v_ready[st]);
+            ++seen;
+        };
+        auto pump = [&](uint64_t* bar, uint32_t parity) {   // waits for bar
+            const long long t0 = clock64();
+            while (ok && !__all_sync(0xffffffffu, mbar_test_wait(bar, parity & 1))) {
+                if (seen < c && __all_sync(0xffffffffu, mbar_test_wait(&v_full[seen & 1], (seen >> 1) & 1))) pass_on();
+                if (__any_sync(0xffffffffu, *abort_flag || clock64() - t0 > WAIT_CYCLES)) ok = false;
+            }
+            return ok;
+        };
+        for (SpanSeg e; pump(&item_full[taken % SPAN_ITEMS], taken / SPAN_ITEMS) && take(e, ok); ++nq) {
+            done_with();
+            for (int q = 0; q < 2; ++q) {
+                if (nq && !pump(&q_empty[q], nq - 1)) break;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&q_full[q], (D / 64) * tps * grp * 128);
 #pragma unroll
                     for (int i = 0; i < D / 64; ++i)
-                        tma_load_page(smem_u32(ring + st * TILE + i * PATOM + lane * page * 128), map, 0, i, e.h, pid, smem_u32(&full[st]));
+                        tma_load_heads(smem_u32(smem + L::Q + q * TILE + i * PATOM), &tmQ, i, e.h * grp,
+                                       e.tok0 + (e.two ? q * tps : 0), smem_u32(&q_full[q]));
                 }
             }
-        }
-        if (warp == 0 && !cut && lane == 0) *reinterpret_cast<int4*>(cuts + blockIdx.x) = make_int4(0, 0, 0, 0);
-        if (!ok && lane == 0) give_up();
-        // copies in flight land before the CTA may end, whatever became of their readers
-        auto land = [&](uint64_t* bar, uint32_t parity) {
-            const long long t0 = clock64();
-            while (!mbar_try_wait(bar, parity) && clock64() - t0 < WAIT_CYCLES) {
-            }
-        };
-        for (int k = max(0, c - 2); k < c; ++k) land(&full[k & 1], (k >> 1) & 1);
-        if (!ok && warp == 2) {   // (otherwise the scores of every Q tile have been waited for)
-            if (nq0) land(&q_full[0], (nq0 - 1) & 1);
-            if (nq1) land(&q_full[1], (nq1 - 1) & 1);
-        }
-    } else if (warp == 3) {
-        // ---- looks through the values of masked tiles ----
-        int c = 0;
-        bool ok = true;
-        for (SpanSeg e; take(e, ok); done_with()) {
-            for (int j = 0; j < e.n; ++j, ++c) {
-                const int st = c & 1;
-                ok = __all_sync(0xffffffffu, wait(&v_full[st], (c >> 1) & 1));
-                if (!ok) break;
-                if (!all_seen(e, tile_at(e, j))) {
-                    constexpr uint32_t M = Elem<T>::EXP_MASK * 0x10001u, U = (Elem<T>::EXP_MASK & -Elem<T>::EXP_MASK) * 0x10001u;
-                    uint8_t* vt = smem + L::V + st * TILE;
-                    uint32_t any = 0;
-#pragma unroll 8
-                    for (int i = lane; i < TILE / 16; i += 32) {
-                        const uint4 w = *reinterpret_cast<const uint4*>(vt + i * 16);
-                        // an exponent of all ones and one more carries out of its field
-                        any |= ((w.x & M) + U) | ((w.y & M) + U) | ((w.z & M) + U) | ((w.w & M) + U);
-                    }
-                    const bool odd = __any_sync(0xffffffffu, any & 0x80008000u);
-                    if (odd) {
-                        uint8_t* bits = smem + L::ODD + st * 128 * (D / 8);
-                        for (int i = lane; i < TILE / 16; i += 32) {
-                            // 16-byte piece i: block of 64 channels, key, piece of it (swizzled by the key)
-                            const int key = i >> 3 & 127, ch = (i >> 10) * 8 + ((i & 7) ^ (key & 7));
-                            uint4 w = *reinterpret_cast<const uint4*>(vt + i * 16);
-                            uint32_t* v = reinterpret_cast<uint32_t*>(&w);
-                            uint32_t mark = 0;
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const uint32_t f = (v[k] & M) + U;
-                                if (f & 0x8000u) mark |= 1u << (2 * k), v[k] &= 0xffff0000u;
-                                if (f & 0x80000000u) mark |= 2u << (2 * k), v[k] &= 0xffffu;
-                            }
-                            bits[key * (D / 8) + ch] = (uint8_t)mark;
-                            if (mark) *reinterpret_cast<uint4*>(vt + i * 16) = w;
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    }
-                    if (lane == 0) odd_tile[st] = odd;
-                    __syncwarp();
-                }
-                if (lane == 0) mbar_arrive(&v_ready[st]);
+            if (!ok) break;
+            int next = look(e, 0);
+            for (int j = 0; j < e.n; ++j) {
+                const int pid = next, st = c & 1;
+                if (j + 1 < e.n) next = look(e, j + 1);
+                if (c >= 2 && !pump(&v_empty[st], (c >> 1) - 1)) break;
+                masked = (masked & ~(1u << st)) | (uint32_t)!all_seen(e, tile_at(e, j), PK) << st;
+                load_tile(e, j, pid, &tmV, smem + L::V + st * TILE, &v_full[st]);
+                ++c;
             }
         }
-        if (!ok && lane == 0) give_up();
-    } else if (warp == 1) {
-        // ---- MMA: the whole warp walks, one elected lane issues.  All 512 columns of
-        // TMEM are this CTA's, so their addresses start at 0 ----
+        while (ok && seen < c) {
+            ok = __all_sync(0xffffffffu, wait(&v_full[seen & 1], (seen >> 1) & 1));
+            if (ok) pass_on();
+        }
+        if (!ok) {
+            if (lane == 0) give_up();
+            for (int k = max(0, c - 2); k < c; ++k) land(&v_full[k & 1], (k >> 1) & 1);
+            // (otherwise the scores of every Q tile have been waited for)
+            for (int q = 0; q < 2; ++q)
+                if (nq) land(&q_full[q], (nq - 1) & 1);
+            land(&q_full[0], nq & 1);   // A's of an item whose B could not be asked for (if there is none, this runs out)
+        }
+    } else if (warp == 1 || warp == 3) {
+        // ---- MMA of a stream: the whole warp walks, one elected lane issues.  All 512 columns of TMEM are this CTA's, so
+        // their addresses start at 0.  The tensor core takes an MMA when the one before is nearly done (12 MMAs of 620
+        // cycles take 620 to issue to an idle pipe), so what an issuing warp does between two is lost to the pipe unless
+        // another warp issues meanwhile: a warp for each stream ----
+        const int q = warp >> 1;
         constexpr uint32_t id_o = pfx_idesc<T>(D, true);
         // a negative scale: the scores of -Q
-        const uint32_t id_s = pfx_idesc<T>(PK, false) | (a.scale_log2 < 0.f ? 1u << 13 : 0u);
+        const uint32_t id_s = pfx_idesc<T>(HK, false) | (a.scale_log2 < 0.f ? 1u << 13 : 0u);
         const uint32_t base = (smem_u32(pfx_raw) + 1023u) & ~1023u;
-        int c0 = 0;                         // tiles of the segments before
-        uint32_t np0 = 0, np1 = 0;          // PVs issued per stream
-        uint32_t nq0 = 0, nq1 = 0;          // Q tiles used per stream
+        int c0 = 0;          // tiles of the items before
+        uint32_t g = 0;      // steps (64 keys) of the items before
+        uint32_t nq = 0;     // items
         bool ok = true;
-        auto scores = [&](int q, int kc, bool last_use, bool last) {
-            const uint32_t sq = base + L::Q + q * TILE, sk = base + L::K + (kc & 1) * TILE;
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-                const uint32_t o = (k >> 2) * PATOM + (k & 3) * 32;
-                tc_mma_f16(q * 128, sw128_kmajor_desc(sq + o), sw128_kmajor_desc(sk + o), id_s, k != 0);
-            }
-            tc_commit(&s_full[q]);
-            if (last_use) tc_commit(&k_empty[kc & 1]);
-            if (last) tc_commit(&q_empty[q]);
-        };
-        auto values = [&](int q, int vc, bool first, bool last_use, bool done) {
-            const uint32_t sv = base + L::V + (vc & 1) * TILE, o = 256 + q * 128;
-#pragma unroll
-            for (int k = 0; k < PK / 16; ++k) {
-                const uint32_t p = q * 128 + 8 * k;   // 16 keys: 8 columns
-                tc_mma_f16_ts(o, p, sw128_mnmajor_desc(sv + k * 2048), id_o, !first || k);
-            }
-            if (last_use) tc_commit(&v_empty[vc & 1]);
-            if (done) tc_commit(&o_full[q]);
-        };
+        const uint32_t q_lo = desc_lo(base + L::Q, 1) + q * (TILE >> 4);
+        const uint32_t k_lo = desc_lo(base + L::K, 1), v_lo = desc_lo(base + L::V, PATOM >> 4);
         for (SpanSeg e; take(e, ok); done_with()) {
-            const int n = uniform(e.n);
             const bool two = uniform(e.two);
-            const int steps = two ? 2 * n : n;
-            // step i: the stream's PV of its tile before (step i - 2), then its S of this one.  What the
-            // step needs is waited for by four lanes at once.
-            for (int i = 0; ok && i < steps + 2; ++i) {
-                const int q = i & 1;
-                const bool pv = i >= 2, sc = i < steps;
-                const int vc = c0 + (two ? (i - 2) >> 1 : i - 2), kc = c0 + (two ? i >> 1 : i);
-                if (!pv && !sc) continue;   // a run of one tile: stream B has none
+            const int n = uniform(e.n), steps = two ? 2 * n : n;
+            // steps -2 and -1: scores of steps 0 and 1; step i: PV of step i, then scores of step i + 2, whose buffer
+            // the weights of step i were in.  What a step needs is waited for by four lanes at once.
+            for (int i = -2; ok && i < steps; ++i) {
+                const bool pv = i >= 0, sc = i + 2 < steps;
+                const int vc = c0 + (two ? i >> 1 : i), kc = c0 + (two ? (i + 2) >> 1 : i + 2);
+                if (!pv && !sc) continue;   // (an item of one step)
                 uint64_t* bar = nullptr;
                 uint32_t parity = 0;
                 if (lane == 0 && sc) bar = &k_full[kc & 1], parity = kc >> 1;
                 if (lane == 1 && pv) bar = &v_ready[vc & 1], parity = vc >> 1;
-                if (lane == 2 && pv) bar = &p_full[q], parity = q ? np1 : np0;
-                if (lane == 3 && !pv) bar = &q_full[q], parity = q ? nq1 : nq0;
+                if (lane == 2 && pv) bar = &p_full[2 * q + ((g + i) & 1)], parity = (g + i) >> 1;
+                if (lane == 3 && i == -2) bar = &q_full[q], parity = nq;
                 ok = __all_sync(0xffffffffu, !bar || wait(bar, parity & 1));
-                if (pv) (q ? np1 : np0)++;
-                else (q ? nq1 : nq0)++;
                 if (!ok) break;
                 tc_fence_after();
+                // a stream takes both halves of a tile, or one
+                const int half = two ? i & 1 : q;
+                const bool used = !two || (i & 1);
+                const uint32_t buffer = q * 128 + ((g + i) & 1) * HK, o = 256 + q * 128;
+                const uint32_t vl = v_lo + (vc & 1) * (TILE >> 4) + half * (HK * 128 >> 4);
+                const uint32_t kl = k_lo + (kc & 1) * (TILE >> 4) + half * (HK * 128 >> 4);
                 if (elect_one()) {
-                    if (pv) values(q, vc, i < 4, !two || q == 1, !sc);
-                    if (sc) scores(q, kc, !two || q == 1, i >= steps - 2);
+                    if (pv) {
+#pragma unroll
+                        for (int k = 0; k < HK / 16; ++k)   // 16 keys: 8 columns of weights
+                            mma_ts(o, buffer + 8 * k, vl + k * (2048 >> 4), id_o, k || i);
+                        if (i + 2 >= steps) tc_commit(&o_full[q]);
+                        if (used) tc_commit(&v_empty[vc & 1]);
+                    }
+                    if (sc) {
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k) {
+                            const uint32_t x = ((k >> 2) * PATOM + (k & 3) * 32) >> 4;
+                            mma_ss(buffer, q_lo + x, kl + x, id_s, k != 0);
+                        }
+                        tc_commit(&s_full[2 * q + ((g + i) & 1)]);
+                        if (used) tc_commit(&k_empty[kc & 1]);
+                        if (i + 3 == steps) tc_commit(&q_empty[q]);
+                    }
                 }
                 __syncwarp();
             }
             c0 += n;
+            g += steps;
+            ++nq;
         }
         if (!ok && lane == 0) give_up();
         if (elect_one()) tc_commit(drain);   // MMAs in flight end before TMEM goes
@@ -596,133 +646,133 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         float* sums = reinterpret_cast<float*>(smem + L::SUM);   // [stream][128]
         float* tops = reinterpret_cast<float*>(smem + L::TOP);
         ulonglong2* hits = reinterpret_cast<ulonglong2*>(smem + L::HIT);
-        constexpr float GROW = 8.f;
-        int ns = 0, nv = 0, no0 = 0, no1 = 0, np = 0;   // scores taken, tiles of the items before, results of A and B, meetings
+        constexpr float GROW = 14.f;
+        uint32_t g = 0, no = 0;  // steps (64 keys) so far, alike for both streams; o_full so far
+        int nv = 0, np = 0;      // tiles of the items before, meetings
         bool ok = true;
         auto got = [&](uint64_t* bar, uint32_t parity) {
-            if (ok) ok = __all_sync(0xffffffffu, wait(bar, parity));
+            if (ok) ok = __all_sync(0xffffffffu, wait(bar, parity & 1));
             return ok;
         };
         auto meet = [&]() {   // with the other stream's warp on the same rows
             __syncwarp();
             if (lane == 0) mbar_arrive(&pair[quad]);
-            got(&pair[quad], np++ & 1);
+            got(&pair[quad], np++);
         };
         const int tok_r = r / grp, head_r = r - tok_r * grp;   // of this row in its stream
         for (SpanSeg e; take(e, ok); done_with()) {
-            const int mine = e.two ? e.n : (e.n + 1 - q) >> 1;   // this stream's tiles
+            const int steps = e.two ? 2 * e.n : e.n;
             const int tok = (e.two ? q * tps : 0) + tok_r;       // the row's token in the item
             const bool there = tok_r < tps && tok * grp < e.rows;
             const int pos = min(e.pf + tok, e.pl), node = e.tok0 - e.seq0 + pos - e.pf;
             unsigned long long hit[2] = {0, 0};
             float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-            for (int j = 0; j < mine; ++j, ++ns) {
-                const int jt = e.two ? j : 2 * j + q, at = tile_at(e, jt);
-                const bool masked = !all_seen(e, at);
-                unsigned long long live[2] = {~0ull, ~0ull};   // keys that the row sees
-                if (masked) {
-                    live[0] = span_sees(a, pos, at, node, e.seq0);
-                    live[1] = span_sees(a, pos, at + 64, node, e.seq0);
-                }
-                if (!got(&s_full[q], ns & 1)) break;
+            for (int i = 0; i < steps; ++i, ++g) {
+                const int jt = e.two ? i >> 1 : i, tile = tile_at(e, jt), at = tile + (e.two ? i & 1 : q) * HK;
+                const bool looked = !all_seen(e, tile, PK);   // through the tile's values
+                unsigned long long live = ~0ull;              // keys that the row sees
+                if (looked && !all_seen(e, at, HK)) live = span_sees(a, pos, at, node, e.seq0);
+                const uint32_t sb = sa + (g & 1) * HK;
+                if (!got(&s_full[2 * q + (g & 1)], g >> 1)) break;
                 tc_fence_after();
-                if (*holes) {   // pages out of range: their keys are left out
+                const int hole = *holes;
+                float sv[HK];
+                tmem_ld64(sb, sv);
+                if (hole) {   // pages out of range: their keys are left out
                     const int* row = a.table + e.slot * a.table_row;
-                    for (int k = 0; k < PK; k += min(page, 64)) {
+                    for (int k = 0; k < HK; k += min(page, HK)) {
                         const int p = (at + k) & -page;
                         const int pid = in_sight(e, p) ? __ldg(row + (p >> a.pool.shift)) : 0;
-                        if (pid < 0 || pid >= a.pool.pages) {
-                            const unsigned long long gone = ~((page >= 64 ? ~0ull : (1ull << page) - 1ull) << (k & 63));
-                            if (k < 64) live[0] &= gone;
-                            else live[1] &= gone;
-                        }
+                        if (pid < 0 || pid >= a.pool.pages) live &= ~((page >= HK ? ~0ull : (1ull << page) - 1ull) << k);
                     }
                 }
-                float sv[128], mx[4];
-                tmem_ld128(sa, sv);
-                if (__any_sync(0xffffffffu, (live[0] & live[1]) != ~0ull)) {
+                if (looked || hole) {
+                    const uint32_t lo = (uint32_t)live, hi = (uint32_t)(live >> 32);
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const uint32_t b = (uint32_t)(live[w >> 1] >> (32 * (w & 1)));
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) sv[32 * w + k] = b >> k & 1u ? sv[32 * w + k] : -INFINITY;
+                    for (int k = 0; k < 32; ++k) {
+                        sv[k] = lo >> k & 1u ? sv[k] : -INFINITY;
+                        sv[32 + k] = hi >> k & 1u ? sv[32 + k] : -INFINITY;
                     }
                 }
+                float mx[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) mx[k] = fmaxf(sv[2 * k], sv[2 * k + 1]);
 #pragma unroll
-                for (int k = 8; k < 128; k += 2) mx[(k >> 1) & 3] = max3(mx[(k >> 1) & 3], sv[k], sv[k + 1]);
+                for (int k = 8; k < HK; k += 2) mx[(k >> 1) & 3] = max3(mx[(k >> 1) & 3], sv[k], sv[k + 1]);
                 const float tmax = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale;
-                // a row's maximum moves only when it grew by more than 2^8; weights stay below 256
+                // a row's reference moves only when its maximum is more than 2^14 above it: weights stay below that (fp16 ends at
+                // 2^16), and one of the first keys, among few, is often some octaves below the row's maximum
                 float corr = 1.f;
                 if (tmax > m + GROW) {
-                    corr = ex2(m - tmax);   // 0 on the first tile
+                    corr = m == -INFINITY ? 1.f : ex2(m - tmax);   // (nothing is summed before the first key that the row sees)
                     m = tmax;
                 }
                 l *= corr;
-                if (j && __any_sync(0xffffffffu, corr != 1.f)) {
-                    // s_full covers the PV before it, so O is at rest
+                if (i && __any_sync(0xffffffffu, corr != 1.f)) {
+                    // O is at rest once the PV before is done: the scores after these came after it, or it was the last but one
+                    if (i + 1 < steps ? !got(&s_full[2 * q + ((g + 1) & 1)], (g + 1) >> 1) : !got(&o_full[q], no)) break;
+                    tc_fence_after();
 #pragma unroll 1
-                    for (int i = 0; i < D; i += 16) {
-                        float v[16];
-                        tmem_ld16(oa + q * 128 + i, v);
+                    for (int c = 0; c < D; c += 32) {
+                        float v[32];
+                        tmem_ld32(oa + q * 128 + c, v);
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) v[k] *= corr;
-                        tmem_st16(oa + q * 128 + i, v);
+                        for (int k = 0; k < 32; ++k) v[k] *= corr;
+                        tmem_st16_nowait(oa + q * 128 + c, reinterpret_cast<const uint32_t*>(v));
+                        tmem_st16_nowait(oa + q * 128 + c + 16, reinterpret_cast<const uint32_t*>(v + 16));
                     }
                 }
                 const uint64_t scale2 = two_of(scale, scale), u2 = m == -INFINITY ? 0ull : two_of(-m, -m);
                 uint64_t sum0 = 0ull, sum1 = 0ull;
 #pragma unroll
-                for (int i = 0; i < 128; i += 32) {
+                for (int c = 0; c < HK; c += 32) {
                     uint32_t pk[16];   // 32 weights in 16 columns, over the scores
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                         float p0, p1;
-                        halves(fma2(two_of(sv[i + 2 * k], sv[i + 2 * k + 1]), scale2, u2), p0, p1);
+                        halves(fma2(two_of(sv[c + 2 * k], sv[c + 2 * k + 1]), scale2, u2), p0, p1);
                         p0 = ex2(p0);
                         p1 = ex2(p1);
                         (k & 1 ? sum1 : sum0) = add2(k & 1 ? sum1 : sum0, two_of(p0, p1));
                         pk[k] = Elem<T>::pack(p0, p1);
                     }
-                    tmem_st16_nowait(sa + (i >> 1), pk);
+                    tmem_st16_nowait(sb + (c >> 1), pk);
                 }
                 float s0, s1;
                 halves(add2(sum0, sum1), s0, s1);
                 l += s0 + s1;
-                if (masked) {
+                if (looked) {
                     // the tile's values are looked through, and stay until this stream's weights are used
                     const int c = nv + jt, st = c & 1;
-                    if (got(&v_ready[st], (c >> 1) & 1) && odd_tile[st]) {
-                        const uint8_t* bits = smem + L::ODD + st * 128 * (D / 8);
+                    if (got(&v_ready[st], c >> 1) && odd_tile[st]) {
+                        const uint8_t* bits = smem + L::ODD + (st * 128 + at - tile) * (D / 8);
 #pragma unroll 1
-                        for (int k = 0; k < PK; ++k) {
-                            if (!((k < 64 ? live[0] : live[1]) >> (k & 63) & 1ull)) continue;
+                        for (int k = 0; k < HK; ++k) {
+                            if (!(live >> k & 1ull)) continue;
                             hit[0] |= *reinterpret_cast<const unsigned long long*>(bits + k * (D / 8));
                             if (D == 128) hit[1] |= *reinterpret_cast<const unsigned long long*>(bits + k * (D / 8) + 8 * (D / 128));
                         }
                     }
                 }
+                if (i && i + 1 == steps && !got(&o_full[q], no++)) break;   // (in its turn: a phase passed over cannot be told)
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[q]);
+                if (lane == 0) mbar_arrive(&p_full[2 * q + (g & 1)]);
             }
             nv += e.n;
             // ---- the item's rows: what A and B have of them, when they share them ----
-            if (!e.two || q == 0) got(&o_full[0], no0 & 1);
-            if (e.two ? q == 1 : e.both) got(&o_full[1], no1 & 1);
-            ++no0;
-            no1 += e.both;
+            got(&o_full[q], no++);
             tc_fence_after();
             float e0 = 1.f, e1 = 1.f;   // weights of A's and B's accumulators
             if (!e.two) {
                 sums[q * 128 + r] = l;
                 tops[q * 128 + r] = m;
                 hits[q * 128 + r] = make_ulonglong2(hit[0], hit[1]);
-                meet();
-                const float ma = tops[r], mb = tops[128 + r];   // (B's is -inf when it had no tile)
+                meet();   // (and the other stream's accumulator is complete, too)
+                tc_fence_after();
+                const float ma = tops[r], mb = tops[128 + r];
                 m = fmaxf(ma, mb);
                 const float u = m == -INFINITY ? 0.f : m;
                 e0 = ex2(ma - u);
@@ -744,9 +794,9 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                 tmem_ld32(oa + (e.two ? q * 128 : 0) + c, v);
                 if (!e.two) {
                     float w[32];
-                    if (e.both) tmem_ld32(oa + 128 + c, w);
+                    tmem_ld32(oa + 128 + c, w);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) v[k] = e.both ? v[k] * e0 + w[k] * e1 : v[k] * e0;
+                    for (int k = 0; k < 32; ++k) v[k] = v[k] * e0 + w[k] * e1;
                 }
                 const uint32_t odd = (uint32_t)(hit[c >> 6] >> (c & 63));
                 if (odd) {

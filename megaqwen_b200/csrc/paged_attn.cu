@@ -665,7 +665,7 @@ Shape shape_of(const mq_paged_attend_params* p) {
 // tensor map, whose strides are positive).
 bool tc_span(const mq_paged_span_params* p) {
     const int grp = p->num_q_heads / p->pool->num_kv_heads;
-    return (long long)p->total_q * grp > 16ll * p->num_seqs && grp <= PROWS / 2 && (p->q_token > 0 || p->total_q == 1) &&
+    return (long long)p->total_q * grp > 16ll * p->num_seqs && grp <= PROWS / 2 && p->num_seqs <= SPAN_SEQS && (p->q_token > 0 || p->total_q == 1) &&
            (p->q_head > 0 || p->num_q_heads == 1);
 }
 size_t span_workspace(const mq_paged_span_params* p, SpanCut** cuts, float** slots, void* base) {
@@ -726,7 +726,10 @@ int run_span_tc(const RowArgs& a, SpanCut* cuts, const mq_paged_pool& pool, cuda
     cudaError_t e = allow_smem(kernel, smem, limit);
     const int grid = sm_count();
     if (e == cudaSuccess) e = launch(kernel, dim3(grid), dim3(SPAN_THREADS), smem, st, tq, tk, tv, a, cuts);
-    if (e == cudaSuccess) e = launch(span_join_kernel<T, D>, dim3(grid, PROWS / SPAN_JOIN_ROWS), dim3(256), 0, st, a, (const SpanCut*)cuts);
+    // a warp to a row of a cut item for few rows, whose latency counts, four rows otherwise
+    const int rows = (int)std::min<long long>(PROWS, (long long)a.total_q * a.grp), each = rows <= 64 ? 1 : 4;
+    if (e == cudaSuccess)
+        e = launch(span_join_kernel<T, D>, dim3(grid, ceil_div(rows, 8 * each)), dim3(256), 0, st, a, (const SpanCut*)cuts, each);
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "paged attention under a mask");
 }
 

@@ -34,6 +34,7 @@ namespace paged {
 
 constexpr int SPAN_THREADS = 384;   // warps: 0 items and K, 1 MMA of A, 2 Q and V (loads, and looks through V), 3 MMA of B, 4-7 softmax of A, 8-11 of B
 constexpr int HK = 64;              // keys to a step of a stream
+constexpr int SPAN_SEQS = 448;      // sequences of a call: their schedule is in shared memory
 constexpr int SPAN_ITEMS = 4;       // ring of items between the first warp and the others
 
 template <int D>
@@ -45,8 +46,9 @@ struct SpanSmem {
     static constexpr int TOP = SUM + 2 * 128 * 4;             // fp32 [2 streams][128] their reference
     static constexpr int HIT = TOP + 2 * 128 * 4;             // u64 [2 streams][128][2]: channels in which a row met a value that is not finite
     static constexpr int ODD = HIT + 2 * 128 * 16;            // [2 stages][128 keys][D / 8]: a bit for each such value
-    static constexpr int SCHED = ODD + 2 * 128 * (D / 8);
-    static constexpr size_t bytes(int B) { return SCHED + (size_t)(2 * B + 1) * 4 + 1024; }
+    static constexpr int STAGE = ODD + 2 * 128 * (D / 8);     // [8 warps][32 rows][64 bytes] of the output
+    static constexpr int SCHED = STAGE + 8 * 2048;
+    static constexpr size_t bytes(int B) { return SCHED + (size_t)(4 * B + 2) * 4 + 1024; }
 };
 
 // An item that is cut: the worker with its first tile leaves this for the join.
@@ -182,7 +184,7 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
     volatile int* holes = abort_flag + 1;      // a page out of range has been met
     volatile int* odd_tile = abort_flag + 2;   // [2] stages: the tile holds values that are not finite
-    __shared__ uint32_t scratch[NT / 32];
+    __shared__ unsigned long long scratch[NT / 32];
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -226,53 +228,85 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
 
     // ---- the line: off[b] units before sequence b, for one kv head ----
     uint32_t* off = reinterpret_cast<uint32_t*>(smem + L::SCHED);   // [B + 1]
-    int* lens = reinterpret_cast<int*>(off + a.B + 1);              // [B], 0 where nothing is read
+    int* first = reinterpret_cast<int*>(off + a.B + 1);             // [B + 1] query tokens before
+    int* lens = first + a.B + 1;                                    // [B], 0 where nothing is read
+    int* slots = lens + a.B;                                        // [B]
     const int grp = a.grp, page = a.pool.page, tps = PROWS / 2 / grp, tpt = 2 * tps;   // tokens to a stream and to a row tile
-    bool bad = false;
-    if (a.q_starts) {
-        for (int b = threadIdx.x; b < a.B; b += NT)
-            if (__ldg(a.q_starts + b + 1) < __ldg(a.q_starts + b)) bad = true;
-        if (threadIdx.x == 0 && (__ldg(a.q_starts) != 0 || __ldg(a.q_starts + a.B) != a.total_q)) bad = true;
-    }
-    bool in_order = !__syncthreads_or(bad);
-    {
-        unsigned long long carry = 0;
-        for (int b0 = 0; in_order && b0 < a.B; b0 += NT) {
-            const int b = b0 + threadIdx.x;
-            unsigned long long cost = 0;
-            if (b < a.B) {
-                const int slot = __ldg(a.slots + b), ql = q_start(a, b + 1) - q_start(a, b);
-                int len = 0, code = 0;
-                if (slot < 0 || slot >= a.num_slots) {
-                    code = MQ_ERR_BAD_SLOT;
-                } else {
-                    len = __ldg(a.lengths + slot);
-                    if (len < 0 || pages_for(len, a.pool.shift) > a.cols) code = MQ_ERR_BAD_POSITION;
-                    else if (a.parents && ql > MAX_TREE) code = MQ_ERR_INVALID_ARGUMENT;
-                }
-                if (code) {
-                    len = 0;
-                    if (blockIdx.x == 0) note_status(a.status, code);
-                }
-                lens[b] = len;
+    constexpr uint32_t LATER = 0xffffffffu;   // a sequence of many row tiles: their costs are summed by a warp
+    bool bad = false, later = false;
+    for (int b = threadIdx.x; b <= a.B; b += NT) {
+        const int q0 = q_start(a, b);
+        first[b] = q0;
+        if (b == a.B) {
+            bad |= q0 != a.total_q;
+            break;
+        }
+        const int slot = __ldg(a.slots + b), ql = q_start(a, b + 1) - q0;
+        bad |= ql < 0 || (b == 0 && q0 != 0);
+        int len = 0, code = 0;
+        if (slot < 0 || slot >= a.num_slots) {
+            code = MQ_ERR_BAD_SLOT;
+        } else {
+            len = __ldg(a.lengths + slot);
+            if (len < 0 || pages_for(len, a.pool.shift) > a.cols) code = MQ_ERR_BAD_POSITION;
+            else if (a.parents && ql > MAX_TREE) code = MQ_ERR_INVALID_ARGUMENT;
+        }
+        if (code) {
+            len = 0;
+            if (blockIdx.x == 0 && ql >= 0) note_status(a.status, code);
+        }
+        lens[b] = len;
+        slots[b] = slot;
+        uint32_t cost = 0;
+        if (len && ql > 0) {
+            if (ql > 4 * tpt) {
+                cost = LATER;
+                later = true;
+            } else {
                 int st, wt;
-                for (int i = 0; len && i < ql; i += tpt) {
+                for (int i = 0; i < ql; i += tpt) {
                     const int n = span_tiles(a, len - ql + i, len - ql + min(i + tpt, ql) - 1, st, wt);
                     cost += n ? n + ITEM_UNITS : 0;
                 }
             }
+        }
+        off[b] = cost;
+    }
+    bool in_order = !__syncthreads_or(bad);
+    if (__syncthreads_or(later && in_order)) {
+        for (int b = warp; b < a.B; b += NT / 32) {
+            if (off[b] != LATER) continue;
+            const int ql = first[b + 1] - first[b], p0 = lens[b] - ql;
+            unsigned long long cost = 0;
+            for (int i0 = lane; (long long)i0 * tpt < ql; i0 += 32) {
+                const int i = i0 * tpt;
+                int st, wt;
+                const int n = span_tiles(a, p0 + i, p0 + min(i + tpt, ql) - 1, st, wt);
+                cost += n ? n + ITEM_UNITS : 0;
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) cost += __shfl_xor_sync(0xffffffffu, cost, o);
+            __syncwarp();
+            if (lane == 0) off[b] = (uint32_t)(cost < 0x7fffffffull ? cost : 0x7fffffffull);   // (a sum that long is refused below)
+        }
+        __syncthreads();
+    }
+    {
+        unsigned long long carry = 0;
+        for (int b0 = 0; in_order && b0 < a.B; b0 += NT) {
+            const int b = b0 + threadIdx.x;
+            const unsigned long long cost = b < a.B ? off[b] : 0;
             unsigned long long x = cost;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
                 if (lane >= o) x += y;
             }
-            const bool big = x > 0x7fffffffull;   // a sum that does not fit is refused below
-            if (lane == 31) scratch[warp] = big ? 0x7fffffffu : (uint32_t)x;
+            if (lane == 31) scratch[warp] = x;
             __syncthreads();
             unsigned long long before = carry;
             for (int w = 0; w < NT / 32; ++w) {
-                const uint32_t v = scratch[w];
+                const unsigned long long v = scratch[w];
                 if (w < warp) before += v;
                 carry += v;
             }
@@ -293,9 +327,9 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     SpanSeg cur;
     auto open = [&](int b) {
         it_b = b;
-        cur.slot = __ldg(a.slots + b);
-        cur.seq0 = q_start(a, b);
-        it_ql = q_start(a, b + 1) - cur.seq0;
+        cur.slot = slots[b];
+        cur.seq0 = first[b];
+        it_ql = first[b + 1] - cur.seq0;
         it_p0 = lens[b] - it_ql;
     };
     auto locate = [&]() -> int {   // units of the item before x
@@ -645,6 +679,7 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         const uint32_t sa = tmem + lane_off + q * 128, oa = tmem + lane_off + 256;   // O of A, that of B 128 columns on
         float* sums = reinterpret_cast<float*>(smem + L::SUM);   // [stream][128]
         float* tops = reinterpret_cast<float*>(smem + L::TOP);
+        uint8_t* stage = smem + L::STAGE + (warp - 4) * 2048;
         ulonglong2* hits = reinterpret_cast<ulonglong2*>(smem + L::HIT);
         constexpr float GROW = 14.f;
         uint32_t g = 0, no = 0;  // steps (64 keys) so far, alike for both streams; o_full so far
@@ -785,24 +820,36 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
             const float inv = l != 0.f ? 1.f / l : 0.f;   // a row that sees nothing is zero (NaN stays NaN)
             // this thread's columns: the row's, or with two streams on it half of them
             const int c_lo = e.two ? 0 : q * (D / 2), c_hi = e.two ? D : c_lo + D / 2;
+            const uint32_t own = oa + (e.two ? q * 128 : 0);
             float* part = there ? a.ws.pfx_slots + ((2ll * blockIdx.x + e.start) * PROWS + tok * grp + head_r) * LD : nullptr;
             uint16_t* out = there ? a.out + ((long long)(e.tok0 + tok) * a.hq + e.h * grp + head_r) * D : nullptr;
+            if (__any_sync(0xffffffffu, (hit[0] | hit[1]) != 0)) {   // channels in which a row met a value that is not finite
+#pragma unroll 1
+                for (int c = c_lo; ok && c < c_hi; c += 16) {
+                    float v[16];
+                    tmem_ld16(own + c, v);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        if (hit[c >> 6] >> ((c & 63) + k) & 1ull) v[k] = NAN;
+                    tmem_st16(own + c, v);
+                }
+            }
+            uint16_t* rows[4];   // where this lane's piece of row 8 k + lane / 4 of the warp goes
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                rows[k] = from_lane(out, 8 * k + (lane >> 2));
+                if (rows[k]) rows[k] += (lane & 3) * 8;
+            }
             if (!e.whole && ok && there && (e.two || q == 0)) *reinterpret_cast<float4*>(part) = make_float4(m, l, 0.f, 0.f);
 #pragma unroll 1
             for (int c = c_lo; ok && c < c_hi; c += 32) {
                 float v[32];
-                tmem_ld32(oa + (e.two ? q * 128 : 0) + c, v);
+                tmem_ld32(own + c, v);
                 if (!e.two) {
                     float w[32];
                     tmem_ld32(oa + 128 + c, w);
 #pragma unroll
                     for (int k = 0; k < 32; ++k) v[k] = v[k] * e0 + w[k] * e1;
-                }
-                const uint32_t odd = (uint32_t)(hit[c >> 6] >> (c & 63));
-                if (odd) {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k)
-                        if (odd >> k & 1u) v[k] = NAN;
                 }
                 if (!e.whole) {
                     if (there) {
@@ -812,29 +859,21 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                     }
                     continue;
                 }
-                // four pieces of 16 bytes; four lanes turn theirs into whole 64 bytes of their four rows, so that a
-                // store touches eight rows and not 32
-                uint32_t w[4][4];
+                // through shared memory (pieces of 16 bytes, swizzled), so that a store touches 64 bytes of each of eight
+                // rows and not 16 of 32
 #pragma unroll
-                for (int k = 0; k < 16; ++k) w[k >> 2][k & 3] = Elem<T>::pack(v[2 * k] * inv, v[2 * k + 1] * inv);
-#pragma unroll
-                for (int x = 1; x < 4; x <<= 1) {
-                    const bool high = lane & x;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (i & x) continue;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint32_t other = __shfl_xor_sync(0xffffffffu, high ? w[i][k] : w[i | x][k], x);
-                            (high ? w[i][k] : w[i | x][k]) = other;
-                        }
-                    }
-                }
+                for (int k = 0; k < 4; ++k)
+                    *reinterpret_cast<uint4*>(stage + lane * 64 + ((k ^ (lane >> 1 & 3)) << 4)) =
+                        make_uint4(Elem<T>::pack(v[8 * k] * inv, v[8 * k + 1] * inv), Elem<T>::pack(v[8 * k + 2] * inv, v[8 * k + 3] * inv),
+                                   Elem<T>::pack(v[8 * k + 4] * inv, v[8 * k + 5] * inv), Elem<T>::pack(v[8 * k + 6] * inv, v[8 * k + 7] * inv));
+                __syncwarp();
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    uint16_t* to = from_lane(out, (lane & ~3) + k);
-                    if (to) *reinterpret_cast<uint4*>(to + c + (lane & 3) * 8) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+                    const int row = 8 * k + (lane >> 2);
+                    const uint4 w = *reinterpret_cast<const uint4*>(stage + row * 64 + (((lane & 3) ^ (row >> 1 & 3)) << 4));
+                    if (rows[k]) *reinterpret_cast<uint4*>(rows[k] + c) = w;
                 }
+                __syncwarp();
             }
             tc_fence_before();
             if (!e.two) meet();   // both accumulators are read
@@ -853,7 +892,7 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
             for (int t = wid; t < a.total_q; t += warps) clear(t, t + 1);
         } else {
             for (int b = wid; b < a.B; b += warps) {
-                const int t0 = q_start(a, b), ql = q_start(a, b + 1) - t0;
+                const int t0 = first[b], ql = first[b + 1] - t0;
                 int none = ql;   // tokens of row tiles that stand before the first position
                 if (lens[b]) none = lens[b] >= ql ? 0 : min(ql, (ql - lens[b]) / tpt * tpt);
                 if (none > 0) clear(t0, t0 + none);
@@ -869,70 +908,69 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
 }
 
 // The join of the items that were cut: acc = sum acc_i 2^(m_i - M) over sum l_i 2^(m_i - M).  blockIdx.y: a CTA's rows of
-// the cut; a warp to a row.
-constexpr int SPAN_JOIN_ROWS = 8;
+// the cut; a warp takes `each` of them.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) span_join_kernel(const RowArgs a, const SpanCut* __restrict__ cuts) {
+__global__ void __launch_bounds__(256) span_join_kernel(const RowArgs a, const SpanCut* __restrict__ cuts, int each) {
     constexpr int LD = D + 4, V = D / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
     pdl_trigger();
     const int4 cut = __ldcg(reinterpret_cast<const int4*>(cuts + blockIdx.x));
-    const int row = blockIdx.y * SPAN_JOIN_ROWS + warp;
-    if (row >= cut.z) return;
-    const float* slots = a.ws.pfx_slots + (2ll * blockIdx.x * PROWS + row) * LD;
-    auto part = [&](int i) { return slots + (2ll * i + (i == 0)) * PROWS * LD; };
-    float M = -INFINITY, Ls = 0.f, acc[V];
+    for (int row = (blockIdx.y * 8 + warp) * each, end = min(row + each, cut.z); row < end; ++row) {
+        const float* slots = a.ws.pfx_slots + (2ll * blockIdx.x * PROWS + row) * LD;
+        auto part = [&](int i) { return slots + (2ll * i + (i == 0)) * PROWS * LD; };
+        float M = -INFINITY, Ls = 0.f, acc[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = 0.f;
-    for (int i0 = 0; i0 < cut.w; i0 += 32) {
-        const int cnt = min(32, cut.w - i0);
-        const float2 ml = lane < cnt ? __ldcg(reinterpret_cast<const float2*>(part(i0 + lane))) : make_float2(-INFINITY, 0.f);
-        float bm = ml.x;
+        for (int i = 0; i < V; ++i) acc[i] = 0.f;
+        for (int i0 = 0; i0 < cut.w; i0 += 32) {
+            const int cnt = min(32, cut.w - i0);
+            const float2 ml = lane < cnt ? __ldcg(reinterpret_cast<const float2*>(part(i0 + lane))) : make_float2(-INFINITY, 0.f);
+            float bm = ml.x;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, o));
-        const float N = fmaxf(M, bm), U = N == -INFINITY ? 0.f : N;
-        const float c = exp2f(M - U), e = exp2f(ml.x - U);   // 0 for what is not there
-        M = N;
-        float l = ml.y * e;
+            for (int o = 16; o > 0; o >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, o));
+            const float N = fmaxf(M, bm), U = N == -INFINITY ? 0.f : N;
+            const float c = exp2f(M - U), e = exp2f(ml.x - U);   // 0 for what is not there
+            M = N;
+            float l = ml.y * e;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        Ls = Ls * c + l;
+            for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            Ls = Ls * c + l;
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] *= c;
+            for (int i = 0; i < V; ++i) acc[i] *= c;
 #pragma unroll 1
-        for (int k = 0; k < cnt; k += 4) {
-            float v[4][V], w[4];
+            for (int k = 0; k < cnt; k += 4) {
+                float v[4][V], w[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                w[q] = __shfl_sync(0xffffffffu, e, (k + q) & 31);
+                for (int q = 0; q < 4; ++q) {
+                    w[q] = __shfl_sync(0xffffffffu, e, (k + q) & 31);
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[q][i] = 0.f;
-                if (k + q < cnt) {
-                    const float* p = part(i0 + k + q) + 4 + lane * V;
-                    if (V == 4) {
-                        const float4 x = __ldcg(reinterpret_cast<const float4*>(p));
-                        v[q][0] = x.x; v[q][1] = x.y; v[q][V - 2] = x.z; v[q][V - 1] = x.w;
-                    } else {
-                        const float2 x = __ldcg(reinterpret_cast<const float2*>(p));
-                        v[q][0] = x.x; v[q][1] = x.y;
+                    for (int i = 0; i < V; ++i) v[q][i] = 0.f;
+                    if (k + q < cnt) {
+                        const float* p = part(i0 + k + q) + 4 + lane * V;
+                        if (V == 4) {
+                            const float4 x = __ldcg(reinterpret_cast<const float4*>(p));
+                            v[q][0] = x.x; v[q][1] = x.y; v[q][V - 2] = x.z; v[q][V - 1] = x.w;
+                        } else {
+                            const float2 x = __ldcg(reinterpret_cast<const float2*>(p));
+                            v[q][0] = x.x; v[q][1] = x.y;
+                        }
                     }
                 }
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) acc[i] += v[q][i] * (k + q < cnt ? w[q] : 0.f);
             }
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-                for (int i = 0; i < V; ++i) acc[i] += v[q][i] * (k + q < cnt ? w[q] : 0.f);
         }
+        const float inv = Ls != 0.f ? 1.f / Ls : 0.f;
+        const int tok = row / a.grp;
+        uint16_t* out = a.out + ((long long)(cut.x + tok) * a.hq + cut.y * a.grp + row - tok * a.grp) * D;
+        if (V == 4)
+            *reinterpret_cast<uint2*>(out + lane * 4) =
+                make_uint2(Elem<T>::pack(acc[0] * inv, acc[1] * inv), Elem<T>::pack(acc[V - 2] * inv, acc[V - 1] * inv));
+        else
+            *reinterpret_cast<uint32_t*>(out + lane * 2) = Elem<T>::pack(acc[0] * inv, acc[1] * inv);
     }
-    const float inv = Ls != 0.f ? 1.f / Ls : 0.f;
-    const int tok = row / a.grp;
-    uint16_t* out = a.out + ((long long)(cut.x + tok) * a.hq + cut.y * a.grp + row - tok * a.grp) * D;
-    if (V == 4)
-        *reinterpret_cast<uint2*>(out + lane * 4) =
-            make_uint2(Elem<T>::pack(acc[0] * inv, acc[1] * inv), Elem<T>::pack(acc[V - 2] * inv, acc[V - 1] * inv));
-    else
-        *reinterpret_cast<uint32_t*>(out + lane * 2) = Elem<T>::pack(acc[0] * inv, acc[1] * inv);
 }
 
 }  // namespace paged

@@ -726,10 +726,9 @@ int run_span_tc(const RowArgs& a, SpanCut* cuts, const mq_paged_pool& pool, cuda
     cudaError_t e = allow_smem(kernel, smem, limit);
     const int grid = sm_count();
     if (e == cudaSuccess) e = launch(kernel, dim3(grid), dim3(SPAN_THREADS), smem, st, tq, tk, tv, a, cuts);
-    // a warp to a row of a cut item for few rows, whose latency counts, four rows otherwise
-    const int rows = (int)std::min<long long>(PROWS, (long long)a.total_q * a.grp), each = rows <= 64 ? 1 : 4;
+    const int rows = (int)std::min<long long>(PROWS, (long long)a.total_q * a.grp);   // of an item, at most
     if (e == cudaSuccess)
-        e = launch(span_join_kernel<T, D>, dim3(grid, ceil_div(rows, 8 * each)), dim3(256), 0, st, a, (const SpanCut*)cuts, each);
+        e = launch(span_join_kernel<T, D>, dim3(grid, ceil_div(rows, 8)), dim3(256), 0, st, a, (const SpanCut*)cuts);
     return e == cudaSuccess ? MQ_OK : note_cuda(e, "paged attention under a mask");
 }
 

@@ -16,9 +16,18 @@
 //
 // Bound: HBM reads the row once, 4 or 2 bytes a token; what is done with it costs
 // more.  A cluster of up to 8 CTAs takes a row, each a contiguous share of it,
-// and keeps it in shared memory, so that the passes (maximum; a histogram over
-// the logits; the tokens of the bin in which a border lies, sorted; the sums)
-// stay on the SMs.
+// and keeps it in shared memory as fp32.  What follows depends on the rules:
+//   a top_k of up to FEW: the top_k-th largest of the threads' own maxima is a bound
+//     that top_k tokens reach; the few hundred that do go to the first CTA, which
+//     does the rest alone, in descending order and then by number;
+//   top_p alone: a histogram of the logits beside the sum of all weights tells which
+//     bins the border can lie in; the tokens of those, and the sums of the tokens
+//     above them, go to the first CTA, which finds the border and the piece of the row
+//     in which the token lies;
+//   neither: sums of pieces of the row, in the order of the tokens.
+// Rows that do not fit these (thousands of equal logits at a border, a large top_k, a
+// row longer than shared memory) take the general form: a histogram with exact sums
+// for each border, refined until the border's bin can be sorted.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -42,7 +51,9 @@ using u64 = unsigned long long;
 constexpr int NT = 512, NW = NT / 32;
 constexpr int BINS = 2048;          // four to a thread
 constexpr int CAP = 1024;           // tokens that are sorted
+constexpr int FEW = 512;            // the largest top_k whose tokens one CTA takes
 constexpr int MAX_RANKS = 8;
+constexpr int TABLE = 128;          // of 2^(j / TABLE)
 constexpr int FRAC = 43;            // a weight of 1 is 2^43
 constexpr int MAX_VOCAB = 1 << 20;  // a row's sum stays below 2^63
 constexpr float COUNT_SPAN = 40.f;  // logits below the maximum that the histogram of a count spreads over its bins
@@ -102,6 +113,12 @@ __device__ __forceinline__ uint32_t peer_ld(uint32_t at) {
     return v;
 }
 
+__device__ __forceinline__ uint32_t peer_add(uint32_t at, uint32_t v) {
+    uint32_t old;
+    asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(at), "r"(v) : "memory");
+    return old;
+}
+
 // What a CTA needs beside its share of the row.
 struct Shared {
     uint32_t count[BINS];             // of this CTA
@@ -110,32 +127,33 @@ struct Shared {
     u64 slot[2][MAX_RANKS][4];        // what the CTAs tell each other, two turns of it
     u64 warp_sum[NW];
     u64 found[4];
-    double two_to[32];                // 2^(j / 32)
+    double two_to[TABLE];             // 2^(j / TABLE)
+    u64 pieces[MAX_RANKS * NW];       // sums of the warps' pieces of the row, in the first CTA
+    u64 told[4];                      // what the first CTA tells the others
     int taken;
 };
 
-// The row's weights.  2^y by a table of 2^(j / 32) and the Taylor polynomial of 2^f, |f| <= 1 / 64, up to f^5 (the next
-// term is below 2^-48).
+// The row's weights.  2^y by a table of 2^(j / 128) and the Taylor polynomial of 2^(r / 128), |r| <= 1 / 2, up to r^4 (the
+// next term is below 2^-49).
 struct Weight {
-    double scale, top;   // log2(e) / T; the maximum
+    double scale, top;   // 128 log2(e) / T; the maximum
     float max;
-    __device__ __forceinline__ double octaves(float l) const { return l == max ? 0.0 : ((double)l - top) * scale; }
-    __device__ __forceinline__ u64 of(double y, const double* two_to) const {
-        if (!(y > -(double)FRAC - 1.0)) return 0;
+    __device__ __forceinline__ double place(float l) const { return l == max ? 0.0 : ((double)l - top) * scale; }   // 128 y
+    __device__ __forceinline__ u64 of(double z, const double* two_to) const {
+        if (!(z > -(FRAC + 1.0) * TABLE)) return 0;
         constexpr double MAGIC = 6755399441055744.0;   // 1.5 x 2^52: rounds to whole numbers
-        const double t = fma(y, 32.0, MAGIC), f = fma(t - MAGIC, -1.0 / 32.0, y);
+        const double t = z + MAGIC, r = z - (t - MAGIC);
         const int n = __double2loint(t);
-        double p = 1.3333558146428443e-03;             // ln(2)^k / k!
-        p = fma(p, f, 9.6181291076284772e-03);
-        p = fma(p, f, 5.5504108664821580e-02);
-        p = fma(p, f, 2.4022650695910071e-01);
-        p = fma(p, f, 6.9314718055994531e-01);
-        p = fma(p, f, 1.0) * two_to[n & 31];
+        double p = 3.583032305400251e-11;             // (ln(2) / 128)^k / k!
+        p = fma(p, r, 2.6466421444330967e-08);
+        p = fma(p, r, 1.4662262387640423e-05);
+        p = fma(p, r, 5.4152123481245725e-03);
+        p = fma(p, r, 1.0) * two_to[n & (TABLE - 1)];
         const u64 b = (u64)__double_as_longlong(p);
-        const int s = 52 - FRAC - ((int)(b >> 52) - 1023) - (n >> 5);   // 9 or more: rounded to the nearest
+        const int s = 52 - FRAC - ((int)(b >> 52) - 1023) - (n >> 7);   // 9 or more: rounded to the nearest
         return ((b & 0xfffffffffffffull | 1ull << 52) + (1ull << (s - 1))) >> s;
     }
-    __device__ __forceinline__ u64 of(float l, const double* two_to) const { return of(octaves(l), two_to); }
+    __device__ __forceinline__ u64 of(float l, const double* two_to) const { return of(place(l), two_to); }
 };
 
 // Exclusive sum over the CTA's threads; total for every thread.
@@ -159,6 +177,24 @@ __device__ __forceinline__ V block_scan(V v, u64* sm, V* total) {
     }
     __syncthreads();
     *total = all;
+    return before + x - v;
+}
+
+// The same for an estimate.
+__device__ __forceinline__ double block_scan_double(double v, double* sm) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    double x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) sm[warp] = x;
+    __syncthreads();
+    double before = 0;
+    for (int w = 0; w < warp; ++w) before += sm[w];
+    __syncthreads();
     return before + x - v;
 }
 
@@ -194,26 +230,34 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
     const T* row = reinterpret_cast<const T*>(a.logits) + (long long)r * a.row;
     const int lo = min(a.vocab, rank * a.share), n = min(a.vocab, lo + a.share) - lo;
     const T* x = row + lo;
-    if (tid < 32) s.two_to[tid] = exp2((double)tid / 32.0);
-    // the share, 16 bytes at a time, where it lies as in global memory to 16 bytes
-    u64 best = 0;
-    float least = INFINITY;
+    if (tid < TABLE) s.two_to[tid] = exp2((double)tid / TABLE);
+    if (tid == 0) s.taken = 0;
+    // the share, 16 bytes at a time; in shared memory it lies as in global memory to 16 bytes, with minus infinity before
+    // and behind
+    float best = -INFINITY, least = INFINITY;
+    int best_at = 0;
     auto look = [&](float v, int i) {
-        v = v == v ? v + 0.f : -INFINITY;   // NaN is never drawn; -0 is 0
-        best = max(best, place_key(v, lo + i));
+        if (v > best) best = v, best_at = i;   // (a thread's tokens ascend: the first of equal ones)
         if (v > -INFINITY) least = fminf(least, v);
     };
+    auto clean = [](float v) { return v == v ? v + 0.f : -INFINITY; };   // NaN is never drawn; -0 is 0
     constexpr int PER = 16 / sizeof(T);
     const int off = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));   // elements past a 16-byte border
-    T* near = reinterpret_cast<T*>(sample_raw + ((sizeof(Shared) + 15) & ~(size_t)15));
+    float* near = reinterpret_cast<float*>(sample_raw + ((sizeof(Shared) + 15) & ~(size_t)15));
+    const int quads = (off + n + 3) / 4;
     {
         const int head = min(n, off ? PER - off : 0), body = (n - head) / PER, tail = n - head - body * PER;
+        if (NEAR) {
+            if (tid < off) near[tid] = -INFINITY;
+            if (tid < 4 && off + n + tid < 4 * quads) near[off + n + tid] = -INFINITY;
+        }
         if (tid < head) {
-            look(up(x[tid]), tid);
-            if (NEAR) near[off + tid] = x[tid];
+            const float v = clean(up(x[tid]));
+            look(v, tid);
+            if (NEAR) near[off + tid] = v;
         }
         const uint4* from = reinterpret_cast<const uint4*>(x + head);
-        uint4* to = reinterpret_cast<uint4*>(near + (off ? PER : 0));
+        float4* to = reinterpret_cast<float4*>(near + (off ? PER : 0));
         constexpr int DEEP = 4;
         for (int i0 = tid; i0 < body; i0 += NT * DEEP) {
             uint4 v[DEEP];
@@ -224,21 +268,42 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
             for (int k = 0; k < DEEP; ++k) {
                 const int i = i0 + k * NT;
                 if (i >= body) break;
-                if (NEAR) to[i] = v[k];
                 const T* e = reinterpret_cast<const T*>(&v[k]);
+                float f[PER];
 #pragma unroll
-                for (int c = 0; c < PER; ++c) look(up(e[c]), head + i * PER + c);
+                for (int c = 0; c < PER; ++c) {
+                    f[c] = clean(up(e[c]));
+                    look(f[c], head + i * PER + c);
+                }
+                if (NEAR) {
+#pragma unroll
+                    for (int c = 0; c < PER; c += 4) to[i * (PER / 4) + c / 4] = make_float4(f[c], f[c + 1], f[c + 2], f[c + 3]);
+                }
             }
         }
         if (tid < tail) {
             const int i = head + body * PER + tid;
-            look(up(x[i]), i);
-            if (NEAR) near[off + i] = x[i];
+            const float v = clean(up(x[i]));
+            look(v, i);
+            if (NEAR) near[off + i] = v;
         }
     }
-    auto at = [&](int i) -> float {
-        const float v = NEAR ? up(near[off + i]) : up(__ldg(x + i));
-        return v == v ? v + 0.f : -INFINITY;
+    const float own_best = best;   // this thread's
+    auto at = [&](int i) -> float { return NEAR ? near[off + i] : clean(up(__ldg(x + i))); };
+    // f(logit, place in the share) for every token, four of a thread at a time, where any of a warp's is `low` or more; by
+    // whole warps, with minus infinity behind the end
+    auto each = [&](float low, auto f) {
+        const float4* q4 = reinterpret_cast<const float4*>(near);
+        for (int j0 = warp * 32; j0 < quads; j0 += NT) {
+            const int j = j0 + lane;
+            const float4 q = j < quads ? q4[j] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (!__any_sync(0xffffffffu, fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) >= low)) continue;
+            const int i = 4 * j - off;
+            f(q.x, i);
+            f(q.y, i + 1);
+            f(q.z, i + 2);
+            f(q.w, i + 3);
+        }
     };
     int turn = 0;
     // every CTA's four words to every CTA, all threads' writes before visible to all
@@ -249,36 +314,39 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         if (tid < 4 * ranks) peer_st(peer(&s.slot[turn][rank][tid & 3], tid >> 2), s.found[tid & 3]);
         cluster_sync();
     };
+    u64 first;   // the largest logit, the first of equal ones
     {   // the maximum and the smallest finite logit
+        u64 b = place_key(best, lo + best_at);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
-            best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+            b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
             least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
         }
         if (lane == 0) {
-            s.warp_sum[warp] = best;
+            s.warp_sum[warp] = b;
             s.list[warp] = order_key(least);
         }
         __syncthreads();
-        u64 b = 0, l = ~0ull;
+        u64 l = ~0ull;
+        b = 0;
         for (int w = 0; w < NW; ++w) {
             b = max(b, s.warp_sum[w]);
             l = min(l, s.list[w]);
         }
         if (ranks > 1) cluster_sync();   // every CTA runs: its shared memory may be written
         tell(b, l, 0, 0);
-        best = 0;
+        first = 0;
         l = ~0ull;
         for (int c = 0; c < ranks; ++c) {
-            best = max(best, s.slot[turn][c][0]);
+            first = max(first, s.slot[turn][c][0]);
             l = min(l, s.slot[turn][c][1]);
         }
         least = logit_of(l << 32);
     }
-    const float top = logit_of(best);
+    const float top = logit_of(first);
     const float temp = a.temperature ? __ldg(a.temperature + r) : a.temperature_v;
     if (!(temp > 0.f) || top == -INFINITY) {   // all CTAs alike
-        if (rank == 0 && tid == 0) a.out[r] = top == -INFINITY ? -1 : token_of(best);
+        if (rank == 0 && tid == 0) a.out[r] = top == -INFINITY ? -1 : token_of(first);
         return;
     }
     const int top_k = a.top_k ? __ldg(a.top_k + r) : a.top_k_v;
@@ -286,20 +354,291 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
     const float min_p = a.min_p ? __ldg(a.min_p + r) : a.min_p_v;
     const float u = __ldg(a.u + r);
     const bool by_count = top_k > 0 && top_k < a.vocab, by_mass = top_p < 1.f;
-    const Weight w = {1.4426950408889634 / (double)temp, (double)top, top};
-    const double floor_y = min_p > 0.f ? log2((double)fminf(min_p, 1.f)) : -INFINITY;
+    const Weight w = {TABLE * 1.4426950408889634 / (double)temp, (double)top, top};
+    const double floor_z = min_p > 0.f ? TABLE * log2((double)fminf(min_p, 1.f)) : -INFINITY;   // w >= min_p: 128 y from here on
+    // the first sum in units of 2^-43 that exceeds u times the total
+    auto aim = [&](u64 total) -> u64 {
+        const double x = (u > 0.f ? (double)u : 0.0) * (double)total;   // (NaN counts as 0)
+        return x < (double)total ? min((u64)x, total - 1) : total - 1;
+    };
+    // bins of equal width in the logit, from the maximum down
+    float fine = 0.f;
+    auto spread = [&](float span) {
+        span = fminf(top - least, span);
+        fine = span > 0.f ? (float)BINS / span : 0.f;
+    };
+    auto bin_of = [&](float l) -> int {
+        const float d = (top - l) * fine;   // (the maximum at +infinity: NaN for itself, +infinity for others)
+        return l == top ? 0 : d < (float)(BINS - 1) ? (int)d : BINS - 1;
+    };
+    const float mass_span = (float)(MASS_SPAN * TABLE / w.scale);
+    // every CTA's counts of this thread's four bins
+    auto sum_bins = [&](uint32_t (&c4)[4]) {
+        c4[0] = c4[1] = c4[2] = c4[3] = 0;
+        for (int c = 0; c < ranks; ++c) {
+            const uint4 q = peer_ld4(peer(&s.count[4 * tid], c));
+            c4[0] += q.x, c4[1] += q.y, c4[2] += q.z, c4[3] += q.w;
+        }
+    };
+    // a token into the first CTA's list, by whole warps; what does not fit is counted all the same
+    auto hand_in = [&](bool take, u64 key) {
+        const unsigned who = __ballot_sync(0xffffffffu, take);
+        if (!who) return;
+        uint32_t place = 0;
+        const int leader = __ffs((int)who) - 1;
+        if (lane == leader) place = peer_add(peer(&s.taken, 0), __popc(who));
+        place = __shfl_sync(0xffffffffu, place, leader) + __popc(who & ((1u << lane) - 1u));
+        if (take && place < CAP) peer_st(peer(&s.list[place], 0), key);
+    };
+    // the list in descending order (n <= CAP), whose first `top` places are wanted: few by their rank, many by a sort
+    auto arrange = [&](int n) {
+        if (n > 256) {
+            sort_down(s.list, n);
+            return;
+        }
+        const u64 mine = tid < n ? s.list[tid] : 0;
+        int rank_of = 0;
+        for (int i = 0; i < n; ++i) rank_of += s.list[i] > mine;
+        __syncthreads();
+        if (tid < n) s.list[rank_of] = mine;
+        __syncthreads();
+    };
+
+    if (NEAR && by_count && top_k <= FEW) {
+        // ---- few tokens: the first CTA takes them ----
+        spread(COUNT_SPAN);
+        for (int i = tid; i < BINS; i += NT) s.count[i] = 0;
+        __syncthreads();
+        if (own_best > -INFINITY) atomicAdd(&s.count[bin_of(own_best)], 1u);
+        if (ranks > 1) cluster_sync();
+        else __syncthreads();
+        uint32_t c4[4], total;
+        sum_bins(c4);
+        uint32_t before = block_scan<uint32_t>(c4[0] + c4[1] + c4[2] + c4[3], s.warp_sum, &total);
+        if (tid == 0) s.found[0] = BINS - 1;   // fewer threads with a token than top_k: every token
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (before < (uint32_t)top_k && (uint32_t)top_k <= before + c4[k]) s.found[0] = 4 * tid + k;
+            before += c4[k];
+        }
+        __syncthreads();
+        const int bin = (int)s.found[0];
+        // (a token of the bin is not below this; the bin itself decides)
+        const float low = bin == BINS - 1 || fine == 0.f ? -3.402823466e38f : top - (float)(bin + 2) / fine;
+        each(low, [&](float l, int i) { hand_in(l > -INFINITY && bin_of(l) <= bin, place_key(l, lo + i)); });
+        if (ranks > 1) cluster_sync();
+        else __syncthreads();
+        const uint32_t listed = rank == 0 ? (uint32_t)s.taken : peer_ld(peer(&s.taken, 0));
+        if (ranks > 1) cluster_sync();   // (the count is read by all before the first CTA goes on)
+        if (listed <= CAP) {
+            if (rank) return;
+            arrange((int)listed);
+            const int kept = min(top_k, (int)listed);
+            // weights, a token to a thread; those before which less than top_p lies; those of min_p or more
+            const float l = tid < kept ? logit_of(s.list[tid]) : 0.f;
+            const double z = w.place(l);
+            const u64 mass = tid < kept ? w.of(z, s.two_to) : 0;
+            u64 sum, lies = block_scan<u64>(mass, s.warp_sum, &sum);
+            bool stays = tid < kept;
+            if (by_mass) {
+                const double t = (double)top_p * (double)sum;
+                stays = stays && (tid == 0 || (double)lies < t);
+            }
+            stays = stays && z >= floor_z;
+            const int number = tid < kept ? token_of(s.list[tid]) : 0;
+            u64 all;
+            block_scan<u64>(stays ? mass : 0, s.warp_sum, &all);
+            // what stays is the beginning of the list; sums by number, each token for itself
+            u64* masses = reinterpret_cast<u64*>(s.low);
+            masses[tid] = stays ? mass : 0;
+            int* numbers = reinterpret_cast<int*>(s.high);
+            numbers[tid] = number;
+            const int left = __syncthreads_count(stays);
+            const u64 target = aim(all);
+            if (tid < left) {
+                u64 under = 0;
+                for (int i = 0; i < left; ++i) under += numbers[i] < number ? masses[i] : 0;
+                if (under <= target && target < under + mass) a.out[r] = number;
+            }
+            return;
+        }
+    } else if (NEAR && by_mass && !by_count) {
+        // ---- top_p alone ----
+        spread(mass_span);
+        for (int i = tid; i < BINS; i += NT) s.count[i] = 0;
+        __syncthreads();
+        u64 sum = 0;
+        each(-3.402823466e38f, [&](float l, int) {
+            if (l == -INFINITY) return;
+            atomicAdd(&s.count[bin_of(l)], 1u);
+            sum += w.of(l, s.two_to);
+        });
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) s.warp_sum[warp] = sum;
+        __syncthreads();
+        sum = 0;
+        for (int k = 0; k < NW; ++k) sum += s.warp_sum[k];
+        tell(sum, 0, 0, 0);   // (the counts are there, too)
+        u64 all = 0;
+        for (int c = 0; c < ranks; ++c) all += s.slot[turn][c][0];
+        const double t = (double)top_p * (double)all;
+        const u64 target = max(t > 0.0 ? (u64)ceil(t) : 0, 1ull);   // the last token before which less than this lies
+        // The bins in which that token can lie: a bin's weights are between those of its edges (and one bin to the side of
+        // each, for the rounding of the edges).  The last bin has no lower edge.
+        uint32_t c4[4];
+        sum_bins(c4);
+        const double step = fine > 0.f ? exp2(-w.scale / (TABLE * (double)fine)) : 1.0;   // of a bin's weights
+        double edge = fine > 0.f ? exp2(-w.scale * (4.0 * tid) / (TABLE * (double)fine)) * 8796093022208.0 : 8796093022208.0;
+        double most[4], sum4 = 0.0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            most[k] = c4[k] * edge;   // at the upper edge; at the lower one `step` times that
+            sum4 += most[k];
+            edge *= step;
+        }
+        double up_to = block_scan_double(sum4, reinterpret_cast<double*>(s.warp_sum));
+        if (tid == 0) s.found[0] = BINS - 1, s.found[1] = BINS - 1;
+        __syncthreads();
+        int lo_bin = BINS - 1, hi_bin = BINS - 1;
+        const double margin = 1.0 + 1e-5;   // of the sums' own rounding, and the edges'
+#pragma unroll
+        for (int k = 3; k >= 0; --k) {   // (from the last on: the first that qualifies remains)
+            double here = up_to;
+            for (int i = 0; i <= k; ++i) here += most[i];
+            if (here * margin >= (double)target) lo_bin = 4 * tid + k;
+            if (here * step / margin >= (double)target + 1.0 && 4 * tid + k < BINS - 1) hi_bin = 4 * tid + k;
+        }
+        if (lo_bin < BINS - 1) atomicMin(reinterpret_cast<unsigned*>(&s.found[0]), (unsigned)lo_bin);
+        if (hi_bin < BINS - 1) atomicMin(reinterpret_cast<unsigned*>(&s.found[1]), (unsigned)hi_bin);
+        __syncthreads();
+        lo_bin = max((int)(unsigned)s.found[0] - 1, 0);
+        hi_bin = min((int)(unsigned)s.found[1] + 1, BINS - 1);
+        // tokens above those bins stay: their weights, and those of min_p or more by pieces of the row; the bins' own tokens
+        // go to the first CTA.  A piece is a run of quads to a warp.
+        const int piece = ceil_div(quads, NW), q0 = min(quads, warp * piece), q1 = min(quads, q0 + piece);
+        const float low = hi_bin == BINS - 1 || fine == 0.f ? -3.402823466e38f : top - (float)(hi_bin + 2) / fine;
+        u64 above = 0, stay = 0;
+        for (int j = q0 + lane; j < ((q1 - q0 + 31) & ~31) + q0; j += 32) {
+            const float4 q = j < q1 ? reinterpret_cast<const float4*>(near)[j] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (!__any_sync(0xffffffffu, fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) >= low)) continue;
+            const float l4[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int b = bin_of(l4[k]);
+                const bool there = l4[k] > -INFINITY;
+                if (there && b < lo_bin) {
+                    const double z = w.place(l4[k]);
+                    const u64 v = w.of(z, s.two_to);
+                    above += v;
+                    if (z >= floor_z) stay += v;
+                }
+                hand_in(there && b >= lo_bin && b <= hi_bin, place_key(l4[k], lo + 4 * j + k - off));
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            above += __shfl_xor_sync(0xffffffffu, above, o);
+            stay += __shfl_xor_sync(0xffffffffu, stay, o);
+        }
+        if (lane == 0) {
+            s.warp_sum[warp] = above;
+            peer_st(peer(&s.pieces[rank * NW + warp], 0), stay);
+        }
+        __syncthreads();
+        above = 0;
+        for (int k = 0; k < NW; ++k) above += s.warp_sum[k];
+        tell(above, 0, 0, 0);
+        const uint32_t listed = rank == 0 ? (uint32_t)s.taken : peer_ld(peer(&s.taken, 0));
+        u64 before = 0;
+        for (int c = 0; c < ranks; ++c) before += s.slot[turn][c][0];
+        if (listed <= CAP) {   // all CTAs alike
+            if (rank == 0) {
+                arrange((int)listed);
+                // the last token of the list before which less than `target` lies, and the tokens up to it that stay
+                constexpr int EACH = CAP / NT;
+                double z[EACH];
+                u64 v[EACH], mine = 0, total;
+#pragma unroll
+                for (int k = 0; k < EACH; ++k) {
+                    const int i = tid * EACH + k;
+                    z[k] = i < (int)listed ? w.place(logit_of(s.list[i])) : -INFINITY;
+                    v[k] = w.of(z[k], s.two_to);
+                    mine += v[k];
+                }
+                u64 lies = before + block_scan<u64>(mine, s.warp_sum, &total);
+                uint32_t last = 0;
+#pragma unroll
+                for (int k = 0; k < EACH; ++k) {
+                    const int i = tid * EACH + k;
+                    if (i < (int)listed && lies < target) {
+                        last = i + 1;
+                        if (z[k] >= floor_z) {
+                            const int number = token_of(s.list[i]), c = number / a.share;
+                            const int o = (int)((reinterpret_cast<uintptr_t>(row + (long long)c * a.share) & 15) / sizeof(T));
+                            const int in = number - c * a.share + o, all_in = min(a.vocab - c * a.share, a.share) + o;
+                            atomicAdd(&s.pieces[c * NW + in / 4 / ceil_div((all_in + 3) / 4, NW)], v[k]);
+                        }
+                    }
+                    lies += v[k];
+                }
+                last = __reduce_max_sync(0xffffffffu, last);
+                __syncthreads();
+                if (lane == 0) s.warp_sum[warp] = last;
+                __syncthreads();
+                u64 most_at = 1;
+                for (int k = 0; k < NW; ++k) most_at = max(most_at, s.warp_sum[k]);
+                __syncthreads();   // (read by all before the next scan writes there)
+                // the piece in which the token lies
+                const u64 here = tid < ranks * NW ? s.pieces[tid] : 0;
+                u64 left_over;
+                u64 passed = block_scan<u64>(here, s.warp_sum, &left_over);
+                const u64 goal = aim(left_over);
+                if (passed <= goal && goal < passed + here) {
+                    for (int c = 0; c < ranks; ++c) {
+                        peer_st(peer(&s.told[0], c), (u64)tid);
+                        peer_st(peer(&s.told[1], c), goal - passed);
+                        peer_st(peer(&s.told[2], c), listed ? s.list[most_at - 1] : 0);
+                    }
+                }
+            }
+            if (ranks > 1) cluster_sync();
+            else __syncthreads();
+            if ((int)(s.told[0] / NW) != rank) return;
+            const u64 goal = s.told[1], bar = s.told[2];
+            const int p0 = min(quads, (int)(s.told[0] % NW) * piece), p1 = min(quads, p0 + piece);
+            const int per = ceil_div(p1 - p0, NT), j0 = min(p1, p0 + tid * per), j1 = min(p1, j0 + per);
+            auto weight_at = [&](int e) -> u64 {   // of place e among the quads
+                const float l = near[e];
+                if (l == -INFINITY) return 0;
+                // above the bins, or of the bins and not below the border
+                if (place_key(l, lo + e - off) < bar) return 0;
+                const double z = w.place(l);
+                return z >= floor_z ? w.of(z, s.two_to) : 0;
+            };
+            u64 mine = 0, total;
+            for (int e = 4 * j0; e < 4 * j1; ++e) mine += weight_at(e);
+            u64 here = block_scan<u64>(mine, s.warp_sum, &total);
+            if (here <= goal && goal < here + mine)
+                for (int e = 4 * j0; e < 4 * j1; ++e) {
+                    here += weight_at(e);
+                    if (goal < here) {
+                        a.out[r] = lo + e - off;
+                        break;
+                    }
+                }
+            return;
+        }
+    }
+
+    // ---- the general form ----
 
     u64 bar = 0;   // tokens whose key is below this are out
     // The key of the last token that stays: by count the want-th, by mass the last one before which less than top_p of the
     // sum lies.  `before` of it (tokens or weight) has passed when the keys from lo_key to hi_key begin.
     auto border = [&](bool mass, u64 want) -> u64 {
-        // first level: bins of equal width in the logit, from the maximum down
-        const float span = fminf(top - least, mass ? (float)(MASS_SPAN / w.scale) : COUNT_SPAN);
-        const float fine = span > 0.f ? (float)BINS / span : 0.f;
-        auto bin_of = [&](float l) -> int {
-            const float d = (top - l) * fine;   // (the maximum at +infinity: NaN for itself, +infinity for others)
-            return l == top ? 0 : d < (float)(BINS - 1) ? (int)d : BINS - 1;
-        };
+        spread(mass ? mass_span : COUNT_SPAN);
         u64 lo_key = 0, hi_key = ~0ull, before = 0, target = want, count = 0;
         bool first = true;
         int bin = 0, shift = 0;
@@ -459,8 +798,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
     auto weight_at = [&](int i) -> u64 {
         const float l = at(i);
         if (place_key(l, lo + i) < bar) return 0;
-        const double y = w.octaves(l);
-        return y >= floor_y ? w.of(y, s.two_to) : 0;
+        const double z = w.place(l);
+        return z >= floor_z ? w.of(z, s.two_to) : 0;
     };
     const int piece = ceil_div(ceil_div(max(n, 1), NW), 32) * 32, i0 = min(n, warp * piece), i1 = min(n, i0 + piece);
     u64 sum = 0;
@@ -477,16 +816,15 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         if (c == rank) begin = total;
         total += s.slot[turn][c][0];
     }
-    const double aim = (u > 0.f ? (double)u : 0.0) * (double)total;   // (NaN counts as 0)
-    const u64 target = aim < (double)total ? min((u64)aim, total - 1) : total - 1;   // the first sum above it
+    const u64 target = aim(total);
     if (target < begin || target - begin >= mine) return;
     u64 passed = begin;
     int k = 0;
     for (; k < NW - 1 && target >= passed + s.warp_sum[k]; ++k) passed += s.warp_sum[k];
     __syncthreads();
     // the piece, over all threads
-    const int p0 = min(n, k * piece), p1 = min(n, p0 + piece), each = ceil_div(p1 - p0, NT);
-    const int j0 = min(p1, p0 + tid * each), j1 = min(p1, j0 + each);
+    const int p0 = min(n, k * piece), p1 = min(n, p0 + piece), per = ceil_div(p1 - p0, NT);
+    const int j0 = min(p1, p0 + tid * per), j1 = min(p1, j0 + per);
     sum = 0;
     for (int i = j0; i < j1; ++i) sum += weight_at(i);
     u64 all;
@@ -501,8 +839,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         }
 }
 
-size_t smem_of(int share, int size, bool near) {
-    return ((sizeof(Shared) + 15) & ~(size_t)15) + (near ? (size_t)share * size + 32 : 0);
+size_t smem_of(int share, bool near) {
+    return ((sizeof(Shared) + 15) & ~(size_t)15) + (near ? (size_t)share * 4 + 64 : 0);
 }
 
 template <typename T>
@@ -511,8 +849,8 @@ int run(Args a, cudaStream_t st) {
     unsigned ranks = 1;
     while (ranks < MAX_RANKS && a.vocab > 4096 * (int)ranks) ranks *= 2;
     a.share = (ceil_div(a.vocab, (int)ranks) + 7) & ~7;
-    const bool near = smem_of(a.share, sizeof(T), true) <= 220 * 1024;
-    const size_t smem = smem_of(a.share, sizeof(T), near);
+    const bool near = smem_of(a.share, true) <= 220 * 1024;
+    const size_t smem = smem_of(a.share, near);
     static SmemLimit limits[2];
     const auto kernel = near ? sample_kernel<T, true> : sample_kernel<T, false>;
     cudaError_t e = allow_smem(kernel, smem, limits[near]);

@@ -175,6 +175,19 @@ def test_many_draws_of_one_row(sample):
     check(sample, x, torch.rand(1000, device="cuda", generator=g))
 
 
+@pytest.mark.parametrize("rule", [dict(top_p=0.5), dict(top_p=0.9), dict(top_p=0.3, min_p=0.01), dict(top_k=40, top_p=0.9), dict(top_k=700),
+                                  dict()])
+def test_many_rows_many_times(sample, rule):
+    """More clusters than fit the GPU at once, again and again: always the same tokens."""
+    g = gen(12)
+    x, u = rows(g, 64, 151936, torch.float32, 2.0), torch.rand(64, device="cuda", generator=g)
+    x[::9, 7000:] = -math.inf
+    want = sample(x, u, **rule)
+    assert want.tolist() == expect(x, u, **rule)
+    for _ in range(30):
+        assert torch.equal(sample(x, u, **rule), want)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_strides_and_offsets(sample, dtype):
     g = gen(10)

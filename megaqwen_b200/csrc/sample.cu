@@ -130,6 +130,7 @@ struct Shared {
     double two_to[TABLE];             // 2^(j / TABLE)
     u64 pieces[MAX_RANKS * NW];       // sums of the warps' pieces of the row, in the first CTA
     u64 told[4];                      // what the first CTA tells the others
+    u64 ends[2 * NW];                 // the warps' smallest and largest keys
     int taken;
 };
 
@@ -404,6 +405,26 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         __syncthreads();
     };
 
+    // The smallest and the largest of the CTA's keys, for every thread.
+    auto span_of = [&](u64& kl, u64& kh) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            kl = min(kl, __shfl_xor_sync(0xffffffffu, kl, o));
+            kh = max(kh, __shfl_xor_sync(0xffffffffu, kh, o));
+        }
+        if (lane == 0) {
+            s.ends[warp] = kl;
+            s.ends[NW + warp] = kh;
+        }
+        __syncthreads();
+        for (int k = 0; k < NW; ++k) {
+            kl = min(kl, s.ends[k]);
+            kh = max(kh, s.ends[NW + k]);
+        }
+    };
+    bool bracketed = false;   // a border by mass is known to lie between two keys
+    u64 bracket[4] = {0, 0, 0, 0};
+
     if (NEAR && by_count && top_k <= FEW) {
         // ---- few tokens: the first CTA takes them ----
         spread(COUNT_SPAN);
@@ -519,7 +540,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         // go to the first CTA.  A piece is a run of quads to a warp.
         const int piece = ceil_div(quads, NW), q0 = min(quads, warp * piece), q1 = min(quads, q0 + piece);
         const float low = hi_bin == BINS - 1 || fine == 0.f ? -3.402823466e38f : top - (float)(hi_bin + 2) / fine;
-        u64 above = 0, stay = 0;
+        u64 above = 0, stay = 0, kl = ~0ull, kh = 0;   // kl, kh: of the bins' tokens
         for (int j = q0 + lane; j < ((q1 - q0 + 31) & ~31) + q0; j += 32) {
             const float4 q = j < q1 ? reinterpret_cast<const float4*>(near)[j] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
             if (!__any_sync(0xffffffffu, fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) >= low)) continue;
@@ -534,7 +555,10 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
                     above += v;
                     if (z >= floor_z) stay += v;
                 }
-                hand_in(there && b >= lo_bin && b <= hi_bin, place_key(l4[k], lo + 4 * j + k - off));
+                const bool take = there && b >= lo_bin && b <= hi_bin;
+                const u64 key = place_key(l4[k], lo + 4 * j + k - off);
+                if (take) kl = min(kl, key), kh = max(kh, key);
+                hand_in(take, key);
             }
         }
 #pragma unroll
@@ -549,10 +573,17 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         __syncthreads();
         above = 0;
         for (int k = 0; k < NW; ++k) above += s.warp_sum[k];
-        tell(above, 0, 0, 0);
+        span_of(kl, kh);
+        tell(above, kl, kh, 0);
         const uint32_t listed = rank == 0 ? (uint32_t)s.taken : peer_ld(peer(&s.taken, 0));
         u64 before = 0;
-        for (int c = 0; c < ranks; ++c) before += s.slot[turn][c][0];
+        for (int c = 0; c < ranks; ++c) {
+            before += s.slot[turn][c][0];
+            kl = min(kl, s.slot[turn][c][1]);
+            kh = max(kh, s.slot[turn][c][2]);
+        }
+        bracketed = true;
+        bracket[0] = target, bracket[1] = kl, bracket[2] = kh, bracket[3] = before;
         if (listed <= CAP) {   // all CTAs alike
             if (rank == 0) {
                 arrange((int)listed);
@@ -633,23 +664,34 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
     }
 
     // ---- the general form ----
-
     u64 bar = 0;   // tokens whose key is below this are out
-    // The key of the last token that stays: by count the want-th, by mass the last one before which less than top_p of the
-    // sum lies.  `before` of it (tokens or weight) has passed when the keys from lo_key to hi_key begin.
-    auto border = [&](bool mass, u64 want) -> u64 {
-        spread(mass ? mass_span : COUNT_SPAN);
-        u64 lo_key = 0, hi_key = ~0ull, before = 0, target = want, count = 0;
-        bool first = true;
+    // f(logit, place in the share) as `each`, of a row that shared memory holds or not
+    auto scan = [&](float low, auto f) {
+        if (NEAR) {
+            each(low, f);
+        } else {
+            for (int i0 = warp * 32; i0 < n; i0 += NT) f(i0 + lane < n ? at(i0 + lane) : -INFINITY, i0 + lane);
+        }
+    };
+    auto low_of = [&](u64 key) { return key ? logit_of(key) : -3.402823466e38f; };
+    // The key of the last token that stays: by count the want-th, by mass the last one before which less than `want` lies
+    // (0: top_p of the sum).  The range of keys in which it is looked for is cut into bins, from the top down, until a bin's
+    // tokens can be sorted; `before` of the order (tokens or weight) has passed when the range begins.  With `first`, the
+    // range is everything, and the bins are of equal width in the logit.
+    auto border = [&](bool mass, u64 want, bool first_level, u64 lo_key, u64 hi_key, u64 before) -> u64 {
+        if (first_level) spread(mass ? mass_span : COUNT_SPAN);
+        u64 target = want, count = 0;
         int bin = 0, shift = 0;
+        auto cut = [&]() { shift = max(0, 64 - __clzll((long long)(hi_key - lo_key)) - 11); };   // 2048 bins
+        if (!first_level) cut();
         while (true) {
             for (int i = tid; i < BINS; i += NT) s.count[i] = s.low[i] = s.high[i] = 0;
             __syncthreads();
-            for (int i = tid; i < n; i += NT) {
-                const float l = at(i);
+            const u64 from = max(bar, lo_key);
+            scan(low_of(from), [&](float l, int i) {
                 const u64 key = place_key(l, lo + i);
-                if (key < bar || key < lo_key || key > hi_key) continue;
-                const int b = first ? bin_of(l) : (int)((hi_key - key) >> shift);
+                if (l == -INFINITY || key < from || key > hi_key) return;
+                const int b = first_level ? bin_of(l) : (int)((hi_key - key) >> shift);
                 atomicAdd(&s.count[b], 1u);
                 if (mass) {
                     const u64 v = w.of(l, s.two_to);
@@ -659,32 +701,31 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
                         if (hi32) atomicAdd(&s.high[b], hi32);
                     }
                 }
-            }
+            });
             if (ranks > 1) cluster_sync();
             else __syncthreads();
             // four bins to a thread, over all CTAs
-            uint32_t c4[4] = {0, 0, 0, 0};
-            u64 m4[4] = {0, 0, 0, 0};
-            for (int c = 0; c < ranks; ++c) {
-                const uint4 q = peer_ld4(peer(&s.count[4 * tid], c));
-                c4[0] += q.x, c4[1] += q.y, c4[2] += q.z, c4[3] += q.w;
-                if (mass) {
+            uint32_t c4[4];
+            sum_bins(c4);
+            u64 m4[4] = {c4[0], c4[1], c4[2], c4[3]};
+            if (mass) {
+                m4[0] = m4[1] = m4[2] = m4[3] = 0;
+                for (int c = 0; c < ranks; ++c) {
                     const uint4 l = peer_ld4(peer(&s.low[4 * tid], c)), h = peer_ld4(peer(&s.high[4 * tid], c));
                     m4[0] += (u64)h.x << 32 | l.x, m4[1] += (u64)h.y << 32 | l.y;
                     m4[2] += (u64)h.z << 32 | l.z, m4[3] += (u64)h.w << 32 | l.w;
                 }
             }
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (!mass) m4[k] = c4[k];
             u64 total;
             u64 at_bin = before + block_scan<u64>(m4[0] + m4[1] + m4[2] + m4[3], s.warp_sum, &total);
-            if (mass && first) {
-                // a token stays while less than top_p of the sum lies before it: the border is the last one before which
-                // less than `target` units lie
+            if (!mass && before + total < target) {   // fewer tokens than that: all stay
+                if (ranks > 1) cluster_sync();        // (the counts are read by all before they are cleared again)
+                else __syncthreads();
+                return bar;
+            }
+            if (mass && !target) {
                 const double t = (double)top_p * (double)total;
-                target = t > 0.0 ? (u64)ceil(t) : 0;
-                target = max(target, 1ull);
+                target = max(t > 0.0 ? (u64)ceil(t) : 0, 1ull);
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -700,31 +741,21 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
             before = s.found[1];
             count = s.found[2];
             __syncthreads();
+            if (!first_level) {
+                hi_key -= (u64)bin << shift;
+                lo_key = max(lo_key, hi_key - ((1ull << shift) - 1));
+            }
             if (count <= CAP) break;
             // too many: the keys of the bin, cut again
-            if (first) {
+            if (first_level) {
                 u64 kl = ~0ull, kh = 0;
-                for (int i = tid; i < n; i += NT) {
-                    const float l = at(i);
+                scan(low_of(bar), [&](float l, int i) {
                     const u64 key = place_key(l, lo + i);
-                    if (key < bar || bin_of(l) != bin) continue;
+                    if (l == -INFINITY || key < bar || bin_of(l) != bin) return;
                     kl = min(kl, key);
                     kh = max(kh, key);
-                }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    kl = min(kl, __shfl_xor_sync(0xffffffffu, kl, o));
-                    kh = max(kh, __shfl_xor_sync(0xffffffffu, kh, o));
-                }
-                if (lane == 0) {
-                    s.warp_sum[warp] = kl;
-                    s.list[warp] = kh;
-                }
-                __syncthreads();
-                for (int k = 0; k < NW; ++k) {
-                    kl = min(kl, s.warp_sum[k]);
-                    kh = max(kh, s.list[k]);
-                }
+                });
+                span_of(kl, kh);
                 tell(kl, kh, 0, 0);
                 lo_key = ~0ull;
                 hi_key = 0;
@@ -732,34 +763,27 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
                     lo_key = min(lo_key, s.slot[turn][c][0]);
                     hi_key = max(hi_key, s.slot[turn][c][1]);
                 }
-            } else {
-                hi_key -= (u64)bin << shift;
-                lo_key = max(lo_key, hi_key - ((1ull << shift) - 1));
-                if (ranks > 1) cluster_sync();   // the counts are read before they are cleared
+                first_level = false;
+            } else if (ranks > 1) {
+                cluster_sync();   // the counts are read before they are cleared
             }
-            first = false;
-            const u64 range = hi_key - lo_key;
-            shift = max(0, 64 - __clzll((long long)range) - 11);   // 2048 bins
+            cut();
         }
         // the bin's tokens, in every CTA's list
-        if (!first) {
-            hi_key -= (u64)bin << shift;
-            lo_key = max(lo_key, hi_key - ((1ull << shift) - 1));
-        }
         uint32_t base = 0;
         for (int c = 0; c < rank; ++c) base += peer_ld(peer(&s.count[bin], c));
         if (tid == 0) s.taken = 0;
         __syncthreads();
-        for (int i = tid; i < n; i += NT) {
-            const float l = at(i);
+        const u64 from = max(bar, lo_key);
+        scan(low_of(from), [&](float l, int i) {
             const u64 key = place_key(l, lo + i);
-            if (key < bar || key < lo_key || key > hi_key || (first && bin_of(l) != bin)) continue;
+            if (l == -INFINITY || key < from || key > hi_key || (first_level && bin_of(l) != bin)) return;
             const uint32_t place = base + atomicAdd(&s.taken, 1);
             for (int c = 0; c < ranks; ++c) peer_st(peer(&s.list[place], c), key);
-        }
+        });
         if (ranks > 1) cluster_sync();
         else __syncthreads();
-        sort_down(s.list, (int)count);
+        arrange((int)count);
         if (!mass) {
             const u64 key = s.list[target - before - 1];
             __syncthreads();
@@ -791,19 +815,34 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         __syncthreads();
         return key;
     };
-    if (by_count) bar = border(false, (u64)top_k);
-    if (by_mass) bar = border(true, 0);
+    if (bracketed) {
+        bar = border(true, bracket[0], false, bracket[1], bracket[2], bracket[3]);
+    } else {
+        if (by_count) bar = border(false, (u64)top_k, true, 0, ~0ull, 0);
+        if (by_mass) bar = border(true, 0, true, 0, ~0ull, 0);
+    }
 
-    // the sums of what stays, in the order of the tokens: a contiguous piece to a warp
-    auto weight_at = [&](int i) -> u64 {
+    // the sums of what stays, in the order of the tokens: a run of the share to a warp
+    const int units = NEAR ? quads : ceil_div(n, 4), lead = NEAR ? off : 0;   // of four places each
+    const float low = low_of(bar);
+    auto weight_at = [&](int e) -> u64 {   // of place e
+        const int i = e - lead;
+        if (i < 0 || i >= n) return 0;
         const float l = at(i);
-        if (place_key(l, lo + i) < bar) return 0;
+        if (!(l >= low) || place_key(l, lo + i) < bar) return 0;
         const double z = w.place(l);
         return z >= floor_z ? w.of(z, s.two_to) : 0;
     };
-    const int piece = ceil_div(ceil_div(max(n, 1), NW), 32) * 32, i0 = min(n, warp * piece), i1 = min(n, i0 + piece);
+    const int piece = ceil_div(units, NW), q0 = min(units, warp * piece), q1 = min(units, q0 + piece);
     u64 sum = 0;
-    for (int i = i0 + lane; i < i1; i += 32) sum += weight_at(i);
+    for (int j = q0 + lane; j < q1; j += 32) {
+        if (NEAR) {
+            const float4 q = reinterpret_cast<const float4*>(near)[j];
+            if (!(fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) >= low)) continue;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum += weight_at(4 * j + k);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s.warp_sum[warp] = sum;
@@ -822,18 +861,18 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
     int k = 0;
     for (; k < NW - 1 && target >= passed + s.warp_sum[k]; ++k) passed += s.warp_sum[k];
     __syncthreads();
-    // the piece, over all threads
-    const int p0 = min(n, k * piece), p1 = min(n, p0 + piece), per = ceil_div(p1 - p0, NT);
+    // the run, over all threads
+    const int p0 = 4 * min(units, k * piece), p1 = 4 * min(units, (k + 1) * piece), per = ceil_div(p1 - p0, NT);
     const int j0 = min(p1, p0 + tid * per), j1 = min(p1, j0 + per);
     sum = 0;
-    for (int i = j0; i < j1; ++i) sum += weight_at(i);
+    for (int e = j0; e < j1; ++e) sum += weight_at(e);
     u64 all;
     u64 here = passed + block_scan<u64>(sum, s.warp_sum, &all);
     if (here <= target && target < here + sum)
-        for (int i = j0; i < j1; ++i) {
-            here += weight_at(i);
+        for (int e = j0; e < j1; ++e) {
+            here += weight_at(e);
             if (target < here) {
-                a.out[r] = lo + i;
+                a.out[r] = lo + e - lead;
                 break;
             }
         }

@@ -50,11 +50,12 @@ using u64 = unsigned long long;
 
 constexpr int NT = 512, NW = NT / 32;
 constexpr int BINS = 2048;          // four to a thread
-constexpr int CAP = 1024;           // tokens that are sorted
-constexpr int FEW = 512;            // the largest top_k whose tokens one CTA takes
+constexpr int CAP = 4096;           // tokens that are sorted
+constexpr int FEW = 2048;           // the largest top_k whose tokens one CTA takes
 constexpr int MAX_RANKS = 8;
 constexpr int TABLE = 128;          // of 2^(j / TABLE)
 constexpr int FRAC = 43;            // a weight of 1 is 2^43
+constexpr double ONE = 8796093022208.0;
 constexpr int MAX_VOCAB = 1 << 20;  // a row's sum stays below 2^63
 constexpr float COUNT_SPAN = 40.f;  // logits below the maximum that the histogram of a count spreads over its bins
 constexpr double MASS_SPAN = 44.0;  // octaves below the maximum past which a weight is nothing
@@ -140,18 +141,24 @@ struct Weight {
     double scale, top;   // 128 log2(e) / T; the maximum
     float max;
     __device__ __forceinline__ double place(float l) const { return l == max ? 0.0 : ((double)l - top) * scale; }   // 128 y
-    __device__ __forceinline__ u64 of(double z, const double* two_to) const {
-        if (!(z > -(FRAC + 1.0) * TABLE)) return 0;
+    // 2^(z / 128), z <= 0; what is below 2^-1000 is 0
+    __device__ __forceinline__ double as_double(double z, const double* two_to) const {
+        if (!(z > -1000.0 * TABLE)) return 0.0;
         constexpr double MAGIC = 6755399441055744.0;   // 1.5 x 2^52: rounds to whole numbers
         const double t = z + MAGIC, r = z - (t - MAGIC);
         const int n = __double2loint(t);
-        double p = 3.583032305400251e-11;             // (ln(2) / 128)^k / k!
+        double p = 3.583032305400251e-11;              // (ln(2) / 128)^k / k!
         p = fma(p, r, 2.6466421444330967e-08);
         p = fma(p, r, 1.4662262387640423e-05);
         p = fma(p, r, 5.4152123481245725e-03);
         p = fma(p, r, 1.0) * two_to[n & (TABLE - 1)];
-        const u64 b = (u64)__double_as_longlong(p);
-        const int s = 52 - FRAC - ((int)(b >> 52) - 1023) - (n >> 7);   // 9 or more: rounded to the nearest
+        return __hiloint2double(__double2hiint(p) + (n >> 7) * (1 << 20), __double2loint(p));
+    }
+    // in multiples of 2^-43, rounded to the nearest
+    __device__ __forceinline__ u64 of(double z, const double* two_to) const {
+        if (!(z > -(FRAC + 1.0) * TABLE)) return 0;
+        const u64 b = (u64)__double_as_longlong(as_double(z, two_to));
+        const int s = 52 - FRAC - ((int)(b >> 52) - 1023);
         return ((b & 0xfffffffffffffull | 1ull << 52) + (1ull << (s - 1))) >> s;
     }
     __device__ __forceinline__ u64 of(float l, const double* two_to) const { return of(place(l), two_to); }
@@ -181,6 +188,16 @@ __device__ __forceinline__ V block_scan(V v, u64* sm, V* total) {
     return before + x - v;
 }
 
+__device__ __forceinline__ int block_sum_of(int v, u64* sm) {
+    v = (int)__reduce_add_sync(0xffffffffu, (unsigned)v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = (u64)v;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < NW; ++w) all += (int)sm[w];
+    __syncthreads();
+    return all;
+}
 // The same for an estimate.
 __device__ __forceinline__ double block_scan_double(double v, double* sm) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -291,13 +308,28 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
     }
     const float own_best = best;   // this thread's
     auto at = [&](int i) -> float { return NEAR ? near[off + i] : clean(up(__ldg(x + i))); };
+    // Places 4 j .. 4 j + 3 of the share, of which the first `off` lie before it: minus infinity there and behind the end.
+    auto quad = [&](int j) -> float4 {
+        if (NEAR) return reinterpret_cast<const float4*>(near)[j];
+        const int i = 4 * j - off;
+        if (i >= 0 && i + 4 <= n) {
+            if (sizeof(T) == 4) {
+                const float4 q = __ldg(reinterpret_cast<const float4*>(x + i));
+                return make_float4(clean(q.x), clean(q.y), clean(q.z), clean(q.w));
+            }
+            const uint2 q = __ldg(reinterpret_cast<const uint2*>(x + i));
+            const T* e = reinterpret_cast<const T*>(&q);
+            return make_float4(clean(up(e[0])), clean(up(e[1])), clean(up(e[2 % (8 / sizeof(T))])), clean(up(e[3 % (8 / sizeof(T))])));
+        }
+        auto one = [&](int k) { return i + k >= 0 && i + k < n ? clean(up(__ldg(x + i + k))) : -INFINITY; };
+        return make_float4(one(0), one(1), one(2), one(3));
+    };
     // f(logit, place in the share) for every token, four of a thread at a time, where any of a warp's is `low` or more; by
-    // whole warps, with minus infinity behind the end
+    // whole warps, with minus infinity where there is none
     auto each = [&](float low, auto f) {
-        const float4* q4 = reinterpret_cast<const float4*>(near);
         for (int j0 = warp * 32; j0 < quads; j0 += NT) {
             const int j = j0 + lane;
-            const float4 q = j < quads ? q4[j] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            const float4 q = j < quads ? quad(j) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
             if (!__any_sync(0xffffffffu, fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) >= low)) continue;
             const int i = 4 * j - off;
             f(q.x, i);
@@ -425,12 +457,18 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
     bool bracketed = false;   // a border by mass is known to lie between two keys
     u64 bracket[4] = {0, 0, 0, 0};
 
-    if (NEAR && by_count && top_k <= FEW) {
+    if (by_count && top_k <= FEW) {
         // ---- few tokens: the first CTA takes them ----
         spread(COUNT_SPAN);
         for (int i = tid; i < BINS; i += NT) s.count[i] = 0;
         __syncthreads();
-        if (own_best > -INFINITY) atomicAdd(&s.count[bin_of(own_best)], 1u);
+        if (2 * top_k <= NT * ranks) {   // the threads' own maxima: top_k of them reach the bound, and so do that many tokens
+            if (own_best > -INFINITY) atomicAdd(&s.count[bin_of(own_best)], 1u);
+        } else {
+            each(-3.402823466e38f, [&](float l, int) {
+                if (l > -INFINITY) atomicAdd(&s.count[bin_of(l)], 1u);
+            });
+        }
         if (ranks > 1) cluster_sync();
         else __syncthreads();
         uint32_t c4[4], total;
@@ -456,62 +494,95 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
             if (rank) return;
             arrange((int)listed);
             const int kept = min(top_k, (int)listed);
-            // weights, a token to a thread; those before which less than top_p lies; those of min_p or more
-            const float l = tid < kept ? logit_of(s.list[tid]) : 0.f;
-            const double z = w.place(l);
-            const u64 mass = tid < kept ? w.of(z, s.two_to) : 0;
-            u64 sum, lies = block_scan<u64>(mass, s.warp_sum, &sum);
-            bool stays = tid < kept;
-            if (by_mass) {
-                const double t = (double)top_p * (double)sum;
-                stays = stays && (tid == 0 || (double)lies < t);
+            // weights; the tokens before which less than top_p lies; those of min_p or more: each a beginning of the list
+            u64* masses = reinterpret_cast<u64*>(s.low);   // [FEW], over the sums (which no one reads now)
+            constexpr int EACH = FEW / NT;
+            u64 sum = 0;
+            int left = 0;
+            for (int i = tid; i < kept; i += NT) {
+                const double z = w.place(logit_of(s.list[i]));
+                masses[i] = w.of(z, s.two_to);
+                left += z >= floor_z;
             }
-            stays = stays && z >= floor_z;
-            const int number = tid < kept ? token_of(s.list[tid]) : 0;
-            u64 all;
-            block_scan<u64>(stays ? mass : 0, s.warp_sum, &all);
-            // what stays is the beginning of the list; sums by number, each token for itself
-            u64* masses = reinterpret_cast<u64*>(s.low);
-            masses[tid] = stays ? mass : 0;
-            int* numbers = reinterpret_cast<int*>(s.high);
-            numbers[tid] = number;
-            const int left = __syncthreads_count(stays);
+            left = block_sum_of(left, s.warp_sum);
+            const int i0 = tid * EACH;
+            u64 v[EACH], all;
+#pragma unroll
+            for (int k = 0; k < EACH; ++k) {
+                v[k] = i0 + k < kept ? masses[i0 + k] : 0;
+                sum += v[k];
+            }
+            u64 lies = block_scan<u64>(sum, s.warp_sum, &all);
+            if (by_mass) {
+                const double t = (double)top_p * (double)all;
+                int in = 0;
+#pragma unroll
+                for (int k = 0; k < EACH; ++k) {
+                    in += i0 + k < kept && (i0 + k == 0 || (double)lies < t);
+                    lies += v[k];
+                }
+                left = min(left, block_sum_of(in, s.warp_sum));
+            }
+            // what stays, by number
+            sum = 0;
+#pragma unroll
+            for (int k = 0; k < EACH; ++k) sum += i0 + k < left ? v[k] : 0;
+            block_scan<u64>(sum, s.warp_sum, &all);
             const u64 target = aim(all);
-            if (tid < left) {
-                u64 under = 0;
-                for (int i = 0; i < left; ++i) under += numbers[i] < number ? masses[i] : 0;
-                if (under <= target && target < under + mass) a.out[r] = number;
+            if (left <= 256) {   // each token sums the ones of lower numbers for itself
+                if (tid < left) {
+                    const int number = token_of(s.list[tid]);
+                    u64 under = 0;
+                    for (int i = 0; i < left; ++i) under += token_of(s.list[i]) < number ? masses[i] : 0;
+                    if (under <= target && target < under + masses[tid]) a.out[r] = number;
+                }
+                return;
+            }
+            for (int i = tid; i < left; i += NT) s.list[i] = (u64)(uint32_t)s.list[i] << 32 | (uint32_t)i;   // (a key's low word is ~number)
+            sort_down(s.list, left);
+            sum = 0;
+#pragma unroll
+            for (int k = 0; k < EACH; ++k) {
+                v[k] = i0 + k < left ? masses[(uint32_t)s.list[i0 + k]] : 0;
+                sum += v[k];
+            }
+            u64 here = block_scan<u64>(sum, s.warp_sum, &all);
+#pragma unroll
+            for (int k = 0; k < EACH; ++k) {
+                if (here <= target && target < here + v[k]) a.out[r] = (int)~(uint32_t)(s.list[i0 + k] >> 32);
+                here += v[k];
             }
             return;
         }
-    } else if (NEAR && by_mass && !by_count) {
+    } else if (by_mass && !by_count) {
         // ---- top_p alone ----
         spread(mass_span);
         for (int i = tid; i < BINS; i += NT) s.count[i] = 0;
         __syncthreads();
-        u64 sum = 0;
+        // (the total in 64-bit floating point, in an order of its own, the same on every run)
+        double sum = 0.0;
         each(-3.402823466e38f, [&](float l, int) {
             if (l == -INFINITY) return;
             atomicAdd(&s.count[bin_of(l)], 1u);
-            sum += w.of(l, s.two_to);
+            sum += w.as_double(w.place(l), s.two_to);
         });
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) s.warp_sum[warp] = sum;
+        if (lane == 0) s.warp_sum[warp] = (u64)__double_as_longlong(sum);
         __syncthreads();
-        sum = 0;
-        for (int k = 0; k < NW; ++k) sum += s.warp_sum[k];
-        tell(sum, 0, 0, 0);   // (the counts are there, too)
-        u64 all = 0;
-        for (int c = 0; c < ranks; ++c) all += s.slot[turn][c][0];
-        const double t = (double)top_p * (double)all;
+        sum = 0.0;
+        for (int k = 0; k < NW; ++k) sum += __longlong_as_double((long long)s.warp_sum[k]);
+        tell((u64)__double_as_longlong(sum), 0, 0, 0);   // (the counts are there, too)
+        sum = 0.0;
+        for (int c = 0; c < ranks; ++c) sum += __longlong_as_double((long long)s.slot[turn][c][0]);
+        const double t = (double)top_p * sum * ONE;
         const u64 target = max(t > 0.0 ? (u64)ceil(t) : 0, 1ull);   // the last token before which less than this lies
-        // The bins in which that token can lie: a bin's weights are between those of its edges (and one bin to the side of
-        // each, for the rounding of the edges).  The last bin has no lower edge.
+        // The bins in which that token can lie: a bin's weights are between those of its edges.  The last bin has no lower edge.
         uint32_t c4[4];
         sum_bins(c4);
-        const double step = fine > 0.f ? exp2(-w.scale / (TABLE * (double)fine)) : 1.0;   // of a bin's weights
-        double edge = fine > 0.f ? exp2(-w.scale * (4.0 * tid) / (TABLE * (double)fine)) * 8796093022208.0 : 8796093022208.0;
+        const float octaves = fine > 0.f ? (float)w.scale / TABLE / fine : 0.f;   // of a bin
+        const double step = exp2f(-octaves);                                      // of a bin's weights
+        double edge = exp2f(-octaves * (4.f * tid)) * ONE;
         double most[4], sum4 = 0.0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -523,7 +594,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         if (tid == 0) s.found[0] = BINS - 1, s.found[1] = BINS - 1;
         __syncthreads();
         int lo_bin = BINS - 1, hi_bin = BINS - 1;
-        const double margin = 1.0 + 1e-5;   // of the sums' own rounding, and the edges'
+        // of the sums' rounding and of the edges' (fp32: 44 octaves to 2^-24 of them, 2^-18 of a weight)
+        const double margin = 1.0 + 2e-5;
 #pragma unroll
         for (int k = 3; k >= 0; --k) {   // (from the last on: the first that qualifies remains)
             double here = up_to;
@@ -534,15 +606,15 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         if (lo_bin < BINS - 1) atomicMin(reinterpret_cast<unsigned*>(&s.found[0]), (unsigned)lo_bin);
         if (hi_bin < BINS - 1) atomicMin(reinterpret_cast<unsigned*>(&s.found[1]), (unsigned)hi_bin);
         __syncthreads();
-        lo_bin = max((int)(unsigned)s.found[0] - 1, 0);
-        hi_bin = min((int)(unsigned)s.found[1] + 1, BINS - 1);
+        lo_bin = (int)(unsigned)s.found[0];
+        hi_bin = (int)(unsigned)s.found[1];
         // tokens above those bins stay: their weights, and those of min_p or more by pieces of the row; the bins' own tokens
         // go to the first CTA.  A piece is a run of quads to a warp.
         const int piece = ceil_div(quads, NW), q0 = min(quads, warp * piece), q1 = min(quads, q0 + piece);
         const float low = hi_bin == BINS - 1 || fine == 0.f ? -3.402823466e38f : top - (float)(hi_bin + 2) / fine;
         u64 above = 0, stay = 0, kl = ~0ull, kh = 0;   // kl, kh: of the bins' tokens
         for (int j = q0 + lane; j < ((q1 - q0 + 31) & ~31) + q0; j += 32) {
-            const float4 q = j < q1 ? reinterpret_cast<const float4*>(near)[j] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            const float4 q = j < q1 ? quad(j) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
             if (!__any_sync(0xffffffffu, fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) >= low)) continue;
             const float l4[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -641,7 +713,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
             const int p0 = min(quads, (int)(s.told[0] % NW) * piece), p1 = min(quads, p0 + piece);
             const int per = ceil_div(p1 - p0, NT), j0 = min(p1, p0 + tid * per), j1 = min(p1, j0 + per);
             auto weight_at = [&](int e) -> u64 {   // of place e among the quads
-                const float l = near[e];
+                const float l = e >= off && e - off < n ? at(e - off) : -INFINITY;
                 if (l == -INFINITY) return 0;
                 // above the bins, or of the bins and not below the border
                 if (place_key(l, lo + e - off) < bar) return 0;
@@ -665,14 +737,6 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
 
     // ---- the general form ----
     u64 bar = 0;   // tokens whose key is below this are out
-    // f(logit, place in the share) as `each`, of a row that shared memory holds or not
-    auto scan = [&](float low, auto f) {
-        if (NEAR) {
-            each(low, f);
-        } else {
-            for (int i0 = warp * 32; i0 < n; i0 += NT) f(i0 + lane < n ? at(i0 + lane) : -INFINITY, i0 + lane);
-        }
-    };
     auto low_of = [&](u64 key) { return key ? logit_of(key) : -3.402823466e38f; };
     // The key of the last token that stays: by count the want-th, by mass the last one before which less than `want` lies
     // (0: top_p of the sum).  The range of keys in which it is looked for is cut into bins, from the top down, until a bin's
@@ -688,7 +752,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
             for (int i = tid; i < BINS; i += NT) s.count[i] = s.low[i] = s.high[i] = 0;
             __syncthreads();
             const u64 from = max(bar, lo_key);
-            scan(low_of(from), [&](float l, int i) {
+            each(low_of(from), [&](float l, int i) {
                 const u64 key = place_key(l, lo + i);
                 if (l == -INFINITY || key < from || key > hi_key) return;
                 const int b = first_level ? bin_of(l) : (int)((hi_key - key) >> shift);
@@ -749,7 +813,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
             // too many: the keys of the bin, cut again
             if (first_level) {
                 u64 kl = ~0ull, kh = 0;
-                scan(low_of(bar), [&](float l, int i) {
+                each(low_of(bar), [&](float l, int i) {
                     const u64 key = place_key(l, lo + i);
                     if (l == -INFINITY || key < bar || bin_of(l) != bin) return;
                     kl = min(kl, key);
@@ -775,7 +839,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         if (tid == 0) s.taken = 0;
         __syncthreads();
         const u64 from = max(bar, lo_key);
-        scan(low_of(from), [&](float l, int i) {
+        each(low_of(from), [&](float l, int i) {
             const u64 key = place_key(l, lo + i);
             if (l == -INFINITY || key < from || key > hi_key || (first_level && bin_of(l) != bin)) return;
             const uint32_t place = base + atomicAdd(&s.taken, 1);
@@ -823,25 +887,27 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
     }
 
     // the sums of what stays, in the order of the tokens: a run of the share to a warp
-    const int units = NEAR ? quads : ceil_div(n, 4), lead = NEAR ? off : 0;   // of four places each
     const float low = low_of(bar);
     auto weight_at = [&](int e) -> u64 {   // of place e
-        const int i = e - lead;
+        const int i = e - off;
         if (i < 0 || i >= n) return 0;
         const float l = at(i);
         if (!(l >= low) || place_key(l, lo + i) < bar) return 0;
         const double z = w.place(l);
         return z >= floor_z ? w.of(z, s.two_to) : 0;
     };
-    const int piece = ceil_div(units, NW), q0 = min(units, warp * piece), q1 = min(units, q0 + piece);
+    const int piece = ceil_div(quads, NW), q0 = min(quads, warp * piece), q1 = min(quads, q0 + piece);
     u64 sum = 0;
     for (int j = q0 + lane; j < q1; j += 32) {
-        if (NEAR) {
-            const float4 q = reinterpret_cast<const float4*>(near)[j];
-            if (!(fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) >= low)) continue;
-        }
+        const float4 q = quad(j);
+        if (!(fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) >= low)) continue;
+        const float l4[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sum += weight_at(4 * j + k);
+        for (int k = 0; k < 4; ++k) {
+            if (!(l4[k] >= low) || place_key(l4[k], lo + 4 * j + k - off) < bar) continue;
+            const double z = w.place(l4[k]);
+            if (z >= floor_z) sum += w.of(z, s.two_to);
+        }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -862,7 +928,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
     for (; k < NW - 1 && target >= passed + s.warp_sum[k]; ++k) passed += s.warp_sum[k];
     __syncthreads();
     // the run, over all threads
-    const int p0 = 4 * min(units, k * piece), p1 = 4 * min(units, (k + 1) * piece), per = ceil_div(p1 - p0, NT);
+    const int p0 = 4 * min(quads, k * piece), p1 = 4 * min(quads, (k + 1) * piece), per = ceil_div(p1 - p0, NT);
     const int j0 = min(p1, p0 + tid * per), j1 = min(p1, j0 + per);
     sum = 0;
     for (int e = j0; e < j1; ++e) sum += weight_at(e);
@@ -872,7 +938,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         for (int e = j0; e < j1; ++e) {
             here += weight_at(e);
             if (target < here) {
-                a.out[r] = lo + e - lead;
+                a.out[r] = lo + e - off;
                 break;
             }
         }
@@ -884,11 +950,16 @@ size_t smem_of(int share, bool near) {
 
 template <typename T>
 int run(Args a, cudaStream_t st) {
-    // as many CTAs to a row as leave each 4096 tokens or more
+    // As many CTAs to a row (a power of two) as all rows have room for at once, two to an SM, and as leave each 4096 tokens
+    // or more: a CTA does the last steps of its row alone, so with more of them most would wait (256 rows of 152k in bf16:
+    // REPLACE).  The share stays in shared memory where that keeps all CTAs resident; otherwise the passes read it
+    // from L2 (64 rows of 152k in fp32: REPLACE).
+    const int sms = sm_count();
     unsigned ranks = 1;
-    while (ranks < MAX_RANKS && a.vocab > 4096 * (int)ranks) ranks *= 2;
+    while (ranks < MAX_RANKS && a.vocab > 4096 * (int)ranks && (long long)a.n * ranks * 2 <= 2 * sms) ranks *= 2;
     a.share = (ceil_div(a.vocab, (int)ranks) + 7) & ~7;
-    const bool near = smem_of(a.share, true) <= 220 * 1024;
+    const size_t held = smem_of(a.share, true);
+    const bool near = held <= 220 * 1024 && (long long)a.n * ranks <= (held <= 112 * 1024 ? 2ll : 1ll) * sms;
     const size_t smem = smem_of(a.share, near);
     static SmemLimit limits[2];
     const auto kernel = near ? sample_kernel<T, true> : sample_kernel<T, false>;

@@ -41,7 +41,6 @@ using paged::allow_smem;
 using paged::ceil_div;
 using paged::cluster_rank;
 using paged::cluster_size;
-using paged::cluster_sync;
 using paged::launch_cluster;
 using paged::SmemLimit;
 using paged::sm_count;
@@ -50,8 +49,8 @@ using u64 = unsigned long long;
 
 constexpr int NT = 512, NW = NT / 32;
 constexpr int BINS = 2048;          // four to a thread
-constexpr int CAP = 4096;           // tokens that are sorted
-constexpr int FEW = 2048;           // the largest top_k whose tokens one CTA takes
+constexpr int CAP = 2048;           // tokens that are sorted
+constexpr int FEW = 1024;           // the largest top_k whose tokens one CTA takes
 constexpr int MAX_RANKS = 8;
 constexpr int TABLE = 128;          // of 2^(j / TABLE)
 constexpr int FRAC = 43;            // a weight of 1 is 2^43
@@ -74,14 +73,18 @@ struct Args {
     int* out;
 };
 
+// Two 16-bit values of a word (no word holds two of fp32, and none is asked for).
 template <typename T>
-__device__ __forceinline__ float up(T x);
-template <>
-__device__ __forceinline__ float up(float x) { return x; }
-template <>
-__device__ __forceinline__ float up(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <>
-__device__ __forceinline__ float up(__half x) { return __half2float(x); }
+__device__ __forceinline__ float2 two_up(uint32_t w) {
+    if (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return make_float2(bf16lo(w), bf16hi(w));
+}
+
+template <typename T>
+__device__ __forceinline__ float load_one(const T* p) {
+    if (sizeof(T) == 4) return __ldg(reinterpret_cast<const float*>(p));
+    return two_up<T>(__ldg(reinterpret_cast<const unsigned short*>(p))).x;
+}
 
 __device__ __forceinline__ uint32_t order_key(float x) {
     const uint32_t b = __float_as_uint(x);
@@ -92,6 +95,12 @@ __device__ __forceinline__ int token_of(u64 key) { return (int)~(uint32_t)key; }
 __device__ __forceinline__ float logit_of(u64 key) {
     const uint32_t k = (uint32_t)(key >> 32);
     return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
+// The cluster's barrier, for warps whose threads may come to it one by one (loops and branches lie before it).
+__device__ __forceinline__ void cluster_meet() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // Remote shared memory of the cluster.
@@ -123,8 +132,12 @@ __device__ __forceinline__ uint32_t peer_add(uint32_t at, uint32_t v) {
 // What a CTA needs beside its share of the row.
 struct Shared {
     uint32_t count[BINS];             // of this CTA
-    uint32_t low[BINS], high[BINS];   // its weights' sums
-    u64 list[CAP];
+    union {                           // the bins' sums are read before tokens are listed
+        struct {
+            uint32_t low[BINS], high[BINS];   // of its weights
+        };
+        u64 list[CAP];
+    };
     u64 slot[2][MAX_RANKS][4];        // what the CTAs tell each other, two turns of it
     u64 warp_sum[NW];
     u64 found[4];
@@ -140,10 +153,13 @@ struct Shared {
 struct Weight {
     double scale, top;   // 128 log2(e) / T; the maximum
     float max;
-    __device__ __forceinline__ double place(float l) const { return l == max ? 0.0 : ((double)l - top) * scale; }   // 128 y
-    // 2^(z / 128), z <= 0; what is below 2^-1000 is 0
+    __device__ __forceinline__ double place(float l) const {   // 128 y
+        const double d = ((double)l - top) * scale;
+        return l == max ? 0.0 : d;
+    }
+    // 2^(z / 128), z <= 0, at least 2^-1000
     __device__ __forceinline__ double as_double(double z, const double* two_to) const {
-        if (!(z > -1000.0 * TABLE)) return 0.0;
+        z = z > -1000.0 * TABLE ? z : -1000.0 * TABLE;
         constexpr double MAGIC = 6755399441055744.0;   // 1.5 x 2^52: rounds to whole numbers
         const double t = z + MAGIC, r = z - (t - MAGIC);
         const int n = __double2loint(t);
@@ -156,7 +172,7 @@ struct Weight {
     }
     // in multiples of 2^-43, rounded to the nearest
     __device__ __forceinline__ u64 of(double z, const double* two_to) const {
-        if (!(z > -(FRAC + 1.0) * TABLE)) return 0;
+        if (!(z > -(FRAC + 1.0) * TABLE)) return 0;   // (NaN, too)
         const u64 b = (u64)__double_as_longlong(as_double(z, two_to));
         const int s = 52 - FRAC - ((int)(b >> 52) - 1023);
         return ((b & 0xfffffffffffffull | 1ull << 52) + (1ull << (s - 1))) >> s;
@@ -270,7 +286,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
             if (tid < 4 && off + n + tid < 4 * quads) near[off + n + tid] = -INFINITY;
         }
         if (tid < head) {
-            const float v = clean(up(x[tid]));
+            const float v = clean(load_one(x + tid));
             look(v, tid);
             if (NEAR) near[off + tid] = v;
         }
@@ -286,13 +302,20 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
             for (int k = 0; k < DEEP; ++k) {
                 const int i = i0 + k * NT;
                 if (i >= body) break;
-                const T* e = reinterpret_cast<const T*>(&v[k]);
+                const uint32_t e[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
                 float f[PER];
 #pragma unroll
-                for (int c = 0; c < PER; ++c) {
-                    f[c] = clean(up(e[c]));
-                    look(f[c], head + i * PER + c);
+                for (int c = 0; c < 4; ++c) {
+                    if (PER == 4) {
+                        f[c] = clean(__uint_as_float(e[c]));
+                    } else {
+                        const float2 a = two_up<T>(e[c]);
+                        f[2 * c % PER] = clean(a.x);
+                        f[(2 * c + 1) % PER] = clean(a.y);
+                    }
                 }
+#pragma unroll
+                for (int c = 0; c < PER; ++c) look(f[c], head + i * PER + c);
                 if (NEAR) {
 #pragma unroll
                     for (int c = 0; c < PER; c += 4) to[i * (PER / 4) + c / 4] = make_float4(f[c], f[c + 1], f[c + 2], f[c + 3]);
@@ -301,13 +324,13 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         }
         if (tid < tail) {
             const int i = head + body * PER + tid;
-            const float v = clean(up(x[i]));
+            const float v = clean(load_one(x + i));
             look(v, i);
             if (NEAR) near[off + i] = v;
         }
     }
     const float own_best = best;   // this thread's
-    auto at = [&](int i) -> float { return NEAR ? near[off + i] : clean(up(__ldg(x + i))); };
+    auto at = [&](int i) -> float { return NEAR ? near[off + i] : clean(load_one(x + i)); };
     // Places 4 j .. 4 j + 3 of the share, of which the first `off` lie before it: minus infinity there and behind the end.
     auto quad = [&](int j) -> float4 {
         if (NEAR) return reinterpret_cast<const float4*>(near)[j];
@@ -318,18 +341,21 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
                 return make_float4(clean(q.x), clean(q.y), clean(q.z), clean(q.w));
             }
             const uint2 q = __ldg(reinterpret_cast<const uint2*>(x + i));
-            const T* e = reinterpret_cast<const T*>(&q);
-            return make_float4(clean(up(e[0])), clean(up(e[1])), clean(up(e[2 % (8 / sizeof(T))])), clean(up(e[3 % (8 / sizeof(T))])));
+            const float2 a = two_up<T>(q.x), b = two_up<T>(q.y);
+            return make_float4(clean(a.x), clean(a.y), clean(b.x), clean(b.y));
         }
-        auto one = [&](int k) { return i + k >= 0 && i + k < n ? clean(up(__ldg(x + i + k))) : -INFINITY; };
+        auto one = [&](int k) { return i + k >= 0 && i + k < n ? clean(load_one(x + i + k)) : -INFINITY; };
         return make_float4(one(0), one(1), one(2), one(3));
     };
+    auto own_quad = [&](int j, int end) { return j < end ? quad(j) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY); };
     // f(logit, place in the share) for every token, four of a thread at a time, where any of a warp's is `low` or more; by
     // whole warps, with minus infinity where there is none
     auto each = [&](float low, auto f) {
+        float4 next = own_quad(warp * 32 + lane, quads);
         for (int j0 = warp * 32; j0 < quads; j0 += NT) {
             const int j = j0 + lane;
-            const float4 q = j < quads ? quad(j) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            const float4 q = next;
+            next = own_quad(j + NT, quads);   // on its way while this one is worked on
             if (!__any_sync(0xffffffffu, fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) >= low)) continue;
             const int i = 4 * j - off;
             f(q.x, i);
@@ -345,7 +371,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         __syncthreads();
         turn ^= 1;
         if (tid < 4 * ranks) peer_st(peer(&s.slot[turn][rank][tid & 3], tid >> 2), s.found[tid & 3]);
-        cluster_sync();
+        cluster_meet();
     };
     u64 first;   // the largest logit, the first of equal ones
     {   // the maximum and the smallest finite logit
@@ -366,7 +392,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
             b = max(b, s.warp_sum[w]);
             l = min(l, s.list[w]);
         }
-        if (ranks > 1) cluster_sync();   // every CTA runs: its shared memory may be written
+        if (ranks > 1) cluster_meet();   // every CTA runs: its shared memory may be written
         tell(b, l, 0, 0);
         first = 0;
         l = ~0ull;
@@ -401,8 +427,10 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         fine = span > 0.f ? (float)BINS / span : 0.f;
     };
     auto bin_of = [&](float l) -> int {
-        const float d = (top - l) * fine;   // (the maximum at +infinity: NaN for itself, +infinity for others)
-        return l == top ? 0 : d < (float)(BINS - 1) ? (int)d : BINS - 1;
+        // a whole number by adding 2^23 (an int conversion takes four times as long); past 2^23 + BINS - 1 the last bin, as
+        // minus infinity; the maximum at +infinity would be NaN
+        const float d = fminf(fmaf(top - l, fine, 8388607.5f), 8388608.f + (float)(BINS - 1));
+        return l == top ? 0 : (int)(__float_as_uint(d) & 0x7fffffu);
     };
     const float mass_span = (float)(MASS_SPAN * TABLE / w.scale);
     // every CTA's counts of this thread's four bins
@@ -469,7 +497,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
                 if (l > -INFINITY) atomicAdd(&s.count[bin_of(l)], 1u);
             });
         }
-        if (ranks > 1) cluster_sync();
+        if (ranks > 1) cluster_meet();
         else __syncthreads();
         uint32_t c4[4], total;
         sum_bins(c4);
@@ -486,16 +514,17 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         // (a token of the bin is not below this; the bin itself decides)
         const float low = bin == BINS - 1 || fine == 0.f ? -3.402823466e38f : top - (float)(bin + 2) / fine;
         each(low, [&](float l, int i) { hand_in(l > -INFINITY && bin_of(l) <= bin, place_key(l, lo + i)); });
-        if (ranks > 1) cluster_sync();
+        if (ranks > 1) cluster_meet();
         else __syncthreads();
         const uint32_t listed = rank == 0 ? (uint32_t)s.taken : peer_ld(peer(&s.taken, 0));
-        if (ranks > 1) cluster_sync();   // (the count is read by all before the first CTA goes on)
+        if (ranks > 1) cluster_meet();   // (the count is read by all before the first CTA goes on)
         if (listed <= CAP) {
             if (rank) return;
             arrange((int)listed);
             const int kept = min(top_k, (int)listed);
             // weights; the tokens before which less than top_p lies; those of min_p or more: each a beginning of the list
-            u64* masses = reinterpret_cast<u64*>(s.low);   // [FEW], over the sums (which no one reads now)
+            u64* masses = s.list + CAP - FEW;   // [FEW], over what is behind the top_k
+            static_assert(2 * FEW <= CAP, "the list's second half");
             constexpr int EACH = FEW / NT;
             u64 sum = 0;
             int left = 0;
@@ -560,12 +589,21 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         for (int i = tid; i < BINS; i += NT) s.count[i] = 0;
         __syncthreads();
         // (the total in 64-bit floating point, in an order of its own, the same on every run)
+        // Four tokens side by side and without branches: a weight is a chain of a dozen operations.  (Minus infinity counts
+        // for the last bin, whose number is only ever an upper bound, with a weight of 2^-1000.)
         double sum = 0.0;
-        each(-3.402823466e38f, [&](float l, int) {
-            if (l == -INFINITY) return;
-            atomicAdd(&s.count[bin_of(l)], 1u);
-            sum += w.as_double(w.place(l), s.two_to);
-        });
+        float4 q = own_quad(tid, quads);
+        for (int j = tid; j < quads; j += NT) {
+            const float4 next = own_quad(j + NT, quads);
+            const float l4[4] = {q.x, q.y, q.z, q.w};
+            double v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = w.as_double(w.place(l4[k]), s.two_to);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) atomicAdd(&s.count[bin_of(l4[k])], 1u);
+            sum += (v[0] + v[1]) + (v[2] + v[3]);
+            q = next;
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) s.warp_sum[warp] = (u64)__double_as_longlong(sum);
@@ -613,24 +651,32 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         const int piece = ceil_div(quads, NW), q0 = min(quads, warp * piece), q1 = min(quads, q0 + piece);
         const float low = hi_bin == BINS - 1 || fine == 0.f ? -3.402823466e38f : top - (float)(hi_bin + 2) / fine;
         u64 above = 0, stay = 0, kl = ~0ull, kh = 0;   // kl, kh: of the bins' tokens
+        float4 ahead = own_quad(q0 + lane, q1);
         for (int j = q0 + lane; j < ((q1 - q0 + 31) & ~31) + q0; j += 32) {
-            const float4 q = j < q1 ? quad(j) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            const float4 q = ahead;
+            ahead = own_quad(j + 32, q1);
             if (!__any_sync(0xffffffffu, fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) >= low)) continue;
             const float l4[4] = {q.x, q.y, q.z, q.w};
+            bool take[4], any = false;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int b = bin_of(l4[k]);
                 const bool there = l4[k] > -INFINITY;
+                take[k] = there && b >= lo_bin && b <= hi_bin;
+                any |= take[k];
                 if (there && b < lo_bin) {
                     const double z = w.place(l4[k]);
                     const u64 v = w.of(z, s.two_to);
                     above += v;
                     if (z >= floor_z) stay += v;
                 }
-                const bool take = there && b >= lo_bin && b <= hi_bin;
+            }
+            if (!__any_sync(0xffffffffu, any)) continue;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
                 const u64 key = place_key(l4[k], lo + 4 * j + k - off);
-                if (take) kl = min(kl, key), kh = max(kh, key);
-                hand_in(take, key);
+                if (take[k]) kl = min(kl, key), kh = max(kh, key);
+                hand_in(take[k], key);
             }
         }
 #pragma unroll
@@ -706,7 +752,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
                     }
                 }
             }
-            if (ranks > 1) cluster_sync();
+            if (ranks > 1) cluster_meet();
             else __syncthreads();
             if ((int)(s.told[0] / NW) != rank) return;
             const u64 goal = s.told[1], bar = s.told[2];
@@ -766,7 +812,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
                     }
                 }
             });
-            if (ranks > 1) cluster_sync();
+            if (ranks > 1) cluster_meet();
             else __syncthreads();
             // four bins to a thread, over all CTAs
             uint32_t c4[4];
@@ -783,7 +829,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
             u64 total;
             u64 at_bin = before + block_scan<u64>(m4[0] + m4[1] + m4[2] + m4[3], s.warp_sum, &total);
             if (!mass && before + total < target) {   // fewer tokens than that: all stay
-                if (ranks > 1) cluster_sync();        // (the counts are read by all before they are cleared again)
+                if (ranks > 1) cluster_meet();        // (the counts are read by all before they are cleared again)
                 else __syncthreads();
                 return bar;
             }
@@ -829,7 +875,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
                 }
                 first_level = false;
             } else if (ranks > 1) {
-                cluster_sync();   // the counts are read before they are cleared
+                cluster_meet();   // the counts are read before they are cleared
             }
             cut();
         }
@@ -837,7 +883,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         uint32_t base = 0;
         for (int c = 0; c < rank; ++c) base += peer_ld(peer(&s.count[bin], c));
         if (tid == 0) s.taken = 0;
-        __syncthreads();
+        if (ranks > 1) cluster_meet();   // the sums are read by all
+        else __syncthreads();
         const u64 from = max(bar, lo_key);
         each(low_of(from), [&](float l, int i) {
             const u64 key = place_key(l, lo + i);
@@ -845,7 +892,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
             const uint32_t place = base + atomicAdd(&s.taken, 1);
             for (int c = 0; c < ranks; ++c) peer_st(peer(&s.list[place], c), key);
         });
-        if (ranks > 1) cluster_sync();
+        if (ranks > 1) cluster_meet();
         else __syncthreads();
         arrange((int)count);
         if (!mass) {
@@ -950,16 +997,12 @@ size_t smem_of(int share, bool near) {
 
 template <typename T>
 int run(Args a, cudaStream_t st) {
-    // As many CTAs to a row (a power of two) as all rows have room for at once, two to an SM, and as leave each 4096 tokens
-    // or more: a CTA does the last steps of its row alone, so with more of them most would wait (256 rows of 152k in bf16:
-    // REPLACE).  The share stays in shared memory where that keeps all CTAs resident; otherwise the passes read it
-    // from L2 (64 rows of 152k in fp32: REPLACE).
-    const int sms = sm_count();
+    // As many CTAs to a row as leave each 4096 tokens or more.  Two of a row of 152k fit an SM; with one CTA to a row, and
+    // passes that read it from L2, 256 rows took 466 us and not 390 (64 rows: 129 and 92).
     unsigned ranks = 1;
-    while (ranks < MAX_RANKS && a.vocab > 4096 * (int)ranks && (long long)a.n * ranks * 2 <= 2 * sms) ranks *= 2;
+    while (ranks < MAX_RANKS && a.vocab > 4096 * (int)ranks) ranks *= 2;
     a.share = (ceil_div(a.vocab, (int)ranks) + 7) & ~7;
-    const size_t held = smem_of(a.share, true);
-    const bool near = held <= 220 * 1024 && (long long)a.n * ranks <= (held <= 112 * 1024 ? 2ll : 1ll) * sms;
+    const bool near = smem_of(a.share, true) <= 220 * 1024;
     const size_t smem = smem_of(a.share, near);
     static SmemLimit limits[2];
     const auto kernel = near ? sample_kernel<T, true> : sample_kernel<T, false>;

@@ -421,15 +421,15 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         return x < (double)total ? min((u64)x, total - 1) : total - 1;
     };
     // bins of equal width in the logit, from the maximum down
-    float fine = 0.f;
-    auto spread = [&](float span) {
-        span = fminf(top - least, span);
+    float fine = 0.f, span = 0.f;
+    auto spread = [&](float most) {
+        span = fminf(top - least, most);
         fine = span > 0.f ? (float)BINS / span : 0.f;
     };
     auto bin_of = [&](float l) -> int {
         // a whole number by adding 2^23 (an int conversion takes four times as long); past 2^23 + BINS - 1 the last bin, as
-        // minus infinity; the maximum at +infinity would be NaN
-        const float d = fminf(fmaf(top - l, fine, 8388607.5f), 8388608.f + (float)(BINS - 1));
+        // minus infinity; below 2^23 (a quarter of a bin from the maximum) the first; the maximum at +infinity would be NaN
+        const float d = fmaxf(fminf(fmaf(top - l, fine, 8388607.5f), 8388608.f + (float)(BINS - 1)), 8388608.f);
         return l == top ? 0 : (int)(__float_as_uint(d) & 0x7fffffu);
     };
     const float mass_span = (float)(MASS_SPAN * TABLE / w.scale);
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         // The bins in which that token can lie: a bin's weights are between those of its edges.  The last bin has no lower edge.
         uint32_t c4[4];
         sum_bins(c4);
-        const float octaves = fine > 0.f ? (float)w.scale / TABLE / fine : 0.f;   // of a bin
+        const float octaves = (float)(w.scale * (double)span / (TABLE * BINS));   // of a bin, 44 / BINS at most
         const double step = exp2f(-octaves);                                      // of a bin's weights
         double edge = exp2f(-octaves * (4.f * tid)) * ONE;
         double most[4], sum4 = 0.0;

@@ -161,6 +161,24 @@ def test_odd_logits(sample, rule):
     check(sample, x, torch.linspace(0, 0.99, len(x), device="cuda"), **rule)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rule", [dict(top_k=2), dict(top_k=30), dict(top_k=5000), dict(top_p=0.4), dict(top_p=0.95), dict(min_p=0.999),
+                                  dict(top_p=0.4, temperature=1e-37), dict(top_p=0.9, temperature=1e-42),
+                                  dict(top_k=7000, top_p=0.9, temperature=1e-42), dict(top_p=0.4, temperature=1e-7)])
+def test_next_to_the_largest(sample, dtype, rule):
+    """The next logits are one step of the type below the largest, or subnormal steps."""
+    g, vocab = gen(13), 20011
+    x = rows(g, 5, vocab, dtype)
+    up = 1024 if dtype == torch.float16 else 2.0 ** 20
+    step = torch.finfo(dtype).eps / 2   # below a power of two
+    at = torch.randint(0, vocab, (5, 40), device="cuda", generator=g)
+    x.scatter_(1, at, (up * (1 - step * (torch.arange(40, device="cuda") % 4))).to(dtype).expand(5, -1))
+    x[1] = (torch.arange(vocab, device="cuda") % 5 == 0).to(dtype) * torch.finfo(dtype).tiny
+    x[2] = torch.where(torch.arange(vocab, device="cuda") % 7 == 0, 1.0, 1.0 - step).to(dtype)
+    x[3, 100:] = -math.inf
+    check(sample, x, torch.rand(5, device="cuda", generator=g), **rule)
+
+
 def test_numbers_at_the_ends(sample):
     x = rows(gen(8), 6, 5003, torch.float32)
     u = torch.tensor([0.0, -1.0, 1.0, 2.0, math.nan, 1 - 2.0 ** -24], device="cuda")

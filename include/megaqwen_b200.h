@@ -445,6 +445,9 @@ int mq_paged_accept(const mq_paged_pool* pool, const mq_page_table* t, const int
  * (2i, 2i + 1) with interleaved.  cos/sin: fp32 [max_pos, rotary_dim / 2],
  * y0 = x0 c - x1 s, y1 = x1 c + x0 s, each product and sum rounded to fp32.
  * inverse turns the other way (the gradient of the rotation).
+ * places: K and V are written at these positions of the sequence and rotated by
+ * positions[i] all the same (the nodes of a drafted tree lie one after another,
+ * and nodes of one depth turn alike).
  * With an index in the pool, a page whose last row is written gets its record:
  * the channel-wise bounds of its keys as whole numbers HI[D], LO[D] times 2^e,
  * then e: e = clamp(floor(log2 a) - 6, -60, 40) for the largest magnitude a of
@@ -478,6 +481,7 @@ typedef struct mq_rope_params {
     int num_slots;
     int table_cols;
     int* status;                 /* device int32, optional */
+    const int* places;           /* device int32 [n], optional, with pool */
 } mq_rope_params;
 
 int mq_rope(const mq_rope_params* params, cudaStream_t stream);

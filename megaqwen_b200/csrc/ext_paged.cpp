@@ -283,7 +283,7 @@ Tensor rope(Tensor x, Tensor positions, Tensor cos, Tensor sin, bool interleaved
 
 Tensor rope_append(Tensor q, Tensor k, Tensor v, Tensor k_pages, Tensor v_pages, Tensor table, Tensor slots,
                    Tensor positions, Tensor cos, Tensor sin, int64_t layer, bool interleaved, OptTensor index,
-                   OptTensor status) {
+                   OptTensor status, OptTensor places) {
     const mq_paged_pool pool = pool_of(k_pages, v_pages, index);
     const auto dev = k_pages.device();
     const int64_t D = pool.head_dim, n = q.dim() == 3 ? q.size(0) : -1;
@@ -308,6 +308,7 @@ Tensor rope_append(Tensor q, Tensor k, Tensor v, Tensor k_pages, Tensor v_pages,
     p.v_token = v.stride(0); p.v_head = v.stride(1);
     p.positions = ints(positions, dev, "positions", n);
     p.slots = ints(slots, dev, "slots", n);
+    if (places.has_value()) p.places = ints(*places, dev, "places", n);
     p.n = (int)n;
     p.num_q_heads = (int)q.size(1);
     p.head_dim = (int)D;
@@ -495,7 +496,7 @@ void bind_paged(py::module_& m) {
     m.def("paged_rope_append", &rope_append, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("k_pages"),
           py::arg("v_pages"), py::arg("page_table"), py::arg("slots"), py::arg("positions"), py::arg("cos"),
           py::arg("sin"), py::arg("layer"), py::arg("interleaved") = false, py::arg("index") = none,
-          py::arg("status") = none);
+          py::arg("status") = none, py::arg("places") = none);
     m.def("paged_free", &paged_free, py::arg("page_table"), py::arg("lengths"), py::arg("refs"), py::arg("slots"),
           py::arg("page_size"), py::arg("status") = none);
     m.def("paged_reserve", &paged_reserve, py::arg("page_table"), py::arg("lengths"), py::arg("refs"), py::arg("slots"),

@@ -22,6 +22,7 @@ struct RopeArgs {
     const uint16_t* v;
     long long q_tok, q_head, o_tok, o_head, k_tok, k_head, v_tok, v_head;
     const int* positions;
+    const int* places;   // null: the positions
     const int* slots;
     const float* cos_t;
     const float* sin_t;
@@ -49,7 +50,7 @@ struct Place {
     int pos, page, row;
     bool ok;   // the position is inside the tables
 };
-__device__ __forceinline__ Place place_of(const RopeArgs& a, int pos, int slot, bool report) {
+__device__ __forceinline__ Place place_of(const RopeArgs& a, int pos, int at, int slot, bool report) {
     Place p;
     p.pos = pos;
     p.page = -1;
@@ -58,16 +59,16 @@ __device__ __forceinline__ Place place_of(const RopeArgs& a, int pos, int slot, 
     if (!p.ok) {
         if (report) note_status(a.status, MQ_ERR_BAD_POSITION);
     } else if (a.kp) {
-        const int c = pos >> a.shift;
+        const int c = at >> a.shift;
         if (slot < 0 || slot >= a.slots_n) {
             if (report) note_status(a.status, MQ_ERR_BAD_SLOT);
-        } else if (c >= a.cols) {
+        } else if (at < 0 || c >= a.cols) {
             if (report) note_status(a.status, MQ_ERR_BAD_POSITION);
         } else {
             const int g = __ldg(a.table + slot * a.table_row + c);
             if (g >= 0 && g < a.pages) {
                 p.page = g;
-                p.row = pos & (a.page - 1);
+                p.row = at & (a.page - 1);
             } else if (report) {
                 note_status(a.status, MQ_ERR_BAD_PAGE);
             }
@@ -123,14 +124,14 @@ __global__ void __launch_bounds__(ROPE_THREADS, 8) rope_kernel(const RopeArgs a,
     };
     int t = blockIdx.x, h = lane_h;
     if (t >= n) return;
-    int pos = __ldg(a.positions + t), slot = a.kp ? __ldg(a.slots + t) : 0;
+    int pos = __ldg(a.positions + t), slot = a.kp ? __ldg(a.slots + t) : 0, at = a.places ? __ldg(a.places + t) : pos;
     read(t, h, 0);
     read(t, h, 1);
     Place p;
     float cs[8], sn[8];
     while (t < n) {
         if (h == lane_h) {   // a new token
-            p = place_of(a, pos, slot, threadIdx.x == 0);
+            p = place_of(a, pos, at, slot, threadIdx.x == 0);
             if (turn0 && p.ok) {
 #pragma unroll
                 for (int i = 0; i < 8; i += 4) {
@@ -149,6 +150,7 @@ __global__ void __launch_bounds__(ROPE_THREADS, 8) rope_kernel(const RopeArgs a,
             if (t + (int)gridDim.x < n) {
                 pos = __ldg(a.positions + t + gridDim.x);
                 if (a.kp) slot = __ldg(a.slots + t + gridDim.x);
+                at = a.places ? __ldg(a.places + t + gridDim.x) : pos;
             }
         }
         int t1 = t, h1 = h + 2 * LANES;   // the next step
@@ -204,7 +206,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_any_kernel(const RopeArgs a
     pdl_wait();
     pdl_trigger();
     const int t = blockIdx.x, half = a.rot / 2;
-    const Place p = place_of(a, __ldg(a.positions + t), a.kp ? __ldg(a.slots + t) : 0, threadIdx.x == 0);
+    const int pos = __ldg(a.positions + t);
+    const Place p = place_of(a, pos, a.places ? __ldg(a.places + t) : pos, a.kp ? __ldg(a.slots + t) : 0, threadIdx.x == 0);
     const int heads = a.hq + (a.kp ? 2 * a.hkv : 0);
     for (int e = threadIdx.x; e < heads * (D / 2); e += ROPE_THREADS) {
         const int h = e / (D / 2), i = e - h * (D / 2);
@@ -251,8 +254,9 @@ __global__ void __launch_bounds__(INDEX_THREADS) index_kernel(const RopeArgs a, 
         const int t = blockIdx.x * INDEX_TOKENS + i + threadIdx.x;
         if (t >= n) break;
         const int pos = __ldg(a.positions + t), slot = __ldg(a.slots + t);
-        if ((pos & (a.page - 1)) == a.page - 1) {
-            const Place p = place_of(a, pos, slot, false);
+        const int at = a.places ? __ldg(a.places + t) : pos;
+        if ((at & (a.page - 1)) == a.page - 1) {
+            const Place p = place_of(a, pos, at, slot, false);
             if (p.page >= 0) list[atomicAdd(&count, 1)] = p.page;
         }
     }
@@ -414,6 +418,7 @@ extern "C" int mq_rope(const mq_rope_params* p, cudaStream_t st) {
         a.k_tok = p->k_token; a.k_head = p->k_head;
         a.v_tok = p->v_token; a.v_head = p->v_head;
         a.slots = p->slots;
+        a.places = p->places;
         a.hkv = o.num_kv_heads;
         a.kp = (uint16_t*)o.k + p->layer * o.k_layer;
         a.vp = (uint16_t*)o.v + p->layer * o.v_layer;

@@ -14,7 +14,8 @@ synchronises, and outputs come from the current stream's allocator):
 
 ``rope_tables``    cos / sin tables, optionally scaled for long contexts
 ``rope``           rotary positions (half or interleaved pairs, part of the head)
-``rope_append``    the same for q, fused with the write of rotated k and of v
+``rope_append``    the same for q, fused with the write of rotated k and of v (at ``places``, where those are not the
+                   positions: a drafted tree's nodes)
 ``reserve`` ``fork`` ``free`` ``copy`` ``compact``   pages and their bookkeeping
 ``attend``         attention, shared prefixes read once per group
 ``sparse_attend``  attention over the pages that a cheap score selects
@@ -55,7 +56,7 @@ INDEX_PAD = 16   # bytes of an index record after the two bounds: the exponent a
 
 BAD_TOKEN = 4
 STATUS = {
-    1: "starts out of order",
+    1: "starts out of order, or parents or sizes of a drafted tree that are wrong",
     3: "a wait of a kernel ran out",
     BAD_TOKEN: "token id out of range",
     5: "position out of range",
@@ -207,9 +208,9 @@ class PagedKVCache:
         self.status.copy_(torch.where(self.status == 0, new.status, self.status))
         return new
 
-    def append(self, layer: int, q, k, v, slots, positions, cos, sin, interleaved: bool = False) -> torch.Tensor:
+    def append(self, layer: int, q, k, v, slots, positions, cos, sin, interleaved: bool = False, places=None) -> torch.Tensor:
         return rope_append(q, k, v, self.k_pages, self.v_pages, self.page_table, slots, positions, cos, sin, layer=layer,
-                           interleaved=interleaved, index=self.index, status=self.status)
+                           interleaved=interleaved, index=self.index, status=self.status, places=places)
 
     def attend(self, layer: int, q, slots, q_starts=None, group_starts=None, prefix_pages=None, scale=None) -> torch.Tensor:
         return attend(q, self.k_pages, self.v_pages, self.page_table, self.lengths, slots, layer=layer, q_starts=q_starts,

@@ -4,7 +4,9 @@
 plain matrix products and everything around the cache on the operators of
 :mod:`megaqwen_b200.paged`: rotary positions and the write of K and V in one
 pass, pages reserved, forked and freed on the device, attention that reads a
-shared prompt once for all its samples, or a chosen part of a long context.
+shared prompt once for all its samples, a chosen part of a long context, or a
+window of it; and trees of drafted tokens checked in one pass.  Tokens are drawn
+from the logits by :mod:`megaqwen_b200.sampling`.
 The batched decoder of the native library (``MegakernelBatchDecoder``) is the
 faster one for sequences that share nothing.
 
@@ -16,14 +18,17 @@ cache operators' type.
 from __future__ import annotations
 
 from collections import Counter
-from itertools import count
-from typing import List, Optional, Sequence, Tuple
+from itertools import accumulate, count
+from typing import Callable, List, Optional, Sequence, Tuple
 
 import torch
 import torch.nn.functional as F
 
 from .paged import BAD_TOKEN, PagedKVCache, to_device
+from .sampling import sample
 from .weights import (HEAD_DIM, NUM_KV_HEADS, NUM_Q_HEADS, Q_SIZE, KV_SIZE, RMS_NORM_EPS, Qwen3Weights, rope_tables)
+
+MAX_NODES = 256   # of a drafted tree
 
 
 def _rms_norm(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
@@ -44,7 +49,9 @@ class PagedDecoder:
     """``max_seqs`` sequences on a pool of ``num_pages`` pages.
 
     ``sparse_pages``: decode steps read at most this many pages per query and
-    kv head (chosen by score); ``None`` reads everything.
+    kv head (chosen by score); ``None`` reads everything.  ``window``: a token
+    sees the last ``window`` positions, itself among them, and the first
+    ``sinks``, in prompts and in steps; not together with ``sparse_pages``.
 
     The host keeps account of lengths and pages, so a call that the cache would
     refuse raises before anything is changed on either side.  :meth:`check`
@@ -53,7 +60,12 @@ class PagedDecoder:
     """
 
     def __init__(self, weights: Qwen3Weights, num_pages: int, max_seqs: int, max_seq_len: int = 4096, page_size: int = 64,
-                 sparse_pages: Optional[int] = None):
+                 sparse_pages: Optional[int] = None, window: Optional[int] = None, sinks: int = 0):
+        if window is not None and sparse_pages is not None:
+            raise ValueError("window and sparse_pages exclude each other")
+        if sinks < 0 or (window is None and sinks) or (window is not None and window < 1):
+            raise ValueError("window must be positive, and sinks go with a window")
+        self.window, self.sinks = window, sinks
         dev = weights.embed.device
         self.embed, self.final_norm, self.sparse_pages = weights.embed, weights.final_norm.float(), sparse_pages
         self.layers = []
@@ -121,8 +133,9 @@ class PagedDecoder:
         status.copy_(torch.where((safe != ids).any() & (status == 0), BAD_TOKEN, status))
         return safe
 
-    def _forward(self, ids, slots, positions, attend) -> torch.Tensor:
-        """Hidden states of the tokens after the final norm; ``attend(layer, q)`` reads the cache."""
+    def _forward(self, ids, slots, positions, attend, places=None) -> torch.Tensor:
+        """Hidden states of the tokens after the final norm; ``attend(layer, q)`` reads the cache.  Keys lie at ``places``,
+        or at the positions."""
         h = self.embed[ids].float()
         n = h.shape[0]
         for li, w in enumerate(self.layers):
@@ -131,7 +144,7 @@ class PagedDecoder:
             q = _rms_norm(q.view(n, NUM_Q_HEADS, HEAD_DIM), w["q_norm"]).to(self.embed.dtype)
             k = _rms_norm(k.view(n, NUM_KV_HEADS, HEAD_DIM), w["k_norm"]).to(self.embed.dtype)
             v = v.view(n, NUM_KV_HEADS, HEAD_DIM).to(self.embed.dtype)
-            q = self.cache.append(li, q, k, v, slots, positions, self.cos, self.sin)
+            q = self.cache.append(li, q, k, v, slots, positions, self.cos, self.sin, places=places)
             h = h + _product(attend(li, q).view(n, Q_SIZE), w["o_proj"])
             x = _rms_norm(h, w["post_attention_layernorm"])
             gate, up = _product(x, w["gate_up"]).chunk(2, -1)
@@ -153,9 +166,14 @@ class PagedDecoder:
         self.cache.reserve([slot], [start + n])
         one = self._ints([slot])
         starts = self._ints([0, n])
+        if self.window is None:
+            def attend(li, q):
+                return self.cache.attend(li, q, one, q_starts=starts)
+        else:
+            def attend(li, q):
+                return self.cache.window_attend(li, q, one, self.window, self.sinks, q_starts=starts)
         h = self._forward(ids, one.expand(n).contiguous(),
-                          torch.arange(start, start + n, dtype=torch.int32, device=self.embed.device),
-                          lambda li, q: self.cache.attend(li, q, one, q_starts=starts))
+                          torch.arange(start, start + n, dtype=torch.int32, device=self.embed.device), attend)
         return self._logits(h[-1:])[0]
 
     def fork(self, parent: int, children: Sequence[int]) -> None:
@@ -229,7 +247,10 @@ class PagedDecoder:
         _, back, dev_slots, starts, pages = self._groups(slots)
         positions = self.cache.lengths[dev_slots]
         self.cache.reserve(dev_slots, positions + 1)
-        if self.sparse_pages is None:
+        if self.window is not None:
+            def attend(li, q):
+                return self.cache.window_attend(li, q, dev_slots, self.window, self.sinks)
+        elif self.sparse_pages is None:
             def attend(li, q):
                 return self.cache.attend(li, q, dev_slots, group_starts=starts, prefix_pages=pages)
         else:
@@ -239,6 +260,88 @@ class PagedDecoder:
         out = torch.empty_like(h)
         out[back] = h
         return self._logits(out)
+
+    @staticmethod
+    def draw(logits: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+             generator: Optional[torch.Generator] = None) -> torch.Tensor:
+        """A token for each row of logits (int32), drawn with ``generator``'s random numbers by the rules of
+        :func:`megaqwen_b200.sampling.sample`.  No host synchronisation."""
+        logits = logits.reshape(-1, logits.shape[-1])
+        u = torch.rand(logits.shape[0], generator=generator, device=logits.device)
+        return sample(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+
+    @torch.no_grad()
+    def verify(self, slots: Sequence[int], tokens: Sequence[Sequence[int]], parents: Sequence[Sequence[int]],
+               choose: Optional[Callable[[torch.Tensor], torch.Tensor]] = None) -> List[List[int]]:
+        """Drafted trees checked in one pass: the tokens that each sequence goes on with.
+
+        ``tokens[i]`` are the nodes of sequence ``slots[i]``, at most 256, the first one the token that a step would take
+        next; ``parents[i]`` their parents' numbers, -1 for the first and smaller than the node's own for the others.
+        ``choose(logits)`` picks a token at each node, all sequences' nodes one after another (the largest logit, or
+        :meth:`draw` with its arguments).  A sequence keeps the first node and those drafted ones that were chosen at
+        the node before them, and the list returned holds the tokens chosen at the kept nodes: its last one is not in the
+        cache yet.  The other nodes' room is given back.  Where ``choose`` raises, each sequence keeps its first node, as
+        after a step.  Reads the counts, so it synchronises.
+        """
+        slots, tokens, parents = list(slots), [list(t) for t in tokens], [list(p) for p in parents]
+        self._known(slots)
+        if self.window is not None:
+            raise ValueError("drafted trees are not checked through a window")
+        if len(tokens) != len(slots) or [len(t) for t in tokens] != [len(p) for p in parents]:
+            raise ValueError("there must be a tree for each sequence and a parent for each node")
+        depths: List[int] = []
+        for t in parents:
+            if not 1 <= len(t) <= MAX_NODES or t[0] != -1 or any(not 0 <= up < i for i, up in enumerate(t) if i):
+                raise ValueError(f"a tree has 1 to {MAX_NODES} nodes, each behind its parent, and one root")
+            first = len(depths)
+            for up in t:
+                depths.append(depths[first + up] + 1 if up >= 0 else 0)
+        sizes = [len(t) for t in tokens]
+        old = [self.lengths[s] for s in slots]
+        ends = [n + k for n, k in zip(old, sizes)]
+        if any(n > self.max_seq_len for n in ends):
+            raise ValueError("a sequence would exceed max_seq_len")
+        ids = self._tokens([x for t in tokens for x in t], sum(sizes))
+        if not slots:
+            return []
+        self._grow(slots, ends)
+        dev_slots, nodes = self._ints(slots), self._ints([x for t in tokens for x in t])
+        self.cache.reserve(dev_slots, ends)
+        up = self._ints([x for t in parents for x in t])
+        starts = self._ints([0, *accumulate(sizes)])
+        base = [n for n, k in zip(old, sizes) for _ in range(k)]
+        positions = self._ints([n + d for n, d in zip(base, depths)])
+        places = self._ints([n + i for n, k in zip(old, sizes) for i in range(k)])
+        h = self._forward(ids, self._ints([s for s, k in zip(slots, sizes) for _ in range(k)]), positions,
+                          lambda li, q: self.cache.tree_attend(li, q, dev_slots, up, q_starts=starts), places)
+        logits = self._logits(h)
+        failed = None
+        try:
+            chosen = self.draw(logits, temperature=0.0) if choose is None else choose(logits)
+            if chosen.numel() != nodes.numel():
+                raise ValueError("there must be a chosen token for each node")
+            chosen = self._ints(chosen.reshape(-1))
+        except Exception as e:   # (a step has no such callback: the trees must not stay in the cache)
+            failed, chosen = e, torch.full_like(nodes, -1)
+        _, emitted, count = self.cache.accept(dev_slots, up, nodes, chosen, q_starts=starts)
+        emitted, kept = emitted.tolist(), count.tolist()
+        if not all(kept):   # refused on the device, where nothing was cut
+            self._take_over()
+            self.check()
+            raise RuntimeError("paged cache: the trees were refused")
+        out, at = [], 0
+        for s, n, size, k in zip(slots, old, sizes, kept):
+            out.append(emitted[at:at + k])
+            at += size
+            self.lengths[s] = n + k
+            full = -(-(n + k) // self.cache.page_size)
+            for p in self._pages[s][full:]:   # no one else's: they were reserved for the tree
+                del self._held[p]
+                self._free_pages += 1
+            del self._pages[s][full:]
+        if failed is not None:
+            raise failed
+        return out
 
     def check(self) -> None:
         """Raises if a device-side check failed, with lengths and pages then as the device has them (synchronises)."""

@@ -181,8 +181,9 @@ __device__ __forceinline__ int window_groups(const RowArgs& a, int len) {
     return min(groups_of(len), sink_groups(a, len) + ((a.window + tokens - 2) >> 4) + 2);
 }
 
+template <bool MASK>   // MASK: of a call with a window or trees
 __device__ __forceinline__ int own_groups(const RowArgs& a, const Sched& s, int b) {
-    if (a.window) return window_groups(a, s.len[b]);
+    if (MASK && a.window) return window_groups(a, s.len[b]);
     const int lo = s.grp[b] >= 0 ? s.eff[s.grp[b]] << a.pool.shift : 0;
     return s.len[b] > lo ? ((s.len[b] - lo - 1) >> 4) + 1 : 0;
 }
@@ -199,7 +200,7 @@ __device__ __forceinline__ int pfx_tiles(const RowArgs& a, int rows) {
 // Returns false (for every thread) when the starts are out of order or the
 // line is longer than 2^31 units.  PFX: the prefixes alone (s.len and s.grp
 // are not used).  NT threads.
-template <bool PFX, int NT>
+template <bool PFX, int NT, bool MASK = false>
 __device__ inline bool build_sched(const RowArgs& a, const Sched& s, unsigned long long* scratch /* [NT / 32] */) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     bool bad = false;
@@ -242,7 +243,7 @@ __device__ inline bool build_sched(const RowArgs& a, const Sched& s, unsigned lo
                     if (!PFX && blockIdx.x == 0) note_status(a.status, MQ_ERR_BAD_POSITION);
                     len = 0;
                 }
-                if (a.parents && ql > MAX_TREE) {
+                if (MASK && a.parents && ql > MAX_TREE) {
                     if (!PFX && blockIdx.x == 0) note_status(a.status, MQ_ERR_INVALID_ARGUMENT);
                     len = 0;
                 }
@@ -285,7 +286,7 @@ __device__ inline bool build_sched(const RowArgs& a, const Sched& s, unsigned lo
         } else {
             const int b = e - a.NG;
             tiles = row_tiles(a, (q_start(a, b + 1) - q_start(a, b)) * a.grp);
-            ng = own_groups(a, s, b);
+            ng = own_groups<MASK>(a, s, b);
         }
         return ng ? (unsigned long long)(unsigned)tiles * (unsigned)(ng + ITEM_UNITS) : 0;
     };
@@ -643,7 +644,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     const int sp_nrt = row_tiles(a, grp), sp_ng = a.top_k << (shift - 4);
     if (LINE) {
         s = sched_of(smem + ROW_WARPS * W::RING, a.B, a.NG);
-        const bool ok = build_sched<false, ROW_THREADS>(a, s, scratch);
+        const bool ok = build_sched<false, ROW_THREADS, MODE == 3>(a, s, scratch);
         if (!ok) {
             if (blockIdx.x == 0 && threadIdx.x == 0) {
                 note_status(a.status, MQ_ERR_INVALID_ARGUMENT);
@@ -680,7 +681,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
             } else {
                 b0 = e - a.NG;
                 b1 = b0 + 1;
-                ng = own_groups(a, s, b0);
+                ng = own_groups<MODE == 3>(a, s, b0);
                 other = s.grp[b0] >= 0 && s.eff[s.grp[b0]] > 0;
                 base = other ? s.eff[s.grp[b0]] << shift : 0;
             }
@@ -959,7 +960,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
             const int q0 = q_start(a, b), q1 = q_start(a, b + 1), gr = s.grp[b];
             TokInfo ti = {};
             ti.own_base = s.off[a.NG + b] * a.hkv - origin;
-            ti.own_ng = own_groups(a, s, b);
+            ti.own_ng = own_groups<MODE == 3>(a, s, b);
             ti.own_nrt = row_tiles(a, (q1 - q0) * grp);
             int p0 = 0;
             if (gr >= 0 && s.eff[gr] > 0) {

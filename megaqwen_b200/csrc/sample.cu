@@ -143,7 +143,6 @@ struct Shared {
     u64 found[4];
     double two_to[TABLE];             // 2^(j / TABLE)
     u64 pieces[MAX_RANKS * NW];       // sums of the warps' pieces of the row, in the first CTA
-    u64 told[4];                      // what the first CTA tells the others
     u64 ends[2 * NW];                 // the warps' smallest and largest keys
     int taken;
 };
@@ -641,11 +640,11 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
             if (here * margin >= (double)target) lo_bin = 4 * tid + k;
             if (here * step / margin >= (double)target + 1.0 && 4 * tid + k < BINS - 1) hi_bin = 4 * tid + k;
         }
-        if (lo_bin < BINS - 1) atomicMin(reinterpret_cast<unsigned*>(&s.found[0]), (unsigned)lo_bin);
-        if (hi_bin < BINS - 1) atomicMin(reinterpret_cast<unsigned*>(&s.found[1]), (unsigned)hi_bin);
+        if (lo_bin < BINS - 1) atomicMin(&s.found[0], (u64)lo_bin);
+        if (hi_bin < BINS - 1) atomicMin(&s.found[1], (u64)hi_bin);
         __syncthreads();
-        lo_bin = (int)(unsigned)s.found[0];
-        hi_bin = (int)(unsigned)s.found[1];
+        lo_bin = (int)s.found[0];
+        hi_bin = (int)s.found[1];
         // tokens above those bins stay: their weights, and those of min_p or more by pieces of the row; the bins' own tokens
         // go to the first CTA.  A piece is a run of quads to a warp.
         const int piece = ceil_div(quads, NW), q0 = min(quads, warp * piece), q1 = min(quads, q0 + piece);
@@ -703,77 +702,76 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         bracketed = true;
         bracket[0] = target, bracket[1] = kl, bracket[2] = kh, bracket[3] = before;
         if (listed <= CAP) {   // all CTAs alike
-            if (rank == 0) {
-                arrange((int)listed);
-                // the last token of the list before which less than `target` lies, and the tokens up to it that stay
-                constexpr int EACH = CAP / NT;
-                double z[EACH];
-                u64 v[EACH], mine = 0, total;
+            if (ranks > 1) cluster_meet();   // (the number is read by all before the first CTA goes on)
+            if (rank) return;                // the rest is too little for all: other rows have the room
+            arrange((int)listed);
+            // the last token of the list before which less than `target` lies, and the tokens up to it that stay
+            constexpr int EACH = CAP / NT;
+            double z[EACH];
+            u64 v[EACH], mine = 0, total;
 #pragma unroll
-                for (int k = 0; k < EACH; ++k) {
-                    const int i = tid * EACH + k;
-                    z[k] = i < (int)listed ? w.place(logit_of(s.list[i])) : -INFINITY;
-                    v[k] = w.of(z[k], s.two_to);
-                    mine += v[k];
-                }
-                u64 lies = before + block_scan<u64>(mine, s.warp_sum, &total);
-                uint32_t last = 0;
-#pragma unroll
-                for (int k = 0; k < EACH; ++k) {
-                    const int i = tid * EACH + k;
-                    if (i < (int)listed && lies < target) {
-                        last = i + 1;
-                        if (z[k] >= floor_z) {
-                            const int number = token_of(s.list[i]), c = number / a.share;
-                            const int o = (int)((reinterpret_cast<uintptr_t>(row + (long long)c * a.share) & 15) / sizeof(T));
-                            const int in = number - c * a.share + o, all_in = min(a.vocab - c * a.share, a.share) + o;
-                            atomicAdd(&s.pieces[c * NW + in / 4 / ceil_div((all_in + 3) / 4, NW)], v[k]);
-                        }
-                    }
-                    lies += v[k];
-                }
-                last = __reduce_max_sync(0xffffffffu, last);
-                __syncthreads();
-                if (lane == 0) s.warp_sum[warp] = last;
-                __syncthreads();
-                u64 most_at = 1;
-                for (int k = 0; k < NW; ++k) most_at = max(most_at, s.warp_sum[k]);
-                __syncthreads();   // (read by all before the next scan writes there)
-                // the piece in which the token lies
-                const u64 here = tid < ranks * NW ? s.pieces[tid] : 0;
-                u64 left_over;
-                u64 passed = block_scan<u64>(here, s.warp_sum, &left_over);
-                const u64 goal = aim(left_over);
-                if (passed <= goal && goal < passed + here) {
-                    for (int c = 0; c < ranks; ++c) {
-                        peer_st(peer(&s.told[0], c), (u64)tid);
-                        peer_st(peer(&s.told[1], c), goal - passed);
-                        peer_st(peer(&s.told[2], c), listed ? s.list[most_at - 1] : 0);
-                    }
-                }
+            for (int k = 0; k < EACH; ++k) {
+                const int i = tid * EACH + k;
+                z[k] = i < (int)listed ? w.place(logit_of(s.list[i])) : -INFINITY;
+                v[k] = w.of(z[k], s.two_to);
+                mine += v[k];
             }
-            if (ranks > 1) cluster_meet();
-            else __syncthreads();
-            if ((int)(s.told[0] / NW) != rank) return;
-            const u64 goal = s.told[1], bar = s.told[2];
-            const int p0 = min(quads, (int)(s.told[0] % NW) * piece), p1 = min(quads, p0 + piece);
-            const int per = ceil_div(p1 - p0, NT), j0 = min(p1, p0 + tid * per), j1 = min(p1, j0 + per);
+            u64 lies = before + block_scan<u64>(mine, s.warp_sum, &total);
+            uint32_t last = 0;
+#pragma unroll
+            for (int k = 0; k < EACH; ++k) {
+                const int i = tid * EACH + k;
+                if (i < (int)listed && lies < target) {
+                    last = i + 1;
+                    if (z[k] >= floor_z) {
+                        const int number = token_of(s.list[i]), c = number / a.share;
+                        const int o = (int)((reinterpret_cast<uintptr_t>(row + (long long)c * a.share) & 15) / sizeof(T));
+                        const int in = number - c * a.share + o, all_in = min(a.vocab - c * a.share, a.share) + o;
+                        atomicAdd(&s.pieces[c * NW + in / 4 / ceil_div((all_in + 3) / 4, NW)], v[k]);
+                    }
+                }
+                lies += v[k];
+            }
+            last = __reduce_max_sync(0xffffffffu, last);
+            __syncthreads();
+            if (lane == 0) s.warp_sum[warp] = last;
+            __syncthreads();
+            u64 most_at = 1;
+            for (int k = 0; k < NW; ++k) most_at = max(most_at, s.warp_sum[k]);
+            __syncthreads();   // (read by all before the next scan writes there)
+            // the piece in which the token lies, and what its tokens' sum has to exceed
+            const u64 bar = listed ? s.list[most_at - 1] : 0;
+            const u64 here = tid < ranks * NW ? s.pieces[tid] : 0;
+            u64 left_over;
+            if (tid == 0) s.found[0] = s.found[1] = 0;
+            const u64 passed = block_scan<u64>(here, s.warp_sum, &left_over);
+            const u64 goal = aim(left_over);
+            if (passed <= goal && goal < passed + here) s.found[0] = (u64)tid, s.found[1] = goal - passed;
+            __syncthreads();
+            const unsigned which = (unsigned)s.found[0];
+            const int c = (int)(which / NW);
+            const u64 rest = s.found[1];
+            const T* xc = row + (long long)c * a.share;   // of that CTA's share
+            const int oc = (int)((reinterpret_cast<uintptr_t>(xc) & 15) / sizeof(T)), nc = min(a.vocab - c * a.share, a.share);
+            const int qc = (oc + nc + 3) / 4, pc = ceil_div(qc, NW);
+            const int p0 = min(qc, (int)(which % NW) * pc), p1 = min(qc, p0 + pc);
+            const int per = ceil_div(4 * (p1 - p0), NT), e0 = min(4 * p1, 4 * p0 + tid * per), e1 = min(4 * p1, e0 + per);
             auto weight_at = [&](int e) -> u64 {   // of place e among the quads
-                const float l = e >= off && e - off < n ? at(e - off) : -INFINITY;
-                if (l == -INFINITY) return 0;
-                // above the bins, or of the bins and not below the border
-                if (place_key(l, lo + e - off) < bar) return 0;
+                const int i = e - oc;
+                if (i < 0 || i >= nc) return 0;
+                const float l = clean(load_one(xc + i));
+                if (l == -INFINITY || place_key(l, c * a.share + i) < bar) return 0;
                 const double z = w.place(l);
                 return z >= floor_z ? w.of(z, s.two_to) : 0;
             };
-            u64 mine = 0, total;
-            for (int e = 4 * j0; e < 4 * j1; ++e) mine += weight_at(e);
-            u64 here = block_scan<u64>(mine, s.warp_sum, &total);
-            if (here <= goal && goal < here + mine)
-                for (int e = 4 * j0; e < 4 * j1; ++e) {
-                    here += weight_at(e);
-                    if (goal < here) {
-                        a.out[r] = lo + e - off;
+            u64 sum_here = 0, all;
+            for (int e = e0; e < e1; ++e) sum_here += weight_at(e);
+            u64 at_e = block_scan<u64>(sum_here, s.warp_sum, &all);
+            if (at_e <= rest && rest < at_e + sum_here)
+                for (int e = e0; e < e1; ++e) {
+                    at_e += weight_at(e);
+                    if (rest < at_e) {
+                        a.out[r] = c * a.share + e - oc;
                         break;
                     }
                 }

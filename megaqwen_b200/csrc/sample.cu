@@ -57,7 +57,7 @@ constexpr int FRAC = 43;            // a weight of 1 is 2^43
 constexpr double ONE = 8796093022208.0;
 constexpr int MAX_VOCAB = 1 << 20;  // a row's sum stays below 2^63
 constexpr float COUNT_SPAN = 40.f;  // logits below the maximum that the histogram of a count spreads over its bins
-constexpr double MASS_SPAN = 44.0;  // octaves below the maximum past which a weight is nothing
+constexpr double MASS_SPAN = 20.0;  // octaves below the maximum that the histogram of a mass spreads over its bins
 
 struct Args {
     const void* logits;
@@ -214,7 +214,7 @@ __device__ __forceinline__ int block_sum_of(int v, u64* sm) {
     return all;
 }
 // The same for an estimate.
-__device__ __forceinline__ double block_scan_double(double v, double* sm) {
+__device__ __forceinline__ double block_scan_double(double v, double* sm, double* total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     double x = v;
 #pragma unroll
@@ -225,9 +225,13 @@ __device__ __forceinline__ double block_scan_double(double v, double* sm) {
     __syncthreads();
     if (lane == 31) sm[warp] = x;
     __syncthreads();
-    double before = 0;
-    for (int w = 0; w < warp; ++w) before += sm[w];
+    double before = 0, all = 0;
+    for (int w = 0; w < NW; ++w) {
+        if (w < warp) before += sm[w];
+        all += sm[w];
+    }
     __syncthreads();
+    *total = all;
     return before + x - v;
 }
 
@@ -627,18 +631,27 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
             sum4 += most[k];
             edge *= step;
         }
-        double up_to = block_scan_double(sum4, reinterpret_cast<double*>(s.warp_sum));
+        if (tid == NT - 1) s.ends[0] = (u64)__double_as_longlong(most[3]);
+        double all_bins;
+        double here = block_scan_double(sum4, reinterpret_cast<double*>(s.warp_sum), &all_bins);
+        const double last_bin = __longlong_as_double((long long)s.ends[0]);
         if (tid == 0) s.found[0] = BINS - 1, s.found[1] = BINS - 1;
         __syncthreads();
         int lo_bin = BINS - 1, hi_bin = BINS - 1;
-        // of the sums' rounding and of the edges' (fp32: 44 octaves to 2^-24 of them, 2^-18 of a weight)
-        const double margin = 1.0 + 2e-5;
+        // The tokens up to a bin are at least and at most so much by the bins up to it, and by the total less the bins behind
+        // it: whichever is less far from its edges (at a top_p of 0.9 the latter, by nine times).
+        // margin: of the sums' rounding and of the edges' (fp32: 20 octaves to 2^-24 of them, 2^-19 of a weight); slack: of
+        // the total's and of the weights' rounding to units
+        const double margin = 1.0 + 2e-5, whole = sum * ONE, slack = whole * 1e-11 + (double)a.vocab;
 #pragma unroll
-        for (int k = 3; k >= 0; --k) {   // (from the last on: the first that qualifies remains)
-            double here = up_to;
-            for (int i = 0; i <= k; ++i) here += most[i];
-            if (here * margin >= (double)target) lo_bin = 4 * tid + k;
-            if (here * step / margin >= (double)target + 1.0 && 4 * tid + k < BINS - 1) hi_bin = 4 * tid + k;
+        for (int k = 0; k < 4; ++k) {
+            here += most[k];
+            const double behind = all_bins - here;
+            const double high = fmin(here * margin, whole - fmax(behind - last_bin, 0.0) * step / margin) + slack;
+            const double least_sum = fmax(here * step / margin, whole - behind * margin) - slack;
+            const int b = 4 * tid + k;
+            if (high >= (double)target) lo_bin = min(lo_bin, b);
+            if (least_sum >= (double)target + 1.0 && b < BINS - 1) hi_bin = min(hi_bin, b);
         }
         if (lo_bin < BINS - 1) atomicMin(&s.found[0], (u64)lo_bin);
         if (hi_bin < BINS - 1) atomicMin(&s.found[1], (u64)hi_bin);

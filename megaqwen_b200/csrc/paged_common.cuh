@@ -114,6 +114,7 @@ __device__ __forceinline__ uint32_t cluster_size() {
     return r;
 }
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();   // the aligned form takes whole warps
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void st_peer(uint32_t addr, uint32_t rank, uint32_t v) {

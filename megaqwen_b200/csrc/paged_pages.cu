@@ -571,6 +571,9 @@ __global__ void __launch_bounds__(MOVE_THREADS) compact_move_kernel(Geo g, Tab t
 // down first, and put back where any sequence turns out wrong.  The move kernel takes (sequence, tensor, four layers, head)
 // to a warp, ACCEPT_ROWS rows of each layer in flight: a row only ever moves down, from row path[i] >= i of the tree to
 // row i, so a batch of rows that is read before it is written cannot overwrite what a later batch reads.
+//
+// 32 trees of 64 nodes, 8 accepted, 28 layers, with the room reserved before: 21 us (reserve 6, plan 12, move 10, each alone),
+// 51 MB read and written; bound by the chain of reads of the plan.
 constexpr int ACCEPT_TREE = 256;    // nodes
 constexpr int ACCEPT_ROWS = 8, ACCEPT_LAYERS = 4;
 

@@ -23,6 +23,16 @@
 // through the masked tiles' values, puts zeros in their place and notes where they
 // were, and a row that does see one has a NaN in that channel at the end.
 //
+// Bound: the tensor core and the softmax beside it, about equal.  A step of 64 keys of both streams is four products of 256
+// rows' halves, 4 x 128 x 64 x D: 768 cycles at D = 128 by the pipe's own rate (48 a k-step of 16 for 64 columns, of which
+// 16 only fill it), and 128 x 64 exponentials a stream, 1060 cycles of the function unit.  What is longer than either
+// is the chain score, weights, product of a stream.  Windows of 8064 keys for 4736 tokens: 925 TFLOP/s, 0.56 of cuBLAS.
+// 8 prompts of 2000 in a window of 1024: 174 us, 0.29: an item's 128 tokens see 1024 keys each in 10 or 11 tiles of 128, three
+// or four of them masked and their values looked through, and items are short against their start and end.  32 trees of 64
+// on 8192: 154 us here and 11 in the join, alone; 811 MB of K and V at 5.3 TB/s, 0.80 of the copy rate.
+//
+// Tried: tiles prefetched into L2, 128 keys in one buffer, rolled loops over the MMAs, MMA code specialised by case: all slower.
+//
 // An item that a run's end cuts leaves a part (m, l, acc) per row and run, which
 // the join adds in the order of the positions.
 #pragma once

@@ -29,7 +29,7 @@
 // is the chain score, weights, product of a stream.  Windows of 8064 keys for 4736 tokens: 925 TFLOP/s, 0.56 of cuBLAS.
 // 8 prompts of 2000 in a window of 1024: 174 us, 0.29: an item's 128 tokens see 1024 keys each in 10 or 11 tiles of 128, three
 // or four of them masked and their values looked through, and items are short against their start and end.  32 trees of 64
-// on 8192: 154 us here and 11 in the join, alone; 811 MB of K and V at 5.3 TB/s, 0.80 of the copy rate.
+// on 8192: 154 us here and 11 in the join, alone; 811 MB of K and V at 5.4 TB/s, 0.82 of the copy rate.
 //
 // Tried: tiles prefetched into L2, 128 keys in one buffer, rolled loops over the MMAs, MMA code specialised by case: all slower.
 //

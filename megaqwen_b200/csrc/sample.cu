@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
     // bins of equal width in the logit, from the maximum down
     float fine = 0.f, span = 0.f;
     auto spread = [&](float most) {
-        span = fminf(top - least, most);
+        span = fminf(fminf(top - least, most), 3.402823466e38f);   // (of a number: past it lies the last bin)
         fine = span > 0.f ? (float)BINS / span : 0.f;
     };
     auto bin_of = [&](float l) -> int {

@@ -281,7 +281,7 @@ class PagedDecoder:
         :meth:`draw` with its arguments).  A sequence keeps the first node and those drafted ones that were chosen at
         the node before them, and the list returned holds the tokens chosen at the kept nodes: its last one is not in the
         cache yet.  The other nodes' room is given back.  Where ``choose`` raises, each sequence keeps its first node, as
-        after a step.  Reads the counts, so it synchronises.
+        after a step.  Reads the whole context, whatever ``sparse_pages``; synchronises, for the counts.
         """
         slots, tokens, parents = list(slots), [list(t) for t in tokens], [list(p) for p in parents]
         self._known(slots)

@@ -179,6 +179,18 @@ def test_next_to_the_largest(sample, dtype, rule):
     check(sample, x, torch.rand(5, device="cuda", generator=g), **rule)
 
 
+@pytest.mark.parametrize("rule", [dict(), dict(top_p=0.3), dict(top_p=0.95), dict(top_k=700, top_p=0.6), dict(top_k=9000, top_p=0.6)])
+def test_differences_past_the_largest_number(sample, rule):
+    """Logits further apart than fp32 goes, at temperatures that bring them together."""
+    g, vocab = gen(14), 20011
+    x = (torch.rand(4, vocab, device="cuda", generator=g) * 2 - 1) * 3.3e38
+    x[2, 9:] = -3e38
+    t = torch.tensor([3e38, 1e38, 2e38, 3e37], device="cuda")
+    check(sample, x, torch.rand(4, device="cuda", generator=g), temperature=t, **rule)
+    flat = torch.full((4,), math.inf, device="cuda")    # all weights alike
+    check(sample, x, torch.rand(4, device="cuda", generator=g), temperature=flat, **rule)
+
+
 def test_numbers_at_the_ends(sample):
     x = rows(gen(8), 6, 5003, torch.float32)
     u = torch.tensor([0.0, -1.0, 1.0, 2.0, math.nan, 1 - 2.0 ** -24], device="cuda")

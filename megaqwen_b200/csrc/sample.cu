@@ -172,12 +172,10 @@ struct Weight {
         p = fma(p, r, 1.0) * two_to[n & (TABLE - 1)];
         return __hiloint2double(__double2hiint(p) + (n >> 7) * (1 << 20), __double2loint(p));
     }
-    // in multiples of 2^-43, rounded to the nearest
+    // in multiples of 2^-43, rounded to the nearest: the last place of numbers from 2^9 to 2^10
     __device__ __forceinline__ u64 of(double z, const double* two_to) const {
-        if (!(z > -(FRAC + 1.0) * TABLE)) return 0;   // (NaN, too)
-        const u64 b = (u64)__double_as_longlong(as_double(z, two_to));
-        const int s = 52 - FRAC - ((int)(b >> 52) - 1023);
-        return ((b & 0xfffffffffffffull | 1ull << 52) + (1ull << (s - 1))) >> s;
+        static_assert(FRAC == 43, "the last place of 2^9");
+        return (u64)__double_as_longlong(as_double(z, two_to) + 512.0) - (u64)0x4080000000000000ull;
     }
     __device__ __forceinline__ u64 of(float l, const double* two_to) const { return of(place(l), two_to); }
 };
@@ -673,18 +671,23 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
             if (!__any_sync(0xffffffffu, fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) >= low)) continue;
             const float l4[4] = {q.x, q.y, q.z, q.w};
             bool take[4], any = false;
+            unsigned over = 0;   // tokens above the bins
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int b = bin_of(l4[k]);
                 const bool there = l4[k] > -INFINITY;
                 take[k] = there && b >= lo_bin && b <= hi_bin;
                 any |= take[k];
-                if (there && b < lo_bin) {
-                    const double z = w.place(l4[k]);
-                    const u64 v = w.of(z, s.two_to);
-                    above += v;
-                    if (z >= floor_z) stay += v;
-                }
+                over |= (unsigned)(there && b < lo_bin) << k;
+            }
+            while (__any_sync(0xffffffffu, over)) {   // few of a warp's 128, as a rule: each lane's next one
+                const int k = __ffs((int)over) - 1;
+                const float l = k == 0 ? q.x : k == 1 ? q.y : k == 2 ? q.z : q.w;
+                const double z = w.place(l);
+                const u64 v = over ? w.of(z, s.two_to) : 0;
+                above += v;
+                if (z >= floor_z) stay += v;
+                over &= over - 1;
             }
             if (!__any_sync(0xffffffffu, any)) continue;
 #pragma unroll

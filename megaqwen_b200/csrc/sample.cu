@@ -29,7 +29,7 @@
 //
 // Bound: latency for one row (15 us of 152k tokens: six meetings of the cluster of 1 to 2 us each, the first CTA's steps);
 // for many, a nucleus is a chain per row of load, histogram, sums, sort, on two CTAs an SM: 256 rows of 152k in 16 bits
-// 309 us (0.25 TB/s), 64 rows with rules of their own, fp32, 83 us (0.47 TB/s).  Profiled: issue slots 40 % busy, 64-bit
+// 306 us (0.25 TB/s), 64 rows with rules of their own, fp32, 83 us (0.47 TB/s).  Profiled: issue slots 40 % busy, 64-bit
 // floating point 13 %, a third of the warps' time in barriers.
 #include <algorithm>
 #include <cmath>

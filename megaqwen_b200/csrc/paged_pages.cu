@@ -567,12 +567,12 @@ __global__ void __launch_bounds__(MOVE_THREADS) compact_move_kernel(Geo g, Tab t
 // the sequence ends behind them, and pages past its end are given back.
 //
 // One cluster plans, a warp to a sequence: the walk looks at 32 nodes at a time (a ballot finds the lowest child), which
-// is the latency of a chain of reads for each node passed.  As for free, the counts of the pages to give back are taken
-// down first, and put back where any sequence turns out wrong.  The move kernel takes (sequence, tensor, four layers, head)
+// is the latency of a chain of reads for each node passed.  When all that is written has been checked, the counts of the
+// pages to give back are taken down, as for free, and put back where one was not there to take.  The move kernel takes (sequence, tensor, four layers, head)
 // to a warp, ACCEPT_ROWS rows of each layer in flight: a row only ever moves down, from row path[i] >= i of the tree to
 // row i, so a batch of rows that is read before it is written cannot overwrite what a later batch reads.
 //
-// 32 trees of 64 nodes, 8 accepted, 28 layers, with the room reserved before: 21 us (reserve 6, plan 12, move 10, each alone),
+// 32 trees of 64 nodes, 8 accepted, 28 layers, with the room reserved before: 22 us (reserve 6, plan 13, move 10, each alone),
 // 51 MB read and written; bound by the chain of reads of the plan.
 constexpr int ACCEPT_TREE = 256;    // nodes
 constexpr int ACCEPT_ROWS = 8, ACCEPT_LAYERS = 4;
@@ -597,12 +597,12 @@ __device__ __forceinline__ int tree_start(const AcceptArgs& a, int i) { return a
 
 __global__ void __launch_bounds__(PLAN_THREADS) accept_plan_kernel(Tab t, AcceptArgs a) {
     __shared__ unsigned bits[MAX_SLOTS / 32];
-    __shared__ int wrong;   // the highest code found
+    __shared__ int wrong[2];   // the highest code found, by the checks and by the counts
     pdl_wait();
     pdl_trigger();
     const int ranks = (int)cluster_size(), rank = (int)cluster_rank();   // (the grid is one cluster)
     const int per = blockDim.x / 32, lane = threadIdx.x & 31, warp = rank * per + (threadIdx.x >> 5), warps = ranks * per;
-    if (threadIdx.x == 0) wrong = 0;
+    if (threadIdx.x == 0) wrong[0] = wrong[1] = 0;
     int code = 0;
     if (a.q_starts) {
         for (int i = threadIdx.x; i < a.n; i += blockDim.x)
@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) accept_plan_kernel(Tab t, Accept
     if (!in_order) {   // all CTAs alike
         if (rank == 0 && code) note_status(t.status, code);
         for (long long i = (long long)rank * blockDim.x + threadIdx.x; i < max(a.total, a.n); i += ranks * blockDim.x) {
-            if (i < a.total) a.path[i] = a.emitted[i] = -1;
+            if (i < a.total) a.path[i] = a.emitted[i] = a.positions[i] = -1;
             if (i < a.n) a.count[i] = 0;
         }
         if (rank == 0 && threadIdx.x == 0) a.head[0] = 0;
@@ -694,19 +694,33 @@ __global__ void __launch_bounds__(PLAN_THREADS) accept_plan_kernel(Tab t, Accept
             const int sp = row[(base + from) >> shift], dp = row[(base + k) >> shift];
             if (sp < 0 || sp >= t.pages || dp < 0 || dp >= t.pages || t.refs[dp] != 1) bad = true;
         }
-        if (give_back(row, pages_of(base + m, t.page), pages_of(len, t.page), -1)) bad = true;
         if (bad) code = max(code, (int)MQ_ERR_BAD_PAGE);
     }
-    if (code) atomicMax(&wrong, code);
-    __syncthreads();
-    if (ranks > 1) {
-        const int mine = wrong;
+    // the highest code of all threads of the cluster; also a barrier
+    auto agree = [&](int k) {
+        if (code) atomicMax(&wrong[k], code);
         __syncthreads();
-        if (mine && threadIdx.x < ranks) red_peer_max(smem_u32(&wrong), threadIdx.x, mine);
-        __syncwarp();
-        cluster_sync();   // also orders the counts taken before those put back
+        if (ranks > 1) {
+            const int mine = wrong[k];
+            __syncthreads();
+            if (mine && threadIdx.x < ranks) red_peer_max(smem_u32(&wrong[k]), threadIdx.x, mine);
+            __syncwarp();
+            cluster_sync();
+        }
+        code = *(volatile int*)&wrong[k];
+    };
+    agree(0);
+    // No count is taken before every page that is written has been seen to have one holder: a holder that gives it back in
+    // this call may still read its rows.
+    const bool taken = !code;
+    if (taken) {
+        for (int i = warp; i < a.n; i += warps) {
+            const int s = a.slots[i], len = t.lengths[s], m = a.count[i];
+            const int base = len - (tree_start(a, i + 1) - tree_start(a, i));
+            if (give_back(t.table + s * t.row, pages_of(base + m, t.page), pages_of(len, t.page), -1)) code = MQ_ERR_BAD_PAGE;
+        }
+        agree(1);   // also orders the counts taken before those put back
     }
-    code = *(volatile int*)&wrong;
     if (rank == 0 && threadIdx.x == 0) {
         if (code) note_status(t.status, code);
         a.head[0] = code == 0;
@@ -717,8 +731,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) accept_plan_kernel(Tab t, Accept
         const int base = len - ql, keep = pages_of(base + m, t.page), used = pages_of(len, t.page);
         __syncwarp();
         if (code) {
-            if (m > 0) give_back(row, keep, used, 1);   // (below 1: its pages were not looked at)
-            for (int k = lane; k < ql; k += 32) a.path[q0 + k] = a.emitted[q0 + k] = -1;
+            if (taken) give_back(row, keep, used, 1);
+            for (int k = lane; k < ql; k += 32) a.path[q0 + k] = a.emitted[q0 + k] = a.positions[q0 + k] = -1;
             if (lane == 0) a.count[i] = 0;
             continue;
         }

@@ -224,6 +224,41 @@ def test_wrong_calls_change_nothing(paged):
     refused(m, 9, lambda c: c.refs.__setitem__(page, 0))
 
 
+def test_refused_calls_leave_the_index(paged):
+    """What a call finds in its workspace (places of full pages, here) must not reach the index when it is refused."""
+    trees = [random_tree(i, 20, back=3) for i in range(18)]
+    m = Model(paged, [40] * 18, trees, 16, layers=2, index=True, seed=5)
+    m.cache.index.fill_(99)
+    slots, parents, tokens, chosen, starts = m.args()
+    wrong = list(parents)
+    wrong[7] = 9
+    for args, code in (((slots, wrong, tokens, chosen, starts), 1), (([*slots[:-1], slots[0]], parents, tokens, chosen, starts), 8)):
+        left = [torch.full((len(parents) * 6 + 64,), 15, dtype=torch.int32, device="cuda") for _ in range(4)]
+        del left   # 15: a slot, and the last row of a page
+        refused(m, code, lambda c: None, args)
+        m.cache.status.zero_()
+
+
+def test_a_written_page_given_back_by_another(paged):
+    """Two sequences that share the pages of their trees: neither may write there, whatever the other gives back."""
+    page, n = 16, 48
+    for chosen_of_other in (5, 99):
+        c = paged.PagedKVCache(12, 3, 6, num_layers=1, num_kv_heads=1, head_dim=64, page_size=page)
+        c.reserve([0], [page + n])
+        c.k_pages.normal_()
+        c.fork([0], [1])
+        before = [x.clone() for x in (c.k_pages, c.v_pages, c.page_table, c.lengths, c.refs)]
+        # the first takes its second branch, of 40 nodes behind 7 others; the other one all or only its root
+        parents = [-1, 0, 1, 2, 3, 4, 5, 6] + [0] + list(range(8, 47))
+        tokens = [0] + [1] * 7 + [2] + [3] * 39
+        chosen = [2] + [9] * 7 + [3] * 39 + [4]
+        other = [chosen_of_other] * n
+        path, emitted, count = c.accept([0, 1], parents * 2, tokens * 2, chosen + other, [0, n, 2 * n])
+        assert c.status.item() == 9 and not bool(count.any()) and bool((path == -1).all())
+        for a, b in zip(before, (c.k_pages, c.v_pages, c.page_table, c.lengths, c.refs)):
+            assert torch.equal(a, b)
+
+
 def test_too_many_nodes(paged):
     m = Model(paged, [3, 4], [[-1] * 257, [-1, 0]], 16)
     refused(m, 1, lambda c: None)

@@ -7,7 +7,7 @@
 // CTA per SM), each item as long as it has tiles.
 //
 // A CTA runs two streams, A and B, each with its own rows of Q, two buffers for the
-// scores of 64 keys (weights overwrite their scores as 16-bit values) and its own
+// scores of 64 keys (weights overwrite their scores, two 16-bit pieces each) and its own
 // accumulator in TMEM.  With more than 128 rows each has half of them and takes both
 // halves of every tile; with up to 128 both take the same rows, A the first half of
 // each tile and B the second, and the accumulators, side by side in TMEM, are joined
@@ -651,8 +651,10 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                 if (elect_one()) {
                     if (pv) {
 #pragma unroll
-                        for (int k = 0; k < HK / 16; ++k)   // 16 keys: 8 columns of weights
+                        for (int k = 0; k < HK / 16; ++k) {   // 16 keys: 8 columns of weights, 8 of their second pieces
                             mma_ts(o, buffer + 8 * k, vl + k * (2048 >> 4), id_o, k || i);
+                            mma_ts(o, buffer + HK / 2 + 8 * k, vl + k * (2048 >> 4), id_o, true);
+                        }
                         if (i + 2 >= steps) tc_commit(&o_full[q]);
                         if (used) tc_commit(&v_empty[vc & 1]);
                     }
@@ -769,20 +771,28 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                     }
                 }
                 const uint64_t scale2 = two_of(scale, scale), u2 = m == -INFINITY ? 0ull : two_of(-m, -m);
+                const uint64_t minus1 = two_of(-1.f, -1.f);
                 uint64_t sum0 = 0ull, sum1 = 0ull;
 #pragma unroll
                 for (int c = 0; c < HK; c += 32) {
-                    uint32_t pk[16];   // 32 weights in 16 columns, over the scores
+                    // 32 weights in 16 columns and what they are short of in 16 more, over the scores: with one piece the
+                    // result would be as far off as its own rounding
+                    uint32_t pk[16], rest[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                         float p0, p1;
                         halves(fma2(two_of(sv[c + 2 * k], sv[c + 2 * k + 1]), scale2, u2), p0, p1);
                         p0 = ex2(p0);
                         p1 = ex2(p1);
-                        (k & 1 ? sum1 : sum0) = add2(k & 1 ? sum1 : sum0, two_of(p0, p1));
+                        const uint64_t both = two_of(p0, p1);
+                        (k & 1 ? sum1 : sum0) = add2(k & 1 ? sum1 : sum0, both);
                         pk[k] = Elem<T>::pack(p0, p1);
+                        const float2 b = Elem<T>::up2(pk[k]);
+                        halves(fma2(two_of(b.x, b.y), minus1, both), p0, p1);
+                        rest[k] = Elem<T>::pack(p0, p1);
                     }
                     tmem_st16_nowait(sb + (c >> 1), pk);
+                    tmem_st16_nowait(sb + HK / 2 + (c >> 1), rest);
                 }
                 float s0, s1;
                 halves(add2(sum0, sum1), s0, s1);

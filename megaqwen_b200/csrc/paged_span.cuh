@@ -693,7 +693,11 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         float* tops = reinterpret_cast<float*>(smem + L::TOP);
         uint8_t* stage = smem + L::STAGE + (warp - 4) * 2048;
         ulonglong2* hits = reinterpret_cast<ulonglong2*>(smem + L::HIT);
-        constexpr float GROW = 14.f;
+        // fp16 ends 24 octaves below 1 and 16 above it: weights stand 5 octaves higher there and may grow to 2^15.5, so that what
+        // is lost of one is at most 2^-30 of the row's largest, and 2^17 of them are 2^-13 of it.  8 prompts of 2000, as the
+        // sums are rescaled more often the less room is left: 5 octaves 202 us, 6 211, 10 239.
+        constexpr bool HALF = Elem<T>::MAX < 1e5f;
+        constexpr float GROW = HALF ? 15.5f : 14.f, BELOW = HALF ? 5.f : 0.f;
         uint32_t g = 0, no = 0;  // steps (64 keys) so far, alike for both streams; o_full so far
         int nv = 0, np = 0;      // tiles of the items before, meetings
         bool ok = true;
@@ -748,12 +752,13 @@ span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
 #pragma unroll
                 for (int k = 8; k < HK; k += 2) mx[(k >> 1) & 3] = max3(mx[(k >> 1) & 3], sv[k], sv[k + 1]);
                 const float tmax = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale;
-                // a row's reference moves only when its maximum is more than 2^14 above it: weights stay below that (fp16 ends at
-                // 2^16), and one of the first keys, among few, is often some octaves below the row's maximum
+                // a row's reference is its maximum (fp16: some octaves below it) and moves only when a maximum is many octaves above it:
+                // weights stay below 2^GROW, and one of the first keys, among few, is often some octaves below the row's maximum
                 float corr = 1.f;
                 if (tmax > m + GROW) {
-                    corr = m == -INFINITY ? 1.f : ex2(m - tmax);   // (nothing is summed before the first key that the row sees)
-                    m = tmax;
+                    const float to = tmax - BELOW;
+                    corr = m == -INFINITY ? 1.f : ex2(m - to);   // (nothing is summed before the first key that the row sees)
+                    m = to;
                 }
                 l *= corr;
                 if (i && __any_sync(0xffffffffu, corr != 1.f)) {

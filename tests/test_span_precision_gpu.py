@@ -66,3 +66,53 @@ def test_one_key_far_above_the_sinks(paged, dtype, above):
          tree_mask([-1] * n, t)),
     ):
         close(got, reference(p, 0, q, seen, 1.0, 1)[0], vmax)
+
+
+class Flat:
+    """Sequences of one length on the same pages: the first key `above` nats above all others, its value -1, theirs 1."""
+
+    def __init__(self, seqs, length, hkv, d, dtype, above, page=128):
+        pages = -(-length // page)
+        self.k = torch.zeros(pages, 1, hkv, page, d, dtype=dtype, device="cuda")
+        self.v = torch.ones_like(self.k)
+        self.k[0, 0, :, 0, 3] = above / 4
+        self.v[0, 0, :, 0] = -1
+        self.table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(seqs, 1)
+        self.lengths = torch.full((seqs,), length, dtype=torch.int32, device="cuda")
+        self.slots = torch.arange(seqs, dtype=torch.int32, device="cuda")
+
+    def q(self, tokens, heads):
+        q = torch.zeros(tokens, heads, self.k.shape[4], dtype=self.k.dtype, device="cuda")
+        q[..., 3] = 4
+        return q
+
+
+def flat_result(above, keys):
+    """Of the first key and `keys - 1` others; `above` as the type has it."""
+    w = (keys - 1) * math.exp(-above)
+    return (w - 1) / (w + 1)
+
+
+ABOVE = [8.0, 16.5, 17.0, 17.25, 18.5, 20.0]   # times 1/4 they are 16-bit numbers; near 2^-24 and below
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("above", ABOVE)
+@pytest.mark.parametrize("length,n", [(30000, 9), (100000, 9), (30000, 70)])
+def test_many_small_weights_behind_a_sink(paged, dtype, above, length, n):
+    """Weights of 2^-25 of a row's largest count when there are enough of them (many rows to a sequence, and sequences enough
+    for one to be a CTA's work from its first position to its last)."""
+    seqs = 300
+    p = Flat(seqs, length, 1, 64, dtype, above)
+    q = p.q(seqs * n, 2)
+    starts = torch.arange(0, seqs * n + 1, n, dtype=torch.int32, device="cuda")
+    got = paged.window_attend(q, p.k, p.v, p.table, p.lengths, p.slots, layer=0, window=length, q_starts=starts, scale=1.0)
+    ref = torch.tensor([flat_result(above, length - n + 1 + i) for i in range(n)], dtype=torch.float64, device="cuda")
+    close(got, ref.repeat(seqs)[:, None, None].expand_as(got), 1.0)
+    got = paged.window_attend(q, p.k, p.v, p.table, p.lengths, p.slots, layer=0, window=length // 2, sinks=1, q_starts=starts, scale=1.0)
+    ref = torch.full_like(got, flat_result(above, length // 2 + 1), dtype=torch.float64)
+    close(got, ref, 1.0)
+    tree = [-1] * n
+    got = paged.tree_attend(q, p.k, p.v, p.table, p.lengths, p.slots, dev(tree * seqs), layer=0, q_starts=starts, scale=1.0)
+    ref = torch.full_like(got, flat_result(above, length - n + 1), dtype=torch.float64)
+    close(got, ref, 1.0)

@@ -403,6 +403,9 @@ struct RowWarp {
     __device__ __forceinline__ void step(int stage, const int (&lim)[NT][2], bool mixed, float scale) {
         const uint32_t ks = ring + stage * STAGE, vs = ks + TILE;
         const int g = lane >> 2, mat = lane >> 3, r8 = lane & 7;
+        // Under a mask, where a few sinks may stand far above a long window, fp16 weights are held in units of 2^-14: one of 2^-25 is
+        // then no subnormal number of the type, of which half would be lost.  (Sums and parts are in the same unit.)
+        constexpr float UNIT = MASK && Elem<T>::MAX < 1e5f ? 16384.f : 1.f;
         auto sees = [&](int p, int lim_r) { return MASK ? (lim_r >> p & 1) != 0 : p < lim_r; };
         // S^T = K Q^T: positions g, g + 8; rows 2 t, 2 t + 1.  Even and odd k-steps in chains of their own.
         float s[NT][4], s2[NT][4];
@@ -440,7 +443,7 @@ struct RowWarp {
                 u[i] = mn == -INFINITY ? 0.f : mn;
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][i] = ex2(s[n][i] - u[i & 1]);
+            for (int i = 0; i < 4; ++i) s[n][i] = ex2(s[n][i] - u[i & 1]) * UNIT;
             l[n][0] = l[n][0] * corr[n][0] + (s[n][0] + s[n][2]);
             l[n][1] = l[n][1] * corr[n][1] + (s[n][1] + s[n][3]);
             // two pieces of the 16-bit type: one would cost as much accuracy as rounding the output does

@@ -116,3 +116,18 @@ def test_many_small_weights_behind_a_sink(paged, dtype, above, length, n):
     got = paged.tree_attend(q, p.k, p.v, p.table, p.lengths, p.slots, dev(tree * seqs), layer=0, q_starts=starts, scale=1.0)
     ref = torch.full_like(got, flat_result(above, length - n + 1), dtype=torch.float64)
     close(got, ref, 1.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("above", ABOVE)
+@pytest.mark.parametrize("n", [1, 2])
+def test_many_small_weights_single_tokens(paged, dtype, above, n):
+    """The same for few rows to a sequence, where a warp has thousands of positions."""
+    length, seqs = 40000, 2000
+    p = Flat(seqs, length, 2, 64, dtype, above)
+    q = p.q(seqs * n, 4)
+    starts = torch.arange(0, seqs * n + 1, n, dtype=torch.int32, device="cuda")
+    got = paged.window_attend(q, p.k, p.v, p.table, p.lengths, p.slots, layer=0, window=30000, sinks=1, q_starts=starts, scale=1.0)
+    close(got, torch.full_like(got, flat_result(above, 30001), dtype=torch.float64), 1.0)
+    got = paged.tree_attend(q, p.k, p.v, p.table, p.lengths, p.slots, dev([-1] * (seqs * n)), layer=0, q_starts=starts, scale=1.0)
+    close(got, torch.full_like(got, flat_result(above, length - n + 1), dtype=torch.float64), 1.0)

@@ -61,6 +61,10 @@ struct SpanSmem {
     static constexpr size_t bytes(int B) { return SCHED + (size_t)(4 * B + 2) * 4 + 1024; }
 };
 
+// the limit of a CTA, with the kernel's own sums of a warp
+static_assert(SpanSmem<128>::bytes(SPAN_SEQS) + SPAN_THREADS / 32 * sizeof(unsigned long long) <= 227 * 1024,
+              "the schedule of SPAN_SEQS sequences");
+
 // An item that is cut: the worker with its first tile leaves this for the join.
 struct alignas(16) SpanCut {
     int tok0, h, rows, runs;   // rows 0: none

@@ -636,7 +636,9 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         double all_bins;
         double here = block_scan_double(sum4, reinterpret_cast<double*>(s.warp_sum), &all_bins);
         const double last_bin = __longlong_as_double((long long)s.ends[0]);
-        if (tid == 0) s.found[0] = BINS - 1, s.found[1] = BINS - 1;
+        // (a spread too small to be divided into bins: all that is below the maximum is in the last one, above its edges too)
+        const bool told = fine < INFINITY;
+        if (tid == 0) s.found[0] = told ? BINS - 1 : 0, s.found[1] = BINS - 1;
         __syncthreads();
         int lo_bin = BINS - 1, hi_bin = BINS - 1;
         // The tokens up to a bin are at least and at most so much by the bins up to it, and by the total less the bins behind
@@ -655,7 +657,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
             if (least_sum >= (double)target + 1.0 && b < BINS - 1) hi_bin = min(hi_bin, b);
         }
         if (lo_bin < BINS - 1) atomicMin(&s.found[0], (u64)lo_bin);
-        if (hi_bin < BINS - 1) atomicMin(&s.found[1], (u64)hi_bin);
+        if (hi_bin < BINS - 1 && told) atomicMin(&s.found[1], (u64)hi_bin);
         __syncthreads();
         lo_bin = (int)s.found[0];
         hi_bin = (int)s.found[1];

@@ -592,17 +592,16 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         spread(mass_span);
         for (int i = tid; i < BINS; i += NT) s.count[i] = 0;
         __syncthreads();
-        // (the total in 64-bit floating point, in an order of its own, the same on every run)
         // Four tokens side by side and without branches: a weight is a chain of a dozen operations.  (Minus infinity counts
-        // for the last bin, whose number is only ever an upper bound, with a weight of 2^-1000.)
-        double sum = 0.0;
+        // for the last bin, whose number is only ever an upper bound, with a weight of 2^-1000: no unit.)
+        u64 sum = 0;
         float4 q = own_quad(tid, quads);
         for (int j = tid; j < quads; j += NT) {
             const float4 next = own_quad(j + NT, quads);
             const float l4[4] = {q.x, q.y, q.z, q.w};
-            double v[4];
+            u64 v[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = w.as_double(w.place(l4[k]), s.two_to);
+            for (int k = 0; k < 4; ++k) v[k] = w.of(l4[k], s.two_to);
 #pragma unroll
             for (int k = 0; k < 4; ++k) atomicAdd(&s.count[bin_of(l4[k])], 1u);
             sum += (v[0] + v[1]) + (v[2] + v[3]);
@@ -610,14 +609,14 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) s.warp_sum[warp] = (u64)__double_as_longlong(sum);
+        if (lane == 0) s.warp_sum[warp] = sum;
         __syncthreads();
-        sum = 0.0;
-        for (int k = 0; k < NW; ++k) sum += __longlong_as_double((long long)s.warp_sum[k]);
-        tell((u64)__double_as_longlong(sum), 0, 0, 0);   // (the counts are there, too)
-        sum = 0.0;
-        for (int c = 0; c < ranks; ++c) sum += __longlong_as_double((long long)s.slot[turn][c][0]);
-        const double t = (double)top_p * sum * ONE;
+        sum = 0;
+        for (int k = 0; k < NW; ++k) sum += s.warp_sum[k];
+        tell(sum, 0, 0, 0);   // (the counts are there, too)
+        sum = 0;
+        for (int c = 0; c < ranks; ++c) sum += s.slot[turn][c][0];
+        const double whole = (double)sum, t = (double)top_p * whole;
         const u64 target = max(t > 0.0 ? (u64)ceil(t) : 0, 1ull);   // the last token before which less than this lies
         // The bins in which that token can lie: a bin's weights are between those of its edges.  The last bin has no lower edge.
         uint32_t c4[4];
@@ -645,7 +644,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         // it: whichever is less far from its edges (at a top_p of 0.9 the latter, by nine times).
         // margin: of the sums' rounding and of the edges' (fp32: 20 octaves to 2^-24 of them, 2^-19 of a weight); slack: of
         // the total's and of the weights' rounding to units
-        const double margin = 1.0 + 2e-5, whole = sum * ONE, slack = whole * 1e-11 + (double)a.vocab;
+        const double margin = 1.0 + 2e-5, slack = whole * 1e-11 + (double)a.vocab;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             here += most[k];

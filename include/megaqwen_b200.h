@@ -428,7 +428,8 @@ int mq_paged_compact(const mq_paged_pool* src, const mq_paged_pool* dst, const m
  * layout of the nodes and -1 behind the last; count [n]: how many they are, 0
  * for a sequence without nodes.  The accepted rows of K and V move to the
  * tree's first positions (all layers), the sequence ends behind them, and pages
- * past its end lose a holder.  A page that is written must have no other holder.
+ * past its end lose a holder.  A page that is written must have no other holder,
+ * nor one inside which a sequence is cut (its next token is written there).
  * With an index in the pool, the records of the pages that are full then are
  * written again.  A call that is wrong anywhere changes nothing but its outputs
  * (-1 and 0).  t->workspace: mq_paged_accept_workspace_bytes(total) bytes,

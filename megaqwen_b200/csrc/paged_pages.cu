@@ -685,7 +685,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) accept_plan_kernel(Tab t, Accept
         for (int k = m + lane; k < ql; k += 32) a.path[q0 + k] = a.emitted[q0 + k] = -1;
         if (lane == 0) a.count[i] = m;
         __syncwarp();
-        // the pages of the rows that move, those written with no other holder
+        // the pages of the rows that move, those written, now or by the next token, with no other holder
         const int base = len - ql;
         bool bad = false;
         for (int k = lane; k < m; k += 32) {
@@ -693,6 +693,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) accept_plan_kernel(Tab t, Accept
             if (from == k) continue;
             const int sp = row[(base + from) >> shift], dp = row[(base + k) >> shift];
             if (sp < 0 || sp >= t.pages || dp < 0 || dp >= t.pages || t.refs[dp] != 1) bad = true;
+        }
+        if (lane == 0 && m < ql && ((base + m) & (t.page - 1))) {   // cut within a page: the next token is written there
+            const int p = row[(base + m - 1) >> shift];
+            if (p < 0 || p >= t.pages || t.refs[p] != 1) bad = true;
         }
         if (bad) code = max(code, (int)MQ_ERR_BAD_PAGE);
     }

@@ -321,7 +321,7 @@ class PagedDecoder:
             if chosen.numel() != nodes.numel():
                 raise ValueError("there must be a chosen token for each node")
             chosen = self._ints(chosen.reshape(-1))
-        except Exception as e:   # (a step has no such callback: the trees must not stay in the cache)
+        except BaseException as e:   # (a step has no such callback: the trees must not stay in the cache)
             failed, chosen = e, torch.full_like(nodes, -1)
         _, emitted, count = self.cache.accept(dev_slots, up, nodes, chosen, q_starts=starts)
         emitted, kept = emitted.tolist(), count.tolist()

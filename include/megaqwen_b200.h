@@ -553,7 +553,7 @@ typedef struct mq_paged_span_params {
     const int* lengths;          /* device int32 [num_slots], the query tokens included */
     const int* slots;            /* device int32 [num_seqs] */
     const int* q_starts;         /* device int32 [num_seqs + 1], optional */
-    int num_seqs;                /* at most 2048 */
+    int num_seqs;                /* at most 2048; many tokens to a sequence are fast up to 448 */
     int total_q;
     int num_q_heads;             /* a multiple of the pool's kv heads */
     int layer;

@@ -663,8 +663,8 @@ Shape shape_of(const mq_paged_attend_params* p) {
 }
 // The tensor-core kernel takes calls of more rows to a sequence than the 16 of a rows_kernel item on average (q through a
 // tensor map, whose strides are positive).  16 q and 8 kv heads x 128, rows_kernel against it: one tree of 16 nodes on 1000
-// positions 18.1 and 17.4 us, 16 trees of 31 on up to 6000 174 and 81, 32 of 64 on 8192 877 and 185; 8 prompts of 2000 in a
-// window of 1024 1151 and 174.  Below that its 128-row tiles are empty but for a few rows.
+// positions 18.1 and 18.5 us, 16 trees of 31 on up to 6000 174 and 91, 32 of 64 on 8192 877 and 210; 8 prompts of 2000 in a
+// window of 1024 1151 and 206.  Below that its 128-row tiles are empty but for a few rows.
 bool tc_span(const mq_paged_span_params* p) {
     const int grp = p->num_q_heads / p->pool->num_kv_heads;
     return (long long)p->total_q * grp > 16ll * p->num_seqs && grp <= PROWS / 2 && p->num_seqs <= SPAN_SEQS && (p->q_token > 0 || p->total_q == 1) &&

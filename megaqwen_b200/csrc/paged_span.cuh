@@ -23,13 +23,14 @@
 // through the masked tiles' values, puts zeros in their place and notes where they
 // were, and a row that does see one has a NaN in that channel at the end.
 //
-// Bound: the tensor core and the softmax beside it, about equal.  A step of 64 keys of both streams is four products of 256
-// rows' halves, 4 x 128 x 64 x D: 768 cycles at D = 128 by the pipe's own rate (48 a k-step of 16 for 64 columns, of which
-// 16 only fill it), and 128 x 64 exponentials a stream, 1060 cycles of the function unit.  What is longer than either
-// is the chain score, weights, product of a stream.  Windows of 8064 keys for 4736 tokens: 925 TFLOP/s, 0.56 of cuBLAS.
-// 8 prompts of 2000 in a window of 1024: 174 us, 0.29: an item's 128 tokens see 1024 keys each in 10 or 11 tiles of 128, three
-// or four of them masked and their values looked through, and items are short against their start and end.  32 trees of 64
-// on 8192: 154 us here and 11 in the join, alone; 811 MB of K and V at 5.4 TB/s, 0.82 of the copy rate.
+// Bound: the tensor core and the softmax beside it.  A step of 64 keys of both streams is the scores, 2 x 128 x 64 x D, and
+// twice that for the two pieces of the weights: 1536 cycles at D = 128 at the pipe's rate of 4096 products a cycle; beside
+// them 128 x 64 exponentials a stream, 1024 cycles of the function unit.  What is longer than either is the chain score,
+// weights, product of a stream.  Windows of 8064 keys for 4736 tokens: 372 us, 841 TFLOP/s (a weight's product counted once),
+// 0.50 of cuBLAS.  8 prompts of 2000 in a window of 1024: 206 us, 0.24: an item's 128 tokens see 1024 keys each in 10 or 11
+// tiles of 128, three or four of them masked and their values looked through, and items are short against their start and
+// end.  32 trees of 64 on 8192: 171 us here and 10 in the join, alone; 811 MB of K and V at 4.7 TB/s, 0.72 of the copy rate,
+// the tensor pipe active 49 % of the time.  One piece a weight was 338, 174 and 154 us.
 //
 // Tried: tiles prefetched into L2, 128 keys in one buffer, rolled loops over the MMAs, MMA code specialised by case: all slower.
 //

@@ -27,10 +27,10 @@
 // Rows that do not fit these (thousands of equal logits at a border, a large top_k) take the general form: a histogram
 // with exact sums for each border, refined until the border's bin can be sorted.
 //
-// Bound: latency for one row (15 us of 152k tokens: six meetings of the cluster of 1 to 2 us each, the first CTA's steps);
+// Bound: latency for one row (14 us of 152k tokens: five meetings of the cluster of 1 to 2 us each, the first CTA's steps);
 // for many, a nucleus is a chain per row of load, histogram, sums, sort, on two CTAs an SM: 256 rows of 152k in 16 bits
-// 306 us (0.25 TB/s), 64 rows with rules of their own, fp32, 83 us (0.47 TB/s).  Profiled: issue slots 40 % busy, 64-bit
-// floating point 13 %, a third of the warps' time in barriers.
+// 309 us (0.25 TB/s), 64 rows with rules of their own, fp32, 80 us (0.48 TB/s).  Profiled, the 256 rows: issue slots 55 %
+// busy, 64-bit floating point 16 %, integers 48 %, 27 % of the warps' time in barriers.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         place = __shfl_sync(0xffffffffu, place, leader) + __popc(who & ((1u << lane) - 1u));
         if (take && place < CAP) peer_st(peer(&s.list[place], 0), key);
     };
-    // the list in descending order (n <= CAP), whose first `top` places are wanted: few by their rank, many by a sort
+    // the first n of the list in descending order (n <= CAP): few by their rank, many by a sort
     auto arrange = [&](int n) {
         if (n > 256) {
             sort_down(s.list, n);
@@ -621,7 +621,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         // The bins in which that token can lie: a bin's weights are between those of its edges.  The last bin has no lower edge.
         uint32_t c4[4];
         sum_bins(c4);
-        const float octaves = (float)(w.scale * (double)span / (TABLE * BINS));   // of a bin, 44 / BINS at most
+        const float octaves = (float)(w.scale * (double)span / (TABLE * BINS));   // of a bin, MASS_SPAN / BINS at most
         const double step = exp2f(-octaves);                                      // of a bin's weights
         double edge = exp2f(-octaves * (4.f * tid)) * ONE;
         double most[4], sum4 = 0.0;
@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Args a) {
         // The tokens up to a bin are at least and at most so much by the bins up to it, and by the total less the bins behind
         // it: whichever is less far from its edges (at a top_p of 0.9 the latter, by nine times).
         // margin: of the sums' rounding and of the edges' (fp32: 20 octaves to 2^-24 of them, 2^-19 of a weight); slack: of
-        // the total's and of the weights' rounding to units
+        // these sums against the weights in units
         const double margin = 1.0 + 2e-5, slack = whole * 1e-11 + (double)a.vocab;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -1016,7 +1016,7 @@ size_t smem_of(int share, bool near) {
 template <typename T>
 int run(Args a, cudaStream_t st) {
     // As many CTAs to a row as leave each 4096 tokens or more.  Two of a row of 152k fit an SM; with one CTA to a row, and
-    // passes that read it from L2, 256 rows took 466 us and not 390 (64 rows: 129 and 92).
+    // passes that read it from L2, 256 rows took 466 us and not 390 as the kernel was then (64 rows: 129 and 92).
     unsigned ranks = 1;
     while (ranks < MAX_RANKS && a.vocab > 4096 * (int)ranks) ranks *= 2;
     a.share = (ceil_div(a.vocab, (int)ranks) + 7) & ~7;
